@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define RCH_ABI_VERSION 21
+#define RCH_ABI_VERSION 22
 
 /* Status codes (mapped to reelcache errors by the host). */
 #define RCH_OK 0
@@ -509,6 +509,104 @@ int rch_cholesky_inverse(const double* a_dev, double* x_dev, int32_t* info_dev, 
 #define RCH_SPAN_SPLITS 64
 int rch_fit_span(const rch_fit_matrix* mats_dev, int n_mats, int channels, int64_t max_rows, int max_rank,
                  int with_coefficients, void* stream);
+
+/* Pairings of rch_rotary: channels (2j, 2j + 1), or (j, pairs + j) of the first 2 * pairs. */
+#define RCH_PAIRS_INTERLEAVED 0
+#define RCH_PAIRS_HALF 1
+
+/*
+ * One tensor [batch, tokens, heads, head_dim] (any strides but the last, which is 1; in elements) of
+ * rch_rotary.  The first 2 * pairs channels of a head turn, the rest are copied; pairs = 0 copies all.
+ * Token t of batch b lies at the place rows[b, t, axis] (rows_ptr, int32), or, without rows_ptr, at
+ * (row_t + frame, row_h + y, row_w + x) of its grid (axes = 3) or at row_t + t (axes = 1).  Pair j
+ * belongs to axis 0 below sec_t, to axis 1 below sec_t + sec_h, else to axis 2; pairs_ptr is the fp32
+ * table [rows, pairs, 2] of (cos, sin).  A place outside [0, limit_*) turns to NaN.
+ * With slots_ptr (int32 [tokens], batch 1) token t goes to row slot % page_tokens of page
+ * slot / page_tokens: dst_batch_stride is the page's stride; a slot outside [0, slots) is dropped.
+ */
+typedef struct rch_rotary_job {
+    int64_t src_ptr, dst_ptr;
+    int64_t batch, tokens, heads, head_dim, pairs;
+    int64_t src_batch_stride, src_token_stride, src_head_stride;
+    int64_t dst_batch_stride, dst_token_stride, dst_head_stride;
+    int64_t pairs_ptr, axes, sec_t, sec_h, limit_t, limit_h, limit_w;
+    int64_t row_t, row_h, row_w, grid_h, grid_w;
+    int64_t rows_ptr, rows_batch_stride, rows_token_stride, rows_axis_stride;
+    int64_t slots_ptr, slots, page_tokens;
+    int64_t inverse;         /* 1: turn back (the transpose, which is the gradient's rotation) */
+    int64_t reserved;
+} rch_rotary_job;            /* 34 x int64 = 272 bytes */
+
+/*
+ * Rotates (or copies) up to four tensors of one dtype in one launch; jobs_host is read before the call
+ * returns.  Source and destination of a tensor are the same memory with the same strides, or disjoint.
+ * Rounding as in the restore kernels: fp32 products rounded apart, one rounding to the dtype.
+ */
+int rch_rotary_size(void);
+int rch_rotary(const rch_rotary_job* jobs_host, int n_jobs, int dtype, int pairing, void* stream);
+
+/*
+ * The pools of a paged cache for rch_pages_copy: pools_ptr is a device int64 [pools] of their
+ * addresses.  A page is `segments` (stride segment_stride) of page_rows token rows (stride row_stride)
+ * of row_bytes contiguous bytes; strides in bytes, at most 2 GiB a page.  alignment: the bits that any
+ * pool address has set (their bitwise or).
+ */
+typedef struct rch_pages {
+    int64_t pools_ptr, pools, pages, page_stride;
+    int64_t page_rows, segments, segment_stride, row_stride, row_bytes, alignment;
+} rch_pages;                 /* 10 x int64 = 80 bytes */
+
+/*
+ * Copies pages in every pool: moves_host int32 [n_moves][3] of (source page, destination page, leading
+ * token rows).  No destination is a source or a destination of another move (the caller's rule).  The
+ * moves travel in the launch's arguments, RCH_PAGE_MOVES to a launch.
+ */
+#define RCH_PAGE_MOVES 256
+int rch_pages_copy(const rch_pages* pages_host, const int32_t* moves_host, int n_moves, void* stream);
+
+/*
+ * Attention of new tokens over a paged cache.  A plan is a device int32 buffer built by the host:
+ * items (RCH_ATTEND_ITEM words each), merges (RCH_ATTEND_MERGE words each) and page tables; its first
+ * RCH_ATTEND_ZEROS words are zero (rows that no page holds are read there).
+ *
+ * A row is a (query token, query head) of one key head: row r of a sequence is token r / group, head
+ * kv_head * group + r % group.  Query token i of a sequence stands at place p = length - queries + i and
+ * sees key j < length if j's page is no hole (an entry outside [0, pages) is one),
+ *   block: j < (floor(p / block) + 1) * block      window: j > p - window
+ * (0: no such bound).  out = sum softmax(scale q.k) v over what it sees, 0 where it sees nothing; lse is
+ * the natural log of the sum of exponentials (-inf where nothing is seen).  K, V rows that a query does
+ * not see have no influence, whatever they hold.
+ *
+ * Item: [table (word index of the sequence's first page), length, first query row of q, queries,
+ *   row_begin, row_end, kv_head, key_begin, key_end, part (first row of the fp32 partials it writes, or
+ *   -1: the output itself), 0, 0].  Merge: [first query row of q, row_begin, rows, kv_head, first partial
+ *   row, parts, 0, 0]: part i of row r is partial row first + i * rows + (r - row_begin).
+ * Partials: fp32 [partial_rows, head_dim] sums, then fp32 [partial_rows, 2] of (reference exponent, sum).
+ */
+#define RCH_ATTEND_ITEM 12
+#define RCH_ATTEND_MERGE 8
+#define RCH_ATTEND_ZEROS 128
+#define RCH_ATTEND_MAX_DIM 256   /* head_dim of the general form */
+#define RCH_ATTEND_FAST_DIM 128  /* head_dim of the others: multiples of 8 up to this, 16-byte aligned rows */
+
+typedef struct rch_attend {
+    int64_t q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr; /* lse_ptr: fp32 [query rows, heads], or 0 */
+    int64_t plan_ptr, partial_ptr;
+    int64_t q_token_stride, q_head_stride;         /* all strides in elements, unit over the channels */
+    int64_t k_page_stride, k_token_stride, k_head_stride;
+    int64_t v_page_stride, v_token_stride, v_head_stride;
+    int64_t out_token_stride, out_head_stride;
+    int64_t group, heads, head_dim, page_tokens, pages, block, window;
+    int64_t scale_bits;      /* fp32 bits of scale * log2(e); scale > 0 */
+    int64_t partial_rows;
+    int64_t items;           /* word index of the first item */
+    int64_t n_general, n_rows, n_tokens; /* items of the general, the row-tiled and the few-rows form, in order */
+    int64_t merges, n_merges, most_rows; /* word index, count, most rows of a merge */
+    int64_t holes;           /* 1: page tables may hold holes */
+} rch_attend;                /* 34 x int64 = 272 bytes */
+
+int rch_attend_size(void);
+int rch_attend_run(const rch_attend* args_host, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ import numpy as np
 from .errors import ConfigurationError, UnsupportedError
 
 LIBRARY = Path(__file__).resolve().with_name("libreelcache_hip.so")
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 # Status codes (RCH_E_*).
 OK, E_CONFIG, E_UNSUPPORTED, E_LAUNCH = 0, 1, 2, 3
@@ -67,6 +67,21 @@ QUANTIZE_FIELDS = ("values_ptr", "rows", "cols", "stride", "affine_ptr", "codes_
 QUANTIZE_DTYPE = np.dtype([(name, "<i8") for name in QUANTIZE_FIELDS])
 GAUSS_FIELDS = ("dst_ptr", "rows", "cols", "stride", "seed", "reserved0", "reserved1", "reserved2")
 GAUSS_DTYPE = np.dtype([(name, "<i8") for name in GAUSS_FIELDS])
+# rch_rotary_job, rch_pages (int64 structs read on the host during the call), pairings and moves per launch.
+ROTARY_FIELDS = ("src_ptr", "dst_ptr", "batch", "tokens", "heads", "head_dim", "pairs", "src_batch_stride",
+                 "src_token_stride", "src_head_stride", "dst_batch_stride", "dst_token_stride", "dst_head_stride",
+                 "pairs_ptr", "axes", "sec_t", "sec_h", "limit_t", "limit_h", "limit_w", "row_t", "row_h", "row_w",
+                 "grid_h", "grid_w", "rows_ptr", "rows_batch_stride", "rows_token_stride", "rows_axis_stride",
+                 "slots_ptr", "slots", "page_tokens", "inverse", "reserved")
+PAGES_FIELDS = ("pools_ptr", "pools", "pages", "page_stride", "page_rows", "segments", "segment_stride", "row_stride",
+                "row_bytes", "alignment")
+ATTEND_FIELDS = ("q_ptr", "k_ptr", "v_ptr", "out_ptr", "lse_ptr", "plan_ptr", "partial_ptr", "q_token_stride",
+                 "q_head_stride", "k_page_stride", "k_token_stride", "k_head_stride", "v_page_stride", "v_token_stride",
+                 "v_head_stride", "out_token_stride", "out_head_stride", "group", "heads", "head_dim", "page_tokens",
+                 "pages", "block", "window", "scale_bits", "partial_rows", "items", "n_general", "n_rows", "n_tokens",
+                 "merges", "n_merges", "most_rows", "holes")
+ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 128
+PAIRS_INTERLEAVED, PAIRS_HALF = 0, 1
 
 _i, _i64, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _SIGNATURES = {
@@ -99,6 +114,11 @@ _SIGNATURES = {
     "rch_cholesky_inverse": ([_p, _p, _p, _i, _i, _p], _i),
     "rch_fit_span": ([_p, _i, _i, _i64, _i, _i, _p], _i),
     "rch_fit_gaussian": ([_p, _i, _i64, _p], _i),
+    "rch_rotary_size": ([], _i),
+    "rch_rotary": ([_p, _i, _i, _i, _p], _i),
+    "rch_pages_copy": ([_p, _p, _i, _p], _i),
+    "rch_attend_size": ([], _i),
+    "rch_attend_run": ([_p, _i, _p], _i),
 }
 # Further entry points registered by other modules are bound when present.
 _OPTIONAL_SIGNATURES: dict = {}
@@ -128,7 +148,9 @@ def _load():
     if lib.rch_abi_version() != ABI_VERSION:
         raise UnsupportedError(f"{LIBRARY.name} has ABI {lib.rch_abi_version()}, expected {ABI_VERSION}; rebuild it")
     if (lib.rch_job_size() != JOB_DTYPE.itemsize or lib.rch_pack_size() != PACK_DTYPE.itemsize
-            or lib.rch_fit_matrix_size() != FIT_DTYPE.itemsize or lib.rch_call_size() != 8 * len(CALL_FIELDS)):
+            or lib.rch_fit_matrix_size() != FIT_DTYPE.itemsize or lib.rch_call_size() != 8 * len(CALL_FIELDS)
+            or lib.rch_rotary_size() != 8 * len(ROTARY_FIELDS)
+            or lib.rch_attend_size() != 8 * len(ATTEND_FIELDS)):
         raise UnsupportedError(f"{LIBRARY.name} descriptor layout differs from this package; rebuild it")
     return lib
 

@@ -1,0 +1,343 @@
+"""Attention of new tokens over a paged cache.
+
+The tokens of a step (a chunk of a video, a prompt, one token of each of many sequences) attend to the
+pages of their sequence, themselves included once they are stored.  :class:`AttentionPlan` lays the
+step's work out on the host once: which rows of queries meet which keys in which workgroup, so that the
+card is filled whatever the lengths; every layer's :func:`attend` then runs that plan
+(``rch_attend_run``).
+
+Masks: a query at place ``p`` of its sequence (the last query stands at the last token) sees every key
+of the sequence, or with ``block`` those before the end of its own block of that many tokens
+(``block=1``: causal; ``block=frame tokens``: causal over frames), and with ``window`` only keys after
+``p - window``.  Dropped pages are not seen.  A query that sees nothing gets zeros.  Keys and values
+that a query does not see have no influence on it, whatever their slots hold.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._checks import count, need, strided
+from .errors import StateError, UnsupportedError
+from .rotary import _DTYPE_CODES, _span, entered, need_gpu
+
+#: Keys of a tile: the step of every split of a sequence's keys.
+KEY_TILE = 64
+#: Query rows (tokens x heads of a key head) of one workgroup's tile, per form.
+GENERAL_ROWS, ROW_TILE, TOKEN_ROWS = 16, 128, 32
+# Workgroups resident on the card at once, per form (256 CUs), and what a workgroup's start, end and
+# partial results cost in key tiles.
+_RESIDENT = {"general": 1024, "rows": 512, "tokens": 256}
+_OVERHEAD = {"general": 1, "rows": 6, "tokens": 4}
+_XCDS = 8
+_MOST_PARTS = 64
+
+
+class _Work:
+    """The row blocks of one form: parallel int64 arrays, one entry per (sequence, key head, row block)."""
+
+    def __init__(self):
+        self.parts = []
+
+    def add(self, sequence, kv_heads, rows, tile, keys_of):
+        begin = np.arange(0, rows, tile, dtype=np.int64)
+        end = np.minimum(begin + tile, rows)
+        first, last = keys_of(begin, end)
+        block = np.stack([np.full_like(begin, sequence), begin, end, first, last], axis=1)
+        heads = np.repeat(np.arange(kv_heads, dtype=np.int64), len(block))
+        self.parts.append(np.concatenate([np.tile(block, (kv_heads, 1)), heads[:, None]], axis=1))
+
+    def rows(self):
+        """int64 [n, 6]: sequence, row begin, row end, first key, last key, key head."""
+        return np.concatenate(self.parts) if self.parts else np.empty((0, 6), np.int64)
+
+
+class AttentionPlan:
+    """The work of one step: ``queries[i]`` new tokens of ``sequences[i]`` of a
+    :class:`~reelcache_amd.paged_cache.PagedCache` attend to it with ``heads`` query heads (a multiple of
+    the cache's), packed sequence after sequence.
+
+    ``block``, ``window``: see the module docstring (``None``: no such bound).  ``scale``: a positive
+    factor of the scores (default ``head_dim ** -0.5``).  The plan is bound to the pages that the
+    sequences have now; it is stale once pages move or are freed.  A captured graph keeps its plan's
+    tables as they are: keep the plan as long as the graph.
+    """
+
+    def __init__(self, cache, sequences, queries, *, heads, block=None, window=None, scale=None):
+        found = cache._several(sequences)
+        queries = [count(n, "a query count") for n in queries]
+        need(len(queries) == len(found), "a plan takes one query count for each sequence")
+        count(heads, "heads", minimum=1)
+        need(heads % cache.heads == 0, "query heads must be a multiple of the cache's heads")
+        for value, name in ((block, "block"), (window, "window")):
+            need(value is None or count(value, name, minimum=1) < 1 << 31, f"{name} must be below 2**31")
+        scale = cache.head_dim ** -0.5 if scale is None else scale
+        need(isinstance(scale, (int, float)) and not isinstance(scale, bool) and math.isfinite(scale) and scale > 0,
+             "scale must be a positive number")
+        if cache.head_dim > _lib.ATTEND_MAX_DIM:
+            raise UnsupportedError(f"attention takes at most {_lib.ATTEND_MAX_DIM} channels to a head")
+        need_gpu(cache.device, "attention")
+        self.cache, self.heads, self.queries = cache, heads, sum(queries)
+        self.group = heads // cache.heads
+        need(self.queries * self.group < 1 << 31, "a step has fewer than 2**31 query rows")
+        self.block, self.window, self.scale = block, window, float(scale)
+        self._stamp = cache._moved
+        self._lay_out(found, queries)
+
+    # -----------------------------------------------------------------------------------------
+
+    def _keys_of(self, length, queries):
+        """Function of row ranges: the keys that any row of a range may see (empty: first == last)."""
+        group, block, window = self.group, self.block, self.window
+
+        def keys(begin, end):
+            place0, place1 = (length - queries + at // group for at in (begin, end - 1))
+            first, last = np.zeros_like(begin), np.full_like(begin, length)
+            if block:
+                last = np.minimum(last, np.where(place1 < 0, 0, (place1 // block + 1) * block))
+            if window:
+                first = np.clip(place0 - window + 1, 0, length)
+            return first, np.maximum(first, last)
+
+        return keys
+
+    def _form(self, rows):
+        cache = self.cache
+        size = cache.keys.element_size()
+        aligned = all(pool.data_ptr() % 16 == 0 and all(pool.stride(a) * size % 16 == 0 for a in range(4))
+                      for pool in (cache.keys, cache.values))
+        if not (aligned and cache.head_dim % 8 == 0 and cache.head_dim <= _lib.ATTEND_FAST_DIM):
+            return "general"
+        return "general"
+
+    def _lay_out(self, found, queries):
+        cache = self.cache
+        work = {name: _Work() for name in _RESIDENT}
+        tiles = {"general": GENERAL_ROWS, "rows": ROW_TILE, "tokens": TOKEN_ROWS}
+        table, at, lengths, starts = [], [], [], []
+        words, row = _lib.ATTEND_ZEROS, 0
+        for number, (item, n) in enumerate(zip(found, queries)):
+            lengths.append(item.tokens)
+            starts.append(row)
+            at.append(words)
+            table.extend(item.pages)
+            words += len(item.pages)
+            row += n
+            if n:
+                form = self._form(n * self.group)
+                work[form].add(number, cache.heads, n * self.group, tiles[form], self._keys_of(item.tokens, n))
+        need(words < 1 << 30, "the step's page tables are too large")
+        self._at = np.asarray(at, dtype=np.int64)
+        self._lengths, self._starts = np.asarray(lengths, dtype=np.int64), np.asarray(starts, dtype=np.int64)
+        self._counts = np.asarray(queries, dtype=np.int64)
+        items, merges, self._partial_rows, counts = [], [], 0, {}
+        for form in ("general", "rows", "tokens"):
+            made = self._split(form, work[form].rows(), merges)
+            counts[form] = len(made)
+            items.append(made)
+        items = np.concatenate(items)
+        merges = np.concatenate(merges) if merges else np.empty((0, _lib.ATTEND_MERGE), np.int64)
+        self._counts_of = (counts["general"], counts["rows"], counts["tokens"])
+        first_item = _lib.ATTEND_ZEROS + len(table)
+        self._items, self._merges = first_item, first_item + items.size
+        self._n_merges = len(merges)
+        self._most_rows = int(merges[:, 2].max()) if len(merges) else 0
+        self._holes = int(any(page < 0 for page in table))
+        need(self._partial_rows < 1 << 31, "the step's partial results are too many")
+        words = np.concatenate([np.zeros(_lib.ATTEND_ZEROS, np.int64), np.asarray(table, np.int64), items.ravel(),
+                                merges.ravel()])
+        from .paged_cache import upload
+
+        with entered(cache.device):
+            self.buffer = upload(words, cache.device)
+
+    def _unit(self):
+        """Tokens that tiles of keys start over at: a page where tiles stay within pages, else a tile."""
+        size = self.cache.page_tokens
+        return size if size >= KEY_TILE else KEY_TILE
+
+    def _tile_of(self, key):
+        """Index of the tile that holds ``key``, and the first key of a tile."""
+        unit = self._unit()
+        return key // unit * -(-unit // KEY_TILE) + key % unit // KEY_TILE
+
+    def _key_of(self, tile):
+        unit = self._unit()
+        per = -(-unit // KEY_TILE)
+        return tile // per * unit + tile % per * KEY_TILE
+
+    def _split(self, form, blocks, merges):
+        """Items of a form's row blocks: the keys of a block in as many parts as fill the card best, in
+        launch order."""
+        if not len(blocks):
+            return np.empty((0, _lib.ATTEND_ITEM), np.int64)
+        sequence, begin, end, first, last, head = blocks.T
+        tile0 = self._tile_of(first)
+        tiles = np.where(last > first, self._tile_of(np.maximum(last - 1, 0)) + 1 - tile0, 0)
+        most = self._longest_part(form, tiles)
+        parts = np.maximum(1, -(-tiles // most))
+        which = np.repeat(np.arange(len(blocks)), parts)
+        part = np.arange(len(which)) - np.repeat(np.cumsum(parts) - parts, parts)
+        n, total = parts[which], tiles[which]
+        low, high = part * total // n, (part + 1) * total // n
+        rows = (end - begin)[which]
+        # Partial rows: part after part of a block, block after block.
+        need_rows = np.where(parts > 1, parts * (end - begin), 0)
+        base = self._partial_rows + np.cumsum(need_rows) - need_rows
+        self._partial_rows += int(need_rows.sum())
+        items = np.zeros((len(which), _lib.ATTEND_ITEM), np.int64)
+        items[:, 0] = self._at[sequence][which]
+        items[:, 1] = self._lengths[sequence][which]
+        items[:, 2] = self._starts[sequence][which]
+        items[:, 3] = self._counts[sequence][which]
+        items[:, 4], items[:, 5], items[:, 6] = begin[which], end[which], head[which]
+        items[:, 7] = np.where(part == 0, first[which], self._key_of(tile0[which] + low))
+        items[:, 8] = np.where(part == n - 1, last[which], np.minimum(last[which], self._key_of(tile0[which] + high)))
+        items[:, 9] = np.where(n > 1, base[which] + part * rows, -1)
+        several = parts > 1
+        if several.any():
+            rows = (end - begin)[several]
+            merge = np.zeros((len(rows), _lib.ATTEND_MERGE), np.int64)
+            merge[:, 0], merge[:, 1], merge[:, 2] = self._starts[sequence[several]], begin[several], rows
+            merge[:, 3], merge[:, 4], merge[:, 5] = head[several], base[several], parts[several]
+            merges.append(merge)
+        return items[self._order(high - low, sequence[which] * self.cache.heads + head[which])]
+
+    def _longest_part(self, form, tiles):
+        """Key tiles of the longest part: the length whose parts finish first by the estimate (rounds of
+        resident workgroups times the longest part and its overhead)."""
+        resident, overhead = _RESIDENT[form], _OVERHEAD[form]
+        longest = int(tiles.max())
+        best, chosen = None, max(1, longest)
+        for parts in range(1, _MOST_PARTS + 1):
+            length = max(1, -(-longest // parts))
+            n = int(np.maximum(1, -(-tiles // length)).sum())
+            cost = float(tiles.sum()) + n * overhead
+            one = length + overhead * (1 if parts == 1 else 1.5)
+            time = max(-(-n // resident) * one if n <= 4 * resident else cost / resident + one / 2, one)
+            if best is None or time < 0.97 * best:
+                best, chosen = time, length
+            if length == 1 or n > 8 * resident:
+                break
+        return chosen
+
+    @staticmethod
+    def _order(cost, owner):
+        """Launch order: workgroup b runs on XCD b % 8, so the items of one (sequence, key head), which
+        share keys, go to one XCD as far as the XCDs stay evenly loaded; long ones first."""
+        n = len(cost)
+        if n <= _XCDS:
+            return np.argsort(-cost, kind="stable")
+        by_owner = np.argsort(owner, kind="stable")
+        load = np.cumsum(cost[by_owner] + 1)
+        xcd = np.minimum((load - 1) * _XCDS // int(load[-1]), _XCDS - 1)
+        buckets = [by_owner[xcd == x] for x in range(_XCDS)]
+        buckets = [bucket[np.argsort(-cost[bucket], kind="stable")] for bucket in buckets]
+        # The i-th items of all buckets, XCD after XCD; a bucket that runs out leaves its place to the next.
+        rank = np.concatenate([np.arange(len(bucket)) for bucket in buckets])
+        return np.concatenate(buckets)[np.argsort(rank, kind="stable")]
+
+    # -----------------------------------------------------------------------------------------
+
+    def _check(self, keys, values):
+        cache = self.cache
+        if self._stamp != cache._moved:
+            raise StateError("pages moved or were freed after this plan was built")
+        shape, k_stride, v_stride = cache.keys.shape[1:], cache.keys.stride()[1:], cache.values.stride()[1:]
+        for pool, stride, name in ((keys, k_stride, "keys"), (values, v_stride, "values")):
+            strided(pool, name)
+            need(pool.shape == shape and pool.stride() == stride and pool.dtype == cache.dtype
+                 and pool.device == cache.device, f"{name} must be a layer's pool like those of the plan's cache")
+
+
+def attend(q, keys, values, plan, *, out=None, return_lse=False):
+    """Attention of ``q`` over one layer's pools by ``plan``.
+
+    ``q``: ``[rows, heads, head_dim]`` of the cache's dtype, any strides; its first ``plan.queries`` rows
+    are the plan's.  ``keys``, ``values``: one layer of the plan's cache.  ``out``: where to write, of
+    q's shape (rows behind the plan's stay as they are); without it a new tensor, zero behind them.
+    ``return_lse``: also the fp32 ``[rows, heads]`` natural logs of the sums of exponentials (-inf for a
+    query that sees nothing), by which the results over two caches join.
+
+    Scores and sums are held in fp32; the output is rounded once.  Runs on the current stream; not
+    differentiable.  Returns ``out``, or ``(out, lse)``.
+    """
+    need(isinstance(plan, AttentionPlan), "attend needs an AttentionPlan")
+    plan._check(keys, values)
+    cache = plan.cache
+    strided(q, "q")
+    need(q.ndim == 3 and q.shape[0] >= plan.queries and q.shape[1] == plan.heads and q.shape[2] == cache.head_dim,
+         "q must be [rows, heads, head_dim] with a row for every query of the plan")
+    need(q.dtype == cache.dtype and q.device == cache.device, "q must have the cache's dtype and device")
+    device = cache.device
+    with entered(device):
+        stream = torch.cuda.current_stream(device)
+        given, q = q, _rows(q.detach())
+        more = q.shape[0] > plan.queries
+        result = out
+        if out is None:
+            result = out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            if more:
+                out[plan.queries:].zero_()
+        else:
+            strided(out, "out")
+            need(out.shape == q.shape and out.dtype == q.dtype and out.device == device, "out must match q")
+            need(not out.requires_grad, "out must not require gradients")
+            need(all(stride != 0 or size <= 1 for size, stride in zip(out.shape, out.stride())),
+                 "out with broadcast (zero) strides aliases itself")
+            low, high = _span(out)
+            for x in (given, keys, values):
+                same = x is given and out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+                first, last = _span(x)
+                need(same or high <= first or last <= low, "out overlaps an input without being q")
+            if not _aligned(out):
+                result = torch.empty(q.shape, dtype=q.dtype, device=device)
+        lse = None
+        if return_lse:
+            lse = torch.empty((q.shape[0], plan.heads), dtype=torch.float32, device=device)
+            if more:
+                lse[plan.queries:].fill_(-math.inf)
+        if plan.queries:
+            _launch(q, keys, values, plan, result, lse, stream)
+            if result is not out:
+                out[:plan.queries].copy_(result[:plan.queries])
+    return (out, lse) if return_lse else out
+
+
+def _aligned(x):
+    size = x.element_size()
+    return (x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * size % 16 == 0 and x.stride(1) * size % 16 == 0)
+
+
+def _rows(q):
+    """``q`` as the kernels read it in place (16-byte rows), else a copy; a head_dim whose rows cannot be
+    16-byte aligned only runs in the general form, which needs unit stride alone."""
+    if _aligned(q) or (q.shape[2] * q.element_size() % 16 and (q.stride(2) == 1 or q.shape[2] == 1)):
+        return q
+    return q.clone(memory_format=torch.contiguous_format)
+
+
+def _launch(q, keys, values, plan, out, lse, stream):
+    cache = plan.cache
+    partials = None
+    if plan._n_merges:
+        partials = torch.empty(plan._partial_rows * (cache.head_dim + 2), dtype=torch.float32, device=q.device)
+    plan.buffer.record_stream(stream)
+    page, token, head = (axis - 1 for axis in cache._axes)
+    k, v = keys.stride(), values.stride()
+    fields = (q.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+              plan.buffer.data_ptr(), 0 if partials is None else partials.data_ptr(), q.stride(0), q.stride(1),
+              k[page], k[token], k[head], v[page], v[token], v[head], out.stride(0), out.stride(1),
+              plan.group, plan.heads, cache.head_dim, cache.page_tokens, cache.pages, plan.block or 0, plan.window or 0,
+              struct.unpack("<i", struct.pack("<f", plan.scale * math.log2(math.e)))[0], plan._partial_rows,
+              plan._items, *plan._counts_of, plan._merges, plan._n_merges, plan._most_rows, plan._holes)
+    _lib.call("rch_attend_run", (ctypes.c_int64 * len(fields))(*fields), _DTYPE_CODES[q.dtype], stream.cuda_stream)
+
+
+__all__ = ["AttentionPlan", "attend"]

@@ -1,0 +1,475 @@
+"""A KV cache in pages: sequences that share, fork, drop and compact their history.
+
+A restored history is written into native cache slots (reelcache/restore_kernels.py:235-305); a
+serving engine keeps such slots in pages so that continuations of one history share it.
+:class:`PagedCache` holds the K and V pools of all layers and, on the host, the pages of each
+sequence.  Every layer uses the same page of a sequence for the same tokens, so a page is copied in
+all layers' K and V pools at once (``rch_pages_copy``).
+
+Pools are ``[layers, pages, page_tokens, heads, head_dim]`` (``layout="BTHD"``) or ``[layers, pages,
+heads, page_tokens, head_dim]`` (``"BHTD"``): one layer's pool is a native cache tensor whose batch
+axis counts pages, so a restore writes into consecutive pages through :meth:`PagedCache.view`, and a
+caller's native caches serve as pools of one page (``PagedCache(k[None], v[None])``).
+
+The page tables are host state.  Whatever allocates takes the lowest free pages, in the order of the
+sequences given, and checks that there are enough before it changes anything.  Device work runs on the
+current stream of the cache's device, in order: callers that use several streams order them.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import heapq
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+from . import _lib
+from ._checks import count, need, one_of, strided
+from .errors import CapacityError, ConfigurationError, StateError
+from .restore_handle import _capturing
+from .restore_model import OUTPUT_DTYPES, NativeView
+from .rotary import entered, launch_rotary, need_gpu, position_fields
+
+HOLE = -1
+_LAYOUTS = ("BTHD", "BHTD")
+
+
+@dataclass(eq=False)
+class Slots:
+    """Where new tokens go: built by :meth:`PagedCache.extend` or :meth:`PagedCache.slots` once per
+    step, used by :meth:`PagedCache.store` in every layer.  ``index``: int32 ``[tokens]`` on the device,
+    page * page_tokens + row of each token."""
+
+    index: torch.Tensor
+    tokens: int
+    cache: "PagedCache"
+    stamp: int
+
+
+class _Sequence:
+    __slots__ = ("pages", "tokens")
+
+    def __init__(self, pages, tokens):
+        self.pages, self.tokens = pages, tokens
+
+
+def upload(values, device):
+    """An int32 array on ``device``, copied from pinned memory on the current stream without a host
+    wait; the pinned block stays reserved until the copy has run."""
+    if _capturing():
+        raise ConfigurationError("page tables, slots and plans are built before a HIP-graph capture, not in it")
+    return torch.from_numpy(np.ascontiguousarray(values, dtype=np.int32)).pin_memory().to(device, non_blocking=True)
+
+
+class PagedCache:
+    """K and V pools of every layer, and the pages of each sequence.
+
+    ``keys``, ``values``: pools as above, of one shape, dtype (bfloat16, float16, float32) and device,
+    with unit stride over the channels; any other strides that keep elements apart.
+    """
+
+    def __init__(self, keys, values, *, layout="BTHD"):
+        one_of(layout, _LAYOUTS, "pool layout")
+        for pool, name in ((keys, "keys"), (values, "values")):
+            strided(pool, name)
+            need(pool.ndim == 5, f"{name} must be [layers, pages, ...] pools of five dimensions")
+            need(pool.dtype in OUTPUT_DTYPES, f"{name} must be bfloat16, float16 or float32")
+            need(min(pool.shape) >= 1, f"{name} must not be empty")
+            need(pool.stride(4) == 1 or pool.shape[4] == 1, f"{name} must have unit stride over the channels")
+            need(_apart(pool), f"{name} must keep its elements apart")
+        need(keys.shape == values.shape and keys.dtype == values.dtype and keys.device == values.device,
+             "keys and values must match in shape, dtype and device")
+        self.keys, self.values, self.layout = keys, values, layout
+        token, head = (2, 3) if layout == "BTHD" else (3, 2)
+        self.layers, self.pages = keys.shape[:2]
+        self.page_tokens, self.heads, self.head_dim = keys.shape[token], keys.shape[head], keys.shape[4]
+        need(self.pages * self.page_tokens < 1 << 31, "a pool holds fewer than 2**31 tokens")
+        self.device, self.dtype = keys.device, keys.dtype
+        self._axes = (1, token, head)
+        self._sequences: dict[int, _Sequence] = {}
+        self._next = 0
+        self._uses = [0] * self.pages
+        self._free = list(range(self.pages))
+        self._moved = 0   # counts what may move or reuse pages: plans and slots built before it are stale
+        self._shared = 0  # counts what may share pages: slots built before it are stale
+        self._copies = None
+
+    @classmethod
+    def allocate(cls, pages, page_tokens, heads, head_dim, *, layers=1, dtype=torch.bfloat16, device="cuda", layout="BTHD"):
+        """A cache over new, uninitialised pools."""
+        one_of(layout, _LAYOUTS, "pool layout")
+        for value, name in ((pages, "pages"), (page_tokens, "page_tokens"), (heads, "heads"), (head_dim, "head_dim"),
+                            (layers, "layers")):
+            count(value, name, minimum=1)
+        rows = (page_tokens, heads) if layout == "BTHD" else (heads, page_tokens)
+        keys, values = (torch.empty((layers, pages, *rows, head_dim), dtype=dtype, device=device) for _ in range(2))
+        return cls(keys, values, layout=layout)
+
+    # -----------------------------------------------------------------------------------------
+    # Sequences
+    # -----------------------------------------------------------------------------------------
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def _get(self, sequence):
+        found = self._sequences.get(sequence) if type(sequence) is int else None
+        if found is None:
+            raise StateError(f"there is no sequence {sequence!r} in this cache")
+        return found
+
+    def _several(self, sequences):
+        sequences = list(sequences)
+        found = [self._get(s) for s in sequences]
+        need(len(set(sequences)) == len(sequences), "a sequence is named twice")
+        return found
+
+    def tokens(self, sequence):
+        return self._get(sequence).tokens
+
+    def pages_of(self, sequence):
+        """The pages of a sequence in order (:data:`HOLE` where one was dropped)."""
+        return list(self._get(sequence).pages)
+
+    def new(self):
+        """A new, empty sequence."""
+        self._sequences[self._next] = _Sequence([], 0)
+        self._next += 1
+        return self._next - 1
+
+    def fork(self, sequence):
+        """A new sequence with the same tokens: it shares every page.  A page that is not full is copied
+        when the first of its sequences goes on."""
+        source = self._get(sequence)
+        for page in source.pages:
+            if page != HOLE:
+                self._uses[page] += 1
+        self._shared += 1
+        child = self.new()
+        self._sequences[child] = _Sequence(list(source.pages), source.tokens)
+        return child
+
+    def _release(self, pages):
+        for page in pages:
+            if page == HOLE:
+                continue
+            self._uses[page] -= 1
+            if self._uses[page] == 0:
+                heapq.heappush(self._free, page)
+
+    def free(self, sequence):
+        """Drop a sequence; pages that no other one shares become free."""
+        pages = self._get(sequence).pages
+        del self._sequences[sequence]
+        self._release(pages)
+        self._moved += 1
+
+    def truncate(self, sequence, tokens):
+        """Rewind a sequence to its first ``tokens`` tokens."""
+        found = self._get(sequence)
+        need(count(tokens, "tokens") <= found.tokens, "a sequence is truncated to what it has")
+        keep = -(-tokens // self.page_tokens)
+        if keep and found.pages[keep - 1] == HOLE:
+            raise StateError("a sequence cannot end in a dropped page")
+        self._release(found.pages[keep:])
+        del found.pages[keep:]
+        found.tokens = tokens
+        self._moved += 1
+
+    def drop(self, sequence, first, pages):
+        """Drop ``pages`` pages of a sequence from its page ``first`` on (a rolling window): their tokens
+        keep their positions and are not attended to any more.  The last page stays."""
+        found = self._get(sequence)
+        count(first, "first"), count(pages, "pages")
+        need(first + pages < max(1, len(found.pages)), "the last page of a sequence cannot be dropped")
+        self._release(found.pages[first:first + pages])
+        found.pages[first:first + pages] = [HOLE] * pages
+        self._moved += 1
+
+    def _begun(self, found):
+        """Rows of the last page in use when it is not full, else 0."""
+        return found.tokens % self.page_tokens
+
+    def extend(self, sequences, counts):
+        """Room for ``counts[i]`` more tokens of ``sequences[i]``: new pages, and a copy (in every layer)
+        of a begun page that other sequences share.  Returns the :class:`Slots` of the new tokens, packed
+        sequence after sequence."""
+        sequences, counts = list(sequences), list(counts)
+        found = self._several(sequences)
+        need(len(counts) == len(found), "extend takes one count for each sequence")
+        for n in counts:
+            count(n, "a token count")
+        need_gpu(self.device, "a paged cache")
+        uses: dict[int, int] = {}
+        wanted = []  # (copies the begun page, new pages) of each sequence
+        for item, n in zip(found, counts):
+            more = -(-(item.tokens + n) // self.page_tokens) - len(item.pages)
+            copies = False
+            if n and self._begun(item):
+                last = item.pages[-1]
+                shared = uses.get(last, self._uses[last])
+                copies = shared > 1
+                uses[last] = shared - copies
+            wanted.append((copies, more))
+        need(sum(item.tokens + n for item, n in zip(found, counts)) < 1 << 31, "a step covers fewer than 2**31 tokens")
+        total = sum(copies + more for copies, more in wanted)
+        if total > len(self._free):
+            raise CapacityError(f"{total} pages are needed and {len(self._free)} are free")
+        if _capturing():
+            raise ConfigurationError("a cache grows before a HIP-graph capture, not in it")
+        moves, starts = [], []
+        for item, n, (copies, more) in zip(found, counts, wanted):
+            if copies:
+                page = self._take()
+                moves.append((item.pages[-1], page, self._begun(item)))
+                self._release(item.pages[-1:])
+                item.pages[-1] = page
+                self._shared += 1
+            item.pages.extend(self._take() for _ in range(more))
+            starts.append(item.tokens)
+            item.tokens += n
+        self._copy(moves)
+        return self._slots(found, starts, counts)
+
+    def _take(self):
+        page = heapq.heappop(self._free)
+        self._uses[page] = 1
+        return page
+
+    def slots(self, sequences, starts, counts):
+        """The :class:`Slots` of tokens ``starts[i] .. starts[i] + counts[i]`` that ``sequences[i]`` has
+        (rows to write again).  Their pages must not be shared."""
+        found = self._several(sequences)
+        starts, counts = list(starts), list(counts)
+        need(len(starts) == len(counts) == len(found), "slots take one start and count for each sequence")
+        for item, start, n in zip(found, starts, counts):
+            need(count(start, "a start") + count(n, "a token count") <= item.tokens, "slots lie within the sequence")
+            if n == 0:
+                continue
+            for page in item.pages[start // self.page_tokens:(start + n - 1) // self.page_tokens + 1]:
+                if page == HOLE:
+                    raise StateError("the slots' page was dropped")
+                if self._uses[page] > 1:
+                    raise StateError("the slots' page is shared with another sequence")
+        need_gpu(self.device, "a paged cache")
+        return self._slots(found, starts, counts)
+
+    def _slots(self, found, starts, counts):
+        parts = []
+        for item, start, n in zip(found, starts, counts):
+            at = np.arange(start, start + n, dtype=np.int64)
+            first = start // self.page_tokens
+            pages = np.asarray(item.pages[first:-(-(start + n) // self.page_tokens)], dtype=np.int64)
+            parts.append(pages[at // self.page_tokens - first] * self.page_tokens + at % self.page_tokens)
+        index = np.concatenate(parts) if parts else np.empty(0, np.int64)
+        with entered(self.device):
+            return Slots(upload(index, self.device), index.size, self, self._moved + self._shared)
+
+    # -----------------------------------------------------------------------------------------
+    # Page copies
+    # -----------------------------------------------------------------------------------------
+
+    def _copy(self, moves):
+        """Copies pages in every pool: ``moves`` of (source, destination, leading rows)."""
+        if not moves:
+            return
+        with entered(self.device):
+            if self._copies is None:
+                self._copies = [_pools(pool, self._axes, self.pages, self.page_tokens)
+                                for pool in self._joined_pools()]
+            flat = [value for move in moves for value in move]
+            table = (ctypes.c_int32 * len(flat))(*flat)
+            stream = torch.cuda.current_stream(self.device)
+            for pools, fields in self._copies:
+                pools.record_stream(stream)
+                _lib.call("rch_pages_copy", fields, table, len(moves), stream.cuda_stream)
+
+    def _joined_pools(self):
+        """K and V pools as one group where their strides agree (one launch), else as two."""
+        if self.keys.stride() == self.values.stride():
+            return [(self.keys, self.values)]
+        return [(self.keys,), (self.values,)]
+
+    def compact(self):
+        """Move pages down until those in use are the lowest ones (the highest in use go to the lowest
+        free, in order).  Returns the moves as (from, to) pairs."""
+        used = [page for page, uses in enumerate(self._uses) if uses]
+        moved = [page for page in used if page >= len(used)]
+        return self._relocate(moved, [page for page in range(len(used)) if not self._uses[page]])
+
+    def make_contiguous(self, sequence):
+        """Move a sequence's pages to the lowest run of consecutive free pages (for :meth:`view`); pages
+        shared with other sequences move for them too.  Nothing moves when they are consecutive."""
+        pages = self._get(sequence).pages
+        if any(page == HOLE for page in pages):
+            raise StateError("a sequence with dropped pages has no consecutive ones")
+        if all(b == a + 1 for a, b in zip(pages, pages[1:])):
+            return []
+        start = run = 0
+        for page in sorted(self._free):
+            run = run + 1 if run and page == start + run else 1
+            start = page if run == 1 else start
+            if run == len(pages):
+                return self._relocate(list(pages), list(range(start, start + run)))
+        raise CapacityError(f"there is no run of {len(pages)} free pages")
+
+    def _relocate(self, source, target):
+        """Copies pages ``source[i]`` to the free pages ``target[i]`` and renames them in every sequence."""
+        if not source:
+            return []
+        need_gpu(self.device, "a paged cache")
+        self._copy([(a, b, self.page_tokens) for a, b in zip(source, target)])
+        names = dict(zip(source, target))
+        for a, b in names.items():
+            self._uses[b], self._uses[a] = self._uses[a], 0
+        for item in self._sequences.values():
+            item.pages = [names.get(page, page) for page in item.pages]
+        self._free = [page for page, uses in enumerate(self._uses) if not uses]  # ascending: a heap
+        self._moved += 1
+        return list(zip(source, target))
+
+    def load_tables(self, tables):
+        """Start over with sequences 0, 1, ... of ``(pages, tokens)`` each (e.g. saved with
+        :meth:`pages_of`); the pools keep what they hold.  Sequences may share pages."""
+        loaded, uses = {}, [0] * self.pages
+        for number, (pages, tokens) in enumerate(tables):
+            pages = [int(page) for page in pages]
+            need(len(pages) == -(-count(tokens, "tokens") // self.page_tokens), "the pages do not hold the tokens")
+            real = [page for page in pages if page != HOLE]
+            need(all(0 <= page < self.pages for page in real), "a page lies outside the pool")
+            need(len(set(real)) == len(real), "a sequence has a page twice")
+            need(not pages or pages[-1] != HOLE, "the last page of a sequence cannot be a hole")
+            for page in real:
+                uses[page] += 1
+            loaded[number] = _Sequence(pages, tokens)
+        self._sequences, self._uses, self._next = loaded, uses, len(loaded)
+        self._free = [page for page, n in enumerate(uses) if not n]
+        self._moved += 1
+        return list(loaded)
+
+    def page_table(self, sequences):
+        """int32 ``[sequences, most pages]`` on the device; :data:`HOLE` behind a sequence's last page."""
+        found = [self._get(s) for s in sequences]
+        need_gpu(self.device, "a paged cache")
+        table = np.full((len(found), max((len(item.pages) for item in found), default=0)), HOLE, dtype=np.int32)
+        for row, item in zip(table, found):
+            row[:len(item.pages)] = item.pages
+        with entered(self.device):
+            return upload(table, self.device)
+
+    # -----------------------------------------------------------------------------------------
+    # Contents
+    # -----------------------------------------------------------------------------------------
+
+    def _layer(self, layer):
+        need(count(layer, "layer") < self.layers, "there is no such layer")
+        return self.keys[layer], self.values[layer]
+
+    def view(self, layer, target, sequence, start, tokens):
+        """The slot of ``tokens`` tokens of a sequence as a restore destination: a
+        :class:`~reelcache_amd.restore_model.NativeView` of the layer's K (``target="k"``) or V (``"v"``)
+        pool.  The tokens lie in one page, or in consecutive pages of a ``"BTHD"`` pool whose token rows
+        follow each other across pages (:meth:`make_contiguous`)."""
+        one_of(target, ("k", "v"), "target")
+        pool = self._layer(layer)[target == "v"]
+        found = self._get(sequence)
+        need(count(start, "start") + count(tokens, "tokens", minimum=1) <= found.tokens, "the view lies within the sequence")
+        first, last = start // self.page_tokens, (start + tokens - 1) // self.page_tokens
+        pages = found.pages[first:last + 1]
+        if HOLE in pages:
+            raise StateError("the view's page was dropped")
+        if any(self._uses[page] > 1 for page in pages):
+            raise StateError("the view's page is shared with another sequence")
+        offset = start - first * self.page_tokens
+        if first == last:
+            return NativeView(pool, self.layout, offset, pages[0])
+        joined = self.layout == "BTHD" and pool.stride(0) == self.page_tokens * pool.stride(1)
+        if not joined or any(b != a + 1 for a, b in zip(pages, pages[1:])):
+            raise StateError("the view's pages do not follow each other; see make_contiguous")
+        flat = pool.as_strided((self.pages * self.page_tokens, self.heads, self.head_dim), pool.stride()[1:])
+        return NativeView(flat, "THD", pages[0] * self.page_tokens + offset)
+
+    def store(self, layer, slots, keys, values, *, positions=None, grid=None):
+        """Write new tokens into their slots: ``keys`` turned by ``positions`` (interleaved pairs, as
+        :func:`reelcache_amd.rotary.rotate`; ``None`` stores them as they are) and ``values``, both
+        ``[tokens, heads, head_dim]`` of the cache's dtype, any strides.  With a ``grid`` the tokens are
+        one chunk."""
+        pools = self._layer(layer)
+        need(isinstance(slots, Slots) and slots.cache is self, "slots come from this cache")
+        if slots.stamp != self._moved + self._shared:
+            raise StateError("pages moved, were freed or became shared after these slots were built")
+        for x, name in ((keys, "keys"), (values, "values")):
+            strided(x, name)
+            need(x.shape == (slots.tokens, self.heads, self.head_dim) and x.dtype == self.dtype
+                 and x.device == self.device, f"{name} must be [tokens, heads, head_dim] of the cache's dtype and device")
+        if slots.tokens == 0:
+            return
+        need_gpu(self.device, "a paged cache")
+        with entered(self.device):
+            stream = torch.cuda.current_stream(self.device)
+            pairs, place = position_fields(positions, grid, slots.tokens, 1, self.head_dim, self.device, stream)
+            jobs = []
+            for x, pool, (turned, at) in zip((keys, values), pools, ((pairs, place), (0, (0,) * 16))):
+                x = x.detach()
+                if x.stride(2) != 1 and self.head_dim > 1:
+                    x = x.contiguous()
+                page, token, head = (pool.stride(axis - 1) for axis in self._axes)
+                jobs.append((x.data_ptr(), pool.data_ptr(), 1, slots.tokens, self.heads, self.head_dim, turned,
+                             0, x.stride(0), x.stride(1), page, token, head, *at, slots.index.data_ptr(),
+                             self.pages * self.page_tokens, self.page_tokens, 0, 0))
+            slots.index.record_stream(stream)
+            launch_rotary(jobs, self.dtype, "interleaved", stream)
+
+    # -----------------------------------------------------------------------------------------
+    # Attention
+    # -----------------------------------------------------------------------------------------
+
+    def plan(self, sequences, queries, *, heads, block=None, window=None, scale=None):
+        """The :class:`~reelcache_amd.attention.AttentionPlan` of one step: ``queries[i]`` new tokens (the
+        last ones) of ``sequences[i]`` attend to it.  Built once, used by :meth:`attend` in every layer."""
+        from .attention import AttentionPlan
+
+        return AttentionPlan(self, sequences, queries, heads=heads, block=block, window=window, scale=scale)
+
+    def attend(self, layer, q, plan, *, out=None, return_lse=False):
+        """:func:`reelcache_amd.attention.attend` over one layer."""
+        from .attention import attend
+
+        return attend(q, *self._layer(layer), plan, out=out, return_lse=return_lse)
+
+
+def _apart(pool):
+    """Whether every element of a strided tensor has a place of its own (strides sorted, each at least the
+    reach of those below it)."""
+    reach = 1
+    for stride, size in sorted((stride, size) for size, stride in zip(pool.shape, pool.stride()) if size > 1):
+        if stride < reach:
+            return False
+        reach = stride * (size - 1) + reach
+    return True
+
+
+def _pools(group, axes, pages, page_tokens):
+    """(device table of pool addresses, ``rch_pages`` fields) of pools with the same strides."""
+    size = group[0].element_size()
+    stride = group[0].stride()
+    page, token, head = (stride[axis] * size for axis in axes)
+    heads, row = group[0].shape[axes[2]], group[0].shape[4] * size
+    addresses = [pool.data_ptr() + layer * stride[0] * size for pool in group for layer in range(pool.shape[0])]
+    if _capturing():
+        raise ConfigurationError("a cache's first page copy cannot be captured: it uploads the pools' addresses")
+    table = torch.tensor(addresses, dtype=torch.int64).to(group[0].device)  # waits: usable on every stream
+    joined = head == row or heads == 1  # a token's heads are one run
+    segments, segment, width = (1, 0, heads * row) if joined else (heads, head, row)
+    mix = 0
+    for address in addresses:
+        mix |= address
+    fields = (table.data_ptr(), len(addresses), pages, page if pages > 1 else 0, page_tokens, segments, segment,
+              token if page_tokens > 1 else width, width, mix)
+    return table, (ctypes.c_int64 * len(fields))(*fields)
+
+
+__all__ = ["HOLE", "PagedCache", "Slots"]

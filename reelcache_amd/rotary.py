@@ -1,0 +1,267 @@
+"""Rotation of queries and keys by positions of several axes (frame, height, width), with gradients.
+
+The restore kernels rotate archived keys as they write them (reelcache/restore_kernels.py:1401-1444,
+:1557-1585); an engine has to turn the queries and keys of its new tokens by the same tables before
+they meet.  :func:`rotate` does that for any layout, for one tensor or for several in one launch
+(``rch_rotary``).  Places come from the job model of the restore:
+
+* :class:`~reelcache_amd.restore_model.RopePositions`: a chunk's first rows, with ``grid`` the token
+  grid of a separable table (a dense table takes one row per token);
+* :class:`TokenRows`: a place of its own for every token, for packed pictures and videos of several
+  sizes, single tokens of several sequences, or text between them.
+
+Arithmetic: fp32 products rounded apart and one rounding to the tensor's type, as the restore rounds.
+The gradient is the rotation back of the output's gradient, by the same kernel.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import weakref
+from dataclasses import dataclass
+from typing import Any
+
+import torch
+
+from . import _lib
+from ._checks import count, need, one_of, strided
+from .errors import ConfigurationError, UnsupportedError
+from .restore_model import _AXES, LAYOUTS, OUTPUT_DTYPES, RopePositions, RopeTable
+
+PAIRINGS = ("interleaved", "half")
+#: Most tensors of one call.
+MAX_TENSORS = 4
+
+_DTYPE_CODES = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32}
+_NULL = contextlib.nullcontext()
+
+
+@dataclass(frozen=True, eq=False)
+class TokenRows:
+    """A :class:`RopeTable` row for every token.
+
+    ``rows``: an int32 tensor on the tokens' device, ``[T, 3]`` or ``[B, T, 3]`` of (frame, height,
+    width) rows for a separable table, ``[T]`` or ``[B, T]`` for a dense one; any strides.  The values
+    stay on the device: a token whose row lies outside its axis turns to NaN.
+    """
+
+    table: RopeTable
+    rows: torch.Tensor
+
+    def __post_init__(self):
+        need(isinstance(self.table, RopeTable), "token rows require a RopeTable")
+        rows = strided(self.rows, "token rows")
+        need(rows.dtype == torch.int32, "token rows must be an int32 tensor")
+        last = 1 if self.table.sections is None else 2
+        need(rows.ndim in (last, last + 1), "token rows are [T, 3] or [B, T, 3] (separable table), [T] or [B, T] (dense)")
+        need(self.table.sections is None or rows.shape[-1] == 3, "separable token rows are (t_row, h_row, w_row)")
+
+    @property
+    def tokens(self):
+        return self.rows.shape[-1 if self.table.sections is None else -2]
+
+    @property
+    def batch(self):
+        """Sequences that have rows of their own, or None when all share them."""
+        return self.rows.shape[0] if self.rows.ndim == (2 if self.table.sections is None else 3) else None
+
+
+def entered(device):
+    """A context in which ``device`` is current (nothing to enter when it is already)."""
+    return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def need_gpu(device, what):
+    if device.type != "cuda":
+        raise UnsupportedError(f"{what} runs on the GPU (HIP, gfx950); move the tensors to a cuda device")
+    _lib.library()  # raises UnsupportedError with the reason when the library is unavailable
+
+
+# Streams that a table's device copy has been used on: its memory comes from the upload stream, so the
+# allocator has to know them before the copy is dropped (once per copy and stream).
+_TABLE_STREAMS: weakref.WeakKeyDictionary = weakref.WeakKeyDictionary()
+
+
+def _table_pairs(table, device, stream):
+    entry = table._kernel_block(device, stream)
+    used = _TABLE_STREAMS.setdefault(entry, set())
+    if stream.cuda_stream not in used:
+        entry.block.record_stream(stream)
+        used.add(stream.cuda_stream)
+    return entry.pairs
+
+
+def position_fields(positions, grid, tokens, batch, head_dim, device, stream):
+    """The place fields of ``rch_rotary_job`` (pairs_ptr .. rows_axis_stride) and the pair count."""
+    if positions is None:
+        return 0, (0,) * 16
+    need(isinstance(positions, (RopePositions, TokenRows)), "positions must be RopePositions or TokenRows")
+    table = positions.table
+    need(table.head_dim <= head_dim, "the table rotates more channels than a head has")
+    limits = (table.rows, 0, 0) if table.sections is None else table.section_rows
+    axes, sections = (1, (0, 0)) if table.sections is None else (3, table.sections[:2])
+    if isinstance(positions, TokenRows):
+        need(grid is None, "token rows take no grid")
+        rows = positions.rows
+        need(rows.device == device, "token rows must be on the tensors' device")
+        need(positions.tokens == tokens and positions.batch in (None, batch), "token rows do not match the tokens")
+        strides = rows.stride() if axes == 3 else (*rows.stride(), 0)
+        place = (0, 0, 0, 0, 0, rows.data_ptr(), strides[0] if len(strides) == 3 else 0, strides[-2], strides[-1])
+    elif axes == 1:
+        need(grid is None, "a dense table takes no grid")
+        need(positions.rows + tokens <= table.rows, "the tokens run past the RoPE table")
+        place = (positions.rows, 0, 0, 0, 0, 0, 0, 0, 0)
+    else:
+        need(grid is not None and len(grid) == 3, "a separable table needs the (frames, height, width) grid of the tokens")
+        for value in grid:
+            count(value, "grid extent", minimum=1)
+        need(grid[0] * grid[1] * grid[2] == tokens, "the grid does not hold the tokens")
+        for first, extent, limit, pairs in zip(positions.rows, grid, limits, table.sections):
+            need(pairs == 0 or first + extent <= limit, "the grid runs past the RoPE table")
+        place = (*positions.rows, grid[1], grid[2], 0, 0, 0, 0)
+    pairs = _table_pairs(table, device, stream)
+    return table.pairs, (pairs.data_ptr(), axes, *sections, *limits, *place)
+
+
+def launch_rotary(jobs, dtype, pairing, stream):
+    """One ``rch_rotary`` launch of ``jobs`` (rows of the struct's fields)."""
+    flat = [value for job in jobs for value in job]
+    _lib.call("rch_rotary", (ctypes.c_int64 * len(flat))(*flat), len(jobs), _DTYPE_CODES[dtype],
+              _lib.PAIRS_HALF if pairing == "half" else _lib.PAIRS_INTERLEAVED, stream.cuda_stream)
+
+
+def _geometry(x, layout):
+    """((batch, tokens, heads, head_dim), element strides of the same) of a tensor."""
+    shape, stride, axes = x.shape, x.stride(), _AXES[layout]
+    sizes = tuple(1 if axis is None else shape[axis] for axis in axes)
+    return sizes, tuple(0 if axis is None else stride[axis] for axis in axes)
+
+
+def _check(x, layout, name):
+    strided(x, name)
+    need(x.ndim == (3 if layout == "THD" else 4), f"{name}: {layout} has the wrong number of dimensions")
+    need(x.dtype in OUTPUT_DTYPES, f"{name} must be bfloat16, float16 or float32")
+
+
+def _span(x):
+    """Byte range [first, last) that a strided tensor touches."""
+    if x.numel() == 0:
+        return 0, 0
+    reach = sum((size - 1) * stride for size, stride in zip(x.shape, x.stride()))
+    return x.data_ptr(), x.data_ptr() + (reach + 1) * x.element_size()
+
+
+def _rotate(tensors, positions, grid, layout, pairing, inverse, outs):
+    """Launches the rotation of checked tensors into ``outs`` (or new tensors); returns the outputs."""
+    device = tensors[0].device
+    results, jobs, copies, places = [], [], [], {}
+    with entered(device):
+        stream = torch.cuda.current_stream(device)
+        for x, out in zip(tensors, outs):
+            (batch, tokens, heads, head_dim), strides = _geometry(x, layout)
+            if strides[3] != 1 and head_dim > 1:
+                x = x.contiguous()
+                strides = _geometry(x, layout)[1]
+            given = out
+            if out is None:
+                out = torch.empty_like(x)
+            to = _geometry(out, layout)[1]
+            if to[3] != 1 and head_dim > 1:  # written through a buffer
+                out = torch.empty(x.shape, dtype=x.dtype, device=device)
+                copies.append((given, out))
+                to = _geometry(out, layout)[1]
+            results.append(given if given is not None else out)
+            key = (tokens, batch, head_dim)
+            if key not in places:  # queries and keys of a call share them
+                places[key] = position_fields(positions, grid, tokens, batch, head_dim, device, stream)
+            pairs, place = places[key]
+            if batch and tokens and heads and head_dim:
+                jobs.append((x.data_ptr(), out.data_ptr(), batch, tokens, heads, head_dim, pairs, *strides[:3], *to[:3],
+                             *place, 0, 0, 0, int(inverse), 0))
+        if jobs:
+            launch_rotary(jobs, tensors[0].dtype, pairing, stream)
+        for given, out in copies:
+            given.copy_(out)
+    return tuple(results)
+
+
+class _Rotation(torch.autograd.Function):
+    """The rotation as a differentiable function of its tensors; linear, so the backward pass is the
+    rotation back (differentiable itself, as it goes through :func:`rotate`)."""
+
+    @staticmethod
+    def forward(ctx, positions, grid, layout, pairing, inverse, *tensors):
+        ctx.arguments = (positions, grid, layout, pairing, inverse)
+        ctx.set_materialize_grads(False)
+        if isinstance(positions, TokenRows):
+            ctx.save_for_backward(positions.rows)  # rows changed in place before the backward pass are refused
+        return _rotate(tensors, positions, grid, layout, pairing, inverse, (None,) * len(tensors))
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, grid, layout, pairing, inverse = ctx.arguments
+        ctx.saved_tensors  # noqa: B018  (checks the rows' version)
+        wanted = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[5 + i]]
+        out = [None] * len(grads)
+        if wanted:
+            turned = rotate(tuple(grads[i] for i in wanted), positions, grid=grid, layout=layout, pairing=pairing,
+                            inverse=not inverse)
+            for i, g in zip(wanted, turned):
+                out[i] = g
+        return (None,) * 5 + tuple(out)
+
+
+def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interleaved", inverse=False, out=None):
+    """Rotate one tensor, or a tuple of up to four in one launch (queries and keys), by ``positions``.
+
+    ``tensors``: bfloat16, float16 or float32 of one dtype and device in ``layout`` (``"BTHD"``,
+    ``"THD"`` or ``"BHTD"``), any strides; head counts may differ.  The first ``positions.table.head_dim``
+    channels of a head turn and the rest are copied.  ``pairing``: channels ``(2j, 2j + 1)`` turn
+    together (``"interleaved"``, as the restored caches have them) or ``(j, n + j)`` of the first ``2n``
+    (``"half"``).  ``inverse`` turns back.  ``out``: a tensor (or a tuple) of the same shapes to write
+    into, which may be the input itself; without it the outputs are new tensors.
+
+    Runs on the current stream of the tensors' device.  Differentiable in the tensors (not with
+    ``out``).  Returns a tensor, or a tuple for a tuple.
+    """
+    single = isinstance(tensors, torch.Tensor)
+    tensors = (tensors,) if single else tuple(tensors)
+    need(1 <= len(tensors) <= MAX_TENSORS, f"one call rotates 1 to {MAX_TENSORS} tensors")
+    one_of(layout, LAYOUTS, "layout")
+    one_of(pairing, PAIRINGS, "pairing")
+    need(isinstance(positions, (RopePositions, TokenRows)), "positions must be RopePositions or TokenRows")
+    first = tensors[0]
+    for x in tensors:
+        _check(x, layout, "a rotated tensor")
+        need(x.dtype == first.dtype and x.device == first.device, "the tensors of one call share dtype and device")
+    need_gpu(first.device, "the rotation")
+    grid = None if grid is None else tuple(grid)
+    if out is None:
+        if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
+            results = _Rotation.apply(positions, grid, layout, pairing, inverse, *tensors)
+        else:
+            results = _rotate(tensors, positions, grid, layout, pairing, inverse, (None,) * len(tensors))
+        return results[0] if single else results
+    outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
+    need(len(outs) == len(tensors), "out must have one tensor for each input")
+    if torch.is_grad_enabled() and any(x.requires_grad for x in (*tensors, *outs)):
+        raise ConfigurationError("out= is not differentiable; rotate without it, or under torch.no_grad()")
+    spans = [_span(x) for x in tensors]
+    for i, (x, o) in enumerate(zip(tensors, outs)):
+        _check(o, layout, "out")
+        need(o.shape == x.shape and o.dtype == x.dtype and o.device == x.device, "out must match its input")
+        need(all(stride != 0 or size <= 1 for size, stride in zip(o.shape, o.stride())),
+             "out with broadcast (zero) strides aliases itself")
+        low, high = _span(o)
+        for j, (a, b) in enumerate(spans):
+            same = i == j and o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+            need(same or high <= a or b <= low, "out overlaps an input without being it")
+        for other in outs[:i]:
+            a, b = _span(other)
+            need(high <= a or b <= low, "the outputs overlap")
+    _rotate(tensors, positions, grid, layout, pairing, inverse, outs)
+    return out
+
+
+__all__ = ["MAX_TENSORS", "PAIRINGS", "TokenRows", "rotate"]

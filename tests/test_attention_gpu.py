@@ -1,0 +1,335 @@
+"""``attention.attend`` on the GPU against its plain form in 64 bits."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from reelcache_amd import attention, paged_cache, rotary
+from reelcache_amd import restore_kernels as rk
+from reelcache_amd.errors import ConfigurationError, StateError
+
+import operator_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _cache(device, lengths, size, heads, dim, dtype, layout="BTHD", layers=1, seed=0, spare=2):
+    """A cache with scattered pages; every row that no sequence has is NaN."""
+    counts = [-(-n // size) for n in lengths]
+    pages = sum(counts) + spare
+    g = torch.Generator().manual_seed(seed)
+    rows = (size, heads) if layout == "BTHD" else (heads, size)
+    pools = [torch.randn((layers, pages, *rows, dim), generator=g).to(dtype).to(device) for _ in range(2)]
+    order = np.random.default_rng(seed).permutation(pages).tolist()
+    cuts = np.cumsum([0, *counts])
+    tables = [order[a:b] for a, b in zip(cuts[:-1], cuts[1:])]
+    cache = paged_cache.PagedCache(*pools, layout=layout)
+    cache.load_tables(list(zip(tables, lengths)))
+    for pool in pools:
+        pool = pool if layout == "BTHD" else pool.transpose(2, 3)
+        for page in order[cuts[-1]:]:
+            pool[:, page] = math.nan
+        for table, n in zip(tables, lengths):
+            if n % size:
+                pool[:, table[-1], n % size:] = math.nan
+    return cache
+
+
+def _check(cache, q, out, lse, lengths, queries, layer=0, **mask):
+    start = 0
+    for sequence, (length, n) in enumerate(zip(lengths, queries)):
+        rows = slice(start, start + n)
+        want, bound, logs, log_bound = oracle.attend(q[rows], cache.keys[layer], cache.values[layer],
+                                                     cache.pages_of(sequence), length, n, cache.page_tokens,
+                                                     layout=cache.layout, **mask)
+        assert oracle.worst(out[rows], want, bound) <= 0, (sequence, length, n)
+        if lse is not None:
+            assert oracle.worst(lse[rows], logs, log_bound) <= 0, (sequence, length, n)
+        start += n
+
+
+def _run(device, lengths, queries, size, kv_heads, group, dim, dtype, layout="BTHD", seed=0, **mask):
+    cache = _cache(device, lengths, size, kv_heads, dim, dtype, layout, seed=seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    q = torch.randn((sum(queries), kv_heads * group, dim), generator=g).to(dtype).to(device)
+    plan = cache.plan(list(range(len(lengths))), queries, heads=kv_heads * group, **mask)
+    out, lse = cache.attend(0, q, plan, return_lse=True)
+    _check(cache, q, out, lse, lengths, queries, **mask)
+    assert torch.equal(out, cache.attend(0, q, plan))  # and the same bits again
+    return cache, q, plan, out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size,kv_heads,group,dim,layout", [
+    (16, 2, 1, 64, "BTHD"), (64, 1, 4, 128, "BTHD"), (100, 2, 2, 80, "BHTD"), (7, 1, 3, 96, "BTHD"), (130, 3, 1, 128, "BHTD"),
+    (16, 1, 2, 20, "BTHD"), (9, 2, 1, 200, "BTHD"), (16, 1, 1, 7, "BHTD"), (64, 1, 1, 8, "BTHD"), (33, 1, 2, 104, "BTHD"),
+])
+def test_single_tokens(device, dtype, size, kv_heads, group, dim, layout):
+    """One token of sequences of one token to several tiles of keys."""
+    lengths = [1, 2, 31, 64, 65, 129, 300]
+    _run(device, lengths, [1] * len(lengths), size, kv_heads, group, dim, dtype, layout)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block", [None, 1, 40])
+@pytest.mark.parametrize("size,kv_heads,group,dim,layout", [
+    (16, 1, 1, 64, "BTHD"), (64, 1, 2, 128, "BTHD"), (100, 1, 1, 80, "BHTD"), (7, 1, 1, 128, "BTHD"), (16, 1, 1, 20, "BTHD"),
+    (150, 1, 1, 96, "BTHD"),
+])
+def test_chunks(device, dtype, block, size, kv_heads, group, dim, layout):
+    """Chunks alone, behind a history, and beside single tokens."""
+    _run(device, [70, 133, 260, 90, 40], [70, 129, 75, 1, 33], size, kv_heads, group, dim, dtype, layout, block=block)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [128, 64, 20])
+def test_windows(device, dtype, dim):
+    for window, block in ((1, 1), (63, 1), (50, None), (130, 16), (1 << 30, None)):
+        _run(device, [300, 20, 77], [140, 20, 1], 16, 1, 1, dim, dtype, window=window, block=block)
+    _run(device, [300, 20, 77], [140, 20, 1], 96, 1, 1, dim, dtype, window=33, block=1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size", [(128, 16), (128, 64), (64, 70), (20, 16)])
+def test_rows_that_see_nothing(device, dtype, dim, size):
+    """More queries than tokens under a causal mask, and an empty history: zeros and -inf."""
+    for lengths, queries in (([5, 0, 130], [9, 3, 140]), ([0], [1]), ([0, 3], [40, 50])):
+        cache, q, plan, out = _run(device, lengths, queries, size, 1, 2, dim, dtype, block=1)
+        assert not out[:max(0, queries[0] - lengths[0])].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size", [(128, 16), (64, 64), (128, 100), (20, 8)])
+def test_dropped_pages(device, dtype, dim, size):
+    """Pages that were dropped are not seen, whatever they hold now; a query may see only such pages."""
+    lengths, queries = [8 * size + 3, 3 * size], [size + 3, 1]
+    cache = _cache(device, lengths, size, 1, dim, dtype)
+    dropped = cache.pages_of(0)[2:5] + cache.pages_of(1)[:2]
+    cache.drop(0, 2, 3)
+    cache.drop(1, 0, 2)
+    for pool in (cache.keys, cache.values):
+        pool[:, dropped] = math.inf
+    q = torch.randn((sum(queries), 2, dim), generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
+    for mask in ({}, {"block": 1}, {"window": size}):
+        plan = cache.plan([0, 1], queries, heads=2, **mask)
+        out, lse = cache.attend(0, q, plan, return_lse=True)
+        _check(cache, q, out, lse, lengths, queries, **mask)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size", [(128, 16), (64, 64), (96, 150), (20, 8)])
+def test_hidden_rows_may_hold_anything(device, dtype, dim, size):
+    """Infinities and NaN in keys and values of tokens that a causal mask hides from earlier queries: those
+    queries are exact, the later ones get what arithmetic gives."""
+    lengths, queries = [210, 20], [150, 20]
+    cache = _cache(device, lengths, size, 1, dim, dtype)
+    q = torch.randn((170, 1, dim), generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
+    bad = 150  # place of the first bad token of sequence 0; its query is row 90
+    pages = cache.pages_of(0)
+    plain = cache.values[0].clone(), cache.keys[0].clone()
+    for at, value, which in ((bad, math.nan, "values"), (bad + 3, math.inf, "values"), (bad + 40, math.nan, "keys"),
+                             (bad + 41, -math.inf, "keys")):
+        getattr(cache, which)[0, pages[at // size], at % size, 0, at % dim] = value
+    plan = cache.plan([0, 1], queries, heads=1, block=1)
+    out = cache.attend(0, q, plan)
+    want, bound, _, _ = oracle.attend(q[:90], plain[1], plain[0], pages, 210, 150, size, block=1)
+    assert oracle.worst(out[:90], want[:90], bound[:90]) <= 0
+    assert out[90:93, 0, bad % dim].isnan().all() and out[131:150].isnan().any(dim=2).all()
+    other = torch.arange(dim, device=device) != bad % dim
+    assert out[90:93, 0, other].isfinite().all() and (out[93:130, 0, (bad + 3) % dim] == math.inf).all()
+    want, bound, _, _ = oracle.attend(q[150:], cache.keys[0], cache.values[0], cache.pages_of(1), 20, 20, size, block=1)
+    assert oracle.worst(out[150:], want, bound) <= 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_large_and_sharp_scores(device, dtype):
+    """Scores far apart (one key takes all), all equal, and growing along the keys, so that the running
+    reference moves in every tile."""
+    size, dim, n = 64, 64, 700
+    cache = _cache(device, [n], size, 1, dim, dtype)
+    pages = torch.tensor(cache.pages_of(0), device=device)
+    ramp = torch.linspace(-1, 1, len(pages) * size, device=device).view(-1, size)
+    q = torch.ones((200, 1, dim), device=device).to(dtype)
+    for scale in (1.0, 20.0):
+        cache.keys[0, pages, :, 0] = (ramp[..., None] * 3).expand(-1, -1, dim).to(dtype)
+        for queries in (200, 1):
+            for block in (None, 1):
+                plan = cache.plan([0], [queries], heads=1, block=block, scale=scale)
+                out, lse = cache.attend(0, q[:queries], plan, return_lse=True)
+                _check(cache, q[:queries], out, lse, [n], [queries], block=block, scale=scale)
+    cache.keys[0, pages] = 0
+    plan = cache.plan([0], [200], heads=1)
+    _check(cache, q, *cache.attend(0, q, plan, return_lse=True), [n], [200])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_histories_split(device, dtype):
+    """Keys split over many workgroups: single tokens and a short chunk over a long history."""
+    _run(device, [9000, 5, 4100], [1, 1, 1], 64, 1, 2, 128, dtype)
+    _run(device, [6000], [40], 16, 1, 1, 64, dtype, block=1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [128, 20])
+def test_strides_outputs_and_rows_behind(device, dtype, dim):
+    lengths, queries = [90, 33], [60, 1]
+    cache = _cache(device, lengths, 16, 2, dim, dtype, layers=2)
+    plan = cache.plan([0, 1], queries, heads=4)
+    wide = torch.randn((70, 5, 2 * dim), generator=torch.Generator().manual_seed(2)).to(dtype).to(device)
+    q = wide[:, 1:, dim:]  # strided, with rows behind the plan's
+    out, lse = cache.attend(1, q, plan, return_lse=True)
+    assert out.shape == q.shape and not out[61:].any() and (lse[61:] == -math.inf).all()
+    _check(cache, q, out, lse, lengths, queries, layer=1)
+    spread = wide[..., ::2][:, 1:, :]
+    _check(cache, spread, cache.attend(1, spread, plan), None, lengths, queries, layer=1)
+    for target in (torch.full((70, 4, dim), 7.0, dtype=dtype, device=device),
+                   torch.full((70, 6, dim + 8), 7.0, dtype=dtype, device=device)[:, 1:5, 8:],
+                   torch.full((70, 4, dim + 1), 7.0, dtype=dtype, device=device)[:, :, 1:],
+                   torch.full((70, 4, dim, 2), 7.0, dtype=dtype, device=device)[..., 1]):
+        assert cache.attend(1, q, plan, out=target) is target
+        assert torch.equal(target[:61], out[:61]) and (target[61:] == 7).all()
+    same = q.contiguous()
+    assert cache.attend(1, same, plan, out=same) is same and torch.equal(same[:61], out[:61])
+    odd = torch.empty(70 * 4 * dim + 1, dtype=dtype, device=device)[1:].view(70, 4, dim).copy_(q)
+    assert torch.equal(cache.attend(1, odd, plan), out)
+
+
+def test_pools_with_gaps_and_native_caches(device):
+    """Pools whose rows have room between them, unaligned pools (general form), and a native cache tensor
+    as a pool of one page that ends inside a tile."""
+    g = torch.Generator().manual_seed(0)
+    wide = [torch.randn((1, 6, 16, 3, 72), generator=g).bfloat16().to(device) for _ in range(2)]
+    q = torch.randn((40, 4, 64), generator=g).bfloat16().to(device)
+    for cut in (8, 3):
+        cache = paged_cache.PagedCache(*(p[:, :, :, 1:, cut:cut + 64] for p in wide))
+        cache.load_tables([([4, 0, 5], 45)])
+        plan = cache.plan([0], [40], heads=4, block=1)
+        _check(cache, q, cache.attend(0, q, plan), None, [45], [40], block=1)
+    for layout, shape in (("BTHD", (1, 275, 2, 64)), ("BHTD", (1, 2, 275, 64))):
+        native = [torch.randn(shape, generator=g).bfloat16().to(device) for _ in range(2)]
+        cache = paged_cache.PagedCache(*(p[None] for p in native), layout=layout)
+        cache.load_tables([([0], 270)])
+        plan = cache.plan([0], [40], heads=4)
+        _check(cache, q, cache.attend(0, q, plan), None, [270], [40])
+
+
+def test_parts_of_a_history_join_by_their_sums(device):
+    """Results over two caches joined by the returned logarithms equal attention over both."""
+    dim, n = 64, 150
+    cache = _cache(device, [n], 10, 1, dim, torch.float32)
+    q = torch.randn((50, 1, dim), generator=torch.Generator().manual_seed(2)).to(device)
+    pages = cache.pages_of(0)
+    whole, logs = cache.attend(0, q, cache.plan([0], [50], heads=1), return_lse=True)
+    parts = []
+    for part in (pages[:7], pages[7:]):
+        half = paged_cache.PagedCache(cache.keys, cache.values)
+        half.load_tables([(part, 10 * len(part))])
+        parts.append(half.attend(0, q, half.plan([0], [50], heads=1), return_lse=True))
+    (a, la), (b, lb) = [(o.double(), x.double()) for o, x in parts]
+    total = torch.logaddexp(la, lb)
+    joined = a * (la - total).exp()[..., None] + b * (lb - total).exp()[..., None]
+    _, bound, _, log_bound = oracle.attend(q, cache.keys[0], cache.values[0], pages, n, 50, 10)
+    assert oracle.worst(whole, joined.cpu(), 4 * bound) <= 0 and oracle.worst(logs, total.cpu(), 4 * log_bound) <= 0
+
+
+def test_refusals(device):
+    cache = _cache(device, [20, 9], 8, 2, 64, torch.bfloat16)
+    plan = cache.plan([0, 1], [4, 1], heads=4)
+    q = torch.zeros((5, 4, 64), dtype=torch.bfloat16, device=device)
+    for bad in (q[:4], q[:, :2], q[..., :32], q.float(), q.cpu(), q[0]):
+        with pytest.raises(ConfigurationError):
+            cache.attend(0, bad, plan)
+    for out in (q.float(), torch.zeros((6, 4, 64), dtype=torch.bfloat16, device=device), q[:, :1].expand(5, 4, 64)):
+        with pytest.raises(ConfigurationError):
+            cache.attend(0, q, plan, out=out)
+    long = torch.zeros((6, 4, 64), dtype=torch.bfloat16, device=device)
+    with pytest.raises(ConfigurationError, match="overlap"):
+        cache.attend(0, long[:5], plan, out=long[1:])
+    with pytest.raises(ConfigurationError):
+        attention.attend(q, cache.keys[0], cache.values[0], None)
+    with pytest.raises(ConfigurationError):
+        cache.attend(1, q, plan)
+    assert cache.attend(0, q[:0], cache.plan([], [], heads=4)).shape == (0, 4, 64)
+    cache.free(1)
+    with pytest.raises(StateError):
+        cache.attend(0, q, plan)
+
+
+def test_streams_and_captured_replays(device):
+    """Two captured calls that share a plan, replayed in turn with eager work between, and a call on
+    another stream."""
+    cache = _cache(device, [3000, 130], 64, 2, 128, torch.bfloat16, layers=2)
+    cache.keys.nan_to_num_(0.0), cache.values.nan_to_num_(0.0)
+    plan = cache.plan([0, 1], [1, 100], heads=4)
+    q = torch.randn((101, 4, 128), generator=torch.Generator().manual_seed(2)).bfloat16().to(device)
+    expected = cache.attend(0, q, plan)
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        other = cache.attend(0, q, plan)
+    stream.synchronize()
+    assert torch.equal(other, expected)
+    graphs, outs = [], []
+    for layer in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(cache.attend(layer, q, plan))
+        graphs.append(graph)
+    for replay in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(10 + replay)))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize(device)
+        for layer in range(2):
+            assert torch.equal(outs[layer], cache.attend(layer, q, plan))
+    first, second = torch.cuda.Stream(device), torch.cuda.Stream(device)
+    torch.cuda.synchronize(device)
+    for graph, side in zip(graphs, (first, second)):  # both at once
+        with torch.cuda.stream(side):
+            graph.replay()
+    torch.cuda.synchronize(device)
+    for layer in range(2):
+        assert torch.equal(outs[layer], cache.attend(layer, q, plan))
+
+
+def test_a_step_of_two_layers(device):
+    """The operators as an engine uses them: history restored into pages, the new chunk's queries and keys
+    rotated, keys and values stored, attention, then a fork that goes on alone."""
+    grid, heads, dim, size = (1, 6, 7), 2, 64, 16
+    n = 42
+    cos, sin, sections = oracle.tables(32, dim // 2)
+    table = rk.RopeTable(cos, sin, sections)
+    cache = paged_cache.PagedCache(*(torch.zeros(2, 16, size, heads, dim, dtype=torch.bfloat16, device=device) for _ in range(2)))
+    g = torch.Generator().manual_seed(0)
+    raw = [[torch.randn((3 * n, heads, dim), generator=g).bfloat16().to(device) for _ in range(2)] for _ in range(2)]
+    a = cache.new()
+    cache.extend([a], [n])
+    for layer, (k, v) in enumerate(raw):
+        jobs = [rk.ReconstructionJob(rk.DenseSource(x[:n].reshape(n, -1)), cache.view(layer, target, a, 0, n), grid, rope=rope)
+                for x, target, rope in zip((k, v), "kv", (rk.RopePositions(table, 0), None))]
+        rk.reconstruct(jobs).release()
+    b = None
+    for chunk in (1, 2):
+        sequence = a if chunk == 1 else b
+        slots, positions = cache.extend([sequence], [n]), rk.RopePositions(table, chunk)
+        plan = cache.plan([sequence], [n], heads=2 * heads)
+        rows = slice(chunk * n, (chunk + 1) * n)
+        for layer, (k, v) in enumerate(raw):
+            q = torch.randn((n, 2 * heads, dim), generator=g).bfloat16().to(device)
+            turned = rotary.rotate(q, positions, grid=grid, layout="THD")
+            cache.store(layer, slots, k[rows], v[rows], positions=positions, grid=grid)
+            out = cache.attend(layer, turned, plan)
+            places = torch.cat([oracle.grid_rows((i, 0, 0), grid) for i in range(chunk + 1)])
+            angles = oracle.token_angles(cos, sin, sections, places)
+            keys = oracle.rotate(k[:rows.stop], *(x[:, None] for x in angles))[0].bfloat16()
+            want, bound, _, _ = oracle.attend(turned, keys[None], v[None, :rows.stop], [0], rows.stop, n, rows.stop)
+            # The stored keys may round the other way where the plain rotation lies at a border: one step of
+            # each key, through the score (both keys of a pair of scores) into the weights.
+            shift = 2 * dim ** -0.5 * 2 * oracle.U[torch.bfloat16] * float((keys.abs().amax(0).float().amax(0) * turned.cpu().abs().float().amax((0, 1))).sum())
+            assert oracle.worst(out, want, bound + shift * float(v.abs().max())) <= 0
+        if chunk == 1:
+            b = cache.fork(a)
+    assert cache.pages_of(a)[:5] == cache.pages_of(b)[:5] and cache.pages_of(a)[5] != cache.pages_of(b)[5]

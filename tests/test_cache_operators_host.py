@@ -1,0 +1,376 @@
+"""Host logic of the cache operators (page tables, slots, plans) and their refusals, without a GPU."""
+
+import contextlib
+import re
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+from reelcache_amd import _lib, attention, paged_cache, rotary
+from reelcache_amd import restore_kernels as rk
+from reelcache_amd.errors import CapacityError, ConfigurationError, StateError, UnsupportedError
+
+import operator_oracle as oracle
+
+HEADER = Path(__file__).resolve().parents[1] / "include" / "reelcache_hip.h"
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The cache's host side alone: tables stay on the CPU, page copies are carried out by torch."""
+    copies = []
+
+    def copy(self, moves):
+        copies.extend(moves)
+        for pool in (self.keys, self.values):
+            for source, target, rows in moves:
+                if self.layout == "BTHD":
+                    pool[:, target, :rows] = pool[:, source, :rows]
+                else:
+                    pool[:, target, :, :rows] = pool[:, source, :, :rows]
+
+    monkeypatch.setattr(paged_cache.PagedCache, "_copy", copy)
+    for module in (paged_cache, attention):
+        monkeypatch.setattr(module, "need_gpu", lambda device, what: None)
+        monkeypatch.setattr(module, "entered", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(paged_cache, "upload", lambda values, device: torch.from_numpy(np.asarray(values, dtype=np.int32)))
+    return copies
+
+
+def make(pages=8, size=4, heads=2, dim=8, layers=2, layout="BTHD", dtype=torch.float32):
+    rows = (size, heads) if layout == "BTHD" else (heads, size)
+    pools = [torch.randn((layers, pages, *rows, dim)).to(dtype) for _ in range(2)]
+    return paged_cache.PagedCache(*pools, layout=layout)
+
+
+def contents(cache, sequence):
+    """The K rows of a sequence in layer 0, gathered through its pages."""
+    pool = cache.keys[0] if cache.layout == "BTHD" else cache.keys[0].transpose(1, 2)
+    return torch.cat([pool[page] for page in cache.pages_of(sequence)])[:cache.tokens(sequence)].clone()
+
+
+def test_sequences_grow_share_and_copy(host):
+    cache = make()
+    a = cache.new()
+    slots = cache.extend([a], [6])
+    assert slots.index.tolist() == [0, 1, 2, 3, 4, 5] and slots.tokens == 6 and cache.pages_of(a) == [0, 1]
+    b, c = cache.fork(a), cache.fork(a)
+    before = contents(cache, a)
+    slots = cache.extend([b, c, a], [3, 1, 1])
+    # b and c copy the begun page; a is its last owner and goes on in it.
+    assert host == [(1, 2, 2), (1, 4, 2)]
+    assert [cache.pages_of(s) for s in (a, b, c)] == [[0, 1], [0, 2, 3], [0, 4]]
+    assert slots.index.tolist() == [10, 11, 12, 18, 6]
+    for s in (a, b, c):
+        assert torch.equal(contents(cache, s)[:6], before)
+    assert cache.free_pages == 3 and [cache.tokens(s) for s in (a, b, c)] == [7, 9, 7]
+    cache.free(b)
+    assert cache.free_pages == 5 and cache.pages_of(a) == [0, 1]
+    assert cache.extend([a], [0]).tokens == 0
+
+
+def test_a_full_last_page_is_not_copied(host):
+    cache = make()
+    a = cache.new()
+    cache.extend([a], [8])
+    b = cache.fork(a)
+    assert cache.extend([b], [1]).index.tolist() == [8] and host == []
+    cache.truncate(b, 5)  # now inside a page that a has too
+    assert cache.extend([b], [1]).index.tolist() == [9] and host == [(1, 2, 1)]
+
+
+def test_capacity_is_checked_before_anything_changes(host):
+    cache = make(pages=3)
+    a = cache.new()
+    cache.extend([a], [6])
+    b, c = cache.fork(a), cache.fork(a)
+    with pytest.raises(CapacityError, match="2 pages are needed and 1 are free"):
+        cache.extend([b, c], [1, 1])
+    assert host == [] and [cache.tokens(s) for s in (a, b, c)] == [6, 6, 6] and cache.free_pages == 1
+
+
+@pytest.mark.parametrize("layout", ["BTHD", "BHTD"])
+def test_compact_moves_the_highest_pages_down(host, layout):
+    cache = make(pages=10, layout=layout)
+    cache.load_tables([([9, 3], 7), ([0, 7, 9], 12), ([5], 2)])
+    kept = [contents(cache, s) for s in range(3)]
+    assert cache.compact() == [(5, 1), (7, 2), (9, 4)]
+    assert [cache.pages_of(s) for s in range(3)] == [[4, 3], [0, 2, 4], [1]]
+    assert all(torch.equal(contents(cache, s), kept[s]) for s in range(3))
+    assert cache.compact() == [] and cache.free_pages == 5
+    cache.extend([cache.new()], [4])
+    assert cache.pages_of(3) == [5]
+
+
+def test_make_contiguous_and_view(host):
+    cache = make(pages=10)
+    cache.load_tables([([7, 0, 4], 11), ([8], 4)])
+    kept = contents(cache, 0)
+    with pytest.raises(StateError, match="make_contiguous"):
+        cache.view(1, "k", 0, 0, 11)
+    one = cache.view(1, "k", 0, 4, 4)
+    assert one.layout == "BTHD" and one.batch_index == 0 and one.token_offset == 0
+    assert torch.equal(one.slot(4), cache.keys[1, 0])
+    assert cache.make_contiguous(0) == [(7, 1), (0, 2), (4, 3)]
+    assert torch.equal(contents(cache, 0), kept) and cache.make_contiguous(0) == []
+    view = cache.view(1, "v", 0, 2, 9)
+    assert view.layout == "THD" and torch.equal(view.slot(9), cache.values[1, 1:4].flatten(0, 1)[2:11])
+    view.slot(9).fill_(3)
+    assert (cache.values[1, 1:4].flatten(0, 1)[2:11] == 3).all()
+    with pytest.raises(CapacityError):
+        small = make(pages=4)
+        small.load_tables([([3, 0], 8)])
+        small.fork(0)
+        small.extend([small.new()], [4])
+        small.make_contiguous(0)
+    heads_first = make(layout="BHTD")
+    heads_first.load_tables([([1, 2], 8)])
+    with pytest.raises(StateError):
+        heads_first.view(0, "k", 0, 0, 8)
+    assert heads_first.view(0, "k", 0, 5, 3).layout == "BHTD"
+
+
+def test_holes(host):
+    cache = make()
+    a = cache.new()
+    cache.extend([a], [18])
+    cache.drop(a, 1, 2)
+    assert cache.pages_of(a) == [0, -1, -1, 3, 4] and cache.free_pages == 5
+    with pytest.raises(ConfigurationError):
+        cache.drop(a, 4, 1)
+    with pytest.raises(StateError, match="dropped"):
+        cache.slots([a], [3], [2])
+    with pytest.raises(StateError, match="dropped"):
+        cache.truncate(a, 6)
+    with pytest.raises(StateError):
+        cache.make_contiguous(a)
+    b = cache.fork(a)
+    assert cache.extend([b], [3]).index.tolist() == [1 * 4 + 2, 1 * 4 + 3, 2 * 4] and host == [(4, 1, 2)]
+    assert cache.page_table([a, b]).tolist() == [[0, -1, -1, 3, 4, -1], [0, -1, -1, 3, 1, 2]]
+
+
+def test_sequence_refusals(host):
+    cache = make()
+    a = cache.new()
+    cache.extend([a], [5])
+    for call in (lambda: cache.tokens(7), lambda: cache.fork("a"), lambda: cache.free(-1), lambda: cache.page_table([3])):
+        with pytest.raises(StateError):
+            call()
+    for call in (lambda: cache.extend([a, a], [1, 1]), lambda: cache.extend([a], [1, 2]), lambda: cache.extend([a], [-1]),
+                 lambda: cache.extend([a], [1.0]), lambda: cache.truncate(a, 6), lambda: cache.slots([a], [2], [4]),
+                 lambda: cache.drop(a, 1, 1), lambda: cache.view(2, "k", a, 0, 1), lambda: cache.view(0, "q", a, 0, 1),
+                 lambda: cache.load_tables([([0], 5)]), lambda: cache.load_tables([([0, 0], 5)]),
+                 lambda: cache.load_tables([([8], 2)]), lambda: cache.load_tables([([-2], 2)]),
+                 lambda: cache.load_tables([([0, -1], 5)])):
+        with pytest.raises(ConfigurationError):
+            call()
+    assert cache.pages_of(a) == [0, 1]
+    cache.fork(a)
+    with pytest.raises(StateError, match="shared"):
+        cache.slots([a], [0], [1])
+    with pytest.raises(StateError, match="shared"):
+        cache.view(0, "k", a, 0, 1)
+
+
+def test_stale_slots_are_refused(host):
+    cache = make()
+    a, b = cache.new(), cache.new()
+    slots = cache.extend([a], [5])
+    x = torch.zeros(5, 2, 8)
+    for change in (lambda: cache.fork(a), lambda: cache.free(b), cache.compact, lambda: cache.load_tables([([0, 1], 5)])):
+        slots = cache.slots([a], [4], [1]) if cache.pages_of(a) and cache._uses[cache.pages_of(a)[-1]] == 1 else slots
+        if change is cache.compact:  # nothing moves: nothing is stale
+            change()
+            continue
+        change()
+        with pytest.raises(StateError, match="after these slots"):
+            cache.store(0, slots, x, x)
+    other = make()
+    with pytest.raises(ConfigurationError, match="come from this cache"):
+        other.store(0, slots, x, x)
+
+
+def test_pool_refusals():
+    good = torch.zeros(1, 2, 4, 2, 8)
+    for keys, values in ((good[0], good[0]), (good, good.half()), (good, torch.zeros(1, 2, 4, 2, 16)),
+                         (good.int(), good.int()), (good, good[..., :0]), (good.expand(3, -1, -1, -1, -1), good.expand(3, -1, -1, -1, -1)),
+                         (torch.zeros(300).as_strided((1, 2, 4, 2, 8), (256, 128, 32, 16, 2)),) * 2,
+                         (torch.zeros(300).as_strided((1, 2, 4, 2, 8), (128, 32, 16, 8, 1)),) * 2):
+        with pytest.raises(ConfigurationError):
+            paged_cache.PagedCache(keys, values)
+    with pytest.raises(ConfigurationError):
+        paged_cache.PagedCache(good, good, layout="THD")
+    with pytest.raises(ConfigurationError):
+        paged_cache.PagedCache.allocate(0, 4, 2, 8, device="cpu")
+    paged_cache.PagedCache(good[:, :, :, :, :4], good[:, :, :, :, :4])  # gaps are fine
+
+
+def test_cpu_tensors_are_refused():
+    cache = make()
+    a = cache.new()
+    table = rk.RopeTable(*oracle.tables(8, 4))
+    x = torch.zeros(1, 6, 2, 8)
+    for call in (lambda: cache.extend([a], [1]), lambda: cache.page_table([a]), lambda: cache.plan([a], [0], heads=2),
+                 lambda: rotary.rotate(x, rk.RopePositions(table, 0), grid=(1, 2, 3))):
+        with pytest.raises(UnsupportedError, match="GPU"):
+            call()
+
+
+def test_rotary_refusals(monkeypatch):
+    monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
+    monkeypatch.setattr(rotary, "entered", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(rotary, "_table_pairs", lambda table, device, stream: torch.zeros(table.rows, table.pairs, 2))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: None)
+    launches = []
+    monkeypatch.setattr(rotary, "launch_rotary", lambda jobs, *rest: launches.append(jobs))
+    cos, sin, sections = oracle.tables(8, 4)
+    table, dense = rk.RopeTable(cos, sin, sections), rk.RopeTable(cos, sin)
+    x, grid, at = torch.zeros(1, 6, 2, 8), (1, 2, 3), rk.RopePositions(table, 0)
+    rows = torch.zeros(6, 3, dtype=torch.int32)
+    rotary.rotate(x, at, grid=grid)
+    rotary.rotate(x, rotary.TokenRows(table, rows))
+    assert len(launches) == 2 and all(len(job) == len(_lib.ROTARY_FIELDS) for jobs in launches for job in jobs)
+    for call in (
+            lambda: rotary.rotate(x, table, grid=grid), lambda: rotary.rotate(x, at), lambda: rotary.rotate(x, at, grid=(1, 2, 2)),
+            lambda: rotary.rotate(x, at, grid=(0, 2, 3)), lambda: rotary.rotate(x, rk.RopePositions(table, (8, 0, 0)), grid=grid),
+            lambda: rotary.rotate(x, rk.RopePositions(dense, 3)), lambda: rotary.rotate(x, rk.RopePositions(dense, 0), grid=grid),
+            lambda: rotary.rotate(x, at, grid=grid, layout="HTD"), lambda: rotary.rotate(x[0], at, grid=grid),
+            lambda: rotary.rotate(x, at, grid=grid, pairing="whole"), lambda: rotary.rotate(x.double(), at, grid=grid),
+            lambda: rotary.rotate((x, x.half()), at, grid=grid), lambda: rotary.rotate((), at, grid=grid),
+            lambda: rotary.rotate((x,) * 5, at, grid=grid), lambda: rotary.rotate(x[..., :6], at, grid=grid),
+            lambda: rotary.rotate(x, rotary.TokenRows(table, rows[:5])), lambda: rotary.rotate(x, rotary.TokenRows(table, rows), grid=grid),
+            lambda: rotary.TokenRows(table, rows.long()), lambda: rotary.TokenRows(table, rows[:, :2]),
+            lambda: rotary.TokenRows(dense, torch.zeros(1, 2, 3, dtype=torch.int32)), lambda: rotary.TokenRows(None, rows),
+            lambda: rotary.rotate(x, rotary.TokenRows(table, rows[None].expand(2, 6, 3))),
+            lambda: rotary.rotate(x, at, grid=grid, out=x[..., :4]), lambda: rotary.rotate(x, at, grid=grid, out=(x, x)),
+            lambda: rotary.rotate(x, at, grid=grid, out=torch.zeros(1, 6, 1, 8).expand(1, 6, 2, 8)),
+            lambda: rotary.rotate(x, at, grid=grid, out=x.flip(1).as_strided(x.shape, x.stride()).requires_grad_(True))):
+        with pytest.raises(ConfigurationError):
+            call()
+    storage = torch.zeros(200)
+    a, b = (storage[i:i + 96].view(1, 6, 2, 8) for i in (0, 16))
+    for call in (lambda: rotary.rotate(a, at, grid=grid, out=b), lambda: rotary.rotate((a, x), at, grid=grid, out=(x, a)),
+                 lambda: rotary.rotate((x, x.clone()), at, grid=grid, out=(a, b))):
+        with pytest.raises(ConfigurationError, match="overlap"):
+            call()
+    assert len(launches) == 2
+
+
+def test_plan_refusals(host):
+    cache = make()
+    a = cache.new()
+    cache.extend([a], [9])
+    for call in (lambda: cache.plan([a], [1], heads=3), lambda: cache.plan([a], [1, 2], heads=2), lambda: cache.plan([a, a], [1, 1], heads=2),
+                 lambda: cache.plan([a], [-1], heads=2), lambda: cache.plan([a], [1], heads=2, block=0),
+                 lambda: cache.plan([a], [1], heads=2, window=0), lambda: cache.plan([a], [1], heads=2, scale=0.0),
+                 lambda: cache.plan([a], [1], heads=2, scale=float("nan")), lambda: cache.plan([a], [1], heads=2, block=1 << 31)):
+        with pytest.raises(ConfigurationError):
+            call()
+    with pytest.raises(UnsupportedError, match="256"):
+        wide = make(dim=264)
+        wide.plan([wide.new()], [0], heads=2)
+    plan = cache.plan([a], [1], heads=2)
+    cache.extend([a], [3])  # pages only added: the plan still holds
+    plan._check(cache.keys[0], cache.values[0])
+    with pytest.raises(ConfigurationError):
+        plan._check(cache.keys[0][:4], cache.values[0])
+    cache.truncate(a, 2)
+    with pytest.raises(StateError, match="after this plan"):
+        plan._check(cache.keys[0], cache.values[0])
+
+
+def _items(plan):
+    words = plan.buffer.numpy()
+    n = sum(plan._counts_of)
+    items = words[plan._items:plan._items + n * _lib.ATTEND_ITEM].reshape(n, _lib.ATTEND_ITEM)
+    merges = words[plan._merges:plan._merges + plan._n_merges * _lib.ATTEND_MERGE].reshape(-1, _lib.ATTEND_MERGE)
+    assert len(words) == plan._merges + merges.size and not words[:_lib.ATTEND_ZEROS].any()
+    return items, merges
+
+
+@pytest.mark.parametrize("size,dim,layout", [(16, 64, "BTHD"), (64, 128, "BTHD"), (100, 80, "BHTD"), (1560, 128, "BTHD"), (5, 20, "BTHD")])
+@pytest.mark.parametrize("block,window", [(None, None), (1, None), (37, None), (None, 50), (1, 200)])
+def test_plan_covers_every_visible_key_once(host, size, dim, layout, block, window):
+    """Items of a plan: every row of every sequence and head once per visible key, keys of a part within
+    its row block's range, parts of a block in disjoint partial rows, every split block merged once."""
+    lengths, queries, group, kv_heads = [1, 333, 700, 40, 0, 2000], [1, 333, 1, 9, 2, 300], 2, 2
+    pages = sum(-(-n // size) for n in lengths)
+    cache = make(pages=pages, size=size, heads=kv_heads, dim=dim, layers=1, layout=layout, dtype=torch.bfloat16)
+    sequences = [cache.new() for _ in lengths]
+    cache.extend(sequences, lengths)
+    plan = cache.plan(sequences, queries, heads=kv_heads * group, block=block, window=window)
+    items, merges = _items(plan)
+    words = plan.buffer.numpy()
+    starts = np.cumsum([0, *queries])
+    seen = {}
+    partial_rows = []
+    for table, length, q_row, n, begin, end, head, low, high, part, *_ in items.tolist():
+        number = [i for i in range(len(lengths)) if starts[i] == q_row and queries[i] == n and lengths[i] == length]
+        assert len(number) == 1 and 0 <= begin < end <= n * group and 0 <= low <= high <= length
+        assert words[table:table + -(-length // size)].tolist() == cache.pages_of(sequences[number[0]])
+        for row in range(begin, end):
+            seen.setdefault((number[0], head, row), []).append((low, high))
+        if part >= 0:
+            partial_rows += list(range(part, part + end - begin))
+            merge = [m for m in merges.tolist() if m[0] == q_row and m[1] == begin and m[3] == head and m[2] == end - begin]
+            assert len(merge) == 1 and (part - merge[0][4]) % (end - begin) == 0
+            assert 0 <= (part - merge[0][4]) // (end - begin) < merge[0][5]
+    assert sorted(partial_rows) == list(range(plan._partial_rows))
+    for number, (length, n) in enumerate(zip(lengths, queries)):
+        for head in range(kv_heads):
+            for row in range(n * group):
+                parts = sorted(seen.pop((number, head, row)))
+                place = length - n + row // group
+                last = min(length, (place // block + 1) * block) if block else length
+                first = max(0, place - window + 1) if window else 0
+                assert all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
+                if first < last:
+                    assert parts[0][0] <= first and parts[-1][1] >= last
+    assert not seen
+
+
+def test_header_matches_the_binding():
+    text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
+    for struct, fields in (("rch_rotary_job", _lib.ROTARY_FIELDS), ("rch_pages", _lib.PAGES_FIELDS), ("rch_attend", _lib.ATTEND_FIELDS)):
+        body = re.search(r"typedef struct " + struct + r" \{(.*?)\}", text, flags=re.S).group(1)
+        assert tuple(name.strip().split()[-1] for line in body.split(";") if line.strip() for name in line.split(",")) == fields
+    defines = {name: int(value) for name, value in re.findall(r"#define (RCH_[A-Z0-9_]+) (\d+)\b", HEADER.read_text())}
+    expected = {"RCH_PAIRS_INTERLEAVED": _lib.PAIRS_INTERLEAVED, "RCH_PAIRS_HALF": _lib.PAIRS_HALF,
+                "RCH_ATTEND_ITEM": _lib.ATTEND_ITEM, "RCH_ATTEND_MERGE": _lib.ATTEND_MERGE, "RCH_ATTEND_ZEROS": _lib.ATTEND_ZEROS,
+                "RCH_ATTEND_MAX_DIM": _lib.ATTEND_MAX_DIM, "RCH_ATTEND_FAST_DIM": _lib.ATTEND_FAST_DIM}
+    assert {name: defines.get(name) for name in expected} == expected
+    lib = _lib.library()
+    assert lib.rch_rotary_size() == 8 * len(_lib.ROTARY_FIELDS) and lib.rch_attend_size() == 8 * len(_lib.ATTEND_FIELDS)
+
+
+def test_abi_refusals():
+    """Bad arguments of the C entry points end in a status and a message, not in a launch."""
+    import ctypes
+
+    def words(fields, **values):
+        return (ctypes.c_int64 * len(fields))(*(values.get(f, 0) for f in fields))
+
+    good = dict(src_ptr=64, dst_ptr=64, batch=1, tokens=1, heads=1, head_dim=8, pairs=0)
+    for bad, count, dtype, pairing in ((dict(head_dim=0), 1, 0, 0), (dict(pairs=5), 1, 0, 0), (dict(pairs=2), 1, 0, 0),
+                                       (dict(slots_ptr=64), 1, 0, 0), ({}, 0, 0, 0), ({}, 5, 0, 0), ({}, 1, 3, 0), ({}, 1, 0, 2)):
+        with pytest.raises(ConfigurationError):
+            _lib.call("rch_rotary", words(_lib.ROTARY_FIELDS, **{**good, **bad}), count, dtype, pairing, None)
+    _lib.call("rch_rotary", words(_lib.ROTARY_FIELDS, **{**good, "tokens": 0}), 1, 0, 0, None)
+    pools = dict(pools_ptr=64, pools=1, pages=4, page_stride=64, page_rows=4, segments=1, row_stride=16, row_bytes=16)
+    for moves in ((0, 4, 1), (4, 0, 1), (-1, 0, 1), (0, 0, 1), (0, 1, 5), (0, 1, -1)):
+        with pytest.raises(ConfigurationError, match="outside the pool"):
+            _lib.call("rch_pages_copy", words(_lib.PAGES_FIELDS, **pools), (ctypes.c_int32 * 3)(*moves), 1, None)
+    with pytest.raises(ConfigurationError):
+        _lib.call("rch_pages_copy", words(_lib.PAGES_FIELDS, **{**pools, "row_stride": 8}), (ctypes.c_int32 * 3)(0, 1, 1), 1, None)
+    with pytest.raises(UnsupportedError):
+        _lib.call("rch_pages_copy", words(_lib.PAGES_FIELDS, **{**pools, "row_bytes": 1 << 30, "row_stride": 1 << 30}),
+                  (ctypes.c_int32 * 3)(0, 1, 1), 1, None)
+    _lib.call("rch_pages_copy", words(_lib.PAGES_FIELDS, **pools), None, 0, None)
+    step = dict(group=1, heads=1, head_dim=8, page_tokens=4, pages=1, n_general=1)
+    for bad, dtype in ((dict(head_dim=257), 0), (dict(page_tokens=0), 0), (dict(group=0), 0), (dict(n_merges=1), 0), ({}, 0),
+                       (dict(n_general=-1), 0)):
+        with pytest.raises(ConfigurationError):
+            _lib.call("rch_attend_run", words(_lib.ATTEND_FIELDS, **{**step, **bad}), dtype, None)
+    _lib.call("rch_attend_run", words(_lib.ATTEND_FIELDS, **{**step, "n_general": 0}), 0, None)

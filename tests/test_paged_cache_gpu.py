@@ -1,0 +1,179 @@
+"""``PagedCache`` on the GPU: page copies, stores into slots, restores into pages, captured calls."""
+
+import numpy as np
+import pytest
+import torch
+
+from reelcache_amd import paged_cache, rotary
+from reelcache_amd import restore_kernels as rk
+
+import operator_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _pools(device, layers, pages, size, heads, dim, dtype, layout, seed=0):
+    rows = (size, heads) if layout == "BTHD" else (heads, size)
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn((layers, pages, *rows, dim), generator=g).to(dtype).to(device) for _ in range(2)]
+
+
+def _token_major(pool, layout):
+    return pool if layout == "BTHD" else pool.transpose(2, 3)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 128), (torch.float16, 20), (torch.float32, 3), (torch.bfloat16, 1), (torch.bfloat16, 6)])
+@pytest.mark.parametrize("layout", ["BTHD", "BHTD"])
+@pytest.mark.parametrize("gap", [False, True])
+def test_copies_match_indexing(device, dtype, dim, layout, gap):
+    layers, pages, size, heads = 3, 9, 7, 3
+    if gap:  # rows with room behind them
+        keys, values = (p[..., :dim] for p in _pools(device, layers, pages, size, heads, dim + 8, dtype, layout))
+    else:
+        keys, values = _pools(device, layers, pages, size, heads, dim, dtype, layout)
+    cache = paged_cache.PagedCache(keys, values, layout=layout)
+    cache.load_tables([([8, 2], 10), ([7], 7)])
+    children = [cache.fork(0), cache.fork(0)]
+    expected = [_token_major(p, layout).clone() for p in (keys, values)]
+    cache.extend(children, [1, 5])  # pages 0 and 1 (three rows of page 2 each), then page 3
+    assert [cache.pages_of(c) for c in children] == [[8, 0], [8, 1, 3]]
+    for pool in expected:
+        pool[:, [0, 1], :3] = pool[:, 2:3, :3]
+    for pool, want in zip((keys, values), expected):
+        assert torch.equal(_token_major(pool, layout), want)
+    moves = cache.compact()
+    assert moves == [(7, 4), (8, 5)]
+    for pool in expected:
+        pool[:, [4, 5]] = pool[:, [7, 8]]
+    for pool, want in zip((keys, values), expected):
+        assert torch.equal(_token_major(pool, layout), want)
+    assert cache.page_table(children + [1]).tolist() == [[5, 0, -1], [5, 1, 3], [4, -1, -1]]
+
+
+def test_pools_of_different_strides_and_many_moves(device):
+    """K and V pools in different memory orders, and more moves than one launch carries."""
+    size, pages = 2, 700
+    keys = torch.randn(2, pages, size, 2, 8, device=device)
+    values = torch.randn(2, pages, 2, size, 8, device=device).transpose(2, 3)
+    cache = paged_cache.PagedCache(keys, values)
+    table = list(range(pages - 1, 349, -1))
+    cache.load_tables([(table, len(table) * size)])
+    before = [p[:, table].clone() for p in (keys, values)]
+    assert len(cache.compact()) == 350
+    after = cache.pages_of(0)
+    assert sorted(after) == list(range(350))
+    for pool, want in zip((keys, values), before):
+        assert torch.equal(pool[:, after], want)
+    before = [p[:, after].clone() for p in (keys, values)]
+    assert len(cache.make_contiguous(0)) == 350 and cache.pages_of(0) == list(range(350, 700))
+    for pool, want in zip((keys, values), before):
+        assert torch.equal(pool[:, 350:], want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["BTHD", "BHTD"])
+@pytest.mark.parametrize("size,heads,dim,rotated", [(16, 3, 64, 64), (5, 1, 22, 14), (7, 2, 80, 40)])
+def test_store_writes_slots_and_nothing_else(device, dtype, layout, size, heads, dim, rotated):
+    pages = 12
+    keys, values = _pools(device, 2, pages, size, heads, dim, dtype, layout)
+    cache = paged_cache.PagedCache(keys, values, layout=layout)
+    cache.load_tables([([7, 3], 2 * size - 2), ([11, 0, 4], 2 * size + 1), ([], 0)])
+    counts = [size, 3, 0]
+    slots = cache.extend([0, 1, 2], counts)
+    n = sum(counts)
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn((n, heads, dim), generator=g).to(dtype).to(device) for _ in range(2))
+    cos, sin, sections = oracle.tables(20, rotated // 2)
+    table = rk.RopeTable(cos, sin, sections)
+    rows = torch.randint(0, 20, (n, 3), generator=g, dtype=torch.int32)
+    before = [_token_major(p, layout).clone() for p in (keys, values)]
+    cache.store(1, slots, k, v, positions=rotary.TokenRows(table, rows.to(device)))
+    turned = rotary.rotate(k, rotary.TokenRows(table, rows.to(device)), layout="THD")
+    c, s = oracle.token_angles(cos, sin, sections, rows)
+    assert oracle.worst(turned, *oracle.rotate(k, c[:, None], s[:, None])) <= 0
+    at = slots.index.long().cpu()
+    page, row = at // size, at % size
+    assert at.tolist()[:2] == [3 * size + size - 2, 3 * size + size - 1]
+    for pool, want, x in zip((keys, values), before, (turned, v)):
+        want[1, page, row] = x
+        assert torch.equal(_token_major(pool, layout), want)
+    # Again as they are, from strided rows.
+    wide = torch.randn((n, heads + 1, 2 * dim), generator=g).to(dtype).to(device)
+    cache.store(0, slots, wide[:, 1:, ::2], wide[:, :heads, dim:])
+    for pool, x in zip((keys, values), (wide[:, 1:, ::2], wide[:, :heads, dim:])):
+        assert torch.equal(_token_major(pool, layout)[0, page, row], x)
+
+
+def test_slots_outside_the_pool_are_dropped(device):
+    keys, values = _pools(device, 1, 4, 4, 2, 8, torch.float32, "BTHD")
+    cache = paged_cache.PagedCache(keys, values)
+    cache.load_tables([([0, 1], 8)])
+    slots = cache.slots([0], [2], [4])
+    slots.index.copy_(torch.tensor([2, -1, 16, 1 << 30], dtype=torch.int32))
+    before = keys.clone()
+    x = torch.ones(4, 2, 8, device=device)
+    cache.store(0, slots, x, x)
+    before[0, 0, 2] = 1
+    assert torch.equal(keys, before)
+
+
+def test_restore_into_pages_equals_store(device):
+    """A dense restore through :meth:`view` (consecutive pages, RoPE by the chunk's grid) and the store of
+    the same tokens write the same bits."""
+    grid, size, heads, dim = (2, 5, 6), 16, 3, 128
+    cos, sin, sections = oracle.tables(32, dim // 2)
+    table, n = rk.RopeTable(cos, sin, sections), 60
+    positions = rk.RopePositions(table, (4, 0, 1))
+    raw = [torch.randn(n, heads * dim, generator=torch.Generator().manual_seed(i)).bfloat16().to(device) for i in (1, 2)]
+    caches = [paged_cache.PagedCache(*(torch.zeros(1, 16, size, heads, dim, dtype=torch.bfloat16, device=device)
+                                       for _ in range(2))) for _ in range(2)]
+    for cache in caches:
+        cache.load_tables([([8, 1], 20), ([5], 16)])
+        cache.free(1)
+    slots = caches[0].extend([0], [n])
+    caches[0].store(0, slots, *(x.view(n, heads, dim) for x in raw), positions=positions, grid=grid)
+    caches[1].extend([0], [n])
+    caches[1].make_contiguous(0)
+    jobs = [rk.ReconstructionJob(rk.DenseSource(x), caches[1].view(0, target, 0, 20, n), grid, rope=rope)
+            for x, target, rope in zip(raw, "kv", (positions, None))]
+    rk.reconstruct(jobs).release()
+    for name in ("keys", "values"):
+        a, b = (torch.cat([getattr(c, name)[0, page] for page in c.pages_of(0)])[20:20 + n] for c in caches)
+        assert torch.equal(a, b) and a.any()
+
+
+def test_captured_store_and_copies(device):
+    keys, values = _pools(device, 2, 8, 4, 2, 64, torch.bfloat16, "BTHD")
+    cache = paged_cache.PagedCache(keys, values)
+    a = cache.new()
+    slots = cache.extend([a], [6])
+    k, v = (torch.randn(6, 2, 64, device=device).bfloat16() for _ in range(2))
+    cos, sin, sections = oracle.tables(16, 32)
+    table = rk.RopeTable(cos.to(device), sin.to(device), sections)
+    rows = torch.zeros(6, 3, dtype=torch.int32, device=device)
+    positions = rotary.TokenRows(table, rows)
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        cache.store(1, slots, k, v, positions=positions)
+    torch.cuda.synchronize(device)
+    rk.reserve_capture_staging(1 << 16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        cache.store(1, slots, k, v, positions=positions)
+        with pytest.raises(Exception, match="capture"):
+            cache.extend([a], [1])
+        with pytest.raises(Exception, match="capture"):
+            cache.slots([a], [0], [1])
+    assert cache.tokens(a) == 6
+    for replay in range(3):
+        k.copy_(torch.randn(6, 2, 64, generator=torch.Generator().manual_seed(replay)))
+        rows.fill_(replay + 1)
+        keys.zero_()
+        graph.replay()
+        torch.cuda.synchronize(device)
+        expected = torch.zeros_like(keys)
+        turned = rotary.rotate(k, positions, layout="THD")
+        expected[1, 0], expected[1, 1, :2] = turned[:4], turned[4:]
+        assert torch.equal(keys, expected)
