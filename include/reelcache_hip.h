@@ -603,7 +603,9 @@ typedef struct rch_attend {
     int64_t n_general, n_rows, n_tokens; /* items of the general, the row-tiled and the few-rows form, in order */
     int64_t merges, n_merges, most_rows; /* word index, count, most rows of a merge */
     int64_t holes;           /* 1: page tables may hold holes */
-} rch_attend;                /* 34 x int64 = 272 bytes */
+    int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64 */
+    int64_t reserved;
+} rch_attend;                /* 36 x int64 = 288 bytes */
 
 int rch_attend_size(void);
 int rch_attend_run(const rch_attend* args_host, int dtype, void* stream);

@@ -79,7 +79,7 @@ ATTEND_FIELDS = ("q_ptr", "k_ptr", "v_ptr", "out_ptr", "lse_ptr", "plan_ptr", "p
                  "q_head_stride", "k_page_stride", "k_token_stride", "k_head_stride", "v_page_stride", "v_token_stride",
                  "v_head_stride", "out_token_stride", "out_head_stride", "group", "heads", "head_dim", "page_tokens",
                  "pages", "block", "window", "scale_bits", "partial_rows", "items", "n_general", "n_rows", "n_tokens",
-                 "merges", "n_merges", "most_rows", "holes")
+                 "merges", "n_merges", "most_rows", "holes", "tile_unit", "reserved")
 ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 128
 PAIRS_INTERLEAVED, PAIRS_HALF = 0, 1
 

@@ -114,7 +114,9 @@ class AttentionPlan:
                       for pool in (cache.keys, cache.values))
         if not (aligned and cache.head_dim % 8 == 0 and cache.head_dim <= _lib.ATTEND_FAST_DIM):
             return "general"
-        return "general"
+        if size == 4 or max(cache.keys.stride(cache._axes[1]), cache.values.stride(cache._axes[1])) > 1 << 23:
+            return "general"
+        return "rows"
 
     def _lay_out(self, found, queries):
         cache = self.cache
@@ -160,7 +162,8 @@ class AttentionPlan:
     def _unit(self):
         """Tokens that tiles of keys start over at: a page where tiles stay within pages, else a tile."""
         size = self.cache.page_tokens
-        return size if size >= KEY_TILE else KEY_TILE
+        # A page's last tile is part empty; beyond an eighth of the page, tiles across pages cost less.
+        return size if -(-size // KEY_TILE) * KEY_TILE * 8 <= 9 * size else KEY_TILE
 
     def _tile_of(self, key):
         """Index of the tile that holds ``key``, and the first key of a tile."""
@@ -336,7 +339,8 @@ def _launch(q, keys, values, plan, out, lse, stream):
               k[page], k[token], k[head], v[page], v[token], v[head], out.stride(0), out.stride(1),
               plan.group, plan.heads, cache.head_dim, cache.page_tokens, cache.pages, plan.block or 0, plan.window or 0,
               struct.unpack("<i", struct.pack("<f", plan.scale * math.log2(math.e)))[0], plan._partial_rows,
-              plan._items, *plan._counts_of, plan._merges, plan._n_merges, plan._most_rows, plan._holes)
+              plan._items, *plan._counts_of, plan._merges, plan._n_merges, plan._most_rows, plan._holes,
+              plan._unit(), 0)
     _lib.call("rch_attend_run", (ctypes.c_int64 * len(fields))(*fields), _DTYPE_CODES[q.dtype], stream.cuda_stream)
 
 

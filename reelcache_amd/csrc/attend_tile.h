@@ -1,0 +1,418 @@
+// Tiles of keys and values for the attention forms on the matrix cores (16-bit types).
+//
+// A wave works on 32 query rows, as the columns of the products:
+//   S^T [32 keys x 32 rows] = K [keys x D] Q^T    (v_mfma_f32_32x32x16: A = K from LDS, B = Q in registers)
+//   O^T [32 channels x 32 rows] += V^T [channels x keys] P^T
+// The lane of column n (lane % 32, half h = lane / 32) holds, of S^T, keys 8 (i / 4) + 4 h + i % 4 of its
+// row n for i = 0..15.  A product's inner index may run over the keys in any order that both operands
+// share, so registers 8 q .. 8 q + 7, rounded to 16 bits, are the B operand of keys 16 q .. 16 q + 15 as
+// they are, and the A operand V^T takes the same order: two transposed LDS reads of four keys each.
+// Everything a row's softmax needs lies in two lanes: maxima meet by one half-wave swap per tile, and
+// the sums only at the end.
+//
+// K and V rows travel from memory to LDS directly (buffer / global loads to LDS), 16 bytes a lane; the
+// lane order is the LDS order, so the bank swizzle is applied to the channel piece that a lane fetches:
+// piece c of row r lies at piece c ^ (r % pieces) in K (rows are read 8 at a time at one c) and at
+// c ^ 4 (r % 4) in V (rows are read 4 at a time, 64 bytes of each).
+#pragma once
+
+#include <type_traits>
+
+#include "attend.h"
+
+namespace rch {
+
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(4))) const int32_t const_int;
+
+template <int DT>
+struct Half;
+template <>
+struct Half<RCH_DT_BF16> {
+    typedef __bf16 type;
+    typedef bf8 vec8;
+    typedef __bf16 vec4 __attribute__((ext_vector_type(4)));
+    // Weights are rounded to bf16 for the second product: relative 2**-8 each, averaged over the keys.
+    static constexpr float kBias = 0.0f;
+    static constexpr uint32_t kExponent = 0x7f80u;
+    static __device__ __forceinline__ f16v mfma(vec8 a, vec8 b, f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Half<RCH_DT_F16> {
+    typedef _Float16 type;
+    typedef h8 vec8;
+    typedef _Float16 vec4 __attribute__((ext_vector_type(4)));
+    // fp16 weights carry a factor 2**7 (divided out with the sum): the largest is 2**15, and small ones stay
+    // above the subnormals down to 2**-21.
+    static constexpr float kBias = 7.0f;
+    static constexpr uint32_t kExponent = 0x7c00u;
+    static __device__ __forceinline__ f16v mfma(vec8 a, vec8 b, f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// The running reference of a row's exponents moves when a score passes it by more than 2**kSlack: any
+// reference gives the same quotient, and the sums are rarely multiplied.
+constexpr float kSlack = 8.0f;
+
+// The larger of the two lanes of a row.
+__device__ __forceinline__ float row_max(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(both[0]) + __uint_as_float(both[1]);
+}
+
+// 16 bytes a lane from memory to LDS at `lds` (wave-uniform) + 16 * lane, not waited for.  In assembly, so
+// that the compiler does not wait for them before every LDS read: the callers' own waits and barriers
+// order them.  Nothing is written but LDS.
+__device__ __forceinline__ void fetch_buffer(u4 rsrc, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void fetch_global(int64_t address, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(address) : "memory", "m0");
+}
+
+__device__ __forceinline__ u4 tile_rsrc(int64_t base, uint32_t bytes) {
+    u4 r;
+    r[0] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base));
+    r[1] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(base >> 32) & 0xffffu);
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);
+    r[3] = kBufferWord3;
+    return r;
+}
+
+// Where a row of queries stands: its token and head, the keys it sees.
+struct QueryRow {
+    int token, head, first, last;
+    bool valid;
+};
+
+__device__ __forceinline__ QueryRow query_row(const rch_attend& A, const AttendItem& I, int row) {
+    QueryRow R;
+    const int group = static_cast<int>(A.group);
+    R.valid = row < I.row_end;
+    const int r = R.valid ? row : I.row_end - 1;
+    R.token = r / group;
+    R.head = I.kv_head * group + r - R.token * group;
+    attend_range(A, I, R.token, R.first, R.last);
+    return R;
+}
+
+// A table entry by a per-lane index.
+__device__ __forceinline__ int page_entry(const const_int* table, int index) {
+    return gin<int32_t>(static_cast<int64_t>(reinterpret_cast<uintptr_t>(table)))[index];
+}
+
+// The walk over an item's key tiles.  PAGED: tiles of KT keys start over at each page and lie in one page
+// (its table entry is one scalar load); otherwise tiles are KT consecutive keys of any pages.
+template <int KT, bool PAGED>
+struct KeyWalk {
+    const const_int* table;
+    int unit, end, pages;  // tokens that tiles start over at, last key, pages of the pool
+    int page, off, id;     // current tile: its page index and first row there (PAGED), else key / unit and key % unit
+
+    __device__ __forceinline__ int base() const { return page * unit + off; }
+    __device__ __forceinline__ bool done() const { return base() >= end; }
+    __device__ __forceinline__ void settle() {  // skips dropped pages
+        if constexpr (PAGED) {
+            while (!done()) {
+                id = table[page];
+                if (id >= 0 && id < pages) return;
+                ++page;
+                off = 0;
+            }
+        }
+    }
+    __device__ __forceinline__ void begin(int key) {
+        page = key / unit;
+        off = (key - page * unit) / KT * KT;
+        settle();
+    }
+    // The next tile after `tiles` tiles.
+    __device__ __forceinline__ void next() {
+        off += KT;
+        if (off >= unit) {
+            ++page;
+            off = 0;
+            settle();
+        }
+    }
+    // Keys of the current tile.
+    __device__ __forceinline__ int count() const {
+        int n = end - base();
+        if constexpr (PAGED) n = min(n, unit - off);
+        return min(n, KT);
+    }
+};
+
+// Fetches the calling wave's share of a K and a V tile: NI instructions of 1024 bytes from instruction
+// `first` on.  RB: LDS bytes of a row.
+template <int KT, int RB, int NI, bool PAGED>
+struct Fetch {
+    static constexpr int kRows = 1024 / RB, kPieces = RB / 16;
+    uint32_t k_at[PAGED ? NI : 1], v_at[PAGED ? NI : 1];  // PAGED: byte offsets within the tile
+    int row0, k_piece, v_piece;                             // else: row of instruction 0, bytes of its piece (-1: none)
+    uint32_t magic;
+
+    __device__ __forceinline__ void init(const rch_attend& A, int first, int lane) {
+        const int pieces = static_cast<int>(A.head_dim) / 8;
+        row0 = first * kRows + lane / kPieces;
+        const int at = lane % kPieces;
+        // A wave's instructions are kRows rows apart: 4 or 8, and first * kRows is a multiple of 16, so the
+        // swizzles repeat where they depend on row % 4; K's takes the row of each instruction.
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int row = row0 + i * kRows;
+                const int kc = at ^ (row % kPieces), vc = at ^ v_swizzle(row);
+                k_at[i] = kc < pieces ? row * static_cast<uint32_t>(A.k_token_stride * 2) + kc * 16 : kOutOfRange;
+                v_at[i] = vc < pieces ? row * static_cast<uint32_t>(A.v_token_stride * 2) + vc * 16 : kOutOfRange;
+            }
+        } else {
+            k_piece = at;
+            v_piece = pieces;
+            const uint32_t size = static_cast<uint32_t>(A.page_tokens);
+            magic = (65536u + size - 1) / size;  // x / size for x < 128, size <= 64
+        }
+    }
+    static __device__ __forceinline__ int v_swizzle(int row) { return kPieces == 16 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
+
+    __device__ __forceinline__ void issue(const rch_attend& A, const KeyWalk<KT, PAGED>& W, int64_t k_head, int64_t v_head,
+                                          uint32_t k_lds, uint32_t v_lds) const {
+        if constexpr (PAGED) {
+            const int64_t k = k_head + 2 * (W.id * A.k_page_stride + W.off * A.k_token_stride);
+            const int64_t v = v_head + 2 * (W.id * A.v_page_stride + W.off * A.v_token_stride);
+            const int rows = W.count() - 1;
+            const uint32_t row_bytes = static_cast<uint32_t>(A.head_dim) * 2;
+            const u4 kr = tile_rsrc(k, rows * static_cast<uint32_t>(A.k_token_stride * 2) + row_bytes);
+            const u4 vr = tile_rsrc(v, rows * static_cast<uint32_t>(A.v_token_stride * 2) + row_bytes);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) fetch_buffer(kr, k_at[i], k_lds + i * 1024);
+#pragma unroll
+            for (int i = 0; i < NI; ++i) fetch_buffer(vr, v_at[i], v_lds + i * 1024);
+        } else {
+            const int base = W.base(), keys = W.end - base;
+            const int size = static_cast<int>(A.page_tokens);
+            const int page0 = base / size, off0 = base - page0 * size;
+            int id[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int row = row0 + i * kRows, x = off0 + row;
+                const int q = size > 64 ? (x >= size ? 1 : 0) : static_cast<int>((x * magic) >> 16);
+                id[i] = row < keys ? page_entry(W.table, page0 + q) : -1;
+            }
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int row = row0 + i * kRows, x = off0 + row;
+                const int q = size > 64 ? (x >= size ? 1 : 0) : static_cast<int>((x * magic) >> 16);
+                const int in_page = x - q * size;
+                const bool held = id[i] >= 0 && id[i] < A.pages;
+                const int kc = k_piece ^ (row % kPieces), vc = k_piece ^ v_swizzle(row);
+                const int64_t k = k_head + 2 * (id[i] * A.k_page_stride + in_page * A.k_token_stride) + kc * 16;
+                const int64_t v = v_head + 2 * (id[i] * A.v_page_stride + in_page * A.v_token_stride) + vc * 16;
+                // Rows that no page holds, and pieces behind the head, read the plan's zeros.
+                fetch_global(held && kc < v_piece ? k : A.plan_ptr, k_lds + i * 1024);
+                fetch_global(held && vc < v_piece ? v : A.plan_ptr, v_lds + i * 1024);
+            }
+        }
+    }
+};
+
+// One wave's state over the tiles and the arithmetic of a tile of KB * 32 keys.
+template <int DT, int NB, int KB>
+struct RowTile {
+    typedef Half<DT> H;
+    typedef typename H::type T;
+    typedef typename H::vec8 vec8;
+    typedef typename H::vec4 vec4;
+    static constexpr int RB = NB <= 2 ? 128 : 256, kPieces = RB / 16, KT = 32 * KB;
+
+    vec8 q[2 * NB];
+    f16v o[NB];
+    float reference, sum;
+    uint32_t k_lane[2 * NB], v_lane[NB];  // LDS byte offsets within a tile
+
+    __device__ __forceinline__ void init(const rch_attend& A, const AttendItem& I, const QueryRow& R, int lane) {
+        const int n = lane & 31, h = lane >> 5;
+        const int64_t at = A.q_ptr + 2 * ((I.q_row + R.token) * A.q_token_stride + R.head * A.q_head_stride);
+#pragma unroll
+        for (int s = 0; s < 2 * NB; ++s) {
+            const int d = 16 * s + 8 * h;
+            q[s] = __builtin_bit_cast(vec8, *gin<u4>(R.valid && d < A.head_dim ? at + 2 * d : A.plan_ptr));  // or zeros
+            k_lane[s] = n * RB + (((2 * s + h) ^ (n % kPieces)) * 16);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            v_lane[b] = value_offset(b, lane);
+            o[b] = f16v{};
+        }
+        reference = kNoReference;
+        sum = 0.0f;
+    }
+
+    // One tile.  [first, last): keys of the tile that the lane's row sees; held: keys in pages (bits).  masked
+    // (wave-uniform): whether a row of the wave may see fewer than all.  RARE: the values may be infinite or NaN
+    // where masked (the callers go on in a loop of its own then: its registers would cost the usual one).
+    template <bool RARE>
+    __device__ __forceinline__ void step(const lds_char* k_tile, const lds_char* v_tile, float scale, int first, int last,
+                                         uint64_t held, bool masked, int lane) {
+        const int h = lane >> 5;
+        f16v s[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            s[b] = f16v{};
+#pragma unroll
+            for (int c = 0; c < 2 * NB; ++c) {
+                const vec8 k = *reinterpret_cast<const __attribute__((address_space(3))) vec8*>(k_tile + k_lane[c] + b * 32 * RB);
+                s[b] = H::mfma(k, q[c], s[b]);
+            }
+        }
+        if (masked) {
+            uint32_t seen[KB];
+            seen_keys(seen, first, last, held, h);
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[b][i] = seen[b] >> i & 1u ? s[b][i] : -INFINITY;
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+        top = row_max(top) * scale - H::kBias;
+        if (__any(top > reference + kSlack)) {
+            const float next = fmaxf(reference, top), fade = exp2_of(reference - next);
+            reference = next;
+            sum *= fade;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[b][i] *= fade;
+        }
+        vec8 p[2 * KB];
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float w = exp2_of(__builtin_fmaf(s[b][i], scale, -reference));
+                part[i & 3] += w;
+                p[2 * b + (i >> 3)][i & 7] = static_cast<T>(w);
+            }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        if constexpr (RARE) {
+            if (masked) {
+                Rare rare;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) rare.o[b] = o[b];
+#pragma unroll
+                for (int c = 0; c < 2 * KB; ++c) rare.p[c] = p[c];
+                seen_keys(rare.seen, first, last, held, h);
+                add_infinite(&rare, v_tile, lane);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) o[b] = rare.o[b];
+                return;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 2 * KB; ++c)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b] = H::mfma(values(v_tile + v_lane[b], c), p[c], o[b]);
+    }
+
+    // Bit i of seen[b]: whether the row sees the key of register i of block b.
+    static __device__ __forceinline__ void seen_keys(uint32_t (&seen)[KB], int first, int last, uint64_t held, int h) {
+        // Bits of keys [first, last) of the tile, then those of this lane's half.
+        uint64_t bits = first >= 64 || last <= 0 || last <= first ? 0 : ~uint64_t{0} << max(first, 0);
+        if (last < 64) bits &= (uint64_t{1} << max(last, 0)) - 1;
+        bits &= held;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const uint32_t w = static_cast<uint32_t>(bits >> (32 * b)) >> (4 * h);
+            seen[b] = (w & 0xfu) | (w >> 4 & 0xf0u) | (w >> 8 & 0xf00u) | (w >> 12 & 0xf000u);
+        }
+    }
+
+    // Whether a value of the tile is infinite or NaN: with a weight of 0 (a key that a row does not see) its
+    // product would be NaN.
+    static __device__ __forceinline__ bool any_infinite(const lds_char* v_tile, int lane) {
+        uint32_t found = 0;
+#pragma unroll 4
+        for (int i = 0; i < KT * RB / 1024; ++i) {
+            const u4 raw = *reinterpret_cast<const __attribute__((address_space(3))) u4*>(v_tile + i * 1024 + lane * 16);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+                found |= ((raw[w] & H::kExponent) == H::kExponent) | ((raw[w] >> 16 & H::kExponent) == H::kExponent);
+        }
+        return __any(found != 0);
+    }
+
+    // The second product of a tile with infinite or NaN values: the finite ones as always, and beside them a
+    // product of ones for the keys that a row sees with a code for the others (1: inf, 128: -inf, 16384: NaN;
+    // at most 64 of each), from whose exact sum the channel's result follows.  A call through memory, out of
+    // the registers of the tiles' arithmetic.
+    struct Rare {
+        f16v o[NB];
+        vec8 p[2 * KB];
+        uint32_t seen[KB];
+    };
+    static __device__ __attribute__((noinline)) void add_infinite(Rare* rare, const lds_char* v_tile, int lane) {
+#pragma unroll 1
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t at = value_offset(b, lane);
+            f16v code = f16v{}, sum = rare->o[b];
+#pragma unroll 1
+            for (int c = 0; c < 2 * KB; ++c) {
+                vec8 v = values(v_tile + at, c), mark, one;
+                const uint32_t seen = rare->seen[c >> 1] >> (8 * (c & 1));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = static_cast<float>(v[e]);
+                    mark[e] = static_cast<T>(x != x ? 16384.0f : (x == INFINITY ? 1.0f : (x == -INFINITY ? 128.0f : 0.0f)));
+                    v[e] = __builtin_fabsf(x) < INFINITY ? v[e] : static_cast<T>(0.0f);
+                    one[e] = static_cast<T>(seen >> e & 1u ? 1.0f : 0.0f);
+                }
+                sum = H::mfma(v, rare->p[c], sum);
+                code = H::mfma(mark, one, code);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int n = static_cast<int>(code[i]);
+                if (n & 127) sum[i] += INFINITY;
+                if (n >> 7 & 127) sum[i] -= INFINITY;
+                if (n >= 16384) sum[i] = __builtin_nanf("");
+            }
+            rare->o[b] = sum;
+        }
+    }
+
+    // A lane's offset, within a tile, of the A operand V^T of channels 32 b .. 32 b + 31, and the operand of
+    // keys 16 c .. 16 c + 15 from there.
+    static __device__ __forceinline__ uint32_t value_offset(int b, int lane) {
+        const int p = lane & 15, key = 4 * (lane >> 5) + (p >> 2), half = (lane >> 4) & 1;
+        const int piece = (4 * b + 2 * half + ((p & 3) >> 1)) ^ Fetch<KT, RB, 1, true>::v_swizzle(key);
+        return key * RB + piece * 16 + (p & 1) * 8;
+    }
+    static __device__ __forceinline__ vec8 values(const lds_char* at, int c) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        const s4 low = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + c * 16 * RB));
+        const s4 high = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + c * 16 * RB + 8 * RB));
+        return __builtin_bit_cast(vec8, static_cast<s8>(__builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7)));
+    }
+
+    // Channel of register i of block b.
+    static __device__ __forceinline__ int channel_of(int b, int i, int h) { return 32 * b + 8 * (i >> 2) + 4 * h + (i & 3); }
+};
+
+}  // namespace rch
