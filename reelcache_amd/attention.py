@@ -112,9 +112,9 @@ class AttentionPlan:
         size = cache.keys.element_size()
         aligned = all(pool.data_ptr() % 16 == 0 and all(pool.stride(a) * size % 16 == 0 for a in range(4))
                       for pool in (cache.keys, cache.values))
-        if not (aligned and cache.head_dim % 8 == 0 and cache.head_dim <= _lib.ATTEND_FAST_DIM):
+        if not (aligned and cache.head_dim * size % 16 == 0 and cache.head_dim <= _lib.ATTEND_FAST_DIM):
             return "general"
-        if size == 4 or max(cache.keys.stride(cache._axes[1]), cache.values.stride(cache._axes[1])) > 1 << 23:
+        if max(cache.keys.stride(cache._axes[1]), cache.values.stride(cache._axes[1])) > 1 << 22:
             return "general"
         return "rows"
 

@@ -141,12 +141,9 @@ int run(const rch_attend& A, hipStream_t stream) {
         if (status != RCH_OK) return status;
         first += static_cast<int>(A.n_general);
     }
-    if constexpr (DT != RCH_DT_F32) {
-        if (A.n_rows) {
-            const int status = launch_attend_rows(A, DT, first, stream);
-            if (status != RCH_OK) return status;
-            first += static_cast<int>(A.n_rows);
-        }
+    if (A.n_rows) {
+        const int status = launch_attend_rows(A, DT, first, stream);
+        if (status != RCH_OK) return status;
     }
     if (A.n_merges) {
         const uint32_t blocks = static_cast<uint32_t>((A.most_rows * A.head_dim + 255) / 256);
@@ -182,11 +179,11 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
         const int64_t size = dtype == RCH_DT_F32 ? 4 : 2;
         const int64_t mix = A.q_token_stride | A.q_head_stride | A.k_page_stride | A.k_token_stride | A.k_head_stride
                             | A.v_page_stride | A.v_token_stride | A.v_head_stride | A.out_token_stride | A.out_head_stride;
-        if (dtype == RCH_DT_F32 || A.head_dim % 8 || A.head_dim > RCH_ATTEND_FAST_DIM || mix * size % 16
+        if (A.head_dim * size % 16 || A.head_dim > RCH_ATTEND_FAST_DIM || mix * size % 16
             || (A.q_ptr | A.k_ptr | A.v_ptr | A.out_ptr | A.plan_ptr) % 16)
-            return fail(RCH_E_UNSUPPORTED, "rch_attend_run: the tiled forms need aligned 16-bit rows of 8n <= %d channels",
+            return fail(RCH_E_UNSUPPORTED, "rch_attend_run: the tiled form needs aligned rows of whole 16-byte pieces and at most %d channels",
                         RCH_ATTEND_FAST_DIM);
-        if (A.k_token_stride < 0 || A.v_token_stride < 0 || A.k_token_stride > (1 << 23) || A.v_token_stride > (1 << 23))
+        if (A.k_token_stride < 0 || A.v_token_stride < 0 || A.k_token_stride > (1 << 22) || A.v_token_stride > (1 << 22))
             return fail(RCH_E_UNSUPPORTED, "rch_attend_run: token rows too far apart for the tiled forms");
         if (!(A.tile_unit == 64 || (A.tile_unit == A.page_tokens && A.page_tokens >= 64)))
             return fail(RCH_E_CONFIG, "rch_attend_run: tiles start over at a page of 64 or more tokens, or at 64 keys");

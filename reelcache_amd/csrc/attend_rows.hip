@@ -2,7 +2,7 @@
 // each over all keys of the item.
 //
 // Bound: the matrix cores (4 * D operations for every row and key) with the exponentials beside them.
-// A tile of 64 keys and values is fetched into one half of LDS while the waves work on the other half;
+// A tile of 64 (fp32: 32) keys and values is fetched into one half of LDS while the waves work on the other half;
 // one barrier to a tile.  Two workgroups fit a CU, so one's products cover the other's softmax.
 #include "attend_tile.h"
 
@@ -12,9 +12,8 @@ namespace {
 
 template <int DT, int NB, bool PAGED>
 __global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A, int first_item) {
-    typedef RowTile<DT, NB, 2> Tile;
-    typedef typename Tile::T T;
-    constexpr int RB = Tile::RB, KT = Tile::KT, kTileBytes = KT * RB, NI = kTileBytes / 1024 / 4;
+    typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2> Tile;
+    constexpr int RB = Tile::RB, KT = Tile::KT, ES = Tile::ES, kTileBytes = KT * RB, NI = kTileBytes / 1024 / 4;
     __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -30,9 +29,9 @@ __global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A,
     walk.end = I.key_end;
     walk.pages = static_cast<int>(A.pages);
     walk.begin(I.key_begin);
-    Fetch<KT, RB, NI, PAGED> fetch;
+    Fetch<Tile, NI, PAGED> fetch;
     fetch.init(A, wave * NI, lane);
-    const int64_t k_head = A.k_ptr + 2 * I.kv_head * A.k_head_stride, v_head = A.v_ptr + 2 * I.kv_head * A.v_head_stride;
+    const int64_t k_head = A.k_ptr + ES * I.kv_head * A.k_head_stride, v_head = A.v_ptr + ES * I.kv_head * A.v_head_stride;
     lds_char* const tiles = (lds_char*)lds;
     const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tiles)) + wave * NI * 1024;
 
@@ -95,17 +94,15 @@ __global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A,
         return;
     }
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int64_t to = A.out_ptr + 2 * ((I.q_row + R.token) * A.out_token_stride + R.head * A.out_head_stride);
-    typedef typename Tile::vec4 vec4;
+    const int64_t to = A.out_ptr + ES * ((I.q_row + R.token) * A.out_token_stride + R.head * A.out_head_stride);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             const int d = Tile::channel_of(b, i, h);
-            vec4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(tile.o[b][i + e] * inverse);
-            if (d < A.head_dim) *gout<u2>(to + 2 * d) = __builtin_bit_cast(u2, v);
+            if (d < A.head_dim)
+                Tile::store4(to + ES * d, f4{tile.o[b][i] * inverse, tile.o[b][i + 1] * inverse, tile.o[b][i + 2] * inverse,
+                                             tile.o[b][i + 3] * inverse});
         }
     if (h == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[(I.q_row + R.token) * A.heads + R.head] = row_lse(tile.reference, sum);
 }
@@ -128,6 +125,7 @@ void launch_dim(const rch_attend& A, int first, hipStream_t stream) {
 
 int launch_attend_rows(const rch_attend& A, int dtype, int first, hipStream_t stream) {
     if (dtype == RCH_DT_F16) launch_dim<RCH_DT_F16>(A, first, stream);
+    else if (dtype == RCH_DT_F32) launch_dim<RCH_DT_F32>(A, first, stream);
     else launch_dim<RCH_DT_BF16>(A, first, stream);
     return check_launch("rch_attend_run (rows)");
 }

@@ -154,46 +154,41 @@ struct KeyWalk {
 };
 
 // Fetches the calling wave's share of a K and a V tile: NI instructions of 1024 bytes from instruction
-// `first` on.  RB: LDS bytes of a row.
-template <int KT, int RB, int NI, bool PAGED>
+// `first` on.  Tile: the arithmetic's layout (ES: bytes of an element, RB: LDS bytes of a row, the swizzles).
+template <typename Tile, int NI, bool PAGED>
 struct Fetch {
-    static constexpr int kRows = 1024 / RB, kPieces = RB / 16;
+    static constexpr int KT = Tile::KT, RB = Tile::RB, ES = Tile::ES, kRows = 1024 / RB, kPieces = RB / 16;
     uint32_t k_at[PAGED ? NI : 1], v_at[PAGED ? NI : 1];  // PAGED: byte offsets within the tile
-    int row0, k_piece, v_piece;                             // else: row of instruction 0, bytes of its piece (-1: none)
+    int row0, piece, pieces;                                // row of instruction 0, the lane's piece, pieces of a head
     uint32_t magic;
 
     __device__ __forceinline__ void init(const rch_attend& A, int first, int lane) {
-        const int pieces = static_cast<int>(A.head_dim) / 8;
+        pieces = static_cast<int>(A.head_dim) * ES / 16;
         row0 = first * kRows + lane / kPieces;
-        const int at = lane % kPieces;
-        // A wave's instructions are kRows rows apart: 4 or 8, and first * kRows is a multiple of 16, so the
-        // swizzles repeat where they depend on row % 4; K's takes the row of each instruction.
+        piece = lane % kPieces;
         if constexpr (PAGED) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 const int row = row0 + i * kRows;
-                const int kc = at ^ (row % kPieces), vc = at ^ v_swizzle(row);
-                k_at[i] = kc < pieces ? row * static_cast<uint32_t>(A.k_token_stride * 2) + kc * 16 : kOutOfRange;
-                v_at[i] = vc < pieces ? row * static_cast<uint32_t>(A.v_token_stride * 2) + vc * 16 : kOutOfRange;
+                const int kc = piece ^ Tile::k_swizzle(row), vc = piece ^ Tile::v_swizzle(row);
+                k_at[i] = kc < pieces ? row * static_cast<uint32_t>(A.k_token_stride * ES) + kc * 16 : kOutOfRange;
+                v_at[i] = vc < pieces ? row * static_cast<uint32_t>(A.v_token_stride * ES) + vc * 16 : kOutOfRange;
             }
         } else {
-            k_piece = at;
-            v_piece = pieces;
             const uint32_t size = static_cast<uint32_t>(A.page_tokens);
             magic = (65536u + size - 1) / size;  // x / size for x < 128, size <= 64
         }
     }
-    static __device__ __forceinline__ int v_swizzle(int row) { return kPieces == 16 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
 
     __device__ __forceinline__ void issue(const rch_attend& A, const KeyWalk<KT, PAGED>& W, int64_t k_head, int64_t v_head,
                                           uint32_t k_lds, uint32_t v_lds) const {
         if constexpr (PAGED) {
-            const int64_t k = k_head + 2 * (W.id * A.k_page_stride + W.off * A.k_token_stride);
-            const int64_t v = v_head + 2 * (W.id * A.v_page_stride + W.off * A.v_token_stride);
+            const int64_t k = k_head + ES * (W.id * A.k_page_stride + W.off * A.k_token_stride);
+            const int64_t v = v_head + ES * (W.id * A.v_page_stride + W.off * A.v_token_stride);
             const int rows = W.count() - 1;
-            const uint32_t row_bytes = static_cast<uint32_t>(A.head_dim) * 2;
-            const u4 kr = tile_rsrc(k, rows * static_cast<uint32_t>(A.k_token_stride * 2) + row_bytes);
-            const u4 vr = tile_rsrc(v, rows * static_cast<uint32_t>(A.v_token_stride * 2) + row_bytes);
+            const uint32_t row_bytes = static_cast<uint32_t>(A.head_dim) * ES;
+            const u4 kr = tile_rsrc(k, rows * static_cast<uint32_t>(A.k_token_stride * ES) + row_bytes);
+            const u4 vr = tile_rsrc(v, rows * static_cast<uint32_t>(A.v_token_stride * ES) + row_bytes);
 #pragma unroll
             for (int i = 0; i < NI; ++i) fetch_buffer(kr, k_at[i], k_lds + i * 1024);
 #pragma unroll
@@ -215,16 +210,41 @@ struct Fetch {
                 const int q = size > 64 ? (x >= size ? 1 : 0) : static_cast<int>((x * magic) >> 16);
                 const int in_page = x - q * size;
                 const bool held = id[i] >= 0 && id[i] < A.pages;
-                const int kc = k_piece ^ (row % kPieces), vc = k_piece ^ v_swizzle(row);
-                const int64_t k = k_head + 2 * (id[i] * A.k_page_stride + in_page * A.k_token_stride) + kc * 16;
-                const int64_t v = v_head + 2 * (id[i] * A.v_page_stride + in_page * A.v_token_stride) + vc * 16;
+                const int kc = piece ^ Tile::k_swizzle(row), vc = piece ^ Tile::v_swizzle(row);
+                const int64_t k = k_head + ES * (id[i] * A.k_page_stride + in_page * A.k_token_stride) + kc * 16;
+                const int64_t v = v_head + ES * (id[i] * A.v_page_stride + in_page * A.v_token_stride) + vc * 16;
                 // Rows that no page holds, and pieces behind the head, read the plan's zeros.
-                fetch_global(held && kc < v_piece ? k : A.plan_ptr, k_lds + i * 1024);
-                fetch_global(held && vc < v_piece ? v : A.plan_ptr, v_lds + i * 1024);
+                fetch_global(held && kc < pieces ? k : A.plan_ptr, k_lds + i * 1024);
+                fetch_global(held && vc < pieces ? v : A.plan_ptr, v_lds + i * 1024);
             }
         }
     }
 };
+
+    // Bit i of seen[b]: whether the row sees the key of register i of block b.
+    template <int KB>
+__device__ __forceinline__ void seen_keys(uint32_t (&seen)[KB], int first, int last, uint64_t held, int h) {
+        // Bits of keys [first, last) of the tile, then those of this lane's half.
+        uint64_t bits = first >= 64 || last <= 0 || last <= first ? 0 : ~uint64_t{0} << max(first, 0);
+        if (last < 64) bits &= (uint64_t{1} << max(last, 0)) - 1;
+        bits &= held;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const uint32_t w = static_cast<uint32_t>(bits >> (32 * b)) >> (4 * h);
+            seen[b] = (w & 0xfu) | (w >> 4 & 0xf0u) | (w >> 8 & 0xf00u) | (w >> 12 & 0xf000u);
+        }
+    }
+
+// Adds what the codes of infinite and NaN values (below) say.
+__device__ __forceinline__ void add_marks(f16v& sum, const f16v& code) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int n = static_cast<int>(code[i]);
+        if (n & 127) sum[i] += INFINITY;
+        if (n >> 7 & 127) sum[i] -= INFINITY;
+        if (n >= 16384) sum[i] = __builtin_nanf("");
+    }
+}
 
 // One wave's state over the tiles and the arithmetic of a tile of KB * 32 keys.
 template <int DT, int NB, int KB>
@@ -233,7 +253,9 @@ struct RowTile {
     typedef typename H::type T;
     typedef typename H::vec8 vec8;
     typedef typename H::vec4 vec4;
-    static constexpr int RB = NB <= 2 ? 128 : 256, kPieces = RB / 16, KT = 32 * KB;
+    static constexpr int ES = 2, RB = NB <= 2 ? 128 : 256, kPieces = RB / 16, KT = 32 * KB;
+    static __device__ __forceinline__ int k_swizzle(int row) { return row % kPieces; }
+    static __device__ __forceinline__ int v_swizzle(int row) { return kPieces == 16 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
 
     vec8 q[2 * NB];
     f16v o[NB];
@@ -247,7 +269,7 @@ struct RowTile {
         for (int s = 0; s < 2 * NB; ++s) {
             const int d = 16 * s + 8 * h;
             q[s] = __builtin_bit_cast(vec8, *gin<u4>(R.valid && d < A.head_dim ? at + 2 * d : A.plan_ptr));  // or zeros
-            k_lane[s] = n * RB + (((2 * s + h) ^ (n % kPieces)) * 16);
+            k_lane[s] = n * RB + (((2 * s + h) ^ k_swizzle(n)) * 16);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -329,19 +351,6 @@ struct RowTile {
             for (int b = 0; b < NB; ++b) o[b] = H::mfma(values(v_tile + v_lane[b], c), p[c], o[b]);
     }
 
-    // Bit i of seen[b]: whether the row sees the key of register i of block b.
-    static __device__ __forceinline__ void seen_keys(uint32_t (&seen)[KB], int first, int last, uint64_t held, int h) {
-        // Bits of keys [first, last) of the tile, then those of this lane's half.
-        uint64_t bits = first >= 64 || last <= 0 || last <= first ? 0 : ~uint64_t{0} << max(first, 0);
-        if (last < 64) bits &= (uint64_t{1} << max(last, 0)) - 1;
-        bits &= held;
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const uint32_t w = static_cast<uint32_t>(bits >> (32 * b)) >> (4 * h);
-            seen[b] = (w & 0xfu) | (w >> 4 & 0xf0u) | (w >> 8 & 0xf00u) | (w >> 12 & 0xf000u);
-        }
-    }
-
     // Whether a value of the tile is infinite or NaN: with a weight of 0 (a key that a row does not see) its
     // product would be NaN.
     static __device__ __forceinline__ bool any_infinite(const lds_char* v_tile, int lane) {
@@ -384,13 +393,7 @@ struct RowTile {
                 sum = H::mfma(v, rare->p[c], sum);
                 code = H::mfma(mark, one, code);
             }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int n = static_cast<int>(code[i]);
-                if (n & 127) sum[i] += INFINITY;
-                if (n >> 7 & 127) sum[i] -= INFINITY;
-                if (n >= 16384) sum[i] = __builtin_nanf("");
-            }
+            add_marks(sum, code);
             rare->o[b] = sum;
         }
     }
@@ -399,7 +402,7 @@ struct RowTile {
     // keys 16 c .. 16 c + 15 from there.
     static __device__ __forceinline__ uint32_t value_offset(int b, int lane) {
         const int p = lane & 15, key = 4 * (lane >> 5) + (p >> 2), half = (lane >> 4) & 1;
-        const int piece = (4 * b + 2 * half + ((p & 3) >> 1)) ^ Fetch<KT, RB, 1, true>::v_swizzle(key);
+        const int piece = (4 * b + 2 * half + ((p & 3) >> 1)) ^ v_swizzle(key);
         return key * RB + piece * 16 + (p & 1) * 8;
     }
     static __device__ __forceinline__ vec8 values(const lds_char* at, int c) {
@@ -411,8 +414,146 @@ struct RowTile {
         return __builtin_bit_cast(vec8, static_cast<s8>(__builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7)));
     }
 
-    // Channel of register i of block b.
+    // Channel of register i of block b, and a row's channels i .. i + 3 into memory.
     static __device__ __forceinline__ int channel_of(int b, int i, int h) { return 32 * b + 8 * (i >> 2) + 4 * h + (i & 3); }
+    static __device__ __forceinline__ void store4(int64_t to, f4 v) {
+        vec4 r;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = static_cast<T>(v[e]);
+        *gout<u2>(to) = __builtin_bit_cast(u2, r);
+    }
+};
+
+// The same for fp32, 32 keys to a tile, by v_mfma_f32_32x32x2: its inner index is the lane's half alone, so a
+// 16-byte piece of K (and of Q) feeds four products, and register i of S^T is, as it is, the B operand of the
+// keys that registers i of both halves hold; V^T is read one value a lane.
+template <int NB>
+struct RowTile<RCH_DT_F32, NB, 1> {
+    typedef float T;
+    static constexpr int ES = 4, RB = NB <= 2 ? 256 : 512, kPieces = RB / 16, KT = 32;
+    static __device__ __forceinline__ int k_swizzle(int row) { return row % kPieces; }
+    // The two halves read keys 4 apart at the same channels: half a 256-byte bank row apart.
+    static __device__ __forceinline__ int v_swizzle(int row) { return ((row >> 2) & 1) * 8; }
+
+    f4 q[4 * NB];
+    f16v o[NB];
+    float reference, sum;
+    uint32_t k_lane, v_lane, k_turn;
+
+    __device__ __forceinline__ void init(const rch_attend& A, const AttendItem& I, const QueryRow& R, int lane) {
+        const int n = lane & 31, h = lane >> 5;
+        const int64_t at = A.q_ptr + 4 * ((I.q_row + R.token) * A.q_token_stride + R.head * A.q_head_stride);
+#pragma unroll
+        for (int s = 0; s < 4 * NB; ++s) {
+            const int d = 8 * s + 4 * h;
+            q[s] = __builtin_bit_cast(f4, *gin<u4>(R.valid && d < A.head_dim ? at + 4 * d : A.plan_ptr));  // or zeros
+        }
+        k_lane = n * RB;
+        k_turn = (k_swizzle(n) ^ h) * 16;
+        v_lane = 4 * h * RB + ((n >> 2) ^ v_swizzle(4 * h)) * 16 + (n & 3) * 4;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] = f16v{};
+        reference = kNoReference;
+        sum = 0.0f;
+    }
+
+    template <bool RARE>
+    __device__ __forceinline__ void step(const lds_char* k_tile, const lds_char* v_tile, float scale, int first, int last,
+                                         uint64_t held, bool masked, int lane) {
+        const int h = lane >> 5;
+        f16v s = f16v{};
+#pragma unroll
+        for (int c = 0; c < 4 * NB; ++c) {
+            const f4 k = *reinterpret_cast<const __attribute__((address_space(3))) f4*>(k_tile + k_lane + (k_turn ^ (c * 32)));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[c][j], s, 0, 0, 0);
+        }
+        uint32_t seen[1] = {0xffffu};
+        if (masked) {
+            seen_keys(seen, first, last, held, h);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = seen[0] >> i & 1u ? s[i] : -INFINITY;
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = row_max(top) * scale;
+        if (__any(top > reference + kSlack)) {
+            const float next = fmaxf(reference, top), fade = exp2_of(reference - next);
+            reference = next;
+            sum *= fade;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[b][i] *= fade;
+        }
+        float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = exp2_of(__builtin_fmaf(s[i], scale, -reference));
+            part[i & 3] += s[i];
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        if constexpr (RARE) {
+            if (masked) {
+                Rare rare;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) rare.o[b] = o[b];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) rare.p[i] = s[i];
+                rare.seen = seen[0];
+                add_infinite(&rare, v_tile, v_lane);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) o[b] = rare.o[b];
+                return;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(v_tile, v_lane, b, i), s[i], o[b], 0, 0, 0);
+    }
+
+    // Key 8 (i / 4) + 4 h + i % 4 (its row's swizzle depends on h alone), channel 32 b + lane % 32.
+    static __device__ __forceinline__ float value(const lds_char* v_tile, uint32_t v_lane, int b, int i) {
+        const uint32_t row = (8 * (i >> 2) + (i & 3)) * RB;
+        return *reinterpret_cast<const __attribute__((address_space(3))) float*>(v_tile + row + (v_lane ^ (b * 128)));
+    }
+
+    static __device__ __forceinline__ bool any_infinite(const lds_char* v_tile, int lane) {
+        uint32_t found = 0;
+#pragma unroll 4
+        for (int i = 0; i < KT * RB / 1024; ++i) {
+            const u4 raw = *reinterpret_cast<const __attribute__((address_space(3))) u4*>(v_tile + i * 1024 + lane * 16);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) found |= (raw[w] & 0x7f800000u) == 0x7f800000u;
+        }
+        return __any(found != 0);
+    }
+
+    struct Rare {
+        f16v o[NB];
+        float p[16];
+        uint32_t seen;
+    };
+    static __device__ __attribute__((noinline)) void add_infinite(Rare* rare, const lds_char* v_tile, uint32_t v_lane) {
+#pragma unroll 1
+        for (int b = 0; b < NB; ++b) {
+            f16v code = f16v{}, sum = rare->o[b];
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+                const float x = value(v_tile, v_lane, b, i);
+                const float mark = x != x ? 16384.0f : (x == INFINITY ? 1.0f : (x == -INFINITY ? 128.0f : 0.0f));
+                sum = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_fabsf(x) < INFINITY ? x : 0.0f, rare->p[i], sum, 0, 0, 0);
+                code = __builtin_amdgcn_mfma_f32_32x32x2f32(mark, rare->seen >> i & 1u ? 1.0f : 0.0f, code, 0, 0, 0);
+            }
+            add_marks(sum, code);
+            rare->o[b] = sum;
+        }
+    }
+
+    static __device__ __forceinline__ int channel_of(int b, int i, int h) { return 32 * b + 8 * (i >> 2) + 4 * h + (i & 3); }
+    static __device__ __forceinline__ void store4(int64_t to, f4 v) { *gout<f4>(to) = v; }
 };
 
 }  // namespace rch
