@@ -564,6 +564,11 @@ typedef struct rch_pages {
 #define RCH_PAGE_MOVES 256
 int rch_pages_copy(const rch_pages* pages_host, const int32_t* moves_host, int n_moves, void* stream);
 
+/* Writes count int32 words to the device; words_host is read before the call returns and travels in the
+ * launches' arguments, RCH_ARGUMENT_WORDS to a launch. */
+#define RCH_ARGUMENT_WORDS 960
+int rch_words_store(void* words_dev, const int32_t* words_host, int count, void* stream);
+
 /*
  * Attention of new tokens over a paged cache.  A plan is a device int32 buffer built by the host:
  * items (RCH_ATTEND_ITEM words each), merges (RCH_ATTEND_MERGE words each) and page tables; its first

@@ -30,8 +30,10 @@ def count(value: Any, name: str, minimum: int = 0) -> int:
 
 def strided(value: Any, name: str) -> torch.Tensor:
     """A strided tensor with real storage (no sparse layouts, no meta tensors)."""
-    need(isinstance(value, torch.Tensor) and value.layout == torch.strided, f"{name} must be a strided torch.Tensor")
-    need(value.device.type != "meta", f"{name} cannot be a meta tensor")
+    if not (isinstance(value, torch.Tensor) and value.layout == torch.strided):
+        raise ConfigurationError(f"{name} must be a strided torch.Tensor")
+    if value.is_meta:
+        raise ConfigurationError(f"{name} cannot be a meta tensor")
     return value
 
 

@@ -117,6 +117,7 @@ _SIGNATURES = {
     "rch_rotary_size": ([], _i),
     "rch_rotary": ([_p, _i, _i, _i, _p], _i),
     "rch_pages_copy": ([_p, _p, _i, _p], _i),
+    "rch_words_store": ([_p, _p, _i, _p], _i),
     "rch_attend_size": ([], _i),
     "rch_attend_run": ([_p, _i, _p], _i),
 }
@@ -190,21 +191,29 @@ def register(signatures: dict) -> None:
                 function.argtypes, function.restype = arguments, result
 
 
-def call(name: str, *arguments) -> None:
-    """Calls an entry point; maps a nonzero status to the declared error classes."""
-    lib = library()
-    function = getattr(lib, name, None)
-    if function is None:
+def function(name: str):
+    """The bound entry point ``name`` (for callers that keep it; its status goes to :func:`check`)."""
+    found = getattr(library(), name, None)
+    if found is None:
         raise UnsupportedError(f"{LIBRARY.name} does not export {name}; rebuild it")
-    status = function(*arguments)
+    return found
+
+
+def check(status: int) -> None:
+    """Maps a nonzero status to the declared error classes."""
     if status == OK:
         return
-    message = (lib.rch_last_error() or b"").decode(errors="replace")
+    message = (library().rch_last_error() or b"").decode(errors="replace")
     if status == E_CONFIG:
         raise ConfigurationError(message)
     if status == E_UNSUPPORTED:
         raise UnsupportedError(message)
     raise RuntimeError(f"HIP launch failed: {message}")
+
+
+def call(name: str, *arguments) -> None:
+    """Calls an entry point; maps a nonzero status to the declared error classes."""
+    check(function(name)(*arguments))
 
 
 def occupancy(precision: int, source_kind: int, max_ksteps: int, head_dim: int, out_dtype: int,

@@ -24,8 +24,8 @@ import torch
 
 from . import _lib
 from ._checks import count, need, strided
-from .errors import StateError, UnsupportedError
-from .rotary import _DTYPE_CODES, _span, entered, need_gpu
+from .errors import ConfigurationError, StateError, UnsupportedError
+from .rotary import _DTYPE_CODES, _span, entered, known_calls, need_gpu, raw_stream
 
 #: Keys of a tile: the step of every split of a sequence's keys.
 KEY_TILE = 64
@@ -156,8 +156,10 @@ class AttentionPlan:
                                 merges.ravel()])
         from .paged_cache import upload
 
+        self._tiled = counts["rows"] + counts["tokens"]
         with entered(cache.device):
             self.buffer = upload(words, cache.device)
+            self._stream = raw_stream(cache.device)
 
     def _unit(self):
         """Tokens that tiles of keys start over at: a page where tiles stay within pages, else a tile."""
@@ -250,13 +252,27 @@ class AttentionPlan:
 
     def _check(self, keys, values):
         cache = self.cache
-        if self._stamp != cache._moved:
-            raise StateError("pages moved or were freed after this plan was built")
         shape, k_stride, v_stride = cache.keys.shape[1:], cache.keys.stride()[1:], cache.values.stride()[1:]
         for pool, stride, name in ((keys, k_stride, "keys"), (values, v_stride, "values")):
             strided(pool, name)
             need(pool.shape == shape and pool.stride() == stride and pool.dtype == cache.dtype
                  and pool.device == cache.device, f"{name} must be a layer's pool like those of the plan's cache")
+            need(self._tiled == 0 or pool.data_ptr() % 16 == 0, f"{name} must be aligned as the plan's cache is")
+
+    def _fields(self, q_stride, out_stride):
+        """The ``rch_attend`` image of a call: everything but the addresses."""
+        cache = self.cache
+        page, token, head = cache._axes
+        k, v = cache.keys.stride(), cache.values.stride()
+        scale = struct.unpack("<i", struct.pack("<f", self.scale * math.log2(math.e)))[0]
+        fields = (0, 0, 0, 0, 0, 0, 0, *q_stride, k[page], k[token], k[head], v[page], v[token], v[head], *out_stride,
+                  self.group, self.heads, cache.head_dim, cache.page_tokens, cache.pages, self.block or 0, self.window or 0,
+                  scale, self._partial_rows, self._items, *self._counts_of, self._merges, self._n_merges, self._most_rows,
+                  self._holes, self._unit(), 0)
+        return bytes(_Image(*fields))
+
+
+_Image = ctypes.c_int64 * len(_lib.ATTEND_FIELDS)
 
 
 def attend(q, keys, values, plan, *, out=None, return_lse=False):
@@ -273,49 +289,77 @@ def attend(q, keys, values, plan, *, out=None, return_lse=False):
     """
     need(isinstance(plan, AttentionPlan), "attend needs an AttentionPlan")
     plan._check(keys, values)
+    return run(q, keys.data_ptr(), values.data_ptr(), plan, out, return_lse, (keys, values))
+
+
+def run(q, k_address, v_address, plan, out, return_lse, pools=None):
+    """:func:`attend` over a layer's checked pools, given by their addresses."""
     cache = plan.cache
+    if plan._stamp != cache._moved:
+        raise StateError("pages moved or were freed after this plan was built")
     strided(q, "q")
-    need(q.ndim == 3 and q.shape[0] >= plan.queries and q.shape[1] == plan.heads and q.shape[2] == cache.head_dim,
-         "q must be [rows, heads, head_dim] with a row for every query of the plan")
-    need(q.dtype == cache.dtype and q.device == cache.device, "q must have the cache's dtype and device")
+    shape = q.shape
+    if len(shape) != 3 or shape[0] < plan.queries or shape[1] != plan.heads or shape[2] != cache.head_dim:
+        raise ConfigurationError("q must be [rows, heads, head_dim] with a row for every query of the plan")
     device = cache.device
+    if q.dtype != cache.dtype or q.device != device:
+        raise ConfigurationError("q must have the cache's dtype and device")
     with entered(device):
-        stream = torch.cuda.current_stream(device)
-        given, q = q, _rows(q.detach())
-        more = q.shape[0] > plan.queries
+        given, q = q, _rows(q)
+        more = shape[0] > plan.queries
         result = out
         if out is None:
-            result = out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            result = out = torch.empty(shape, dtype=q.dtype, device=device)
             if more:
                 out[plan.queries:].zero_()
         else:
-            strided(out, "out")
-            need(out.shape == q.shape and out.dtype == q.dtype and out.device == device, "out must match q")
-            need(not out.requires_grad, "out must not require gradients")
-            need(all(stride != 0 or size <= 1 for size, stride in zip(out.shape, out.stride())),
-                 "out with broadcast (zero) strides aliases itself")
-            low, high = _span(out)
-            for x in (given, keys, values):
-                same = x is given and out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
-                first, last = _span(x)
-                need(same or high <= first or last <= low, "out overlaps an input without being q")
-            if not _aligned(out):
-                result = torch.empty(q.shape, dtype=q.dtype, device=device)
+            result = _output(out, given, pools or (cache.keys, cache.values))
         lse = None
         if return_lse:
-            lse = torch.empty((q.shape[0], plan.heads), dtype=torch.float32, device=device)
+            lse = torch.empty((shape[0], plan.heads), dtype=torch.float32, device=device)
             if more:
                 lse[plan.queries:].fill_(-math.inf)
         if plan.queries:
-            _launch(q, keys, values, plan, result, lse, stream)
+            known = known_calls(plan)
+            key = (q.stride(), result.stride())
+            image = known.get(key)
+            if image is None:
+                image = known[key] = plan._fields(q.stride()[:2], result.stride()[:2])
+            fields = _Image.from_buffer_copy(image)
+            partials = None
+            if plan._n_merges:
+                partials = torch.empty(plan._partial_rows * (cache.head_dim + 2), dtype=torch.float32, device=device)
+                fields[6] = partials.data_ptr()
+            stream = raw_stream(device)
+            if stream != plan._stream:  # the allocator learns of a stream that the tables were not made on
+                plan.buffer.record_stream(torch.cuda.current_stream(device))
+            fields[0], fields[1], fields[2], fields[3] = q.data_ptr(), k_address, v_address, result.data_ptr()
+            fields[4], fields[5] = 0 if lse is None else lse.data_ptr(), plan.buffer.data_ptr()
+            _lib.check(_lib.function("rch_attend_run")(fields, _DTYPE_CODES[q.dtype], stream))
             if result is not out:
                 out[:plan.queries].copy_(result[:plan.queries])
     return (out, lse) if return_lse else out
 
 
+def _output(out, q, pools):
+    """Where the kernels write for a given ``out``: itself, or a buffer when its rows are not aligned."""
+    strided(out, "out")
+    need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must match q")
+    need(not out.requires_grad, "out must not require gradients")
+    need(all(stride != 0 or size <= 1 for size, stride in zip(out.shape, out.stride())),
+         "out with broadcast (zero) strides aliases itself")
+    low, high = _span(out)
+    for x in (q, *pools):
+        same = x is q and out.data_ptr() == x.data_ptr() and out.stride() == x.stride()
+        first, last = _span(x)
+        need(same or high <= first or last <= low, "out overlaps an input without being q")
+    return out if _aligned(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
+
+
 def _aligned(x):
     size = x.element_size()
-    return (x.stride(2) == 1 and x.data_ptr() % 16 == 0 and x.stride(0) * size % 16 == 0 and x.stride(1) * size % 16 == 0)
+    a, b, c = x.stride()
+    return c == 1 and (x.data_ptr() | a * size | b * size) % 16 == 0
 
 
 def _rows(q):
@@ -324,24 +368,6 @@ def _rows(q):
     if _aligned(q) or (q.shape[2] * q.element_size() % 16 and (q.stride(2) == 1 or q.shape[2] == 1)):
         return q
     return q.clone(memory_format=torch.contiguous_format)
-
-
-def _launch(q, keys, values, plan, out, lse, stream):
-    cache = plan.cache
-    partials = None
-    if plan._n_merges:
-        partials = torch.empty(plan._partial_rows * (cache.head_dim + 2), dtype=torch.float32, device=q.device)
-    plan.buffer.record_stream(stream)
-    page, token, head = (axis - 1 for axis in cache._axes)
-    k, v = keys.stride(), values.stride()
-    fields = (q.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-              plan.buffer.data_ptr(), 0 if partials is None else partials.data_ptr(), q.stride(0), q.stride(1),
-              k[page], k[token], k[head], v[page], v[token], v[head], out.stride(0), out.stride(1),
-              plan.group, plan.heads, cache.head_dim, cache.page_tokens, cache.pages, plan.block or 0, plan.window or 0,
-              struct.unpack("<i", struct.pack("<f", plan.scale * math.log2(math.e)))[0], plan._partial_rows,
-              plan._items, *plan._counts_of, plan._merges, plan._n_merges, plan._most_rows, plan._holes,
-              plan._unit(), 0)
-    _lib.call("rch_attend_run", (ctypes.c_int64 * len(fields))(*fields), _DTYPE_CODES[q.dtype], stream.cuda_stream)
 
 
 __all__ = ["AttentionPlan", "attend"]

@@ -53,11 +53,35 @@ __global__ void __launch_bounds__(kThreads) pages_copy_kernel(rch_pages P, const
     }
 }
 
+// Words that travel in the launch's arguments: a table of a few hundred entries reaches the device without
+// pinned memory and without a copy engine.
+struct Words {
+    int32_t word[RCH_ARGUMENT_WORDS];
+};
+__global__ void __launch_bounds__(256) words_store_kernel(int64_t to, const Words words, int count) {
+    for (int i = threadIdx.x; i < count; i += 256) gout<int32_t>(to)[i] = words.word[i];
+}
+
 }  // namespace
 
 }  // namespace rch
 
 extern "C" {
+
+int rch_words_store(void* words_dev, const int32_t* words_host, int count, void* stream) {
+    using namespace rch;
+    if (count < 0 || (count > 0 && (!words_dev || !words_host))) return fail(RCH_E_CONFIG, "rch_words_store: invalid arguments");
+    for (int first = 0; first < count; first += RCH_ARGUMENT_WORDS) {
+        const int n = count - first < RCH_ARGUMENT_WORDS ? count - first : RCH_ARGUMENT_WORDS;
+        Words words;
+        for (int i = 0; i < n; ++i) words.word[i] = words_host[first + i];
+        const int64_t to = reinterpret_cast<int64_t>(words_dev) + 4 * static_cast<int64_t>(first);
+        hipLaunchKernelGGL(words_store_kernel, dim3(1), dim3(256), 0, as_stream(stream), to, words, n);
+        const int status = check_launch("rch_words_store");
+        if (status != RCH_OK) return status;
+    }
+    return RCH_OK;
+}
 
 int rch_pages_copy(const rch_pages* pages_host, const int32_t* moves_host, int n_moves, void* stream) {
     using namespace rch;

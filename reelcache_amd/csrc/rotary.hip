@@ -37,7 +37,7 @@ struct Element<RCH_DT_BF16> {
     typedef __bf16 type;
 };
 
-// N values from / to consecutive elements, in 16-byte pieces where N * size allows it.
+// N values from / to consecutive elements, in 16- or 8-byte pieces where N * size allows it.
 template <typename T, int N>
 struct Piece {
     T v[N];
@@ -51,6 +51,9 @@ __device__ __forceinline__ Piece<T, N> load_piece(const RCH_GLOBAL T* p) {
             const u4 raw = reinterpret_cast<const RCH_GLOBAL u4*>(p)[i];
             __builtin_memcpy(reinterpret_cast<char*>(out.v) + 16 * i, &raw, 16);
         }
+    } else if constexpr (N * sizeof(T) == 8) {
+        const u2 raw = *reinterpret_cast<const RCH_GLOBAL u2*>(p);
+        __builtin_memcpy(out.v, &raw, 8);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) out.v[i] = p[i];
@@ -66,6 +69,10 @@ __device__ __forceinline__ void store_piece(RCH_GLOBAL T* p, const Piece<T, N>& 
             __builtin_memcpy(&raw, reinterpret_cast<const char*>(in.v) + 16 * i, 16);
             reinterpret_cast<RCH_GLOBAL u4*>(p)[i] = raw;
         }
+    } else if constexpr (N * sizeof(T) == 8) {
+        u2 raw;
+        __builtin_memcpy(&raw, in.v, 8);
+        *reinterpret_cast<RCH_GLOBAL u2*>(p) = raw;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) p[i] = in.v[i];
@@ -80,8 +87,8 @@ __device__ __forceinline__ void rotate_pair(float& e, float& o, float c, float s
 }
 
 // One piece is V channels: V / 2 interleaved pairs, or V pairs of the half pairing (channels j and
-// pairs + j: two pieces).  V = 8 needs 16-byte aligned rows and a rotated width of whole pieces; V = 2
-// (interleaved) and 1 (half, or no rotation) take everything else.
+// pairs + j: two pieces).  V = 8 and V = 4 need rows aligned to a piece (16 bytes at most) and widths of
+// whole pieces; V = 2 (interleaved) and 1 (half, or no rotation) take everything else.
 // A thread takes U heads, whose loads are in flight together.
 template <int DT, bool HALF, int V, int U>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryJobs jobs) {
@@ -187,12 +194,14 @@ void launch_heads(const RotaryJobs& jobs, dim3 grid, int per_thread, hipStream_t
 }
 
 template <int DT>
-void launch(const RotaryJobs& jobs, bool half, bool wide, dim3 grid, int per_thread, hipStream_t stream) {
+void launch(const RotaryJobs& jobs, bool half, int width, dim3 grid, int per_thread, hipStream_t stream) {
     if (half) {
-        if (wide) launch_heads<DT, true, 8>(jobs, grid, per_thread, stream);
+        if (width == 8) launch_heads<DT, true, 8>(jobs, grid, per_thread, stream);
+        else if (width == 4) launch_heads<DT, true, 4>(jobs, grid, per_thread, stream);
         else launch_heads<DT, true, 1>(jobs, grid, per_thread, stream);
     } else {
-        if (wide) launch_heads<DT, false, 8>(jobs, grid, per_thread, stream);
+        if (width == 8) launch_heads<DT, false, 8>(jobs, grid, per_thread, stream);
+        else if (width == 4) launch_heads<DT, false, 4>(jobs, grid, per_thread, stream);
         else launch_heads<DT, false, 2>(jobs, grid, per_thread, stream);
     }
 }
@@ -218,7 +227,7 @@ int rch_rotary(const rch_rotary_job* jobs_host, int n_jobs, int dtype, int pairi
     half = half || !turns;  // a plain copy has no pairs to keep together
     const int64_t size = dtype == RCH_DT_F32 ? 4 : 2;
     RotaryJobs jobs;
-    bool wide = true;
+    int64_t mix = 0, channels = 0;
     for (int i = 0; i < n_jobs; ++i) {
         const rch_rotary_job& J = jobs.job[i] = jobs_host[i];
         if (J.batch < 0 || J.tokens < 0 || J.heads < 1 || J.head_dim < 1 || J.pairs < 0 || 2 * J.pairs > J.head_dim
@@ -229,21 +238,19 @@ int rch_rotary(const rch_rotary_job* jobs_host, int n_jobs, int dtype, int pairi
             return fail(RCH_E_CONFIG, "rch_rotary: invalid positions of tensor %d", i);
         if (J.slots_ptr && (J.batch != 1 || J.page_tokens < 1))
             return fail(RCH_E_CONFIG, "rch_rotary: slots take one batch and a page size (tensor %d)", i);
-        // The wide variant: 16-byte rows of whole 8-channel pieces on both sides.
         const int64_t strides = J.src_batch_stride | J.src_token_stride | J.src_head_stride | J.dst_batch_stride
                                 | J.dst_token_stride | J.dst_head_stride;
-        wide = wide && ((J.src_ptr | J.dst_ptr) % 16 == 0) && (strides * size) % 16 == 0 && J.head_dim % 8 == 0
-               && (half ? J.pairs % 8 == 0 : J.pairs % 4 == 0);
+        mix |= J.src_ptr | J.dst_ptr | strides * size;
+        channels |= J.head_dim | (half ? J.pairs : 2 * J.pairs);  // every width a piece divides
     }
-    // The narrow interleaved pieces are pairs: the channels behind them must be pairs too.
-    if (!wide && !half)
-        for (int i = 0; i < n_jobs; ++i)
-            if (jobs.job[i].head_dim % 2)
-                return fail(RCH_E_UNSUPPORTED, "rch_rotary: interleaved pairs need an even head_dim");
+    // The widest piece that divides every width and whose rows are aligned.
+    const int width = channels % 8 == 0 && mix % 16 == 0 ? 8
+                      : channels % 4 == 0 && mix % (4 * size) == 0 ? 4 : half ? 1 : 2;
+    if (width == 2 && channels % 2) return fail(RCH_E_UNSUPPORTED, "rch_rotary: interleaved pairs need an even head_dim");
     int64_t units = 0, heads = 0, work = 0;
     for (int i = 0; i < n_jobs; ++i) {
         const rch_rotary_job& J = jobs.job[i];
-        const int v = wide ? 8 : (half ? 1 : 2);
+        const int v = width;
         const int64_t pieces = (half ? J.pairs / v : 2 * J.pairs / v) + (J.head_dim - 2 * J.pairs) / v;
         const int64_t n = J.batch * J.tokens * pieces;
         units = n > units ? n : units;
@@ -259,9 +266,9 @@ int rch_rotary(const rch_rotary_job* jobs_host, int n_jobs, int dtype, int pairi
     const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(groups), static_cast<uint32_t>(n_jobs));
     hipStream_t s = as_stream(stream);
     switch (dtype) {
-        case RCH_DT_F32: launch<RCH_DT_F32>(jobs, half, wide, grid, per_thread, s); break;
-        case RCH_DT_F16: launch<RCH_DT_F16>(jobs, half, wide, grid, per_thread, s); break;
-        default: launch<RCH_DT_BF16>(jobs, half, wide, grid, per_thread, s); break;
+        case RCH_DT_F32: launch<RCH_DT_F32>(jobs, half, width, grid, per_thread, s); break;
+        case RCH_DT_F16: launch<RCH_DT_F16>(jobs, half, width, grid, per_thread, s); break;
+        default: launch<RCH_DT_BF16>(jobs, half, width, grid, per_thread, s); break;
     }
     return check_launch("rch_rotary");
 }

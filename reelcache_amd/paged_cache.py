@@ -28,9 +28,8 @@ import torch
 from . import _lib
 from ._checks import count, need, one_of, strided
 from .errors import CapacityError, ConfigurationError, StateError
-from .restore_handle import _capturing
 from .restore_model import OUTPUT_DTYPES, NativeView
-from .rotary import entered, launch_rotary, need_gpu, position_fields
+from .rotary import Launch, addresses_of, capturing, entered, known_calls, need_gpu, position_fields, raw_stream
 
 HOLE = -1
 _LAYOUTS = ("BTHD", "BHTD")
@@ -46,6 +45,7 @@ class Slots:
     tokens: int
     cache: "PagedCache"
     stamp: int
+    stream: int
 
 
 class _Sequence:
@@ -55,12 +55,24 @@ class _Sequence:
         self.pages, self.tokens = pages, tokens
 
 
+# Tables of at most this many words travel in launch arguments: two launches and no pinned memory, where a
+# copy costs about four launches on the host.
+_ARGUMENT_WORDS = 1920
+# Slots of so few tokens are listed one by one (the array form has a fixed cost of about sixty of them).
+_FEW_TOKENS = 64
+
+
 def upload(values, device):
-    """An int32 array on ``device``, copied from pinned memory on the current stream without a host
-    wait; the pinned block stays reserved until the copy has run."""
-    if _capturing():
+    """An int32 array on ``device``, written on its current stream without a host wait: small ones in
+    launch arguments, larger ones from pinned memory (the block stays reserved until the copy has run)."""
+    if capturing():
         raise ConfigurationError("page tables, slots and plans are built before a HIP-graph capture, not in it")
-    return torch.from_numpy(np.ascontiguousarray(values, dtype=np.int32)).pin_memory().to(device, non_blocking=True)
+    values = np.ascontiguousarray(values, dtype=np.int32)
+    if values.size > _ARGUMENT_WORDS:
+        return torch.from_numpy(values).pin_memory().to(device, non_blocking=True)
+    out = torch.empty(values.shape, dtype=torch.int32, device=device)
+    _lib.check(_lib.function("rch_words_store")(out.data_ptr(), values.ctypes.data, values.size, raw_stream(device)))
+    return out
 
 
 class PagedCache:
@@ -88,6 +100,7 @@ class PagedCache:
         need(self.pages * self.page_tokens < 1 << 31, "a pool holds fewer than 2**31 tokens")
         self.device, self.dtype = keys.device, keys.dtype
         self._axes = (1, token, head)
+        self._geometry = (keys.shape[1:], keys.stride()[1:], values.stride()[1:], keys.dtype, keys.device)
         self._sequences: dict[int, _Sequence] = {}
         self._next = 0
         self._uses = [0] * self.pages
@@ -218,7 +231,7 @@ class PagedCache:
         total = sum(copies + more for copies, more in wanted)
         if total > len(self._free):
             raise CapacityError(f"{total} pages are needed and {len(self._free)} are free")
-        if _capturing():
+        if capturing():
             raise ConfigurationError("a cache grows before a HIP-graph capture, not in it")
         moves, starts = [], []
         for item, n, (copies, more) in zip(found, counts, wanted):
@@ -258,15 +271,29 @@ class PagedCache:
         return self._slots(found, starts, counts)
 
     def _slots(self, found, starts, counts):
-        parts = []
+        size = self.page_tokens
+        if sum(counts) <= _FEW_TOKENS:
+            index = np.asarray([item.pages[at // size] * size + at % size for item, start, n in zip(found, starts, counts)
+                                for at in range(start, start + n)], dtype=np.int32)
+            return self._made(index)
+        pages, base = [], []  # the pages of all tokens, and where each sequence's page 0 would lie among them
         for item, start, n in zip(found, starts, counts):
-            at = np.arange(start, start + n, dtype=np.int64)
-            first = start // self.page_tokens
-            pages = np.asarray(item.pages[first:-(-(start + n) // self.page_tokens)], dtype=np.int64)
-            parts.append(pages[at // self.page_tokens - first] * self.page_tokens + at % self.page_tokens)
-        index = np.concatenate(parts) if parts else np.empty(0, np.int64)
+            first = start // size
+            base.append(len(pages) - first)
+            pages += item.pages[first:-(-(start + n) // size)]
+        counts = np.asarray(counts, dtype=np.int64)
+        ends = np.cumsum(counts)
+        total = int(ends[-1]) if len(ends) else 0
+        at = np.arange(total) + np.repeat(np.asarray(starts, dtype=np.int64) - ends + counts, counts)
+        page = at // size
+        index = at - page * size
+        if total:
+            index += np.asarray(pages, dtype=np.int64)[page + np.repeat(np.asarray(base, dtype=np.int64), counts)] * size
+        return self._made(index)
+
+    def _made(self, index):
         with entered(self.device):
-            return Slots(upload(index, self.device), index.size, self, self._moved + self._shared)
+            return Slots(upload(index, self.device), index.size, self, self._moved + self._shared, raw_stream(self.device))
 
     # -----------------------------------------------------------------------------------------
     # Page copies
@@ -338,8 +365,8 @@ class PagedCache:
         for number, (pages, tokens) in enumerate(tables):
             pages = [int(page) for page in pages]
             need(len(pages) == -(-count(tokens, "tokens") // self.page_tokens), "the pages do not hold the tokens")
-            real = [page for page in pages if page != HOLE]
-            need(all(0 <= page < self.pages for page in real), "a page lies outside the pool")
+            real = [page for page in pages if page != HOLE] if HOLE in pages else pages
+            need(not real or (min(real) >= 0 and max(real) < self.pages), "a page lies outside the pool")
             need(len(set(real)) == len(real), "a sequence has a page twice")
             need(not pages or pages[-1] != HOLE, "the last page of a sequence cannot be a hole")
             for page in real:
@@ -397,31 +424,44 @@ class PagedCache:
         :func:`reelcache_amd.rotary.rotate`; ``None`` stores them as they are) and ``values``, both
         ``[tokens, heads, head_dim]`` of the cache's dtype, any strides.  With a ``grid`` the tokens are
         one chunk."""
-        pools = self._layer(layer)
-        need(isinstance(slots, Slots) and slots.cache is self, "slots come from this cache")
+        if type(layer) is not int or not 0 <= layer < self.layers:
+            raise ConfigurationError("there is no such layer")
+        if not isinstance(slots, Slots) or slots.cache is not self:
+            raise ConfigurationError("slots come from this cache")
         if slots.stamp != self._moved + self._shared:
             raise StateError("pages moved, were freed or became shared after these slots were built")
+        shape = (slots.tokens, self.heads, self.head_dim)
         for x, name in ((keys, "keys"), (values, "values")):
             strided(x, name)
-            need(x.shape == (slots.tokens, self.heads, self.head_dim) and x.dtype == self.dtype
-                 and x.device == self.device, f"{name} must be [tokens, heads, head_dim] of the cache's dtype and device")
+            if x.shape != shape or x.dtype != self.dtype or x.device != self.device:
+                raise ConfigurationError(f"{name} must be [tokens, heads, head_dim] of the cache's dtype and device")
         if slots.tokens == 0:
             return
         need_gpu(self.device, "a paged cache")
+        grid = None if grid is None else tuple(grid)
         with entered(self.device):
-            stream = torch.cuda.current_stream(self.device)
-            pairs, place = position_fields(positions, grid, slots.tokens, 1, self.head_dim, self.device, stream)
-            jobs = []
-            for x, pool, (turned, at) in zip((keys, values), pools, ((pairs, place), (0, (0,) * 16))):
-                x = x.detach()
-                if x.stride(2) != 1 and self.head_dim > 1:
-                    x = x.contiguous()
-                page, token, head = (pool.stride(axis - 1) for axis in self._axes)
-                jobs.append((x.data_ptr(), pool.data_ptr(), 1, slots.tokens, self.heads, self.head_dim, turned,
-                             0, x.stride(0), x.stride(1), page, token, head, *at, slots.index.data_ptr(),
-                             self.pages * self.page_tokens, self.page_tokens, 0, 0))
-            slots.index.record_stream(stream)
-            launch_rotary(jobs, self.dtype, "interleaved", stream)
+            sources = [x if x.stride(2) == 1 or self.head_dim == 1 else x.contiguous() for x in (keys, values)]
+            known = known_calls(slots if positions is None else positions)
+            key = (slots.tokens, grid, self._geometry, *[x.stride() for x in sources])
+            launch = known.get(key)
+            if launch is None:
+                launch = known[key] = self._store_launch(sources, positions, grid, slots.tokens)
+            stream = raw_stream(self.device)
+            step = layer * self.keys.element_size()
+            pools = [pool.data_ptr() + step * pool.stride(0) for pool in (self.keys, self.values)]
+            launch([(sources[0].data_ptr(), pools[0], True), (sources[1].data_ptr(), pools[1], False)],
+                   *addresses_of(positions, self.device, stream), slots.index.data_ptr(), stream)
+            if stream != slots.stream:  # the allocator learns of a stream that the index was not made on
+                slots.index.record_stream(torch.cuda.current_stream(self.device))
+
+    def _store_launch(self, sources, positions, grid, tokens):
+        turned = position_fields(positions, grid, tokens, 1, self.head_dim, self.device)
+        jobs = []
+        for x, pool, (pairs, place) in zip(sources, (self.keys, self.values), (turned, (0, (0,) * 16))):
+            page, token, head = (pool.stride(axis) for axis in self._axes)
+            jobs.append((0, 0, 1, tokens, self.heads, self.head_dim, pairs, 0, x.stride(0), x.stride(1), page, token, head,
+                         *place, 0, self.pages * self.page_tokens, self.page_tokens, 0, 0))
+        return Launch(jobs, self.dtype, "interleaved")
 
     # -----------------------------------------------------------------------------------------
     # Attention
@@ -436,9 +476,15 @@ class PagedCache:
 
     def attend(self, layer, q, plan, *, out=None, return_lse=False):
         """:func:`reelcache_amd.attention.attend` over one layer."""
-        from .attention import attend
+        from .attention import AttentionPlan, attend, run
 
-        return attend(q, *self._layer(layer), plan, out=out, return_lse=return_lse)
+        if type(layer) is not int or not 0 <= layer < self.layers:
+            raise ConfigurationError("there is no such layer")
+        if not isinstance(plan, AttentionPlan) or plan.cache is not self:
+            return attend(q, *self._layer(layer), plan, out=out, return_lse=return_lse)
+        step = layer * self.keys.element_size()
+        return run(q, self.keys.data_ptr() + step * self.keys.stride(0), self.values.data_ptr() + step * self.values.stride(0),
+                   plan, out, return_lse)
 
 
 def _apart(pool):
@@ -459,7 +505,7 @@ def _pools(group, axes, pages, page_tokens):
     page, token, head = (stride[axis] * size for axis in axes)
     heads, row = group[0].shape[axes[2]], group[0].shape[4] * size
     addresses = [pool.data_ptr() + layer * stride[0] * size for pool in group for layer in range(pool.shape[0])]
-    if _capturing():
+    if capturing():
         raise ConfigurationError("a cache's first page copy cannot be captured: it uploads the pools' addresses")
     table = torch.tensor(addresses, dtype=torch.int64).to(group[0].device)  # waits: usable on every stream
     joined = head == row or heads == 1  # a token's heads are one run

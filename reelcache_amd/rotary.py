@@ -72,10 +72,20 @@ def entered(device):
     return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def capturing():
+    """Whether the current stream captures a HIP graph."""
+    return torch.cuda.is_current_stream_capturing()
+
+
 def need_gpu(device, what):
     if device.type != "cuda":
         raise UnsupportedError(f"{what} runs on the GPU (HIP, gfx950); move the tensors to a cuda device")
     _lib.library()  # raises UnsupportedError with the reason when the library is unavailable
+
+
+def raw_stream(device):
+    """The current stream of ``device`` as an integer handle."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 # Streams that a table's device copy has been used on: its memory comes from the upload stream, so the
@@ -84,16 +94,29 @@ _TABLE_STREAMS: weakref.WeakKeyDictionary = weakref.WeakKeyDictionary()
 
 
 def _table_pairs(table, device, stream):
-    entry = table._kernel_block(device, stream)
-    used = _TABLE_STREAMS.setdefault(entry, set())
-    if stream.cuda_stream not in used:
-        entry.block.record_stream(stream)
-        used.add(stream.cuda_stream)
-    return entry.pairs
+    """Address of the table's (cos, sin) pairs on ``device``, valid for work enqueued next on the current
+    stream (``stream``: its handle)."""
+    entry = table._device_cache.get(device)
+    if entry is None or entry.ready is not None or entry.stamp != table._stamp():
+        entry = table._kernel_block(device, torch.cuda.current_stream(device))
+    used = _TABLE_STREAMS.get(entry)
+    if used is None:
+        used = _TABLE_STREAMS[entry] = set()
+    if stream not in used:
+        entry.block.record_stream(torch.cuda.current_stream(device))
+        used.add(stream)
+    return entry.pairs.data_ptr()
 
 
-def position_fields(positions, grid, tokens, batch, head_dim, device, stream):
-    """The place fields of ``rch_rotary_job`` (pairs_ptr .. rows_axis_stride) and the pair count."""
+_PAIRS_AT = _lib.ROTARY_FIELDS.index("pairs_ptr")
+_ROWS_AT = _lib.ROTARY_FIELDS.index("rows_ptr")
+_SLOTS_AT = _lib.ROTARY_FIELDS.index("slots_ptr")
+_WORDS = len(_lib.ROTARY_FIELDS)
+
+
+def position_fields(positions, grid, tokens, batch, head_dim, device):
+    """The place fields of ``rch_rotary_job`` (pairs_ptr .. rows_axis_stride; the addresses are left 0) and
+    the pair count."""
     if positions is None:
         return 0, (0,) * 16
     need(isinstance(positions, (RopePositions, TokenRows)), "positions must be RopePositions or TokenRows")
@@ -107,7 +130,7 @@ def position_fields(positions, grid, tokens, batch, head_dim, device, stream):
         need(rows.device == device, "token rows must be on the tensors' device")
         need(positions.tokens == tokens and positions.batch in (None, batch), "token rows do not match the tokens")
         strides = rows.stride() if axes == 3 else (*rows.stride(), 0)
-        place = (0, 0, 0, 0, 0, rows.data_ptr(), strides[0] if len(strides) == 3 else 0, strides[-2], strides[-1])
+        place = (0, 0, 0, 0, 0, 0, strides[0] if len(strides) == 3 else 0, strides[-2], strides[-1])
     elif axes == 1:
         need(grid is None, "a dense table takes no grid")
         need(positions.rows + tokens <= table.rows, "the tokens run past the RoPE table")
@@ -120,15 +143,53 @@ def position_fields(positions, grid, tokens, batch, head_dim, device, stream):
         for first, extent, limit, pairs in zip(positions.rows, grid, limits, table.sections):
             need(pairs == 0 or first + extent <= limit, "the grid runs past the RoPE table")
         place = (*positions.rows, grid[1], grid[2], 0, 0, 0, 0)
-    pairs = _table_pairs(table, device, stream)
-    return table.pairs, (pairs.data_ptr(), axes, *sections, *limits, *place)
+    return table.pairs, (0, axes, *sections, *limits, *place)
 
 
-def launch_rotary(jobs, dtype, pairing, stream):
-    """One ``rch_rotary`` launch of ``jobs`` (rows of the struct's fields)."""
-    flat = [value for job in jobs for value in job]
-    _lib.call("rch_rotary", (ctypes.c_int64 * len(flat))(*flat), len(jobs), _DTYPE_CODES[dtype],
-              _lib.PAIRS_HALF if pairing == "half" else _lib.PAIRS_INTERLEAVED, stream.cuda_stream)
+class Launch:
+    """A checked ``rch_rotary`` launch of one geometry: everything but the addresses."""
+
+    __slots__ = ("array", "dtype", "image", "jobs", "pairing")
+
+    def __init__(self, jobs, dtype, pairing):
+        self.jobs, self.dtype = len(jobs), _DTYPE_CODES[dtype]
+        self.pairing = _lib.PAIRS_HALF if pairing == "half" else _lib.PAIRS_INTERLEAVED
+        flat = [value for job in jobs for value in job]
+        self.array = ctypes.c_int64 * len(flat)
+        self.image = bytes(self.array(*flat))
+
+    def __call__(self, addresses, pairs, rows, slots, stream):
+        """Launches with the (source, destination) addresses of the jobs and those of the table (for the
+        jobs that turn), the token rows and the slots; 0 where there are none."""
+        fields = self.array.from_buffer_copy(self.image)
+        at = 0
+        for source, target, turns in addresses:
+            fields[at], fields[at + 1] = source, target
+            if turns:
+                fields[at + _PAIRS_AT], fields[at + _ROWS_AT] = pairs, rows
+            fields[at + _SLOTS_AT] = slots
+            at += _WORDS
+        _lib.check(_lib.function("rch_rotary")(fields, self.jobs, self.dtype, self.pairing, stream))
+
+
+def addresses_of(positions, device, stream):
+    """(table pairs, token rows) addresses of a launch's positions."""
+    if positions is None:
+        return 0, 0
+    return (_table_pairs(positions.table, device, stream),
+            positions.rows.data_ptr() if isinstance(positions, TokenRows) else 0)
+
+
+#: Geometries of calls that one position object remembers.
+_MOST_KNOWN = 64
+
+
+def known_calls(holder):
+    """The launches prepared for an object's earlier calls, by their geometry."""
+    known = holder.__dict__.get("_known_calls")
+    if known is None or len(known) >= _MOST_KNOWN:
+        known = holder.__dict__["_known_calls"] = {}
+    return known
 
 
 def _geometry(x, layout):
@@ -140,8 +201,10 @@ def _geometry(x, layout):
 
 def _check(x, layout, name):
     strided(x, name)
-    need(x.ndim == (3 if layout == "THD" else 4), f"{name}: {layout} has the wrong number of dimensions")
-    need(x.dtype in OUTPUT_DTYPES, f"{name} must be bfloat16, float16 or float32")
+    if x.ndim != (3 if layout == "THD" else 4):
+        raise ConfigurationError(f"{name}: {layout} has the wrong number of dimensions")
+    if x.dtype not in OUTPUT_DTYPES:
+        raise ConfigurationError(f"{name} must be bfloat16, float16 or float32")
 
 
 def _span(x):
@@ -152,38 +215,64 @@ def _span(x):
     return x.data_ptr(), x.data_ptr() + (reach + 1) * x.element_size()
 
 
-def _rotate(tensors, positions, grid, layout, pairing, inverse, outs):
-    """Launches the rotation of checked tensors into ``outs`` (or new tensors); returns the outputs."""
+def _prepare(tensors, outs, positions, grid, layout, pairing, inverse):
+    """The :class:`Launch` of tensors into outputs (both with unit channel stride), or None when there is
+    nothing to do."""
     device = tensors[0].device
-    results, jobs, copies, places = [], [], [], {}
-    with entered(device):
-        stream = torch.cuda.current_stream(device)
-        for x, out in zip(tensors, outs):
-            (batch, tokens, heads, head_dim), strides = _geometry(x, layout)
-            if strides[3] != 1 and head_dim > 1:
-                x = x.contiguous()
-                strides = _geometry(x, layout)[1]
-            given = out
-            if out is None:
-                out = torch.empty_like(x)
-            to = _geometry(out, layout)[1]
-            if to[3] != 1 and head_dim > 1:  # written through a buffer
-                out = torch.empty(x.shape, dtype=x.dtype, device=device)
-                copies.append((given, out))
-                to = _geometry(out, layout)[1]
-            results.append(given if given is not None else out)
-            key = (tokens, batch, head_dim)
-            if key not in places:  # queries and keys of a call share them
-                places[key] = position_fields(positions, grid, tokens, batch, head_dim, device, stream)
-            pairs, place = places[key]
-            if batch and tokens and heads and head_dim:
-                jobs.append((x.data_ptr(), out.data_ptr(), batch, tokens, heads, head_dim, pairs, *strides[:3], *to[:3],
-                             *place, 0, 0, 0, int(inverse), 0))
-        if jobs:
-            launch_rotary(jobs, tensors[0].dtype, pairing, stream)
-        for given, out in copies:
-            given.copy_(out)
-    return tuple(results)
+    jobs, places = [], {}
+    for x, out in zip(tensors, outs):
+        (batch, tokens, heads, head_dim), strides = _geometry(x, layout)
+        to = _geometry(out, layout)[1]
+        key = (tokens, batch, head_dim)
+        if key not in places:  # queries and keys of a call share them
+            places[key] = position_fields(positions, grid, tokens, batch, head_dim, device)
+        pairs, place = places[key]
+        jobs.append((0, 0, batch, tokens, heads, head_dim, pairs, *strides[:3], *to[:3], *place, 0, 0, 0, int(inverse), 0))
+    if all(0 in job[2:6] for job in jobs):
+        return None
+    # A tensor without elements rides along as no work.
+    return Launch([job if job[4] and job[5] else (0, 0, 0, 0, 1, 8, 0, *job[7:]) for job in jobs],
+                  tensors[0].dtype, pairing)
+
+
+def _run(launch, tensors, outs, positions):
+    if launch is not None:
+        device = tensors[0].device
+        stream = raw_stream(device)
+        launch([(x.data_ptr(), out.data_ptr(), True) for x, out in zip(tensors, outs)],
+               *addresses_of(positions, device, stream), 0, stream)
+
+
+def _rotate(tensors, positions, grid, layout, pairing, inverse):
+    """The rotation of checked tensors into new ones."""
+    with entered(tensors[0].device):
+        known = known_calls(positions)
+        key = (layout, pairing, inverse, grid, *[(x.shape, x.stride(), x.dtype, x.device) for x in tensors])
+        call = known.get(key)
+        if call is None:
+            plain = all(x.stride(-1) == 1 or x.shape[-1] == 1 for x in tensors)
+            if not plain:
+                tensors = [x if x.stride(-1) == 1 else x.contiguous() for x in tensors]
+            outs = tuple(torch.empty_like(x) for x in tensors)
+            call = (_prepare(tensors, outs, positions, grid, layout, pairing, inverse),)
+            if plain:
+                known[key] = call
+        else:
+            outs = tuple([torch.empty_like(x) for x in tensors])
+        _run(call[0], tensors, outs, positions)
+    return outs
+
+
+def _rotate_into(tensors, outs, positions, grid, layout, pairing, inverse):
+    """The rotation of checked tensors into given ones."""
+    with entered(tensors[0].device):
+        sources = [x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous() for x in tensors]
+        targets = [o if o.stride(-1) == 1 or o.shape[-1] == 1 else torch.empty(o.shape, dtype=o.dtype, device=o.device)
+                   for o in outs]
+        _run(_prepare(sources, targets, positions, grid, layout, pairing, inverse), sources, targets, positions)
+        for out, target in zip(outs, targets):
+            if target is not out:
+                out.copy_(target)
 
 
 class _Rotation(torch.autograd.Function):
@@ -196,7 +285,7 @@ class _Rotation(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         if isinstance(positions, TokenRows):
             ctx.save_for_backward(positions.rows)  # rows changed in place before the backward pass are refused
-        return _rotate(tensors, positions, grid, layout, pairing, inverse, (None,) * len(tensors))
+        return _rotate(tensors, positions, grid, layout, pairing, inverse)
 
     @staticmethod
     def backward(ctx, *grads):
@@ -227,21 +316,24 @@ def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interl
     """
     single = isinstance(tensors, torch.Tensor)
     tensors = (tensors,) if single else tuple(tensors)
-    need(1 <= len(tensors) <= MAX_TENSORS, f"one call rotates 1 to {MAX_TENSORS} tensors")
+    if not 1 <= len(tensors) <= MAX_TENSORS:
+        raise ConfigurationError(f"one call rotates 1 to {MAX_TENSORS} tensors")
     one_of(layout, LAYOUTS, "layout")
     one_of(pairing, PAIRINGS, "pairing")
-    need(isinstance(positions, (RopePositions, TokenRows)), "positions must be RopePositions or TokenRows")
+    if not isinstance(positions, (RopePositions, TokenRows)):
+        raise ConfigurationError("positions must be RopePositions or TokenRows")
     first = tensors[0]
     for x in tensors:
         _check(x, layout, "a rotated tensor")
-        need(x.dtype == first.dtype and x.device == first.device, "the tensors of one call share dtype and device")
+        if x.dtype != first.dtype or x.device != first.device:
+            raise ConfigurationError("the tensors of one call share dtype and device")
     need_gpu(first.device, "the rotation")
     grid = None if grid is None else tuple(grid)
     if out is None:
-        if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
+        if torch.is_grad_enabled() and any([x.requires_grad for x in tensors]):
             results = _Rotation.apply(positions, grid, layout, pairing, inverse, *tensors)
         else:
-            results = _rotate(tensors, positions, grid, layout, pairing, inverse, (None,) * len(tensors))
+            results = _rotate(tensors, positions, grid, layout, pairing, inverse)
         return results[0] if single else results
     outs = (out,) if isinstance(out, torch.Tensor) else tuple(out)
     need(len(outs) == len(tensors), "out must have one tensor for each input")
@@ -260,7 +352,7 @@ def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interl
         for other in outs[:i]:
             a, b = _span(other)
             need(high <= a or b <= low, "the outputs overlap")
-    _rotate(tensors, positions, grid, layout, pairing, inverse, outs)
+    _rotate_into(tensors, outs, positions, grid, layout, pairing, inverse)
     return out
 
 

@@ -35,6 +35,8 @@ def host(monkeypatch):
     for module in (paged_cache, attention):
         monkeypatch.setattr(module, "need_gpu", lambda device, what: None)
         monkeypatch.setattr(module, "entered", lambda device: contextlib.nullcontext())
+        monkeypatch.setattr(module, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(paged_cache, "capturing", lambda: False)
     monkeypatch.setattr(paged_cache, "upload", lambda values, device: torch.from_numpy(np.asarray(values, dtype=np.int32)))
     return copies
 
@@ -221,17 +223,17 @@ def test_cpu_tensors_are_refused():
 def test_rotary_refusals(monkeypatch):
     monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
     monkeypatch.setattr(rotary, "entered", lambda device: contextlib.nullcontext())
-    monkeypatch.setattr(rotary, "_table_pairs", lambda table, device, stream: torch.zeros(table.rows, table.pairs, 2))
-    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: None)
+    monkeypatch.setattr(rotary, "_table_pairs", lambda table, device, stream: 64)
+    monkeypatch.setattr(rotary, "raw_stream", lambda device: 0)
     launches = []
-    monkeypatch.setattr(rotary, "launch_rotary", lambda jobs, *rest: launches.append(jobs))
+    monkeypatch.setattr(rotary.Launch, "__call__", lambda self, addresses, *rest: launches.append((self, addresses)))
     cos, sin, sections = oracle.tables(8, 4)
     table, dense = rk.RopeTable(cos, sin, sections), rk.RopeTable(cos, sin)
     x, grid, at = torch.zeros(1, 6, 2, 8), (1, 2, 3), rk.RopePositions(table, 0)
     rows = torch.zeros(6, 3, dtype=torch.int32)
     rotary.rotate(x, at, grid=grid)
     rotary.rotate(x, rotary.TokenRows(table, rows))
-    assert len(launches) == 2 and all(len(job) == len(_lib.ROTARY_FIELDS) for jobs in launches for job in jobs)
+    assert len(launches) == 2 and all(len(launch.image) == 8 * len(_lib.ROTARY_FIELDS) for launch, _ in launches)
     for call in (
             lambda: rotary.rotate(x, table, grid=grid), lambda: rotary.rotate(x, at), lambda: rotary.rotate(x, at, grid=(1, 2, 2)),
             lambda: rotary.rotate(x, at, grid=(0, 2, 3)), lambda: rotary.rotate(x, rk.RopePositions(table, (8, 0, 0)), grid=grid),
@@ -278,7 +280,7 @@ def test_plan_refusals(host):
         plan._check(cache.keys[0][:4], cache.values[0])
     cache.truncate(a, 2)
     with pytest.raises(StateError, match="after this plan"):
-        plan._check(cache.keys[0], cache.values[0])
+        cache.attend(0, torch.zeros(1, 2, 8), plan)
 
 
 def _items(plan):
