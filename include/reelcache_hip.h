@@ -584,13 +584,14 @@ int rch_words_store(void* words_dev, const int32_t* words_host, int count, void*
  *
  * Item: [table (word index of the sequence's first page), length, first query row of q, queries,
  *   row_begin, row_end, kv_head, key_begin, key_end, part (first row of the fp32 partials it writes, or
- *   -1: the output itself), 0, 0].  Merge: [first query row of q, row_begin, rows, kv_head, first partial
+ *   -1: the output itself), 0, 0]; one with row_begin >= row_end is empty.  Merge: [first query row of q, row_begin, rows, kv_head, first partial
  *   row, parts, 0, 0]: part i of row r is partial row first + i * rows + (r - row_begin).
  * Partials: fp32 [partial_rows, head_dim] sums, then fp32 [partial_rows, 2] of (reference exponent, sum).
  */
 #define RCH_ATTEND_ITEM 12
 #define RCH_ATTEND_MERGE 8
 #define RCH_ATTEND_ZEROS 128
+#define RCH_ATTEND_FEW_PARTS 8
 #define RCH_ATTEND_MAX_DIM 256   /* head_dim of the general form */
 #define RCH_ATTEND_FAST_DIM 128  /* head_dim of the others: multiples of 8 up to this, 16-byte aligned rows */
 
@@ -605,11 +606,13 @@ typedef struct rch_attend {
     int64_t scale_bits;      /* fp32 bits of scale * log2(e); scale > 0 */
     int64_t partial_rows;
     int64_t items;           /* word index of the first item */
-    int64_t n_general, n_rows, n_tokens; /* items of the general, the row-tiled and the few-rows form, in order */
-    int64_t merges, n_merges, most_rows; /* word index, count, most rows of a merge */
+    int64_t n_general, n_rows; /* items of the general and of the tiled form, in order */
+    int64_t merges, n_merges;      /* word index and count */
+    int64_t n_many;                /* the first ones: merges of more than RCH_ATTEND_FEW_PARTS parts, or of rows
+                                      that are no aligned multiples of eight channels up to 128 */
+    int64_t most_rows_many, most_rows; /* most rows of one of those, and of one of the others */
     int64_t holes;           /* 1: page tables may hold holes */
     int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64 */
-    int64_t reserved;
 } rch_attend;                /* 36 x int64 = 288 bytes */
 
 int rch_attend_size(void);

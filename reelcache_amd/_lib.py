@@ -78,9 +78,10 @@ PAGES_FIELDS = ("pools_ptr", "pools", "pages", "page_stride", "page_rows", "segm
 ATTEND_FIELDS = ("q_ptr", "k_ptr", "v_ptr", "out_ptr", "lse_ptr", "plan_ptr", "partial_ptr", "q_token_stride",
                  "q_head_stride", "k_page_stride", "k_token_stride", "k_head_stride", "v_page_stride", "v_token_stride",
                  "v_head_stride", "out_token_stride", "out_head_stride", "group", "heads", "head_dim", "page_tokens",
-                 "pages", "block", "window", "scale_bits", "partial_rows", "items", "n_general", "n_rows", "n_tokens",
-                 "merges", "n_merges", "most_rows", "holes", "tile_unit", "reserved")
+                 "pages", "block", "window", "scale_bits", "partial_rows", "items", "n_general", "n_rows",
+                 "merges", "n_merges", "n_many", "most_rows_many", "most_rows", "holes", "tile_unit")
 ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 128
+ATTEND_FEW_PARTS = 8
 PAIRS_INTERLEAVED, PAIRS_HALF = 0, 1
 
 _i, _i64, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p

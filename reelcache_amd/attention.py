@@ -16,6 +16,7 @@ that a query does not see have no influence on it, whatever their slots hold.
 from __future__ import annotations
 
 import ctypes
+import heapq
 import math
 import struct
 
@@ -30,13 +31,14 @@ from .rotary import _DTYPE_CODES, _span, entered, known_calls, need_gpu, raw_str
 #: Keys of a tile: the step of every split of a sequence's keys.
 KEY_TILE = 64
 #: Query rows (tokens x heads of a key head) of one workgroup's tile, per form.
-GENERAL_ROWS, ROW_TILE, TOKEN_ROWS = 16, 128, 32
+GENERAL_ROWS, ROW_TILE = 16, 128
 # Workgroups resident on the card at once, per form (256 CUs), and what a workgroup's start, end and
 # partial results cost in key tiles.
-_RESIDENT = {"general": 1024, "rows": 512, "tokens": 256}
-_OVERHEAD = {"general": 1, "rows": 6, "tokens": 4}
+_RESIDENT = {"general": 1024, "rows": 512}
+_OVERHEAD = {"general": 1, "rows": 3}
+#: Fewest key tiles of a part, and about the most parts of an item within an XCD.
+_SHORTEST_PART, _MOST_PARTS = 3, 32
 _XCDS = 8
-_MOST_PARTS = 64
 
 
 class _Work:
@@ -56,6 +58,111 @@ class _Work:
     def rows(self):
         """int64 [n, 6]: sequence, row begin, row end, first key, last key, key head."""
         return np.concatenate(self.parts) if self.parts else np.empty((0, 6), np.int64)
+
+
+def _ending_by(costs, order, resident, overhead, limit):
+    """Parts ``{item: [(first, last), ...]}`` of the items that are cut so that ``resident`` workgroups end by
+    ``limit``, or None: what an item has beyond ``limit`` goes to workgroups of its own, the rest to the
+    least loaded one, cut at the room there is."""
+    room_of_one = limit - overhead
+    cuts, small, busy = {}, [], 0
+    for item in order:
+        cost = costs[item]
+        if cost <= room_of_one:
+            small.append((cost, item, 0))
+            continue
+        full, left = divmod(cost, room_of_one)
+        if left and left < _SHORTEST_PART:  # a short rest comes off the last full part
+            full, left = full - 1, left + room_of_one
+            last = cost - _SHORTEST_PART
+            cuts[item] = [(i * room_of_one, (i + 1) * room_of_one) for i in range(full)]
+            if last > full * room_of_one:
+                cuts[item].append((full * room_of_one, last))
+                full += 1
+            small.append((_SHORTEST_PART, item, last))
+        else:
+            cuts[item] = [(i * room_of_one, (i + 1) * room_of_one) for i in range(full)]
+            if left:
+                small.append((left, item, full * room_of_one))
+        busy += full
+    if busy > resident or (busy == resident and small):
+        return None
+    small.sort(key=lambda piece: -piece[0])
+    loads = [0] * (resident - busy)
+    for left, item, at in small:
+        while left:
+            room = room_of_one - loads[0]
+            piece = left
+            if left > room:
+                if room < _SHORTEST_PART:
+                    return None
+                piece = room if left - room >= _SHORTEST_PART else left - _SHORTEST_PART
+            heapq.heapreplace(loads, loads[0] + piece + overhead)
+            if piece < costs[item]:
+                cuts.setdefault(item, []).append((at, at + piece))
+            at, left = at + piece, left - piece
+    return cuts
+
+
+def _cut(costs, resident, overhead):
+    """Cuts items of ``costs`` key tiles into parts, so that ``resident`` workgroups that take parts in
+    order, longest first, end together as early as they can.  Returns ``{item: [(first, last), ...]}`` of
+    the items that are cut."""
+    n, longest, total = len(costs), max(costs), sum(costs)
+    if longest < 2 * _SHORTEST_PART or n > 4 * resident:
+        return {}
+    order = sorted(range(n), key=lambda item: -costs[item])
+    if n <= resident:
+        uncut = longest + overhead
+    else:
+        loads = [0] * resident
+        for item in order:
+            heapq.heapreplace(loads, loads[0] + costs[item] + overhead)
+        uncut = max(loads)
+    shortest = max(_SHORTEST_PART, -(-longest // _MOST_PARTS))
+    low, high, cuts = max((total + n * overhead) // resident, shortest + overhead), uncut, {}
+    while low < 0.98 * high:  # the earliest end that parts reach, within a fiftieth
+        middle = (low + high) // 2
+        found = _ending_by(costs, order, resident, overhead, middle)
+        if found is None:
+            low = middle + 1
+        else:
+            high, cuts = middle, found
+    return cuts if high <= 0.95 * uncut else {}  # joining the parts would cost what little they save
+
+
+def _share_out(tiles, owner, resident, overhead):
+    """The parts of items of ``tiles`` key tiles: int64 [parts, 4] of (item, first tile, last tile, XCD), item
+    after item.  The items of one ``owner`` (they share keys) go to one XCD as far as the XCDs stay evenly
+    loaded, and are cut for the workgroups of that XCD."""
+    order = np.argsort(owner, kind="stable")
+    ends = np.cumsum(tiles[order] + overhead)
+    starts = ends - tiles[order] - overhead
+    whole = int(ends[-1])
+    parts = []
+    for xcd in range(_XCDS):
+        begin, end = xcd * whole // _XCDS, (xcd + 1) * whole // _XCDS
+        # Items that overlap this XCD's share of the work; those on a border are cut there.
+        inside = np.arange(np.searchsorted(ends, begin, side="right"), np.searchsorted(starts, end, side="left"))
+        if not len(inside):
+            continue
+        limit = tiles[order[inside]]
+        low, high = (np.clip(at - starts[inside], 0, limit) for at in (begin, end))
+        # A piece too short to be worth a workgroup joins the neighbour's.
+        low, high = (np.where((at < limit) & (at < _SHORTEST_PART), 0, np.where(limit - at < _SHORTEST_PART, limit, at))
+                     for at in (low, high))
+        # An item without keys is a part of its own where it begins.
+        kept = (high > low) | ((limit == 0) & (starts[inside] >= begin))
+        inside, low, high = inside[kept], low[kept], high[kept]
+        if not len(inside):
+            continue
+        costs = (high - low).tolist()
+        cuts = _cut(costs, resident // _XCDS, overhead)
+        for index, (item, first, cost) in enumerate(zip(order[inside].tolist(), low.tolist(), costs)):
+            for a, b in cuts.get(index, ((0, cost),)):
+                parts.append((item, first + a, first + b, xcd))
+    parts = np.asarray(parts, dtype=np.int64)
+    return parts[np.lexsort((parts[:, 1], parts[:, 0]))]
 
 
 class AttentionPlan:
@@ -121,7 +228,7 @@ class AttentionPlan:
     def _lay_out(self, found, queries):
         cache = self.cache
         work = {name: _Work() for name in _RESIDENT}
-        tiles = {"general": GENERAL_ROWS, "rows": ROW_TILE, "tokens": TOKEN_ROWS}
+        tiles = {"general": GENERAL_ROWS, "rows": ROW_TILE}
         table, at, lengths, starts = [], [], [], []
         words, row = _lib.ATTEND_ZEROS, 0
         for number, (item, n) in enumerate(zip(found, queries)):
@@ -139,24 +246,28 @@ class AttentionPlan:
         self._lengths, self._starts = np.asarray(lengths, dtype=np.int64), np.asarray(starts, dtype=np.int64)
         self._counts = np.asarray(queries, dtype=np.int64)
         items, merges, self._partial_rows, counts = [], [], 0, {}
-        for form in ("general", "rows", "tokens"):
+        for form in ("general", "rows"):
             made = self._split(form, work[form].rows(), merges)
             counts[form] = len(made)
             items.append(made)
         items = np.concatenate(items)
         merges = np.concatenate(merges) if merges else np.empty((0, _lib.ATTEND_MERGE), np.int64)
-        self._counts_of = (counts["general"], counts["rows"], counts["tokens"])
+        self._counts_of = (counts["general"], counts["rows"])
         first_item = _lib.ATTEND_ZEROS + len(table)
         self._items, self._merges = first_item, first_item + items.size
-        self._n_merges = len(merges)
-        self._most_rows = int(merges[:, 2].max()) if len(merges) else 0
+        # Merges that take a workgroup to a row come first (the kernels' rule).
+        joined = counts["general"] == 0 and cache.head_dim % 8 == 0 and cache.head_dim <= 128
+        many = (merges[:, 5] > _lib.ATTEND_FEW_PARTS) | (not joined)
+        merges = np.concatenate([merges[many], merges[~many]])
+        self._n_merges, self._n_many = len(merges), int(many.sum())
+        self._most_rows = [int(part[:, 2].max(initial=0)) for part in np.split(merges, [self._n_many])]
         self._holes = int(any(page < 0 for page in table))
         need(self._partial_rows < 1 << 31, "the step's partial results are too many")
         words = np.concatenate([np.zeros(_lib.ATTEND_ZEROS, np.int64), np.asarray(table, np.int64), items.ravel(),
                                 merges.ravel()])
         from .paged_cache import upload
 
-        self._tiled = counts["rows"] + counts["tokens"]
+        self._tiled = counts["rows"]
         with entered(cache.device):
             self.buffer = upload(words, cache.device)
             self._stream = raw_stream(cache.device)
@@ -178,19 +289,18 @@ class AttentionPlan:
         return tile // per * unit + tile % per * KEY_TILE
 
     def _split(self, form, blocks, merges):
-        """Items of a form's row blocks: the keys of a block in as many parts as fill the card best, in
-        launch order."""
+        """Items of a form's row blocks, in launch order: the keys of a block in one part, or in as many as
+        let the card's workgroups end together."""
         if not len(blocks):
             return np.empty((0, _lib.ATTEND_ITEM), np.int64)
         sequence, begin, end, first, last, head = blocks.T
         tile0 = self._tile_of(first)
         tiles = np.where(last > first, self._tile_of(np.maximum(last - 1, 0)) + 1 - tile0, 0)
-        most = self._longest_part(form, tiles)
-        parts = np.maximum(1, -(-tiles // most))
-        which = np.repeat(np.arange(len(blocks)), parts)
+        owner = sequence * self.cache.heads + head
+        which, low, high, xcd = _share_out(tiles, owner, _RESIDENT[form], _OVERHEAD[form]).T
+        parts = np.bincount(which, minlength=len(blocks))
         part = np.arange(len(which)) - np.repeat(np.cumsum(parts) - parts, parts)
-        n, total = parts[which], tiles[which]
-        low, high = part * total // n, (part + 1) * total // n
+        n = parts[which]
         rows = (end - begin)[which]
         # Partial rows: part after part of a block, block after block.
         need_rows = np.where(parts > 1, parts * (end - begin), 0)
@@ -212,41 +322,20 @@ class AttentionPlan:
             merge[:, 0], merge[:, 1], merge[:, 2] = self._starts[sequence[several]], begin[several], rows
             merge[:, 3], merge[:, 4], merge[:, 5] = head[several], base[several], parts[several]
             merges.append(merge)
-        return items[self._order(high - low, sequence[which] * self.cache.heads + head[which])]
-
-    def _longest_part(self, form, tiles):
-        """Key tiles of the longest part: the length whose parts finish first by the estimate (rounds of
-        resident workgroups times the longest part and its overhead)."""
-        resident, overhead = _RESIDENT[form], _OVERHEAD[form]
-        longest = int(tiles.max())
-        best, chosen = None, max(1, longest)
-        for parts in range(1, _MOST_PARTS + 1):
-            length = max(1, -(-longest // parts))
-            n = int(np.maximum(1, -(-tiles // length)).sum())
-            cost = float(tiles.sum()) + n * overhead
-            one = length + overhead * (1 if parts == 1 else 1.5)
-            time = max(-(-n // resident) * one if n <= 4 * resident else cost / resident + one / 2, one)
-            if best is None or time < 0.97 * best:
-                best, chosen = time, length
-            if length == 1 or n > 8 * resident:
-                break
-        return chosen
+        return self._ordered(items, high - low, xcd)
 
     @staticmethod
-    def _order(cost, owner):
-        """Launch order: workgroup b runs on XCD b % 8, so the items of one (sequence, key head), which
-        share keys, go to one XCD as far as the XCDs stay evenly loaded; long ones first."""
-        n = len(cost)
-        if n <= _XCDS:
-            return np.argsort(-cost, kind="stable")
-        by_owner = np.argsort(owner, kind="stable")
-        load = np.cumsum(cost[by_owner] + 1)
-        xcd = np.minimum((load - 1) * _XCDS // int(load[-1]), _XCDS - 1)
-        buckets = [by_owner[xcd == x] for x in range(_XCDS)]
-        buckets = [bucket[np.argsort(-cost[bucket], kind="stable")] for bucket in buckets]
-        # The i-th items of all buckets, XCD after XCD; a bucket that runs out leaves its place to the next.
-        rank = np.concatenate([np.arange(len(bucket)) for bucket in buckets])
-        return np.concatenate(buckets)[np.argsort(rank, kind="stable")]
+    def _ordered(items, cost, xcd):
+        """Items in launch order: workgroup b runs on XCD b % 8, so the i-th longest item of XCD x stands at
+        8 i + x; empty items fill up the XCDs that have fewer."""
+        if len(items) <= _XCDS:
+            return items[np.argsort(-cost, kind="stable")]
+        buckets = [np.flatnonzero(xcd == x) for x in range(_XCDS)]
+        out = np.zeros((max(len(bucket) for bucket in buckets), _XCDS, _lib.ATTEND_ITEM), np.int64)
+        out[:, :, 9] = -1
+        for x, bucket in enumerate(buckets):
+            out[:len(bucket), x] = items[bucket[np.argsort(-cost[bucket], kind="stable")]]
+        return out.reshape(-1, _lib.ATTEND_ITEM)
 
     # -----------------------------------------------------------------------------------------
 
@@ -267,8 +356,8 @@ class AttentionPlan:
         scale = struct.unpack("<i", struct.pack("<f", self.scale * math.log2(math.e)))[0]
         fields = (0, 0, 0, 0, 0, 0, 0, *q_stride, k[page], k[token], k[head], v[page], v[token], v[head], *out_stride,
                   self.group, self.heads, cache.head_dim, cache.page_tokens, cache.pages, self.block or 0, self.window or 0,
-                  scale, self._partial_rows, self._items, *self._counts_of, self._merges, self._n_merges, self._most_rows,
-                  self._holes, self._unit(), 0)
+                  scale, self._partial_rows, self._items, *self._counts_of, self._merges, self._n_merges, self._n_many,
+                  *self._most_rows, self._holes, self._unit())
         return bytes(_Image(*fields))
 
 

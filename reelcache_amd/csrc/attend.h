@@ -64,8 +64,7 @@ __device__ __forceinline__ int64_t partial_stats(const rch_attend& A, int64_t ro
     return A.partial_ptr + A.partial_rows * A.head_dim * 4 + row * 8;
 }
 
-// Launches the forms' items (row-tiled and few-rows kernels).
+// Launches the items of the tiled form.
 int launch_attend_rows(const rch_attend& A, int dtype, int first, hipStream_t stream);
-int launch_attend_tokens(const rch_attend& A, int dtype, int first, hipStream_t stream);
 
 }  // namespace rch

@@ -7,8 +7,8 @@
 // are base 2 (scale carries log2 e).  Two parts of a row's keys join the same way.
 //
 // The general form takes every head_dim up to 256, alignment and element type: one wave per row, a
-// lane per key for the scores, a lane per channel for the sums.  The forms that tile for the matrix
-// cores are in attend_rows.hip and attend_tokens.hip.
+// lane per key for the scores, a lane per channel for the sums.  The form that tiles for the matrix
+// cores is in attend_rows.hip.
 #include "attend.h"
 
 namespace rch {
@@ -102,34 +102,130 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A,
     }
 }
 
-// Joins the parts of rows whose keys were split: a thread per row and channel, parts in order.
+// Joins the parts of rows whose keys were split (the same order whatever the timing).  Rows of many parts
+// (single tokens over long histories) take a workgroup each, whose waves share the parts; rows of few, a
+// thread per eight channels.
+constexpr int kMergeRows = 16, kFewParts = RCH_ATTEND_FEW_PARTS;
+
+struct MergedRow {
+    int64_t out, lse;  // element offsets of the row's output and logarithm
+};
+__device__ __forceinline__ MergedRow merged_row(const rch_attend& A, int q_row, int row, int kv_head) {
+    const int group = static_cast<int>(A.group), token = row / group, head = kv_head * group + row - token * group;
+    return {(q_row + token) * A.out_token_stride + head * A.out_head_stride, (q_row + token) * A.heads + head};
+}
+
+template <int DT>
+__global__ void __launch_bounds__(256) attend_merge_many_kernel(const rch_attend A) {
+    typedef typename AttendType<DT>::type T;
+    constexpr int C = RCH_ATTEND_MAX_DIM / 64;
+    __shared__ float sums[4][RCH_ATTEND_MAX_DIM], stat[4][2];
+    const RCH_GLOBAL int32_t* w = gin<int32_t>(A.plan_ptr) + A.merges + static_cast<int64_t>(blockIdx.x) * RCH_ATTEND_MERGE;
+    const int rows = w[2], parts = w[5], dim = static_cast<int>(A.head_dim), r = blockIdx.y;
+    if (r >= rows) return;
+    const int64_t first = static_cast<int64_t>(w[4]) + r;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // A wave takes parts wave, wave + 4, ..: its own reference, sum and weighted sums.
+    float reference = kNoReference, sum = 0.0f, acc[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = 0.0f;
+    for (int base = wave; base < parts; base += 256) {
+        const int part = base + 4 * lane;
+        f2 stats = {kNoReference, 0.0f};
+        if (part < parts) stats = *gin<f2>(partial_stats(A, first + static_cast<int64_t>(part) * rows));
+        float next = stats[1] != 0.0f ? stats[0] : kNoReference;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) next = fmaxf(next, __shfl_xor(next, o));
+        next = fmaxf(next, reference);
+        const float old = exp2_of(reference - next), mine = stats[1] != 0.0f ? exp2_of(stats[0] - next) : 0.0f;
+        reference = next;
+        float total = stats[1] * mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+        sum = __builtin_fmaf(sum, old, total);
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] *= old;
+        const int count = min(64, (parts - base + 3) / 4);
+#pragma unroll 8
+        for (int p = 0; p < count; ++p) {
+            const float fade = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), p));
+            const RCH_GLOBAL float* from = gin<float>(partial_sums(A, first + static_cast<int64_t>(base + 4 * p) * rows));
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (64 * c < dim) acc[c] = __builtin_fmaf(from[min(lane + 64 * c, dim - 1)], fade, acc[c]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+        if (lane + 64 * c < dim) sums[wave][lane + 64 * c] = acc[c];
+    if (lane == 0) {
+        stat[wave][0] = reference;
+        stat[wave][1] = sum;
+    }
+    __syncthreads();
+    const int d = threadIdx.x;
+    reference = kNoReference;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (stat[i][1] != 0.0f) reference = fmaxf(reference, stat[i][0]);
+    float value = 0.0f;
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float fade = stat[i][1] != 0.0f ? exp2_of(stat[i][0] - reference) : 0.0f;
+        sum = __builtin_fmaf(stat[i][1], fade, sum);
+        if (d < dim) value = __builtin_fmaf(sums[i][d], fade, value);
+    }
+    const MergedRow M = merged_row(A, w[0], w[1] + r, w[3]);
+    if (d < dim) gout<T>(A.out_ptr)[M.out + d] = static_cast<T>(value * (sum == 0.0f ? 0.0f : 1.0f / sum));
+    if (d == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[M.lse] = row_lse(reference, sum);
+}
+
 template <int DT>
 __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
     typedef typename AttendType<DT>::type T;
-    const RCH_GLOBAL int32_t* w = gin<int32_t>(A.plan_ptr) + A.merges + static_cast<int64_t>(blockIdx.x) * RCH_ATTEND_MERGE;
-    const int q_row = w[0], row_begin = w[1], rows = w[2], kv_head = w[3], first = w[4], parts = w[5];
-    const int dim = static_cast<int>(A.head_dim), group = static_cast<int>(A.group);
-    const int index = blockIdx.y * 256 + threadIdx.x;
-    const int r = index / dim, d = index - r * dim;
-    if (r >= rows) return;
-    const int token = (row_begin + r) / group, head = kv_head * group + (row_begin + r) % group;
+    const RCH_GLOBAL int32_t* w = gin<int32_t>(A.plan_ptr) + A.merges
+                                  + (static_cast<int64_t>(blockIdx.x) + A.n_many) * RCH_ATTEND_MERGE;
+    const int rows = w[2], parts = w[5], dim = static_cast<int>(A.head_dim);
+    const int64_t first = w[4];
+    const int r = blockIdx.y * kMergeRows + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+    if (r >= rows || d >= dim) return;
+    const MergedRow M = merged_row(A, w[0], w[1] + r, w[3]);
+    f2 stats[kFewParts];
+    f4 low[kFewParts], high[kFewParts];
     float reference = kNoReference;
-    for (int p = 0; p < parts; ++p) {
-        const f2 stats = *gin<f2>(partial_stats(A, first + static_cast<int64_t>(p) * rows + r));
-        if (stats[1] != 0.0f) reference = fmaxf(reference, stats[0]);
+#pragma unroll
+    for (int p = 0; p < kFewParts; ++p) {
+        if (p < parts) {
+            const int64_t at = first + static_cast<int64_t>(p) * rows + r;
+            stats[p] = *gin<f2>(partial_stats(A, at));
+            low[p] = gin<f4>(partial_sums(A, at) + 4 * d)[0];
+            high[p] = gin<f4>(partial_sums(A, at) + 4 * d)[1];
+        }
     }
-    float sum = 0.0f, acc = 0.0f;
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-        const int64_t at = first + static_cast<int64_t>(p) * rows + r;
-        const f2 stats = *gin<f2>(partial_stats(A, at));
-        const float fade = stats[1] != 0.0f ? exp2_of(stats[0] - reference) : 0.0f;
-        sum = __builtin_fmaf(stats[1], fade, sum);
-        acc = __builtin_fmaf(gin<float>(partial_sums(A, at))[d], fade, acc);
+#pragma unroll
+    for (int p = 0; p < kFewParts; ++p)
+        if (p < parts && stats[p][1] != 0.0f) reference = fmaxf(reference, stats[p][0]);
+    float sum = 0.0f, acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int p = 0; p < kFewParts; ++p) {
+        if (p < parts) {
+            const float fade = stats[p][1] != 0.0f ? exp2_of(stats[p][0] - reference) : 0.0f;
+            sum = __builtin_fmaf(stats[p][1], fade, sum);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                acc[e] = __builtin_fmaf(low[p][e], fade, acc[e]);
+                acc[4 + e] = __builtin_fmaf(high[p][e], fade, acc[4 + e]);
+            }
+        }
     }
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    gout<T>(A.out_ptr)[(q_row + token) * A.out_token_stride + head * A.out_head_stride + d] = static_cast<T>(acc * inverse);
-    if (d == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[(q_row + token) * A.heads + head] = row_lse(reference, sum);
+    typedef T t8 __attribute__((ext_vector_type(8)));
+    t8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = static_cast<T>(acc[e] * inverse);
+    *reinterpret_cast<RCH_GLOBAL t8*>(gout<T>(A.out_ptr) + M.out + d) = v;
+    if (d == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[M.lse] = row_lse(reference, sum);
 }
 
 template <int DT>
@@ -145,9 +241,15 @@ int run(const rch_attend& A, hipStream_t stream) {
         const int status = launch_attend_rows(A, DT, first, stream);
         if (status != RCH_OK) return status;
     }
-    if (A.n_merges) {
-        const uint32_t blocks = static_cast<uint32_t>((A.most_rows * A.head_dim + 255) / 256);
-        hipLaunchKernelGGL(attend_merge_kernel<DT>, dim3(static_cast<uint32_t>(A.n_merges), blocks), dim3(256), 0, stream, A);
+    if (A.n_many) {
+        const dim3 grid(static_cast<uint32_t>(A.n_many), static_cast<uint32_t>(A.most_rows_many));
+        hipLaunchKernelGGL(attend_merge_many_kernel<DT>, grid, dim3(256), 0, stream, A);
+        const int status = check_launch("rch_attend_run (merge)");
+        if (status != RCH_OK) return status;
+    }
+    if (A.n_merges > A.n_many) {
+        const dim3 grid(static_cast<uint32_t>(A.n_merges - A.n_many), static_cast<uint32_t>((A.most_rows + kMergeRows - 1) / kMergeRows));
+        hipLaunchKernelGGL(attend_merge_kernel<DT>, grid, dim3(256), 0, stream, A);
         return check_launch("rch_attend_run (merge)");
     }
     return RCH_OK;
@@ -168,12 +270,18 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
     if (A.group < 1 || A.heads < 1 || A.head_dim < 1 || A.head_dim > RCH_ATTEND_MAX_DIM || A.page_tokens < 1 || A.pages < 1
         || A.page_tokens > 0x7fffffff || A.pages > 0x7fffffff || A.block < 0 || A.window < 0 || A.block > 0x7fffffff)
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid sizes");
-    if (A.n_general < 0 || A.n_rows < 0 || A.n_tokens < 0 || A.n_merges < 0 || A.n_general + A.n_rows + A.n_tokens > 0x7fffffff)
+    if (A.n_general < 0 || A.n_rows < 0 || A.n_merges < 0 || A.n_general + A.n_rows > 0x7fffffff)
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid item counts");
-    if (A.n_merges && (!A.partial_ptr || A.most_rows < 1)) return fail(RCH_E_CONFIG, "rch_attend_run: merges need partials");
-    if (A.n_general + A.n_rows + A.n_tokens == 0) return RCH_OK;
+    if (A.n_merges && (!A.partial_ptr || A.n_many < 0 || A.n_many > A.n_merges || A.most_rows < 0 || A.most_rows_many < 0
+                       || A.most_rows_many > 65535))
+        return fail(RCH_E_CONFIG, "rch_attend_run: invalid merges");
+    // Rows of few parts are joined in aligned pieces of eight channels.
+    if (A.n_merges > A.n_many && (A.head_dim % 8 || A.head_dim > 128 || A.out_ptr % 16
+                                  || (A.out_token_stride | A.out_head_stride) * (dtype == RCH_DT_F32 ? 4 : 2) % 16))
+        return fail(RCH_E_CONFIG, "rch_attend_run: merges of few parts need aligned rows of 8n <= 128 channels");
+    if (A.n_general + A.n_rows == 0) return RCH_OK;
     if (!A.q_ptr || !A.k_ptr || !A.v_ptr || !A.out_ptr || !A.plan_ptr) return fail(RCH_E_CONFIG, "rch_attend_run: null address");
-    if (A.n_rows + A.n_tokens) {
+    if (A.n_rows) {
         // The tiled forms: whole 16-byte pieces, a tile's rows within 2 GiB, tiles that start over at a page of
         // at least a tile or at 64 keys.
         const int64_t size = dtype == RCH_DT_F32 ? 4 : 2;

@@ -10,70 +10,84 @@ namespace rch {
 
 namespace {
 
-template <int DT, int NB, bool PAGED>
+template <int DT, int NB, int MODE>
 __global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A, int first_item) {
     typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2> Tile;
-    constexpr int RB = Tile::RB, KT = Tile::KT, ES = Tile::ES, kTileBytes = KT * RB, NI = kTileBytes / 1024 / 4;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
+    constexpr int KT = Tile::KT, ES = Tile::ES, kTileBytes = KT * Tile::RB;
+    constexpr int kStageBytes = 2 * kTileBytes;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStageBytes];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const AttendItem I = attend_item(A, first_item + blockIdx.x);
+    if (I.row_begin >= I.row_end) return;  // a plan's filling
     const QueryRow R = query_row(A, I, I.row_begin + 32 * wave + (lane & 31));
     const float scale = __int_as_float(static_cast<int>(A.scale_bits));
     Tile tile;
     tile.init(A, I, R, lane);
+    WaveRange range;
+    range.init(R);
 
-    KeyWalk<KT, PAGED> walk;
-    walk.table = (const const_int*)(uintptr_t)(A.plan_ptr + 4 * static_cast<int64_t>(I.table));
-    walk.unit = static_cast<int>(A.tile_unit);
-    walk.end = I.key_end;
-    walk.pages = static_cast<int>(A.pages);
-    walk.begin(I.key_begin);
-    Fetch<Tile, NI, PAGED> fetch;
-    fetch.init(A, wave * NI, lane);
-    const int64_t k_head = A.k_ptr + ES * I.kv_head * A.k_head_stride, v_head = A.v_ptr + ES * I.kv_head * A.v_head_stride;
+    KeyWalk<KT, MODE> walk;
+    walk.begin(A, I, ES);
+    Fetch<Tile, MODE> fetch;
+    fetch.init(A, wave, lane);
     lds_char* const tiles = (lds_char*)lds;
-    const uint32_t lds_base = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tiles)) + wave * NI * 1024;
+    const uint32_t mine = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tiles)) + wave * (kTileBytes / 4);
 
-    if (!walk.done()) fetch.issue(A, walk, k_head, v_head, lds_base, lds_base + kTileBytes);
-    int stage = 2 * kTileBytes, first = 0, last = 0;
+    // The tile on its way: its first key and keys; `walk` is the one after it.
+    bool coming = false;
+    int next_key = 0, next_keys = 0, at = kStageBytes, key = 0, keys = 0, first = 0, last = 0;
     uint64_t held = ~uint64_t{0};
-    // Waits for the next tile, fetches the one after it, and finds what the wave's rows see of it.
-    auto advance = [&]() {
-        const int base = walk.base(), count = walk.count();
+    auto send = [&](int to) {
+        coming = !walk.done();
+        if (!coming) return;
+        next_key = walk.base;
+        next_keys = walk.count();
+        fetch.issue(A, walk, mine + to, mine + to + kTileBytes);
         walk.next();
-        const int other = stage;
-        stage = 2 * kTileBytes - stage;
+        fetch.look_up(walk);
+    };
+    fetch.look_up(walk);
+    send(0);
+    // Waits for the tile on its way, fetches another one, and tells whether the wave's rows see any of it.
+    auto advance = [&]() {
         // The tile has landed in every wave's share, and no wave reads the other half any more.
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (!walk.done()) fetch.issue(A, walk, k_head, v_head, lds_base + other, lds_base + other + kTileBytes);
-        first = R.first - base;
-        last = min(R.last - base, count);
-        if constexpr (!PAGED) {
+        key = next_key;
+        keys = next_keys;
+        const int other = at;
+        at = kStageBytes - at;
+        send(other);
+        if constexpr (MODE != kPage) {
             if (A.holes) {
-                const int key = min(base + lane, I.key_end - 1);
-                const int id = page_entry(walk.table, key / static_cast<int>(A.page_tokens));
+                const int id = page_entry(walk.table, min(key + lane, I.key_end - 1) / static_cast<int>(A.page_tokens));
                 held = __ballot(id >= 0 && id < A.pages);
             }
         }
-        return __any(first < KT && last > 0 && last > first);
+        return range.sees(key, keys);
     };
-    auto masked = [&]() { return __any(first > 0 || last < KT) || held != ~uint64_t{0}; };
+    auto masked = [&]() {
+        first = R.first - key;
+        last = min(R.last - key, keys);
+        return range.masked(key, keys, KT) || held != ~uint64_t{0};
+    };
     bool rare = false;
-    while (!walk.done()) {
+    while (coming) {
         if (!advance()) continue;
         const bool some = masked();
-        if (some && Tile::any_infinite(tiles + stage + kTileBytes, lane)) {
+        if (some && Tile::any_infinite(tiles + at + kTileBytes, lane)) {
             rare = true;
             break;
         }
-        tile.template step<false>(tiles + stage, tiles + stage + kTileBytes, scale, first, last, held, some, lane);
+        tile.template step<false>(tiles + at, tiles + at + kTileBytes, scale, first, last, held, some, lane);
     }
     if (rare) {
         for (bool seen = true;; seen = advance()) {
-            if (seen)
-                tile.template step<true>(tiles + stage, tiles + stage + kTileBytes, scale, first, last, held, masked(), lane);
-            if (walk.done()) break;
+            if (seen) {
+                const bool some = masked();
+                tile.template step<true>(tiles + at, tiles + at + kTileBytes, scale, first, last, held, some, lane);
+            }
+            if (!coming) break;
         }
     }
 
@@ -110,8 +124,10 @@ __global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A,
 template <int DT, int NB>
 void launch(const rch_attend& A, int first, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(A.n_rows));
-    if (A.tile_unit == A.page_tokens) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, true>), grid, dim3(256), 0, stream, A, first);
-    else hipLaunchKernelGGL((attend_rows_kernel<DT, NB, false>), grid, dim3(256), 0, stream, A, first);
+    constexpr int kShareRows = RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2>::KT / 4;
+    if (A.tile_unit == A.page_tokens) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kPage>), grid, dim3(256), 0, stream, A, first);
+    else if (A.page_tokens % kShareRows == 0) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kShare>), grid, dim3(256), 0, stream, A, first);
+    else hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kRow>), grid, dim3(256), 0, stream, A, first);
 }
 
 template <int DT>

@@ -111,108 +111,154 @@ __device__ __forceinline__ int page_entry(const const_int* table, int index) {
     return gin<int32_t>(static_cast<int64_t>(reinterpret_cast<uintptr_t>(table)))[index];
 }
 
-// The walk over an item's key tiles.  PAGED: tiles of KT keys start over at each page and lie in one page
-// (its table entry is one scalar load); otherwise tiles are KT consecutive keys of any pages.
-template <int KT, bool PAGED>
+// How a tile's rows are found: kPage: tiles start over at each page and lie in one page; kShare: a tile is KT
+// consecutive keys, and the KT / 4 rows that a wave fetches lie in one page (its size is a multiple of that);
+// kRow: any page size.  The first two take a scalar base to a fetch, the last an address to a lane.
+enum TileMode { kPage, kShare, kRow };
+
+// The walk over an item's key tiles.
+template <int KT, int MODE>
 struct KeyWalk {
     const const_int* table;
-    int unit, end, pages;  // tokens that tiles start over at, last key, pages of the pool
-    int page, off, id;     // current tile: its page index and first row there (PAGED), else key / unit and key % unit
+    int unit, end, pages;     // tokens that tiles start over at, last key, pages of the pool
+    int base, left, page;     // current tile: first key, keys from it to the unit's end, page index (kPage)
+    int64_t k, v;             // kPage: addresses of the tile's first K and V row
+    int64_t k_head, v_head, k_page, v_page;  // of the item's head in page 0; bytes of a page
+    int k_tile, v_tile;       // bytes of KT rows
 
-    __device__ __forceinline__ int base() const { return page * unit + off; }
-    __device__ __forceinline__ bool done() const { return base() >= end; }
-    __device__ __forceinline__ void settle() {  // skips dropped pages
-        if constexpr (PAGED) {
-            while (!done()) {
-                id = table[page];
-                if (id >= 0 && id < pages) return;
-                ++page;
-                off = 0;
+    __device__ __forceinline__ bool done() const { return base >= end; }
+    // Enters the page of `base` (at row `off`), skipping dropped ones.
+    __device__ __forceinline__ void enter(int off) {
+        while (!done()) {
+            const int id = table[page];
+            if (id >= 0 && id < pages) {
+                k = k_head + id * k_page + static_cast<int64_t>(off / KT) * k_tile;
+                v = v_head + id * v_page + static_cast<int64_t>(off / KT) * v_tile;
+                return;
             }
-        }
-    }
-    __device__ __forceinline__ void begin(int key) {
-        page = key / unit;
-        off = (key - page * unit) / KT * KT;
-        settle();
-    }
-    // The next tile after `tiles` tiles.
-    __device__ __forceinline__ void next() {
-        off += KT;
-        if (off >= unit) {
+            base += left;
+            left = unit;
             ++page;
             off = 0;
-            settle();
+        }
+    }
+    __device__ __forceinline__ void begin(const rch_attend& A, const AttendItem& I, int es) {
+        table = (const const_int*)(uintptr_t)(A.plan_ptr + 4 * static_cast<int64_t>(I.table));
+        unit = static_cast<int>(A.tile_unit);
+        end = I.key_end;
+        pages = static_cast<int>(A.pages);
+        k_head = A.k_ptr + es * I.kv_head * A.k_head_stride;
+        v_head = A.v_ptr + es * I.kv_head * A.v_head_stride;
+        k_page = es * A.k_page_stride;
+        v_page = es * A.v_page_stride;
+        k_tile = static_cast<int>(es * KT * A.k_token_stride);
+        v_tile = static_cast<int>(es * KT * A.v_token_stride);
+        page = I.key_begin / unit;
+        const int off = (I.key_begin - page * unit) / KT * KT;
+        base = page * unit + off;
+        left = unit - off;
+        if constexpr (MODE == kPage) enter(off);
+    }
+    __device__ __forceinline__ void next() {
+        if constexpr (MODE == kPage) {
+            if (left > KT) {
+                base += KT;
+                left -= KT;
+                k += k_tile;
+                v += v_tile;
+                return;
+            }
+            base += left;
+            left = unit;
+            ++page;
+            enter(0);
+        } else {
+            base += KT;
         }
     }
     // Keys of the current tile.
-    __device__ __forceinline__ int count() const {
-        int n = end - base();
-        if constexpr (PAGED) n = min(n, unit - off);
-        return min(n, KT);
-    }
+    __device__ __forceinline__ int count() const { return min(end - base, MODE == kPage ? min(left, KT) : KT); }
 };
 
-// Fetches the calling wave's share of a K and a V tile: NI instructions of 1024 bytes from instruction
-// `first` on.  Tile: the arithmetic's layout (ES: bytes of an element, RB: LDS bytes of a row, the swizzles).
-template <typename Tile, int NI, bool PAGED>
+// Fetches the calling wave's quarter of a K and a V tile: NI instructions of 1024 bytes each.  Tile: the
+// arithmetic's layout (ES: bytes of an element, RB: LDS bytes of a row, the swizzles).
+template <typename Tile, int MODE>
 struct Fetch {
-    static constexpr int KT = Tile::KT, RB = Tile::RB, ES = Tile::ES, kRows = 1024 / RB, kPieces = RB / 16;
-    uint32_t k_at[PAGED ? NI : 1], v_at[PAGED ? NI : 1];  // PAGED: byte offsets within the tile
-    int row0, piece, pieces;                                // row of instruction 0, the lane's piece, pieces of a head
-    uint32_t magic;
+    static constexpr int KT = Tile::KT, RB = Tile::RB, ES = Tile::ES, kRows = 1024 / RB, kPieces = RB / 16, kShareRows = KT / 4;
+    static constexpr int NI = kShareRows / kRows;
+    uint32_t k_at[MODE == kRow ? 1 : NI], v_at[MODE == kRow ? 1 : NI];  // byte offsets from the scalar base
+    int share, row0, piece, pieces;  // the share's first row, the lane's first one, its piece, pieces of a head
+    uint32_t size, magic, row_bytes, k_row, v_row;
+    int ids[MODE == kRow ? NI : 1];  // pages of the walk's tile
 
-    __device__ __forceinline__ void init(const rch_attend& A, int first, int lane) {
+    __device__ __forceinline__ void init(const rch_attend& A, int wave, int lane) {
         pieces = static_cast<int>(A.head_dim) * ES / 16;
-        row0 = first * kRows + lane / kPieces;
+        share = wave * kShareRows;
+        row0 = share + lane / kPieces;
         piece = lane % kPieces;
-        if constexpr (PAGED) {
+        row_bytes = static_cast<uint32_t>(A.head_dim) * ES;
+        k_row = static_cast<uint32_t>(A.k_token_stride * ES);
+        v_row = static_cast<uint32_t>(A.v_token_stride * ES);
+        size = static_cast<uint32_t>(A.page_tokens);
+        magic = (65536u + size - 1) / size;  // x / size for x < 128, size <= 64
+        if constexpr (MODE != kRow) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int row = row0 + i * kRows;
+                const int row = row0 + i * kRows, from = MODE == kPage ? row : row - share;
                 const int kc = piece ^ Tile::k_swizzle(row), vc = piece ^ Tile::v_swizzle(row);
-                k_at[i] = kc < pieces ? row * static_cast<uint32_t>(A.k_token_stride * ES) + kc * 16 : kOutOfRange;
-                v_at[i] = vc < pieces ? row * static_cast<uint32_t>(A.v_token_stride * ES) + vc * 16 : kOutOfRange;
+                k_at[i] = kc < pieces ? from * k_row + kc * 16 : kOutOfRange;
+                v_at[i] = vc < pieces ? from * v_row + vc * 16 : kOutOfRange;
             }
+        }
+    }
+    // Pages from the first key's that row x (counted from that page's start) lies in.
+    __device__ __forceinline__ int page_of(uint32_t x) const {
+        return size < 64 ? static_cast<int>((x * magic) >> 16) : (x >= size ? 1 : 0);
+    }
+
+    // Looks up the pages of the walk's tile (called when the walk arrives there, a tile before its fetch, so that
+    // the fetch waits for no table).
+    __device__ __forceinline__ void look_up(const KeyWalk<KT, MODE>& W) {
+        if (MODE == kPage || W.done()) return;
+        const int keys = W.end - W.base, page0 = W.base / static_cast<int>(size);
+        const int off0 = W.base - page0 * static_cast<int>(size);
+        // Rows behind the last key: its page.
+        if constexpr (MODE == kShare) {
+            ids[0] = W.table[page0 + page_of(off0 + min(share, keys - 1))];
         } else {
-            const uint32_t size = static_cast<uint32_t>(A.page_tokens);
-            magic = (65536u + size - 1) / size;  // x / size for x < 128, size <= 64
+#pragma unroll
+            for (int i = 0; i < NI; ++i) ids[i] = page_entry(W.table, page0 + page_of(off0 + min(row0 + i * kRows, keys - 1)));
         }
     }
 
-    __device__ __forceinline__ void issue(const rch_attend& A, const KeyWalk<KT, PAGED>& W, int64_t k_head, int64_t v_head,
-                                          uint32_t k_lds, uint32_t v_lds) const {
-        if constexpr (PAGED) {
-            const int64_t k = k_head + ES * (W.id * A.k_page_stride + W.off * A.k_token_stride);
-            const int64_t v = v_head + ES * (W.id * A.v_page_stride + W.off * A.v_token_stride);
-            const int rows = W.count() - 1;
-            const uint32_t row_bytes = static_cast<uint32_t>(A.head_dim) * ES;
-            const u4 kr = tile_rsrc(k, rows * static_cast<uint32_t>(A.k_token_stride * ES) + row_bytes);
-            const u4 vr = tile_rsrc(v, rows * static_cast<uint32_t>(A.v_token_stride * ES) + row_bytes);
+    __device__ __forceinline__ void issue(const rch_attend& A, const KeyWalk<KT, MODE>& W, uint32_t k_lds, uint32_t v_lds) const {
+        if constexpr (MODE != kRow) {
+            int64_t k = W.k, v = W.v;
+            int rows = W.count();
+            if constexpr (MODE == kShare) {
+                // Rows behind the last key, and those of a dropped page, are out of the buffer's range: zeros.
+                const int x = W.base % static_cast<int>(size) + share, in_page = x - page_of(x) * static_cast<int>(size);
+                rows = ids[0] >= 0 && ids[0] < W.pages ? min(rows - share, kShareRows) : 0;
+                k = W.k_head + ids[0] * W.k_page + in_page * static_cast<int64_t>(k_row);
+                v = W.v_head + ids[0] * W.v_page + in_page * static_cast<int64_t>(v_row);
+                if (rows <= 0) k = v = A.plan_ptr;
+            }
+            const u4 kr = tile_rsrc(k, rows > 0 ? (rows - 1) * k_row + row_bytes : 0);
+            const u4 vr = tile_rsrc(v, rows > 0 ? (rows - 1) * v_row + row_bytes : 0);
 #pragma unroll
             for (int i = 0; i < NI; ++i) fetch_buffer(kr, k_at[i], k_lds + i * 1024);
 #pragma unroll
             for (int i = 0; i < NI; ++i) fetch_buffer(vr, v_at[i], v_lds + i * 1024);
         } else {
-            const int base = W.base(), keys = W.end - base;
-            const int size = static_cast<int>(A.page_tokens);
-            const int page0 = base / size, off0 = base - page0 * size;
-            int id[NI];
+            const int keys = W.end - W.base, off0 = W.base % static_cast<int>(size);
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int row = row0 + i * kRows, x = off0 + row;
-                const int q = size > 64 ? (x >= size ? 1 : 0) : static_cast<int>((x * magic) >> 16);
-                id[i] = row < keys ? page_entry(W.table, page0 + q) : -1;
-            }
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int row = row0 + i * kRows, x = off0 + row;
-                const int q = size > 64 ? (x >= size ? 1 : 0) : static_cast<int>((x * magic) >> 16);
-                const int in_page = x - q * size;
-                const bool held = id[i] >= 0 && id[i] < A.pages;
+                const int row = row0 + i * kRows, x = off0 + row, in_page = x - page_of(x) * static_cast<int>(size);
+                const int id = row < keys ? ids[i] : -1;
+                const bool held = id >= 0 && id < W.pages;
                 const int kc = piece ^ Tile::k_swizzle(row), vc = piece ^ Tile::v_swizzle(row);
-                const int64_t k = k_head + ES * (id[i] * A.k_page_stride + in_page * A.k_token_stride) + kc * 16;
-                const int64_t v = v_head + ES * (id[i] * A.v_page_stride + in_page * A.v_token_stride) + vc * 16;
+                const int64_t k = W.k_head + id * W.k_page + in_page * static_cast<int64_t>(k_row) + kc * 16;
+                const int64_t v = W.v_head + id * W.v_page + in_page * static_cast<int64_t>(v_row) + vc * 16;
                 // Rows that no page holds, and pieces behind the head, read the plan's zeros.
                 fetch_global(held && kc < pieces ? k : A.plan_ptr, k_lds + i * 1024);
                 fetch_global(held && vc < pieces ? v : A.plan_ptr, v_lds + i * 1024);
@@ -221,7 +267,33 @@ struct Fetch {
     }
 };
 
-    // Bit i of seen[b]: whether the row sees the key of register i of block b.
+// What the rows of a wave see, as scalars.
+struct WaveRange {
+    int first_low, first_high, last_low, last_high;
+
+    __device__ __forceinline__ void init(const QueryRow& R) {
+        first_low = first_high = R.first;
+        last_low = last_high = R.last;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            first_low = min(first_low, __shfl_xor(first_low, o));
+            first_high = max(first_high, __shfl_xor(first_high, o));
+            last_low = min(last_low, __shfl_xor(last_low, o));
+            last_high = max(last_high, __shfl_xor(last_high, o));
+        }
+        first_low = __builtin_amdgcn_readfirstlane(first_low);
+        first_high = __builtin_amdgcn_readfirstlane(first_high);
+        last_low = __builtin_amdgcn_readfirstlane(last_low);
+        last_high = __builtin_amdgcn_readfirstlane(last_high);
+    }
+    // Whether a row may see a key of a tile, and whether one may not see all of its KT keys.
+    __device__ __forceinline__ bool sees(int base, int count) const { return base + count > first_low && base < last_high; }
+    __device__ __forceinline__ bool masked(int base, int count, int kt) const {
+        return base < first_high || base + kt > last_low || count < kt;
+    }
+};
+
+// Bit i of seen[b]: whether the row sees the key of register i of block b.
     template <int KB>
 __device__ __forceinline__ void seen_keys(uint32_t (&seen)[KB], int first, int last, uint64_t held, int h) {
         // Bits of keys [first, last) of the tile, then those of this lane's half.
@@ -289,13 +361,21 @@ struct RowTile {
         const int h = lane >> 5;
         f16v s[KB];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            s[b] = f16v{};
+        for (int b = 0; b < KB; ++b) s[b] = f16v{};
+        // The blocks' chains side by side, the reads kAhead products ahead.
 #pragma unroll
-            for (int c = 0; c < 2 * NB; ++c) {
+        for (int c = 0; c < 2 * NB; ++c)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
                 const vec8 k = *reinterpret_cast<const __attribute__((address_space(3))) vec8*>(k_tile + k_lane[c] + b * 32 * RB);
                 s[b] = H::mfma(k, q[c], s[b]);
             }
+        constexpr int kAhead = 6, kProducts = 2 * NB * KB;
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            if (i + kAhead < kProducts) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         if (masked) {
             uint32_t seen[KB];
@@ -304,6 +384,12 @@ struct RowTile {
             for (int b = 0; b < KB; ++b)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[b][i] = seen[b] >> i & 1u ? s[b][i] : -INFINITY;
+        }
+        // The first values, on their way while the weights are computed.
+        vec8 v[NB];
+        if constexpr (!RARE) {
+#pragma unroll
+            for (int b = 0; b < NB; ++b) v[b] = values(v_tile + v_lane[b], 0);
         }
         float top = s[0][0];
 #pragma unroll
@@ -348,7 +434,11 @@ struct RowTile {
 #pragma unroll
         for (int c = 0; c < 2 * KB; ++c)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) o[b] = H::mfma(values(v_tile + v_lane[b], c), p[c], o[b]);
+            for (int b = 0; b < NB; ++b) {
+                const vec8 now = RARE ? values(v_tile + v_lane[b], c) : v[b];
+                if (!RARE && c + 1 < 2 * KB) v[b] = values(v_tile + v_lane[b], c + 1);
+                o[b] = H::mfma(now, p[c], o[b]);
+            }
     }
 
     // Whether a value of the tile is infinite or NaN: with a weight of 0 (a key that a row does not see) its

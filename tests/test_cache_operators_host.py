@@ -309,6 +309,8 @@ def test_plan_covers_every_visible_key_once(host, size, dim, layout, block, wind
     seen = {}
     partial_rows = []
     for table, length, q_row, n, begin, end, head, low, high, part, *_ in items.tolist():
+        if begin >= end:  # filling
+            continue
         number = [i for i in range(len(lengths)) if starts[i] == q_row and queries[i] == n and lengths[i] == length]
         assert len(number) == 1 and 0 <= begin < end <= n * group and 0 <= low <= high <= length
         assert words[table:table + -(-length // size)].tolist() == cache.pages_of(sequences[number[0]])
@@ -341,7 +343,7 @@ def test_header_matches_the_binding():
     defines = {name: int(value) for name, value in re.findall(r"#define (RCH_[A-Z0-9_]+) (\d+)\b", HEADER.read_text())}
     expected = {"RCH_PAIRS_INTERLEAVED": _lib.PAIRS_INTERLEAVED, "RCH_PAIRS_HALF": _lib.PAIRS_HALF,
                 "RCH_ATTEND_ITEM": _lib.ATTEND_ITEM, "RCH_ATTEND_MERGE": _lib.ATTEND_MERGE, "RCH_ATTEND_ZEROS": _lib.ATTEND_ZEROS,
-                "RCH_ATTEND_MAX_DIM": _lib.ATTEND_MAX_DIM, "RCH_ATTEND_FAST_DIM": _lib.ATTEND_FAST_DIM}
+                "RCH_ATTEND_MAX_DIM": _lib.ATTEND_MAX_DIM, "RCH_ATTEND_FEW_PARTS": _lib.ATTEND_FEW_PARTS, "RCH_ATTEND_FAST_DIM": _lib.ATTEND_FAST_DIM}
     assert {name: defines.get(name) for name in expected} == expected
     lib = _lib.library()
     assert lib.rch_rotary_size() == 8 * len(_lib.ROTARY_FIELDS) and lib.rch_attend_size() == 8 * len(_lib.ATTEND_FIELDS)
