@@ -24,6 +24,7 @@ __global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A,
     const float scale = __int_as_float(static_cast<int>(A.scale_bits));
     Tile tile;
     tile.init(A, I, R, lane);
+    const bool active = I.row_begin + 32 * wave < I.row_end;  // a wave without rows only fetches
     WaveRange range;
     range.init(R);
 
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A,
                 held = __ballot(id >= 0 && id < A.pages);
             }
         }
-        return range.sees(key, keys);
+        return active && range.sees(key, keys);
     };
     auto masked = [&]() {
         first = R.first - key;
