@@ -615,6 +615,15 @@ typedef struct rch_attend {
     int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64 */
 } rch_attend;                /* 36 x int64 = 288 bytes */
 
+/*
+ * Cuts the row blocks of a plan into parts (host only): block i has tiles[i] key tiles and belongs to owner[i]
+ * (blocks of one owner share keys).  parts: int64 [capacity][4] of (block, first tile, last tile, XCD), block
+ * after block; *count of them, at most n + 2 * resident + 16.  resident: workgroups that the card runs at
+ * once; overhead: what one spends besides its tiles, in tiles.
+ */
+int rch_attend_share(const int64_t* tiles, const int64_t* owner, int64_t n, int64_t resident, int64_t overhead, int64_t* parts,
+                     int64_t capacity, int64_t* count);
+
 int rch_attend_size(void);
 int rch_attend_run(const rch_attend* args_host, int dtype, void* stream);
 

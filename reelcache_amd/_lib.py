@@ -119,6 +119,7 @@ _SIGNATURES = {
     "rch_rotary": ([_p, _i, _i, _i, _p], _i),
     "rch_pages_copy": ([_p, _p, _i, _p], _i),
     "rch_words_store": ([_p, _p, _i, _p], _i),
+    "rch_attend_share": ([_p, _p, _i64, _i64, _i64, _p, _i64, _p], _i),
     "rch_attend_size": ([], _i),
     "rch_attend_run": ([_p, _i, _p], _i),
 }
@@ -192,11 +193,17 @@ def register(signatures: dict) -> None:
                 function.argtypes, function.restype = arguments, result
 
 
+_FUNCTIONS: dict = {}
+
+
 def function(name: str):
-    """The bound entry point ``name`` (for callers that keep it; its status goes to :func:`check`)."""
-    found = getattr(library(), name, None)
+    """The bound entry point ``name`` (its status goes to :func:`check`)."""
+    found = _FUNCTIONS.get(name)
     if found is None:
-        raise UnsupportedError(f"{LIBRARY.name} does not export {name}; rebuild it")
+        found = getattr(library(), name, None)
+        if found is None:
+            raise UnsupportedError(f"{LIBRARY.name} does not export {name}; rebuild it")
+        _FUNCTIONS[name] = found
     return found
 
 

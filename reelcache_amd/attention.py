@@ -16,7 +16,6 @@ that a query does not see have no influence on it, whatever their slots hold.
 from __future__ import annotations
 
 import ctypes
-import heapq
 import math
 import struct
 
@@ -36,8 +35,6 @@ GENERAL_ROWS, ROW_TILE = 16, 128
 # partial results cost in key tiles.
 _RESIDENT = {"general": 1024, "rows": 512}
 _OVERHEAD = {"general": 1, "rows": 3}
-#: Fewest key tiles of a part, and about the most parts of an item within an XCD.
-_SHORTEST_PART, _MOST_PARTS = 3, 32
 _XCDS = 8
 
 
@@ -60,109 +57,16 @@ class _Work:
         return np.concatenate(self.parts) if self.parts else np.empty((0, 6), np.int64)
 
 
-def _ending_by(costs, order, resident, overhead, limit):
-    """Parts ``{item: [(first, last), ...]}`` of the items that are cut so that ``resident`` workgroups end by
-    ``limit``, or None: what an item has beyond ``limit`` goes to workgroups of its own, the rest to the
-    least loaded one, cut at the room there is."""
-    room_of_one = limit - overhead
-    cuts, small, busy = {}, [], 0
-    for item in order:
-        cost = costs[item]
-        if cost <= room_of_one:
-            small.append((cost, item, 0))
-            continue
-        full, left = divmod(cost, room_of_one)
-        if left and left < _SHORTEST_PART:  # a short rest comes off the last full part
-            full, left = full - 1, left + room_of_one
-            last = cost - _SHORTEST_PART
-            cuts[item] = [(i * room_of_one, (i + 1) * room_of_one) for i in range(full)]
-            if last > full * room_of_one:
-                cuts[item].append((full * room_of_one, last))
-                full += 1
-            small.append((_SHORTEST_PART, item, last))
-        else:
-            cuts[item] = [(i * room_of_one, (i + 1) * room_of_one) for i in range(full)]
-            if left:
-                small.append((left, item, full * room_of_one))
-        busy += full
-    if busy > resident or (busy == resident and small):
-        return None
-    small.sort(key=lambda piece: -piece[0])
-    loads = [0] * (resident - busy)
-    for left, item, at in small:
-        while left:
-            room = room_of_one - loads[0]
-            piece = left
-            if left > room:
-                if room < _SHORTEST_PART:
-                    return None
-                piece = room if left - room >= _SHORTEST_PART else left - _SHORTEST_PART
-            heapq.heapreplace(loads, loads[0] + piece + overhead)
-            if piece < costs[item]:
-                cuts.setdefault(item, []).append((at, at + piece))
-            at, left = at + piece, left - piece
-    return cuts
-
-
-def _cut(costs, resident, overhead):
-    """Cuts items of ``costs`` key tiles into parts, so that ``resident`` workgroups that take parts in
-    order, longest first, end together as early as they can.  Returns ``{item: [(first, last), ...]}`` of
-    the items that are cut."""
-    n, longest, total = len(costs), max(costs), sum(costs)
-    if longest < 2 * _SHORTEST_PART or n > 4 * resident:
-        return {}
-    order = sorted(range(n), key=lambda item: -costs[item])
-    if n <= resident:
-        uncut = longest + overhead
-    else:
-        loads = [0] * resident
-        for item in order:
-            heapq.heapreplace(loads, loads[0] + costs[item] + overhead)
-        uncut = max(loads)
-    shortest = max(_SHORTEST_PART, -(-longest // _MOST_PARTS))
-    low, high, cuts = max((total + n * overhead) // resident, shortest + overhead), uncut, {}
-    while low < 0.98 * high:  # the earliest end that parts reach, within a fiftieth
-        middle = (low + high) // 2
-        found = _ending_by(costs, order, resident, overhead, middle)
-        if found is None:
-            low = middle + 1
-        else:
-            high, cuts = middle, found
-    return cuts if high <= 0.95 * uncut else {}  # joining the parts would cost what little they save
-
-
 def _share_out(tiles, owner, resident, overhead):
-    """The parts of items of ``tiles`` key tiles: int64 [parts, 4] of (item, first tile, last tile, XCD), item
-    after item.  The items of one ``owner`` (they share keys) go to one XCD as far as the XCDs stay evenly
-    loaded, and are cut for the workgroups of that XCD."""
-    order = np.argsort(owner, kind="stable")
-    ends = np.cumsum(tiles[order] + overhead)
-    starts = ends - tiles[order] - overhead
-    whole = int(ends[-1])
-    parts = []
-    for xcd in range(_XCDS):
-        begin, end = xcd * whole // _XCDS, (xcd + 1) * whole // _XCDS
-        # Items that overlap this XCD's share of the work; those on a border are cut there.
-        inside = np.arange(np.searchsorted(ends, begin, side="right"), np.searchsorted(starts, end, side="left"))
-        if not len(inside):
-            continue
-        limit = tiles[order[inside]]
-        low, high = (np.clip(at - starts[inside], 0, limit) for at in (begin, end))
-        # A piece too short to be worth a workgroup joins the neighbour's.
-        low, high = (np.where((at < limit) & (at < _SHORTEST_PART), 0, np.where(limit - at < _SHORTEST_PART, limit, at))
-                     for at in (low, high))
-        # An item without keys is a part of its own where it begins.
-        kept = (high > low) | ((limit == 0) & (starts[inside] >= begin))
-        inside, low, high = inside[kept], low[kept], high[kept]
-        if not len(inside):
-            continue
-        costs = (high - low).tolist()
-        cuts = _cut(costs, resident // _XCDS, overhead)
-        for index, (item, first, cost) in enumerate(zip(order[inside].tolist(), low.tolist(), costs)):
-            for a, b in cuts.get(index, ((0, cost),)):
-                parts.append((item, first + a, first + b, xcd))
-    parts = np.asarray(parts, dtype=np.int64)
-    return parts[np.lexsort((parts[:, 1], parts[:, 0]))]
+    """The parts of row blocks of ``tiles`` key tiles (``rch_attend_share``): int64 [parts, 4] of (block,
+    first tile, last tile, XCD), block after block.  The blocks of one ``owner`` (they share keys) go to one
+    XCD as far as the XCDs stay evenly loaded, and are cut so that an XCD's workgroups end together."""
+    tiles, owner = (np.ascontiguousarray(x, dtype=np.int64) for x in (tiles, owner))
+    parts = np.empty((len(tiles) + 2 * resident + 16, 4), np.int64)
+    count = ctypes.c_int64(0)
+    _lib.check(_lib.function("rch_attend_share")(tiles.ctypes.data, owner.ctypes.data, len(tiles), resident, overhead,
+                                                 parts.ctypes.data, len(parts), ctypes.byref(count)))
+    return parts[:count.value]
 
 
 class AttentionPlan:

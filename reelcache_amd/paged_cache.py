@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 import heapq
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -65,14 +66,28 @@ _FEW_TOKENS = 64
 def upload(values, device):
     """An int32 array on ``device``, written on its current stream without a host wait: small ones in
     launch arguments, larger ones from pinned memory (the block stays reserved until the copy has run)."""
+    values = np.ascontiguousarray(values, dtype=np.int32)
+    if values.size <= _ARGUMENT_WORDS:
+        return upload_words(values.tobytes(), values.shape, device)
+    _refuse_capture()
+    return torch.from_numpy(values).pin_memory().to(device, non_blocking=True)
+
+
+def upload_words(words, shape, device):
+    """The same of a small table that the caller packed into bytes."""
+    _refuse_capture()
+    out = torch.empty(shape, dtype=torch.int32, device=device)
+    _lib.check(_lib.function("rch_words_store")(out.data_ptr(), words, len(words) // 4, raw_stream(device)))
+    return out
+
+
+def _refuse_capture():
     if capturing():
         raise ConfigurationError("page tables, slots and plans are built before a HIP-graph capture, not in it")
-    values = np.ascontiguousarray(values, dtype=np.int32)
-    if values.size > _ARGUMENT_WORDS:
-        return torch.from_numpy(values).pin_memory().to(device, non_blocking=True)
-    out = torch.empty(values.shape, dtype=torch.int32, device=device)
-    _lib.check(_lib.function("rch_words_store")(out.data_ptr(), values.ctypes.data, values.size, raw_stream(device)))
-    return out
+
+
+def _pack(words):
+    return struct.pack(f"{len(words)}i", *words)
 
 
 class PagedCache:
@@ -202,55 +217,55 @@ class PagedCache:
         found.pages[first:first + pages] = [HOLE] * pages
         self._moved += 1
 
-    def _begun(self, found):
-        """Rows of the last page in use when it is not full, else 0."""
-        return found.tokens % self.page_tokens
-
     def extend(self, sequences, counts):
         """Room for ``counts[i]`` more tokens of ``sequences[i]``: new pages, and a copy (in every layer)
         of a begun page that other sequences share.  Returns the :class:`Slots` of the new tokens, packed
         sequence after sequence."""
-        sequences, counts = list(sequences), list(counts)
+        counts = list(counts)
         found = self._several(sequences)
         need(len(counts) == len(found), "extend takes one count for each sequence")
         for n in counts:
             count(n, "a token count")
         need_gpu(self.device, "a paged cache")
-        uses: dict[int, int] = {}
-        wanted = []  # (copies the begun page, new pages) of each sequence
+        _refuse_capture()
+        size, in_use, shared = self.page_tokens, self._uses, {}
+        wanted, total, most = [], 0, 0  # (rows of a begun page to copy, or 0; new pages) of each sequence
         for item, n in zip(found, counts):
-            more = -(-(item.tokens + n) // self.page_tokens) - len(item.pages)
-            copies = False
-            if n and self._begun(item):
+            tokens = item.tokens
+            more = -(-(tokens + n) // size) - len(item.pages)
+            begun = tokens % size if n else 0
+            if begun:
                 last = item.pages[-1]
-                shared = uses.get(last, self._uses[last])
-                copies = shared > 1
-                uses[last] = shared - copies
-            wanted.append((copies, more))
-        need(sum(item.tokens + n for item, n in zip(found, counts)) < 1 << 31, "a step covers fewer than 2**31 tokens")
-        total = sum(copies + more for copies, more in wanted)
-        if total > len(self._free):
-            raise CapacityError(f"{total} pages are needed and {len(self._free)} are free")
-        if capturing():
-            raise ConfigurationError("a cache grows before a HIP-graph capture, not in it")
+                owners = shared.get(last, in_use[last])
+                if owners > 1:
+                    shared[last] = owners - 1
+                else:
+                    begun = 0
+            wanted.append((begun, more))
+            total += more + (begun > 0)
+            most += tokens + n
+        need(most < 1 << 31, "a step covers fewer than 2**31 tokens")
+        free = self._free
+        if total > len(free):
+            raise CapacityError(f"{total} pages are needed and {len(free)} are free")
         moves, starts = [], []
-        for item, n, (copies, more) in zip(found, counts, wanted):
-            if copies:
-                page = self._take()
-                moves.append((item.pages[-1], page, self._begun(item)))
-                self._release(item.pages[-1:])
-                item.pages[-1] = page
+        for item, n, (begun, more) in zip(found, counts, wanted):
+            pages = item.pages
+            if begun:
+                page = heapq.heappop(free)
+                in_use[page] = 1
+                in_use[pages[-1]] -= 1
+                moves += (pages[-1], page, begun)
+                pages[-1] = page
                 self._shared += 1
-            item.pages.extend(self._take() for _ in range(more))
+            for _ in range(more):
+                page = heapq.heappop(free)
+                in_use[page] = 1
+                pages.append(page)
             starts.append(item.tokens)
             item.tokens += n
         self._copy(moves)
         return self._slots(found, starts, counts)
-
-    def _take(self):
-        page = heapq.heappop(self._free)
-        self._uses[page] = 1
-        return page
 
     def slots(self, sequences, starts, counts):
         """The :class:`Slots` of tokens ``starts[i] .. starts[i] + counts[i]`` that ``sequences[i]`` has
@@ -273,9 +288,10 @@ class PagedCache:
     def _slots(self, found, starts, counts):
         size = self.page_tokens
         if sum(counts) <= _FEW_TOKENS:
-            index = np.asarray([item.pages[at // size] * size + at % size for item, start, n in zip(found, starts, counts)
-                                for at in range(start, start + n)], dtype=np.int32)
-            return self._made(index)
+            words = [item.pages[at // size] * size + at % size for item, start, n in zip(found, starts, counts)
+                     for at in range(start, start + n)]
+            with entered(self.device):
+                return self._made(upload_words(_pack(words), (len(words),), self.device))
         pages, base = [], []  # the pages of all tokens, and where each sequence's page 0 would lie among them
         for item, start, n in zip(found, starts, counts):
             first = start // size
@@ -289,30 +305,30 @@ class PagedCache:
         index = at - page * size
         if total:
             index += np.asarray(pages, dtype=np.int64)[page + np.repeat(np.asarray(base, dtype=np.int64), counts)] * size
-        return self._made(index)
+        with entered(self.device):
+            return self._made(upload(index, self.device))
 
     def _made(self, index):
-        with entered(self.device):
-            return Slots(upload(index, self.device), index.size, self, self._moved + self._shared, raw_stream(self.device))
+        return Slots(index, index.shape[0], self, self._moved + self._shared, raw_stream(self.device))
 
     # -----------------------------------------------------------------------------------------
     # Page copies
     # -----------------------------------------------------------------------------------------
 
     def _copy(self, moves):
-        """Copies pages in every pool: ``moves`` of (source, destination, leading rows)."""
+        """Copies pages in every pool: ``moves`` is flat, (source, destination, leading rows) of each."""
         if not moves:
             return
         with entered(self.device):
             if self._copies is None:
                 self._copies = [_pools(pool, self._axes, self.pages, self.page_tokens)
                                 for pool in self._joined_pools()]
-            flat = [value for move in moves for value in move]
-            table = (ctypes.c_int32 * len(flat))(*flat)
-            stream = torch.cuda.current_stream(self.device)
-            for pools, fields in self._copies:
-                pools.record_stream(stream)
-                _lib.call("rch_pages_copy", fields, table, len(moves), stream.cuda_stream)
+            table, stream = _pack(moves), raw_stream(self.device)
+            for pools, fields, streams in self._copies:
+                if stream not in streams:  # the allocator learns of a stream that the table was not made on
+                    pools.record_stream(torch.cuda.current_stream(self.device))
+                    streams.add(stream)
+                _lib.check(_lib.function("rch_pages_copy")(fields, table, len(moves) // 3, stream))
 
     def _joined_pools(self):
         """K and V pools as one group where their strides agree (one launch), else as two."""
@@ -323,9 +339,9 @@ class PagedCache:
     def compact(self):
         """Move pages down until those in use are the lowest ones (the highest in use go to the lowest
         free, in order).  Returns the moves as (from, to) pairs."""
-        used = [page for page, uses in enumerate(self._uses) if uses]
-        moved = [page for page in used if page >= len(used)]
-        return self._relocate(moved, [page for page in range(len(used)) if not self._uses[page]])
+        n = self.pages - len(self._free)  # pages in use
+        uses = self._uses
+        return self._relocate([page for page in range(n, self.pages) if uses[page]], sorted(page for page in self._free if page < n))
 
     def make_contiguous(self, sequence):
         """Move a sequence's pages to the lowest run of consecutive free pages (for :meth:`view`); pages
@@ -348,22 +364,28 @@ class PagedCache:
         if not source:
             return []
         need_gpu(self.device, "a paged cache")
-        self._copy([(a, b, self.page_tokens) for a, b in zip(source, target)])
-        names = dict(zip(source, target))
-        for a, b in names.items():
-            self._uses[b], self._uses[a] = self._uses[a], 0
+        _refuse_capture()
+        moves, size, uses, names = [], self.page_tokens, self._uses, {}
+        for a, b in zip(source, target):
+            moves += (a, b, size)
+            uses[b], uses[a] = uses[a], 0
+            names[a] = b
         for item in self._sequences.values():
-            item.pages = [names.get(page, page) for page in item.pages]
-        self._free = [page for page, uses in enumerate(self._uses) if not uses]  # ascending: a heap
+            pages = item.pages
+            for at, page in enumerate(pages):
+                if page in names:
+                    pages[at] = names[page]
+        self._free = [page for page, n in enumerate(uses) if not n]  # ascending: a heap
         self._moved += 1
-        return list(zip(source, target))
+        self._copy(moves)
+        return list(names.items())
 
     def load_tables(self, tables):
         """Start over with sequences 0, 1, ... of ``(pages, tokens)`` each (e.g. saved with
         :meth:`pages_of`); the pools keep what they hold.  Sequences may share pages."""
         loaded, uses = {}, [0] * self.pages
         for number, (pages, tokens) in enumerate(tables):
-            pages = [int(page) for page in pages]
+            pages = list(map(int, pages))
             need(len(pages) == -(-count(tokens, "tokens") // self.page_tokens), "the pages do not hold the tokens")
             real = [page for page in pages if page != HOLE] if HOLE in pages else pages
             need(not real or (min(real) >= 0 and max(real) < self.pages), "a page lies outside the pool")
@@ -379,13 +401,18 @@ class PagedCache:
 
     def page_table(self, sequences):
         """int32 ``[sequences, most pages]`` on the device; :data:`HOLE` behind a sequence's last page."""
-        found = [self._get(s) for s in sequences]
+        tables = [self._get(s).pages for s in sequences]
         need_gpu(self.device, "a paged cache")
-        table = np.full((len(found), max((len(item.pages) for item in found), default=0)), HOLE, dtype=np.int32)
-        for row, item in zip(table, found):
-            row[:len(item.pages)] = item.pages
+        width = max(map(len, tables), default=0)
+        words = []
+        for pages in tables:
+            words += pages
+            words += [HOLE] * (width - len(pages))
+        shape = (len(tables), width)
         with entered(self.device):
-            return upload(table, self.device)
+            if len(words) <= _ARGUMENT_WORDS:
+                return upload_words(_pack(words), shape, self.device)
+            return upload(np.asarray(words, dtype=np.int32).reshape(shape), self.device)
 
     # -----------------------------------------------------------------------------------------
     # Contents
@@ -499,14 +526,13 @@ def _apart(pool):
 
 
 def _pools(group, axes, pages, page_tokens):
-    """(device table of pool addresses, ``rch_pages`` fields) of pools with the same strides."""
+    """(device table of pool addresses, ``rch_pages`` fields, streams the table is known to) of pools with the
+    same strides."""
     size = group[0].element_size()
     stride = group[0].stride()
     page, token, head = (stride[axis] * size for axis in axes)
     heads, row = group[0].shape[axes[2]], group[0].shape[4] * size
     addresses = [pool.data_ptr() + layer * stride[0] * size for pool in group for layer in range(pool.shape[0])]
-    if capturing():
-        raise ConfigurationError("a cache's first page copy cannot be captured: it uploads the pools' addresses")
     table = torch.tensor(addresses, dtype=torch.int64).to(group[0].device)  # waits: usable on every stream
     joined = head == row or heads == 1  # a token's heads are one run
     segments, segment, width = (1, 0, heads * row) if joined else (heads, head, row)
@@ -515,7 +541,7 @@ def _pools(group, axes, pages, page_tokens):
         mix |= address
     fields = (table.data_ptr(), len(addresses), pages, page if pages > 1 else 0, page_tokens, segments, segment,
               token if page_tokens > 1 else width, width, mix)
-    return table, (ctypes.c_int64 * len(fields))(*fields)
+    return table, (ctypes.c_int64 * len(fields))(*fields), {raw_stream(group[0].device)}
 
 
 __all__ = ["HOLE", "PagedCache", "Slots"]

@@ -1,6 +1,7 @@
 """Host logic of the cache operators (page tables, slots, plans) and their refusals, without a GPU."""
 
 import contextlib
+import heapq
 import re
 from pathlib import Path
 
@@ -23,6 +24,7 @@ def host(monkeypatch):
     copies = []
 
     def copy(self, moves):
+        moves = list(zip(*[iter(moves)] * 3))
         copies.extend(moves)
         for pool in (self.keys, self.values):
             for source, target, rows in moves:
@@ -37,7 +39,9 @@ def host(monkeypatch):
         monkeypatch.setattr(module, "entered", lambda device: contextlib.nullcontext())
         monkeypatch.setattr(module, "raw_stream", lambda device: 0)
     monkeypatch.setattr(paged_cache, "capturing", lambda: False)
-    monkeypatch.setattr(paged_cache, "upload", lambda values, device: torch.from_numpy(np.asarray(values, dtype=np.int32)))
+    monkeypatch.setattr(paged_cache, "upload", lambda values, device: torch.from_numpy(np.array(values, dtype=np.int32)))
+    monkeypatch.setattr(paged_cache, "upload_words", lambda words, shape, device:
+                        torch.from_numpy(np.frombuffer(words, dtype=np.int32).reshape(shape).copy()))
     return copies
 
 
@@ -335,6 +339,33 @@ def test_plan_covers_every_visible_key_once(host, size, dim, layout, block, wind
     assert not seen
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_parts_cover_their_blocks_and_share_the_work(seed):
+    """Every tile of every block lies in one part; the parts of an XCD end within a tenth (and one shortest
+    part) of what its workgroups cannot do without."""
+    rng = np.random.default_rng(seed)
+    n, resident, overhead = int(rng.integers(1, 1500)), int(rng.choice([8, 64, 512])), int(rng.integers(0, 7))
+    tiles = rng.integers(0, int(rng.choice([2, 20, 600])) + 1, n) if seed % 3 else np.full(n, int(rng.integers(1, 700)))
+    parts = attention._share_out(tiles, np.arange(n) // int(rng.integers(1, 40)), resident, overhead)
+    block, first, last, xcd = parts.T
+    at = 0
+    for index, (count, total) in enumerate(zip(np.bincount(block, minlength=n), tiles)):
+        own = slice(at, at + count)
+        assert count >= 1 and (block[own] == index).all() and first[at] == 0 and last[at + count - 1] == total
+        assert (first[own][1:] == last[own][:-1]).all() and ((last[own] > first[own]) | (total == 0)).all()
+        at += count
+    assert at == len(parts) and xcd.min() >= 0 and xcd.max() < 8
+    if n > resident // 2:
+        return
+    for x in range(8):
+        costs = np.sort((last - first)[xcd == x])[::-1]
+        loads = [0] * max(1, resident // 8)
+        for cost in costs.tolist():
+            heapq.heapreplace(loads, loads[0] + cost + overhead)
+        least = max((costs.sum() + len(costs) * overhead) / len(loads), -(-int(tiles.max()) // 32))
+        assert max(loads) <= 1.1 * least + 2 * (overhead + 6)
+
+
 def test_header_matches_the_binding():
     text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
     for struct, fields in (("rch_rotary_job", _lib.ROTARY_FIELDS), ("rch_pages", _lib.PAGES_FIELDS), ("rch_attend", _lib.ATTEND_FIELDS)):
@@ -378,3 +409,11 @@ def test_abi_refusals():
         with pytest.raises(ConfigurationError):
             _lib.call("rch_attend_run", words(_lib.ATTEND_FIELDS, **{**step, **bad}), dtype, None)
     _lib.call("rch_attend_run", words(_lib.ATTEND_FIELDS, **{**step, "n_general": 0}), 0, None)
+    tiles = (ctypes.c_int64 * 2)(5, 7)
+    parts, found = (ctypes.c_int64 * 8)(), ctypes.c_int64(0)
+    for arguments in ((tiles, tiles, 2, 0, 0, parts, 2), (tiles, tiles, -1, 8, 0, parts, 2), (None, tiles, 2, 8, 0, parts, 2),
+                      ((ctypes.c_int64 * 2)(5, -1), tiles, 2, 8, 0, parts, 2), (tiles, tiles, 2, 8, 0, parts, 0)):
+        with pytest.raises(ConfigurationError):
+            _lib.call("rch_attend_share", *arguments, ctypes.byref(found))
+    with pytest.raises(ConfigurationError):
+        _lib.call("rch_words_store", None, (ctypes.c_int32 * 1)(1), 1, None)
