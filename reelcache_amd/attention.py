@@ -76,8 +76,9 @@ class AttentionPlan:
 
     ``block``, ``window``: see the module docstring (``None``: no such bound).  ``scale``: a positive
     factor of the scores (default ``head_dim ** -0.5``).  The plan is bound to the pages that the
-    sequences have now; it is stale once pages move or are freed.  A captured graph keeps its plan's
-    tables as they are: keep the plan as long as the graph.
+    sequences have now; it is stale once pages move or are freed.  Its tables are written on the stream
+    that is current (other streams wait for it).  A captured graph keeps its plan's tables as they are:
+    keep the plan as long as the graph.
     """
 
     def __init__(self, cache, sequences, queries, *, heads, block=None, window=None, scale=None):
@@ -297,6 +298,8 @@ def run(q, k_address, v_address, plan, out, return_lse, pools=None):
     device = cache.device
     if q.dtype != cache.dtype or q.device != device:
         raise ConfigurationError("q must have the cache's dtype and device")
+    if q.requires_grad and torch.is_grad_enabled():
+        raise ConfigurationError("attention over a cache is not differentiable; run it under torch.no_grad()")
     with entered(device):
         given, q = q, _rows(q)
         more = shape[0] > plan.queries

@@ -13,7 +13,8 @@ caller's native caches serve as pools of one page (``PagedCache(k[None], v[None]
 
 The page tables are host state.  Whatever allocates takes the lowest free pages, in the order of the
 sequences given, and checks that there are enough before it changes anything.  Device work runs on the
-current stream of the cache's device, in order: callers that use several streams order them.
+current stream of the cache's device, in order: callers that use several streams order them, and threads
+that share a cache take turns.
 """
 
 from __future__ import annotations
@@ -28,7 +29,7 @@ import torch
 
 from . import _lib
 from ._checks import count, need, one_of, strided
-from .errors import CapacityError, ConfigurationError, StateError
+from .errors import CapacityError, ConfigurationError, StateError, UnsupportedError
 from .restore_model import OUTPUT_DTYPES, NativeView
 from .rotary import Launch, addresses_of, capturing, entered, known_calls, need_gpu, position_fields, raw_stream
 
@@ -40,7 +41,8 @@ _LAYOUTS = ("BTHD", "BHTD")
 class Slots:
     """Where new tokens go: built by :meth:`PagedCache.extend` or :meth:`PagedCache.slots` once per
     step, used by :meth:`PagedCache.store` in every layer.  ``index``: int32 ``[tokens]`` on the device,
-    page * page_tokens + row of each token."""
+    page * page_tokens + row of each token, written on the stream that was current then (other streams
+    wait for it)."""
 
     index: torch.Tensor
     tokens: int
@@ -106,6 +108,7 @@ class PagedCache:
             need(min(pool.shape) >= 1, f"{name} must not be empty")
             need(pool.stride(4) == 1 or pool.shape[4] == 1, f"{name} must have unit stride over the channels")
             need(_apart(pool), f"{name} must keep its elements apart")
+            need(not pool.requires_grad, f"{name} must not require gradients")
         need(keys.shape == values.shape and keys.dtype == values.dtype and keys.device == values.device,
              "keys and values must match in shape, dtype and device")
         self.keys, self.values, self.layout = keys, values, layout
@@ -115,7 +118,7 @@ class PagedCache:
         need(self.pages * self.page_tokens < 1 << 31, "a pool holds fewer than 2**31 tokens")
         self.device, self.dtype = keys.device, keys.dtype
         self._axes = (1, token, head)
-        self._geometry = (keys.shape[1:], keys.stride()[1:], values.stride()[1:], keys.dtype, keys.device)
+        self._geometry = (layout, keys.shape[1:], keys.stride()[1:], values.stride()[1:], keys.dtype, keys.device)
         self._sequences: dict[int, _Sequence] = {}
         self._next = 0
         self._uses = [0] * self.pages
@@ -246,6 +249,8 @@ class PagedCache:
             most += tokens + n
         need(most < 1 << 31, "a step covers fewer than 2**31 tokens")
         free = self._free
+        if shared:
+            self._need_copies()
         if total > len(free):
             raise CapacityError(f"{total} pages are needed and {len(free)} are free")
         moves, starts = [], []
@@ -315,6 +320,11 @@ class PagedCache:
     # Page copies
     # -----------------------------------------------------------------------------------------
 
+    def _need_copies(self):
+        """Refuses (before anything changes) what the page copy cannot take."""
+        if self.page_tokens * self.heads * self.head_dim * self.keys.element_size() >= 1 << 31:
+            raise UnsupportedError("pages of 2 GiB or more cannot be copied")
+
     def _copy(self, moves):
         """Copies pages in every pool: ``moves`` is flat, (source, destination, leading rows) of each."""
         if not moves:
@@ -365,6 +375,7 @@ class PagedCache:
             return []
         need_gpu(self.device, "a paged cache")
         _refuse_capture()
+        self._need_copies()
         moves, size, uses, names = [], self.page_tokens, self._uses, {}
         for a, b in zip(source, target):
             moves += (a, b, size)
@@ -462,6 +473,8 @@ class PagedCache:
             strided(x, name)
             if x.shape != shape or x.dtype != self.dtype or x.device != self.device:
                 raise ConfigurationError(f"{name} must be [tokens, heads, head_dim] of the cache's dtype and device")
+            if x.requires_grad and torch.is_grad_enabled():
+                raise ConfigurationError("a store is not differentiable; run it under torch.no_grad()")
         if slots.tokens == 0:
             return
         need_gpu(self.device, "a paged cache")

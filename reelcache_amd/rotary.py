@@ -290,15 +290,19 @@ class _Rotation(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         positions, grid, layout, pairing, inverse = ctx.arguments
-        ctx.saved_tensors  # noqa: B018  (checks the rows' version)
+        if isinstance(positions, TokenRows):
+            ctx.saved_tensors  # noqa: B018  (checks the rows' version)
         wanted = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[5 + i]]
         out = [None] * len(grads)
         if wanted:
-            turned = rotate(tuple(grads[i] for i in wanted), positions, grid=grid, layout=layout, pairing=pairing,
-                            inverse=not inverse)
+            given = tuple([grads[i] for i in wanted])
+            if torch.is_grad_enabled():  # a graph of the gradients is asked for
+                turned = rotate(given, positions, grid=grid, layout=layout, pairing=pairing, inverse=not inverse)
+            else:
+                turned = _rotate(given, positions, grid, layout, pairing, not inverse)
             for i, g in zip(wanted, turned):
                 out[i] = g
-        return (None,) * 5 + tuple(out)
+        return (None, None, None, None, None, *out)
 
 
 def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interleaved", inverse=False, out=None):

@@ -196,12 +196,17 @@ def test_stale_slots_are_refused(host):
     other = make()
     with pytest.raises(ConfigurationError, match="come from this cache"):
         other.store(0, slots, x, x)
+    slots = cache.slots([0], [0], [5])
+    for call in (lambda: cache.store(2, slots, x, x), lambda: cache.store(0, slots, x[:4], x), lambda: cache.store(0, slots, x, x.half()),
+                 lambda: cache.store(0, slots, x.clone().requires_grad_(True), x)):
+        with pytest.raises(ConfigurationError):
+            call()
 
 
 def test_pool_refusals():
     good = torch.zeros(1, 2, 4, 2, 8)
     for keys, values in ((good[0], good[0]), (good, good.half()), (good, torch.zeros(1, 2, 4, 2, 16)),
-                         (good.int(), good.int()), (good, good[..., :0]), (good.expand(3, -1, -1, -1, -1), good.expand(3, -1, -1, -1, -1)),
+                         (good.int(), good.int()), (good, good[..., :0]), (good.clone().requires_grad_(True), good), (good.expand(3, -1, -1, -1, -1), good.expand(3, -1, -1, -1, -1)),
                          (torch.zeros(300).as_strided((1, 2, 4, 2, 8), (256, 128, 32, 16, 2)),) * 2,
                          (torch.zeros(300).as_strided((1, 2, 4, 2, 8), (128, 32, 16, 8, 1)),) * 2):
         with pytest.raises(ConfigurationError):
@@ -264,6 +269,21 @@ def test_rotary_refusals(monkeypatch):
     assert len(launches) == 2
 
 
+def test_pages_too_large_to_copy_are_refused_before_anything_changes(host, monkeypatch):
+    cache = make()
+    a = cache.new()
+    cache.extend([a], [5])
+    b = cache.fork(a)
+    monkeypatch.setattr(cache, "head_dim", 1 << 30)
+    with pytest.raises(UnsupportedError, match="2 GiB"):
+        cache.extend([b], [1])
+    cache.truncate(b, 4)
+    with pytest.raises(UnsupportedError, match="2 GiB"):
+        cache.load_tables([([7], 2)])
+        cache.compact()
+    assert cache.pages_of(0) == [7] and host == []
+
+
 def test_plan_refusals(host):
     cache = make()
     a = cache.new()
@@ -282,6 +302,8 @@ def test_plan_refusals(host):
     plan._check(cache.keys[0], cache.values[0])
     with pytest.raises(ConfigurationError):
         plan._check(cache.keys[0][:4], cache.values[0])
+    with pytest.raises(ConfigurationError, match="differentiable"):
+        cache.attend(0, torch.zeros(1, 2, 8, requires_grad=True), plan)
     cache.truncate(a, 2)
     with pytest.raises(StateError, match="after this plan"):
         cache.attend(0, torch.zeros(1, 2, 8), plan)
