@@ -102,10 +102,16 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A,
     }
 }
 
-// Joins the parts of rows whose keys were split (the same order whatever the timing).  Rows of many parts
-// (single tokens over long histories) take a workgroup each, whose waves share the parts; rows of few, a
-// thread per eight channels.
-constexpr int kMergeRows = 16, kFewParts = RCH_ATTEND_FEW_PARTS;
+// Joins the parts of rows whose keys were split (the same order whatever the timing).  Bound: the latency of
+// the partial results (other XCDs wrote them), so all or many of a row's loads are in flight at once.  Rows of
+// more than kFewParts parts (single tokens over long histories) take a workgroup each, whose waves share the
+// parts; rows of fewer a thread per eight channels.  Rows of 128 channels: 228 blocks of 128 rows in 3 and 7 parts
+// take 10.4 us so and 43 us with a workgroup each (29184 workgroups); 32 blocks of 4 rows in 11 or 16 parts 4.0 us
+// with a workgroup each and, with a thread per eight channels over groups of 8 parts, 5.8 and 7.4 us.
+// A workgroup has 16 waves where at most kWideRows rows are joined (8 rows in 159 parts: 7.2 us, with 4 waves
+// 14.9 us; 32 rows in 32 parts: 4.6, 5.0 us), else 4 (128 rows in 16 parts: 4.0 us, with 16 waves 4.4 us; 2048
+// rows in 16 parts: 6.5, 19.5 us).
+constexpr int kMergeRows = 16, kFewParts = RCH_ATTEND_FEW_PARTS, kWideRows = 64;
 
 struct MergedRow {
     int64_t out, lse;  // element offsets of the row's output and logarithm
@@ -115,22 +121,22 @@ __device__ __forceinline__ MergedRow merged_row(const rch_attend& A, int q_row, 
     return {(q_row + token) * A.out_token_stride + head * A.out_head_stride, (q_row + token) * A.heads + head};
 }
 
-template <int DT>
-__global__ void __launch_bounds__(256) attend_merge_many_kernel(const rch_attend A) {
+template <int DT, int C, int W>
+__global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_attend A) {
     typedef typename AttendType<DT>::type T;
-    constexpr int C = RCH_ATTEND_MAX_DIM / 64;
-    __shared__ float sums[4][RCH_ATTEND_MAX_DIM], stat[4][2];
+    constexpr int kAhead = 32 / C;  // parts in flight in a wave
+    __shared__ float sums[W][64 * C], stat[W][2];
     const RCH_GLOBAL int32_t* w = gin<int32_t>(A.plan_ptr) + A.merges + static_cast<int64_t>(blockIdx.x) * RCH_ATTEND_MERGE;
     const int rows = w[2], parts = w[5], dim = static_cast<int>(A.head_dim), r = blockIdx.y;
     if (r >= rows) return;
     const int64_t first = static_cast<int64_t>(w[4]) + r;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // A wave takes parts wave, wave + 4, ..: its own reference, sum and weighted sums.
+    // A wave takes parts wave, wave + W, ..: its own reference, sum and weighted sums.
     float reference = kNoReference, sum = 0.0f, acc[C];
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.0f;
-    for (int base = wave; base < parts; base += 256) {
-        const int part = base + 4 * lane;
+    for (int base = wave; base < parts; base += 64 * W) {
+        const int part = base + W * lane;
         f2 stats = {kNoReference, 0.0f};
         if (part < parts) stats = *gin<f2>(partial_stats(A, first + static_cast<int64_t>(part) * rows));
         float next = stats[1] != 0.0f ? stats[0] : kNoReference;
@@ -145,14 +151,23 @@ __global__ void __launch_bounds__(256) attend_merge_many_kernel(const rch_attend
         sum = __builtin_fmaf(sum, old, total);
 #pragma unroll
         for (int c = 0; c < C; ++c) acc[c] *= old;
-        const int count = min(64, (parts - base + 3) / 4);
-#pragma unroll 8
-        for (int p = 0; p < count; ++p) {
-            const float fade = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), p));
-            const RCH_GLOBAL float* from = gin<float>(partial_sums(A, first + static_cast<int64_t>(base + 4 * p) * rows));
+        const int count = min(64, (parts - base + W - 1) / W);
+        for (int p0 = 0; p0 < count; p0 += kAhead) {
+            float x[kAhead][C];
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (64 * c < dim) acc[c] = __builtin_fmaf(from[min(lane + 64 * c, dim - 1)], fade, acc[c]);
+            for (int i = 0; i < kAhead; ++i) {
+                const int p = min(p0 + i, count - 1);
+                const RCH_GLOBAL float* from = gin<float>(partial_sums(A, first + static_cast<int64_t>(base + W * p) * rows));
+#pragma unroll
+                for (int c = 0; c < C; ++c) x[i][c] = from[min(lane + 64 * c, dim - 1)];
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (p0 + i >= count) break;
+                const float fade = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), p0 + i));
+#pragma unroll
+                for (int c = 0; c < C; ++c) acc[c] = __builtin_fmaf(x[i][c], fade, acc[c]);
+            }
         }
     }
 #pragma unroll
@@ -166,12 +181,12 @@ __global__ void __launch_bounds__(256) attend_merge_many_kernel(const rch_attend
     const int d = threadIdx.x;
     reference = kNoReference;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < W; ++i)
         if (stat[i][1] != 0.0f) reference = fmaxf(reference, stat[i][0]);
     float value = 0.0f;
     sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W; ++i) {
         const float fade = stat[i][1] != 0.0f ? exp2_of(stat[i][0] - reference) : 0.0f;
         sum = __builtin_fmaf(stat[i][1], fade, sum);
         if (d < dim) value = __builtin_fmaf(sums[i][d], fade, value);
@@ -228,6 +243,14 @@ __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
     if (d == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[M.lse] = row_lse(reference, sum);
 }
 
+template <int DT, int C>
+int merge_many(const rch_attend& A, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(A.n_many), static_cast<uint32_t>(A.most_rows_many));
+    if (A.n_many * A.most_rows_many <= kWideRows) hipLaunchKernelGGL((attend_merge_many_kernel<DT, C, 16>), grid, dim3(1024), 0, stream, A);
+    else hipLaunchKernelGGL((attend_merge_many_kernel<DT, C, 4>), grid, dim3(256), 0, stream, A);
+    return check_launch("rch_attend_run (merge)");
+}
+
 template <int DT>
 int run(const rch_attend& A, hipStream_t stream) {
     int first = 0;
@@ -242,9 +265,7 @@ int run(const rch_attend& A, hipStream_t stream) {
         if (status != RCH_OK) return status;
     }
     if (A.n_many) {
-        const dim3 grid(static_cast<uint32_t>(A.n_many), static_cast<uint32_t>(A.most_rows_many));
-        hipLaunchKernelGGL(attend_merge_many_kernel<DT>, grid, dim3(256), 0, stream, A);
-        const int status = check_launch("rch_attend_run (merge)");
+        const int status = A.head_dim <= 128 ? merge_many<DT, 2>(A, stream) : merge_many<DT, 4>(A, stream);
         if (status != RCH_OK) return status;
     }
     if (A.n_merges > A.n_many) {

@@ -9,14 +9,17 @@
 // Bound: memory, one read and one write of each value.  A thread holds one 8-channel piece (two for
 // the "half" pairing) of a token and walks over heads of it, so the places, table rows and cosines
 // are fetched once for all of those heads; neighbouring threads hold neighbouring pieces, so a wave
-// reads and writes whole rows of a head.
+// reads and writes whole rows of a head.  Four heads to a thread, their loads in flight together: q and k
+// of 16 / 1024 / 4680 / 18720 tokens x 12 heads x 128 bf16 take 4.6 / 5.7 / 12.4 / 36.3 us (the last
+// 6.3 TB/s, mostly from the caches), with one head 4.5 / 6.6 / 18.0 / 57.3, two 4.5 / 5.8 / 13.8 / 38.6,
+// eight 4.4 / 5.9 / 12.2 / 36.5.
 #include "common.h"
 
 namespace rch {
 
 namespace {
 
-constexpr int kMaxRotary = 4;
+constexpr int kMaxRotary = 4, kHeads = 4;
 
 struct RotaryJobs {
     rch_rotary_job job[kMaxRotary];
@@ -89,10 +92,11 @@ __device__ __forceinline__ void rotate_pair(float& e, float& o, float c, float s
 // One piece is V channels: V / 2 interleaved pairs, or V pairs of the half pairing (channels j and
 // pairs + j: two pieces).  V = 8 and V = 4 need rows aligned to a piece (16 bytes at most) and widths of
 // whole pieces; V = 2 (interleaved) and 1 (half, or no rotation) take everything else.
-// A thread takes U heads, whose loads are in flight together.
-template <int DT, bool HALF, int V, int U>
+// A thread takes U heads.
+template <int DT, bool HALF, int V>
 __global__ void __launch_bounds__(256) rotary_kernel(RotaryJobs jobs) {
     typedef typename Element<DT>::type T;
+    constexpr int U = kHeads;
     const rch_rotary_job& J = jobs.job[blockIdx.z];
     const int pairs = static_cast<int>(J.pairs), dim = static_cast<int>(J.head_dim);
     // Work items of a token's head: pieces that turn, then pieces that are copied.
@@ -187,22 +191,16 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryJobs jobs) {
     }
 }
 
-template <int DT, bool HALF, int V>
-void launch_heads(const RotaryJobs& jobs, dim3 grid, int per_thread, hipStream_t stream) {
-    if (per_thread == 1) hipLaunchKernelGGL((rotary_kernel<DT, HALF, V, 1>), grid, dim3(256), 0, stream, jobs);
-    else hipLaunchKernelGGL((rotary_kernel<DT, HALF, V, 4>), grid, dim3(256), 0, stream, jobs);
-}
-
 template <int DT>
-void launch(const RotaryJobs& jobs, bool half, int width, dim3 grid, int per_thread, hipStream_t stream) {
+void launch(const RotaryJobs& jobs, bool half, int width, dim3 grid, hipStream_t stream) {
     if (half) {
-        if (width == 8) launch_heads<DT, true, 8>(jobs, grid, per_thread, stream);
-        else if (width == 4) launch_heads<DT, true, 4>(jobs, grid, per_thread, stream);
-        else launch_heads<DT, true, 1>(jobs, grid, per_thread, stream);
+        if (width == 8) hipLaunchKernelGGL((rotary_kernel<DT, true, 8>), grid, dim3(256), 0, stream, jobs);
+        else if (width == 4) hipLaunchKernelGGL((rotary_kernel<DT, true, 4>), grid, dim3(256), 0, stream, jobs);
+        else hipLaunchKernelGGL((rotary_kernel<DT, true, 1>), grid, dim3(256), 0, stream, jobs);
     } else {
-        if (width == 8) launch_heads<DT, false, 8>(jobs, grid, per_thread, stream);
-        else if (width == 4) launch_heads<DT, false, 4>(jobs, grid, per_thread, stream);
-        else launch_heads<DT, false, 2>(jobs, grid, per_thread, stream);
+        if (width == 8) hipLaunchKernelGGL((rotary_kernel<DT, false, 8>), grid, dim3(256), 0, stream, jobs);
+        else if (width == 4) hipLaunchKernelGGL((rotary_kernel<DT, false, 4>), grid, dim3(256), 0, stream, jobs);
+        else hipLaunchKernelGGL((rotary_kernel<DT, false, 2>), grid, dim3(256), 0, stream, jobs);
     }
 }
 
@@ -247,7 +245,7 @@ int rch_rotary(const rch_rotary_job* jobs_host, int n_jobs, int dtype, int pairi
     const int width = channels % 8 == 0 && mix % 16 == 0 ? 8
                       : channels % 4 == 0 && mix % (4 * size) == 0 ? 4 : half ? 1 : 2;
     if (width == 2 && channels % 2) return fail(RCH_E_UNSUPPORTED, "rch_rotary: interleaved pairs need an even head_dim");
-    int64_t units = 0, heads = 0, work = 0;
+    int64_t units = 0, heads = 0;
     for (int i = 0; i < n_jobs; ++i) {
         const rch_rotary_job& J = jobs.job[i];
         const int v = width;
@@ -255,20 +253,16 @@ int rch_rotary(const rch_rotary_job* jobs_host, int n_jobs, int dtype, int pairi
         const int64_t n = J.batch * J.tokens * pieces;
         units = n > units ? n : units;
         heads = J.heads > heads ? J.heads : heads;
-        work += n * J.heads;
     }
     if (units == 0) return RCH_OK;
-    // Heads per thread: one while the call has too few pieces to fill the card (256 CUs, 2048 threads
-    // each), four once it has.
-    const int per_thread = work >= 4 * 256 * 2048 / 2 ? 4 : 1;
-    const int64_t blocks = (units + 255) / 256, groups = (heads + per_thread - 1) / per_thread;
+    const int64_t blocks = (units + 255) / 256, groups = (heads + kHeads - 1) / kHeads;
     if (blocks > 0x7fffffff || groups > 65535) return fail(RCH_E_CONFIG, "rch_rotary: grid too large");
     const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(groups), static_cast<uint32_t>(n_jobs));
     hipStream_t s = as_stream(stream);
     switch (dtype) {
-        case RCH_DT_F32: launch<RCH_DT_F32>(jobs, half, width, grid, per_thread, s); break;
-        case RCH_DT_F16: launch<RCH_DT_F16>(jobs, half, width, grid, per_thread, s); break;
-        default: launch<RCH_DT_BF16>(jobs, half, width, grid, per_thread, s); break;
+        case RCH_DT_F32: launch<RCH_DT_F32>(jobs, half, width, grid, s); break;
+        case RCH_DT_F16: launch<RCH_DT_F16>(jobs, half, width, grid, s); break;
+        default: launch<RCH_DT_BF16>(jobs, half, width, grid, s); break;
     }
     return check_launch("rch_rotary");
 }

@@ -173,6 +173,16 @@ def test_long_histories_split(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [128, 72, 20, 200])
+@pytest.mark.parametrize("lengths,rows,least", [([20000], 8, 64), ([20000, 9000], 16, 9), ([2500] * 10, 80, 9)])
+def test_rows_of_many_parts(device, dtype, dim, lengths, rows, least):
+    """Few rows in very many parts, and more rows in several, of every head size."""
+    _, _, plan, _ = _run(device, lengths, [1] * len(lengths), 64, 1, 8, dim, dtype)
+    merges = plan.buffer[plan._merges:plan._merges + 8 * plan._n_merges].view(-1, 8)
+    assert merges[:, 2].sum() == rows and merges[:, 5].max() >= least
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", [128, 20])
 def test_strides_outputs_and_rows_behind(device, dtype, dim):
     lengths, queries = [90, 33], [60, 1]
