@@ -593,7 +593,7 @@ int rch_words_store(void* words_dev, const int32_t* words_host, int count, void*
 #define RCH_ATTEND_ZEROS 128
 #define RCH_ATTEND_FEW_PARTS 8
 #define RCH_ATTEND_MAX_DIM 256   /* head_dim of the general form */
-#define RCH_ATTEND_FAST_DIM 128  /* head_dim of the others: multiples of 8 up to this, 16-byte aligned rows */
+#define RCH_ATTEND_FAST_DIM 256  /* head_dim of the others: multiples of 8 up to this, 16-byte aligned rows */
 
 typedef struct rch_attend {
     int64_t q_ptr, k_ptr, v_ptr, out_ptr, lse_ptr; /* lse_ptr: fp32 [query rows, heads], or 0 */
@@ -609,7 +609,7 @@ typedef struct rch_attend {
     int64_t n_general, n_rows; /* items of the general and of the tiled form, in order */
     int64_t merges, n_merges;      /* word index and count */
     int64_t n_many;                /* the first ones: merges of more than RCH_ATTEND_FEW_PARTS parts, or of rows
-                                      that are no aligned multiples of eight channels up to 128 */
+                                      that are no aligned multiples of eight channels */
     int64_t most_rows_many, most_rows; /* most rows of one of those, and of one of the others */
     int64_t holes;           /* 1: page tables may hold holes */
     int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64 */

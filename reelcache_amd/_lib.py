@@ -80,7 +80,7 @@ ATTEND_FIELDS = ("q_ptr", "k_ptr", "v_ptr", "out_ptr", "lse_ptr", "plan_ptr", "p
                  "v_head_stride", "out_token_stride", "out_head_stride", "group", "heads", "head_dim", "page_tokens",
                  "pages", "block", "window", "scale_bits", "partial_rows", "items", "n_general", "n_rows",
                  "merges", "n_merges", "n_many", "most_rows_many", "most_rows", "holes", "tile_unit")
-ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 128
+ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 256
 ATTEND_FEW_PARTS = 8
 PAIRS_INTERLEAVED, PAIRS_HALF = 0, 1
 

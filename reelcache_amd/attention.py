@@ -31,10 +31,9 @@ from .rotary import _DTYPE_CODES, _span, entered, known_calls, need_gpu, raw_str
 KEY_TILE = 64
 #: Query rows (tokens x heads of a key head) of one workgroup's tile, per form.
 GENERAL_ROWS, ROW_TILE = 16, 128
-# Workgroups resident on the card at once, per form (256 CUs), and what a workgroup's start, end and
-# partial results cost in key tiles.
-_RESIDENT = {"general": 1024, "rows": 512}
+# What a workgroup's start, end and partial results cost in key tiles, per form.
 _OVERHEAD = {"general": 1, "rows": 3}
+_CUS = 256
 _XCDS = 8
 
 
@@ -132,7 +131,7 @@ class AttentionPlan:
 
     def _lay_out(self, found, queries):
         cache = self.cache
-        work = {name: _Work() for name in _RESIDENT}
+        work = {name: _Work() for name in _OVERHEAD}
         tiles = {"general": GENERAL_ROWS, "rows": ROW_TILE}
         table, at, lengths, starts = [], [], [], []
         words, row = _lib.ATTEND_ZEROS, 0
@@ -161,7 +160,7 @@ class AttentionPlan:
         first_item = _lib.ATTEND_ZEROS + len(table)
         self._items, self._merges = first_item, first_item + items.size
         # Merges that take a workgroup to a row come first (the kernels' rule).
-        joined = counts["general"] == 0 and cache.head_dim % 8 == 0 and cache.head_dim <= 128
+        joined = counts["general"] == 0 and cache.head_dim % 8 == 0
         many = (merges[:, 5] > _lib.ATTEND_FEW_PARTS) | (not joined)
         merges = np.concatenate([merges[many], merges[~many]])
         self._n_merges, self._n_many = len(merges), int(many.sum())
@@ -188,6 +187,13 @@ class AttentionPlan:
         held = -(-size // KEY_TILE) * KEY_TILE  # rows of tiles that a page takes
         return size if held == size or (size % share and 5 * held <= 6 * size) else KEY_TILE
 
+    def _resident(self, form):
+        """Workgroups of a form that the card holds at once."""
+        if form == "general":
+            return _CUS * 4
+        dim = self.cache.head_dim  # its tiles fill LDS and registers
+        return _CUS * (3 if dim <= 64 else 2 if dim <= 128 else 1)
+
     def _tile_of(self, key):
         """Index of the tile that holds ``key``, and the first key of a tile."""
         unit = self._unit()
@@ -207,7 +213,7 @@ class AttentionPlan:
         tile0 = self._tile_of(first)
         tiles = np.where(last > first, self._tile_of(np.maximum(last - 1, 0)) + 1 - tile0, 0)
         owner = sequence * self.cache.heads + head
-        which, low, high, xcd = _share_out(tiles, owner, _RESIDENT[form], _OVERHEAD[form]).T
+        which, low, high, xcd = _share_out(tiles, owner, self._resident(form), _OVERHEAD[form]).T
         parts = np.bincount(which, minlength=len(blocks))
         part = np.arange(len(which)) - np.repeat(np.cumsum(parts) - parts, parts)
         n = parts[which]

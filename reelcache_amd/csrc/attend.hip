@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A,
 // A workgroup has 16 waves where at most kWideRows rows are joined (8 rows in 159 parts: 7.2 us, with 4 waves
 // 14.9 us; 32 rows in 32 parts: 4.6, 5.0 us), else 4 (128 rows in 16 parts: 4.0 us, with 16 waves 4.4 us; 2048
 // rows in 16 parts: 6.5, 19.5 us).
-constexpr int kMergeRows = 16, kFewParts = RCH_ATTEND_FEW_PARTS, kWideRows = 64;
+constexpr int kFewParts = RCH_ATTEND_FEW_PARTS, kWideRows = 64;
 
 struct MergedRow {
     int64_t out, lse;  // element offsets of the row's output and logarithm
@@ -196,14 +196,15 @@ __global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_att
     if (d == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[M.lse] = row_lse(reference, sum);
 }
 
-template <int DT>
+// TPR: threads of a row (8 channels each).
+template <int DT, int TPR>
 __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
     typedef typename AttendType<DT>::type T;
     const RCH_GLOBAL int32_t* w = gin<int32_t>(A.plan_ptr) + A.merges
                                   + (static_cast<int64_t>(blockIdx.x) + A.n_many) * RCH_ATTEND_MERGE;
     const int rows = w[2], parts = w[5], dim = static_cast<int>(A.head_dim);
     const int64_t first = w[4];
-    const int r = blockIdx.y * kMergeRows + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+    const int r = blockIdx.y * (256 / TPR) + threadIdx.x / TPR, d = threadIdx.x % TPR * 8;
     if (r >= rows || d >= dim) return;
     const MergedRow M = merged_row(A, w[0], w[1] + r, w[3]);
     f2 stats[kFewParts];
@@ -251,6 +252,13 @@ int merge_many(const rch_attend& A, hipStream_t stream) {
     return check_launch("rch_attend_run (merge)");
 }
 
+template <int DT, int TPR>
+int merge_few(const rch_attend& A, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(A.n_merges - A.n_many), static_cast<uint32_t>((A.most_rows * TPR + 255) / 256));
+    hipLaunchKernelGGL((attend_merge_kernel<DT, TPR>), grid, dim3(256), 0, stream, A);
+    return check_launch("rch_attend_run (merge)");
+}
+
 template <int DT>
 int run(const rch_attend& A, hipStream_t stream) {
     int first = 0;
@@ -268,11 +276,7 @@ int run(const rch_attend& A, hipStream_t stream) {
         const int status = A.head_dim <= 128 ? merge_many<DT, 2>(A, stream) : merge_many<DT, 4>(A, stream);
         if (status != RCH_OK) return status;
     }
-    if (A.n_merges > A.n_many) {
-        const dim3 grid(static_cast<uint32_t>(A.n_merges - A.n_many), static_cast<uint32_t>((A.most_rows + kMergeRows - 1) / kMergeRows));
-        hipLaunchKernelGGL(attend_merge_kernel<DT>, grid, dim3(256), 0, stream, A);
-        return check_launch("rch_attend_run (merge)");
-    }
+    if (A.n_merges > A.n_many) return A.head_dim <= 128 ? merge_few<DT, 16>(A, stream) : merge_few<DT, 32>(A, stream);
     return RCH_OK;
 }
 
@@ -297,9 +301,9 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
                        || A.most_rows_many > 65535))
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid merges");
     // Rows of few parts are joined in aligned pieces of eight channels.
-    if (A.n_merges > A.n_many && (A.head_dim % 8 || A.head_dim > 128 || A.out_ptr % 16
+    if (A.n_merges > A.n_many && (A.head_dim % 8 || A.out_ptr % 16
                                   || (A.out_token_stride | A.out_head_stride) * (dtype == RCH_DT_F32 ? 4 : 2) % 16))
-        return fail(RCH_E_CONFIG, "rch_attend_run: merges of few parts need aligned rows of 8n <= 128 channels");
+        return fail(RCH_E_CONFIG, "rch_attend_run: merges of few parts need aligned rows of 8n channels");
     if (A.n_general + A.n_rows == 0) return RCH_OK;
     if (!A.q_ptr || !A.k_ptr || !A.v_ptr || !A.out_ptr || !A.plan_ptr) return fail(RCH_E_CONFIG, "rch_attend_run: null address");
     if (A.n_rows) {

@@ -3,7 +3,8 @@
 //
 // Bound: the matrix cores (4 * D operations for every row and key) with the exponentials beside them.
 // A tile of 64 (fp32: 32) keys and values is fetched into one half of LDS while the waves work on the other half;
-// one barrier to a tile.  Two workgroups fit a CU, so one's products cover the other's softmax.
+// one barrier to a tile.  Two workgroups (heads of up to 64 channels: three, of more than 128: one) fill a CU's
+// registers and LDS, so one's products cover the other's softmax.
 #include "attend_tile.h"
 
 namespace rch {
@@ -11,7 +12,7 @@ namespace rch {
 namespace {
 
 template <int DT, int NB, int MODE>
-__global__ void __launch_bounds__(256, 2) attend_rows_kernel(const rch_attend A, int first_item) {
+__global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_rows_kernel(const rch_attend A, int first_item) {
     typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2> Tile;
     constexpr int KT = Tile::KT, ES = Tile::ES, kTileBytes = KT * Tile::RB;
     constexpr int kStageBytes = 2 * kTileBytes;
@@ -135,7 +136,9 @@ template <int DT>
 void launch_dim(const rch_attend& A, int first, hipStream_t stream) {
     if (A.head_dim <= 64) launch<DT, 2>(A, first, stream);
     else if (A.head_dim <= 96) launch<DT, 3>(A, first, stream);
-    else launch<DT, 4>(A, first, stream);
+    else if (A.head_dim <= 128) launch<DT, 4>(A, first, stream);
+    else if (A.head_dim <= 192) launch<DT, 6>(A, first, stream);
+    else launch<DT, 8>(A, first, stream);
 }
 
 }  // namespace

@@ -325,14 +325,18 @@ struct RowTile {
     typedef typename H::type T;
     typedef typename H::vec8 vec8;
     typedef typename H::vec4 vec4;
-    static constexpr int ES = 2, RB = NB <= 2 ? 128 : 256, kPieces = RB / 16, KT = 32 * KB;
+    static constexpr int ES = 2, RB = NB <= 2 ? 128 : NB <= 4 ? 256 : 512, kPieces = RB / 16, KT = 32 * KB;
     static __device__ __forceinline__ int k_swizzle(int row) { return row % kPieces; }
-    static __device__ __forceinline__ int v_swizzle(int row) { return kPieces == 16 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
+    static __device__ __forceinline__ int v_swizzle(int row) { return kPieces >= 16 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
 
     vec8 q[2 * NB];
     f16v o[NB];
     float reference, sum;
-    uint32_t k_lane[2 * NB], v_lane[NB];  // LDS byte offsets within a tile
+    // LDS byte offsets within a tile; of wide heads the first, from which the others follow by an exclusive or.
+    static constexpr bool kWide = NB > 4;
+    uint32_t k_lane[kWide ? 1 : 2 * NB], v_lane[kWide ? 1 : NB];
+    __device__ __forceinline__ uint32_t k_at(int s) const { return kWide ? k_lane[0] ^ (s * 32) : k_lane[s]; }
+    __device__ __forceinline__ uint32_t v_at(int b) const { return kWide ? v_lane[0] ^ (b * 64) : v_lane[b]; }
 
     __device__ __forceinline__ void init(const rch_attend& A, const AttendItem& I, const QueryRow& R, int lane) {
         const int n = lane & 31, h = lane >> 5;
@@ -341,11 +345,11 @@ struct RowTile {
         for (int s = 0; s < 2 * NB; ++s) {
             const int d = 16 * s + 8 * h;
             q[s] = __builtin_bit_cast(vec8, *gin<u4>(R.valid && d < A.head_dim ? at + 2 * d : A.plan_ptr));  // or zeros
-            k_lane[s] = n * RB + (((2 * s + h) ^ k_swizzle(n)) * 16);
+            if (!kWide || s == 0) k_lane[s] = n * RB + (((2 * s + h) ^ k_swizzle(n)) * 16);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            v_lane[b] = value_offset(b, lane);
+            if (!kWide || b == 0) v_lane[b] = value_offset(b, lane);
             o[b] = f16v{};
         }
         reference = kNoReference;
@@ -367,7 +371,7 @@ struct RowTile {
         for (int c = 0; c < 2 * NB; ++c)
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                const vec8 k = *reinterpret_cast<const __attribute__((address_space(3))) vec8*>(k_tile + k_lane[c] + b * 32 * RB);
+                const vec8 k = *reinterpret_cast<const __attribute__((address_space(3))) vec8*>(k_tile + k_at(c) + b * 32 * RB);
                 s[b] = H::mfma(k, q[c], s[b]);
             }
         constexpr int kAhead = 6, kProducts = 2 * NB * KB;
@@ -386,10 +390,11 @@ struct RowTile {
                 for (int i = 0; i < 16; ++i) s[b][i] = seen[b] >> i & 1u ? s[b][i] : -INFINITY;
         }
         // The first values, on their way while the weights are computed.
-        vec8 v[NB];
+        constexpr int kRing = kWide ? 4 : NB;  // values read ahead
+        vec8 v[kRing];
         if constexpr (!RARE) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) v[b] = values(v_tile + v_lane[b], 0);
+            for (int b = 0; b < kRing; ++b) v[b] = values(v_tile + v_at(b), 0);
         }
         float top = s[0][0];
 #pragma unroll
@@ -435,8 +440,9 @@ struct RowTile {
         for (int c = 0; c < 2 * KB; ++c)
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
-                const vec8 now = RARE ? values(v_tile + v_lane[b], c) : v[b];
-                if (!RARE && c + 1 < 2 * KB) v[b] = values(v_tile + v_lane[b], c + 1);
+                const int at = c * NB + b, next = at + kRing;
+                const vec8 now = RARE ? values(v_tile + v_at(b), c) : v[at % kRing];
+                if (!RARE && next < 2 * KB * NB) v[at % kRing] = values(v_tile + v_at(next % NB), next / NB);
                 o[b] = H::mfma(now, p[c], o[b]);
             }
     }
@@ -520,7 +526,7 @@ struct RowTile {
 template <int NB>
 struct RowTile<RCH_DT_F32, NB, 1> {
     typedef float T;
-    static constexpr int ES = 4, RB = NB <= 2 ? 256 : 512, kPieces = RB / 16, KT = 32;
+    static constexpr int ES = 4, RB = NB <= 2 ? 256 : NB <= 4 ? 512 : 1024, kPieces = RB / 16, KT = 32;
     static __device__ __forceinline__ int k_swizzle(int row) { return row % kPieces; }
     // The two halves read keys 4 apart at the same channels: half a 256-byte bank row apart.
     static __device__ __forceinline__ int v_swizzle(int row) { return ((row >> 2) & 1) * 8; }

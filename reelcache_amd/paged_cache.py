@@ -58,11 +58,13 @@ class _Sequence:
         self.pages, self.tokens = pages, tokens
 
 
-# Tables of at most this many words travel in launch arguments: two launches and no pinned memory, where a
-# copy costs about four launches on the host.
-_ARGUMENT_WORDS = 1920
-# Slots of so few tokens are listed one by one (the array form has a fixed cost of about sixty of them).
-_FEW_TOKENS = 64
+# Tables of at most this many words travel in the arguments of one launch: 64 words take 6.5 us of the host
+# so and 9.8 us through pinned memory, 960 words 7.7 and 10.0 us; at 1920 (two launches) it is 11.9 and 10.3 us.
+_ARGUMENT_WORDS = 960
+# Slots of at most this many tokens are listed one by one, more by array operations: slots of one token take
+# 9.7 and 15.7 us of the host, of 128 tokens 15.3 and 15.9 us, of 256 tokens 21.4 and 17.2 us; of one token of
+# each of 128 sequences 73 and 85 us.
+_FEW_TOKENS = 128
 
 
 def upload(values, device):

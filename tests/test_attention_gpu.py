@@ -183,6 +183,38 @@ def test_rows_of_many_parts(device, dtype, dim, lengths, rows, least):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("block", [None, 1])
+@pytest.mark.parametrize("size,kv_heads,group,dim,layout", [
+    (64, 1, 1, 256, "BTHD"), (16, 2, 2, 192, "BHTD"), (7, 1, 1, 136, "BTHD"), (100, 1, 3, 200, "BTHD"), (9, 1, 1, 248, "BTHD"),
+    (16, 1, 1, 252, "BTHD"), (64, 1, 2, 250, "BTHD"),
+])
+def test_wide_heads(device, dtype, block, size, kv_heads, group, dim, layout):
+    """Heads of more than 128 channels: single tokens, chunks, and histories in several parts."""
+    _run(device, [70, 133, 260, 90, 1500, 1], [70, 129, 75, 1, 33, 1], size, kv_heads, group, dim, dtype, layout, block=block)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size", [(256, 16), (192, 64), (160, 100)])
+def test_hidden_rows_of_wide_heads_may_hold_anything(device, dtype, dim, size):
+    """Infinite and NaN values behind a mask, in a dropped page and behind the last token."""
+    lengths, queries = [5 * size + 3], [2 * size]
+    cache = _cache(device, lengths, size, 1, dim, dtype)
+    pages = cache.pages_of(0)
+    q = torch.randn((2 * size, 2, dim), generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
+    cache.drop(0, 1, 1)
+    for pool in (cache.keys, cache.values):
+        pool[:, pages[1]] = math.inf
+        pool[:, pages[5], 1] = -math.inf  # a token that only the last rows see under the causal mask
+        pool[:, pages[5], 2] = math.nan   # and one that only the last row sees
+    plan = cache.plan([0], queries, heads=2, block=1)
+    out = cache.attend(0, q, plan)
+    want, bound, _, _ = oracle.attend(q[:-2], cache.keys[0], cache.values[0], cache.pages_of(0), lengths[0] - 2,
+                                      queries[0] - 2, size, block=1)
+    assert oracle.worst(out[:-2], want, bound) <= 0
+    assert torch.isnan(out[-1]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", [128, 20])
 def test_strides_outputs_and_rows_behind(device, dtype, dim):
     lengths, queries = [90, 33], [60, 1]
