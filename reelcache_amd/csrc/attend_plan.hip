@@ -14,7 +14,10 @@ namespace rch {
 namespace {
 
 constexpr int kXcds = 8;
-// Fewest key tiles of a part, and about the most parts of an item within an XCD.
+// Fewest key tiles of a part (of 64 keys), and about the most parts of an item within an XCD.  Single tokens of 8
+// short sequences (37 to 1000 tokens) take 13.1 / 14.3 / 21.5 us with parts of at least 2 / 3 / 4 tiles, of 16
+// sequences of 2000 tokens 23.9 / 19.8 us with 2 / 3; of 2 of 16000 tokens 31.7 us with up to 64 parts, 23.1 with 32
+// (their merge grows).
 constexpr int64_t kShortestPart = 3, kMostParts = 32;
 
 struct Piece {

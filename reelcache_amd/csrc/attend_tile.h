@@ -1,4 +1,4 @@
-// Tiles of keys and values for the attention forms on the matrix cores (16-bit types).
+// Tiles of keys and values for the attention on the matrix cores.
 //
 // A wave works on 32 query rows, as the columns of the products:
 //   S^T [32 keys x 32 rows] = K [keys x D] Q^T    (v_mfma_f32_32x32x16: A = K from LDS, B = Q in registers)
@@ -366,7 +366,7 @@ struct RowTile {
         f16v s[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b) s[b] = f16v{};
-        // The blocks' chains side by side, the reads kAhead products ahead.
+        // The blocks' chains side by side, the reads kAhead products ahead (2, 4 or 6: the same within 1 %).
 #pragma unroll
         for (int c = 0; c < 2 * NB; ++c)
 #pragma unroll

