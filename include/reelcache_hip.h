@@ -603,7 +603,7 @@ typedef struct rch_attend {
     int64_t v_page_stride, v_token_stride, v_head_stride;
     int64_t out_token_stride, out_head_stride;
     int64_t group, heads, head_dim, page_tokens, pages, block, window;
-    int64_t scale_bits;      /* fp32 bits of scale * log2(e); scale > 0 */
+    int64_t scale_bits;      /* fp32 bits of scale * log2(e), a positive normal number */
     int64_t partial_rows;
     int64_t items;           /* word index of the first item */
     int64_t n_general, n_rows; /* items of the general and of the tiled form, in order */

@@ -37,6 +37,13 @@ def strided(value: Any, name: str) -> torch.Tensor:
     return value
 
 
+def in_memory(value: Any, name: str) -> torch.Tensor:
+    """A strided tensor whose storage holds its values (no negation that is still to be done)."""
+    if strided(value, name).is_neg():
+        raise ConfigurationError(f"{name} has a negation pending; resolve_neg() it")
+    return value
+
+
 def matrix(value: Any, name: str, dtypes: tuple, what: str) -> torch.Tensor:
     """A strided 2-D tensor of one of ``dtypes``; ``what`` describes the accepted form."""
     value = strided(value, name)

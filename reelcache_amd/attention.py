@@ -23,9 +23,9 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._checks import count, need, strided
+from ._checks import count, in_memory, need
 from .errors import ConfigurationError, StateError, UnsupportedError
-from .rotary import _DTYPE_CODES, _span, entered, known_calls, need_gpu, raw_stream
+from .rotary import _DTYPE_CODES, _span, changed, entered, known_calls, need_gpu, raw_stream
 
 #: Keys of a tile: the step of every split of a sequence's keys.
 KEY_TILE = 64
@@ -36,6 +36,8 @@ GENERAL_ROWS, ROW_TILE = 16, 128
 _OVERHEAD = {"general": 1, "rows": 6}
 _CUS = 256
 _XCDS = 8
+# Scales that stay normal fp32 numbers with log2(e) in them.
+_LEAST_SCALE, _MOST_SCALE = 2.0 ** -126, 2.0 ** 127
 
 
 class _Work:
@@ -90,8 +92,8 @@ class AttentionPlan:
         for value, name in ((block, "block"), (window, "window")):
             need(value is None or count(value, name, minimum=1) < 1 << 31, f"{name} must be below 2**31")
         scale = cache.head_dim ** -0.5 if scale is None else scale
-        need(isinstance(scale, (int, float)) and not isinstance(scale, bool) and math.isfinite(scale) and scale > 0,
-             "scale must be a positive number")
+        need(isinstance(scale, (int, float)) and not isinstance(scale, bool) and _LEAST_SCALE <= scale <= _MOST_SCALE,
+             "scale must be a positive number that fp32 holds")
         if cache.head_dim > _lib.ATTEND_MAX_DIM:
             raise UnsupportedError(f"attention takes at most {_lib.ATTEND_MAX_DIM} channels to a head")
         need_gpu(cache.device, "attention")
@@ -260,7 +262,7 @@ class AttentionPlan:
         cache = self.cache
         shape, k_stride, v_stride = cache.keys.shape[1:], cache.keys.stride()[1:], cache.values.stride()[1:]
         for pool, stride, name in ((keys, k_stride, "keys"), (values, v_stride, "values")):
-            strided(pool, name)
+            in_memory(pool, name)
             need(pool.shape == shape and pool.stride() == stride and pool.dtype == cache.dtype
                  and pool.device == cache.device, f"{name} must be a layer's pool like those of the plan's cache")
             need(self._tiled == 0 or pool.data_ptr() % 16 == 0, f"{name} must be aligned as the plan's cache is")
@@ -303,7 +305,7 @@ def run(q, k_address, v_address, plan, out, return_lse, pools=None):
     cache = plan.cache
     if plan._stamp != cache._moved:
         raise StateError("pages moved or were freed after this plan was built")
-    strided(q, "q")
+    in_memory(q, "q")
     shape = q.shape
     if len(shape) != 3 or shape[0] < plan.queries or shape[1] != plan.heads or shape[2] != cache.head_dim:
         raise ConfigurationError("q must be [rows, heads, head_dim] with a row for every query of the plan")
@@ -314,7 +316,7 @@ def run(q, k_address, v_address, plan, out, return_lse, pools=None):
         raise ConfigurationError("attention over a cache is not differentiable; run it under torch.no_grad()")
     with entered(device):
         given, q = q, _rows(q)
-        more = shape[0] > plan.queries
+        more, given_out = shape[0] > plan.queries, out is not None
         result = out
         if out is None:
             result = out = torch.empty(shape, dtype=q.dtype, device=device)
@@ -346,12 +348,14 @@ def run(q, k_address, v_address, plan, out, return_lse, pools=None):
             _lib.check(_lib.function("rch_attend_run")(fields, _DTYPE_CODES[q.dtype], stream))
             if result is not out:
                 out[:plan.queries].copy_(result[:plan.queries])
+            elif given_out:
+                changed(out)
     return (out, lse) if return_lse else out
 
 
 def _output(out, q, pools):
     """Where the kernels write for a given ``out``: itself, or a buffer when its rows are not aligned."""
-    strided(out, "out")
+    in_memory(out, "out")
     need(out.shape == q.shape and out.dtype == q.dtype and out.device == q.device, "out must match q")
     need(not out.requires_grad, "out must not require gradients")
     need(all(stride != 0 or size <= 1 for size, stride in zip(out.shape, out.stride())),

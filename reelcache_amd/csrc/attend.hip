@@ -307,6 +307,8 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
                                   || (A.out_token_stride | A.out_head_stride) * (dtype == RCH_DT_F32 ? 4 : 2) % 16))
         return fail(RCH_E_CONFIG, "rch_attend_run: merges of few parts need aligned rows of 8n channels");
     if (A.n_general + A.n_rows == 0) return RCH_OK;
+    const uint32_t scale = static_cast<uint32_t>(A.scale_bits);
+    if (scale < 0x00800000u || scale >= 0x7f800000u) return fail(RCH_E_CONFIG, "rch_attend_run: scale must be a positive normal number");
     if (!A.q_ptr || !A.k_ptr || !A.v_ptr || !A.out_ptr || !A.plan_ptr) return fail(RCH_E_CONFIG, "rch_attend_run: null address");
     if (A.n_rows) {
         // The tiled forms: whole 16-byte pieces, a tile's rows within 2 GiB, tiles that start over at a page of

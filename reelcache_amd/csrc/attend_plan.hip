@@ -1,9 +1,9 @@
 // Host side of an attention plan: the cut of its row blocks into parts for the card's workgroups.  No device
 // code; a step's plan is made once per step and has to cost less than a layer's launches.
 #include <algorithm>
+#include <exception>
 #include <functional>
 #include <map>
-#include <new>
 #include <queue>
 #include <vector>
 
@@ -186,8 +186,8 @@ int rch_attend_share(const int64_t* tiles, const int64_t* owner, int64_t n, int6
         if (tiles[i] < 0 || tiles[i] > (int64_t{1} << 31)) return fail(RCH_E_CONFIG, "rch_attend_share: invalid tile count");
     try {
         return share_out(tiles, owner, n, resident, overhead, parts, capacity, count);
-    } catch (const std::bad_alloc&) {
-        return fail(RCH_E_LAUNCH, "rch_attend_share: out of host memory");
+    } catch (const std::exception& e) {
+        return fail(RCH_E_LAUNCH, "rch_attend_share: %s", e.what());
     }
 }
 

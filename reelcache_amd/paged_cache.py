@@ -28,7 +28,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._checks import count, need, one_of, strided
+from ._checks import count, in_memory, need, one_of
 from .errors import CapacityError, ConfigurationError, StateError, UnsupportedError
 from .restore_model import OUTPUT_DTYPES, NativeView
 from .rotary import Launch, addresses_of, capturing, entered, known_calls, need_gpu, position_fields, raw_stream
@@ -73,20 +73,22 @@ def upload(values, device):
     values = np.ascontiguousarray(values, dtype=np.int32)
     if values.size <= _ARGUMENT_WORDS:
         return upload_words(values.tobytes(), values.shape, device)
-    _refuse_capture()
+    _refuse_capture(device)
     return torch.from_numpy(values).pin_memory().to(device, non_blocking=True)
 
 
 def upload_words(words, shape, device):
     """The same of a small table that the caller packed into bytes."""
-    _refuse_capture()
+    _refuse_capture(device)
     out = torch.empty(shape, dtype=torch.int32, device=device)
     _lib.check(_lib.function("rch_words_store")(out.data_ptr(), words, len(words) // 4, raw_stream(device)))
     return out
 
 
-def _refuse_capture():
-    if capturing():
+def _refuse_capture(device):
+    with entered(device):
+        captured = capturing()
+    if captured:
         raise ConfigurationError("page tables, slots and plans are built before a HIP-graph capture, not in it")
 
 
@@ -104,7 +106,7 @@ class PagedCache:
     def __init__(self, keys, values, *, layout="BTHD"):
         one_of(layout, _LAYOUTS, "pool layout")
         for pool, name in ((keys, "keys"), (values, "values")):
-            strided(pool, name)
+            in_memory(pool, name)
             need(pool.ndim == 5, f"{name} must be [layers, pages, ...] pools of five dimensions")
             need(pool.dtype in OUTPUT_DTYPES, f"{name} must be bfloat16, float16 or float32")
             need(min(pool.shape) >= 1, f"{name} must not be empty")
@@ -232,7 +234,7 @@ class PagedCache:
         for n in counts:
             count(n, "a token count")
         need_gpu(self.device, "a paged cache")
-        _refuse_capture()
+        _refuse_capture(self.device)
         size, in_use, shared = self.page_tokens, self._uses, {}
         wanted, total, most = [], 0, 0  # (rows of a begun page to copy, or 0; new pages) of each sequence
         for item, n in zip(found, counts):
@@ -332,11 +334,12 @@ class PagedCache:
         if not moves:
             return
         with entered(self.device):
-            if self._copies is None:
-                self._copies = [_pools(pool, self._axes, self.pages, self.page_tokens)
-                                for pool in self._joined_pools()]
+            where = self.keys.data_ptr(), self.values.data_ptr()
+            if self._copies is None or self._copies[0] != where:  # a copied cache has pools of its own
+                self._copies = where, [_pools(pool, self._axes, self.pages, self.page_tokens)
+                                       for pool in self._joined_pools()]
             table, stream = _pack(moves), raw_stream(self.device)
-            for pools, fields, streams in self._copies:
+            for pools, fields, streams in self._copies[1]:
                 if stream not in streams:  # the allocator learns of a stream that the table was not made on
                     pools.record_stream(torch.cuda.current_stream(self.device))
                     streams.add(stream)
@@ -376,7 +379,7 @@ class PagedCache:
         if not source:
             return []
         need_gpu(self.device, "a paged cache")
-        _refuse_capture()
+        _refuse_capture(self.device)
         self._need_copies()
         moves, size, uses, names = [], self.page_tokens, self._uses, {}
         for a, b in zip(source, target):
@@ -472,7 +475,7 @@ class PagedCache:
             raise StateError("pages moved, were freed or became shared after these slots were built")
         shape = (slots.tokens, self.heads, self.head_dim)
         for x, name in ((keys, "keys"), (values, "values")):
-            strided(x, name)
+            in_memory(x, name)
             if x.shape != shape or x.dtype != self.dtype or x.device != self.device:
                 raise ConfigurationError(f"{name} must be [tokens, heads, head_dim] of the cache's dtype and device")
             if x.requires_grad and torch.is_grad_enabled():

@@ -25,7 +25,7 @@ from typing import Any
 import torch
 
 from . import _lib
-from ._checks import count, need, one_of, strided
+from ._checks import count, in_memory, need, one_of, strided
 from .errors import ConfigurationError, UnsupportedError
 from .restore_model import _AXES, LAYOUTS, OUTPUT_DTYPES, RopePositions, RopeTable
 
@@ -200,11 +200,17 @@ def _geometry(x, layout):
 
 
 def _check(x, layout, name):
-    strided(x, name)
+    in_memory(x, name)
     if x.ndim != (3 if layout == "THD" else 4):
         raise ConfigurationError(f"{name}: {layout} has the wrong number of dimensions")
     if x.dtype not in OUTPUT_DTYPES:
         raise ConfigurationError(f"{name} must be bfloat16, float16 or float32")
+
+
+def changed(x):
+    """Tells autograd that a kernel has written into a caller's tensor."""
+    if not x.is_inference():
+        torch.autograd.graph.increment_version(x)
 
 
 def _span(x):
@@ -273,6 +279,8 @@ def _rotate_into(tensors, outs, positions, grid, layout, pairing, inverse):
         for out, target in zip(outs, targets):
             if target is not out:
                 out.copy_(target)
+            else:
+                changed(out)
 
 
 class _Rotation(torch.autograd.Function):
@@ -315,8 +323,8 @@ def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interl
     (``"half"``).  ``inverse`` turns back.  ``out``: a tensor (or a tuple) of the same shapes to write
     into, which may be the input itself; without it the outputs are new tensors.
 
-    Runs on the current stream of the tensors' device.  Differentiable in the tensors (not with
-    ``out``).  Returns a tensor, or a tuple for a tuple.
+    Runs on the current stream of the tensors' device.  Differentiable in the tensors (in
+    reverse mode; not with ``out``).  Returns a tensor, or a tuple for a tuple.
     """
     single = isinstance(tensors, torch.Tensor)
     tensors = (tensors,) if single else tuple(tensors)

@@ -388,6 +388,33 @@ def test_parts_cover_their_blocks_and_share_the_work(seed):
         assert max(loads) <= 1.1 * least + 2 * (overhead + 6)
 
 
+@pytest.mark.parametrize("scale", [1e-46, 2.0 ** -127, 1e39, 10 ** 400, -1.0, float("inf"), True, "1"])
+def test_scales_that_fp32_does_not_hold_are_refused(host, scale):
+    cache = make()
+    a = cache.new()
+    cache.extend([a], [1])
+    with pytest.raises(ConfigurationError, match="scale"):
+        cache.plan([a], [1], heads=2, scale=scale)
+    cache.plan([a], [1], heads=2, scale=2.0 ** -126)
+
+
+def test_pending_negations_are_refused(host, monkeypatch):
+    """The imaginary part of a conjugate holds its values negated."""
+    monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
+    negated = torch.randn(1, 2, 8, dtype=torch.complex64).conj().imag
+    assert negated.is_neg()
+    cache = make()
+    a = cache.new()
+    slots = cache.extend([a], [1])
+    cos, sin, sections = oracle.tables(8, 4)
+    plan = cache.plan([a], [1], heads=2)
+    for call in (lambda: rotary.rotate(negated, rk.RopePositions(rk.RopeTable(cos, sin, sections), 0), grid=(1, 1, 1), layout="THD"),
+                 lambda: cache.store(0, slots, negated, torch.zeros(1, 2, 8)), lambda: cache.attend(0, negated, plan),
+                 lambda: paged_cache.PagedCache(negated[None, None], torch.zeros(1, 1, 1, 2, 8))):
+        with pytest.raises(ConfigurationError, match="negation"):
+            call()
+
+
 def test_header_matches_the_binding():
     text = re.sub(r"/\*.*?\*/", "", HEADER.read_text(), flags=re.S)
     for struct, fields in (("rch_rotary_job", _lib.ROTARY_FIELDS), ("rch_pages", _lib.PAGES_FIELDS), ("rch_attend", _lib.ATTEND_FIELDS)):

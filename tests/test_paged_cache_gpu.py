@@ -1,5 +1,7 @@
 """``PagedCache`` on the GPU: page copies, stores into slots, restores into pages, captured calls."""
 
+import copy
+
 import numpy as np
 import pytest
 import torch
@@ -141,6 +143,25 @@ def test_restore_into_pages_equals_store(device):
     for name in ("keys", "values"):
         a, b = (torch.cat([getattr(c, name)[0, page] for page in c.pages_of(0)])[20:20 + n] for c in caches)
         assert torch.equal(a, b) and a.any()
+
+
+def test_a_copied_cache_has_pools_of_its_own(device):
+    """Page copies of a deep copy stay in its own pools, whatever was copied before."""
+    cache = paged_cache.PagedCache.allocate(6, 4, 2, 8, layers=2, device=device)
+    cache.keys.normal_(), cache.values.normal_()
+    a = cache.new()
+    cache.extend([a], [6])
+    b = cache.fork(a)
+    cache.extend([b], [1])  # a copy of the begun page
+    twin = copy.deepcopy(cache)
+    before = cache.keys.clone(), cache.values.clone()
+    c = twin.fork(a)
+    twin.extend([c], [1])
+    source, target = twin.pages_of(a)[1], twin.pages_of(c)[1]
+    assert source != target
+    assert torch.equal(twin.keys[:, target, :2], twin.keys[:, source, :2])
+    assert torch.equal(twin.values[:, target, :2], twin.values[:, source, :2])
+    assert torch.equal(cache.keys, before[0]) and torch.equal(cache.values, before[1])
 
 
 def test_captured_store_and_copies(device):

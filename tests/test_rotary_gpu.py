@@ -207,6 +207,21 @@ def test_other_stream(device):
     assert torch.equal(out, expected)
 
 
+def test_outputs_that_autograd_saved(device):
+    """A result written into a tensor that a backward pass needs is noticed by that pass."""
+    cos, sin, sections = oracle.tables(16, 8)
+    at = rk.RopePositions(rk.RopeTable(cos.to(device), sin.to(device), sections), 0)
+    x, saved = torch.randn(1, 6, 1, 16, device=device), torch.randn(1, 6, 1, 16, device=device)
+    weight = torch.randn(1, 6, 1, 16, device=device, requires_grad=True)
+    product = (weight * saved).sum()
+    with torch.no_grad():
+        rotary.rotate(x, at, grid=(1, 2, 3), out=saved)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    with torch.inference_mode():
+        rotary.rotate(x, at, grid=(1, 2, 3), out=torch.empty_like(x))
+
+
 def test_rotation_has_the_restores_bits(device):
     """Dense rows restored with RoPE and the same rows rotated: the same bits."""
     cos, sin, sections = oracle.tables(32, 64)
