@@ -569,6 +569,11 @@ int rch_pages_copy(const rch_pages* pages_host, const int32_t* moves_host, int n
 #define RCH_ARGUMENT_WORDS 960
 int rch_words_store(void* words_dev, const int32_t* words_host, int count, void* stream);
 
+/* Writes runs of ascending int32 words, one behind the other, `words` in all: runs_host int32 [n_runs][2] of
+ * (first value, count), read before the call returns; RCH_ARGUMENT_RUNS to a launch. */
+#define RCH_ARGUMENT_RUNS 320
+int rch_runs_store(void* words_dev, const int32_t* runs_host, int n_runs, int64_t words, void* stream);
+
 /*
  * Attention of new tokens over a paged cache.  A plan is a device int32 buffer built by the host:
  * items (RCH_ATTEND_ITEM words each), merges (RCH_ATTEND_MERGE words each) and page tables; its first

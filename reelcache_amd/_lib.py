@@ -119,6 +119,7 @@ _SIGNATURES = {
     "rch_rotary": ([_p, _i, _i, _i, _p], _i),
     "rch_pages_copy": ([_p, _p, _i, _p], _i),
     "rch_words_store": ([_p, _p, _i, _p], _i),
+    "rch_runs_store": ([_p, _p, _i, _i64, _p], _i),
     "rch_attend_share": ([_p, _p, _i64, _i64, _i64, _p, _i64, _p], _i),
     "rch_attend_size": ([], _i),
     "rch_attend_run": ([_p, _i, _p], _i),

@@ -64,6 +64,16 @@ __global__ void __launch_bounds__(256) words_store_kernel(int64_t to, const Word
     for (int i = threadIdx.x; i < count; i += 256) gout<int32_t>(to)[i] = words.word[i];
 }
 
+// Runs of ascending words: run i writes first, first + 1, .. to `count` words from `at`.  The slots of a step's new
+// tokens are one run for each sequence and page, so thousands of them travel in one launch's arguments.
+struct Runs {
+    int32_t first[RCH_ARGUMENT_RUNS], count[RCH_ARGUMENT_RUNS], at[RCH_ARGUMENT_RUNS];
+};
+__global__ void __launch_bounds__(256) runs_store_kernel(int64_t to, const Runs runs) {
+    const int run = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+    if (i < runs.count[run]) gout<int32_t>(to)[static_cast<int64_t>(runs.at[run]) + i] = runs.first[run] + i;
+}
+
 }  // namespace
 
 }  // namespace rch
@@ -80,6 +90,37 @@ int rch_words_store(void* words_dev, const int32_t* words_host, int count, void*
         const int64_t to = reinterpret_cast<int64_t>(words_dev) + 4 * static_cast<int64_t>(first);
         hipLaunchKernelGGL(words_store_kernel, dim3(1), dim3(256), 0, as_stream(stream), to, words, n);
         const int status = check_launch("rch_words_store");
+        if (status != RCH_OK) return status;
+    }
+    return RCH_OK;
+}
+
+int rch_runs_store(void* words_dev, const int32_t* runs_host, int n_runs, int64_t words, void* stream) {
+    using namespace rch;
+    if (n_runs < 0 || words < 0 || words > 0x7fffffff || (n_runs > 0 && (!words_dev || !runs_host)))
+        return fail(RCH_E_CONFIG, "rch_runs_store: invalid arguments");
+    int64_t at = 0;
+    for (int i = 0; i < n_runs; ++i) {
+        if (runs_host[2 * i + 1] < 0) return fail(RCH_E_CONFIG, "rch_runs_store: run %d has a negative count", i);
+        at += runs_host[2 * i + 1];
+    }
+    if (at != words) return fail(RCH_E_CONFIG, "rch_runs_store: the runs have %lld words, not %lld", static_cast<long long>(at), static_cast<long long>(words));
+    at = 0;
+    for (int first = 0; first < n_runs; first += RCH_ARGUMENT_RUNS) {
+        const int n = n_runs - first < RCH_ARGUMENT_RUNS ? n_runs - first : RCH_ARGUMENT_RUNS;
+        Runs runs;
+        int32_t longest = 0;
+        for (int i = 0; i < n; ++i) {
+            runs.first[i] = runs_host[2 * (first + i)];
+            runs.count[i] = runs_host[2 * (first + i) + 1];
+            runs.at[i] = static_cast<int32_t>(at);
+            at += runs.count[i];
+            longest = runs.count[i] > longest ? runs.count[i] : longest;
+        }
+        if (longest == 0) continue;
+        const dim3 grid(static_cast<uint32_t>((static_cast<int64_t>(longest) + 255) / 256), static_cast<uint32_t>(n));
+        hipLaunchKernelGGL(runs_store_kernel, grid, dim3(256), 0, as_stream(stream), reinterpret_cast<int64_t>(words_dev), runs);
+        const int status = check_launch("rch_runs_store");
         if (status != RCH_OK) return status;
     }
     return RCH_OK;

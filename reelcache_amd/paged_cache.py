@@ -4,7 +4,8 @@ A restored history is written into native cache slots (reelcache/restore_kernels
 serving engine keeps such slots in pages so that continuations of one history share it.
 :class:`PagedCache` holds the K and V pools of all layers and, on the host, the pages of each
 sequence.  Every layer uses the same page of a sequence for the same tokens, so a page is copied in
-all layers' K and V pools at once (``rch_pages_copy``).
+all layers' K and V pools at once (``rch_pages_copy``), and the slots of new tokens are written as runs of
+consecutive rows (``rch_runs_store``).
 
 Pools are ``[layers, pages, page_tokens, heads, head_dim]`` (``layout="BTHD"``) or ``[layers, pages,
 heads, page_tokens, head_dim]`` (``"BHTD"``): one layer's pool is a native cache tensor whose batch
@@ -61,10 +62,11 @@ class _Sequence:
 # Tables of at most this many words travel in the arguments of one launch: 64 words take 6.5 us of the host
 # so and 9.8 us through pinned memory, 960 words 7.7 and 10.0 us; at 1920 (two launches) it is 11.9 and 10.3 us.
 _ARGUMENT_WORDS = 960
-# Slots of at most this many tokens are listed one by one, more by array operations: slots of one token take
-# 9.7 and 15.7 us of the host, of 128 tokens 15.3 and 15.9 us, of 256 tokens 21.4 and 17.2 us; of one token of
-# each of 128 sequences 73 and 85 us.
-_FEW_TOKENS = 128
+# Slots of at most this many runs (a run: the tokens of a sequence in one page) travel as runs in the arguments
+# of a launch, more as an array: slots of one token take 9.9 and 16.6 us of the host, of 512 in two pages 11.2 and
+# 19.4 us, of 1024 in 64 pages 20.6 and 26.1 us, of 2048 in 128 pages 30.8 and 30.9 us, of 4096 in 256 pages 51.6 and
+# 40.7 us.
+_FEW_RUNS = 128
 
 
 def upload(values, device):
@@ -82,6 +84,14 @@ def upload_words(words, shape, device):
     _refuse_capture(device)
     out = torch.empty(shape, dtype=torch.int32, device=device)
     _lib.check(_lib.function("rch_words_store")(out.data_ptr(), words, len(words) // 4, raw_stream(device)))
+    return out
+
+
+def upload_runs(runs, total, device):
+    """An int32 array of runs of ascending values: ``runs`` is flat, (first value, count) of each."""
+    _refuse_capture(device)
+    out = torch.empty(total, dtype=torch.int32, device=device)
+    _lib.check(_lib.function("rch_runs_store")(out.data_ptr(), _pack(runs), len(runs) // 2, total, raw_stream(device)))
     return out
 
 
@@ -178,13 +188,13 @@ class PagedCache:
     def fork(self, sequence):
         """A new sequence with the same tokens: it shares every page.  A page that is not full is copied
         when the first of its sequences goes on."""
-        source = self._get(sequence)
+        source, uses, child = self._get(sequence), self._uses, self._next
         for page in source.pages:
             if page != HOLE:
-                self._uses[page] += 1
+                uses[page] += 1
         self._shared += 1
-        child = self.new()
-        self._sequences[child] = _Sequence(list(source.pages), source.tokens)
+        self._sequences[child] = _Sequence(source.pages[:], source.tokens)
+        self._next = child + 1
         return child
 
     def _release(self, pages):
@@ -296,11 +306,18 @@ class PagedCache:
 
     def _slots(self, found, starts, counts):
         size = self.page_tokens
-        if sum(counts) <= _FEW_TOKENS:
-            words = [item.pages[at // size] * size + at % size for item, start, n in zip(found, starts, counts)
-                     for at in range(start, start + n)]
+        pieces = sum([-(-(start + n) // size) - start // size for start, n in zip(starts, counts) if n])
+        if pieces <= _FEW_RUNS:
+            runs = []
+            for item, at, left in zip(found, starts, counts):
+                while left:
+                    page, row = divmod(at, size)
+                    n = min(left, size - row)
+                    runs += (item.pages[page] * size + row, n)
+                    at += n
+                    left -= n
             with entered(self.device):
-                return self._made(upload_words(_pack(words), (len(words),), self.device))
+                return self._made(upload_runs(runs, sum(counts), self.device))
         pages, base = [], []  # the pages of all tokens, and where each sequence's page 0 would lie among them
         for item, start, n in zip(found, starts, counts):
             first = start // size

@@ -42,6 +42,8 @@ def host(monkeypatch):
     monkeypatch.setattr(paged_cache, "upload", lambda values, device: torch.from_numpy(np.array(values, dtype=np.int32)))
     monkeypatch.setattr(paged_cache, "upload_words", lambda words, shape, device:
                         torch.from_numpy(np.frombuffer(words, dtype=np.int32).reshape(shape).copy()))
+    monkeypatch.setattr(paged_cache, "upload_runs", lambda runs, total, device: torch.cat(
+        [torch.arange(a, a + n, dtype=torch.int32) for a, n in zip(runs[::2], runs[1::2])] or [torch.empty(0, dtype=torch.int32)]))
     return copies
 
 
@@ -466,3 +468,9 @@ def test_abi_refusals():
             _lib.call("rch_attend_share", *arguments, ctypes.byref(found))
     with pytest.raises(ConfigurationError):
         _lib.call("rch_words_store", None, (ctypes.c_int32 * 1)(1), 1, None)
+    run = (ctypes.c_int32 * 2)(5, 3)
+    for arguments in ((None, run, 1, 3), (64, None, 1, 3), (64, run, 1, 4), (64, run, 1, 2), (64, run, -1, 0), (64, (ctypes.c_int32 * 2)(5, -1), 1, -1),
+                      (64, (ctypes.c_int32 * 2)(5, -1), 1, 0)):
+        with pytest.raises(ConfigurationError):
+            _lib.call("rch_runs_store", *arguments, None)
+    _lib.call("rch_runs_store", None, None, 0, 0, None)

@@ -145,6 +145,30 @@ def test_restore_into_pages_equals_store(device):
         assert torch.equal(a, b) and a.any()
 
 
+@pytest.mark.parametrize("size,lengths,counts", [
+    (4, [0], [1]), (4, [3, 0, 7], [1, 0, 6]), (1, [0, 5], [70, 1]), (256, [0, 255], [1000, 2]), (16, [5] * 40, [20] * 40), (16, [5] * 90, [20] * 90),
+    (3, [1] * 30, [1] * 30), (2, [0], [700]), (512, [100], [4000]), (4, [2, 2], [0, 0]),
+])
+def test_slots_name_the_tokens_places(device, size, lengths, counts):
+    """Few and many runs, of one token and of whole pages."""
+    pages = sum(-(-(n + more) // size) for n, more in zip(lengths, counts)) + 3
+    cache = paged_cache.PagedCache.allocate(pages, size, 1, 1, device=device)
+    sequences = [cache.new() for _ in lengths]
+    cache.extend(sequences, lengths)
+    for slots in (cache.extend(sequences, counts), cache.slots(sequences, lengths, counts)):
+        want = [cache.pages_of(s)[at // size] * size + at % size for s, n, more in zip(sequences, lengths, counts)
+                for at in range(n, n + more)]
+        assert slots.tokens == len(want) and slots.index.tolist() == want
+
+
+def test_runs_of_more_than_one_launch(device):
+    """1000 runs in four launches, some of them empty."""
+    runs = [value for i in range(1000) for value in (7 * i, i % 5 if i % 50 else 300)]
+    total = sum(runs[1::2])
+    out = paged_cache.upload_runs(runs, total, device)
+    assert out.tolist() == [a + j for a, n in zip(runs[::2], runs[1::2]) for j in range(n)]
+
+
 def test_a_copied_cache_has_pools_of_its_own(device):
     """Page copies of a deep copy stay in its own pools, whatever was copied before."""
     cache = paged_cache.PagedCache.allocate(6, 4, 2, 8, layers=2, device=device)
