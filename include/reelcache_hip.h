@@ -613,8 +613,9 @@ typedef struct rch_attend {
     int64_t items;           /* word index of the first item */
     int64_t n_general, n_rows; /* items of the general and of the tiled form, in order */
     int64_t merges, n_merges;      /* word index and count */
-    int64_t n_many;                /* the first ones: merges of more than RCH_ATTEND_FEW_PARTS parts, or of rows
-                                      that are no aligned multiples of eight channels */
+    int64_t n_many;                /* the first ones, which take a workgroup to a row: all merges of more than
+                                      RCH_ATTEND_FEW_PARTS parts, or of rows that are no aligned multiples of
+                                      eight channels, and others as the caller likes */
     int64_t most_rows_many, most_rows; /* most rows of one of those, and of one of the others */
     int64_t holes;           /* 1: page tables may hold holes */
     int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64 */

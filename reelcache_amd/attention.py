@@ -35,6 +35,9 @@ GENERAL_ROWS, ROW_TILE = 16, 128
 # 211 to 5003 tokens takes 58.0 us at 0, 55.4 at 3, 54.8 at 6 and 55.0 at 8; others do not change by more than 2 %).
 _OVERHEAD = {"general": 1, "rows": 6}
 _CUS = 256
+# At most this many rows are joined a workgroup to a row, whatever their parts, in one launch (512 rows of 4 parts take
+# 4.1 us so, 4.1-5.1 us with a thread per eight channels; a second launch costs 5 us).
+_FEW_ROWS = 512
 _XCDS = 8
 # Scales that stay normal fp32 numbers with log2(e) in them.
 _LEAST_SCALE, _MOST_SCALE = 2.0 ** -126, 2.0 ** 127
@@ -165,6 +168,8 @@ class AttentionPlan:
         # Merges that take a workgroup to a row come first (the kernels' rule).
         joined = counts["general"] == 0 and cache.head_dim % 8 == 0
         many = (merges[:, 5] > _lib.ATTEND_FEW_PARTS) | (not joined)
+        if len(merges) * merges[:, 2].max(initial=0) <= _FEW_ROWS:
+            many[:] = True
         merges = np.concatenate([merges[many], merges[~many]])
         self._n_merges, self._n_many = len(merges), int(many.sum())
         self._most_rows = [int(part[:, 2].max(initial=0)) for part in np.split(merges, [self._n_many])]

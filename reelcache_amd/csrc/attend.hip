@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A,
 
 // Joins the parts of rows whose keys were split (the same order whatever the timing).  Bound: the latency of
 // the partial results (other XCDs wrote them), so all or many of a row's loads are in flight at once.  Rows of
-// more than kFewParts parts (single tokens over long histories) take a workgroup each, whose waves share the
-// parts; rows of fewer a thread per eight channels.  Rows of 128 channels: 228 blocks of 128 rows in 3 and 7 parts
+// more than kFewParts parts (single tokens over long histories), or of a step with few, take a workgroup each, whose
+// waves share the parts; the others a thread per eight channels.  Rows of 128 channels: 228 blocks of 128 rows in 3 and 7 parts
 // take 10.4 us so and 43 us with a workgroup each (29184 workgroups); 32 blocks of 4 rows in 11 or 16 parts 4.0 us
 // with a workgroup each and, with a thread per eight channels over groups of 8 parts, 5.8 and 7.4 us.
 // A workgroup has 16 waves where at most kWideRows rows are joined (8 rows in 159 parts: 7.2 us, with 4 waves

@@ -183,6 +183,15 @@ def test_rows_of_many_parts(device, dtype, dim, lengths, rows, least):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [128, 72, 256, 136])
+def test_chunks_in_several_parts(device, dtype, dim):
+    """Whole blocks of rows in two to eight parts, beside single tokens in more."""
+    _, _, plan, _ = _run(device, [620, 2400], [250, 1], 64, 4, 1, dim, dtype, block=50)
+    merges = plan.buffer[plan._merges:plan._merges + 8 * plan._n_merges].view(-1, 8)
+    assert plan._n_many < plan._n_merges and merges[:, 2].max() == 128 and merges[plan._n_many:, 5].max() <= 8
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("block", [None, 1])
 @pytest.mark.parametrize("size,kv_heads,group,dim,layout", [
     (64, 1, 1, 256, "BTHD"), (16, 2, 2, 192, "BHTD"), (7, 1, 1, 136, "BTHD"), (100, 1, 3, 200, "BTHD"), (9, 1, 1, 248, "BTHD"),
