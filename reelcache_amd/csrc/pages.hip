@@ -6,7 +6,7 @@
 // `rows` token rows, which are one piece of memory where the rows lie next to each other.  A
 // workgroup copies 16 KiB of one page of one pool; a thread has four 16-byte loads in flight.  Twelve pages
 // of 256 tokens x 12 heads x 128 bf16 in 60 pools (1.13 GB read and written) take 218 us, 5.2 TB/s; eight
-// forks of 96 rows (159 MB) 35.7 us, 4.5 TB/s.
+// forks of 96 rows (159 MB) 36 us, 4.4 TB/s.
 #include "common.h"
 
 namespace rch {
