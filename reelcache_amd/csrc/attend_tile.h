@@ -366,7 +366,8 @@ struct RowTile {
         f16v s[KB];
 #pragma unroll
         for (int b = 0; b < KB; ++b) s[b] = f16v{};
-        // The blocks' chains side by side, the reads kAhead products ahead (2, 4 or 6: the same within 1 %).
+        // The blocks' chains side by side, the reads kAhead products ahead (2, 4 or 6: the same within 1 %; in the
+        // compiler's own order a chunk takes 951 us against 943).
 #pragma unroll
         for (int c = 0; c < 2 * NB; ++c)
 #pragma unroll
