@@ -71,9 +71,10 @@ __device__ __forceinline__ float row_sum(float x) {
 
 // 16 bytes a lane from memory to LDS at `lds` (wave-uniform) + 16 * lane, not waited for.  In assembly, so
 // that the compiler does not wait for them before every LDS read: the callers' own waits and barriers
-// order them.  Nothing is written but LDS.
+// order them.  Nothing is written but LDS.  The compiler counts no wait states into an assembly block: m0 needs one
+// before the load, and a resource's registers five after a vector instruction (v_readfirstlane) wrote them.
 __device__ __forceinline__ void fetch_buffer(u4 rsrc, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rsrc)
                  : "memory", "m0");
 }
 __device__ __forceinline__ void fetch_global(int64_t address, uint32_t lds) {
