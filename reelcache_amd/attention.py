@@ -190,7 +190,10 @@ class AttentionPlan:
         # where a wave's rows of a tile (16, fp32: 8) lie in one page, and 30 % more (an address for every row)
         # where they do not: a chunk's 2340 queries over 9360 keys, 12 heads, take 169-174 us either way, 225 us
         # with addresses, and 193 us in pages of 390 tokens, 230 us in pages of 200, 274 us in pages of 100.
+        # The kernels look a tile's page up once where tiles stay within pages, so those hold a tile at least.
         size = self.cache.page_tokens
+        if size < KEY_TILE:
+            return KEY_TILE
         share = 16 if self.cache.keys.element_size() == 2 else 8
         held = -(-size // KEY_TILE) * KEY_TILE  # rows of tiles that a page takes
         return size if held == size or (size % share and 5 * held <= 6 * size) else KEY_TILE

@@ -384,3 +384,21 @@ def test_a_step_of_two_layers(device):
         if chunk == 1:
             b = cache.fork(a)
     assert cache.pages_of(a)[:5] == cache.pages_of(b)[:5] and cache.pages_of(a)[5] != cache.pages_of(b)[5]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [54, 60, 63])
+@pytest.mark.parametrize("layout", ["BTHD", "BHTD"])
+def test_pages_just_below_a_tile(device, dtype, size, layout):
+    """Single tokens, chunks and a dropped page in pages of a few tokens less than a tile."""
+    _run(device, [1, size, size + 1, 300], [1, 1, 1, 1], size, 2, 2, 64, dtype, layout)
+    _run(device, [133, 260, 40], [129, 75, 33], size, 1, 2, 128, dtype, layout, block=1)
+    lengths, queries = [5 * size + 3], [size]
+    cache = _cache(device, lengths, size, 1, 64, dtype, layout)
+    dropped = cache.pages_of(0)[2]
+    cache.drop(0, 2, 1)
+    for pool in (cache.keys, cache.values):
+        pool[:, dropped] = math.inf
+    q = torch.randn((size, 2, 64), generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
+    plan = cache.plan([0], queries, heads=2, block=1)
+    _check(cache, q, *cache.attend(0, q, plan, return_lse=True), lengths, queries, block=1)

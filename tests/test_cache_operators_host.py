@@ -3,6 +3,7 @@
 import contextlib
 import heapq
 import re
+import types
 from pathlib import Path
 
 import numpy as np
@@ -474,3 +475,13 @@ def test_abi_refusals():
         with pytest.raises(ConfigurationError):
             _lib.call("rch_runs_store", *arguments, None)
     _lib.call("rch_runs_store", None, None, 0, 0, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tiles_start_over_where_the_kernels_take_them(dtype):
+    """Every page size gets tiles that the kernels accept: of 64 keys, or within pages that hold one."""
+    plan = object.__new__(attention.AttentionPlan)
+    for size in range(1, 2000):
+        plan.cache = types.SimpleNamespace(page_tokens=size, keys=torch.empty(0, dtype=dtype))
+        unit = plan._unit()
+        assert unit == attention.KEY_TILE or (unit == size and size >= attention.KEY_TILE), (size, unit)
