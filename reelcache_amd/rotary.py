@@ -259,12 +259,17 @@ def _rotate(tensors, positions, grid, layout, pairing, inverse):
             plain = all(x.stride(-1) == 1 or x.shape[-1] == 1 for x in tensors)
             if not plain:
                 tensors = [x if x.stride(-1) == 1 else x.contiguous() for x in tensors]
+            # As the input lies in memory, unless that takes the channels apart (overlapping rows).
             outs = tuple(torch.empty_like(x) for x in tensors)
-            call = (_prepare(tensors, outs, positions, grid, layout, pairing, inverse),)
+            form = torch.preserve_format
+            if any(out.stride(-1) != 1 and out.shape[-1] > 1 for out in outs):
+                form = torch.contiguous_format
+                outs = tuple(torch.empty_like(x, memory_format=form) for x in tensors)
+            call = _prepare(tensors, outs, positions, grid, layout, pairing, inverse), form
             if plain:
                 known[key] = call
         else:
-            outs = tuple([torch.empty_like(x) for x in tensors])
+            outs = tuple([torch.empty_like(x, memory_format=call[1]) for x in tensors])
         _run(call[0], tensors, outs, positions)
     return outs
 

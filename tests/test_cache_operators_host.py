@@ -485,3 +485,25 @@ def test_tiles_start_over_where_the_kernels_take_them(dtype):
         plan.cache = types.SimpleNamespace(page_tokens=size, keys=torch.empty(0, dtype=dtype))
         unit = plan._unit()
         assert unit == attention.KEY_TILE or (unit == size and size >= attention.KEY_TILE), (size, unit)
+
+
+def test_outputs_of_overlapping_rows_have_their_channels_side_by_side(monkeypatch):
+    """Rows that overlap in memory (a window of one step): the launch writes a head's channels one after another,
+    so the output has them so."""
+    monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
+    monkeypatch.setattr(rotary, "entered", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(rotary, "_table_pairs", lambda table, device, stream: 64)
+    monkeypatch.setattr(rotary, "raw_stream", lambda device: 0)
+    launches = []
+    monkeypatch.setattr(rotary.Launch, "__call__", lambda self, addresses, *rest: launches.append(
+        dict(zip(_lib.ROTARY_FIELDS, np.frombuffer(self.image, np.int64).tolist()))))
+    cos, sin, sections = oracle.tables(40, 32)
+    positions = rk.RopePositions(rk.RopeTable(cos, sin, sections), 0)
+    x = torch.randn(200).as_strided((9, 1, 64), (1, 64, 1))
+    for _ in range(2):
+        out = rotary.rotate(x, positions, grid=(1, 3, 3), layout="THD")
+        assert out.shape == x.shape and out.stride(-1) == 1
+    assert len(launches) == 2
+    for fields in launches:
+        assert (fields["dst_token_stride"], fields["dst_head_stride"]) == out.stride()[:2]
+        assert fields["src_token_stride"] == 1

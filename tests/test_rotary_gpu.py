@@ -232,3 +232,21 @@ def test_rotation_has_the_restores_bits(device):
     job = rk.ReconstructionJob(rk.DenseSource(x.reshape(70, 384)), rk.NativeView(cache), grid, rope=positions)
     rk.reconstruct([job]).release()
     assert torch.equal(cache[0], rotary.rotate(x, positions, grid=grid, layout="THD"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pairing", rotary.PAIRINGS)
+def test_rows_that_overlap(device, dtype, pairing):
+    """Windows of one step over a line of values, forward and as a gradient."""
+    cos, sin, sections = oracle.tables(40, 32)
+    table = rk.RopeTable(cos, sin, sections)
+    line = _normal((200,), dtype, device, 1)
+    x = line.as_strided((9, 2, 64), (1, 70, 1))
+    c, s = (a[:, None] for a in oracle.token_angles(cos, sin, sections, oracle.grid_rows((2, 0, 1), (1, 3, 3))))
+    positions = rk.RopePositions(table, (2, 0, 1))
+    for _ in range(2):
+        out = rotary.rotate(x, positions, grid=(1, 3, 3), layout="THD", pairing=pairing)
+        assert oracle.worst(out, *oracle.rotate(x, c, s, pairing)) <= 0
+    leaf = _normal((9, 2, 64), dtype, device, 2).requires_grad_(True)
+    grad, = torch.autograd.grad(rotary.rotate(leaf, positions, grid=(1, 3, 3), layout="THD", pairing=pairing), (leaf,), x)
+    assert oracle.worst(grad, *oracle.rotate(x, c, -s, pairing)) <= 0
