@@ -26,7 +26,7 @@ import torch
 
 from . import _lib
 from ._checks import count, in_memory, need, one_of, strided
-from .errors import ConfigurationError, UnsupportedError
+from .errors import ConfigurationError, StateError, UnsupportedError
 from .restore_model import _AXES, LAYOUTS, OUTPUT_DTYPES, RopePositions, RopeTable
 
 PAIRINGS = ("interleaved", "half")
@@ -288,6 +288,12 @@ def _rotate_into(tensors, outs, positions, grid, layout, pairing, inverse):
                 changed(out)
 
 
+def _table_state(table, device):
+    """What a table's angles on ``device`` go by: its stamp, and the device copy where the stamp counts no
+    updates (inference tensors, whose owner drops the copy)."""
+    return table._stamp(), table._device_cache.get(device) if table._inference else None
+
+
 class _Rotation(torch.autograd.Function):
     """The rotation as a differentiable function of its tensors; linear, so the backward pass is the
     rotation back (differentiable itself, as it goes through :func:`rotate`)."""
@@ -298,23 +304,28 @@ class _Rotation(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         if isinstance(positions, TokenRows):
             ctx.save_for_backward(positions.rows)  # rows changed in place before the backward pass are refused
-        return _rotate(tensors, positions, grid, layout, pairing, inverse)
+        outs = _rotate(tensors, positions, grid, layout, pairing, inverse)
+        ctx.table = _table_state(positions.table, tensors[0].device)  # a table changed before the backward pass is refused
+        return outs
 
     @staticmethod
     def backward(ctx, *grads):
         positions, grid, layout, pairing, inverse = ctx.arguments
-        if isinstance(positions, TokenRows):
-            ctx.saved_tensors  # noqa: B018  (checks the rows' version)
         wanted = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[5 + i]]
         out = [None] * len(grads)
-        if wanted:
-            given = tuple([grads[i] for i in wanted])
-            if torch.is_grad_enabled():  # a graph of the gradients is asked for
-                turned = rotate(given, positions, grid=grid, layout=layout, pairing=pairing, inverse=not inverse)
-            else:
-                turned = _rotate(given, positions, grid, layout, pairing, not inverse)
-            for i, g in zip(wanted, turned):
-                out[i] = g
+        if not wanted:
+            return (None, None, None, None, None, *out)
+        given = tuple([grads[i] for i in wanted])
+        if isinstance(positions, TokenRows):
+            ctx.saved_tensors  # noqa: B018  (checks the rows' version)
+        if _table_state(positions.table, given[0].device) != ctx.table:
+            raise StateError("the RoPE table was changed between a rotation and its backward pass")
+        if torch.is_grad_enabled():  # a graph of the gradients is asked for
+            turned = rotate(given, positions, grid=grid, layout=layout, pairing=pairing, inverse=not inverse)
+        else:
+            turned = _rotate(given, positions, grid, layout, pairing, not inverse)
+        for i, g in zip(wanted, turned):
+            out[i] = g
         return (None, None, None, None, None, *out)
 
 
@@ -329,7 +340,8 @@ def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interl
     into, which may be the input itself; without it the outputs are new tensors.
 
     Runs on the current stream of the tensors' device.  Differentiable in the tensors (in
-    reverse mode; not with ``out``).  Returns a tensor, or a tuple for a tuple.
+    reverse mode; not with ``out``); a table or token rows changed in place before the backward pass are
+    refused there.  Returns a tensor, or a tuple for a tuple.
     """
     single = isinstance(tensors, torch.Tensor)
     tensors = (tensors,) if single else tuple(tensors)

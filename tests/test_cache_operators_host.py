@@ -507,3 +507,24 @@ def test_outputs_of_overlapping_rows_have_their_channels_side_by_side(monkeypatc
     for fields in launches:
         assert (fields["dst_token_stride"], fields["dst_head_stride"]) == out.stride()[:2]
         assert fields["src_token_stride"] == 1
+
+
+@pytest.mark.parametrize("tokens", [False, True])
+@pytest.mark.parametrize("which", ["cos", "sin"])
+def test_tables_changed_before_the_backward_pass_are_refused(monkeypatch, tokens, which):
+    monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
+    monkeypatch.setattr(rotary, "entered", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(rotary, "_table_pairs", lambda table, device, stream: 64)
+    monkeypatch.setattr(rotary, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(rotary.Launch, "__call__", lambda self, addresses, *rest: None)
+    cos, sin, sections = oracle.tables(8, 4)
+    table = rk.RopeTable(cos, sin, sections)
+    positions = rotary.TokenRows(table, torch.zeros(6, 3, dtype=torch.int32)) if tokens else rk.RopePositions(table, 0)
+    x = torch.zeros(1, 6, 2, 8, requires_grad=True)
+    call = lambda: rotary.rotate(x, positions, grid=None if tokens else (1, 2, 3)).sum()
+    call().backward()
+    out = call()
+    getattr(table, which).mul_(0.5)
+    with pytest.raises(StateError, match="table was changed"):
+        out.backward()
+    call().backward()

@@ -6,6 +6,7 @@ import torch
 
 from reelcache_amd import restore_kernels as rk
 from reelcache_amd import rotary
+from reelcache_amd.errors import StateError
 
 import operator_oracle as oracle
 
@@ -250,3 +251,19 @@ def test_rows_that_overlap(device, dtype, pairing):
     leaf = _normal((9, 2, 64), dtype, device, 2).requires_grad_(True)
     grad, = torch.autograd.grad(rotary.rotate(leaf, positions, grid=(1, 3, 3), layout="THD", pairing=pairing), (leaf,), x)
     assert oracle.worst(grad, *oracle.rotate(x, c, -s, pairing)) <= 0
+
+
+def test_inference_tables_dropped_before_the_backward_pass_are_refused(device):
+    """Tables of inference tensors count no updates: their owner drops the copies, and a gradient by others is refused."""
+    cos, sin, sections = oracle.tables(16, 8)
+    with torch.inference_mode():
+        table = rk.RopeTable(cos.clone(), sin.clone(), sections)
+    at = rk.RopePositions(table, 0)
+    x = _normal((1, 6, 1, 16), torch.float32, device, 1).requires_grad_(True)
+    rotary.rotate(x, at, grid=(1, 2, 3)).sum().backward()
+    out = rotary.rotate(x, at, grid=(1, 2, 3))
+    with torch.inference_mode():
+        table.cos.mul_(0.5)
+    table.invalidate()
+    with pytest.raises(StateError, match="table was changed"):
+        out.sum().backward()
