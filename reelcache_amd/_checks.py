@@ -12,6 +12,7 @@ from typing import Any
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .errors import ConfigurationError
 
@@ -38,9 +39,12 @@ def strided(value: Any, name: str) -> torch.Tensor:
 
 
 def in_memory(value: Any, name: str) -> torch.Tensor:
-    """A strided tensor whose storage holds its values (no negation that is still to be done)."""
+    """A strided tensor whose storage holds its values (no negation that is still to be done) and nothing
+    besides (no tangent of forward-mode differentiation, which a kernel would drop)."""
     if strided(value, name).is_neg():
         raise ConfigurationError(f"{name} has a negation pending; resolve_neg() it")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(value).tangent is not None:
+        raise ConfigurationError(f"{name} has a forward-mode tangent; only reverse mode is differentiated")
     return value
 
 

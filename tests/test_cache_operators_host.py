@@ -528,3 +528,24 @@ def test_tables_changed_before_the_backward_pass_are_refused(monkeypatch, tokens
     with pytest.raises(StateError, match="table was changed"):
         out.backward()
     call().backward()
+
+
+def test_forward_mode_tangents_are_refused(host, monkeypatch):
+    monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
+    cache = make()
+    a = cache.new()
+    slots = cache.extend([a], [1])
+    cos, sin, sections = oracle.tables(8, 4)
+    positions = rk.RopePositions(rk.RopeTable(cos, sin, sections), 0)
+    plan = cache.plan([a], [1], heads=2)
+    plain = torch.randn(1, 2, 8)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(plain, torch.ones_like(plain))
+        pool = torch.autograd.forward_ad.make_dual(cache.keys[0], torch.ones_like(cache.keys[0]))
+        for call in (lambda: rotary.rotate(dual, positions, grid=(1, 1, 1), layout="THD"),
+                     lambda: rotary.rotate(plain, positions, grid=(1, 1, 1), layout="THD", out=dual),
+                     lambda: cache.store(0, slots, dual, plain), lambda: cache.store(0, slots, plain, dual),
+                     lambda: cache.attend(0, dual, plan), lambda: attention.attend(plain, pool, cache.values[0], plan),
+                     lambda: paged_cache.PagedCache(dual[None, None], plain[None, None])):
+            with pytest.raises(ConfigurationError, match="tangent"):
+                call()
