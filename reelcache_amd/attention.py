@@ -274,6 +274,8 @@ class AttentionPlan:
             need(pool.shape == shape and pool.stride() == stride and pool.dtype == cache.dtype
                  and pool.device == cache.device, f"{name} must be a layer's pool like those of the plan's cache")
             need(self._tiled == 0 or pool.data_ptr() % 16 == 0, f"{name} must be aligned as the plan's cache is")
+            need(not (pool.requires_grad and torch.is_grad_enabled()),
+                 "attention over a cache is not differentiable; run it under torch.no_grad()")
 
     def _fields(self, q_stride, out_stride):
         """The ``rch_attend`` image of a call: everything but the addresses."""

@@ -549,3 +549,18 @@ def test_forward_mode_tangents_are_refused(host, monkeypatch):
                      lambda: paged_cache.PagedCache(dual[None, None], plain[None, None])):
             with pytest.raises(ConfigurationError, match="tangent"):
                 call()
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_attention_refuses_pools_that_require_gradients(host, which):
+    cache = make()
+    a = cache.new()
+    cache.extend([a], [1])
+    plan = cache.plan([a], [1], heads=2)
+    pools = [cache.keys[0].clone(), cache.values[0].clone()]
+    plan._check(*pools)
+    pools[which].requires_grad_(True)
+    with pytest.raises(ConfigurationError, match="differentiable"):
+        attention.attend(torch.zeros(1, 2, 8), *pools, plan)
+    with torch.no_grad():
+        plan._check(*pools)
