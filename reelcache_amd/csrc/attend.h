@@ -49,8 +49,9 @@ struct AttendType<RCH_DT_BF16> {
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// A reference exponent below every score: a row that has seen nothing keeps it, and its sum stays 0.
-constexpr float kNoReference = -3.0e38f;
+// A reference exponent that no score lies below (the lowest fp32): a row that has seen nothing keeps it, and its sum
+// stays 0.
+constexpr float kNoReference = -3.402823466e38f;
 constexpr float kLn2 = 0.693147180559945309f;
 
 __device__ __forceinline__ float row_lse(float reference, float sum) {

@@ -114,7 +114,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
                 const int d = Tile::channel_of(b, i, h);
                 if (d < A.head_dim) *gout<f4>(to + 4 * d) = f4{tile.o[b][i], tile.o[b][i + 1], tile.o[b][i + 2], tile.o[b][i + 3]};
             }
-        if (h == 0) *gout<f2>(partial_stats(A, at)) = f2{tile.reference, sum};
+        if (h == 0) *gout<f2>(partial_stats(A, at)) = f2{tile.reference.whole(scale), sum};
         return;
     }
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
                 Tile::store4(to + ES * d, f4{tile.o[b][i] * inverse, tile.o[b][i + 1] * inverse, tile.o[b][i + 2] * inverse,
                                              tile.o[b][i + 3] * inverse});
         }
-    if (h == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[(I.q_row + R.token) * A.heads + R.head] = row_lse(tile.reference, sum);
+    if (h == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[(I.q_row + R.token) * A.heads + R.head] = row_lse(tile.reference.whole(scale), sum);
 }
 
 template <int DT, int NB>

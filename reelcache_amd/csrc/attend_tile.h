@@ -57,6 +57,46 @@ struct Half<RCH_DT_F16> {
 // reference gives the same quotient, and the sums are rarely multiplied.
 constexpr float kSlack = 8.0f;
 
+// A weight's exponent is the score times the scale less the reference, rounded once; the reference is such a product
+// rounded by itself.  The two differ by the product's rounding: 2**-5 at most up to this size.  Farther out that
+// rounding alone would be whole powers of two (32 at 2**30), so a row's scores are taken less their largest first (an
+// exact difference for those that count): every tile of such a row takes the branch that moves references.
+constexpr float kFarScore = 1048576.0f;
+
+// What a row's exponents refer to: (score - shift) * scale - value.  The shift is 0 but for rows far out.
+struct Reference {
+    float value, shift, limit;  // limit: a largest score (scaled, less the bias) above it moves the reference
+
+    __device__ __forceinline__ void init() {
+        value = limit = kNoReference;
+        shift = 0.0f;
+    }
+    // Moves it to a tile's largest score (top: scaled, less the bias), where that is larger.  Returns the factor of the
+    // row's sums.
+    template <typename Scores>
+    __device__ __forceinline__ float move(float largest, float top, float scale, float bias, Scores& s) {
+        float next = fmaxf(value, top), fade = exp2_of(value - next);
+        limit = next + kSlack;
+        const bool out = shift != 0.0f || (__builtin_fabsf(top) > kFarScore && top > value);
+        if (__builtin_expect(__any(out), 0)) {
+            const float to = shift != 0.0f ? fmaxf(shift, largest) : largest;
+            const float far = value == kNoReference ? 1.0f : exp2_of((shift - to) * scale + (value + bias));
+            fade = out ? far : fade;
+            next = out ? -bias : next;
+            limit = out ? -INFINITY : limit;
+            shift = out ? to : 0.0f;
+#pragma unroll
+            for (auto& block : s)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) block[i] -= shift;
+        }
+        value = next;
+        return fade;
+    }
+    // As one number, for a part's partial results and the logarithm of the sum.
+    __device__ __forceinline__ float whole(float scale) const { return shift * scale + value; }
+};
+
 // The larger of the two lanes of a row.
 __device__ __forceinline__ float row_max(float x) {
     const uint32_t u = __float_as_uint(x);
@@ -332,7 +372,8 @@ struct RowTile {
 
     vec8 q[2 * NB];
     f16v o[NB];
-    float reference, sum;
+    Reference reference;
+    float sum;
     // LDS byte offsets within a tile; of wide heads the first, from which the others follow by an exclusive or.
     static constexpr bool kWide = NB > 4;
     uint32_t k_lane[kWide ? 1 : 2 * NB], v_lane[kWide ? 1 : NB];
@@ -353,7 +394,7 @@ struct RowTile {
             if (!kWide || b == 0) v_lane[b] = value_offset(b, lane);
             o[b] = f16v{};
         }
-        reference = kNoReference;
+        reference.init();
         sum = 0.0f;
     }
 
@@ -403,10 +444,10 @@ struct RowTile {
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-        top = row_max(top) * scale - H::kBias;
-        if (__any(top > reference + kSlack)) {
-            const float next = fmaxf(reference, top), fade = exp2_of(reference - next);
-            reference = next;
+        top = row_max(top);
+        const float scaled = top * scale - H::kBias;
+        if (__any(scaled > reference.limit)) {
+            const float fade = reference.move(top, scaled, scale, H::kBias, s);
             sum *= fade;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -419,7 +460,7 @@ struct RowTile {
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float w = exp2_of(__builtin_fmaf(s[b][i], scale, -reference));
+                const float w = exp2_of(__builtin_fmaf(s[b][i], scale, -reference.value));
                 part[i & 3] += w;
                 p[2 * b + (i >> 3)][i & 7] = static_cast<T>(w);
             }
@@ -535,7 +576,8 @@ struct RowTile<RCH_DT_F32, NB, 1> {
 
     f4 q[4 * NB];
     f16v o[NB];
-    float reference, sum;
+    Reference reference;
+    float sum;
     uint32_t k_lane, v_lane, k_turn;
 
     __device__ __forceinline__ void init(const rch_attend& A, const AttendItem& I, const QueryRow& R, int lane) {
@@ -551,7 +593,7 @@ struct RowTile<RCH_DT_F32, NB, 1> {
         v_lane = 4 * h * RB + ((n >> 2) ^ v_swizzle(4 * h)) * 16 + (n & 3) * 4;
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[b] = f16v{};
-        reference = kNoReference;
+        reference.init();
         sum = 0.0f;
     }
 
@@ -559,26 +601,25 @@ struct RowTile<RCH_DT_F32, NB, 1> {
     __device__ __forceinline__ void step(const lds_char* k_tile, const lds_char* v_tile, float scale, int first, int last,
                                          uint64_t held, bool masked, int lane) {
         const int h = lane >> 5;
-        f16v s = f16v{};
+        f16v s[1] = {f16v{}};
 #pragma unroll
         for (int c = 0; c < 4 * NB; ++c) {
             const f4 k = *reinterpret_cast<const __attribute__((address_space(3))) f4*>(k_tile + k_lane + (k_turn ^ (c * 32)));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[c][j], s, 0, 0, 0);
+            for (int j = 0; j < 4; ++j) s[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[j], q[c][j], s[0], 0, 0, 0);
         }
         uint32_t seen[1] = {0xffffu};
         if (masked) {
             seen_keys(seen, first, last, held, h);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = seen[0] >> i & 1u ? s[i] : -INFINITY;
+            for (int i = 0; i < 16; ++i) s[0][i] = seen[0] >> i & 1u ? s[0][i] : -INFINITY;
         }
-        float top = s[0];
+        float top = s[0][0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        top = row_max(top) * scale;
-        if (__any(top > reference + kSlack)) {
-            const float next = fmaxf(reference, top), fade = exp2_of(reference - next);
-            reference = next;
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[0][i]);
+        top = row_max(top);
+        if (__any(top * scale > reference.limit)) {
+            const float fade = reference.move(top, top * scale, scale, 0.0f, s);
             sum *= fade;
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -588,8 +629,8 @@ struct RowTile<RCH_DT_F32, NB, 1> {
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[i] = exp2_of(__builtin_fmaf(s[i], scale, -reference));
-            part[i & 3] += s[i];
+            s[0][i] = exp2_of(__builtin_fmaf(s[0][i], scale, -reference.value));
+            part[i & 3] += s[0][i];
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
         if constexpr (RARE) {
@@ -598,7 +639,7 @@ struct RowTile<RCH_DT_F32, NB, 1> {
 #pragma unroll
                 for (int b = 0; b < NB; ++b) rare.o[b] = o[b];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) rare.p[i] = s[i];
+                for (int i = 0; i < 16; ++i) rare.p[i] = s[0][i];
                 rare.seen = seen[0];
                 add_infinite(&rare, v_tile, v_lane);
 #pragma unroll
@@ -609,7 +650,7 @@ struct RowTile<RCH_DT_F32, NB, 1> {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(v_tile, v_lane, b, i), s[i], o[b], 0, 0, 0);
+            for (int b = 0; b < NB; ++b) o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(value(v_tile, v_lane, b, i), s[0][i], o[b], 0, 0, 0);
     }
 
     // Key 8 (i / 4) + 4 h + i % 4 (its row's swizzle depends on h alone), channel 32 b + lane % 32.

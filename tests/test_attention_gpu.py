@@ -402,3 +402,64 @@ def test_pages_just_below_a_tile(device, dtype, size, layout):
     q = torch.randn((size, 2, 64), generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
     plan = cache.plan([0], queries, heads=2, block=1)
     _check(cache, q, *cache.attend(0, q, plan, return_lse=True), lengths, queries, block=1)
+
+
+FAR = [(128, 64, 700, 150), (64, 16, 300, 1), (96, 100, 400, 33), (200, 64, 300, 40), (20, 16, 200, 3), (128, 64, 9000, 2)]
+
+
+def _uniform_keys(cache, n, numbers, dtype, device):
+    """Keys that hold one number in all their channels; the values of the tokens, float64 on the CPU."""
+    place = torch.arange(n)
+    pages, rows = torch.tensor(cache.pages_of(0))[place // cache.page_tokens].to(device), (place % cache.page_tokens).to(device)
+    cache.keys[0, pages, rows, 0] = numbers[:, None].expand(-1, cache.head_dim).to(dtype).to(device)
+    return cache.values[0, pages, rows, 0].double().cpu()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size,n,queries", FAR)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_far_out(device, dtype, dim, size, n, queries, sign):
+    """Scores of 10^8 and more: the keys that share the largest one share the row; the others, more than 10^6 below it,
+    have no weight, whether they come before or after."""
+    cache = _cache(device, [n], size, 1, dim, dtype)
+    q = torch.full((queries, 2, dim), 8192.0, device=device).to(dtype)
+    generator = torch.Generator().manual_seed(5)
+    for largest in (4096.0, 8192.0, 32768.0):
+        # Steps of a sixteenth, which every type holds: the products and their sums are exact in fp32 too.
+        numbers = sign * largest * (1 - sign * torch.randint(1, 8, (n,), generator=generator).double() / 16)
+        top = torch.randint(0, n, (3,), generator=generator).unique()
+        numbers[top] = sign * largest
+        seen = _uniform_keys(cache, n, numbers, dtype, device)[top]
+        for scale in (dim ** -0.5, 1.0):
+            out, lse = cache.attend(0, q, cache.plan([0], [queries], heads=2, scale=scale), return_lse=True)
+            # One weight for all of them: rounded to the type alike (its sum is not), summed and divided in fp32.
+            want, size_of = seen.mean(0), seen.abs().mean(0)
+            bound = 1.01 * size_of * (oracle.U[dtype] + 8 * oracle.F32) + 1.01 * oracle.U[dtype] * want.abs() + oracle.TINY[dtype]
+            assert oracle.worst(out, want.expand(queries, 2, dim), bound.expand(queries, 2, dim)) <= 0, (largest, scale)
+            # The scale with log2 e, the product and the way back round once each.
+            logs = torch.full((queries, 2), sign * largest * dim * 8192.0 * scale + math.log(len(top)), dtype=torch.float64)
+            assert oracle.worst(lse, logs, 8 * oracle.F32 * (1 + logs.abs())) <= 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size,n,queries", FAR)
+@pytest.mark.parametrize("first", [False, True])
+def test_scores_far_below_others(device, dtype, dim, size, n, queries, first):
+    """Scores of -10^8 and less beside ordinary ones, before or behind them: only those have weights."""
+    cache = _cache(device, [n], size, 1, dim, dtype)
+    q = torch.full((queries, 2, dim), 8192.0, device=device).to(dtype)
+    kept = torch.arange(20) if first else torch.arange(n - 20, n)
+    numbers = torch.full((n,), -8192.0, dtype=torch.float64)
+    numbers[kept] = torch.linspace(-2.0 ** -14, 2.0 ** -14, 20, dtype=torch.float64)
+    values = _uniform_keys(cache, n, numbers, dtype, device)
+    out, lse = cache.attend(0, q, cache.plan([0], [queries], heads=2), return_lse=True)
+    score = numbers[kept].to(dtype).double() * dim * 8192.0 * dim ** -0.5
+    weight, seen = torch.softmax(score, 0), values[kept]
+    # Each score: dim products and sums, the scaling, the shift by the largest; then the exponential and the sums.
+    off = (dim + 8) * oracle.F32 * float(score.abs().max()) + 4 * oracle.F32
+    bound = 1.01 * (weight @ seen.abs()) * (oracle.U[dtype] + 2 * off + 64 * oracle.F32) + 1.01 * oracle.U[dtype] * (weight @ seen).abs() + oracle.TINY[dtype]
+    if dtype == torch.float16:
+        bound = bound + seen.abs().sum(0) * 2.0 ** -31
+    assert oracle.worst(out, (weight @ seen).expand(queries, 2, dim), bound.expand(queries, 2, dim)) <= 0
+    logs = torch.full((queries, 2), float(torch.logsumexp(score, 0)), dtype=torch.float64)
+    assert oracle.worst(lse, logs, 1.01 * off + 64 * oracle.F32 * (1 + logs.abs())) <= 0
