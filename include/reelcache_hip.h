@@ -583,15 +583,16 @@ int rch_runs_store(void* words_dev, const int32_t* runs_host, int n_runs, int64_
  * kv_head * group + r % group.  Query token i of a sequence stands at place p = length - queries + i and
  * sees key j < length if j's page is no hole (an entry outside [0, pages) is one),
  *   block: j < (floor(p / block) + 1) * block      window: j > p - window
- * (0: no such bound).  out = sum softmax(scale q.k) v over what it sees, 0 where it sees nothing; lse is
- * the natural log of the sum of exponentials (-inf where nothing is seen).  K, V rows that a query does
+ * (0: no such bound).  out = sum softmax(scale q.k) v over what it sees, 0 where it sees nothing (NaN
+ * where every score of what it sees is -inf); lse is the natural log of the sum of exponentials (-inf in both).  K, V rows that a query does
  * not see have no influence, whatever they hold.
  *
  * Item: [table (word index of the sequence's first page), length, first query row of q, queries,
  *   row_begin, row_end, kv_head, key_begin, key_end, part (first row of the fp32 partials it writes, or
  *   -1: the output itself), 0, 0]; one with row_begin >= row_end is empty.  Merge: [first query row of q, row_begin, rows, kv_head, first partial
  *   row, parts, 0, 0]: part i of row r is partial row first + i * rows + (r - row_begin).
- * Partials: fp32 [partial_rows, head_dim] sums, then fp32 [partial_rows, 2] of (reference exponent, sum).
+ * Partials: fp32 [partial_rows, head_dim] sums, then fp32 [partial_rows, 2] of (reference exponent, sum; -inf and 0
+ * where every score is -inf).
  */
 #define RCH_ATTEND_ITEM 12
 #define RCH_ATTEND_MERGE 8

@@ -300,7 +300,8 @@ def attend(q, keys, values, plan, *, out=None, return_lse=False):
     are the plan's.  ``keys``, ``values``: one layer of the plan's cache.  ``out``: where to write, of
     q's shape (rows behind the plan's stay as they are); without it a new tensor, zero behind them.
     ``return_lse``: also the fp32 ``[rows, heads]`` natural logs of the sums of exponentials (-inf for a
-    query that sees nothing), by which the results over two caches join.
+    query that sees nothing), by which the results over two caches join.  A query whose scores are all
+    -inf gets NaN, as their softmax has no value (and a log of -inf).
 
     Scores and sums are held in fp32; the output is rounded once.  Runs on the current stream; not
     differentiable.  Returns ``out``, or ``(out, lse)``.

@@ -58,6 +58,29 @@ __device__ __forceinline__ float row_lse(float reference, float sum) {
     return sum == 0.0f ? -INFINITY : __fmul_rn(reference + __builtin_amdgcn_logf(sum), kLn2);
 }
 
+// What a row's weighted sums are multiplied by.  Without a weight: 0 where the row sees no key; where it sees some
+// (blank), every score is -inf, and the quotient has no value.
+__device__ __forceinline__ float row_factor(float sum, bool blank) {
+    return sum != 0.0f ? 1.0f / sum : blank ? __builtin_nanf("") : 0.0f;
+}
+// The reference that a part without a weight leaves: kNoReference, or -inf where it is blank.
+__device__ __forceinline__ float part_reference(float reference, float sum, bool blank) {
+    return sum == 0.0f && blank ? -INFINITY : reference;
+}
+__device__ __forceinline__ bool part_blank(float reference, float sum) { return sum == 0.0f && reference == -INFINITY; }
+
+// Whether a row sees a key of an item's (for rows without a weight).
+__device__ __forceinline__ bool sees_any(const rch_attend& A, const AttendItem& I, int first, int last) {
+    first = first > I.key_begin ? first : I.key_begin;
+    last = last < I.key_end ? last : I.key_end;
+    if (first >= last || !A.holes) return first < last;
+    const int size = static_cast<int>(A.page_tokens);
+    const RCH_GLOBAL int32_t* table = gin<int32_t>(A.plan_ptr) + I.table;
+    for (int page = first / size; page <= (last - 1) / size; ++page)
+        if (table[page] >= 0 && table[page] < A.pages) return true;
+    return false;
+}
+
 __device__ __forceinline__ int64_t partial_sums(const rch_attend& A, int64_t row) {
     return A.partial_ptr + row * A.head_dim * 4;
 }

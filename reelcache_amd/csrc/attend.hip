@@ -42,6 +42,7 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A,
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         float reference = kNoReference, sum = 0.0f, acc[RCH_ATTEND_MAX_DIM / 64];
+        bool blank = false;  // a key was seen
 #pragma unroll
         for (int c = 0; c < RCH_ATTEND_MAX_DIM / 64; ++c) acc[c] = 0.0f;
         for (int base = from; base < to; base += 64) {
@@ -60,6 +61,7 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A,
             }
             uint64_t left = __ballot(seen);
             if (left == 0) continue;
+            blank = true;
             float top = score;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
@@ -92,11 +94,11 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A,
 #pragma unroll
             for (int c = 0; c < RCH_ATTEND_MAX_DIM / 64; ++c)
                 if (lane + 64 * c < dim) gout<float>(partial_sums(A, at))[lane + 64 * c] = acc[c];
-            if (lane == 0) *gout<f2>(partial_stats(A, at)) = f2{reference, sum};
+            if (lane == 0) *gout<f2>(partial_stats(A, at)) = f2{part_reference(reference, sum, blank), sum};
             continue;
         }
         RCH_GLOBAL T* out = gout<T>(A.out_ptr) + (I.q_row + token) * A.out_token_stride + head * A.out_head_stride;
-        const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inverse = row_factor(sum, blank);
 #pragma unroll
         for (int c = 0; c < RCH_ATTEND_MAX_DIM / 64; ++c)
             if (lane + 64 * c < dim) out[lane + 64 * c] = static_cast<T>(acc[c] * inverse);
@@ -135,12 +137,14 @@ __global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_att
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // A wave takes parts wave, wave + W, ..: its own reference, sum and weighted sums.
     float reference = kNoReference, sum = 0.0f, acc[C];
+    bool blank = false;
 #pragma unroll
     for (int c = 0; c < C; ++c) acc[c] = 0.0f;
     for (int base = wave; base < parts; base += 64 * W) {
         const int part = base + W * lane;
         f2 stats = {kNoReference, 0.0f};
         if (part < parts) stats = *gin<f2>(partial_stats(A, first + static_cast<int64_t>(part) * rows));
+        blank = blank || __any(part_blank(stats[0], stats[1]));
         float next = stats[1] != 0.0f ? stats[0] : kNoReference;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) next = fmaxf(next, __shfl_xor(next, o));
@@ -176,15 +180,18 @@ __global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_att
     for (int c = 0; c < C; ++c)
         if (lane + 64 * c < dim) sums[wave][lane + 64 * c] = acc[c];
     if (lane == 0) {
-        stat[wave][0] = reference;
+        stat[wave][0] = part_reference(reference, sum, blank);
         stat[wave][1] = sum;
     }
     __syncthreads();
     const int d = threadIdx.x;
     reference = kNoReference;
+    blank = false;
 #pragma unroll
-    for (int i = 0; i < W; ++i)
+    for (int i = 0; i < W; ++i) {
         if (stat[i][1] != 0.0f) reference = fmaxf(reference, stat[i][0]);
+        blank = blank || part_blank(stat[i][0], stat[i][1]);
+    }
     float value = 0.0f;
     sum = 0.0f;
 #pragma unroll
@@ -194,7 +201,7 @@ __global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_att
         if (d < dim) value = __builtin_fmaf(sums[i][d], fade, value);
     }
     const MergedRow M = merged_row(A, w[0], w[1] + r, w[3]);
-    if (d < dim) gout<T>(A.out_ptr)[M.out + d] = static_cast<T>(value * (sum == 0.0f ? 0.0f : 1.0f / sum));
+    if (d < dim) gout<T>(A.out_ptr)[M.out + d] = static_cast<T>(value * row_factor(sum, blank));
     if (d == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[M.lse] = row_lse(reference, sum);
 }
 
@@ -221,9 +228,12 @@ __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
             high[p] = gin<f4>(partial_sums(A, at) + 4 * d)[1];
         }
     }
+    bool blank = false;
 #pragma unroll
-    for (int p = 0; p < kFewParts; ++p)
+    for (int p = 0; p < kFewParts; ++p) {
         if (p < parts && stats[p][1] != 0.0f) reference = fmaxf(reference, stats[p][0]);
+        blank = blank || (p < parts && part_blank(stats[p][0], stats[p][1]));
+    }
     float sum = 0.0f, acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int p = 0; p < kFewParts; ++p) {
@@ -237,7 +247,7 @@ __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
             }
         }
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inverse = row_factor(sum, blank);
     typedef T t8 __attribute__((ext_vector_type(8)));
     t8 v;
 #pragma unroll

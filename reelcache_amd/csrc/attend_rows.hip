@@ -104,6 +104,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     if (!R.valid) return;
     const int h = lane >> 5, row = I.row_begin + 32 * wave + (lane & 31);
     const float sum = row_sum(tile.sum);
+    const bool blank = sum == 0.0f && sees_any(A, I, R.first, R.last);
     if (I.part >= 0) {
         const int64_t at = I.part + row - I.row_begin;
         const int64_t to = partial_sums(A, at);
@@ -114,10 +115,10 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
                 const int d = Tile::channel_of(b, i, h);
                 if (d < A.head_dim) *gout<f4>(to + 4 * d) = f4{tile.o[b][i], tile.o[b][i + 1], tile.o[b][i + 2], tile.o[b][i + 3]};
             }
-        if (h == 0) *gout<f2>(partial_stats(A, at)) = f2{tile.reference.whole(scale), sum};
+        if (h == 0) *gout<f2>(partial_stats(A, at)) = f2{part_reference(tile.reference.whole(scale), sum, blank), sum};
         return;
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inverse = row_factor(sum, blank);
     const int64_t to = A.out_ptr + ES * ((I.q_row + R.token) * A.out_token_stride + R.head * A.out_head_stride);
 #pragma unroll
     for (int b = 0; b < NB; ++b)

@@ -463,3 +463,39 @@ def test_scores_far_below_others(device, dtype, dim, size, n, queries, first):
     assert oracle.worst(out, (weight @ seen).expand(queries, 2, dim), bound.expand(queries, 2, dim)) <= 0
     logs = torch.full((queries, 2), float(torch.logsumexp(score, 0)), dtype=torch.float64)
     assert oracle.worst(lse, logs, 1.01 * off + 64 * oracle.F32 * (1 + logs.abs())) <= 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size", [(128, 16), (64, 64), (96, 100), (200, 64), (20, 8)])
+@pytest.mark.parametrize("parts", ["one", "few", "many"])
+def test_scores_of_minus_infinity(device, dtype, dim, size, parts):
+    """A query all of whose scores are -inf has no softmax (NaN, and a log of -inf); one that sees nothing has zeros, and
+    one that sees a single finite score has that key's value."""
+    n, queries = {"one": (90, 100), "few": (2400, 2500), "many": (20000, 3)}[parts]
+    block = 1 if parts != "many" else None
+    cache = _cache(device, [n, 2 * size, 5], size, 1, dim, dtype)
+    cache.keys[..., 0] = -math.inf  # of every token, those behind the sequences too
+    lone = cache.pages_of(1)[1], size - 1  # the last key of sequence 1
+    cache.keys[0, lone[0], lone[1], 0] = 0.5
+    q = torch.rand((queries + 3, 2, dim), generator=torch.Generator().manual_seed(1)).add_(0.5).to(dtype).to(device)
+    counts = [queries, 2, 1]
+    out, lse = cache.attend(0, q, cache.plan([0, 1, 2], counts, heads=2, block=block), return_lse=True)
+    hidden = max(0, queries - n) if block else 0
+    assert not out[:hidden].any() and out[hidden:queries].isnan().all() and (lse[:queries] == -math.inf).all()
+    value = cache.values[0, lone[0], lone[1], 0].double().cpu()
+    bound = (oracle.U[dtype] * 2.02 + 8 * oracle.F32) * value.abs() + oracle.TINY[dtype] + (2.0 ** -31 if dtype == torch.float16 else 0.0)
+    sighted = slice(queries + 1, queries + 2) if block else slice(queries, queries + 2)
+    assert oracle.worst(out[sighted], value.expand_as(out[sighted]), bound.expand_as(out[sighted])) <= 0
+    if block:
+        assert out[queries].isnan().all()
+    assert out[queries + 2].isnan().all() and lse[queries + 2].tolist() == [-math.inf] * 2
+    # Behind dropped pages: nothing is seen at all, or only what is left.
+    cache.drop(1, 0, 1)
+    out, lse = cache.attend(0, q[:1], cache.plan([1], [1], heads=2, window=size + 1), return_lse=True)
+    assert oracle.worst(out, value.expand_as(out), bound.expand_as(out)) <= 0
+    cache.keys[0, lone[0], lone[1], 0] = -math.inf
+    out = cache.attend(0, q[:2], cache.plan([1], [2], heads=2))
+    assert out.isnan().all()
+    out, lse = cache.attend(0, q[:size + 2], cache.plan([1], [size + 2], heads=2, block=1), return_lse=True) if queries > size else (None, None)
+    if out is not None:  # the first two stand in the dropped page
+        assert not out[:2].any() and out[2:].isnan().all() and (lse == -math.inf).all()
