@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_att
         const int part = base + W * lane;
         f2 stats = {kNoReference, 0.0f};
         if (part < parts) stats = *gin<f2>(partial_stats(A, first + static_cast<int64_t>(part) * rows));
-        blank = blank || __any(part_blank(stats[0], stats[1]));
+        blank = blank || part_blank(stats[0], stats[1]);
         float next = stats[1] != 0.0f ? stats[0] : kNoReference;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) next = fmaxf(next, __shfl_xor(next, o));
@@ -179,19 +179,17 @@ __global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_att
 #pragma unroll
     for (int c = 0; c < C; ++c)
         if (lane + 64 * c < dim) sums[wave][lane + 64 * c] = acc[c];
+    if (sum == 0.0f) reference = part_reference(reference, sum, __any(blank));
     if (lane == 0) {
-        stat[wave][0] = part_reference(reference, sum, blank);
+        stat[wave][0] = reference;
         stat[wave][1] = sum;
     }
     __syncthreads();
     const int d = threadIdx.x;
     reference = kNoReference;
-    blank = false;
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
+    for (int i = 0; i < W; ++i)
         if (stat[i][1] != 0.0f) reference = fmaxf(reference, stat[i][0]);
-        blank = blank || part_blank(stat[i][0], stat[i][1]);
-    }
     float value = 0.0f;
     sum = 0.0f;
 #pragma unroll
@@ -200,6 +198,9 @@ __global__ void __launch_bounds__(64 * W) attend_merge_many_kernel(const rch_att
         sum = __builtin_fmaf(stat[i][1], fade, sum);
         if (d < dim) value = __builtin_fmaf(sums[i][d], fade, value);
     }
+    blank = false;
+    if (sum == 0.0f)
+        for (int i = 0; i < W; ++i) blank = blank || part_blank(stat[i][0], stat[i][1]);
     const MergedRow M = merged_row(A, w[0], w[1] + r, w[3]);
     if (d < dim) gout<T>(A.out_ptr)[M.out + d] = static_cast<T>(value * row_factor(sum, blank));
     if (d == 0 && A.lse_ptr) gout<float>(A.lse_ptr)[M.lse] = row_lse(reference, sum);
@@ -228,12 +229,9 @@ __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
             high[p] = gin<f4>(partial_sums(A, at) + 4 * d)[1];
         }
     }
-    bool blank = false;
 #pragma unroll
-    for (int p = 0; p < kFewParts; ++p) {
+    for (int p = 0; p < kFewParts; ++p)
         if (p < parts && stats[p][1] != 0.0f) reference = fmaxf(reference, stats[p][0]);
-        blank = blank || (p < parts && part_blank(stats[p][0], stats[p][1]));
-    }
     float sum = 0.0f, acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int p = 0; p < kFewParts; ++p) {
@@ -246,6 +244,11 @@ __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
                 acc[4 + e] = __builtin_fmaf(high[p][e], fade, acc[4 + e]);
             }
         }
+    }
+    bool blank = false;
+    if (sum == 0.0f) {
+#pragma unroll
+        for (int p = 0; p < kFewParts; ++p) blank = blank || (p < parts && part_blank(stats[p][0], stats[p][1]));
     }
     const float inverse = row_factor(sum, blank);
     typedef T t8 __attribute__((ext_vector_type(8)));
