@@ -40,7 +40,8 @@ struct Element<RCH_DT_BF16> {
     typedef __bf16 type;
 };
 
-// N values from / to consecutive elements, in 16- or 8-byte pieces where N * size allows it.
+// N values from / to consecutive elements, in 16- or 8-byte pieces where the width promises their alignment (two
+// fp32 values do not: their rows may start at any element).
 template <typename T, int N>
 struct Piece {
     T v[N];
@@ -54,7 +55,7 @@ __device__ __forceinline__ Piece<T, N> load_piece(const RCH_GLOBAL T* p) {
             const u4 raw = reinterpret_cast<const RCH_GLOBAL u4*>(p)[i];
             __builtin_memcpy(reinterpret_cast<char*>(out.v) + 16 * i, &raw, 16);
         }
-    } else if constexpr (N * sizeof(T) == 8) {
+    } else if constexpr (N == 4 && sizeof(T) == 2) {
         const u2 raw = *reinterpret_cast<const RCH_GLOBAL u2*>(p);
         __builtin_memcpy(out.v, &raw, 8);
     } else {
@@ -72,7 +73,7 @@ __device__ __forceinline__ void store_piece(RCH_GLOBAL T* p, const Piece<T, N>& 
             __builtin_memcpy(&raw, reinterpret_cast<const char*>(in.v) + 16 * i, 16);
             reinterpret_cast<RCH_GLOBAL u4*>(p)[i] = raw;
         }
-    } else if constexpr (N * sizeof(T) == 8) {
+    } else if constexpr (N == 4 && sizeof(T) == 2) {
         u2 raw;
         __builtin_memcpy(&raw, in.v, 8);
         *reinterpret_cast<RCH_GLOBAL u2*>(p) = raw;

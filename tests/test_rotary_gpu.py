@@ -267,3 +267,19 @@ def test_inference_tables_dropped_before_the_backward_pass_are_refused(device):
     table.invalidate()
     with pytest.raises(StateError, match="table was changed"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pairing", rotary.PAIRINGS)
+def test_rows_that_start_at_any_element(device, dtype, pairing):
+    """Inputs and outputs one element off, and head sizes of 4n + 2 channels."""
+    for dim, rotated in ((64, 64), (66, 64), (70, 62)):
+        cos, sin, _ = oracle.tables(50, rotated // 2)
+        positions = rk.RopePositions(rk.RopeTable(cos, sin), 4)
+        size = 2 * 10 * 3 * dim
+        x = torch.empty(size + 1, dtype=dtype, device=device)[1:].view(2, 10, 3, dim).copy_(_normal((2, 10, 3, dim), dtype, device, 7))
+        expected = oracle.rotate(x, cos[4:14, None], sin[4:14, None], pairing)
+        assert oracle.worst(rotary.rotate(x, positions, pairing=pairing), *expected) <= 0
+        out = torch.empty(size + 3, dtype=dtype, device=device)[3:].view(2, 10, 3, dim)
+        rotary.rotate(x, positions, pairing=pairing, out=out)
+        assert oracle.worst(out, *expected) <= 0
