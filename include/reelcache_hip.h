@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define RCH_ABI_VERSION 22
+#define RCH_ABI_VERSION 23
 
 /* Status codes (mapped to reelcache errors by the host). */
 #define RCH_OK 0
@@ -591,8 +591,8 @@ int rch_runs_store(void* words_dev, const int32_t* runs_host, int n_runs, int64_
  *   row_begin, row_end, kv_head, key_begin, key_end, part (first row of the fp32 partials it writes, or
  *   -1: the output itself), 0, 0]; one with row_begin >= row_end is empty.  Merge: [first query row of q, row_begin, rows, kv_head, first partial
  *   row, parts, 0, 0]: part i of row r is partial row first + i * rows + (r - row_begin).
- * Partials: fp32 [partial_rows, head_dim] sums, then fp32 [partial_rows, 2] of (reference exponent, sum; -inf and 0
- * where every score is -inf).
+ * Partials (16-byte aligned): fp32 [partial_rows, head_dim] sums, then, from an even word on, fp32
+ * [partial_rows, 2] of (reference exponent, sum; -inf and 0 where every score is -inf).
  */
 #define RCH_ATTEND_ITEM 12
 #define RCH_ATTEND_MERGE 8

@@ -349,7 +349,7 @@ def run(q, k_address, v_address, plan, out, return_lse, pools=None):
             fields = _Image.from_buffer_copy(image)
             partials = None
             if plan._n_merges:
-                partials = torch.empty(plan._partial_rows * (cache.head_dim + 2), dtype=torch.float32, device=device)
+                partials = torch.empty(plan._partial_rows * (cache.head_dim + 2) + 1, dtype=torch.float32, device=device)
                 fields[6] = partials.data_ptr()
             stream = raw_stream(device)
             if stream != plan._stream:  # the allocator learns of a stream that the tables were not made on

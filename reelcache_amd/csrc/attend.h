@@ -85,7 +85,7 @@ __device__ __forceinline__ int64_t partial_sums(const rch_attend& A, int64_t row
     return A.partial_ptr + row * A.head_dim * 4;
 }
 __device__ __forceinline__ int64_t partial_stats(const rch_attend& A, int64_t row) {
-    return A.partial_ptr + A.partial_rows * A.head_dim * 4 + row * 8;
+    return A.partial_ptr + (A.partial_rows * A.head_dim + 1) / 2 * 8 + row * 8;
 }
 
 // Launches the items of the tiled form.

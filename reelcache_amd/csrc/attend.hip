@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(256) attend_merge_kernel(const rch_attend A) {
         for (int p = 0; p < kFewParts; ++p) blank = blank || (p < parts && part_blank(stats[p][0], stats[p][1]));
     }
     const float inverse = row_factor(sum, blank);
-    typedef T t8 __attribute__((ext_vector_type(8)));
+    typedef T t8 __attribute__((ext_vector_type(8), aligned(16)));
     t8 v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = static_cast<T>(acc[e] * inverse);
@@ -312,7 +312,7 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid sizes");
     if (A.n_general < 0 || A.n_rows < 0 || A.n_merges < 0 || A.n_general + A.n_rows > 0x7fffffff)
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid item counts");
-    if (A.n_merges && (!A.partial_ptr || A.n_many < 0 || A.n_many > A.n_merges || A.most_rows < 0 || A.most_rows_many < 0
+    if (A.n_merges && (!A.partial_ptr || A.partial_ptr % 16 || A.n_many < 0 || A.n_many > A.n_merges || A.most_rows < 0 || A.most_rows_many < 0
                        || A.most_rows_many > 65535))
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid merges");
     // Rows of few parts are joined in aligned pieces of eight channels.

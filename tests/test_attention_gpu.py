@@ -499,3 +499,12 @@ def test_scores_of_minus_infinity(device, dtype, dim, size, parts):
     out, lse = cache.attend(0, q[:size + 2], cache.plan([1], [size + 2], heads=2, block=1), return_lse=True) if queries > size else (None, None)
     if out is not None:  # the first two stand in the dropped page
         assert not out[:2].any() and out[2:].isnan().all() and (lse == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,group", [(7, 1), (33, 3), (129, 1)])
+def test_odd_heads_in_odd_parts(device, dtype, dim, group):
+    """Partial rows of an odd number of words, and an odd number of them."""
+    for n in (3000, 3200, 3400):
+        _, _, plan, _ = _run(device, [n], [1], 16, 1, group, dim, dtype)
+        assert plan._n_merges

@@ -564,3 +564,15 @@ def test_attention_refuses_pools_that_require_gradients(host, which):
         attention.attend(torch.zeros(1, 2, 8), *pools, plan)
     with torch.no_grad():
         plan._check(*pools)
+
+
+def test_partial_results_are_aligned():
+    """The statistics of partial rows are pairs of words at even ones, whatever the head size."""
+    import ctypes
+
+    step = dict(group=1, heads=1, head_dim=7, page_tokens=4, pages=1, n_general=1, n_merges=1, n_many=1, most_rows_many=1,
+                partial_rows=3, scale_bits=0x3f800000, q_ptr=64, k_ptr=64, v_ptr=64, out_ptr=64, plan_ptr=64)
+    for address in (0, 4, 8):
+        with pytest.raises(ConfigurationError, match="merges"):
+            _lib.call("rch_attend_run", (ctypes.c_int64 * len(_lib.ATTEND_FIELDS))(
+                *({**step, "partial_ptr": 1024 + address if address else 0}.get(f, 0) for f in _lib.ATTEND_FIELDS)), 0, None)
