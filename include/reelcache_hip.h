@@ -612,7 +612,7 @@ typedef struct rch_attend {
     int64_t scale_bits;      /* fp32 bits of scale * log2(e), a positive normal number */
     int64_t partial_rows;
     int64_t items;           /* word index of the first item */
-    int64_t n_general, n_rows; /* items of the general and of the tiled form, in order */
+    int64_t n_general, n_rows; /* items, of the general or of the tiled form (the other is 0) */
     int64_t merges, n_merges;      /* word index and count */
     int64_t n_many;                /* the first ones, which take a workgroup to a row: all merges of more than
                                       RCH_ATTEND_FEW_PARTS parts, or of rows that are no aligned multiples of

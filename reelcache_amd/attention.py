@@ -44,7 +44,7 @@ _LEAST_SCALE, _MOST_SCALE = 2.0 ** -126, 2.0 ** 127
 
 
 class _Work:
-    """The row blocks of one form: parallel int64 arrays, one entry per (sequence, key head, row block)."""
+    """The row blocks of a step: parallel int64 arrays, one entry per (sequence, key head, row block)."""
 
     def __init__(self):
         self.parts = []
@@ -124,7 +124,8 @@ class AttentionPlan:
 
         return keys
 
-    def _form(self, rows):
+    def _form(self):
+        """The kernels that take the cache: "rows", which tile for the matrix cores, or "general"."""
         cache = self.cache
         size = cache.keys.element_size()
         aligned = all(pool.data_ptr() % 16 == 0 and all(pool.stride(a) * size % 16 == 0 for a in range(4))
@@ -137,8 +138,8 @@ class AttentionPlan:
 
     def _lay_out(self, found, queries):
         cache = self.cache
-        work = {name: _Work() for name in _OVERHEAD}
-        tiles = {"general": GENERAL_ROWS, "rows": ROW_TILE}
+        form, work = self._form(), _Work()
+        tile = ROW_TILE if form == "rows" else GENERAL_ROWS
         table, at, lengths, starts = [], [], [], []
         words, row = _lib.ATTEND_ZEROS, 0
         for number, (item, n) in enumerate(zip(found, queries)):
@@ -149,24 +150,19 @@ class AttentionPlan:
             words += len(item.pages)
             row += n
             if n:
-                form = self._form(n * self.group)
-                work[form].add(number, cache.heads, n * self.group, tiles[form], self._keys_of(item.tokens, n))
+                work.add(number, cache.heads, n * self.group, tile, self._keys_of(item.tokens, n))
         need(words < 1 << 30, "the step's page tables are too large")
         self._at = np.asarray(at, dtype=np.int64)
         self._lengths, self._starts = np.asarray(lengths, dtype=np.int64), np.asarray(starts, dtype=np.int64)
         self._counts = np.asarray(queries, dtype=np.int64)
-        items, merges, self._partial_rows, counts = [], [], 0, {}
-        for form in ("general", "rows"):
-            made = self._split(form, work[form].rows(), merges)
-            counts[form] = len(made)
-            items.append(made)
-        items = np.concatenate(items)
+        merges, self._partial_rows = [], 0
+        items = self._split(form, work.rows(), merges)
         merges = np.concatenate(merges) if merges else np.empty((0, _lib.ATTEND_MERGE), np.int64)
-        self._counts_of = (counts["general"], counts["rows"])
+        self._counts_of = (0, len(items)) if form == "rows" else (len(items), 0)
         first_item = _lib.ATTEND_ZEROS + len(table)
         self._items, self._merges = first_item, first_item + items.size
         # Merges that take a workgroup to a row come first (the kernels' rule).
-        joined = counts["general"] == 0 and cache.head_dim % 8 == 0
+        joined = form == "rows" and cache.head_dim % 8 == 0
         many = (merges[:, 5] > _lib.ATTEND_FEW_PARTS) | (not joined)
         if len(merges) * merges[:, 2].max(initial=0) <= _FEW_ROWS:
             many[:] = True
@@ -179,7 +175,7 @@ class AttentionPlan:
                                 merges.ravel()])
         from .paged_cache import upload
 
-        self._tiled = counts["rows"]
+        self._tiled = self._counts_of[1]
         with entered(cache.device):
             self.buffer = upload(words, cache.device)
             self._stream = raw_stream(cache.device)

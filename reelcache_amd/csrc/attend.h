@@ -89,6 +89,6 @@ __device__ __forceinline__ int64_t partial_stats(const rch_attend& A, int64_t ro
 }
 
 // Launches the items of the tiled form.
-int launch_attend_rows(const rch_attend& A, int dtype, int first, hipStream_t stream);
+int launch_attend_rows(const rch_attend& A, int dtype, hipStream_t stream);
 
 }  // namespace rch

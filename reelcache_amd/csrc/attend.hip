@@ -9,8 +9,8 @@
 // The general form takes every head_dim up to 256, alignment and element type: one wave per row, a
 // lane per key for the scores, a lane per channel for the sums.  Bound by the latency of its loads, element
 // by element: single tokens of 4 sequences of 4000 tokens, 16 heads of 250 bf16, take 450 us (0.57 TB/s).  Only
-// pools, or head sizes, whose rows are no 16-byte pieces come here; the form that tiles for the matrix cores
-// (16 heads of 200: 80 us) is in attend_rows.hip.
+// pools, or head sizes, whose rows are no 16-byte pieces come here, and pools whose token rows lie more than 2^22
+// elements apart; the form that tiles for the matrix cores (16 heads of 200: 80 us) is in attend_rows.hip.
 #include "attend.h"
 
 namespace rch {
@@ -18,13 +18,13 @@ namespace rch {
 namespace {
 
 template <int DT>
-__global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A, int first_item) {
+__global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A) {
     typedef typename AttendType<DT>::type T;
     __shared__ float query[4][RCH_ATTEND_MAX_DIM];
     __shared__ float weight[4][64];
     __shared__ int64_t place_of[4][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const AttendItem I = attend_item(A, first_item + blockIdx.x);
+    const AttendItem I = attend_item(A, blockIdx.x);
     const int dim = static_cast<int>(A.head_dim), group = static_cast<int>(A.group);
     const float scale = __int_as_float(static_cast<int>(A.scale_bits));
     const int size = static_cast<int>(A.page_tokens);
@@ -276,17 +276,9 @@ int merge_few(const rch_attend& A, hipStream_t stream) {
 
 template <int DT>
 int run(const rch_attend& A, hipStream_t stream) {
-    int first = 0;
-    if (A.n_general) {
-        hipLaunchKernelGGL(attend_general_kernel<DT>, dim3(static_cast<uint32_t>(A.n_general)), dim3(256), 0, stream, A, first);
-        const int status = check_launch("rch_attend_run");
-        if (status != RCH_OK) return status;
-        first += static_cast<int>(A.n_general);
-    }
-    if (A.n_rows) {
-        const int status = launch_attend_rows(A, DT, first, stream);
-        if (status != RCH_OK) return status;
-    }
+    if (A.n_general) hipLaunchKernelGGL(attend_general_kernel<DT>, dim3(static_cast<uint32_t>(A.n_general)), dim3(256), 0, stream, A);
+    const int status = A.n_general ? check_launch("rch_attend_run") : launch_attend_rows(A, DT, stream);
+    if (status != RCH_OK) return status;
     if (A.n_many) {
         const int status = A.head_dim <= 128 ? merge_many<DT, 2>(A, stream) : merge_many<DT, 4>(A, stream);
         if (status != RCH_OK) return status;
@@ -310,7 +302,8 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
     if (A.group < 1 || A.heads < 1 || A.head_dim < 1 || A.head_dim > RCH_ATTEND_MAX_DIM || A.page_tokens < 1 || A.pages < 1
         || A.page_tokens > 0x7fffffff || A.pages > 0x7fffffff || A.block < 0 || A.window < 0 || A.block > 0x7fffffff)
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid sizes");
-    if (A.n_general < 0 || A.n_rows < 0 || A.n_merges < 0 || A.n_general + A.n_rows > 0x7fffffff)
+    if (A.n_general < 0 || A.n_rows < 0 || A.n_merges < 0 || (A.n_general && A.n_rows)
+        || A.n_general + A.n_rows > 0x7fffffff)
         return fail(RCH_E_CONFIG, "rch_attend_run: invalid item counts");
     if (A.n_merges && (!A.partial_ptr || A.partial_ptr % 16 || A.n_many < 0 || A.n_many > A.n_merges || A.most_rows < 0 || A.most_rows_many < 0
                        || A.most_rows_many > 65535))

@@ -20,14 +20,14 @@ namespace rch {
 namespace {
 
 template <int DT, int NB, int MODE>
-__global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_rows_kernel(const rch_attend A, int first_item) {
+__global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_rows_kernel(const rch_attend A) {
     typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2> Tile;
     constexpr int KT = Tile::KT, ES = Tile::ES, kTileBytes = KT * Tile::RB;
     constexpr int kStageBytes = 2 * kTileBytes;
     __shared__ __attribute__((aligned(1024))) char lds[2 * kStageBytes];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const AttendItem I = attend_item(A, first_item + blockIdx.x);
+    const AttendItem I = attend_item(A, blockIdx.x);
     if (I.row_begin >= I.row_end) return;  // a plan's filling
     const QueryRow R = query_row(A, I, I.row_begin + 32 * wave + (lane & 31));
     const float scale = __int_as_float(static_cast<int>(A.scale_bits));
@@ -133,29 +133,29 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
 }
 
 template <int DT, int NB>
-void launch(const rch_attend& A, int first, hipStream_t stream) {
+void launch(const rch_attend& A, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(A.n_rows));
     constexpr int kShareRows = RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2>::KT / 4;
-    if (A.tile_unit == A.page_tokens) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kPage>), grid, dim3(256), 0, stream, A, first);
-    else if (A.page_tokens % kShareRows == 0) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kShare>), grid, dim3(256), 0, stream, A, first);
-    else hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kRow>), grid, dim3(256), 0, stream, A, first);
+    if (A.tile_unit == A.page_tokens) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kPage>), grid, dim3(256), 0, stream, A);
+    else if (A.page_tokens % kShareRows == 0) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kShare>), grid, dim3(256), 0, stream, A);
+    else hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kRow>), grid, dim3(256), 0, stream, A);
 }
 
 template <int DT>
-void launch_dim(const rch_attend& A, int first, hipStream_t stream) {
-    if (A.head_dim <= 64) launch<DT, 2>(A, first, stream);
-    else if (A.head_dim <= 96) launch<DT, 3>(A, first, stream);
-    else if (A.head_dim <= 128) launch<DT, 4>(A, first, stream);
-    else if (A.head_dim <= 192) launch<DT, 6>(A, first, stream);
-    else launch<DT, 8>(A, first, stream);
+void launch_dim(const rch_attend& A, hipStream_t stream) {
+    if (A.head_dim <= 64) launch<DT, 2>(A, stream);
+    else if (A.head_dim <= 96) launch<DT, 3>(A, stream);
+    else if (A.head_dim <= 128) launch<DT, 4>(A, stream);
+    else if (A.head_dim <= 192) launch<DT, 6>(A, stream);
+    else launch<DT, 8>(A, stream);
 }
 
 }  // namespace
 
-int launch_attend_rows(const rch_attend& A, int dtype, int first, hipStream_t stream) {
-    if (dtype == RCH_DT_F16) launch_dim<RCH_DT_F16>(A, first, stream);
-    else if (dtype == RCH_DT_F32) launch_dim<RCH_DT_F32>(A, first, stream);
-    else launch_dim<RCH_DT_BF16>(A, first, stream);
+int launch_attend_rows(const rch_attend& A, int dtype, hipStream_t stream) {
+    if (dtype == RCH_DT_F16) launch_dim<RCH_DT_F16>(A, stream);
+    else if (dtype == RCH_DT_F32) launch_dim<RCH_DT_F32>(A, stream);
+    else launch_dim<RCH_DT_BF16>(A, stream);
     return check_launch("rch_attend_run (rows)");
 }
 

@@ -576,3 +576,18 @@ def test_partial_results_are_aligned():
         with pytest.raises(ConfigurationError, match="merges"):
             _lib.call("rch_attend_run", (ctypes.c_int64 * len(_lib.ATTEND_FIELDS))(
                 *({**step, "partial_ptr": 1024 + address if address else 0}.get(f, 0) for f in _lib.ATTEND_FIELDS)), 0, None)
+
+
+def test_a_step_has_items_of_one_form(host):
+    """The cache alone says which kernels take it, and a launch of both is refused."""
+    import ctypes
+
+    for dim, dtype, tiled in ((64, torch.bfloat16, True), (20, torch.bfloat16, False), (20, torch.float32, True), (7, torch.float32, False)):
+        cache = make(pages=40, dim=dim, dtype=dtype, layers=1)
+        sequences = [cache.new(), cache.new()]
+        cache.extend(sequences, [9, 100])
+        general, rows = cache.plan(sequences, [1, 90], heads=2)._counts_of
+        assert (rows > 0 and general == 0) if tiled else (general > 0 and rows == 0)
+    step = dict(group=1, heads=1, head_dim=8, page_tokens=4, pages=1, n_general=1, n_rows=1)
+    with pytest.raises(ConfigurationError, match="item counts"):
+        _lib.call("rch_attend_run", (ctypes.c_int64 * len(_lib.ATTEND_FIELDS))(*(step.get(f, 0) for f in _lib.ATTEND_FIELDS)), 0, None)
