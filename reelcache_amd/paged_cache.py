@@ -32,7 +32,7 @@ from . import _lib
 from ._checks import count, in_memory, need, one_of
 from .errors import CapacityError, ConfigurationError, StateError, UnsupportedError
 from .restore_model import OUTPUT_DTYPES, NativeView
-from .rotary import Launch, addresses_of, capturing, entered, known_calls, need_gpu, position_fields, raw_stream
+from .rotary import Launch, _span, addresses_of, capturing, entered, known_calls, need_gpu, position_fields, raw_stream
 
 HOLE = -1
 _LAYOUTS = ("BTHD", "BHTD")
@@ -132,6 +132,9 @@ class PagedCache:
         need(self.pages * self.page_tokens < 1 << 31, "a pool holds fewer than 2**31 tokens")
         self.device, self.dtype = keys.device, keys.dtype
         self._axes = (1, token, head)
+        self._layer_bytes = tuple(pool.stride(0) * pool.element_size() for pool in (keys, values))
+        # Bytes from a layer's first element to behind its last.
+        self._reach = tuple(_reach(pool[0]) for pool in (keys, values))
         self._geometry = (layout, keys.shape[1:], keys.stride()[1:], values.stride()[1:], keys.dtype, keys.device)
         self._sequences: dict[int, _Sequence] = {}
         self._next = 0
@@ -482,8 +485,8 @@ class PagedCache:
     def store(self, layer, slots, keys, values, *, positions=None, grid=None):
         """Write new tokens into their slots: ``keys`` turned by ``positions`` (interleaved pairs, as
         :func:`reelcache_amd.rotary.rotate`; ``None`` stores them as they are) and ``values``, both
-        ``[tokens, heads, head_dim]`` of the cache's dtype, any strides.  With a ``grid`` the tokens are
-        one chunk."""
+        ``[tokens, heads, head_dim]`` of the cache's dtype, any strides (rows of the pools themselves are
+        copied first).  With a ``grid`` the tokens are one chunk."""
         if type(layer) is not int or not 0 <= layer < self.layers:
             raise ConfigurationError("there is no such layer")
         if not isinstance(slots, Slots) or slots.cache is not self:
@@ -505,13 +508,20 @@ class PagedCache:
             sources = [x if x.stride(2) == 1 or self.head_dim == 1 else x.contiguous() for x in (keys, values)]
             known = known_calls(slots if positions is None else positions)
             key = (slots.tokens, grid, self._geometry, *[x.stride() for x in sources])
-            launch = known.get(key)
-            if launch is None:
-                launch = known[key] = self._store_launch(sources, positions, grid, slots.tokens)
+            call = known.get(key)
+            if call is None:
+                call = known[key] = (self._store_launch(sources, positions, grid, slots.tokens), *map(_reach, sources))
+            launch, *reach = call
             stream = raw_stream(self.device)
-            step = layer * self.keys.element_size()
-            pools = [pool.data_ptr() + step * pool.stride(0) for pool in (self.keys, self.values)]
-            launch([(sources[0].data_ptr(), pools[0], True), (sources[1].data_ptr(), pools[1], False)],
+            k_bytes, v_bytes = self._layer_bytes
+            pools = [self.keys.data_ptr() + layer * k_bytes, self.values.data_ptr() + layer * v_bytes]
+            k, v = sources[0].data_ptr(), sources[1].data_ptr()
+            for pool, room in zip(pools, self._reach):
+                if (k < pool + room and pool < k + reach[0]) or (v < pool + room and pool < v + reach[1]):
+                    # Rows of the pool itself, which are written while others are still read: of copies.
+                    return self.store(layer, slots, *[x.clone(memory_format=torch.contiguous_format) for x in (keys, values)],
+                                      positions=positions, grid=grid)
+            launch([(k, pools[0], True), (v, pools[1], False)],
                    *addresses_of(positions, self.device, stream), slots.index.data_ptr(), stream)
             if stream != slots.stream:  # the allocator learns of a stream that the index was not made on
                 slots.index.record_stream(torch.cuda.current_stream(self.device))
@@ -544,9 +554,8 @@ class PagedCache:
             raise ConfigurationError("there is no such layer")
         if not isinstance(plan, AttentionPlan) or plan.cache is not self:
             return attend(q, *self._layer(layer), plan, out=out, return_lse=return_lse)
-        step = layer * self.keys.element_size()
-        return run(q, self.keys.data_ptr() + step * self.keys.stride(0), self.values.data_ptr() + step * self.values.stride(0),
-                   plan, out, return_lse)
+        k_bytes, v_bytes = self._layer_bytes
+        return run(q, self.keys.data_ptr() + layer * k_bytes, self.values.data_ptr() + layer * v_bytes, plan, out, return_lse)
 
 
 def _apart(pool):
@@ -558,6 +567,12 @@ def _apart(pool):
             return False
         reach = stride * (size - 1) + reach
     return True
+
+
+def _reach(x):
+    """Bytes from a strided tensor's first element to behind its last."""
+    low, high = _span(x)
+    return high - low
 
 
 def _pools(group, axes, pages, page_tokens):

@@ -591,3 +591,29 @@ def test_a_step_has_items_of_one_form(host):
     step = dict(group=1, heads=1, head_dim=8, page_tokens=4, pages=1, n_general=1, n_rows=1)
     with pytest.raises(ConfigurationError, match="item counts"):
         _lib.call("rch_attend_run", (ctypes.c_int64 * len(_lib.ATTEND_FIELDS))(*(step.get(f, 0) for f in _lib.ATTEND_FIELDS)), 0, None)
+
+
+def test_rows_of_the_pools_are_copied_before_a_store(host, monkeypatch):
+    """Sources in the memory that a store writes are read whole first; sources elsewhere are read where they are."""
+    launches = []
+    monkeypatch.setattr(rotary.Launch, "__call__", lambda self, addresses, *rest: launches.append(
+        (addresses, np.frombuffer(self.image, np.int64).reshape(2, -1)[:, 8].tolist())))
+    cache = make()
+    a = cache.new()
+    slots = cache.extend([a], [6])
+    x, y = torch.zeros(6, 2, 8), torch.zeros(6, 2, 16)[..., :8]
+    cache.store(1, slots, x, y)
+    (((k, _, _), (v, _, _)), strides), = launches
+    assert (k, v) == (x.data_ptr(), y.data_ptr()) and strides == [16, 32]
+    rows = [pool[1].flatten(0, 1)[3:9] for pool in (cache.keys, cache.values)]
+    size = cache.keys[1].numel() * 4
+    inside = lambda at: any(pool[1].data_ptr() <= at < pool[1].data_ptr() + size for pool in (cache.keys, cache.values))
+    for keys, values in ((rows[0], y), (x, rows[1]), (rows[1], y), (x, rows[0]), tuple(rows)):
+        launches.clear()
+        cache.store(1, slots, keys, values)
+        (((k, to_k, _), (v, to_v, _)), _), = launches
+        assert not inside(k) and not inside(v)
+        assert (to_k, to_v) == (cache.keys[1].data_ptr(), cache.values[1].data_ptr())
+    launches.clear()
+    cache.store(0, slots, *rows)  # another layer's rows are not written
+    assert launches[0][0][0][0] == rows[0].data_ptr()

@@ -222,3 +222,24 @@ def test_captured_store_and_copies(device):
         turned = rotary.rotate(k, positions, layout="THD")
         expected[1, 0], expected[1, 1, :2] = turned[:4], turned[4:]
         assert torch.equal(keys, expected)
+
+
+@pytest.mark.parametrize("layout", ["BTHD", "BHTD"])
+def test_store_of_rows_of_the_pool(device, layout):
+    """Tokens moved within a layer's pool: every row is read before any is written."""
+    keys, values = _pools(device, 2, 40, 64, 3, 64, torch.bfloat16, layout)
+    cache = paged_cache.PagedCache(keys, values, layout=layout)
+    cache.load_tables([(list(range(40)), 2560)])
+    if layout == "BTHD":  # a step of one token
+        slots = cache.slots([0], [1], [2559])
+        sources = [pool[1].flatten(0, 1)[:2559] for pool in (keys, values)]
+    else:  # a token of every page
+        slots = cache.slots([0], [0], [40])
+        sources = [pool[1, :, :, 5] for pool in (keys, values)]
+    before = [pool.clone() for pool in (keys, values)]
+    given = [x.clone() for x in sources]
+    cache.store(1, slots, *sources)
+    at = slots.index.long()
+    for pool, want, x in zip((keys, values), before, given):
+        _token_major(want, layout)[1, at // 64, at % 64] = x
+        assert torch.equal(pool, want)
