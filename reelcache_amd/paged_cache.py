@@ -133,6 +133,8 @@ class PagedCache:
         self.device, self.dtype = keys.device, keys.dtype
         self._axes = (1, token, head)
         self._layer_bytes = tuple(pool.stride(0) * pool.element_size() for pool in (keys, values))
+        # What autograd may have saved (inference tensors count no updates).
+        self._counted = tuple(pool for pool in (keys, values) if not pool.is_inference())
         # Bytes from a layer's first element to behind its last.
         self._reach = tuple(_reach(pool[0]) for pool in (keys, values))
         self._geometry = (layout, keys.shape[1:], keys.stride()[1:], values.stride()[1:], keys.dtype, keys.device)
@@ -364,6 +366,7 @@ class PagedCache:
                     pools.record_stream(torch.cuda.current_stream(self.device))
                     streams.add(stream)
                 _lib.check(_lib.function("rch_pages_copy")(fields, table, len(moves) // 3, stream))
+            torch.autograd.graph.increment_version(self._counted)
 
     def _joined_pools(self):
         """K and V pools as one group where their strides agree (one launch), else as two."""
@@ -483,7 +486,7 @@ class PagedCache:
         return NativeView(flat, "THD", pages[0] * self.page_tokens + offset)
 
     def store(self, layer, slots, keys, values, *, positions=None, grid=None):
-        """Write new tokens into their slots: ``keys`` turned by ``positions`` (interleaved pairs, as
+        """Write new tokens into their slots (a backward pass that saved a pool notices): ``keys`` turned by ``positions`` (interleaved pairs, as
         :func:`reelcache_amd.rotary.rotate`; ``None`` stores them as they are) and ``values``, both
         ``[tokens, heads, head_dim]`` of the cache's dtype, any strides (rows of the pools themselves are
         copied first).  With a ``grid`` the tokens are one chunk."""
@@ -525,6 +528,7 @@ class PagedCache:
                    *addresses_of(positions, self.device, stream), slots.index.data_ptr(), stream)
             if stream != slots.stream:  # the allocator learns of a stream that the index was not made on
                 slots.index.record_stream(torch.cuda.current_stream(self.device))
+            torch.autograd.graph.increment_version(self._counted)
 
     def _store_launch(self, sources, positions, grid, tokens):
         turned = position_fields(positions, grid, tokens, 1, self.head_dim, self.device)

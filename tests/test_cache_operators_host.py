@@ -617,3 +617,20 @@ def test_rows_of_the_pools_are_copied_before_a_store(host, monkeypatch):
     launches.clear()
     cache.store(0, slots, *rows)  # another layer's rows are not written
     assert launches[0][0][0][0] == rows[0].data_ptr()
+
+
+def test_stores_and_copies_count_as_updates_of_the_pools(host, monkeypatch):
+    """A backward pass that saved a pool notices what was written into it since."""
+    monkeypatch.setattr(rotary.Launch, "__call__", lambda self, addresses, *rest: None)
+    x = torch.zeros(1, 2, 8)
+    with torch.inference_mode():  # pools that count nothing
+        cache = make()
+        cache.store(0, cache.extend([cache.new()], [1]), x, x)
+    cache = make()
+    slots = cache.extend([cache.new()], [1])
+    weight = torch.ones(1, requires_grad=True)
+    for pool in (cache.keys, cache.values):
+        product = (weight * pool).sum()
+        cache.store(0, slots, x, x)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            product.backward()

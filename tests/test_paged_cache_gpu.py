@@ -243,3 +243,24 @@ def test_store_of_rows_of_the_pool(device, layout):
     for pool, want, x in zip((keys, values), before, given):
         _token_major(want, layout)[1, at // 64, at % 64] = x
         assert torch.equal(pool, want)
+
+
+def test_pools_that_autograd_saved(device):
+    """A backward pass that saved a pool notices stores and page copies."""
+    cache = paged_cache.PagedCache.allocate(6, 4, 2, 8, device=device)
+    cache.keys.normal_(), cache.values.normal_()
+    a = cache.new()
+    slots = cache.extend([a], [6])
+    x = torch.ones(6, 2, 8, dtype=torch.bfloat16, device=device)
+    weight = torch.ones(1, device=device, requires_grad=True)
+
+    def go_on():
+        cache.extend([cache.fork(a)], [1])
+
+    for pool in (cache.keys, cache.values):
+        for change in (lambda: cache.store(0, cache.slots([a], [0], [6]), x, x), go_on):
+            product = (weight * pool).sum()
+            change()
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                product.backward()
+        cache.load_tables([([0, 1], 6)])
