@@ -272,24 +272,36 @@ class PagedCache:
             self._need_copies()
         if total > len(free):
             raise CapacityError(f"{total} pages are needed and {len(free)} are free")
-        moves, starts = [], []
-        for item, n, (begun, more) in zip(found, counts, wanted):
-            pages = item.pages
-            if begun:
-                page = heapq.heappop(free)
-                in_use[page] = 1
-                in_use[pages[-1]] -= 1
-                moves += (pages[-1], page, begun)
-                pages[-1] = page
-                self._shared += 1
-            for _ in range(more):
-                page = heapq.heappop(free)
-                in_use[page] = 1
-                pages.append(page)
-            starts.append(item.tokens)
-            item.tokens += n
-        self._copy(moves)
-        return self._slots(found, starts, counts)
+        moves, starts, stamp = [], [], self._shared
+        try:
+            for item, n, (begun, more) in zip(found, counts, wanted):
+                pages = item.pages
+                if begun:
+                    page = heapq.heappop(free)
+                    in_use[page] = 1
+                    in_use[pages[-1]] -= 1
+                    moves += (pages[-1], page, begun)
+                    pages[-1] = page
+                    self._shared += 1
+                for _ in range(more):
+                    page = heapq.heappop(free)
+                    in_use[page] = 1
+                    pages.append(page)
+                starts.append(item.tokens)
+                item.tokens += n
+            self._copy(moves)
+            return self._slots(found, starts, counts)
+        except BaseException:  # no memory, or no launch: as if it had not been called
+            shared = moves[::3]
+            for item, tokens, (begun, more) in zip(found, starts, wanted):
+                pages, item.tokens = item.pages, tokens
+                self._release(pages[len(pages) - more - (begun > 0):])
+                del pages[len(pages) - more:]
+                if begun:
+                    pages[-1] = shared.pop(0)
+                    in_use[pages[-1]] += 1
+            self._shared = stamp
+            raise
 
     def slots(self, sequences, starts, counts):
         """The :class:`Slots` of tokens ``starts[i] .. starts[i] + counts[i]`` that ``sequences[i]`` has
@@ -404,9 +416,9 @@ class PagedCache:
         need_gpu(self.device, "a paged cache")
         _refuse_capture(self.device)
         self._need_copies()
-        moves, size, uses, names = [], self.page_tokens, self._uses, {}
+        size, uses, names = self.page_tokens, self._uses, {}
+        self._copy([word for a, b in zip(source, target) for word in (a, b, size)])  # where it fails, nothing has changed
         for a, b in zip(source, target):
-            moves += (a, b, size)
             uses[b], uses[a] = uses[a], 0
             names[a] = b
         for item in self._sequences.values():
@@ -416,7 +428,6 @@ class PagedCache:
                     pages[at] = names[page]
         self._free = [page for page, n in enumerate(uses) if not n]  # ascending: a heap
         self._moved += 1
-        self._copy(moves)
         return list(names.items())
 
     def load_tables(self, tables):

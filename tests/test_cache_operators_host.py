@@ -634,3 +634,48 @@ def test_stores_and_copies_count_as_updates_of_the_pools(host, monkeypatch):
         cache.store(0, slots, x, x)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             product.backward()
+
+
+def _state(cache):
+    return ([(number, item.pages[:], item.tokens) for number, item in cache._sequences.items()], sorted(cache._free),
+            cache._uses[:], cache._moved + cache._shared)
+
+
+@pytest.mark.parametrize("failing", ["_copy", "_made"])
+def test_a_failed_extend_changes_nothing(host, monkeypatch, failing):
+    """No memory for the slots, or no launch: sequences, pages and their counts are as before."""
+    cache = make(pages=12)
+    a = cache.new()
+    cache.extend([a], [6])
+    b, c, d = cache.fork(a), cache.fork(a), cache.new()
+    cache.extend([d], [3])
+    before = _state(cache)
+
+    def fail(*arguments):
+        raise RuntimeError("out of memory")
+
+    with monkeypatch.context() as patch:
+        patch.setattr(paged_cache.PagedCache, failing, fail)
+        for sequences, counts in (([b, c, a, d], [3, 1, 7, 2]), ([d, a], [0, 1]), ([b], [12]), ([a, b, c], [1, 1, 1])):
+            with pytest.raises(RuntimeError, match="memory"):
+                cache.extend(sequences, counts)
+            assert _state(cache) == before
+    assert cache.extend([b, c, a, d], [3, 1, 7, 2]).index.tolist()[:4] == [3 * 4 + 2, 3 * 4 + 3, 4 * 4, 5 * 4 + 2]
+    assert cache.pages_of(a)[:2] == [0, 1]
+
+
+@pytest.mark.parametrize("call", ["compact", "make_contiguous"])
+def test_failed_page_moves_change_nothing(host, monkeypatch, call):
+    cache = make(pages=10)
+    cache.load_tables([([9, 3], 7), ([0, 7, 9], 12), ([5], 2)])
+    before = _state(cache)
+
+    def fail(*arguments):
+        raise RuntimeError("no launch")
+
+    with monkeypatch.context() as patch:
+        patch.setattr(paged_cache.PagedCache, "_copy", fail)
+        with pytest.raises(RuntimeError, match="launch"):
+            cache.compact() if call == "compact" else cache.make_contiguous(0)
+        assert _state(cache) == before
+    assert cache.compact() == [(5, 1), (7, 2), (9, 4)]
