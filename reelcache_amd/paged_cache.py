@@ -31,7 +31,7 @@ import torch
 from . import _lib
 from ._checks import count, in_memory, need, one_of
 from .errors import CapacityError, ConfigurationError, StateError, UnsupportedError
-from .restore_model import OUTPUT_DTYPES, NativeView
+from .restore_model import OUTPUT_DTYPES, NativeView, Remembering
 from .rotary import Launch, _span, addresses_of, capturing, entered, known_calls, need_gpu, position_fields, raw_stream
 
 HOLE = -1
@@ -39,7 +39,7 @@ _LAYOUTS = ("BTHD", "BHTD")
 
 
 @dataclass(eq=False)
-class Slots:
+class Slots(Remembering):
     """Where new tokens go: built by :meth:`PagedCache.extend` or :meth:`PagedCache.slots` once per
     step, used by :meth:`PagedCache.store` in every layer.  ``index``: int32 ``[tokens]`` on the device,
     page * page_tokens + row of each token, written on the stream that was current then (other streams

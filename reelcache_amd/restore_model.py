@@ -383,8 +383,16 @@ class RopeTable:
         return self._kernel_block(device, stream).pairs
 
 
+class Remembering:
+    """An object that calls prepare launches for (``_known_calls``, by their geometry): those are no part of what is
+    copied or pickled."""
+
+    def __getstate__(self):
+        return {name: value for name, value in self.__dict__.items() if name != "_known_calls"}
+
+
 @dataclass(frozen=True, eq=False)
-class RopePositions:
+class RopePositions(Remembering):
     """Original positions of one chunk in a :class:`RopeTable`.
 
     Separable tables take ``rows=(t_row, h_row, w_row)`` (an int means

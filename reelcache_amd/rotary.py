@@ -27,7 +27,7 @@ import torch
 from . import _lib
 from ._checks import count, in_memory, need, one_of, strided
 from .errors import ConfigurationError, StateError, UnsupportedError
-from .restore_model import _AXES, LAYOUTS, OUTPUT_DTYPES, RopePositions, RopeTable
+from .restore_model import _AXES, LAYOUTS, OUTPUT_DTYPES, Remembering, RopePositions, RopeTable
 
 PAIRINGS = ("interleaved", "half")
 #: Most tensors of one call.
@@ -38,7 +38,7 @@ _NULL = contextlib.nullcontext()
 
 
 @dataclass(frozen=True, eq=False)
-class TokenRows:
+class TokenRows(Remembering):
     """A :class:`RopeTable` row for every token.
 
     ``rows``: an int32 tensor on the tokens' device, ``[T, 3]`` or ``[B, T, 3]`` of (frame, height,

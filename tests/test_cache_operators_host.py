@@ -1,7 +1,9 @@
 """Host logic of the cache operators (page tables, slots, plans) and their refusals, without a GPU."""
 
 import contextlib
+import copy
 import heapq
+import pickle
 import re
 import types
 from pathlib import Path
@@ -679,3 +681,29 @@ def test_failed_page_moves_change_nothing(host, monkeypatch, call):
             cache.compact() if call == "compact" else cache.make_contiguous(0)
         assert _state(cache) == before
     assert cache.compact() == [(5, 1), (7, 2), (9, 4)]
+
+
+def test_positions_and_slots_can_be_pickled_after_their_calls(host, monkeypatch):
+    """What calls prepared is no part of a position's or slots' state."""
+    monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
+    monkeypatch.setattr(rotary, "entered", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(rotary, "_table_pairs", lambda table, device, stream: 64)
+    monkeypatch.setattr(rotary, "raw_stream", lambda device: 0)
+    monkeypatch.setattr(rotary.Launch, "__call__", lambda self, addresses, *rest: None)
+    cos, sin, sections = oracle.tables(8, 4)
+    table = rk.RopeTable(cos, sin, sections)
+    x = torch.zeros(6, 2, 8)
+    cache = make()
+    slots = cache.extend([cache.new()], [6])
+    cache.store(0, slots, x, x)
+    for positions, grid in ((rk.RopePositions(table, (1, 0, 2)), (1, 2, 3)), (rotary.TokenRows(table, torch.ones(6, 3, dtype=torch.int32)), None)):
+        rotary.rotate(x, positions, grid=grid, layout="THD")
+        assert "_known_calls" in vars(positions)
+        for again in (pickle.loads(pickle.dumps(positions)), copy.deepcopy(positions)):
+            assert "_known_calls" not in vars(again) and type(again) is type(positions)
+            assert torch.equal(torch.as_tensor(again.rows), torch.as_tensor(positions.rows))
+            assert torch.equal(again.table.cos, cos)
+            rotary.rotate(x, again, grid=grid, layout="THD")
+    again = pickle.loads(pickle.dumps(slots))
+    assert torch.equal(again.index, slots.index) and again.cache.pages_of(0) == [0, 1]
+    again.cache.store(0, again, x, x)

@@ -1,5 +1,7 @@
 """``rotary.rotate`` on the GPU against its plain form in 64 bits, its gradients and captured calls."""
 
+import pickle
+
 import numpy as np
 import pytest
 import torch
@@ -283,3 +285,14 @@ def test_rows_that_start_at_any_element(device, dtype, pairing):
         out = torch.empty(size + 3, dtype=dtype, device=device)[3:].view(2, 10, 3, dim)
         rotary.rotate(x, positions, pairing=pairing, out=out)
         assert oracle.worst(out, *expected) <= 0
+
+
+def test_positions_are_pickled_after_use(device):
+    cos, sin, sections = oracle.tables(16, 8)
+    positions = rk.RopePositions(rk.RopeTable(cos, sin, sections), (1, 0, 2))
+    x = _normal((1, 6, 1, 16), torch.float32, device, 1)
+    expected = rotary.rotate(x, positions, grid=(1, 2, 3))
+    torch.cuda.synchronize(device)
+    positions.table.invalidate()  # device copies and their events stay here
+    again = pickle.loads(pickle.dumps(positions))
+    assert torch.equal(rotary.rotate(x, again, grid=(1, 2, 3)), expected)
