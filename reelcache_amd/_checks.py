@@ -41,6 +41,9 @@ def strided(value: Any, name: str) -> torch.Tensor:
 def in_memory(value: Any, name: str) -> torch.Tensor:
     """A strided tensor whose storage holds its values (no negation that is still to be done) and nothing
     besides (no tangent of forward-mode differentiation, which a kernel would drop)."""
+    if type(value) is torch.Tensor and value.layout is torch.strided and not (
+            value.is_meta or value.is_neg() or forward_ad._current_level >= 0):
+        return value  # one look: single tokens' calls are bound by the host
     if strided(value, name).is_neg():
         raise ConfigurationError(f"{name} has a negation pending; resolve_neg() it")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(value).tangent is not None:

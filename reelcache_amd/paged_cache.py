@@ -539,7 +539,7 @@ class PagedCache:
                    *addresses_of(positions, self.device, stream), slots.index.data_ptr(), stream)
             if stream != slots.stream:  # the allocator learns of a stream that the index was not made on
                 slots.index.record_stream(torch.cuda.current_stream(self.device))
-            torch.autograd.graph.increment_version(self._counted)
+            torch._C._increment_version(self._counted)
 
     def _store_launch(self, sources, positions, grid, tokens):
         turned = position_fields(positions, grid, tokens, 1, self.head_dim, self.device)

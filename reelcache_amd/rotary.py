@@ -68,8 +68,8 @@ class TokenRows(Remembering):
 
 
 def entered(device):
-    """A context in which ``device`` is current (nothing to enter when it is already)."""
-    return _NULL if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    """A context in which ``device`` (of a tensor that is there) is current; nothing to enter when it is already."""
+    return _NULL if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 def capturing():
@@ -91,6 +91,9 @@ def raw_stream(device):
 # Streams that a table's device copy has been used on: its memory comes from the upload stream, so the
 # allocator has to know them before the copy is dropped (once per copy and stream).
 _TABLE_STREAMS: weakref.WeakKeyDictionary = weakref.WeakKeyDictionary()
+# Device copies that captured calls read: their graphs read them on every replay, whatever becomes of the table, so
+# they stay for the life of the process (as the staging of captured restores does).
+_CAPTURED_TABLES: set = set()
 
 
 def _table_pairs(table, device, stream):
@@ -105,6 +108,8 @@ def _table_pairs(table, device, stream):
     if stream not in used:
         entry.block.record_stream(torch.cuda.current_stream(device))
         used.add(stream)
+    if torch._C._cuda_isCurrentStreamCapturing():
+        _CAPTURED_TABLES.add(entry)
     return entry.pairs.data_ptr()
 
 
@@ -341,7 +346,7 @@ def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interl
 
     Runs on the current stream of the tensors' device.  Differentiable in the tensors (in
     reverse mode; not with ``out``); a table or token rows changed in place before the backward pass are
-    refused there.  Returns a tensor, or a tuple for a tuple.
+    refused there.  A captured call keeps the angles that the table had then.  Returns a tensor, or a tuple for a tuple.
     """
     single = isinstance(tensors, torch.Tensor)
     tensors = (tensors,) if single else tuple(tensors)

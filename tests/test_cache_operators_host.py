@@ -2,10 +2,12 @@
 
 import contextlib
 import copy
+import gc
 import heapq
 import pickle
 import re
 import types
+import weakref
 from pathlib import Path
 
 import numpy as np
@@ -707,3 +709,30 @@ def test_positions_and_slots_can_be_pickled_after_their_calls(host, monkeypatch)
     again = pickle.loads(pickle.dumps(slots))
     assert torch.equal(again.index, slots.index) and again.cache.pages_of(0) == [0, 1]
     again.cache.store(0, again, x, x)
+
+
+def test_tables_of_captured_calls_are_kept(monkeypatch):
+    """A graph reads a table's device copy on every replay: it outlives the table and its updates."""
+    device, state = torch.device("cpu"), {"capturing": False}
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: state["capturing"], raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device: None)
+    monkeypatch.setattr(rotary, "_CAPTURED_TABLES", set())
+    cos, sin, sections = oracle.tables(8, 4)
+    table = rk.RopeTable(cos, sin, sections)
+
+    def use():
+        entry = table._kernel_block(device, None)
+        rotary._TABLE_STREAMS[entry] = {0}
+        assert rotary._table_pairs(table, device, 0) == entry.pairs.data_ptr()
+        return weakref.ref(entry)
+
+    eager = use()
+    table.cos.mul_(0.5)
+    state["capturing"] = True
+    captured = use()
+    state["capturing"] = False
+    table.cos.mul_(0.5)
+    later = use()
+    table.invalidate()
+    gc.collect()
+    assert eager() is None and later() is None and captured() is not None

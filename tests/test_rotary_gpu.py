@@ -296,3 +296,32 @@ def test_positions_are_pickled_after_use(device):
     positions.table.invalidate()  # device copies and their events stay here
     again = pickle.loads(pickle.dumps(positions))
     assert torch.equal(rotary.rotate(x, again, grid=(1, 2, 3)), expected)
+
+
+def test_captured_calls_keep_the_tables_angles(device):
+    """A table updated, dropped and made again after a capture: replays turn by the angles of the capture."""
+    cos, sin, sections = oracle.tables(16, 32)
+    table = rk.RopeTable(cos.to(device), sin.to(device), sections)
+    positions = rk.RopePositions(table, (3, 1, 2))
+    x = _normal((1, 6, 2, 64), torch.bfloat16, device, 1)
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        expected = rotary.rotate(x, positions, grid=(1, 2, 3))
+    torch.cuda.synchronize(device)
+    rk.reserve_capture_staging(1 << 16)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = rotary.rotate(x, positions, grid=(1, 2, 3))
+    for replay in range(3):
+        table.cos.mul_(0.5)
+        assert not torch.equal(rotary.rotate(x, positions, grid=(1, 2, 3)), expected)
+        if replay == 1:
+            table.invalidate()
+        torch.cuda.synchronize(device)
+        junk = [torch.full((size,), 7.0, device=device) for size in (16 * 32 * 4, 1 << 10, 1 << 14) for _ in range(20)]
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize(device)
+        assert torch.equal(out, expected)
+        del junk
