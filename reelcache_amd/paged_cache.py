@@ -23,7 +23,7 @@ from __future__ import annotations
 import ctypes
 import heapq
 import struct
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
@@ -50,6 +50,26 @@ class Slots(Remembering):
     cache: "PagedCache"
     stamp: int
     stream: int
+
+
+@dataclass(frozen=True, eq=False)
+class PageView(NativeView):
+    """A restore destination in a sequence's pages (:meth:`PagedCache.view`).  A restore into it is refused
+    once one of those pages moved, was dropped or freed, or is shared."""
+
+    cache: "PagedCache | None" = field(default=None, repr=False)
+    sequence: int = -1
+    first: int = 0         # index of the first page in the sequence
+    pages: tuple = ()      # the pages it had then
+    item: "_Sequence | None" = field(default=None, repr=False)
+    end: int = 0           # tokens that the sequence had to have
+
+    def check(self):
+        cache, item = self.cache, self.item
+        if (cache._sequences.get(self.sequence) is not item or item.tokens < self.end
+                or tuple(item.pages[self.first:self.first + len(self.pages)]) != self.pages
+                or any(cache._uses[page] > 1 for page in self.pages)):
+            raise StateError("pages moved, were freed or became shared after this view was made")
 
 
 class _Sequence:
@@ -474,8 +494,8 @@ class PagedCache:
 
     def view(self, layer, target, sequence, start, tokens):
         """The slot of ``tokens`` tokens of a sequence as a restore destination: a
-        :class:`~reelcache_amd.restore_model.NativeView` of the layer's K (``target="k"``) or V (``"v"``)
-        pool.  The tokens lie in one page, or in consecutive pages of a ``"BTHD"`` pool whose token rows
+        :class:`~reelcache_amd.restore_model.NativeView` (:class:`PageView`) of the layer's K (``target="k"``)
+        or V (``"v"``) pool, which a restore takes as long as its pages are the sequence's alone.  The tokens lie in one page, or in consecutive pages of a ``"BTHD"`` pool whose token rows
         follow each other across pages (:meth:`make_contiguous`)."""
         one_of(target, ("k", "v"), "target")
         pool = self._layer(layer)[target == "v"]
@@ -488,13 +508,14 @@ class PagedCache:
         if any(self._uses[page] > 1 for page in pages):
             raise StateError("the view's page is shared with another sequence")
         offset = start - first * self.page_tokens
+        where = self, sequence, first, tuple(pages), found, start + tokens
         if first == last:
-            return NativeView(pool, self.layout, offset, pages[0])
+            return PageView(pool, self.layout, offset, pages[0], *where)
         joined = self.layout == "BTHD" and pool.stride(0) == self.page_tokens * pool.stride(1)
         if not joined or any(b != a + 1 for a, b in zip(pages, pages[1:])):
             raise StateError("the view's pages do not follow each other; see make_contiguous")
         flat = pool.as_strided((self.pages * self.page_tokens, self.heads, self.head_dim), pool.stride()[1:])
-        return NativeView(flat, "THD", pages[0] * self.page_tokens + offset)
+        return PageView(flat, "THD", pages[0] * self.page_tokens + offset, 0, *where)
 
     def store(self, layer, slots, keys, values, *, positions=None, grid=None):
         """Write new tokens into their slots (a backward pass that saved a pool notices): ``keys`` turned by ``positions`` (interleaved pairs, as
@@ -609,4 +630,4 @@ def _pools(group, axes, pages, page_tokens):
     return table, (ctypes.c_int64 * len(fields))(*fields), {raw_stream(group[0].device)}
 
 
-__all__ = ["HOLE", "PagedCache", "Slots"]
+__all__ = ["HOLE", "PageView", "PagedCache", "Slots"]

@@ -54,6 +54,9 @@ class NativeView:
     token_offset: int = 0
     batch_index: int = 0
 
+    #: Called before a restore writes into the view, where a view can go stale.
+    check = None
+
     def __post_init__(self):
         tensor = strided(self.tensor, "destination tensor")
         one_of(self.layout, LAYOUTS, "destination layout")

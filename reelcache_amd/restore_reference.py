@@ -43,10 +43,10 @@ def _storage_key(tensor):
 
 class _Facts:
     """What call validation needs of a job, computed once per job object (jobs are immutable):
-    the devices of its tensors, its destination view's geometry, its token span and its
+    the devices of its tensors, its destination view's geometry and check, its token span and its
     matrix-product flops."""
 
-    __slots__ = ("devices", "dst", "flops", "shift", "span", "view")
+    __slots__ = ("check", "devices", "dst", "flops", "shift", "span", "view")
 
     def __init__(self, job):
         view, source = job.destination, job.source
@@ -54,7 +54,7 @@ class _Facts:
         devices = {tensor.device, source.device if isinstance(source, PictureSource) else source.values.device}
         if job.basis is not None:
             devices.add(job.basis.device)
-        self.devices = devices
+        self.devices, self.check = devices, view.check
         self.shift = tensor.storage_offset() * tensor.element_size()
         self.view = (tensor.storage_offset(), tuple(tensor.shape), tensor.stride(), view.layout, view.batch_index,
                      tensor.device)
@@ -93,7 +93,7 @@ def _check_disjoint(jobs, facts=None):
 
 
 def _validate(jobs):
-    """``(jobs tuple, device or None)`` of a job list; raises on mixed devices or overlapping slots."""
+    """``(jobs tuple, device or None)`` of a job list; raises on mixed devices, stale views or overlapping slots."""
     if isinstance(jobs, ReconstructionJob):
         jobs = (jobs,)
     need(isinstance(jobs, Sequence) and not isinstance(jobs, (str, bytes)),
@@ -103,6 +103,9 @@ def _validate(jobs):
     facts = [_facts(job) for job in jobs]
     devices = set().union(*(fact.devices for fact in facts)) if facts else set()
     need(len(devices) <= 1, "all job tensors (except RoPE tables) must share one device")
+    for fact in facts:
+        if fact.check is not None:
+            fact.check()
     _check_disjoint(jobs, facts)
     return jobs, next(iter(devices), None)
 

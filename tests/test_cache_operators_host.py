@@ -736,3 +736,43 @@ def test_tables_of_captured_calls_are_kept(monkeypatch):
     table.invalidate()
     gc.collect()
     assert eager() is None and later() is None and captured() is not None
+
+
+def test_restores_into_stale_views_are_refused(host):
+    """A view is a restore destination as long as its pages are its sequence's alone."""
+    cache = make(pages=12, size=4, heads=2, dim=8, layers=1)
+    cache.load_tables([([7, 2], 8), ([11], 4), ([5], 3)])
+    job = lambda view, tokens: rk.ReconstructionJob(rk.DenseSource(torch.randn(tokens, 16)), view, (1, 1, tokens))
+    restore = rk.reconstruct_reference
+    changes = {
+        "fork": lambda c: c.fork(0), "free": lambda c: c.free(0), "compact": lambda c: c.compact(),
+        "truncate": lambda c: c.truncate(0, 3), "drop": lambda c: c.drop(0, 0, 1), "contiguous": lambda c: c.make_contiguous(0),
+        "load": lambda c: c.load_tables([([7, 2], 8)]),
+    }
+    for name, change in changes.items():
+        cache.load_tables([([7, 2], 8), ([11], 4), ([5], 3)])
+        first = job(cache.view(0, "k", 0, 0, 4), 4)
+        kept = job(cache.view(0, "v", 1, 1, 3), 3)
+        restore([first, kept])
+        assert torch.equal(cache.keys[0, 7], first.source.values.view(4, 2, 8))
+        change(cache)
+        before = cache.keys.clone()
+        with pytest.raises(StateError, match="after this view"):
+            restore([first])
+        with pytest.raises(StateError, match="after this view"):
+            restore([job(first.destination, 4)])
+        assert torch.equal(cache.keys, before)
+        if name in ("fork", "free", "truncate", "drop", "contiguous"):  # other sequences' pages are as they were
+            restore([kept])
+            assert torch.equal(cache.values[0, 11, 1:], kept.source.values.view(3, 2, 8))
+    # Growth of the sequence, and of others, leaves a view as it is.
+    cache.load_tables([([7, 2], 8), ([11], 4), ([5], 3)])
+    kept = job(cache.view(0, "k", 0, 0, 4), 4)
+    other = cache.fork(2)
+    cache.extend([0, other], [2, 1])
+    restore([kept])
+    assert torch.equal(cache.keys[0, 7], kept.source.values.view(4, 2, 8))
+    with pytest.raises(StateError, match="after this view"):
+        stale = job(cache.view(0, "k", 0, 8, 2), 2)
+        cache.fork(0)
+        restore([stale])
