@@ -39,6 +39,7 @@ _CUS = 256
 # 4.1 us so, 4.1-5.1 us with a thread per eight channels; a second launch costs 5 us).
 _FEW_ROWS = 512
 _XCDS = 8
+_MOST_KEYS = 2 ** 31 - 4096
 # Scales that stay normal fp32 numbers with log2(e) in them.
 _LEAST_SCALE, _MOST_SCALE = 2.0 ** -126, 2.0 ** 127
 
@@ -100,6 +101,9 @@ class AttentionPlan:
         if cache.head_dim > _lib.ATTEND_MAX_DIM:
             raise UnsupportedError(f"attention takes at most {_lib.ATTEND_MAX_DIM} channels to a head")
         need_gpu(cache.device, "attention")
+        # The kernels step over keys and pages in 32 bits, up to a few tiles past a sequence's last page.
+        need(all(len(item.pages) * cache.page_tokens <= _MOST_KEYS for item in found),
+             f"attention takes sequences of at most {_MOST_KEYS} tokens, their last page whole")
         self.cache, self.heads, self.queries = cache, heads, sum(queries)
         self.group = heads // cache.heads
         need(self.queries * self.group < 1 << 31, "a step has fewer than 2**31 query rows")

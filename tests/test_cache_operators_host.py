@@ -776,3 +776,16 @@ def test_restores_into_stale_views_are_refused(host):
         stale = job(cache.view(0, "k", 0, 8, 2), 2)
         cache.fork(0)
         restore([stale])
+
+
+def test_sequences_whose_keys_32_bits_do_not_count_are_refused(host):
+    """Dropped pages take no room, so a sequence may be longer than its pool."""
+    size = 1 << 20
+    cache = make(pages=2, size=size, heads=1, dim=1, layers=1)
+    for pages, fits in ((2047, True), (2048, False)):
+        cache.load_tables([([paged_cache.HOLE] * (pages - 1) + [1], (pages - 1) * size + 5)])
+        if fits:
+            cache.plan([0], [1], heads=1)
+        else:
+            with pytest.raises(ConfigurationError, match="tokens"):
+                cache.plan([0], [1], heads=1)
