@@ -70,8 +70,9 @@ struct Runs {
     int32_t first[RCH_ARGUMENT_RUNS], count[RCH_ARGUMENT_RUNS], at[RCH_ARGUMENT_RUNS];
 };
 __global__ void __launch_bounds__(256) runs_store_kernel(int64_t to, const Runs runs) {
-    const int run = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
-    if (i < runs.count[run]) gout<int32_t>(to)[static_cast<int64_t>(runs.at[run]) + i] = runs.first[run] + i;
+    const int run = blockIdx.y;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;  // past 2^31 behind the longest runs
+    if (i < runs.count[run]) gout<int32_t>(to)[runs.at[run] + i] = static_cast<int32_t>(runs.first[run] + i);
 }
 
 }  // namespace
