@@ -311,6 +311,8 @@ class _Rotation(torch.autograd.Function):
             ctx.save_for_backward(positions.rows)  # rows changed in place before the backward pass are refused
         outs = _rotate(tensors, positions, grid, layout, pairing, inverse)
         ctx.table = _table_state(positions.table, tensors[0].device)  # a table changed before the backward pass is refused
+        if not all(ctx.needs_input_grad[5:]):  # a rotated tensor requires a gradient where its input does
+            ctx.mark_non_differentiable(*[out for out, wanted in zip(outs, ctx.needs_input_grad[5:]) if not wanted])
         return outs
 
     @staticmethod

@@ -508,3 +508,37 @@ def test_odd_heads_in_odd_parts(device, dtype, dim, group):
     for n in (3000, 3200, 3400):
         _, _, plan, _ = _run(device, [n], [1], 16, 1, group, dim, dtype)
         assert plan._n_merges
+
+
+@pytest.mark.parametrize("layout", ["BTHD", "BHTD"])
+@pytest.mark.parametrize("dim,size", [(128, 256), (100, 250)])
+def test_pools_past_32_bits(device, layout, dim, size):
+    """Pages that lie more than 2^32 elements into their pools: copies, stores and attention, tiled and general."""
+    heads, dtype = 8, torch.bfloat16
+    pages = (1 << 32) // (size * heads * dim) + 40
+    cache = paged_cache.PagedCache.allocate(pages, size, heads, dim, device=device, layout=layout)
+    assert (pages - 40) * cache.keys.stride(1) * 2 > 1 << 32
+    last = list(range(pages - 12, pages - 4))
+    for pool in (cache.keys, cache.values):
+        assert pool[0, last[0]].data_ptr() - pool.data_ptr() > 1 << 33
+    n = 6 * size + 41
+    cache.load_tables([(last[:7], n - 30), ([*range(pages - 13)], (pages - 13) * size)])  # the lower pages are taken
+    generator = torch.Generator(device).manual_seed(1)
+    for pool in (cache.keys, cache.values):
+        pool[0, pages - 13:] = torch.randn(pool[0, pages - 13:].shape, generator=generator, device=device).to(dtype)
+    child = cache.fork(0)
+    slots = cache.extend([child], [30])  # copies the begun page
+    assert cache.pages_of(child)[-1] != last[6] and min(cache.pages_of(child)) > pages - 14
+    k, v = (torch.randn((30, heads, dim), generator=generator, device=device).to(dtype) for _ in range(2))
+    cache.store(0, slots, k, v)
+    tokens = [torch.cat([(pool[0, page] if layout == "BTHD" else pool[0, page].transpose(0, 1)) for page in cache.pages_of(child)])[:n]
+              for pool in (cache.keys, cache.values)]
+    assert torch.equal(tokens[0][-30:], k) and torch.equal(tokens[1][-30:], v)
+    begun = (n - 30) % size
+    for pool in (cache.keys, cache.values):
+        old, new = (pool[0, page] if layout == "BTHD" else pool[0, page].transpose(0, 1) for page in (last[6], cache.pages_of(child)[6]))
+        assert torch.equal(old[:begun], new[:begun])
+    q = torch.randn((30, heads, dim), generator=generator, device=device).to(dtype)
+    out, lse = cache.attend(0, q, cache.plan([child], [30], heads=heads, block=1), return_lse=True)
+    want, bound, logs, log_bound = oracle.attend(q, tokens[0][None], tokens[1][None], [0], n, 30, n, block=1)
+    assert oracle.worst(out, want, bound) <= 0 and oracle.worst(lse, logs, log_bound) <= 0

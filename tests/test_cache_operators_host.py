@@ -789,3 +789,25 @@ def test_sequences_whose_keys_32_bits_do_not_count_are_refused(host):
         else:
             with pytest.raises(ConfigurationError, match="tokens"):
                 cache.plan([0], [1], heads=1)
+
+
+def test_rotated_tensors_require_gradients_where_their_inputs_do(host, monkeypatch):
+    """Keys without a gradient that turn beside queries with one: they can be stored."""
+    monkeypatch.setattr(rotary, "need_gpu", lambda device, what: None)
+    monkeypatch.setattr(rotary, "entered", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(rotary, "_table_pairs", lambda table, device, stream: 64)
+    monkeypatch.setattr(rotary, "raw_stream", lambda device: 0)
+    launches = []
+    monkeypatch.setattr(rotary.Launch, "__call__", lambda self, addresses, *rest: launches.append(len(addresses)))
+    cos, sin, sections = oracle.tables(8, 4)
+    positions = rk.RopePositions(rk.RopeTable(cos, sin, sections), 0)
+    queries, keys = torch.zeros(6, 4, 8, requires_grad=True), torch.zeros(6, 2, 8)
+    q, k = rotary.rotate((queries, keys), positions, grid=(1, 2, 3), layout="THD")
+    assert q.requires_grad and not k.requires_grad
+    cache = make()
+    cache.store(0, cache.extend([cache.new()], [6]), k, torch.zeros(6, 2, 8))
+    launches.clear()
+    (q.sum() + k.sum()).backward()
+    assert launches == [1] and queries.grad.shape == queries.shape
+    k, q = rotary.rotate((keys, queries), positions, grid=(1, 2, 3), layout="THD")
+    assert q.requires_grad and not k.requires_grad
