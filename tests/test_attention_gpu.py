@@ -542,3 +542,24 @@ def test_pools_past_32_bits(device, layout, dim, size):
     out, lse = cache.attend(0, q, cache.plan([child], [30], heads=heads, block=1), return_lse=True)
     want, bound, logs, log_bound = oracle.attend(q, tokens[0][None], tokens[1][None], [0], n, 30, n, block=1)
     assert oracle.worst(out, want, bound) <= 0 and oracle.worst(lse, logs, log_bound) <= 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size", [(128, 16), (64, 64), (200, 100), (20, 16)])
+@pytest.mark.parametrize("level", [8192.0, -8192.0])
+def test_scores_far_out_under_masks(device, dtype, dim, size, level):
+    """Equal scores of +-10^9 weigh as equal scores of 0 do, whatever a row sees of them: under masks, with a dropped
+    page, beside rows that see nothing, in one part and in several, and beside a sequence of ordinary scores."""
+    lengths, queries = [5 * size + 3, 70, 4000], [2 * size, 90, 3]
+    cache = _cache(device, lengths, size, 1, dim, dtype)
+    cache.drop(0, 1, 1)
+    q = torch.full((sum(queries), 2, dim), 8192.0, device=device).to(dtype)
+    q[2 * size:2 * size + 90] = torch.randn((90, 2, dim), generator=torch.Generator().manual_seed(1)).to(dtype).to(device)
+    ordinary = cache.keys[0, cache.pages_of(1)].clone()
+    for mask in ({}, {"block": 1}, {"block": 7, "window": 3 * size // 2}):
+        cache.keys.fill_(level)
+        cache.keys[0, cache.pages_of(1)] = ordinary
+        out = cache.attend(0, q, cache.plan([0, 1, 2], queries, heads=2, **mask))
+        cache.keys.fill_(0.0)
+        cache.keys[0, cache.pages_of(1)] = ordinary
+        _check(cache, q, out, None, lengths, queries, **mask)
