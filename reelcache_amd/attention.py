@@ -82,7 +82,8 @@ class AttentionPlan:
 
     ``block``, ``window``: see the module docstring (``None``: no such bound).  ``scale``: a positive
     factor of the scores (default ``head_dim ** -0.5``).  The plan is bound to the pages that the
-    sequences have now; it is stale once pages move or are freed.  Its tables are written on the stream
+    sequences have now; it is stale once pages move or are freed, and it keeps reading a begun page that a
+    later ``extend`` copies for its sequence (plans are made after the step's ``extend``).  Its tables are written on the stream
     that is current (other streams wait for it).  A captured graph keeps its plan's tables as they are:
     keep the plan as long as the graph.
     """
@@ -303,7 +304,9 @@ def attend(q, keys, values, plan, *, out=None, return_lse=False):
     query that sees nothing), by which the results over two caches join.  A query whose scores are all
     -inf gets NaN, as their softmax has no value (and a log of -inf).
 
-    Scores and sums are held in fp32; the output is rounded once.  Runs on the current stream; not
+    Scores, weights and sums are held in fp32; for the product with 16-bit values the weights are rounded to
+    their type (half a step each, averaged over the keys), and the output is rounded once.  Keys meet the
+    queries as the pools hold them: both are rotated before.  Runs on the current stream; not
     differentiable.  Returns ``out``, or ``(out, lse)``.
     """
     need(isinstance(plan, AttentionPlan), "attend needs an AttentionPlan")

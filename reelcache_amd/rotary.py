@@ -340,7 +340,8 @@ def rotate(tensors: Any, positions, *, grid=None, layout="BTHD", pairing="interl
     """Rotate one tensor, or a tuple of up to four in one launch (queries and keys), by ``positions``.
 
     ``tensors``: bfloat16, float16 or float32 of one dtype and device in ``layout`` (``"BTHD"``,
-    ``"THD"`` or ``"BHTD"``), any strides; head counts may differ.  The first ``positions.table.head_dim``
+    ``"THD"`` or ``"BHTD"``), any strides; head counts may differ (interleaved pairs need an even
+    ``head_dim``).  The first ``positions.table.head_dim``
     channels of a head turn and the rest are copied.  ``pairing``: channels ``(2j, 2j + 1)`` turn
     together (``"interleaved"``, as the restored caches have them) or ``(j, n + j)`` of the first ``2n``
     (``"half"``).  ``inverse`` turns back.  ``out``: a tensor (or a tuple) of the same shapes to write
