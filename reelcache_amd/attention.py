@@ -83,7 +83,8 @@ class AttentionPlan:
     ``block``, ``window``: see the module docstring (``None``: no such bound).  ``scale``: a positive
     factor of the scores (default ``head_dim ** -0.5``).  The plan is bound to the pages that the
     sequences have now; it is stale once pages move or are freed, and it keeps reading a begun page that a
-    later ``extend`` copies for its sequence (plans are made after the step's ``extend``).  Its tables are written on the stream
+    later ``extend`` copies for its sequence (plans are made after the step's ``extend``).  Its tables are
+    written on the stream
     that is current (other streams wait for it).  A captured graph keeps its plan's tables as they are:
     keep the plan as long as the graph.
     """

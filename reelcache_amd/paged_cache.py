@@ -495,8 +495,9 @@ class PagedCache:
     def view(self, layer, target, sequence, start, tokens):
         """The slot of ``tokens`` tokens of a sequence as a restore destination: a
         :class:`~reelcache_amd.restore_model.NativeView` (:class:`PageView`) of the layer's K (``target="k"``)
-        or V (``"v"``) pool, which a restore takes as long as its pages are the sequence's alone.  The tokens lie in one page, or in consecutive pages of a ``"BTHD"`` pool whose token rows
-        follow each other across pages (:meth:`make_contiguous`)."""
+        or V (``"v"``) pool, which a restore takes as long as its pages are the sequence's alone.  The tokens
+        lie in one page, or in consecutive pages of a ``"BTHD"`` pool whose token rows follow each other across
+        pages (:meth:`make_contiguous`)."""
         one_of(target, ("k", "v"), "target")
         pool = self._layer(layer)[target == "v"]
         found = self._get(sequence)
@@ -518,8 +519,9 @@ class PagedCache:
         return PageView(flat, "THD", pages[0] * self.page_tokens + offset, 0, *where)
 
     def store(self, layer, slots, keys, values, *, positions=None, grid=None):
-        """Write new tokens into their slots (a backward pass that saved a pool notices): ``keys`` turned by ``positions`` (interleaved pairs, as
-        :func:`reelcache_amd.rotary.rotate`; ``None`` stores them as they are) and ``values``, both
+        """Write new tokens into their slots (a backward pass that saved a pool notices): ``keys`` turned by
+        ``positions`` (interleaved pairs, which need an even ``head_dim``, as :func:`reelcache_amd.rotary.rotate`;
+        ``None`` stores them as they are) and ``values``, both
         ``[tokens, heads, head_dim]`` of the cache's dtype, any strides (rows of the pools themselves are
         copied first).  With a ``grid`` the tokens are one chunk."""
         if type(layer) is not int or not 0 <= layer < self.layers:
@@ -550,6 +552,8 @@ class PagedCache:
             stream = raw_stream(self.device)
             k_bytes, v_bytes = self._layer_bytes
             pools = [self.keys.data_ptr() + layer * k_bytes, self.values.data_ptr() + layer * v_bytes]
+            if pools[0] == pools[1]:
+                raise ConfigurationError("a store needs keys and values in pools of their own")
             k, v = sources[0].data_ptr(), sources[1].data_ptr()
             for pool, room in zip(pools, self._reach):
                 if (k < pool + room and pool < k + reach[0]) or (v < pool + room and pool < v + reach[1]):

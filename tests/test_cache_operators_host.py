@@ -811,3 +811,12 @@ def test_rotated_tensors_require_gradients_where_their_inputs_do(host, monkeypat
     assert launches == [1] and queries.grad.shape == queries.shape
     k, q = rotary.rotate((keys, queries), positions, grid=(1, 2, 3), layout="THD")
     assert q.requires_grad and not k.requires_grad
+
+
+def test_a_store_into_one_pool_for_both_is_refused(host):
+    """Keys and values that are one pool can be read and copied, but a store would write each place twice."""
+    pool = torch.zeros(2, 4, 4, 2, 8)
+    cache = paged_cache.PagedCache(pool, pool)
+    slots = cache.extend([cache.new()], [1])
+    with pytest.raises(ConfigurationError, match="pools of their own"):
+        cache.store(1, slots, torch.zeros(1, 2, 8), torch.zeros(1, 2, 8))
