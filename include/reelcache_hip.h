@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define RCH_ABI_VERSION 23
+#define RCH_ABI_VERSION 24
 
 /* Status codes (mapped to reelcache errors by the host). */
 #define RCH_OK 0
@@ -574,6 +574,49 @@ int rch_words_store(void* words_dev, const int32_t* words_host, int count, void*
 #define RCH_ARGUMENT_RUNS 320
 int rch_runs_store(void* words_dev, const int32_t* runs_host, int n_runs, int64_t words, void* stream);
 
+/* What a pool holds: values of the cache's dtype, or 8-bit codes with an fp32 scale for each token and head. */
+#define RCH_CODES_NONE 0
+#define RCH_CODES_INT8 1 /* signed integers */
+#define RCH_CODES_E4M3 2 /* 8-bit floats: 4 exponent and 3 mantissa bits, no infinities */
+
+/*
+ * The K and V of tokens between dense tensors [tokens, heads, head_dim] and the pools of a paged cache in codes
+ * [pages, page_tokens or heads, ..] with scales [pages, heads, page_tokens] (fp32; strides in elements, unit over the
+ * channels, of scales over the tokens).  Token t lies in row slots[t] % page_tokens of page slots[t] / page_tokens.
+ * A code c stands for c * scale, rounded to the dtype.
+ */
+typedef struct rch_codes {
+    int64_t k_ptr, v_ptr;                          /* the dense tensors */
+    int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    int64_t k_codes_ptr, v_codes_ptr;
+    int64_t k_page_stride, k_row_stride, k_codes_head_stride, v_page_stride, v_row_stride, v_codes_head_stride;
+    int64_t k_scales_ptr, v_scales_ptr;
+    int64_t k_scale_page_stride, k_scale_head_stride, v_scale_page_stride, v_scale_head_stride;
+    int64_t tokens, heads, head_dim, pages, page_tokens;
+    int64_t slots_ptr;                             /* int32 [tokens] */
+    int64_t format;                                /* RCH_CODES_INT8 or RCH_CODES_E4M3 */
+    /* rch_codes_store: the places that the keys turn by (interleaved pairs), as in rch_rotary_job */
+    int64_t pairs;
+    int64_t pairs_ptr, axes, sec_t, sec_h, limit_t, limit_h, limit_w;
+    int64_t row_t, row_h, row_w, grid_h, grid_w;
+    int64_t rows_ptr, rows_batch_stride, rows_token_stride, rows_axis_stride;
+} rch_codes;                 /* 44 x int64 = 352 bytes */
+
+#define RCH_CODES_MAX_DIM 256 /* head_dim of pools in codes */
+int rch_codes_size(void);
+/*
+ * Turns the keys (fp32 products rounded apart, as rch_rotary) and writes codes and scales of both tensors; x is the
+ * value in fp32, m the largest |x| of a token's head:
+ *   int8: scale = max(m / 127, 2^-126), code = rint(x * (1 / scale)) within +-127, all in fp32
+ *   e4m3: scale = 2^e, the least e >= -126 with m <= 448 * 2^e; code = x / scale, within +-240 where 256 * scale is more
+ *     than the dtype holds, rounded to nearest even
+ * A head with a value that is infinite or NaN gets scale NaN (it stands for NaN in every channel) and codes 0.  A slot
+ * outside the pool is dropped.
+ */
+int rch_codes_store(const rch_codes* args_host, int dtype, void* stream);
+/* Writes the values that the tokens' codes stand for to the dense tensors; NaN for a slot outside the pool. */
+int rch_codes_read(const rch_codes* args_host, int dtype, void* stream);
+
 /*
  * Attention of new tokens over a paged cache.  A plan is a device int32 buffer built by the host:
  * items (RCH_ATTEND_ITEM words each), merges (RCH_ATTEND_MERGE words each) and page tables; its first
@@ -593,6 +636,13 @@ int rch_runs_store(void* words_dev, const int32_t* runs_host, int n_runs, int64_
  *   row, parts, 0, 0]: part i of row r is partial row first + i * rows + (r - row_begin).
  * Partials (16-byte aligned): fp32 [partial_rows, head_dim] sums, then, from an even word on, fp32
  * [partial_rows, 2] of (reference exponent, sum; -inf and 0 where every score is -inf).
+ *
+ * Pools in codes (codes != RCH_CODES_NONE; q, out in f16 or bf16): keys and values are what the codes stand for,
+ * rounded to the dtype (rch_codes_store).
+ * Lists (lists_ptr != 0): an item's keys are those of chosen blocks of block_tokens keys, which divide a page.  Its
+ * word 10 is the index in lists (int32) of its first entry, the number of a block of the sequence; key_begin and key_end
+ * count tiles of 64 (f32: 32) keys from there, ceil(block_tokens / tile) to an entry.  An entry that is no block of the
+ * sequence, or lies in a hole, has no keys.
  */
 #define RCH_ATTEND_ITEM 12
 #define RCH_ATTEND_MERGE 8
@@ -620,7 +670,11 @@ typedef struct rch_attend {
     int64_t most_rows_many, most_rows; /* most rows of one of those, and of one of the others */
     int64_t holes;           /* 1: page tables may hold holes */
     int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64 */
-} rch_attend;                /* 36 x int64 = 288 bytes */
+    int64_t codes;           /* RCH_CODES_* */
+    int64_t k_scale_ptr, v_scale_ptr; /* of pools in codes; strides in elements */
+    int64_t k_scale_page_stride, k_scale_head_stride, v_scale_page_stride, v_scale_head_stride;
+    int64_t lists_ptr, block_tokens;
+} rch_attend;                /* 45 x int64 = 360 bytes */
 
 /*
  * Cuts the row blocks of a plan into parts (host only): block i has tiles[i] key tiles and belongs to owner[i]
@@ -633,6 +687,39 @@ int rch_attend_share(const int64_t* tiles, const int64_t* owner, int64_t n, int6
 
 int rch_attend_size(void);
 int rch_attend_run(const rch_attend* args_host, int dtype, void* stream);
+
+/*
+ * Chosen blocks of a paged cache's keys: blocks of block_tokens tokens (they divide a page), the mean key of each
+ * (means: [pages, page_tokens / block_tokens, heads, head_dim] of the cache's dtype, contiguous), and for each run of
+ * queries of a sequence and key head the blocks that its queries attend to.
+ */
+typedef struct rch_blocks {
+    int64_t means_ptr, heads, head_dim, pages, page_tokens, block_tokens;
+    /* rch_blocks_update: a layer's keys, and the slots whose blocks' means are written anew */
+    int64_t keys_ptr, page_stride, token_stride, head_stride;
+    int64_t codes, scales_ptr, scale_page_stride, scale_head_stride;
+    int64_t slots_ptr, tokens;
+    /* rch_blocks_select */
+    int64_t q_ptr, q_token_stride, q_head_stride, group;
+    int64_t plan_ptr, runs, n_runs;                /* word index of the first run, their number */
+    int64_t scores_ptr, scores;                    /* uint64 [n_runs, heads, scores], scores >= any run's scored blocks */
+    int64_t lists_ptr, width;                      /* int32 [n_runs, heads, width] */
+    int64_t top;
+} rch_blocks;                /* 28 x int64 = 224 bytes */
+
+#define RCH_BLOCKS_RUN 12
+int rch_blocks_size(void);
+/* The means of the blocks that hold a slot: over all block_tokens rows, summed in FP64, rounded to FP32 and then to
+ * the dtype. */
+int rch_blocks_update(const rch_blocks* args_host, int dtype, void* stream);
+/*
+ * A run: [table (word index of the sequence's first page), first query row of q, queries, first block, last block
+ * (behind it), first scored, last scored, first block taken anyway, last one (behind it), 0, 0, 0].  Of its blocks
+ * [first, last) whose page is no hole, all that are not scored are taken, those in the range taken anyway, and the
+ * `top` best of the others: by the sum of its query rows (queries x group heads) times the mean key, in FP64; NaN above
+ * all, equal ones by the lower number.  lists: the taken blocks in ascending order, -1 behind them.
+ */
+int rch_blocks_select(const rch_blocks* args_host, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,7 +16,7 @@ import numpy as np
 from .errors import ConfigurationError, UnsupportedError
 
 LIBRARY = Path(__file__).resolve().with_name("libreelcache_hip.so")
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 # Status codes (RCH_E_*).
 OK, E_CONFIG, E_UNSUPPORTED, E_LAUNCH = 0, 1, 2, 3
@@ -79,10 +79,25 @@ ATTEND_FIELDS = ("q_ptr", "k_ptr", "v_ptr", "out_ptr", "lse_ptr", "plan_ptr", "p
                  "q_head_stride", "k_page_stride", "k_token_stride", "k_head_stride", "v_page_stride", "v_token_stride",
                  "v_head_stride", "out_token_stride", "out_head_stride", "group", "heads", "head_dim", "page_tokens",
                  "pages", "block", "window", "scale_bits", "partial_rows", "items", "n_general", "n_rows",
-                 "merges", "n_merges", "n_many", "most_rows_many", "most_rows", "holes", "tile_unit")
+                 "merges", "n_merges", "n_many", "most_rows_many", "most_rows", "holes", "tile_unit", "codes", "k_scale_ptr",
+                 "v_scale_ptr", "k_scale_page_stride", "k_scale_head_stride", "v_scale_page_stride", "v_scale_head_stride",
+                 "lists_ptr", "block_tokens")
 ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 256
 ATTEND_FEW_PARTS = 8
 PAIRS_INTERLEAVED, PAIRS_HALF = 0, 1
+# rch_codes and rch_blocks (int64 structs read on the host during the call), formats of codes (RCH_CODES_*).
+CODES_FIELDS = ("k_ptr", "v_ptr", "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride", "k_codes_ptr",
+                "v_codes_ptr", "k_page_stride", "k_row_stride", "k_codes_head_stride", "v_page_stride", "v_row_stride",
+                "v_codes_head_stride", "k_scales_ptr", "v_scales_ptr", "k_scale_page_stride", "k_scale_head_stride",
+                "v_scale_page_stride", "v_scale_head_stride", "tokens", "heads", "head_dim", "pages", "page_tokens",
+                "slots_ptr", "format", "pairs", "pairs_ptr", "axes", "sec_t", "sec_h", "limit_t", "limit_h", "limit_w",
+                "row_t", "row_h", "row_w", "grid_h", "grid_w", "rows_ptr", "rows_batch_stride", "rows_token_stride",
+                "rows_axis_stride")
+BLOCKS_FIELDS = ("means_ptr", "heads", "head_dim", "pages", "page_tokens", "block_tokens", "keys_ptr", "page_stride",
+                 "token_stride", "head_stride", "codes", "scales_ptr", "scale_page_stride", "scale_head_stride", "slots_ptr",
+                 "tokens", "q_ptr", "q_token_stride", "q_head_stride", "group", "plan_ptr", "runs", "n_runs", "scores_ptr",
+                 "scores", "lists_ptr", "width", "top")
+CODES_NONE, CODES_INT8, CODES_E4M3, CODES_MAX_DIM, BLOCKS_RUN = 0, 1, 2, 256, 12
 
 _i, _i64, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _SIGNATURES = {
@@ -123,6 +138,12 @@ _SIGNATURES = {
     "rch_attend_share": ([_p, _p, _i64, _i64, _i64, _p, _i64, _p], _i),
     "rch_attend_size": ([], _i),
     "rch_attend_run": ([_p, _i, _p], _i),
+    "rch_codes_size": ([], _i),
+    "rch_codes_store": ([_p, _i, _p], _i),
+    "rch_codes_read": ([_p, _i, _p], _i),
+    "rch_blocks_size": ([], _i),
+    "rch_blocks_update": ([_p, _i, _p], _i),
+    "rch_blocks_select": ([_p, _i, _p], _i),
 }
 # Further entry points registered by other modules are bound when present.
 _OPTIONAL_SIGNATURES: dict = {}
@@ -154,7 +175,8 @@ def _load():
     if (lib.rch_job_size() != JOB_DTYPE.itemsize or lib.rch_pack_size() != PACK_DTYPE.itemsize
             or lib.rch_fit_matrix_size() != FIT_DTYPE.itemsize or lib.rch_call_size() != 8 * len(CALL_FIELDS)
             or lib.rch_rotary_size() != 8 * len(ROTARY_FIELDS)
-            or lib.rch_attend_size() != 8 * len(ATTEND_FIELDS)):
+            or lib.rch_attend_size() != 8 * len(ATTEND_FIELDS)
+            or lib.rch_codes_size() != 8 * len(CODES_FIELDS) or lib.rch_blocks_size() != 8 * len(BLOCKS_FIELDS)):
         raise UnsupportedError(f"{LIBRARY.name} descriptor layout differs from this package; rebuild it")
     return lib
 

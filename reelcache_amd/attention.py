@@ -89,6 +89,8 @@ class AttentionPlan:
     keep the plan as long as the graph.
     """
 
+    _block_tokens = 0  # of chosen blocks
+
     def __init__(self, cache, sequences, queries, *, heads, block=None, window=None, scale=None):
         found = cache._several(sequences)
         queries = [count(n, "a query count") for n in queries]
@@ -146,23 +148,35 @@ class AttentionPlan:
         cache = self.cache
         form, work = self._form(), _Work()
         tile = ROW_TILE if form == "rows" else GENERAL_ROWS
+        table = self._tables(found, queries)
+        for number, (item, n) in enumerate(zip(found, queries)):
+            if n:
+                work.add(number, cache.heads, n * self.group, tile, self._keys_of(item.tokens, n))
+        merges = []
+        items = self._split(form, work.rows(), merges)
+        self._send(form, table, items, merges)
+
+    def _tables(self, found, queries):
+        """The sequences' pages in one list, and where each sequence stands (``_at``, ``_lengths``, ..)."""
         table, at, lengths, starts = [], [], [], []
         words, row = _lib.ATTEND_ZEROS, 0
-        for number, (item, n) in enumerate(zip(found, queries)):
+        for item, n in zip(found, queries):
             lengths.append(item.tokens)
             starts.append(row)
             at.append(words)
             table.extend(item.pages)
             words += len(item.pages)
             row += n
-            if n:
-                work.add(number, cache.heads, n * self.group, tile, self._keys_of(item.tokens, n))
         need(words < 1 << 30, "the step's page tables are too large")
         self._at = np.asarray(at, dtype=np.int64)
         self._lengths, self._starts = np.asarray(lengths, dtype=np.int64), np.asarray(starts, dtype=np.int64)
         self._counts = np.asarray(queries, dtype=np.int64)
-        merges, self._partial_rows = [], 0
-        items = self._split(form, work.rows(), merges)
+        self._partial_rows = 0
+        return table
+
+    def _send(self, form, table, items, merges, more=None):
+        """Writes the plan's words to the device (``more``: words behind the merges)."""
+        cache = self.cache
         merges = np.concatenate(merges) if merges else np.empty((0, _lib.ATTEND_MERGE), np.int64)
         self._counts_of = (0, len(items)) if form == "rows" else (len(items), 0)
         first_item = _lib.ATTEND_ZEROS + len(table)
@@ -178,7 +192,8 @@ class AttentionPlan:
         self._holes = int(any(page < 0 for page in table))
         need(self._partial_rows < 1 << 31, "the step's partial results are too many")
         words = np.concatenate([np.zeros(_lib.ATTEND_ZEROS, np.int64), np.asarray(table, np.int64), items.ravel(),
-                                merges.ravel()])
+                                merges.ravel(), *([] if more is None else [more])])
+        need(len(words) < 1 << 31, "the step's plan is too large")
         from .paged_cache import upload
 
         self._tiled = self._counts_of[1]
@@ -196,7 +211,7 @@ class AttentionPlan:
         size = self.cache.page_tokens
         if size < KEY_TILE:
             return KEY_TILE
-        share = 16 if self.cache.keys.element_size() == 2 else 8
+        share = 8 if self.cache.keys.element_size() == 4 else 16
         held = -(-size // KEY_TILE) * KEY_TILE  # rows of tiles that a page takes
         return size if held == size or (size % share and 5 * held <= 6 * size) else KEY_TILE
 
@@ -225,9 +240,19 @@ class AttentionPlan:
         sequence, begin, end, first, last, head = blocks.T
         tile0 = self._tile_of(first)
         tiles = np.where(last > first, self._tile_of(np.maximum(last - 1, 0)) + 1 - tile0, 0)
+
+        def keys(which, low, high, part, n):
+            return (np.where(part == 0, first[which], self._key_of(tile0[which] + low)),
+                    np.where(part == n - 1, last[which], np.minimum(last[which], self._key_of(tile0[which] + high))))
+
+        return self._cut(form, sequence, begin, end, head, tiles, keys, merges)
+
+    def _cut(self, form, sequence, begin, end, head, tiles, keys, merges):
+        """Items of row blocks (arrays, one entry to a block) of ``tiles`` key tiles; ``keys`` gives the key range of
+        parts ``(block, first tile, last tile, part, parts)``."""
         owner = sequence * self.cache.heads + head
         which, low, high, xcd = _share_out(tiles, owner, self._resident(form), _OVERHEAD[form]).T
-        parts = np.bincount(which, minlength=len(blocks))
+        parts = np.bincount(which, minlength=len(tiles))
         part = np.arange(len(which)) - np.repeat(np.cumsum(parts) - parts, parts)
         n = parts[which]
         rows = (end - begin)[which]
@@ -241,9 +266,9 @@ class AttentionPlan:
         items[:, 2] = self._starts[sequence][which]
         items[:, 3] = self._counts[sequence][which]
         items[:, 4], items[:, 5], items[:, 6] = begin[which], end[which], head[which]
-        items[:, 7] = np.where(part == 0, first[which], self._key_of(tile0[which] + low))
-        items[:, 8] = np.where(part == n - 1, last[which], np.minimum(last[which], self._key_of(tile0[which] + high)))
+        items[:, 7], items[:, 8] = keys(which, low, high, part, n)
         items[:, 9] = np.where(n > 1, base[which] + part * rows, -1)
+        items[:, 10] = self._lists_of(which)
         several = parts > 1
         if several.any():
             rows = (end - begin)[several]
@@ -252,6 +277,10 @@ class AttentionPlan:
             merge[:, 3], merge[:, 4], merge[:, 5] = head[several], base[several], parts[several]
             merges.append(merge)
         return self._ordered(items, high - low, xcd)
+
+    def _lists_of(self, which):
+        """Where the chosen blocks of row blocks stand among the lists."""
+        return 0
 
     @staticmethod
     def _ordered(items, cost, xcd):
@@ -270,10 +299,11 @@ class AttentionPlan:
 
     def _check(self, keys, values):
         cache = self.cache
+        need(not cache.codes, "pools in codes are attended to by their cache (QuantizedCache.attend), which has their scales")
         shape, k_stride, v_stride = cache.keys.shape[1:], cache.keys.stride()[1:], cache.values.stride()[1:]
         for pool, stride, name in ((keys, k_stride, "keys"), (values, v_stride, "values")):
             in_memory(pool, name)
-            need(pool.shape == shape and pool.stride() == stride and pool.dtype == cache.dtype
+            need(pool.shape == shape and pool.stride() == stride and pool.dtype == cache.keys.dtype
                  and pool.device == cache.device, f"{name} must be a layer's pool like those of the plan's cache")
             need(self._tiled == 0 or pool.data_ptr() % 16 == 0, f"{name} must be aligned as the plan's cache is")
             need(not (pool.requires_grad and torch.is_grad_enabled()),
@@ -288,7 +318,7 @@ class AttentionPlan:
         fields = (0, 0, 0, 0, 0, 0, 0, *q_stride, k[page], k[token], k[head], v[page], v[token], v[head], *out_stride,
                   self.group, self.heads, cache.head_dim, cache.page_tokens, cache.pages, self.block or 0, self.window or 0,
                   scale, self._partial_rows, self._items, *self._counts_of, self._merges, self._n_merges, self._n_many,
-                  *self._most_rows, self._holes, self._unit())
+                  *self._most_rows, self._holes, self._unit(), cache.codes, 0, 0, *cache._scale_strides(), 0, self._block_tokens)
         return bytes(_Image(*fields))
 
 
@@ -310,13 +340,18 @@ def attend(q, keys, values, plan, *, out=None, return_lse=False):
     queries as the pools hold them: both are rotated before.  Runs on the current stream; not
     differentiable.  Returns ``out``, or ``(out, lse)``.
     """
-    need(isinstance(plan, AttentionPlan), "attend needs an AttentionPlan")
+    need(isinstance(plan, AttentionPlan) and not plan._block_tokens,
+         "attend needs an AttentionPlan (a BlockPlan goes with BlockIndex.attend)")
     plan._check(keys, values)
     return run(q, keys.data_ptr(), values.data_ptr(), plan, out, return_lse, (keys, values))
 
 
-def run(q, k_address, v_address, plan, out, return_lse, pools=None):
-    """:func:`attend` over a layer's checked pools, given by their addresses."""
+_SCALES_AT, _LISTS_AT = _lib.ATTEND_FIELDS.index("k_scale_ptr"), _lib.ATTEND_FIELDS.index("lists_ptr")
+
+
+def run(q, k_address, v_address, plan, out, return_lse, pools=None, scales=(0, 0), lists=0):
+    """:func:`attend` over a layer's checked pools, given by their addresses (and those of the scales of pools in codes, and
+    of the lists of chosen blocks)."""
     cache = plan.cache
     if plan._stamp != cache._moved:
         raise StateError("pages moved or were freed after this plan was built")
@@ -359,6 +394,8 @@ def run(q, k_address, v_address, plan, out, return_lse, pools=None):
             if stream != plan._stream:  # the allocator learns of a stream that the tables were not made on
                 plan.buffer.record_stream(torch.cuda.current_stream(device))
             fields[0], fields[1], fields[2], fields[3] = q.data_ptr(), k_address, v_address, result.data_ptr()
+            fields[_SCALES_AT], fields[_SCALES_AT + 1] = scales
+            fields[_LISTS_AT] = lists
             fields[4], fields[5] = 0 if lse is None else lse.data_ptr(), plan.buffer.data_ptr()
             _lib.check(_lib.function("rch_attend_run")(fields, _DTYPE_CODES[q.dtype], stream))
             if result is not out:

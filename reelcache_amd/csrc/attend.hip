@@ -11,18 +11,32 @@
 // by element: single tokens of 4 sequences of 4000 tokens, 16 heads of 250 bf16, take 450 us (0.57 TB/s).  Only
 // pools, or head sizes, whose rows are no 16-byte pieces come here, and pools whose token rows lie more than 2^22
 // elements apart; the form that tiles for the matrix cores (16 heads of 200: 80 us) is in attend_rows.hip.
+#include <type_traits>
+
 #include "attend.h"
+#include "codes.h"
 
 namespace rch {
 
 namespace {
 
-template <int DT>
+// What an element of a pool stands for.
+template <typename T, int FMT, typename Held>
+__device__ __forceinline__ float held_value(Held x, float scale) {
+    if constexpr (FMT == RCH_CODES_NONE) return static_cast<float>(x);
+    else return static_cast<float>(code_value<FMT, T>(x, scale));
+}
+
+// FMT: what the pools hold (RCH_CODES_*).  LIST: the keys are those of chosen blocks, block after block.
+template <int DT, int FMT, bool LIST>
 __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A) {
     typedef typename AttendType<DT>::type T;
+    typedef std::conditional_t<FMT == RCH_CODES_NONE, T, uint8_t> Held;
+    constexpr int kTile = DT == RCH_DT_F32 ? 32 : 64;  // of a list's tiles
     __shared__ float query[4][RCH_ATTEND_MAX_DIM];
     __shared__ float weight[4][64];
     __shared__ int64_t place_of[4][64];
+    __shared__ float scale_of[FMT == RCH_CODES_NONE ? 1 : 4][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const AttendItem I = attend_item(A, blockIdx.x);
     const int dim = static_cast<int>(A.head_dim), group = static_cast<int>(A.group);
@@ -35,7 +49,6 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A)
         const int token = row / group, head = I.kv_head * group + row % group;
         int begin, end;
         attend_range(A, I, token, begin, end);
-        const int from = begin > I.key_begin ? begin : I.key_begin, to = end < I.key_end ? end : I.key_end;
         const RCH_GLOBAL T* q = gin<T>(A.q_ptr) + (I.q_row + token) * A.q_token_stride + head * A.q_head_stride;
         __builtin_amdgcn_wave_barrier();
         for (int d = lane; d < dim; d += 64) query[wave][d] = static_cast<float>(q[d]);
@@ -45,22 +58,24 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A)
         bool blank = false;  // a key was seen
 #pragma unroll
         for (int c = 0; c < RCH_ATTEND_MAX_DIM / 64; ++c) acc[c] = 0.0f;
-        for (int base = from; base < to; base += 64) {
+        auto look = [&](const int base, const int from, const int to) {
             const int key = base + lane;
-            bool seen = key < to;
+            bool seen = key >= from && key < to;
             int page = -1;
             if (seen) page = table[key / size];
             seen = seen && page >= 0 && page < A.pages;
             const int in_page = key % size;
             float score = -INFINITY;
             if (seen) {
-                const RCH_GLOBAL T* k = gin<T>(A.k_ptr) + page * A.k_page_stride + in_page * A.k_token_stride + k_head;
-                float dot = 0.0f;
-                for (int d = 0; d < dim; ++d) dot = __builtin_fmaf(query[wave][d], static_cast<float>(k[d]), dot);
+                const RCH_GLOBAL Held* k = gin<Held>(A.k_ptr) + page * A.k_page_stride + in_page * A.k_token_stride + k_head;
+                float dot = 0.0f, unit = 0.0f;
+                if constexpr (FMT != RCH_CODES_NONE)
+                    unit = gin<float>(A.k_scale_ptr)[page * A.k_scale_page_stride + I.kv_head * A.k_scale_head_stride + in_page];
+                for (int d = 0; d < dim; ++d) dot = __builtin_fmaf(query[wave][d], held_value<T, FMT>(k[d], unit), dot);
                 score = dot * scale;
             }
             uint64_t left = __ballot(seen);
-            if (left == 0) continue;
+            if (left == 0) return;
             blank = true;
             float top = score;
 #pragma unroll
@@ -75,6 +90,9 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A)
             __builtin_amdgcn_wave_barrier();
             weight[wave][lane] = w;
             place_of[wave][lane] = page * A.v_page_stride + in_page * A.v_token_stride + v_head;
+            if constexpr (FMT != RCH_CODES_NONE)
+                scale_of[wave][lane] =
+                    seen ? gin<float>(A.v_scale_ptr)[page * A.v_scale_page_stride + I.kv_head * A.v_scale_head_stride + in_page] : 0.0f;
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -83,11 +101,27 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A)
                 const int j = __builtin_ctzll(left);
                 left &= left - 1;
                 const float wj = weight[wave][j];
-                const RCH_GLOBAL T* v = gin<T>(A.v_ptr) + place_of[wave][j];
+                const RCH_GLOBAL Held* v = gin<Held>(A.v_ptr) + place_of[wave][j];
+                const float unit = FMT == RCH_CODES_NONE ? 0.0f : scale_of[FMT == RCH_CODES_NONE ? 0 : wave][j];
 #pragma unroll
                 for (int c = 0; c < RCH_ATTEND_MAX_DIM / 64; ++c)
-                    if (lane + 64 * c < dim) acc[c] = __builtin_fmaf(wj, static_cast<float>(v[lane + 64 * c]), acc[c]);
+                    if (lane + 64 * c < dim) acc[c] = __builtin_fmaf(wj, held_value<T, FMT>(v[lane + 64 * c], unit), acc[c]);
             }
+        };
+        if constexpr (LIST) {
+            const RCH_GLOBAL int32_t* list = gin<int32_t>(A.lists_ptr) + I.list;
+            const int unit = static_cast<int>(A.block_tokens), per = (unit + kTile - 1) / kTile, blocks = (I.length + unit - 1) / unit;
+            for (int tile = I.key_begin; tile < I.key_end;) {
+                const int block = list[tile / per], sub = tile % per, tiles = min(per - sub, I.key_end - tile);
+                tile += tiles;
+                if (block < 0 || block >= blocks) continue;
+                const int first = block * unit + sub * kTile;
+                const int last = min(min(first + tiles * kTile, block * unit + unit), end);
+                for (int base = first; base < last; base += 64) look(base, begin, last);
+            }
+        } else {
+            const int from = begin > I.key_begin ? begin : I.key_begin, to = end < I.key_end ? end : I.key_end;
+            for (int base = from; base < to; base += 64) look(base, from, to);
         }
         if (I.part >= 0) {
             const int64_t at = I.part + row - I.row_begin;
@@ -274,10 +308,33 @@ int merge_few(const rch_attend& A, hipStream_t stream) {
     return check_launch("rch_attend_run (merge)");
 }
 
+template <int DT, int FMT>
+void general(const rch_attend& A, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(A.n_general));
+    if (A.lists_ptr) hipLaunchKernelGGL((attend_general_kernel<DT, FMT, true>), grid, dim3(256), 0, stream, A);
+    else hipLaunchKernelGGL((attend_general_kernel<DT, FMT, false>), grid, dim3(256), 0, stream, A);
+}
+
+template <int DT>
+int items(const rch_attend& A, hipStream_t stream) {
+    if (!A.n_general) {
+        if (A.codes == RCH_CODES_INT8) return launch_attend_int8(A, DT, stream);
+        if (A.codes == RCH_CODES_E4M3) return launch_attend_e4m3(A, DT, stream);
+        return A.lists_ptr ? launch_attend_lists(A, DT, stream) : launch_attend_rows(A, DT, stream);
+    }
+    if constexpr (DT == RCH_DT_F32) {
+        general<DT, RCH_CODES_NONE>(A, stream);
+    } else {
+        if (A.codes == RCH_CODES_INT8) general<DT, RCH_CODES_INT8>(A, stream);
+        else if (A.codes == RCH_CODES_E4M3) general<DT, RCH_CODES_E4M3>(A, stream);
+        else general<DT, RCH_CODES_NONE>(A, stream);
+    }
+    return check_launch("rch_attend_run");
+}
+
 template <int DT>
 int run(const rch_attend& A, hipStream_t stream) {
-    if (A.n_general) hipLaunchKernelGGL(attend_general_kernel<DT>, dim3(static_cast<uint32_t>(A.n_general)), dim3(256), 0, stream, A);
-    const int status = A.n_general ? check_launch("rch_attend_run") : launch_attend_rows(A, DT, stream);
+    const int status = items<DT>(A, stream);
     if (status != RCH_OK) return status;
     if (A.n_many) {
         const int status = A.head_dim <= 128 ? merge_many<DT, 2>(A, stream) : merge_many<DT, 4>(A, stream);
@@ -316,19 +373,26 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
     const uint32_t scale = static_cast<uint32_t>(A.scale_bits);
     if (scale < 0x00800000u || scale >= 0x7f800000u) return fail(RCH_E_CONFIG, "rch_attend_run: scale must be a positive normal number");
     if (!A.q_ptr || !A.k_ptr || !A.v_ptr || !A.out_ptr || !A.plan_ptr) return fail(RCH_E_CONFIG, "rch_attend_run: null address");
+    if (A.codes != RCH_CODES_NONE) {
+        if (A.codes != RCH_CODES_INT8 && A.codes != RCH_CODES_E4M3) return fail(RCH_E_CONFIG, "rch_attend_run: unknown format of codes");
+        if (dtype == RCH_DT_F32) return fail(RCH_E_UNSUPPORTED, "rch_attend_run: codes stand for f16 or bf16 values");
+        if (!A.k_scale_ptr || !A.v_scale_ptr || (A.k_scale_ptr | A.v_scale_ptr) % 4) return fail(RCH_E_CONFIG, "rch_attend_run: pools in codes need their scales");
+    }
+    if (A.lists_ptr && (A.block_tokens < 1 || A.page_tokens % A.block_tokens || A.lists_ptr % 4))
+        return fail(RCH_E_CONFIG, "rch_attend_run: chosen blocks divide a page");
     if (A.n_rows) {
         // The tiled forms: whole 16-byte pieces, a tile's rows within 2 GiB, tiles that start over at a page of
-        // at least a tile or at 64 keys.
-        const int64_t size = dtype == RCH_DT_F32 ? 4 : 2;
-        const int64_t mix = A.q_token_stride | A.q_head_stride | A.k_page_stride | A.k_token_stride | A.k_head_stride
-                            | A.v_page_stride | A.v_token_stride | A.v_head_stride | A.out_token_stride | A.out_head_stride;
-        if (A.head_dim * size % 16 || A.head_dim > RCH_ATTEND_FAST_DIM || mix * size % 16
+        // at least a tile or at 64 keys (or at each chosen block).
+        const int64_t size = dtype == RCH_DT_F32 ? 4 : 2, held = A.codes == RCH_CODES_NONE ? size : 1;
+        const int64_t mix = (A.q_token_stride | A.q_head_stride | A.out_token_stride | A.out_head_stride) * size
+                            | (A.k_page_stride | A.k_token_stride | A.k_head_stride | A.v_page_stride | A.v_token_stride | A.v_head_stride) * held;
+        if (A.head_dim * held % 16 || A.head_dim > RCH_ATTEND_FAST_DIM || mix % 16
             || (A.q_ptr | A.k_ptr | A.v_ptr | A.out_ptr | A.plan_ptr) % 16)
             return fail(RCH_E_UNSUPPORTED, "rch_attend_run: the tiled form needs aligned rows of whole 16-byte pieces and at most %d channels",
                         RCH_ATTEND_FAST_DIM);
         if (A.k_token_stride < 0 || A.v_token_stride < 0 || A.k_token_stride > (1 << 22) || A.v_token_stride > (1 << 22))
             return fail(RCH_E_UNSUPPORTED, "rch_attend_run: token rows too far apart for the tiled forms");
-        if (!(A.tile_unit == 64 || (A.tile_unit == A.page_tokens && A.page_tokens >= 64)))
+        if (!A.lists_ptr && !(A.tile_unit == 64 || (A.tile_unit == A.page_tokens && A.page_tokens >= 64)))
             return fail(RCH_E_CONFIG, "rch_attend_run: tiles start over at a page of 64 or more tokens, or at 64 keys");
     }
     hipStream_t s = as_stream(stream);

@@ -155,11 +155,25 @@ __device__ __forceinline__ int page_entry(const const_int* table, int index) {
 // How a tile's rows are found: kPage: tiles start over at each page and lie in one page; kShare: a tile is KT
 // consecutive keys, and the KT / 4 rows that a wave fetches lie in one page (its size is a multiple of that);
 // kRow: any page size.  The first two take a scalar base to a fetch, the last an address to a lane.
-enum TileMode { kPage, kShare, kRow };
+// kList: chosen blocks of keys, one after the other; a block lies in one page and tiles start over at each.
+enum TileMode { kPage, kShare, kRow, kList };
+
+// The page of a walk's tile and the tile's first row there, for those who ask (pools in codes find the rows' scales by it).
+template <bool KEPT>
+struct TilePlace {
+    __device__ __forceinline__ void stand(int, int) {}
+    __device__ __forceinline__ void step(int) {}
+};
+template <>
+struct TilePlace<true> {
+    int id, in_page;
+    __device__ __forceinline__ void stand(int page, int row) { id = page, in_page = row; }
+    __device__ __forceinline__ void step(int rows) { in_page += rows; }
+};
 
 // The walk over an item's key tiles.
-template <int KT, int MODE>
-struct KeyWalk {
+template <int KT, int MODE, bool KEPT = false>
+struct KeyWalk : TilePlace<KEPT> {
     const const_int* table;
     int unit, end, pages;     // tokens that tiles start over at, last key, pages of the pool
     int base, left, page;     // current tile: first key, keys from it to the unit's end, page index (kPage)
@@ -175,6 +189,7 @@ struct KeyWalk {
             if (id >= 0 && id < pages) {
                 k = k_head + id * k_page + static_cast<int64_t>(off / KT) * k_tile;
                 v = v_head + id * v_page + static_cast<int64_t>(off / KT) * v_tile;
+                this->stand(id, off);
                 return;
             }
             base += left;
@@ -207,6 +222,7 @@ struct KeyWalk {
                 left -= KT;
                 k += k_tile;
                 v += v_tile;
+                this->step(KT);
                 return;
             }
             base += left;
@@ -219,6 +235,77 @@ struct KeyWalk {
     }
     // Keys of the current tile.
     __device__ __forceinline__ int count() const { return min(end - base, MODE == kPage ? min(left, KT) : KT); }
+};
+
+// The walk over the tiles of an item's chosen blocks.
+template <int KT, bool KEPT>
+struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
+    const const_int *table, *entry;
+    int unit, end, pages, size, blocks;  // tokens of a block, keys and blocks of the sequence, tokens of a page
+    int tiles;                           // of the item, the current one among them
+    int base, left;                      // current tile: first key, keys from it to the block's end
+    int64_t k, v, k_head, v_head, k_page, v_page;
+    int k_tile, v_tile, k_row, v_row;
+
+    __device__ __forceinline__ bool done() const { return tiles <= 0; }
+    // Enters the block of `entry` at its tile `sub`, skipping entries without keys.
+    __device__ __forceinline__ void enter(int sub) {
+        while (tiles > 0) {
+            const int block = *entry;
+            if (block >= 0 && block < blocks) {
+                const int first = block * unit, index = first / size;
+                const int id = table[index];
+                // (a tile behind the sequence's last key has none either)
+                if (id >= 0 && id < pages && first + sub * KT < end) {
+                    const int in_page = first - index * size + sub * KT;
+                    this->stand(id, in_page);
+                    k = k_head + id * k_page + in_page * static_cast<int64_t>(k_row);
+                    v = v_head + id * v_page + in_page * static_cast<int64_t>(v_row);
+                    base = first + sub * KT;
+                    left = unit - sub * KT;
+                    return;
+                }
+            }
+            tiles -= (unit + KT - 1) / KT - sub;
+            sub = 0;
+            ++entry;
+        }
+    }
+    __device__ __forceinline__ void begin(const rch_attend& A, const AttendItem& I, int es) {
+        table = (const const_int*)(uintptr_t)(A.plan_ptr + 4 * static_cast<int64_t>(I.table));
+        unit = static_cast<int>(A.block_tokens);
+        size = static_cast<int>(A.page_tokens);
+        end = I.length;
+        blocks = (end + unit - 1) / unit;
+        pages = static_cast<int>(A.pages);
+        k_head = A.k_ptr + es * I.kv_head * A.k_head_stride;
+        v_head = A.v_ptr + es * I.kv_head * A.v_head_stride;
+        k_page = es * A.k_page_stride;
+        v_page = es * A.v_page_stride;
+        k_row = static_cast<int>(es * A.k_token_stride);
+        v_row = static_cast<int>(es * A.v_token_stride);
+        k_tile = KT * k_row;
+        v_tile = KT * v_row;
+        const int per = (unit + KT - 1) / KT, at = I.key_begin / per;
+        entry = (const const_int*)(uintptr_t)(A.lists_ptr + 4 * static_cast<int64_t>(I.list)) + at;
+        tiles = I.key_end - I.key_begin;
+        enter(I.key_begin - at * per);
+    }
+    __device__ __forceinline__ void next() {
+        --tiles;
+        if (left > KT && base + KT < end) {
+            base += KT;
+            left -= KT;
+            k += k_tile;
+            v += v_tile;
+            this->step(KT);
+            return;
+        }
+        tiles -= (left - 1) / KT;  // tiles of the block behind the sequence's last key
+        ++entry;
+        enter(0);
+    }
+    __device__ __forceinline__ int count() const { return min(end - base, min(left, KT)); }
 };
 
 // Fetches the calling wave's quarter of a K and a V tile: NI instructions of 1024 bytes each.  Tile: the
@@ -245,7 +332,7 @@ struct Fetch {
         if constexpr (MODE != kRow) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int row = row0 + i * kRows, from = MODE == kPage ? row : row - share;
+                const int row = row0 + i * kRows, from = MODE == kShare ? row - share : row;
                 const int kc = piece ^ Tile::k_swizzle(row), vc = piece ^ Tile::v_swizzle(row);
                 k_at[i] = kc < pieces ? from * k_row + kc * 16 : kOutOfRange;
                 v_at[i] = vc < pieces ? from * v_row + vc * 16 : kOutOfRange;
@@ -260,15 +347,17 @@ struct Fetch {
     // Looks up the pages of the walk's tile (called when the walk arrives there, a tile before its fetch, so that
     // the fetch waits for no table).
     __device__ __forceinline__ void look_up(const KeyWalk<KT, MODE>& W) {
-        if (MODE == kPage || W.done()) return;
-        const int keys = W.end - W.base, page0 = W.base / static_cast<int>(size);
-        const int off0 = W.base - page0 * static_cast<int>(size);
-        // Rows behind the last key: its page.
-        if constexpr (MODE == kShare) {
-            ids[0] = W.table[page0 + page_of(off0 + min(share, keys - 1))];
-        } else {
+        if constexpr (MODE == kShare || MODE == kRow) {
+            if (W.done()) return;
+            const int keys = W.end - W.base, page0 = W.base / static_cast<int>(size);
+            const int off0 = W.base - page0 * static_cast<int>(size);
+            // Rows behind the last key: its page.
+            if constexpr (MODE == kShare) {
+                ids[0] = W.table[page0 + page_of(off0 + min(share, keys - 1))];
+            } else {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) ids[i] = page_entry(W.table, page0 + page_of(off0 + min(row0 + i * kRows, keys - 1)));
+                for (int i = 0; i < NI; ++i) ids[i] = page_entry(W.table, page0 + page_of(off0 + min(row0 + i * kRows, keys - 1)));
+            }
         }
     }
 

@@ -13,7 +13,7 @@
 // of 16 / 1024 / 4680 / 18720 tokens x 12 heads x 128 bf16 take 4.6 / 5.7 / 12.4 / 36.3 us (the last
 // 6.3 TB/s, mostly from the caches), with one head 4.5 / 6.6 / 18.0 / 57.3, two 4.5 / 5.8 / 13.8 / 38.6,
 // eight 4.4 / 5.9 / 12.2 / 36.5.
-#include "common.h"
+#include "turn.h"
 
 namespace rch {
 
@@ -83,13 +83,6 @@ __device__ __forceinline__ void store_piece(RCH_GLOBAL T* p, const Piece<T, N>& 
     }
 }
 
-__device__ __forceinline__ void rotate_pair(float& e, float& o, float c, float s) {
-    const float re = __fsub_rn(__fmul_rn(e, c), __fmul_rn(o, s));
-    const float ro = __fadd_rn(__fmul_rn(e, s), __fmul_rn(o, c));
-    e = re;
-    o = ro;
-}
-
 // One piece is V channels: V / 2 interleaved pairs, or V pairs of the half pairing (channels j and
 // pairs + j: two pieces).  V = 8 and V = 4 need rows aligned to a piece (16 bytes at most) and widths of
 // whole pieces; V = 2 (interleaved) and 1 (half, or no rotation) take everything else.
@@ -134,33 +127,14 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryJobs jobs) {
         return;
     }
 
-    // The token's place on each axis; a row outside its axis turns to NaN (nothing is read there).
     int row[3];
-    if (J.rows_ptr) {
-        const RCH_GLOBAL int32_t* r = gin<int32_t>(J.rows_ptr) + batch * J.rows_batch_stride + token * J.rows_token_stride;
-#pragma unroll
-        for (int a = 0; a < 3; ++a) row[a] = a < J.axes ? r[a * J.rows_axis_stride] : 0;
-    } else if (J.axes == 3) {
-        const int t = static_cast<int>(token), plane = static_cast<int>(J.grid_h * J.grid_w), w = static_cast<int>(J.grid_w);
-        const int f = t / plane, y = (t - f * plane) / w;
-        row[0] = static_cast<int>(J.row_t) + f;
-        row[1] = static_cast<int>(J.row_h) + y;
-        row[2] = static_cast<int>(J.row_w) + t - f * plane - y * w;
-    } else {
-        row[0] = static_cast<int>(J.row_t + token);
-        row[1] = row[2] = 0;
-    }
-    const int bound1 = static_cast<int>(J.sec_t), bound2 = bound1 + static_cast<int>(J.sec_h);
+    turning_rows(J, batch, token, row);
     constexpr int P = HALF ? V : V / 2;
     const int j0 = piece * P;
     float c[P], s[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const int j = j0 + i, axis = J.axes == 1 ? 0 : (j < bound1 ? 0 : (j < bound2 ? 1 : 2));
-        const int r = axis == 0 ? row[0] : (axis == 1 ? row[1] : row[2]);
-        const int64_t limit = axis == 0 ? J.limit_t : (axis == 1 ? J.limit_h : J.limit_w);
-        f2 pair = {__builtin_nanf(""), __builtin_nanf("")};
-        if (r >= 0 && r < limit) pair = gin<f2>(J.pairs_ptr)[static_cast<int64_t>(r) * pairs + j];
+        const f2 pair = turning_angle(J, row, j0 + i);
         c[i] = pair[0];
         s[i] = J.inverse ? -pair[1] : pair[1];
     }

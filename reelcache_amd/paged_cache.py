@@ -52,6 +52,11 @@ class Slots(Remembering):
     stream: int
 
 
+class Places(Slots):
+    """The rows that tokens lie in, for reading them: built by :meth:`PagedCache.places`.  Their pages may be shared; no
+    store takes them."""
+
+
 @dataclass(frozen=True, eq=False)
 class PageView(NativeView):
     """A restore destination in a sequence's pages (:meth:`PagedCache.view`).  A restore into it is refused
@@ -133,12 +138,16 @@ class PagedCache:
     with unit stride over the channels; any other strides that keep elements apart.
     """
 
+    _POOL_DTYPES, _POOL_TYPES = OUTPUT_DTYPES, "bfloat16, float16 or float32"
+    #: What the pools hold besides values (RCH_CODES_*).
+    codes = _lib.CODES_NONE
+
     def __init__(self, keys, values, *, layout="BTHD"):
         one_of(layout, _LAYOUTS, "pool layout")
         for pool, name in ((keys, "keys"), (values, "values")):
             in_memory(pool, name)
             need(pool.ndim == 5, f"{name} must be [layers, pages, ...] pools of five dimensions")
-            need(pool.dtype in OUTPUT_DTYPES, f"{name} must be bfloat16, float16 or float32")
+            need(pool.dtype in self._POOL_DTYPES, f"{name} must be {self._POOL_TYPES}")
             need(min(pool.shape) >= 1, f"{name} must not be empty")
             need(pool.stride(4) == 1 or pool.shape[4] == 1, f"{name} must have unit stride over the channels")
             need(_apart(pool), f"{name} must keep its elements apart")
@@ -165,6 +174,9 @@ class PagedCache:
         self._moved = 0   # counts what may move or reuse pages: plans and slots built before it are stale
         self._shared = 0  # counts what may share pages: slots built before it are stale
         self._copies = None
+        # What moves along with the pages, as pools [layers, pages, rows or heads, .., width]: (tensor, (page, row, head) axes,
+        # tokens of a row).
+        self._along = []
 
     @classmethod
     def allocate(cls, pages, page_tokens, heads, head_dim, *, layers=1, dtype=torch.bfloat16, device="cuda", layout="BTHD"):
@@ -326,22 +338,32 @@ class PagedCache:
     def slots(self, sequences, starts, counts):
         """The :class:`Slots` of tokens ``starts[i] .. starts[i] + counts[i]`` that ``sequences[i]`` has
         (rows to write again).  Their pages must not be shared."""
+        return self._slots(*self._stretches(sequences, starts, counts, "slots", False))
+
+    def places(self, sequences, starts, counts):
+        """The :class:`Places` of tokens ``starts[i] .. starts[i] + counts[i]`` that ``sequences[i]`` has, to read them.
+        Their pages may be shared."""
+        return self._slots(*self._stretches(sequences, starts, counts, "places", True), Places)
+
+    def _stretches(self, sequences, starts, counts, what, shared):
+        """Checked (sequences, starts, counts) of tokens that lie in pages."""
         found = self._several(sequences)
         starts, counts = list(starts), list(counts)
-        need(len(starts) == len(counts) == len(found), "slots take one start and count for each sequence")
+        need(len(starts) == len(counts) == len(found), f"{what} take one start and count for each sequence")
         for item, start, n in zip(found, starts, counts):
-            need(count(start, "a start") + count(n, "a token count") <= item.tokens, "slots lie within the sequence")
+            need(count(start, "a start") + count(n, "a token count") <= item.tokens, f"{what} lie within the sequence")
             if n == 0:
                 continue
             for page in item.pages[start // self.page_tokens:(start + n - 1) // self.page_tokens + 1]:
                 if page == HOLE:
-                    raise StateError("the slots' page was dropped")
-                if self._uses[page] > 1:
-                    raise StateError("the slots' page is shared with another sequence")
+                    raise StateError(f"the {what}' page was dropped")
+                if self._uses[page] > 1 and not shared:
+                    raise StateError(f"the {what}' page is shared with another sequence")
+        need(sum(counts) < 1 << 31, f"{what} cover fewer than 2**31 tokens")
         need_gpu(self.device, "a paged cache")
-        return self._slots(found, starts, counts)
+        return found, starts, counts
 
-    def _slots(self, found, starts, counts):
+    def _slots(self, found, starts, counts, kind=Slots):
         size = self.page_tokens
         pieces = sum([-(-(start + n) // size) - start // size for start, n in zip(starts, counts) if n])
         if pieces <= _FEW_RUNS:
@@ -354,7 +376,7 @@ class PagedCache:
                     at += n
                     left -= n
             with entered(self.device):
-                return self._made(upload_runs(runs, sum(counts), self.device))
+                return self._made(upload_runs(runs, sum(counts), self.device), kind)
         pages, base = [], []  # the pages of all tokens, and where each sequence's page 0 would lie among them
         for item, start, n in zip(found, starts, counts):
             first = start // size
@@ -369,10 +391,18 @@ class PagedCache:
         if total:
             index += np.asarray(pages, dtype=np.int64)[page + np.repeat(np.asarray(base, dtype=np.int64), counts)] * size
         with entered(self.device):
-            return self._made(upload(index, self.device))
+            return self._made(upload(index, self.device), kind)
 
-    def _made(self, index):
-        return Slots(index, index.shape[0], self, self._moved + self._shared, raw_stream(self.device))
+    def _made(self, index, kind):
+        stamp = self._moved if kind is Places else self._moved + self._shared
+        return kind(index, index.shape[0], self, stamp, raw_stream(self.device))
+
+    def _current(self, slots):
+        """Refuses slots and places of other caches, and those that pages have moved behind."""
+        if not isinstance(slots, Slots) or slots.cache is not self:
+            raise ConfigurationError("slots come from this cache")
+        if slots.stamp != (self._moved if isinstance(slots, Places) else self._moved + self._shared):
+            raise StateError("pages moved, were freed or became shared after these slots were built")
 
     # -----------------------------------------------------------------------------------------
     # Page copies
@@ -390,15 +420,26 @@ class PagedCache:
         with entered(self.device):
             where = self.keys.data_ptr(), self.values.data_ptr()
             if self._copies is None or self._copies[0] != where:  # a copied cache has pools of its own
-                self._copies = where, [_pools(pool, self._axes, self.pages, self.page_tokens)
+                self._copies = where, [(1, *_pools(pool, self._axes, self.pages, self.page_tokens))
                                        for pool in self._joined_pools()]
+                self._copies[1].extend((tokens, *_pools((pool,), axes, self.pages, pool.shape[axes[1]]))
+                                       for pool, axes, tokens in self._along)
             table, stream = _pack(moves), raw_stream(self.device)
-            for pools, fields, streams in self._copies[1]:
+            for tokens, pools, fields, streams in self._copies[1]:
+                if tokens > 1:  # a row stands for several tokens: the begun one too
+                    table = _pack([-(-word // tokens) if i % 3 == 2 else word for i, word in enumerate(moves)])
                 if stream not in streams:  # the allocator learns of a stream that the table was not made on
                     pools.record_stream(torch.cuda.current_stream(self.device))
                     streams.add(stream)
                 _lib.check(_lib.function("rch_pages_copy")(fields, table, len(moves) // 3, stream))
             torch.autograd.graph.increment_version(self._counted)
+
+    def _take_along(self, pool, axes, tokens=1):
+        """Page copies move a further pool from now on."""
+        self._along.append((pool, axes, tokens))
+        self._copies = None
+        if not pool.is_inference():
+            self._counted += (pool,)
 
     def _joined_pools(self):
         """K and V pools as one group where their strides agree (one launch), else as two."""
@@ -526,10 +567,9 @@ class PagedCache:
         copied first).  With a ``grid`` the tokens are one chunk."""
         if type(layer) is not int or not 0 <= layer < self.layers:
             raise ConfigurationError("there is no such layer")
-        if not isinstance(slots, Slots) or slots.cache is not self:
-            raise ConfigurationError("slots come from this cache")
-        if slots.stamp != self._moved + self._shared:
-            raise StateError("pages moved, were freed or became shared after these slots were built")
+        self._current(slots)
+        if isinstance(slots, Places):
+            raise ConfigurationError("a store takes slots, not places")
         shape = (slots.tokens, self.heads, self.head_dim)
         for x, name in ((keys, "keys"), (values, "values")):
             in_memory(x, name)
@@ -560,11 +600,14 @@ class PagedCache:
                     # Rows of the pool itself, which are written while others are still read: of copies.
                     return self.store(layer, slots, *[x.clone(memory_format=torch.contiguous_format) for x in (keys, values)],
                                       positions=positions, grid=grid)
-            launch([(k, pools[0], True), (v, pools[1], False)],
-                   *addresses_of(positions, self.device, stream), slots.index.data_ptr(), stream)
+            self._launch_store(launch, layer, (k, v), pools, addresses_of(positions, self.device, stream),
+                               slots.index.data_ptr(), stream)
             if stream != slots.stream:  # the allocator learns of a stream that the index was not made on
                 slots.index.record_stream(torch.cuda.current_stream(self.device))
             torch._C._increment_version(self._counted)
+
+    def _launch_store(self, launch, layer, sources, pools, turned, slots, stream):
+        launch([(sources[0], pools[0], True), (sources[1], pools[1], False)], *turned, slots, stream)
 
     def _store_launch(self, sources, positions, grid, tokens):
         turned = position_fields(positions, grid, tokens, 1, self.head_dim, self.device)
@@ -592,10 +635,29 @@ class PagedCache:
 
         if type(layer) is not int or not 0 <= layer < self.layers:
             raise ConfigurationError("there is no such layer")
-        if not isinstance(plan, AttentionPlan) or plan.cache is not self:
+        if not isinstance(plan, AttentionPlan) or plan.cache is not self or plan._block_tokens:
             return attend(q, *self._layer(layer), plan, out=out, return_lse=return_lse)
         k_bytes, v_bytes = self._layer_bytes
-        return run(q, self.keys.data_ptr() + layer * k_bytes, self.values.data_ptr() + layer * v_bytes, plan, out, return_lse)
+        return run(q, self.keys.data_ptr() + layer * k_bytes, self.values.data_ptr() + layer * v_bytes, plan, out, return_lse,
+                   self._pools(), self._scales(layer))
+
+    def _pools(self):
+        """What no output may overlap."""
+        return self.keys, self.values
+
+    def _scales(self, layer):
+        """Addresses of a layer's scales, of pools in codes."""
+        return 0, 0
+
+    def _scale_strides(self):
+        """(page, head) strides of the keys' and the values' scales."""
+        return 0, 0, 0, 0
+
+    def index(self, block_tokens):
+        """A new :class:`~reelcache_amd.sparse_attention.BlockIndex` of the keys, in blocks of ``block_tokens``."""
+        from .sparse_attention import BlockIndex
+
+        return BlockIndex.allocate(self, block_tokens)
 
 
 def _apart(pool):
@@ -634,4 +696,4 @@ def _pools(group, axes, pages, page_tokens):
     return table, (ctypes.c_int64 * len(fields))(*fields), {raw_stream(group[0].device)}
 
 
-__all__ = ["HOLE", "PageView", "PagedCache", "Slots"]
+__all__ = ["HOLE", "PageView", "PagedCache", "Places", "Slots"]

@@ -1,0 +1,371 @@
+"""``BlockIndex`` on the GPU: means of key blocks, their choice, attention to the chosen ones."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from reelcache_amd import paged_cache, quantized_cache, sparse_attention
+from reelcache_amd.errors import ConfigurationError, StateError
+
+import history_oracle as history
+import operator_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+KINDS = [(torch.bfloat16, None), (torch.float16, None), (torch.float32, None), (torch.bfloat16, torch.int8),
+         (torch.float16, torch.float8_e4m3fn)]
+
+
+def _cache(device, lengths, size, heads, dim, dtype, codes=None, layout="BTHD", seed=0):
+    """A cache of stored sequences in scattered pages; rows that no sequence has are (or stand for) NaN."""
+    pages = sum(-(-n // size) for n in lengths) + 2
+    if codes is None:
+        rows = (size, heads) if layout == "BTHD" else (heads, size)
+        cache = paged_cache.PagedCache(*(torch.full((1, pages, *rows, dim), math.nan, dtype=dtype, device=device) for _ in range(2)), layout=layout)
+    else:
+        cache = quantized_cache.QuantizedCache.allocate(pages, size, heads, dim, codes=codes, dtype=dtype, device=device, layout=layout)
+        for pool, scales in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales)):
+            pool.view(torch.uint8).fill_(1), scales.fill_(math.nan)
+    order, tables = np.random.default_rng(seed).permutation(pages).tolist(), []
+    for n in lengths:
+        tables.append((order[:-(-n // size)], n))
+        order = order[-(-n // size):]
+    cache.load_tables(tables)
+    g = torch.Generator().manual_seed(seed)
+    k, v = (torch.randn((sum(lengths), heads, dim), generator=g).to(dtype).to(device) for _ in range(2))
+    cache.store(0, cache.slots(list(range(len(lengths))), [0] * len(lengths), lengths), k, v)
+    return cache
+
+
+def _values(cache):
+    """The layer's pools as values (tensors of the cache's dtype)."""
+    if not cache.codes:
+        return cache.keys[0], cache.values[0]
+    return tuple(history.decode(pool[0], scales[0] if cache.layout == "BHTD" else scales[0].transpose(1, 2), cache.dtype)
+                 for pool, scales in ((cache.keys, cache.key_scales), (cache.values, cache.value_scales)))
+
+
+def _index(cache, size, lengths):
+    index = sparse_attention.BlockIndex.allocate(cache, size)
+    index.update(0, cache.places(list(range(len(lengths))), [0] * len(lengths), lengths))
+    return index
+
+
+class _Means:
+    """A sequence's means in 64 bits, from the index."""
+
+    def __init__(self, index, sequence):
+        self.rows = index.means[0].double().cpu()
+        self.pages, self.heads, self.blocks = index.cache.pages_of(sequence), index.cache.heads, self.rows.shape[1]
+
+    def __call__(self, block, head):
+        return self.rows[self.pages[block // self.blocks], block % self.blocks, head]
+
+
+def _check(cache, index, lengths, queries, q, chosen=None, *, top, query_block=1, first=1, recent=1, **mask):
+    """Chosen blocks against the rule, and the attention over them against 64 bits."""
+    plan = index.plan(list(range(len(lengths))), queries, heads=q.shape[1], top=top, query_block=query_block, first=first,
+                      recent=recent, **mask)
+    blocks = index.select(0, q, plan)
+    out, lse = index.attend(0, q, plan, blocks=blocks, return_lse=True)
+    assert torch.equal(out.isnan(), torch.zeros_like(out, dtype=torch.bool)) or chosen is not None
+    assert torch.equal(out, index.attend(0, q, plan))
+    keys, values = _values(cache)
+    group, size = q.shape[1] // cache.heads, index.block_tokens
+    run, start, widest = 0, 0, 0
+    scale = mask.pop("scale", None)
+    for sequence, (length, n) in enumerate(zip(lengths, queries)):
+        pages = cache.pages_of(sequence)
+        k, v = (history.history(x, cache.layout, pages, length) for x in (keys, values))
+        rows = q[start:start + n].double().cpu()
+        want = history.choice(rows, _Means(index, sequence), pages, length, n, size, cache.page_tokens, top=top,
+                              query_block=query_block, first=first, recent=recent, **mask)
+        held = np.repeat(np.array([page >= 0 for page in pages], dtype=bool), cache.page_tokens)[:length]
+        for at, count, per_head in want:
+            seen = np.array([history.visible(length, length - n + at + i, **mask) for i in range(count)]).reshape(count, length) & held
+            for head, expected in enumerate(per_head):
+                assert blocks[run, head].tolist() == expected + [-1] * (plan.width - len(expected)), (sequence, at, head)
+                widest = max(widest, len(expected))
+                shown = np.zeros(length, dtype=bool)
+                for j in expected:
+                    shown[j * size:(j + 1) * size] = True
+                for member in range(head * group, (head + 1) * group):
+                    value, bound, log, log_bound = history.attend(rows[at:at + count, member], k[:, head], v[:, head],
+                                                                  seen & shown, cache.dtype, scale)
+                    place = slice(start + at, start + at + count)
+                    assert oracle.worst(out[place, member], value, bound) <= 0, (sequence, at, member)
+                    assert oracle.worst(lse[place, member], log, log_bound) <= 0, (sequence, at, member)
+            run += 1
+        start += n
+    assert run == plan.runs and widest == plan.width
+    return plan, blocks, out
+
+
+def _queries(queries, heads, dim, dtype, device, seed=5):
+    return torch.randn((sum(queries), heads, dim), generator=torch.Generator().manual_seed(seed)).to(dtype).to(device)
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+@pytest.mark.parametrize("size,block,heads,dim,layout", [(16, 16, 2, 64, "BTHD"), (64, 32, 3, 128, "BHTD"), (60, 20, 1, 80, "BTHD"),
+                                                         (8, 1, 2, 20, "BTHD"), (12, 4, 9, 7, "BHTD"), (200, 100, 1, 200, "BTHD"),
+                                                         (96, 96, 1, 256, "BTHD")])
+def test_means(device, dtype, codes, size, block, heads, dim, layout):
+    """Means of the touched blocks; the others stay."""
+    lengths = [5 * size, 2 * size + size // 2, 1]
+    cache = _cache(device, lengths, size, heads, dim, dtype, codes, layout)
+    for pool in _values(cache):
+        assert pool.isnan().any()
+    index = sparse_attention.BlockIndex(cache, torch.full((1, cache.pages, size // block, heads, dim), 7.0, dtype=dtype, device=device))
+    begin, count = size // 2, 2 * size
+    slots = cache.slots([0, 1], [begin, size], [count, 1])
+    index.update(0, slots)
+    touched = sorted({s // block for s in slots.index.tolist()})
+    rows = history.rows_of(_values(cache)[0], layout).double().cpu().flatten(0, 1)
+    means = index.means[0].flatten(0, 1).double().cpu()
+    for number in range(means.shape[0]):
+        if number not in touched:
+            assert (means[number] == 7.0).all()
+            continue
+        held = rows[number * block:(number + 1) * block]
+        want = held.mean(dim=0)
+        # A sum in 64 bits, rounded to fp32 and then to the type.
+        bound = (oracle.U[dtype] + (0 if dtype == torch.float32 else oracle.F32) + 2.0 ** -40) * want.abs() * 1.01 + oracle.TINY[dtype]
+        bound += 2.0 ** -45 * held.abs().nan_to_num().sum(dim=0)
+        assert oracle.worst(means[number], want, bound.nan_to_num()) <= 0
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+@pytest.mark.parametrize("size,block,heads,group,dim,layout", [
+    (16, 16, 2, 1, 64, "BTHD"), (64, 32, 1, 4, 128, "BTHD"), (60, 20, 2, 2, 80, "BHTD"), (96, 96, 1, 3, 96, "BTHD"), (8, 2, 1, 2, 20, "BTHD"),
+    (130, 65, 1, 1, 128, "BHTD"), (16, 8, 1, 1, 7, "BTHD"), (200, 100, 1, 2, 208, "BTHD"), (64, 64, 2, 1, 104, "BTHD"),
+])
+def test_single_tokens(device, dtype, codes, size, block, heads, group, dim, layout):
+    """Single tokens over histories of one token up to many blocks."""
+    lengths = [1, 2, 31, 64, 65, 129, 700]
+    queries = [1] * len(lengths)
+    cache = _cache(device, lengths, size, heads, dim, dtype, codes, layout)
+    index = _index(cache, block, lengths)
+    q = _queries(queries, heads * group, dim, dtype, device)
+    for top, first, recent in ((3, 1, 1), (0, 0, 1), (2, 0, 0), (1000, 2, 2)):
+        _check(cache, index, lengths, queries, q, top=top, first=first, recent=recent)
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+@pytest.mark.parametrize("block,window", [(None, None), (1, None), (50, None), (1, 90), (None, 70)])
+@pytest.mark.parametrize("size,length,heads,group,dim,query_block", [(64, 16, 1, 1, 64, 16), (64, 32, 1, 4, 128, 33), (60, 20, 2, 1, 80, 7),
+                                                                     (100, 100, 1, 1, 128, 150), (8, 4, 1, 2, 20, 10)])
+def test_chunks(device, dtype, codes, block, window, size, length, heads, group, dim, query_block):
+    """Chunks alone and behind histories, in runs shorter and longer than a block, and rows that see nothing."""
+    lengths, queries = [70, 333, 260, 90, 3], [70, 129, 75, 1, 9 if block else 3]
+    cache = _cache(device, lengths, size, heads, dim, dtype, codes)
+    index = _index(cache, length, lengths)
+    q = _queries(queries, heads * group, dim, dtype, device)
+    for top, first, recent in ((3, 1, 1), (1, 0, 2)):
+        _check(cache, index, lengths, queries, q, top=top, query_block=query_block, first=first, recent=recent, block=block, window=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_long_histories(device, dtype):
+    """Hundreds of blocks: choices by more than the first eight bits, and lists in several parts."""
+    lengths, queries = [20000, 9001], [1, 1]
+    cache = _cache(device, lengths, 64, 1, 32, dtype)
+    index = _index(cache, 16, lengths)
+    q = _queries(queries, 4, 32, dtype, device)
+    for top in (1, 40, 250, 700, 1249):
+        _check(cache, index, lengths, queries, q, top=top)
+
+
+@pytest.mark.parametrize("codes", [None, torch.int8])
+def test_dropped_pages(device, codes):
+    """Holes are neither scored nor taken, whatever their means and rows hold."""
+    dtype, size, lengths, queries = torch.bfloat16, 32, [500, 96], [40, 1]
+    cache = _cache(device, lengths, size, 1, 64, dtype, codes)
+    index = _index(cache, 16, lengths)
+    dropped = cache.pages_of(0)[2:9] + cache.pages_of(1)[:2]
+    cache.drop(0, 2, 7)
+    cache.drop(1, 0, 2)
+    index.means[:, dropped] = math.nan
+    if codes is None:
+        cache.keys[:, dropped], cache.values[:, dropped] = math.nan, math.inf
+    q = _queries(queries, 2, 64, dtype, device)
+    for mask in ({}, {"block": 1}, {"window": 200}):
+        _check(cache, index, lengths, queries, q, top=2, query_block=16, **mask)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ties_and_numbers_that_are_none(device, dtype):
+    """Equal scores go to the lower block, zeros of either sign are equal, infinities rank as such and a NaN above all."""
+    lengths, queries = [330], [1]
+    cache = _cache(device, lengths, 16, 1, 32, dtype)
+    index = _index(cache, 16, lengths)
+    q = torch.ones((1, 1, 32), dtype=dtype, device=device)
+    means = index.means[0]
+    pages = cache.pages_of(0)
+    def choose(scores, top):
+        for j, value in enumerate(scores):
+            means[pages[j], 0] = 0
+            means[pages[j], 0, 0, 3] = value
+        plan = index.plan([0], queries, heads=1, top=top, first=0, recent=1)
+        return [j for j in index.select(0, q, plan)[0, 0].tolist() if 0 <= j < 20]
+    assert choose([5.0] * 20, 3) == [0, 1, 2]
+    assert choose([0.0, -0.0] * 10, 5) == [0, 1, 2, 3, 4]
+    assert choose([1.0] * 10 + [2.0] * 10, 12) == [0, 1] + list(range(10, 20))
+    assert choose([-1.0] * 19 + [-math.inf], 19) == list(range(19))
+    assert choose([-math.inf] * 20, 4) == [0, 1, 2, 3]
+    assert choose([1.0, math.inf, 2.0, math.nan] + [0.0] * 16, 1) == [3]
+    assert choose([1.0, math.inf, 2.0, math.nan] + [0.0] * 16, 2) == [1, 3]
+    assert choose([3.0, 3.0 + 8 * float(torch.finfo(dtype).eps)] * 10, 10) == list(range(1, 20, 2))
+    assert choose([float(j) for j in range(20)], 20) == list(range(20))
+
+
+def test_a_means_block_that_hides_a_key_is_not_scored(device):
+    """NaN keys that a causal mask hides: their blocks are taken where seen in part, and change nothing elsewhere."""
+    dtype, size = torch.bfloat16, 16
+    cache = _cache(device, [200], size, 1, 64, dtype)
+    q = _queries([100], 1, 64, dtype, device)
+    index = _index(cache, size, [200])
+    arguments = {"heads": 1, "top": 2, "query_block": 10, "block": 1}
+    plan = index.plan([0], [100], **arguments)
+    expected, blocks = index.attend(0, q, plan), index.select(0, q, plan)
+    page = cache.pages_of(0)[150 // size]
+    cache.keys[0, page, 150 % size], cache.values[0, page, 150 % size] = math.nan, math.nan
+    index.update(0, cache.slots([0], [150], [1]))
+    out, now = index.attend(0, q, plan), index.select(0, q, plan)
+    assert torch.equal(now[:5], blocks[:5]) and torch.equal(out[:50], expected[:50]) and out[50:].isnan().any()
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+def test_choices_of_the_callers_own(device, dtype, codes):
+    """Any lists: without order, with numbers that are no blocks, empty ones."""
+    lengths, queries, size = [300, 50], [20, 1], 16
+    cache = _cache(device, lengths, 32, 1, 64, dtype, codes)
+    index = _index(cache, size, lengths)
+    q = _queries(queries, 2, 64, dtype, device)
+    plan = index.plan([0, 1], queries, heads=2, top=4, query_block=8)
+    own = torch.full((plan.runs, 1, plan.width), -1, dtype=torch.int32)
+    lists = [[7, 2, 18], [0], [], [3, 1]]
+    for run, numbers in enumerate(lists):
+        own[run, 0, :len(numbers)] = torch.tensor(numbers, dtype=torch.int32)
+    own[2, 0] = torch.tensor([-5, 19, 1 << 30, -(1 << 31), 400] + [-1] * plan.width)[:plan.width]
+    own[3, 0, 2] = 4  # behind the sequence
+    out, lse = index.attend(0, q, plan, blocks=own.to(device), return_lse=True)
+    keys, values = _values(cache)
+    at = 0
+    for sequence, first, n, numbers in ((0, 0, 8, lists[0]), (0, 8, 8, lists[1]), (0, 16, 4, []), (1, 20, 1, lists[3])):
+        k, v = (history.history(x, "BTHD", cache.pages_of(sequence), lengths[sequence])[:, 0] for x in (keys, values))
+        shown = np.zeros((n, lengths[sequence]), dtype=bool)
+        for j in numbers:
+            shown[:, j * size:(j + 1) * size] = True
+        for member in range(2):
+            want, bound, logs, log_bound = history.attend(q[first:first + n, member].double().cpu(), k, v, shown, dtype)
+            assert oracle.worst(out[first:first + n, member], want, bound) <= 0
+            assert oracle.worst(lse[first:first + n, member], logs, log_bound) <= 0
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+def test_means_move_with_the_pages(device, dtype, codes):
+    """A fork's copied page, compaction and a copied cache: the means follow."""
+    lengths = [100, 70, 33]
+    cache = _cache(device, lengths, 32, 2, 64, dtype, codes)
+    index = _index(cache, 8, lengths)
+    q = _queries([1, 1], 4, 64, dtype, device)
+    child = cache.fork(1)
+    slots = cache.extend([child], [10])  # the begun page is copied with its means
+    g = torch.Generator().manual_seed(8)
+    cache.store(0, slots, *(torch.randn((10, 2, 64), generator=g).to(dtype).to(device) for _ in range(2)))
+    index.update(0, slots)
+    cache.free(0)
+    assert cache.compact() or True
+    sequences = [1, child]
+    lengths = [cache.tokens(s) for s in sequences]
+    plan = index.plan(sequences, [1, 1], heads=4, top=2)
+    blocks = index.select(0, q, plan)
+    for run, sequence in enumerate(sequences):
+        want = history.choice(q[run:run + 1].double().cpu(), _Means(index, sequence), cache.pages_of(sequence), lengths[run], 1, 8, 32,
+                              top=2, query_block=1, first=1, recent=1)
+        assert [[j for j in row if j >= 0] for row in blocks[run].tolist()] == want[0][2]
+    fresh = sparse_attention.BlockIndex.allocate(cache, 8)
+    fresh.update(0, cache.places(sequences, [0, 0], lengths))
+    for sequence, n in zip(sequences, lengths):
+        for j in range(n // 8):
+            page = cache.pages_of(sequence)[j // 4]
+            assert torch.equal(fresh.means[0, page, j % 4], index.means[0, page, j % 4]), (sequence, j)
+
+
+def test_outputs_strides_and_other_rows(device):
+    """``out`` with rows behind the plan's, queries of other orders, an empty plan."""
+    dtype = torch.bfloat16
+    lengths, queries = [300, 200], [5, 7]
+    cache = _cache(device, lengths, 32, 2, 64, dtype)
+    index = _index(cache, 16, lengths)
+    q = _queries([20], 4, 64, dtype, device)
+    plan = index.plan([0, 1], queries, heads=4, top=3, query_block=4, block=1)
+    expected = index.attend(0, q, plan)
+    assert not expected[12:].any()
+    out = torch.full_like(q, 3.0)
+    assert index.attend(0, q, plan, out=out) is out and torch.equal(out[:12], expected[:12]) and (out[12:] == 3).all()
+    other = q.permute(1, 2, 0).contiguous().permute(2, 0, 1)
+    assert torch.equal(index.attend(0, other, plan), expected)
+    empty = index.plan([], [], heads=4, top=3)
+    assert index.select(0, q[:0], empty).shape == (0, 2, 0) and index.attend(0, q[:0], empty).shape == (0, 4, 64)
+    none = index.plan([0], [3], heads=4, top=0, first=0, recent=0)
+    assert (index.select(0, q, none)[:, 0, 0] == 18).all()  # the block that is not full
+    for call in (lambda: cache.attend(0, q, plan), lambda: index.attend(0, q, cache.plan([0], [1], heads=4)),
+                 lambda: index.attend(0, q, plan, blocks=index.select(0, q, plan).long()),
+                 lambda: index.attend(0, q, plan, out=q[1:])):
+        with pytest.raises(ConfigurationError):
+            call()
+    cache.free(1)
+    with pytest.raises(StateError):
+        index.attend(0, q, plan)
+
+
+def test_streams_and_captured_replays(device):
+    """Update, choice and attention in two graphs with one plan, replayed in turn and at once, with eager work between."""
+    dtype = torch.bfloat16
+    cache = _cache(device, [3000, 130], 64, 2, 128, dtype)
+    cache.keys.nan_to_num_(0.0), cache.values.nan_to_num_(0.0)
+    index = _index(cache, 32, [3000, 130])
+    slots = cache.slots([0], [2900], [100])
+    plan = index.plan([0, 1], [100, 1], heads=4, top=5, query_block=25)
+    q = _queries([101], 4, 128, dtype, device)
+    k = torch.randn((100, 2, 128), generator=torch.Generator().manual_seed(1)).to(dtype).to(device)
+
+    def step():
+        cache.store(0, slots, k, k)
+        index.update(0, slots)
+        blocks = index.select(0, q, plan)
+        return blocks, index.attend(0, q, plan, blocks=blocks)
+
+    expected = step()
+    stream = torch.cuda.Stream(device)
+    stream.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(stream):
+        other = step()
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, expected))
+    graphs, outs = [], []
+    for captured in (step, lambda: (index.select(0, q, plan), index.attend(0, q, plan))):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(captured())
+        graphs.append(graph)
+    for replay in range(3):
+        for x in (k, q):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(10 + replay)))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize(device)
+        found = [[t.clone() for t in out] for out in outs]
+        want = step()
+        for out in found:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    sides = [torch.cuda.Stream(device) for _ in graphs]
+    torch.cuda.synchronize(device)
+    for side in sides:  # the attention of both at once (the keys stay as they are)
+        with torch.cuda.stream(side):
+            graphs[1].replay() if side is sides[0] else index.attend(0, q, plan)
+    torch.cuda.synchronize(device)
+    assert all(torch.equal(a, b) for a, b in zip(outs[1], want))
