@@ -583,7 +583,7 @@ int rch_runs_store(void* words_dev, const int32_t* runs_host, int n_runs, int64_
  * The K and V of tokens between dense tensors [tokens, heads, head_dim] and the pools of a paged cache in codes
  * [pages, page_tokens or heads, ..] with scales [pages, heads, page_tokens] (fp32; strides in elements, unit over the
  * channels, of scales over the tokens).  Token t lies in row slots[t] % page_tokens of page slots[t] / page_tokens.
- * A code c stands for c * scale, rounded to the dtype.
+ * A code c stands for c * scale, rounded to the dtype; of the scale of an E4M3 code its power of two counts.
  */
 typedef struct rch_codes {
     int64_t k_ptr, v_ptr;                          /* the dense tensors */
@@ -641,13 +641,14 @@ int rch_codes_read(const rch_codes* args_host, int dtype, void* stream);
  * rounded to the dtype (rch_codes_store).
  * Lists (lists_ptr != 0): an item's keys are those of chosen blocks of block_tokens keys, which divide a page.  Its
  * word 10 is the index in lists (int32) of its first entry, the number of a block of the sequence; key_begin and key_end
- * count tiles of 64 (f32: 32) keys from there, ceil(block_tokens / tile) to an entry.  An entry that is no block of the
+ * count tiles of 64 (f32, or single: 32) keys from there, ceil(block_tokens / tile) to an entry.  An entry that is no block of the
  * sequence, or lies in a hole, has no keys.
  */
 #define RCH_ATTEND_ITEM 12
 #define RCH_ATTEND_MERGE 8
 #define RCH_ATTEND_ZEROS 128
 #define RCH_ATTEND_FEW_PARTS 8
+#define RCH_ATTEND_SINGLE_ROWS 32
 #define RCH_ATTEND_MAX_DIM 256   /* head_dim of the general form */
 #define RCH_ATTEND_FAST_DIM 256  /* head_dim of the others: multiples of 8 up to this, 16-byte aligned rows */
 
@@ -674,7 +675,9 @@ typedef struct rch_attend {
     int64_t k_scale_ptr, v_scale_ptr; /* of pools in codes; strides in elements */
     int64_t k_scale_page_stride, k_scale_head_stride, v_scale_page_stride, v_scale_head_stride;
     int64_t lists_ptr, block_tokens;
-} rch_attend;                /* 45 x int64 = 360 bytes */
+    int64_t single;          /* 1: pools in codes, n_rows items of one query token each (at most RCH_ATTEND_SINGLE_ROWS rows):
+                                a wave to an item, tiles of 32 keys */
+} rch_attend;                /* 46 x int64 = 368 bytes */
 
 /*
  * Cuts the row blocks of a plan into parts (host only): block i has tiles[i] key tiles and belongs to owner[i]
@@ -702,12 +705,14 @@ typedef struct rch_blocks {
     /* rch_blocks_select */
     int64_t q_ptr, q_token_stride, q_head_stride, group;
     int64_t plan_ptr, runs, n_runs;                /* word index of the first run, their number */
-    int64_t scores_ptr, scores;                    /* uint64 [n_runs, heads, scores], scores >= any run's scored blocks */
+    int64_t scores_ptr, scores;                    /* scores >= any run's scored blocks; scratch uint64 [n_runs, heads, scores],
+                                                      or 0 (scores <= RCH_BLOCKS_TOGETHER, in one launch) */
     int64_t lists_ptr, width;                      /* int32 [n_runs, heads, width] */
     int64_t top;
 } rch_blocks;                /* 28 x int64 = 224 bytes */
 
 #define RCH_BLOCKS_RUN 12
+#define RCH_BLOCKS_TOGETHER 4096
 int rch_blocks_size(void);
 /* The means of the blocks that hold a slot: over all block_tokens rows, summed in FP64, rounded to FP32 and then to
  * the dtype. */

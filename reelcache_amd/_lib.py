@@ -81,9 +81,9 @@ ATTEND_FIELDS = ("q_ptr", "k_ptr", "v_ptr", "out_ptr", "lse_ptr", "plan_ptr", "p
                  "pages", "block", "window", "scale_bits", "partial_rows", "items", "n_general", "n_rows",
                  "merges", "n_merges", "n_many", "most_rows_many", "most_rows", "holes", "tile_unit", "codes", "k_scale_ptr",
                  "v_scale_ptr", "k_scale_page_stride", "k_scale_head_stride", "v_scale_page_stride", "v_scale_head_stride",
-                 "lists_ptr", "block_tokens")
+                 "lists_ptr", "block_tokens", "single")
 ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 256
-ATTEND_FEW_PARTS = 8
+ATTEND_FEW_PARTS, ATTEND_SINGLE_ROWS = 8, 32
 PAIRS_INTERLEAVED, PAIRS_HALF = 0, 1
 # rch_codes and rch_blocks (int64 structs read on the host during the call), formats of codes (RCH_CODES_*).
 CODES_FIELDS = ("k_ptr", "v_ptr", "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride", "k_codes_ptr",
@@ -97,7 +97,7 @@ BLOCKS_FIELDS = ("means_ptr", "heads", "head_dim", "pages", "page_tokens", "bloc
                  "token_stride", "head_stride", "codes", "scales_ptr", "scale_page_stride", "scale_head_stride", "slots_ptr",
                  "tokens", "q_ptr", "q_token_stride", "q_head_stride", "group", "plan_ptr", "runs", "n_runs", "scores_ptr",
                  "scores", "lists_ptr", "width", "top")
-CODES_NONE, CODES_INT8, CODES_E4M3, CODES_MAX_DIM, BLOCKS_RUN = 0, 1, 2, 256, 12
+CODES_NONE, CODES_INT8, CODES_E4M3, CODES_MAX_DIM, BLOCKS_RUN, BLOCKS_TOGETHER = 0, 1, 2, 256, 12, 4096
 
 _i, _i64, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _SIGNATURES = {

@@ -31,9 +31,10 @@ from .rotary import _DTYPE_CODES, _span, changed, entered, known_calls, need_gpu
 KEY_TILE = 64
 #: Query rows (tokens x heads of a key head) of one workgroup's tile, per form.
 GENERAL_ROWS, ROW_TILE = 16, 128
+_ROWS = {"general": GENERAL_ROWS, "rows": ROW_TILE, "single": _lib.ATTEND_SINGLE_ROWS}
 # What a workgroup's start, end and partial results cost in key tiles, per form (tiled: a step of six sequences of
 # 211 to 5003 tokens takes 58.0 us at 0, 55.4 at 3, 54.8 at 6 and 55.0 at 8; others do not change by more than 2 %).
-_OVERHEAD = {"general": 1, "rows": 6}
+_OVERHEAD = {"general": 1, "rows": 6, "single": 2}
 _CUS = 256
 # At most this many rows are joined a workgroup to a row, whatever their parts, in one launch (512 rows of 4 parts take
 # 4.1 us so, 4.1-5.1 us with a thread per eight channels; a second launch costs 5 us).
@@ -144,10 +145,17 @@ class AttentionPlan:
             return "general"
         return "rows"
 
+    def _form_of(self, tokens):
+        """The form of row blocks of at most ``tokens`` query tokens: :meth:`_form`, or "single" for single tokens over codes."""
+        form = self._form()
+        if form == "rows" and self.cache.codes and tokens <= 1 and self.group <= _lib.ATTEND_SINGLE_ROWS:
+            return "single"
+        return form
+
     def _lay_out(self, found, queries):
         cache = self.cache
-        form, work = self._form(), _Work()
-        tile = ROW_TILE if form == "rows" else GENERAL_ROWS
+        form, work = self._form_of(max(queries, default=0)), _Work()
+        tile = _ROWS[form]
         table = self._tables(found, queries)
         for number, (item, n) in enumerate(zip(found, queries)):
             if n:
@@ -178,11 +186,12 @@ class AttentionPlan:
         """Writes the plan's words to the device (``more``: words behind the merges)."""
         cache = self.cache
         merges = np.concatenate(merges) if merges else np.empty((0, _lib.ATTEND_MERGE), np.int64)
-        self._counts_of = (0, len(items)) if form == "rows" else (len(items), 0)
+        self._counts_of = (len(items), 0) if form == "general" else (0, len(items))
+        self._single = int(form == "single")
         first_item = _lib.ATTEND_ZEROS + len(table)
         self._items, self._merges = first_item, first_item + items.size
         # Merges that take a workgroup to a row come first (the kernels' rule).
-        joined = form == "rows" and cache.head_dim % 8 == 0
+        joined = form != "general" and cache.head_dim % 8 == 0
         many = (merges[:, 5] > _lib.ATTEND_FEW_PARTS) | (not joined)
         if len(merges) * merges[:, 2].max(initial=0) <= _FEW_ROWS:
             many[:] = True
@@ -220,6 +229,8 @@ class AttentionPlan:
         if form == "general":
             return _CUS * 4
         dim = self.cache.head_dim  # its tiles fill LDS and registers
+        if form == "single":
+            return _CUS * (12 if dim <= 64 else 6 if dim <= 128 else 3)
         return _CUS * (3 if dim <= 64 else 2 if dim <= 128 else 1)
 
     def _tile_of(self, key):
@@ -318,7 +329,7 @@ class AttentionPlan:
         fields = (0, 0, 0, 0, 0, 0, 0, *q_stride, k[page], k[token], k[head], v[page], v[token], v[head], *out_stride,
                   self.group, self.heads, cache.head_dim, cache.page_tokens, cache.pages, self.block or 0, self.window or 0,
                   scale, self._partial_rows, self._items, *self._counts_of, self._merges, self._n_merges, self._n_many,
-                  *self._most_rows, self._holes, self._unit(), cache.codes, 0, 0, *cache._scale_strides(), 0, self._block_tokens)
+                  *self._most_rows, self._holes, self._unit(), cache.codes, 0, 0, *cache._scale_strides(), 0, self._block_tokens, self._single)
         return bytes(_Image(*fields))
 
 

@@ -21,10 +21,10 @@ namespace rch {
 namespace {
 
 // What an element of a pool stands for.
-template <typename T, int FMT, typename Held>
+template <int DT, int FMT, typename Held>
 __device__ __forceinline__ float held_value(Held x, float scale) {
     if constexpr (FMT == RCH_CODES_NONE) return static_cast<float>(x);
-    else return static_cast<float>(code_value<FMT, T>(x, scale));
+    else return static_cast<float>(code_value<DT, FMT>(x, scale));
 }
 
 // FMT: what the pools hold (RCH_CODES_*).  LIST: the keys are those of chosen blocks, block after block.
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A)
                 float dot = 0.0f, unit = 0.0f;
                 if constexpr (FMT != RCH_CODES_NONE)
                     unit = gin<float>(A.k_scale_ptr)[page * A.k_scale_page_stride + I.kv_head * A.k_scale_head_stride + in_page];
-                for (int d = 0; d < dim; ++d) dot = __builtin_fmaf(query[wave][d], held_value<T, FMT>(k[d], unit), dot);
+                for (int d = 0; d < dim; ++d) dot = __builtin_fmaf(query[wave][d], held_value<DT, FMT>(k[d], unit), dot);
                 score = dot * scale;
             }
             uint64_t left = __ballot(seen);
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A)
                 const float unit = FMT == RCH_CODES_NONE ? 0.0f : scale_of[FMT == RCH_CODES_NONE ? 0 : wave][j];
 #pragma unroll
                 for (int c = 0; c < RCH_ATTEND_MAX_DIM / 64; ++c)
-                    if (lane + 64 * c < dim) acc[c] = __builtin_fmaf(wj, held_value<T, FMT>(v[lane + 64 * c], unit), acc[c]);
+                    if (lane + 64 * c < dim) acc[c] = __builtin_fmaf(wj, held_value<DT, FMT>(v[lane + 64 * c], unit), acc[c]);
             }
         };
         if constexpr (LIST) {
@@ -322,7 +322,7 @@ int items(const rch_attend& A, hipStream_t stream) {
         if (A.codes == RCH_CODES_E4M3) return launch_attend_e4m3(A, DT, stream);
         return A.lists_ptr ? launch_attend_lists(A, DT, stream) : launch_attend_rows(A, DT, stream);
     }
-    if constexpr (DT == RCH_DT_F32) {
+    if constexpr (DT == RCH_DT_F32) {  // (codes stand for 16-bit values)
         general<DT, RCH_CODES_NONE>(A, stream);
     } else {
         if (A.codes == RCH_CODES_INT8) general<DT, RCH_CODES_INT8>(A, stream);
@@ -378,6 +378,8 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
         if (dtype == RCH_DT_F32) return fail(RCH_E_UNSUPPORTED, "rch_attend_run: codes stand for f16 or bf16 values");
         if (!A.k_scale_ptr || !A.v_scale_ptr || (A.k_scale_ptr | A.v_scale_ptr) % 4) return fail(RCH_E_CONFIG, "rch_attend_run: pools in codes need their scales");
     }
+    if (A.single && (A.codes == RCH_CODES_NONE || A.n_general || A.group > RCH_ATTEND_SINGLE_ROWS))
+        return fail(RCH_E_CONFIG, "rch_attend_run: the form of single tokens takes codes, and at most %d rows to an item", RCH_ATTEND_SINGLE_ROWS);
     if (A.lists_ptr && (A.block_tokens < 1 || A.page_tokens % A.block_tokens || A.lists_ptr % 4))
         return fail(RCH_E_CONFIG, "rch_attend_run: chosen blocks divide a page");
     if (A.n_rows) {

@@ -11,9 +11,8 @@
 
 namespace rch {
 
-template <typename Tile, int MODE, int FMT>
+template <int DT, typename Tile, int MODE, int FMT>
 struct CodeFetch {
-    typedef typename Tile::T T;
     typedef typename Tile::vec8 vec8;
     static constexpr int KT = Tile::KT, RB = Tile::RB, kLanes = RB / 32, kRows = 64 / kLanes, kShareRows = KT / 4;
     static constexpr int NI = kShareRows / kRows;
@@ -93,16 +92,9 @@ struct CodeFetch {
     // 16 codes' values: two pieces of eight.
     static __device__ __forceinline__ void put(lds_char* row, int first, int swizzle, u4 codes, float scale) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            vec8 x;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-                const f4 n = code_numbers<FMT>(codes[2 * half + w]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * w + i] = static_cast<T>(n[i] * scale);
-            }
-            *reinterpret_cast<__attribute__((address_space(3))) vec8*>(row + ((first + half) ^ swizzle) * 16) = x;
-        }
+        for (int half = 0; half < 2; ++half)
+            *reinterpret_cast<__attribute__((address_space(3))) vec8*>(row + ((first + half) ^ swizzle) * 16) =
+                code_values<DT, FMT>(codes[2 * half], codes[2 * half + 1], scale);
     }
     __device__ __forceinline__ void commit(lds_char* k_tile, lds_char* v_tile) const {
 #pragma unroll

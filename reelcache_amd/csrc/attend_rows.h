@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     constexpr bool kCodes = FMT != RCH_CODES_NONE;
     KeyWalk<KT, MODE, kCodes> walk;
     walk.begin(A, I, kCodes ? 1 : ES);
-    typename std::conditional_t<kCodes, std::common_type<CodeFetch<Tile, MODE, kCodes ? FMT : RCH_CODES_INT8>>,
+    typename std::conditional_t<kCodes, std::common_type<CodeFetch<DT == RCH_DT_F32 ? RCH_DT_BF16 : DT, Tile, MODE, kCodes ? FMT : RCH_CODES_INT8>>,
                                 std::common_type<Fetch<Tile, MODE>>>::type fetch;
     if constexpr (kCodes) fetch.init(A, I, wave, lane);
     else fetch.init(A, wave, lane);
@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     while (coming) {
         if (!advance()) continue;
         const bool some = masked();
-        if (some && Tile::any_infinite(tiles + at + kTileBytes, lane)) {
+        // (Rows behind the last key, and those of a hole, are zeros: only keys that a row does not see may be anything.)
+        if (some && range.hides(key, keys) && Tile::any_infinite(tiles + at + kTileBytes, lane)) {
             rare = true;
             break;
         }

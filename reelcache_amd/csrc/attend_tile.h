@@ -237,44 +237,61 @@ struct KeyWalk : TilePlace<KEPT> {
     __device__ __forceinline__ int count() const { return min(end - base, MODE == kPage ? min(left, KT) : KT); }
 };
 
-// The walk over the tiles of an item's chosen blocks.
+// The walk over the tiles of an item's chosen blocks.  An entry's page is looked up a block before it is entered, and the
+// entry itself two before, so that no tile waits for either.
 template <int KT, bool KEPT>
 struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
     const const_int *table, *entry;
-    int unit, end, pages, size, blocks;  // tokens of a block, keys and blocks of the sequence, tokens of a page
-    int tiles;                           // of the item, the current one among them
-    int base, left;                      // current tile: first key, keys from it to the block's end
+    int unit, end, pages, blocks;   // tokens of a block, keys and blocks of the sequence
+    int per_page, magic;            // blocks of a page, and what finds a block's page
+    int tiles;                      // of the item, the current one among them
+    int entries;                    // of the list that are left to read
+    int base, left;                 // current tile: first key, keys from it to the block's end
+    int block1, page1, off1, block2;  // the next block, its page and place there; the one behind it
     int64_t k, v, k_head, v_head, k_page, v_page;
     int k_tile, v_tile, k_row, v_row;
 
     __device__ __forceinline__ bool done() const { return tiles <= 0; }
-    // Enters the block of `entry` at its tile `sub`, skipping entries without keys.
+    __device__ __forceinline__ int read() {
+        if (entries <= 0) return -1;
+        --entries;
+        return *entry++;
+    }
+    // Moves the entries up by one.
+    __device__ __forceinline__ void shift() {
+        block1 = block2;
+        page1 = -1;
+        if (block1 >= 0 && block1 < blocks) {
+            int index = per_page == 1 ? block1 : static_cast<int>(__umulhi(static_cast<uint32_t>(block1), static_cast<uint32_t>(magic)));
+            if (index * per_page > block1) --index;  // (the reciprocal is rounded up)
+            off1 = (block1 - index * per_page) * unit;
+            page1 = table[index];
+        }
+        block2 = read();
+    }
+    // Enters the next block at its tile `sub`, skipping entries without keys.
     __device__ __forceinline__ void enter(int sub) {
         while (tiles > 0) {
-            const int block = *entry;
-            if (block >= 0 && block < blocks) {
-                const int first = block * unit, index = first / size;
-                const int id = table[index];
-                // (a tile behind the sequence's last key has none either)
-                if (id >= 0 && id < pages && first + sub * KT < end) {
-                    const int in_page = first - index * size + sub * KT;
-                    this->stand(id, in_page);
-                    k = k_head + id * k_page + in_page * static_cast<int64_t>(k_row);
-                    v = v_head + id * v_page + in_page * static_cast<int64_t>(v_row);
-                    base = first + sub * KT;
-                    left = unit - sub * KT;
-                    return;
-                }
+            const int block = block1, id = page1, first = off1 + sub * KT;
+            shift();
+            // (a tile behind the sequence's last key has none either)
+            if (id >= 0 && id < pages && block * unit + sub * KT < end) {
+                this->stand(id, first);
+                k = k_head + id * k_page + first * static_cast<int64_t>(k_row);
+                v = v_head + id * v_page + first * static_cast<int64_t>(v_row);
+                base = block * unit + sub * KT;
+                left = unit - sub * KT;
+                return;
             }
             tiles -= (unit + KT - 1) / KT - sub;
             sub = 0;
-            ++entry;
         }
     }
     __device__ __forceinline__ void begin(const rch_attend& A, const AttendItem& I, int es) {
         table = (const const_int*)(uintptr_t)(A.plan_ptr + 4 * static_cast<int64_t>(I.table));
         unit = static_cast<int>(A.block_tokens);
-        size = static_cast<int>(A.page_tokens);
+        per_page = static_cast<int>(A.page_tokens) / unit;
+        magic = static_cast<int>(0xffffffffu / static_cast<uint32_t>(per_page) + 1);
         end = I.length;
         blocks = (end + unit - 1) / unit;
         pages = static_cast<int>(A.pages);
@@ -289,6 +306,10 @@ struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
         const int per = (unit + KT - 1) / KT, at = I.key_begin / per;
         entry = (const const_int*)(uintptr_t)(A.lists_ptr + 4 * static_cast<int64_t>(I.list)) + at;
         tiles = I.key_end - I.key_begin;
+        entries = tiles > 0 ? (I.key_end + per - 1) / per - at : 0;
+        off1 = 0;
+        block2 = read();
+        shift();
         enter(I.key_begin - at * per);
     }
     __device__ __forceinline__ void next() {
@@ -302,7 +323,6 @@ struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
             return;
         }
         tiles -= (left - 1) / KT;  // tiles of the block behind the sequence's last key
-        ++entry;
         enter(0);
     }
     __device__ __forceinline__ int count() const { return min(end - base, min(left, KT)); }
@@ -418,6 +438,8 @@ struct WaveRange {
     }
     // Whether a row may see a key of a tile, and whether one may not see all of its KT keys.
     __device__ __forceinline__ bool sees(int base, int count) const { return base + count > first_low && base < last_high; }
+    // Whether a row may not see one of the tile's own keys.
+    __device__ __forceinline__ bool hides(int base, int count) const { return base < first_high || base + count > last_low; }
     __device__ __forceinline__ bool masked(int base, int count, int kt) const {
         return base < first_high || base + kt > last_low || count < kt;
     }

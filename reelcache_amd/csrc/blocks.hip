@@ -11,6 +11,19 @@ namespace rch {
 
 namespace {
 
+typedef __attribute__((address_space(4))) const int32_t const_int;
+
+// Quotients of numbers below 2^31 by one divisor.
+struct Divider {
+    uint32_t by, reciprocal;
+    __device__ __forceinline__ explicit Divider(uint32_t d) : by(d), reciprocal(0xffffffffu / d + 1) {}  // (0 for 1)
+    __device__ __forceinline__ int quotient(int x) const {
+        if (by == 1) return x;
+        const uint32_t q = __umulhi(static_cast<uint32_t>(x), reciprocal);  // rounded up: one too many at most
+        return static_cast<int>(q * by > static_cast<uint32_t>(x) ? q - 1 : q);
+    }
+};
+
 template <int DT, int FMT>
 struct Row {
     typedef typename AttendType<DT>::type T;
@@ -19,15 +32,14 @@ struct Row {
     template <int V>
     static __device__ __forceinline__ void load(int64_t at, float scale, double (&x)[V]) {
         if constexpr (FMT != RCH_CODES_NONE) {
-            uint32_t word[V >= 4 ? V / 4 : 1];
             if constexpr (V == 8) {
                 const u2 raw = *gin<u2>(at);
-                word[0] = raw[0], word[1] = raw[1];
-            } else {
-                word[0] = *gin<uint8_t>(at);
-            }
+                const auto value = code_values<DT, FMT>(raw[0], raw[1], scale);
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[i] = static_cast<float>(static_cast<T>(code_numbers<FMT>(word[i / 4])[i % 4] * scale));
+                for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(value[i]);
+            } else {
+                x[0] = static_cast<float>(code_value<DT, FMT>(*gin<uint8_t>(at), scale));
+            }
         } else if constexpr (V == 8) {
             typedef T t8 __attribute__((ext_vector_type(8), aligned(16)));
             const t8 raw = *gin<t8>(at);
@@ -39,27 +51,29 @@ struct Row {
     }
 };
 
-// One workgroup for `share` tokens and a key head: where a token is the last one of its block among its neighbours, the
-// block's rows are summed, V channels and every kRows-th row to a thread.
+// One workgroup for up to 64 tokens (`share`) and a key head: where a token is the last one of its block among its
+// neighbours, the block's rows are summed, V channels and every kRows-th row to a thread.
 template <int DT, int FMT, int V>
 __global__ void __launch_bounds__(256) blocks_update_kernel(const rch_blocks B, int share) {
     typedef typename AttendType<DT>::type T;
     typedef Row<DT, FMT> R;
+    constexpr int kAhead = 8;  // rows in flight
     __shared__ double sums[256 * V];
     const int dim = static_cast<int>(B.head_dim), size = static_cast<int>(B.block_tokens), head = blockIdx.y;
     const int lanes = dim / V, rows = 256 / lanes;  // threads of a row, rows at once
-    const int mine = threadIdx.x / lanes, piece = threadIdx.x - mine * lanes;
+    const int mine = threadIdx.x / lanes, piece = threadIdx.x - mine * lanes, lane = threadIdx.x & 63;
     const RCH_GLOBAL int32_t* slots = gin<int32_t>(B.slots_ptr);
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * share, behind = first + share < B.tokens ? first + share : B.tokens;
     const int64_t limit = B.pages * B.page_tokens, per = B.page_tokens / size;
-    for (int64_t token = first; token < behind; ++token) {
-        const int64_t slot = slots[token];
-        if (slot < 0 || slot >= limit) continue;
-        const int64_t block = slot / size;
-        if (token + 1 < B.tokens) {
-            const int64_t next = slots[token + 1];
-            if (next >= 0 && next < limit && next / size == block) continue;
-        }
+    // Every wave finds the workgroup's blocks, a lane to a token.
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * share + lane;
+    const bool there = lane < share && token < B.tokens;
+    const int slot = there ? slots[token] : -1, next = there && token + 1 < B.tokens ? slots[token + 1] : -1;
+    const bool held = slot >= 0 && slot < limit;
+    const int number = held ? slot / size : -1;
+    uint64_t ends = __ballot(held && !(next >= 0 && next < limit && next / size == number));
+    while (ends) {
+        const int64_t block = __shfl(number, __builtin_ctzll(ends));
+        ends &= ends - 1;
         const int64_t page = block / per, row0 = (block - page * per) * size;
         const int64_t keys = B.keys_ptr + R::kBytes * (page * B.page_stride + row0 * B.token_stride + head * B.head_stride + piece * V);
         const int64_t scales = FMT == RCH_CODES_NONE ? 0 : B.scales_ptr + 4 * (page * B.scale_page_stride + head * B.scale_head_stride + row0);
@@ -67,14 +81,19 @@ __global__ void __launch_bounds__(256) blocks_update_kernel(const rch_blocks B, 
 #pragma unroll
         for (int i = 0; i < V; ++i) sum[i] = 0.0;
         if (mine < rows) {
-#pragma unroll 4
-            for (int row = mine; row < size; row += rows) {
-                double x[V];
-                float scale = 0.0f;
-                if constexpr (FMT != RCH_CODES_NONE) scale = gin<float>(scales)[row];
-                R::template load<V>(keys + R::kBytes * row * B.token_stride, scale, x);
+            for (int row = mine; row < size; row += rows * kAhead) {
+                double x[kAhead][V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) sum[i] += x[i];
+                for (int a = 0; a < kAhead; ++a) {
+                    const int at = min(row + a * rows, size - 1);
+                    float scale = 0.0f;
+                    if constexpr (FMT != RCH_CODES_NONE) scale = gin<float>(scales)[at];
+                    R::template load<V>(keys + R::kBytes * at * B.token_stride, scale, x[a]);
+                }
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum[i] += row + a * rows < size ? x[a][i] : 0.0;
             }
         }
 #pragma unroll
@@ -102,109 +121,189 @@ struct Run {
     int table, q_row, queries, first, last, scored, scored_end, kept, kept_end;
 };
 __device__ __forceinline__ Run run_of(const rch_blocks& B, int index) {
-    const RCH_GLOBAL int32_t* w = gin<int32_t>(B.plan_ptr) + B.runs + static_cast<int64_t>(index) * RCH_BLOCKS_RUN;
+    const const_int* w = (const const_int*)(uintptr_t)(B.plan_ptr + 4 * (B.runs + static_cast<int64_t>(index) * RCH_BLOCKS_RUN));
     return {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8]};
 }
-// The pool's page of a block, or -1 where it lies in a hole.
-__device__ __forceinline__ int page_of(const rch_blocks& B, const Run& R, int block, int per) {
-    const int id = gin<int32_t>(B.plan_ptr)[R.table + block / per];
+// The pool's page that is a run's `index`-th, or -1 for a hole.
+__device__ __forceinline__ int page_of(const rch_blocks& B, const Run& R, int index) {
+    const int id = gin<int32_t>(B.plan_ptr)[R.table + index];
     return id >= 0 && id < B.pages ? id : -1;
 }
 
-constexpr int kScored = 128;  // blocks that a workgroup scores
+constexpr int kScored = 128;     // blocks that a workgroup of the separate scoring takes
+constexpr int kTogether = RCH_BLOCKS_TOGETHER;  // most scored blocks of a run whose numbers fit in LDS, scored and taken by one workgroup
 
-// Scores kScored blocks for a run and key head.  V channels to a lane.
-template <int DT, int V>
-__global__ void __launch_bounds__(256) blocks_score_kernel(const rch_blocks B) {
+// The sum of a run's query rows of a key head, in FP64.  V channels to a thread.
+template <int DT, int V, int THREADS>
+__device__ __forceinline__ void pool_queries(const rch_blocks& B, const Run& R, int head, double* sums, double* pooled) {
     typedef typename AttendType<DT>::type T;
-    typedef Row<DT, RCH_CODES_NONE> K;
-    __shared__ double pooled[256], sums[256 * V];
-    const Run R = run_of(B, blockIdx.x);
-    const int head = blockIdx.z, dim = static_cast<int>(B.head_dim), group = static_cast<int>(B.group);
-    const int begin = R.scored + blockIdx.y * kScored, end = min(begin + kScored, R.scored_end);
-    if (begin >= end) return;
+    constexpr int kAhead = 4;
+    const int dim = static_cast<int>(B.head_dim), group = static_cast<int>(B.group), count = R.queries * group;
     const int lanes = dim / V, rows = 256 / lanes, mine = threadIdx.x / lanes, piece = threadIdx.x - mine * lanes;
-    {
+    const Divider by_group(group);
+    if (threadIdx.x < 256) {
         double sum[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) sum[i] = 0.0;
         if (mine < rows) {
-#pragma unroll 4
-            for (int row = mine; row < R.queries * group; row += rows) {
-                const int token = row / group, member = head * group + row - token * group;
-                double x[V];
-                K::template load<V>(B.q_ptr + static_cast<int64_t>(sizeof(T)) * ((R.q_row + token) * B.q_token_stride + member * B.q_head_stride + piece * V),
-                                    0.0f, x);
+            for (int row = mine; row < count; row += rows * kAhead) {
+                double x[kAhead][V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) sum[i] += x[i];
+                for (int a = 0; a < kAhead; ++a) {
+                    const int at = min(row + a * rows, count - 1), token = by_group.quotient(at), member = head * group + at - token * group;
+                    Row<DT, RCH_CODES_NONE>::template load<V>(
+                        B.q_ptr + static_cast<int64_t>(sizeof(T)) * ((R.q_row + token) * B.q_token_stride + member * B.q_head_stride + piece * V), 0.0f, x[a]);
+                }
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) sum[i] += row + a * rows < count ? x[a][i] : 0.0;
             }
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) sums[i * 256 + threadIdx.x] = sum[i];
-        __syncthreads();
+    }
+    __syncthreads();
+    if (threadIdx.x < 256) {
         const int channel = threadIdx.x;
         double total = 0.0;
         if (channel < dim)
             for (int r = 0; r < rows; ++r) total += sums[channel % V * 256 + r * lanes + channel / V];
         pooled[channel] = total;
-        __syncthreads();
     }
-    // A block's mean lies in W lanes (a power of two).
-    const int per = static_cast<int>(B.page_tokens / B.block_tokens), lane = threadIdx.x & 63;
+    __syncthreads();
+}
+
+// Numbers of blocks [begin, end) of a run and key head, to out(block, number).  A block's mean lies in `width` lanes (a power
+// of two), V channels to a lane; a thread has kAhead blocks in flight (pages first, then means).
+template <int DT, int V, int THREADS, typename Out>
+__device__ __forceinline__ void score_blocks(const rch_blocks& B, const Run& R, int head, int begin, int end, const double* pooled, Out out) {
+    typedef typename AttendType<DT>::type T;
+    constexpr int kAhead = V == 1 ? 1 : THREADS == 256 ? 8 : 4;
+    const int lane = threadIdx.x & 63, dim = static_cast<int>(B.head_dim);
+    const Divider by_page(static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(B.block_tokens));
+    const int per = static_cast<int>(by_page.by);
     int width = 1;
     while (width * V < dim && width < 64) width *= 2;
-    const int at = lane & (width - 1), step = 256 / width;
-    RCH_GLOBAL uint64_t* out = gout<uint64_t>(B.scores_ptr)
-                               + (static_cast<int64_t>(blockIdx.x) * B.heads + head) * B.scores - R.scored;
-    for (int block = begin + threadIdx.x / width; block - static_cast<int>(threadIdx.x) / width < end; block += step) {
-        const int page = block < end ? page_of(B, R, block, per) : -1;
-        double score = 0.0;
-        if (page >= 0) {
-            const int64_t mean = B.means_ptr
-                                 + static_cast<int64_t>(sizeof(T)) * ((static_cast<int64_t>(page) * per + block % per) * B.heads + head) * dim;
-            for (int d = at * V; d < dim; d += width * V) {
-                double x[V];
-                K::template load<V>(mean + static_cast<int64_t>(sizeof(T)) * d, 0.0f, x);
+    const int at = lane & (width - 1), step = THREADS / width;
+    const int64_t base = B.means_ptr + static_cast<int64_t>(sizeof(T)) * head * dim, block_bytes = static_cast<int64_t>(sizeof(T)) * B.heads * dim;
+    double q[V];  // V == 8: all that the lane needs of the queries
 #pragma unroll
-                for (int i = 0; i < V; ++i) score = __builtin_fma(x[i], pooled[d + i], score);
+    for (int i = 0; i < V; ++i) q[i] = at * V + i < dim ? pooled[at * V + i] : 0.0;
+    for (int first = begin; first < end; first += step * kAhead) {
+        int page[kAhead], in_page[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int block = min(first + a * step + static_cast<int>(threadIdx.x) / width, end - 1), index = by_page.quotient(block);
+            in_page[a] = block - index * per;
+            page[a] = page_of(B, R, index);
+        }
+        double score[kAhead];
+        if constexpr (V == 8) {
+            double x[kAhead][V];
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                const bool in = page[a] >= 0 && at * V < dim;
+                // (elsewhere the pool's first mean, which is not used)
+                Row<DT, RCH_CODES_NONE>::template load<V>(
+                    base + (in ? (static_cast<int64_t>(page[a]) * per + in_page[a]) * block_bytes + static_cast<int64_t>(sizeof(T)) * at * V : 0), 0.0f, x[a]);
+                if (!in)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) x[a][i] = 0.0;
+            }
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                score[a] = 0.0;
+#pragma unroll
+                for (int i = 0; i < V; ++i) score[a] = __builtin_fma(x[a][i], q[i], score[a]);
+            }
+        } else {
+            score[0] = 0.0;
+            if (page[0] >= 0) {
+                const int64_t mean = base + (static_cast<int64_t>(page[0]) * per + in_page[0]) * block_bytes;
+                for (int d = at; d < dim; d += width) {
+                    double x[1];
+                    Row<DT, RCH_CODES_NONE>::template load<1>(mean + static_cast<int64_t>(sizeof(T)) * d, 0.0f, x);
+                    score[0] = __builtin_fma(x[0], pooled[d], score[0]);
+                }
             }
         }
-        for (int o = 1; o < width; o <<= 1) score += __shfl_xor(score, o);
-        if (at == 0 && block < end) out[block] = page >= 0 ? order_of(score) : 0;
+        for (int o = 1; o < width; o <<= 1)
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) score[a] += __shfl_xor(score[a], o);
+        if (at == 0)
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                const int block = first + a * step + static_cast<int>(threadIdx.x) / width;
+                if (block < end) out(block, page[a] >= 0 ? order_of(score[a]) : 0);
+            }
     }
 }
 
 // Writes the blocks of a run and key head: all that are not scored, those kept anyway and the `top` best of the others.
-// The top-th best number is found eight bits at a time (a count of each value of the bits among the numbers that agree in
-// the bits before), until the blocks above and at it are just as many.
-__global__ void __launch_bounds__(256) blocks_take_kernel(const rch_blocks B) {
-    __shared__ uint32_t count[256], waves[2][4];
-    __shared__ uint32_t found[3];
-    const Run R = run_of(B, blockIdx.x);
-    const int head = blockIdx.y, per = static_cast<int>(B.page_tokens / B.block_tokens);
+// The top-th best number is found eight bits at a time, from the highest bit in which any two differ on (a count of each
+// value of the bits among the numbers that agree in the bits before), until the numbers that agree are no more than are
+// wanted.  number(block): of a scored one.
+struct Taking {
+    uint32_t count[256], found[3], waves[2][16];
+};
+template <int CONTROL>
+__device__ __forceinline__ uint32_t moved(uint32_t x) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CONTROL, 0xf, 0xf, true));
+}
+template <typename Join>
+__device__ __forceinline__ uint32_t joined(uint32_t x, Join join) {
+    x = join(x, moved<0xb1>(x));   // lanes 1 0 3 2
+    x = join(x, moved<0x4e>(x));   // lanes 2 3 0 1
+    x = join(x, moved<0x141>(x));  // mirrored in 8
+    x = join(x, moved<0x140>(x));  // mirrored in 16
+    x = join(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), 16)));
+    return join(x, static_cast<uint32_t>(__shfl_xor(static_cast<int>(x), 32)));
+}
+template <int THREADS, typename Number>
+__device__ __forceinline__ void take_blocks(const rch_blocks& B, const Run& R, int head, Taking& L, Number number) {
+    const Divider by_page(static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(B.block_tokens));
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-    const RCH_GLOBAL uint64_t* scores = gin<uint64_t>(B.scores_ptr)
-                                        + (static_cast<int64_t>(blockIdx.x) * B.heads + head) * B.scores - R.scored;
     auto chosen_by_score = [&](int block) { return block >= R.scored && block < R.scored_end && !(block >= R.kept && block < R.kept_end); };
 
     // Numbers above `bar` are taken, and the first `even` of those equal to it (in the bits of `mask`).
     uint64_t bar = 0, mask = 0;
     uint32_t even = static_cast<uint32_t>(B.top);
     bool all = false;  // no more candidates than are wanted
-    for (int shift = 56; even && shift >= 0; shift -= 8) {
-        count[t] = 0;
-        __syncthreads();
-        for (int block = R.scored + t; block < R.scored_end; block += 256) {
+    int shift = 0;
+    if (even) {
+        // The bits that all numbers share (of their upper halves).
+        uint32_t every = ~0u, any = 0;
+        for (int block = R.scored + t; block < R.scored_end; block += THREADS) {
             if (!chosen_by_score(block)) continue;
-            const uint64_t number = scores[block];
-            if (number != 0 && (number & mask) == bar) atomicAdd(&count[number >> shift & 255], 1u);
+            const uint64_t n = number(block);
+            if (n != 0) every &= static_cast<uint32_t>(n >> 32), any |= static_cast<uint32_t>(n >> 32);
+        }
+        every = joined(every, [](uint32_t a, uint32_t b) { return a & b; });
+        any = joined(any, [](uint32_t a, uint32_t b) { return a | b; });
+        if (lane == 0) L.waves[0][wave] = every, L.waves[1][wave] = any;
+        __syncthreads();
+        for (int w = 0; w < THREADS / 64; ++w) every &= L.waves[0][w], any |= L.waves[1][w];
+        const uint32_t differ = every ^ any;
+        const int top = differ ? 63 - __builtin_clz(differ) : 31;  // the first bit to look at
+        shift = top - 7;
+        mask = top == 63 ? 0 : ~uint64_t{0} << (top + 1);
+        bar = (static_cast<uint64_t>(every) << 32) & mask;
+    }
+    for (bool first = true; even; first = false) {
+        if (t < 256) L.count[t] = 0;
+        __syncthreads();
+        for (int block = R.scored + t; block < R.scored_end; block += THREADS) {
+            if (!chosen_by_score(block)) continue;
+            const uint64_t n = number(block);
+            if (n != 0 && (n & mask) == bar) atomicAdd(&L.count[n >> shift & 255], 1u);
         }
         __syncthreads();
         if (wave == 0) {
             // From the highest value down: lane i counts values 255 - 4 i .. 252 - 4 i.
             uint32_t c[4], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = count[255 - 4 * lane - i], sum += c[i];
+            for (int i = 0; i < 4; ++i) c[i] = L.count[255 - 4 * lane - i], sum += c[i];
             uint32_t upto = sum;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -212,62 +311,114 @@ __global__ void __launch_bounds__(256) blocks_take_kernel(const rch_blocks B) {
                 if (lane >= o) upto += other;
             }
             uint32_t before = upto - sum;
-            if (lane == 63) found[0] = upto;
+            if (lane == 63) L.found[0] = upto;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {  // the value that the last wanted one has (of one lane, where there are enough)
-                if (before < even && before + c[i] >= even) found[1] = 255 - 4 * lane - i, found[2] = even - before;
+                if (before < even && before + c[i] >= even) {
+                    L.found[1] = 255 - 4 * lane - i;
+                    L.found[2] = even - before | (before + c[i] == even ? 1u << 31 : 0);  // and whether all that have it are wanted
+                }
                 before += c[i];
             }
         }
         __syncthreads();
-        const uint32_t total = found[0], value = found[1], rest = found[2];
+        const uint32_t total = L.found[0], value = L.found[1], rest = L.found[2];
         if (total <= even) {  // every one that agrees so far; at first those are all candidates
-            all = mask == 0;
+            all = first;
             break;
         }
         bar |= static_cast<uint64_t>(value) << shift;
         mask |= uint64_t{255} << shift;
-        even = rest;
+        even = rest & 0x7fffffffu;
+        if (rest >> 31 || shift == 0) break;
+        shift = max(shift - 8, 0);
     }
     // In ascending order: the place of a block is the number of taken ones before it.
     RCH_GLOBAL int32_t* list = gout<int32_t>(B.lists_ptr) + (static_cast<int64_t>(blockIdx.x) * B.heads + head) * B.width;
     int written = 0;
     uint32_t equal = 0;
-    for (int base = R.first; base < R.last; base += 256) {
+    for (int base = R.first; base < R.last; base += THREADS) {
         const int block = base + t;
         bool taken = false, same = false;
-        if (block < R.last && page_of(B, R, block, per) >= 0) {
+        if (block < R.last && page_of(B, R, by_page.quotient(block)) >= 0) {
             if (all || !chosen_by_score(block)) {
                 taken = true;
             } else if (mask) {  // (none is wanted otherwise, and there may be no scores)
-                const uint64_t number = scores[block] & mask;
-                taken = number > bar;
-                same = number == bar;
+                const uint64_t n = number(block) & mask;
+                taken = n > bar;
+                same = n == bar;
             }
         }
         // Equal ones by their number.
         const uint64_t alike = __ballot(same);
-        if (lane == 0) waves[0][wave] = __popcll(alike);
+        if (lane == 0) L.waves[0][wave] = __popcll(alike);
         __syncthreads();
         uint32_t before = equal;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) before += waves[0][w];
-            equal += waves[0][w];
+        for (int w = 0; w < THREADS / 64; ++w) {
+            if (w < wave) before += L.waves[0][w];
+            equal += L.waves[0][w];
         }
         before += __popcll(alike & ((uint64_t{1} << lane) - 1));
         taken = taken || (same && before < even);
         const uint64_t votes = __ballot(taken);
-        if (lane == 0) waves[1][wave] = __popcll(votes);
+        if (lane == 0) L.waves[1][wave] = __popcll(votes);
         __syncthreads();
         int place = written;
-        for (int w = 0; w < 4; ++w) {
-            if (w < wave) place += waves[1][w];
-            written += waves[1][w];
+        for (int w = 0; w < THREADS / 64; ++w) {
+            if (w < wave) place += L.waves[1][w];
+            written += L.waves[1][w];
         }
         place += __popcll(votes & ((uint64_t{1} << lane) - 1));
         if (taken && place < B.width) list[place] = block;
     }
-    for (int at = written + t; at < B.width; at += 256) list[at] = -1;
+    for (int at = written + t; at < B.width; at += THREADS) list[at] = -1;
+}
+
+// Without scratch, runs of at most kTogether scored blocks: one workgroup to a run and key head.
+template <int DT, int V, int THREADS>
+__global__ void __launch_bounds__(THREADS) blocks_select_kernel(const rch_blocks B) {
+    __shared__ double pooled[256];
+    __shared__ union {
+        double sums[256 * V];
+        uint64_t numbers[kTogether];
+    } S;
+    __shared__ Taking L;
+    const Run R = run_of(B, blockIdx.x);
+    const int head = blockIdx.y;
+    if (B.top && R.scored < R.scored_end) {
+        pool_queries<DT, V, THREADS>(B, R, head, S.sums, pooled);
+        score_blocks<DT, V, THREADS>(B, R, head, R.scored, R.scored_end, pooled, [&](int block, uint64_t number) { S.numbers[block - R.scored] = number; });
+        __syncthreads();
+    }
+    take_blocks<THREADS>(B, R, head, L, [&](int block) { return S.numbers[block - R.scored]; });
+}
+
+// With scratch: workgroups of their own score kScored blocks each, and another launch takes them.
+template <int DT, int V>
+__global__ void __launch_bounds__(256) blocks_score_kernel(const rch_blocks B) {
+    __shared__ double pooled[256], sums[256 * V];
+    const Run R = run_of(B, blockIdx.x);
+    const int head = blockIdx.z, begin = R.scored + blockIdx.y * kScored, end = min(begin + kScored, R.scored_end);
+    if (begin >= end) return;
+    pool_queries<DT, V, 256>(B, R, head, sums, pooled);
+    RCH_GLOBAL uint64_t* out = gout<uint64_t>(B.scores_ptr) + (static_cast<int64_t>(blockIdx.x) * B.heads + head) * B.scores - R.scored;
+    score_blocks<DT, V, 256>(B, R, head, begin, end, pooled, [&](int block, uint64_t number) { out[block] = number; });
+}
+
+__global__ void __launch_bounds__(1024) blocks_take_kernel(const rch_blocks B) {
+    __shared__ uint64_t kept[kTogether];
+    __shared__ Taking L;
+    const Run R = run_of(B, blockIdx.x);
+    const int head = blockIdx.y, count = R.scored_end - R.scored;
+    const RCH_GLOBAL uint64_t* numbers = gin<uint64_t>(B.scores_ptr) + (static_cast<int64_t>(blockIdx.x) * B.heads + head) * B.scores;
+    if (count <= kTogether) {
+        if (B.top)
+            for (int i = threadIdx.x; i < count; i += 1024) kept[i] = numbers[i];
+        __syncthreads();
+        take_blocks<1024>(B, R, head, L, [&](int block) { return kept[block - R.scored]; });
+    } else {
+        take_blocks<1024>(B, R, head, L, [&](int block) { return numbers[block - R.scored]; });
+    }
 }
 
 // What both entry points need of the pools' description.
@@ -282,7 +433,7 @@ int invalid(const rch_blocks& B, int dtype, const char* what) {
 template <int DT, int FMT>
 int update(const rch_blocks& B, hipStream_t stream) {
     // Tokens of a workgroup: one while that makes few of them, so that the touched blocks of single tokens run at once.
-    const int64_t wanted = B.tokens * B.heads / 4096;
+    const int64_t wanted = B.tokens * B.heads / 1024;
     const int share = static_cast<int>(wanted < 1 ? 1 : wanted > 64 ? 64 : wanted);
     const dim3 grid(static_cast<uint32_t>((B.tokens + share - 1) / share), static_cast<uint32_t>(B.heads));
     const int64_t bytes = Row<DT, FMT>::kBytes, piece = FMT == RCH_CODES_NONE ? 16 : 8;
@@ -301,20 +452,26 @@ int update_of(const rch_blocks& B, hipStream_t stream) {
     return update<DT, RCH_CODES_NONE>(B, stream);
 }
 
+template <int DT, int V>
+int select_rows(const rch_blocks& B, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(B.n_runs), static_cast<uint32_t>(B.heads));
+    if (!B.scores_ptr) {
+        hipLaunchKernelGGL((blocks_select_kernel<DT, V, 256>), grid, dim3(256), 0, stream, B);
+        return check_launch("rch_blocks_select");
+    }
+    const dim3 scored(static_cast<uint32_t>(B.n_runs), static_cast<uint32_t>((B.scores + kScored - 1) / kScored), static_cast<uint32_t>(B.heads));
+    hipLaunchKernelGGL((blocks_score_kernel<DT, V>), scored, dim3(256), 0, stream, B);
+    const int status = check_launch("rch_blocks_select (scores)");
+    if (status != RCH_OK) return status;
+    hipLaunchKernelGGL(blocks_take_kernel, grid, dim3(1024), 0, stream, B);
+    return check_launch("rch_blocks_select");
+}
+
 template <int DT>
 int select(const rch_blocks& B, hipStream_t stream) {
     const int64_t size = DT == RCH_DT_F32 ? 4 : 2;
-    if (B.scores) {
-        const dim3 grid(static_cast<uint32_t>(B.n_runs), static_cast<uint32_t>((B.scores + kScored - 1) / kScored), static_cast<uint32_t>(B.heads));
-        const bool wide = B.head_dim % 8 == 0 && (B.q_ptr | B.means_ptr) % 16 == 0 && (B.q_token_stride | B.q_head_stride) * size % 16 == 0;
-        if (wide) hipLaunchKernelGGL((blocks_score_kernel<DT, 8>), grid, dim3(256), 0, stream, B);
-        else hipLaunchKernelGGL((blocks_score_kernel<DT, 1>), grid, dim3(256), 0, stream, B);
-        const int status = check_launch("rch_blocks_select (scores)");
-        if (status != RCH_OK) return status;
-    }
-    const dim3 grid(static_cast<uint32_t>(B.n_runs), static_cast<uint32_t>(B.heads));
-    hipLaunchKernelGGL(blocks_take_kernel, grid, dim3(256), 0, stream, B);
-    return check_launch("rch_blocks_select");
+    const bool wide = B.head_dim % 8 == 0 && (B.q_ptr | B.means_ptr) % 16 == 0 && (B.q_token_stride | B.q_head_stride) * size % 16 == 0;
+    return wide ? select_rows<DT, 8>(B, stream) : select_rows<DT, 1>(B, stream);
 }
 
 }  // namespace
@@ -352,7 +509,7 @@ int rch_blocks_select(const rch_blocks* args_host, int dtype, void* stream) {
         || B.top > 0x7fffffff)
         return fail(RCH_E_CONFIG, "rch_blocks_select: invalid runs");
     if (B.n_runs == 0 || B.width == 0) return RCH_OK;
-    if (!B.means_ptr || !B.q_ptr || !B.plan_ptr || !B.lists_ptr || (B.scores && !B.scores_ptr) || B.scores_ptr % 8)
+    if (!B.means_ptr || !B.q_ptr || !B.plan_ptr || !B.lists_ptr || (B.scores > kTogether && !B.scores_ptr) || (B.scores_ptr && !B.scores) || B.scores_ptr % 8)
         return fail(RCH_E_CONFIG, "rch_blocks_select: null or misaligned address");
     hipStream_t s = as_stream(stream);
     if (dtype == RCH_DT_F32) return select<RCH_DT_F32>(B, s);

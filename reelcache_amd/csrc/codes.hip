@@ -19,17 +19,6 @@ namespace {
 
 constexpr int kHeads = 4;
 
-template <int DT>
-struct Native;
-template <>
-struct Native<RCH_DT_F16> {
-    typedef _Float16 type;
-};
-template <>
-struct Native<RCH_DT_BF16> {
-    typedef __bf16 type;
-};
-
 // One side (K or V) of the arguments.
 struct Side {
     int64_t dense, token, head, codes, page, row, codes_head, scales, scale_page, scale_head;
@@ -103,7 +92,7 @@ __device__ __forceinline__ uint32_t encode(f4 x, const Scale& scale) {
 // other head size and alignment, element by element.
 template <int DT, int FMT, int V, int L>
 __global__ void __launch_bounds__(256) codes_store_kernel(const rch_codes A) {
-    typedef typename Native<DT>::type T;
+    typedef typename Coded<DT>::type T;
     const bool values = blockIdx.z != 0;
     const Side S = side_of(A, values);
     const int dim = static_cast<int>(A.head_dim), pairs = values ? 0 : static_cast<int>(A.pairs);
@@ -179,7 +168,7 @@ __global__ void __launch_bounds__(256) codes_store_kernel(const rch_codes A) {
 // V channels to a thread: 16 of aligned rows, or one.
 template <int DT, int FMT, int V>
 __global__ void __launch_bounds__(256) codes_read_kernel(const rch_codes A) {
-    typedef typename Native<DT>::type T;
+    typedef typename Coded<DT>::type T;
     const Side S = side_of(A, blockIdx.z != 0);
     const int pieces = static_cast<int>(A.head_dim) / V;
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, token = unit / pieces;
@@ -205,19 +194,11 @@ __global__ void __launch_bounds__(256) codes_read_kernel(const rch_codes A) {
     for (int u = 0; u < kHeads; ++u) {
         if (u >= heads) break;
         if constexpr (V == 16) {
-            typedef T t8 __attribute__((ext_vector_type(8)));
-            t8 out[2];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const f4 n = code_numbers<FMT>(raw[u][w]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) out[w / 2][4 * (w % 2) + i] = static_cast<T>(n[i] * scale[u]);
-            }
             RCH_GLOBAL u4* at = reinterpret_cast<RCH_GLOBAL u4*>(to + u * S.head);
-            at[0] = __builtin_bit_cast(u4, out[0]);
-            at[1] = __builtin_bit_cast(u4, out[1]);
+            at[0] = __builtin_bit_cast(u4, code_values<DT, FMT>(raw[u][0], raw[u][1], scale[u]));
+            at[1] = __builtin_bit_cast(u4, code_values<DT, FMT>(raw[u][2], raw[u][3], scale[u]));
         } else {
-            to[u * S.head] = code_value<FMT, T>(static_cast<uint8_t>(raw[u][0]), scale[u]);
+            to[u * S.head] = code_value<DT, FMT>(static_cast<uint8_t>(raw[u][0]), scale[u]);
         }
     }
 }

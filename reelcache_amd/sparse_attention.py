@@ -26,12 +26,13 @@ import torch
 
 from . import _lib
 from ._checks import count, in_memory, need
-from .attention import AttentionPlan, GENERAL_ROWS, ROW_TILE, run
+from .attention import AttentionPlan, _ROWS, run
 from .errors import ConfigurationError, StateError, UnsupportedError
 from .paged_cache import HOLE
 from .rotary import _DTYPE_CODES, entered, known_calls, need_gpu, raw_stream
 
 _MOST_SCORED = 65535 * 128  # blocks of a run: one workgroup scores 128
+_FEW_SCORED, _FEW_RUNS = 256, 128
 _Image = ctypes.c_int64 * len(_lib.BLOCKS_FIELDS)
 _AT = {name: index for index, name in enumerate(_lib.BLOCKS_FIELDS)}
 
@@ -74,7 +75,7 @@ class BlockPlan(AttentionPlan):
 
     def _lay_out(self, found, queries):
         cache, group, size = self.cache, self.group, self._block_tokens
-        form = self._form()
+        form = self._form_of(min(self.query_block, max(queries, default=0)))
         table = self._tables(found, queries)
         runs, counts = [], []
         for number, (item, n) in enumerate(zip(found, queries)):
@@ -96,11 +97,14 @@ class BlockPlan(AttentionPlan):
                                                                                             *[taken] * 3)
         self.runs, self.width = len(taken), int(taken.max(initial=0))
         self._scores = int((fields[:, 6] - fields[:, 5]).max(initial=0)) if self.top else 0
+        # Blocks are scored by workgroups of their own, in a launch before the choice, where one to a run would not fill the
+        # card (or its LDS).
+        self._apart = self._scores > (_FEW_SCORED if self.runs * cache.heads < _FEW_RUNS else _lib.BLOCKS_TOGETHER)
         if self._scores > _MOST_SCORED:
             raise UnsupportedError(f"a run scores at most {_MOST_SCORED} blocks")
         need(self.runs * cache.heads * max(1, self.width) < 1 << 31, "the step chooses too many blocks")
         # Row blocks: the rows of a run, in tiles, for each key head.
-        tile = ROW_TILE if form == "rows" else GENERAL_ROWS
+        tile = _ROWS[form]
         row0, row1 = begin * group, end * group
         pieces = -(-(row1 - row0) // tile)
         which = np.repeat(np.arange(self.runs), pieces)
@@ -110,7 +114,7 @@ class BlockPlan(AttentionPlan):
         heads = np.repeat(np.arange(cache.heads, dtype=np.int64), len(which))
         which, low, high = (np.tile(x, cache.heads) for x in (which, low, high))
         self._run_lists = (which * cache.heads + heads) * self.width
-        keys_of_tile = 32 if cache.dtype == torch.float32 else 64
+        keys_of_tile = 32 if cache.dtype == torch.float32 or form == "single" else 64
         tiles, merges = taken[which] * -(-size // keys_of_tile), []
         items = np.empty((0, _lib.ATTEND_ITEM), np.int64)
         if len(which):
@@ -225,7 +229,7 @@ class BlockIndex:
                                                        scores=plan._scores, width=plan.width, top=plan.top))
                 fields = _Image.from_buffer_copy(image)
                 scores = None
-                if plan._scores:
+                if plan._apart:
                     scores = torch.empty(plan.runs * cache.heads * plan._scores, dtype=torch.int64, device=cache.device)
                     fields[_AT["scores_ptr"]] = scores.data_ptr()
                 fields[0], fields[_AT["q_ptr"]], fields[_AT["plan_ptr"]] = address, q.data_ptr(), plan.buffer.data_ptr()

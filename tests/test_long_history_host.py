@@ -345,7 +345,7 @@ def test_header_matches_the_binding():
         assert tuple(name.strip().split()[-1] for line in body.split(";") if line.strip() for name in line.split(",")) == fields
     defines = {name: int(value) for name, value in re.findall(r"#define (RCH_[A-Z0-9_]+) (\d+)\b", HEADER.read_text())}
     expected = {"RCH_CODES_NONE": _lib.CODES_NONE, "RCH_CODES_INT8": _lib.CODES_INT8, "RCH_CODES_E4M3": _lib.CODES_E4M3,
-                "RCH_CODES_MAX_DIM": _lib.CODES_MAX_DIM, "RCH_BLOCKS_RUN": _lib.BLOCKS_RUN}
+                "RCH_CODES_MAX_DIM": _lib.CODES_MAX_DIM, "RCH_BLOCKS_RUN": _lib.BLOCKS_RUN, "RCH_BLOCKS_TOGETHER": _lib.BLOCKS_TOGETHER}
     assert {name: defines.get(name) for name in expected} == expected
     lib = _lib.library()
     assert lib.rch_codes_size() == 8 * len(_lib.CODES_FIELDS) and lib.rch_blocks_size() == 8 * len(_lib.BLOCKS_FIELDS)
@@ -371,7 +371,7 @@ def test_abi_refusals():
     good = dict(means_ptr=64, keys_ptr=64, slots_ptr=64, q_ptr=64, plan_ptr=64, lists_ptr=64, scores_ptr=64, heads=1, head_dim=8, pages=1,
                 page_tokens=4, block_tokens=2, tokens=1, group=1, n_runs=1, width=1, scores=1, top=1)
     for name, cases in (("rch_blocks_update", ({"block_tokens": 3}, {"codes": 3}, {"codes": 1}, {"tokens": -1}, {"keys_ptr": 0}, {"head_dim": 257})),
-                        ("rch_blocks_select", ({"group": 0}, {"n_runs": -1}, {"scores_ptr": 0}, {"scores_ptr": 4}, {"lists_ptr": 0}, {"top": -1},
+                        ("rch_blocks_select", ({"group": 0}, {"n_runs": -1}, {"scores_ptr": 0, "scores": 4097}, {"scores": 0}, {"scores_ptr": 4}, {"lists_ptr": 0}, {"top": -1},
                                                {"width": -1}, {"scores": 1 << 30}, {"block_tokens": 0}))):
         for bad in cases:
             with pytest.raises(ConfigurationError):
@@ -383,6 +383,8 @@ def test_abi_refusals():
     step = dict(group=1, heads=1, head_dim=16, page_tokens=4, pages=1, n_general=1, scale_bits=0x3f800000, q_ptr=64, k_ptr=64, v_ptr=64,
                 out_ptr=64, plan_ptr=64, k_scale_ptr=64, v_scale_ptr=64)
     for bad, dtype, error in (({"codes": 3}, 2, ConfigurationError), ({"codes": 1}, 0, UnsupportedError), ({"codes": 1, "k_scale_ptr": 0}, 2, ConfigurationError),
+                              ({"single": 1}, 2, ConfigurationError), ({"single": 1, "codes": 1}, 2, ConfigurationError),
+                              ({"single": 1, "codes": 1, "n_general": 0, "n_rows": 1, "group": 33}, 2, ConfigurationError),
                               ({"lists_ptr": 64}, 2, ConfigurationError), ({"lists_ptr": 64, "block_tokens": 3}, 2, ConfigurationError),
                               ({"codes": 1, "n_general": 0, "n_rows": 1, "head_dim": 24, "tile_unit": 64}, 2, UnsupportedError)):
         with pytest.raises(error):

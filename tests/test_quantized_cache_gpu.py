@@ -228,7 +228,7 @@ def _check(cache, lengths, queries, q, **mask):
         assert oracle.worst(lse[rows], logs, log_bound) <= 0, (sequence, length, n)
         start += n
     assert torch.equal(out, cache.attend(0, q, plan))
-    if cache.head_dim % 16 == 0:
+    if cache.head_dim % 16 == 0 and not plan._single:  # (single tokens take smaller tiles)
         same = native.plan(list(range(len(lengths))), queries, heads=q.shape[1], **mask)
         assert torch.equal(out, native.attend(0, q, same))
     return out
@@ -293,9 +293,38 @@ def test_long_split_histories(device, codes):
         cache = _filled(device, [9000, 4001], size, 2, 128, codes, torch.bfloat16)
         q = torch.randn((2, 8, 128), generator=torch.Generator().manual_seed(3)).bfloat16().to(device)
         native = _native(cache)
-        out, lse = cache.attend(0, q, cache.plan([0, 1], [1, 1], heads=8), return_lse=True)
-        same = native.attend(0, q, native.plan([0, 1], [1, 1], heads=8), return_lse=True)
-        assert torch.equal(out, same[0]) and torch.equal(lse, same[1])
+        plan = cache.plan([0, 1], [1, 1], heads=8)
+        assert plan._n_merges and plan._single
+        out, lse = cache.attend(0, q, plan, return_lse=True)
+        k, v = (history.rows_of(x[0], "BTHD").double().cpu() for x in (native.keys, native.values))
+        for sequence, length in ((0, 9000), (1, 4001)):
+            pages = torch.tensor(cache.pages_of(sequence))
+            for head in range(8):
+                keys, values = (x[pages][:, :, head // 4].flatten(0, 1)[:length] for x in (k, v))
+                want, bound, logs, log_bound = history.attend(q[sequence:sequence + 1, head].double().cpu(), keys, values,
+                                                              np.ones((1, length), dtype=bool), torch.bfloat16)
+                assert oracle.worst(out[sequence:sequence + 1, head], want, bound) <= 0
+                assert oracle.worst(lse[sequence:sequence + 1, head], logs, log_bound) <= 0
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [16, 64, 96, 128, 192, 256])
+def test_single_tokens_of_many_heads(device, codes, dtype, dim):
+    """Groups of up to 32 heads, and more, over pages in one piece and in many; a window; keys that hide NaN."""
+    for group in (1, 8, 32, 33):
+        for size in (64, 16, 5):
+            cache = _filled(device, [200, 33, 1], size, 1, dim, codes, dtype)
+            q = torch.randn((3, group, dim), generator=torch.Generator().manual_seed(group)).to(dtype).to(device)
+            _check(cache, [200, 33, 1], [1, 1, 1], q)
+            _check(cache, [200, 33, 1], [1, 1, 1], q, window=70)
+            plan = cache.plan([0], [1], heads=group, window=70)
+            assert plan._single == (group <= 32)
+            expected = cache.attend(0, q[:1], plan)
+            for at in (0, 100, 129):  # hidden by the window
+                page = cache.pages_of(0)[at // size]
+                cache.key_scales[0, page, 0, at % size], cache.value_scales[0, page, 0, at % size] = math.nan, math.nan
+            assert torch.equal(cache.attend(0, q[:1], plan), expected)
 
 
 def test_scales_beyond_fp16(device):
