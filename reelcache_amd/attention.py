@@ -230,7 +230,7 @@ class AttentionPlan:
             return _CUS * 4
         dim = self.cache.head_dim  # its tiles fill LDS and registers
         if form == "single":
-            return _CUS * (12 if dim <= 64 else 6 if dim <= 128 else 3)
+            return _CUS * (12 if dim <= 64 else 8 if dim <= 128 else 4)
         return _CUS * (3 if dim <= 64 else 2 if dim <= 128 else 1)
 
     def _tile_of(self, key):

@@ -18,7 +18,9 @@ constexpr int kXcds = 8;
 // short sequences (37 to 1000 tokens) take 13.1 / 14.3 / 21.5 us with parts of at least 2 / 3 / 4 tiles, of 16
 // sequences of 2000 tokens 23.9 / 19.8 us with 2 / 3; of 2 of 16000 tokens 31.7 us with up to 64 parts, 23.1 with 32
 // (their merge grows).
-constexpr int64_t kShortestPart = 3, kMostParts = 32;
+constexpr int64_t kShortestPart = 3, kMostParts = 32, kManyResident = 128;
+// Of waves of single tokens over codes (8 of 37 to 1000 tokens: 14.6 / 15.0 / 16.7 us with parts of at least 1 / 2 / 3).
+constexpr int64_t kShortestSingle = 1;
 
 struct Piece {
     int64_t item, first, last;  // item: rank within the XCD
@@ -28,7 +30,7 @@ typedef std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>
 
 // Cuts items (longest first) so that `resident` workgroups end by `limit`: what an item has beyond `limit` goes to
 // workgroups of its own, the rest to the least loaded one, cut at the room there is.  False if they cannot.
-bool ending_by(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, int64_t limit, std::vector<Piece>& pieces) {
+bool ending_by(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, int64_t fewest, int64_t limit, std::vector<Piece>& pieces) {
     const int64_t room_of_one = limit - overhead;
     struct Rest {
         int64_t cost, item, at;
@@ -41,7 +43,7 @@ bool ending_by(const std::vector<int64_t>& costs, int64_t resident, int64_t over
         const int64_t item = static_cast<int64_t>(i);
         while (cost - at > room_of_one) {
             // A rest too short for a part takes some of the last full one.
-            const int64_t left = cost - at - room_of_one, end = at + room_of_one - (left < kShortestPart ? kShortestPart - left : 0);
+            const int64_t left = cost - at - room_of_one, end = at + room_of_one - (left < fewest ? fewest - left : 0);
             pieces.push_back({item, at, end});
             at = end;
             ++busy;
@@ -57,8 +59,8 @@ bool ending_by(const std::vector<int64_t>& costs, int64_t resident, int64_t over
             const int64_t load = loads.top(), room = room_of_one - load;
             int64_t piece = left;
             if (left > room) {
-                if (room < kShortestPart) return false;
-                piece = left - room >= kShortestPart ? room : left - kShortestPart;
+                if (room < fewest) return false;
+                piece = left - room >= fewest ? room : left - fewest;
                 if (piece < 1) return false;
             }
             loads.pop();
@@ -73,14 +75,14 @@ bool ending_by(const std::vector<int64_t>& costs, int64_t resident, int64_t over
 
 // Cuts items (longest first) so that `resident` workgroups that take parts in order, longest first, end together as
 // early as they can.
-void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, std::vector<Piece>& pieces) {
+void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, int64_t fewest, std::vector<Piece>& pieces) {
     const int64_t n = static_cast<int64_t>(costs.size()), longest = costs[0];
     pieces.clear();
     auto whole = [&]() {
         pieces.clear();
         for (int64_t i = 0; i < n; ++i) pieces.push_back({i, 0, costs[static_cast<size_t>(i)]});
     };
-    if (longest < 2 * kShortestPart || n > 4 * resident) return whole();
+    if (longest < 2 * fewest || n > 4 * resident) return whole();
     int64_t total = 0, uncut = longest + overhead;
     for (const int64_t cost : costs) total += cost;
     if (n > resident) {
@@ -93,12 +95,14 @@ void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, 
             uncut = std::max(uncut, load);
         }
     }
-    const int64_t shortest = std::max(kShortestPart, (longest + kMostParts - 1) / kMostParts);
+    // (a form with more workgroups to an XCD than kManyResident, waves of single tokens, is cut further: it fills the card by parts alone)
+    const int64_t most = resident > kManyResident ? resident / 2 : kMostParts;
+    const int64_t shortest = std::max(fewest, (longest + most - 1) / most);
     int64_t low = std::max((total + n * overhead) / resident, shortest + overhead), high = uncut;
     std::vector<Piece> found;
     while (50 * low < 49 * high) {  // the earliest end that parts reach, within a fiftieth
         const int64_t middle = (low + high) / 2;
-        if (ending_by(costs, resident, overhead, middle, found)) {
+        if (ending_by(costs, resident, overhead, fewest, middle, found)) {
             high = middle;
             pieces.swap(found);
         } else {
@@ -110,6 +114,7 @@ void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, 
 
 int share_out(const int64_t* tiles, const int64_t* owner, int64_t n, int64_t resident, int64_t overhead, int64_t* parts,
               int64_t capacity, int64_t* count) {
+    const int64_t fewest = resident / kXcds > kManyResident ? kShortestSingle : kShortestPart;
     std::vector<int64_t> order(static_cast<size_t>(n)), starts(order.size());
     for (int64_t i = 0; i < n; ++i) order[static_cast<size_t>(i)] = i;
     std::stable_sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return owner[a] < owner[b]; });
@@ -128,8 +133,8 @@ int share_out(const int64_t* tiles, const int64_t* owner, int64_t n, int64_t res
     // A border within an item: too short a piece joins the neighbour's.
     auto border = [&](int64_t at, int64_t limit) {
         at = std::min(std::max<int64_t>(at, 0), limit);
-        if (at < limit && at < kShortestPart) return int64_t{0};
-        return limit - at < kShortestPart ? limit : at;
+        if (at < limit && at < fewest) return int64_t{0};
+        return limit - at < fewest ? limit : at;
     };
     struct Inside {
         int64_t cost, item, low;
@@ -151,7 +156,7 @@ int share_out(const int64_t* tiles, const int64_t* owner, int64_t n, int64_t res
         auto made = known.find(costs);
         if (made == known.end()) {
             std::vector<Piece> pieces;
-            cut(costs, std::max<int64_t>(1, resident / kXcds), overhead, pieces);
+            cut(costs, std::max<int64_t>(1, resident / kXcds), overhead, fewest, pieces);
             made = known.emplace(std::move(costs), std::move(pieces)).first;
         }
         for (const Piece& p : made->second) {

@@ -26,6 +26,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     range.init(R);
 
     constexpr bool kCodes = FMT != RCH_CODES_NONE;
+    if constexpr (kCodes) wait_vector_memory();  // the queries, so that no tile's wait is for them
     KeyWalk<KT, MODE, kCodes> walk;
     walk.begin(A, I, kCodes ? 1 : ES);
     typename std::conditional_t<kCodes, std::common_type<CodeFetch<DT == RCH_DT_F32 ? RCH_DT_BF16 : DT, Tile, MODE, kCodes ? FMT : RCH_CODES_INT8>>,

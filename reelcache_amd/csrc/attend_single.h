@@ -2,7 +2,7 @@
 // key head, at most 32) are one token's.
 //
 // Bound: memory, one byte of every key and value.  A tile of 32 keys and values travels as codes from memory to LDS
-// directly, two tiles ahead, in a ring that is the wave's own: no barrier, and several such waves to a CU keep enough bytes
+// directly, a tile ahead, in a ring that is the wave's own: no barrier, and several such waves to a CU keep enough bytes
 // on their way.  The products are those of attend_tile.h (S^T = K Q^T, O^T += V^T P^T, 32 x 32 x 16); codes become 16-bit
 // operands as they are read.  K: the inner index of the products may run over the channels in any order that K and Q share,
 // so a lane reads 16 codes of its key at once, channels 32 c + 16 h .., and feeds two products.  V: a transposed read of
@@ -52,7 +52,7 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
     typedef CodeTile<NB> Tile;
     typedef RowTile<DT, NB, 1> Layout;  // of the output
     constexpr int KT = Tile::KT, RB = Tile::RB, NI = Tile::NI, kPieces = Tile::kPieces, kRows = Tile::kRows;
-    constexpr int kStages = 3, kLoads = 2 * NI + 1;  // of a tile
+    constexpr int kStages = 2, kLoads = 2 * NI + 1;  // of a tile
     __shared__ __attribute__((aligned(1024))) char lds[kStages * Tile::kBytes];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const AttendItem I = attend_item(A, blockIdx.x);
@@ -61,19 +61,6 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
     const int row_first = __builtin_amdgcn_readfirstlane(R.first), row_last = __builtin_amdgcn_readfirstlane(R.last);
     const float scale = __int_as_float(static_cast<int>(A.scale_bits));
 
-    // Q: product 2 c + e takes channels 32 c + 16 h + 8 e ...
-    vec8 q[2 * NB];
-    f16v o[NB];
-    {
-        const int64_t at = A.q_ptr + 2 * ((I.q_row + R.token) * A.q_token_stride + R.head * A.q_head_stride);
-#pragma unroll
-        for (int c = 0; c < 2 * NB; ++c) {
-            const int d = 32 * (c >> 1) + 16 * h + 8 * (c & 1);
-            q[c] = __builtin_bit_cast(vec8, *gin<u4>(R.valid && d < A.head_dim ? at + 2 * d : A.plan_ptr));  // or zeros
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) o[b] = f16v{};
-    }
     Reference reference;
     reference.init();
     float sum = 0.0f;
@@ -88,6 +75,15 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
     const bool of_values = h != 0;  // the scale that the lane fetches: of key or value n
     const int64_t scale_head = of_values ? A.v_scale_ptr + 4 * I.kv_head * A.v_scale_head_stride : A.k_scale_ptr + 4 * I.kv_head * A.k_scale_head_stride;
     const int64_t scale_page = 4 * (of_values ? A.v_scale_page_stride : A.k_scale_page_stride);
+    uint32_t k_at[MODE == kRow ? 1 : NI], v_at[MODE == kRow ? 1 : NI];  // the lane's byte offsets in a tile of one page
+    if constexpr (MODE != kRow) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int row = i * kRows + row0, kc = spot ^ Tile::k_swizzle(row), vc = spot ^ Tile::v_swizzle(row);
+            k_at[i] = row * k_row + (kc < pieces ? kc * 16 : 0);
+            v_at[i] = row * v_row + (vc < pieces ? vc * 16 : 0);
+        }
+    }
     const uint32_t ring = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_char*)lds));
 
     // Tiles on their way, the oldest first: first key, and the keys that the rows see (bits).
@@ -102,12 +98,19 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
         uint32_t shown = static_cast<uint32_t>(bits);
         if constexpr (MODE == kPage || MODE == kList) {
             const int64_t k = uniform64(walk.k), v = uniform64(walk.v);
+            if (count == KT) {
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int row = i * kRows + row0, from = min(row, count - 1);
-                const int kc = spot ^ Tile::k_swizzle(row), vc = spot ^ Tile::v_swizzle(row);
-                fetch_rows(k, from * k_row + (kc < pieces ? kc * 16 : 0), at + i * 1024);
-                fetch_rows(v, from * v_row + (vc < pieces ? vc * 16 : 0), at + KT * RB + i * 1024);
+                for (int i = 0; i < NI; ++i) {
+                    fetch_rows(k, k_at[i], at + i * 1024);
+                    fetch_rows(v, v_at[i], at + KT * RB + i * 1024);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const int row = i * kRows + row0, back = max(row - (count - 1), 0);  // rows to the last one
+                    fetch_rows(k, k_at[i] - back * k_row, at + i * 1024);
+                    fetch_rows(v, v_at[i] - back * v_row, at + KT * RB + i * 1024);
+                }
             }
             fetch_words(scale_head + walk.id * scale_page + 4 * static_cast<int64_t>(walk.in_page + min(n, count - 1)), at + 2 * KT * RB);
         } else {
@@ -140,6 +143,21 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s)
         if (!walk.done()) seen[s] = issue(s), ++pending;
+
+    // Q: product 2 c + e takes channels 32 c + 16 h + 8 e ...
+    vec8 q[2 * NB];
+    f16v o[NB];
+    {  // (after the first tiles' loads; waited for before the loop, where a wait for them would be one for every tile's)
+        const int64_t at = A.q_ptr + 2 * ((I.q_row + R.token) * A.q_token_stride + R.head * A.q_head_stride);
+#pragma unroll
+        for (int c = 0; c < 2 * NB; ++c) {
+            const int d = 32 * (c >> 1) + 16 * h + 8 * (c & 1);
+            q[c] = __builtin_bit_cast(vec8, *gin<u4>(R.valid && d < A.head_dim ? at + 2 * d : A.plan_ptr));  // or zeros
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[b] = f16v{};
+    }
+    wait_vector_memory();
 
     // A lane's offsets within a tile: of its key's codes at piece h (piece 2 c + h from there by an exclusive or), and of the
     // transposed read of channel block 0 for the first 16 keys.
@@ -203,24 +221,31 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[b][i] *= fade;
         }
+        // bf16: the values' scales go to the weights (rounded once, as they are without; the codes are exact).  fp16 does not
+        // hold such weights: there the scales go to the values.
+        constexpr bool kScaled = DT == RCH_DT_BF16;
+        f4 v_scale[4];  // of the keys of registers 4 i ..
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v_scale[i] = *(lds_f4*)(scales + 32 + 8 * i + 4 * h);
         vec8 w[2];
         float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float x = exp2_of(__builtin_fmaf(s[0][i], scale, -reference.value));
             part[i & 3] += x;
-            w[i >> 3][i & 7] = static_cast<T>(x);
+            w[i >> 3][i & 7] = static_cast<T>(kScaled ? x * v_scale[i >> 2][i & 3] : x);
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const f4 low = *(lds_f4*)(scales + 32 + 16 * half + 4 * h), high = *(lds_f4*)(scales + 32 + 16 * half + 8 + 4 * h);
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 typedef int i2 __attribute__((ext_vector_type(2)));
                 typedef __attribute__((address_space(3))) i2 lds_i2;
                 const i2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(v_tile + v_lane + half * 16 * RB + (v_turn ^ (b * 32))));
-                o[b] = H::mfma(code_values<DT, FMT>(static_cast<uint32_t>(codes[0]), static_cast<uint32_t>(codes[1]), low, high), w[half], o[b]);
+                const uint32_t low = static_cast<uint32_t>(codes[0]), high = static_cast<uint32_t>(codes[1]);
+                if constexpr (kScaled) o[b] = H::mfma(code_values<DT, FMT>(low, high), w[half], o[b]);
+                else o[b] = H::mfma(code_values<DT, FMT>(low, high, v_scale[2 * half], v_scale[2 * half + 1]), w[half], o[b]);
             }
         }
     }

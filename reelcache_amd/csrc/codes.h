@@ -76,6 +76,20 @@ __device__ __forceinline__ typename Coded<DT>::vec8 code_values(uint32_t low, ui
     for (int i = 0; i < 4; ++i) x[i] = static_cast<T>(a[i] * scale_low[i]), x[4 + i] = static_cast<T>(b[i] * scale_high[i]);
     return x;
 }
+// Eight codes as numbers (exact).
+template <int DT, int FMT>
+__device__ __forceinline__ typename Coded<DT>::vec8 code_values(uint32_t low, uint32_t high) {
+    if constexpr (FMT == RCH_CODES_E4M3) {
+        return code_values<DT, FMT>(low, high, 1.0f);
+    } else {
+        typedef typename Coded<DT>::type T;
+        typename Coded<DT>::vec8 x;
+        const f4 a = code_numbers<FMT>(low), b = code_numbers<FMT>(high);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = static_cast<T>(a[i]), x[4 + i] = static_cast<T>(b[i]);
+        return x;
+    }
+}
 template <int DT, int FMT>
 __device__ __forceinline__ typename Coded<DT>::type code_value(uint8_t code, float scale) {
     return code_values<DT, FMT>(code, 0, scale)[0];
