@@ -13,50 +13,74 @@ namespace {
 
 typedef __attribute__((address_space(4))) const int32_t const_int;
 
-// Quotients of numbers below 2^31 by one divisor.
+// Quotients of numbers below 2^31 by one divisor, without a branch: the reciprocal is rounded down, so a product is one too
+// few at most.
 struct Divider {
     uint32_t by, reciprocal;
-    __device__ __forceinline__ explicit Divider(uint32_t d) : by(d), reciprocal(0xffffffffu / d + 1) {}  // (0 for 1)
+    __device__ __forceinline__ explicit Divider(uint32_t d) : by(d), reciprocal(0xffffffffu / d) {}
     __device__ __forceinline__ int quotient(int x) const {
-        if (by == 1) return x;
-        const uint32_t q = __umulhi(static_cast<uint32_t>(x), reciprocal);  // rounded up: one too many at most
-        return static_cast<int>(q * by > static_cast<uint32_t>(x) ? q - 1 : q);
+        const uint32_t q = __umulhi(static_cast<uint32_t>(x), reciprocal);
+        return static_cast<int>(q + (static_cast<uint32_t>(x) - q * by >= by ? 1 : 0));
     }
 };
 
-template <int DT, int FMT>
+// V channels of a row of keys (8, in aligned pieces, or 1): fetched, so that several are in flight, then taken as FP64.
+template <int DT, int FMT, int V>
 struct Row {
     typedef typename AttendType<DT>::type T;
-    static constexpr int kBytes = FMT != RCH_CODES_NONE ? 1 : static_cast<int>(sizeof(T));
-    // Eight channels (or fewer: V) of a row of keys as FP64 values.
-    template <int V>
-    static __device__ __forceinline__ void load(int64_t at, float scale, double (&x)[V]) {
-        if constexpr (FMT != RCH_CODES_NONE) {
-            if constexpr (V == 8) {
-                const u2 raw = *gin<u2>(at);
-                const auto value = code_values<DT, FMT>(raw[0], raw[1], scale);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(value[i]);
-            } else {
-                x[0] = static_cast<float>(code_value<DT, FMT>(*gin<uint8_t>(at), scale));
-            }
-        } else if constexpr (V == 8) {
-            typedef T t8 __attribute__((ext_vector_type(8), aligned(16)));
-            const t8 raw = *gin<t8>(at);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = static_cast<float>(raw[i]);
+    static constexpr int kBytes = FMT != RCH_CODES_NONE ? 1 : static_cast<int>(sizeof(T)), kWords = V * kBytes / 4;
+    uint32_t word[kWords ? kWords : 1];
+    float scale;
+
+    __device__ __forceinline__ void fetch(int64_t at, float s = 0.0f) {
+        scale = s;
+        if constexpr (kWords == 0 && kBytes == 1) {
+            word[0] = *gin<uint8_t>(at);
+        } else if constexpr (kWords == 0) {
+            word[0] = *gin<uint16_t>(at);
+        } else if constexpr (kWords == 1) {
+            word[0] = *gin<uint32_t>(at);
+        } else if constexpr (kWords == 2) {
+            const u2 raw = *gin<u2>(at);
+            word[0] = raw[0], word[1] = raw[1];
         } else {
-            x[0] = static_cast<float>(*gin<T>(at));
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                const u4 raw = gin<u4>(at)[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) word[4 * i + j] = raw[j];
+            }
+        }
+    }
+    __device__ __forceinline__ void clear_unless(bool kept) {
+#pragma unroll
+        for (uint32_t& w : word) w = kept ? w : 0u;
+        if constexpr (FMT != RCH_CODES_NONE) scale = kept ? scale : 0.0f;
+    }
+    __device__ __forceinline__ double value(int i) const {
+        if constexpr (FMT != RCH_CODES_NONE) {
+            if constexpr (V == 8) return static_cast<float>(code_values<DT, FMT>(word[0], word[1], scale)[i]);
+            else return static_cast<float>(code_value<DT, FMT>(static_cast<uint8_t>(word[0]), scale));
+        } else if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(word[i]);
+        } else if constexpr (DT == RCH_DT_BF16) {
+            return __uint_as_float(i % 2 ? word[i / 2] & 0xffff0000u : word[i / 2] << 16);
+        } else {
+            const h2 pair = __builtin_bit_cast(h2, word[i / 2]);
+            return static_cast<float>(pair[i % 2]);
         }
     }
 };
+
+// Keeps loads that are to be in flight together from being waited for one by one.
+__device__ __forceinline__ void all_issued() { __builtin_amdgcn_sched_barrier(0); }
 
 // One workgroup for up to 64 tokens (`share`) and a key head: where a token is the last one of its block among its
 // neighbours, the block's rows are summed, V channels and every kRows-th row to a thread.
 template <int DT, int FMT, int V>
 __global__ void __launch_bounds__(256) blocks_update_kernel(const rch_blocks B, int share) {
     typedef typename AttendType<DT>::type T;
-    typedef Row<DT, FMT> R;
+    typedef Row<DT, FMT, V> R;
     constexpr int kAhead = 8;  // rows in flight
     __shared__ double sums[256 * V];
     const int dim = static_cast<int>(B.head_dim), size = static_cast<int>(B.block_tokens), head = blockIdx.y;
@@ -82,18 +106,21 @@ __global__ void __launch_bounds__(256) blocks_update_kernel(const rch_blocks B, 
         for (int i = 0; i < V; ++i) sum[i] = 0.0;
         if (mine < rows) {
             for (int row = mine; row < size; row += rows * kAhead) {
-                double x[kAhead][V];
+                R x[kAhead];
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) {
                     const int at = min(row + a * rows, size - 1);
                     float scale = 0.0f;
                     if constexpr (FMT != RCH_CODES_NONE) scale = gin<float>(scales)[at];
-                    R::template load<V>(keys + R::kBytes * at * B.token_stride, scale, x[a]);
+                    x[a].fetch(keys + R::kBytes * at * B.token_stride, scale);
                 }
+                all_issued();
 #pragma unroll
-                for (int a = 0; a < kAhead; ++a)
+                for (int a = 0; a < kAhead; ++a) {
+                    x[a].clear_unless(row + a * rows < size);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) sum[i] += row + a * rows < size ? x[a][i] : 0.0;
+                    for (int i = 0; i < V; ++i) sum[i] += x[a].value(i);
+                }
             }
         }
 #pragma unroll
@@ -124,11 +151,9 @@ __device__ __forceinline__ Run run_of(const rch_blocks& B, int index) {
     const const_int* w = (const const_int*)(uintptr_t)(B.plan_ptr + 4 * (B.runs + static_cast<int64_t>(index) * RCH_BLOCKS_RUN));
     return {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8]};
 }
-// The pool's page that is a run's `index`-th, or -1 for a hole.
-__device__ __forceinline__ int page_of(const rch_blocks& B, const Run& R, int index) {
-    const int id = gin<int32_t>(B.plan_ptr)[R.table + index];
-    return id >= 0 && id < B.pages ? id : -1;
-}
+// The entry of a run's table for its `index`-th page, and whether it is no hole.
+__device__ __forceinline__ int page_of(const rch_blocks& B, const Run& R, int index) { return gin<int32_t>(B.plan_ptr)[R.table + index]; }
+__device__ __forceinline__ bool page_held(const rch_blocks& B, int id) { return id >= 0 && id < static_cast<int>(B.pages); }
 
 constexpr int kScored = 128;     // blocks that a workgroup of the separate scoring takes
 constexpr int kTogether = RCH_BLOCKS_TOGETHER;  // most scored blocks of a run whose numbers fit in LDS, scored and taken by one workgroup
@@ -137,7 +162,7 @@ constexpr int kTogether = RCH_BLOCKS_TOGETHER;  // most scored blocks of a run w
 template <int DT, int V, int THREADS>
 __device__ __forceinline__ void pool_queries(const rch_blocks& B, const Run& R, int head, double* sums, double* pooled) {
     typedef typename AttendType<DT>::type T;
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     const int dim = static_cast<int>(B.head_dim), group = static_cast<int>(B.group), count = R.queries * group;
     const int lanes = dim / V, rows = 256 / lanes, mine = threadIdx.x / lanes, piece = threadIdx.x - mine * lanes;
     const Divider by_group(group);
@@ -147,17 +172,19 @@ __device__ __forceinline__ void pool_queries(const rch_blocks& B, const Run& R, 
         for (int i = 0; i < V; ++i) sum[i] = 0.0;
         if (mine < rows) {
             for (int row = mine; row < count; row += rows * kAhead) {
-                double x[kAhead][V];
+                Row<DT, RCH_CODES_NONE, V> x[kAhead];
 #pragma unroll
                 for (int a = 0; a < kAhead; ++a) {
                     const int at = min(row + a * rows, count - 1), token = by_group.quotient(at), member = head * group + at - token * group;
-                    Row<DT, RCH_CODES_NONE>::template load<V>(
-                        B.q_ptr + static_cast<int64_t>(sizeof(T)) * ((R.q_row + token) * B.q_token_stride + member * B.q_head_stride + piece * V), 0.0f, x[a]);
+                    x[a].fetch(B.q_ptr + static_cast<int64_t>(sizeof(T)) * ((R.q_row + token) * B.q_token_stride + member * B.q_head_stride + piece * V));
                 }
+                all_issued();
 #pragma unroll
-                for (int a = 0; a < kAhead; ++a)
+                for (int a = 0; a < kAhead; ++a) {
+                    x[a].clear_unless(row + a * rows < count);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) sum[i] += row + a * rows < count ? x[a][i] : 0.0;
+                    for (int i = 0; i < V; ++i) sum[i] += x[a].value(i);
+                }
             }
         }
 #pragma unroll
@@ -174,12 +201,22 @@ __device__ __forceinline__ void pool_queries(const rch_blocks& B, const Run& R, 
     __syncthreads();
 }
 
+// Lanes with `upper` keep the upper N of 2 N sums, the others the lower ones, each with its neighbour's (lane ^ N) added.
+template <int N>
+__device__ __forceinline__ void fold(double* x, bool upper) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const double give = upper ? x[i] : x[N + i], keep = upper ? x[N + i] : x[i];
+        x[i] = keep + __shfl_xor(give, N);
+    }
+}
+
 // Numbers of blocks [begin, end) of a run and key head, to out(block, number).  A block's mean lies in `width` lanes (a power
 // of two), V channels to a lane; a thread has kAhead blocks in flight (pages first, then means).
 template <int DT, int V, int THREADS, typename Out>
 __device__ __forceinline__ void score_blocks(const rch_blocks& B, const Run& R, int head, int begin, int end, const double* pooled, Out out) {
     typedef typename AttendType<DT>::type T;
-    constexpr int kAhead = V == 1 ? 1 : THREADS == 256 ? 8 : 4;
+    constexpr int kAhead = V == 1 ? 1 : 8;
     const int lane = threadIdx.x & 63, dim = static_cast<int>(B.head_dim);
     const Divider by_page(static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(B.block_tokens));
     const int per = static_cast<int>(by_page.by);
@@ -198,45 +235,58 @@ __device__ __forceinline__ void score_blocks(const rch_blocks& B, const Run& R, 
             in_page[a] = block - index * per;
             page[a] = page_of(B, R, index);
         }
+        all_issued();
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) page[a] = page_held(B, page[a]) ? page[a] : -1;
         double score[kAhead];
         if constexpr (V == 8) {
-            double x[kAhead][V];
+            Row<DT, RCH_CODES_NONE, V> x[kAhead];
+            const bool in = at * V < dim;
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                const bool in = page[a] >= 0 && at * V < dim;
-                // (elsewhere the pool's first mean, which is not used)
-                Row<DT, RCH_CODES_NONE>::template load<V>(
-                    base + (in ? (static_cast<int64_t>(page[a]) * per + in_page[a]) * block_bytes + static_cast<int64_t>(sizeof(T)) * at * V : 0), 0.0f, x[a]);
-                if (!in)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) x[a][i] = 0.0;
+            for (int a = 0; a < kAhead; ++a) {  // (of a hole, page 0's; behind the head's channels, the first ones)
+                const int64_t block = static_cast<int64_t>(max(page[a], 0)) * per + in_page[a];
+                x[a].fetch(base + block * block_bytes + (in ? static_cast<int64_t>(sizeof(T)) * at * V : 0));
             }
+            all_issued();
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
                 score[a] = 0.0;
+                if (first + a * step >= end) continue;
+                x[a].clear_unless(in);
 #pragma unroll
-                for (int i = 0; i < V; ++i) score[a] = __builtin_fma(x[a][i], q[i], score[a]);
+                for (int i = 0; i < V; ++i) score[a] = __builtin_fma(x[a].value(i), q[i], score[a]);
             }
         } else {
             score[0] = 0.0;
-            if (page[0] >= 0) {
-                const int64_t mean = base + (static_cast<int64_t>(page[0]) * per + in_page[0]) * block_bytes;
-                for (int d = at; d < dim; d += width) {
-                    double x[1];
-                    Row<DT, RCH_CODES_NONE>::template load<1>(mean + static_cast<int64_t>(sizeof(T)) * d, 0.0f, x);
-                    score[0] = __builtin_fma(x[0], pooled[d], score[0]);
-                }
+            const int64_t mean = base + (static_cast<int64_t>(max(page[0], 0)) * per + in_page[0]) * block_bytes;
+            for (int d = at; d < dim; d += width) {
+                Row<DT, RCH_CODES_NONE, 1> x;
+                x.fetch(mean + static_cast<int64_t>(sizeof(T)) * d);
+                score[0] = __builtin_fma(x.value(0), pooled[d], score[0]);
             }
         }
-        for (int o = 1; o < width; o <<= 1)
+        const int block = first + static_cast<int>(threadIdx.x) / width;
+        if (kAhead == 8 && width >= 8) {
+            // The sums over a block's lanes: each step joins two of the blocks into one, half of the lanes for each, so that
+            // lane `at` ends with block at % 8.
+            int held = page[0];
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) score[a] += __shfl_xor(score[a], o);
-        if (at == 0)
+            for (int a = 1; a < kAhead; ++a) held = (at & 7) == a ? page[a] : held;
+            fold<4>(score, at & 4);
+            fold<2>(score, at & 2);
+            fold<1>(score, at & 1);
+            double own = score[0];
+            for (int o = 8; o < width; o <<= 1) own += __shfl_xor(own, o);
+            if (at < 8 && block + at * step < end) out(block + at * step, held >= 0 ? order_of(own) : 0);
+        } else {
+            for (int o = 1; o < width; o <<= 1)
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                const int block = first + a * step + static_cast<int>(threadIdx.x) / width;
-                if (block < end) out(block, page[a] >= 0 ? order_of(score[a]) : 0);
-            }
+                for (int a = 0; a < kAhead; ++a) score[a] += __shfl_xor(score[a], o);
+            if (at == 0)
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+                    if (block + a * step < end) out(block + a * step, page[a] >= 0 ? order_of(score[a]) : 0);
+        }
     }
 }
 
@@ -340,7 +390,7 @@ __device__ __forceinline__ void take_blocks(const rch_blocks& B, const Run& R, i
     for (int base = R.first; base < R.last; base += THREADS) {
         const int block = base + t;
         bool taken = false, same = false;
-        if (block < R.last && page_of(B, R, by_page.quotient(block)) >= 0) {
+        if (block < R.last && page_held(B, page_of(B, R, by_page.quotient(block)))) {
             if (all || !chosen_by_score(block)) {
                 taken = true;
             } else if (mask) {  // (none is wanted otherwise, and there may be no scores)
@@ -436,7 +486,7 @@ int update(const rch_blocks& B, hipStream_t stream) {
     const int64_t wanted = B.tokens * B.heads / 1024;
     const int share = static_cast<int>(wanted < 1 ? 1 : wanted > 64 ? 64 : wanted);
     const dim3 grid(static_cast<uint32_t>((B.tokens + share - 1) / share), static_cast<uint32_t>(B.heads));
-    const int64_t bytes = Row<DT, FMT>::kBytes, piece = FMT == RCH_CODES_NONE ? 16 : 8;
+    const int64_t bytes = Row<DT, FMT, 8>::kBytes, piece = FMT == RCH_CODES_NONE ? 16 : 8;
     const bool wide = B.head_dim % 8 == 0 && B.keys_ptr % piece == 0 && (B.page_stride | B.token_stride | B.head_stride) * bytes % piece == 0;
     if (wide) hipLaunchKernelGGL((blocks_update_kernel<DT, FMT, 8>), grid, dim3(256), 0, stream, B, share);
     else hipLaunchKernelGGL((blocks_update_kernel<DT, FMT, 1>), grid, dim3(256), 0, stream, B, share);
