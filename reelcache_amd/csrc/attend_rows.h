@@ -9,10 +9,13 @@ namespace rch {
 // FMT: what the pools hold (RCH_CODES_*).
 template <int DT, int NB, int MODE, int FMT>
 __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_rows_kernel(const rch_attend A) {
-    typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2> Tile;
+    constexpr bool kCodes = FMT != RCH_CODES_NONE;
+    typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2, kCodes && NB != 3 && NB != 6> Tile;
     constexpr int KT = Tile::KT, ES = Tile::ES, kTileBytes = KT * Tile::RB;
     constexpr int kStageBytes = 2 * kTileBytes;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * kStageBytes];
+    typedef typename std::conditional_t<kCodes, std::common_type<CodeFetch<DT == RCH_DT_F32 ? RCH_DT_BF16 : DT, Tile, MODE, kCodes ? FMT : RCH_CODES_INT8>>,
+                                        std::common_type<Fetch<Tile, MODE>>>::type Fetcher;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * kStageBytes + (kCodes ? 4 * kTileBytes / 4 : 0)];  // codes: half as many bytes
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const AttendItem I = attend_item(A, blockIdx.x);
@@ -25,16 +28,17 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     WaveRange range;
     range.init(R);
 
-    constexpr bool kCodes = FMT != RCH_CODES_NONE;
     if constexpr (kCodes) wait_vector_memory();  // the queries, so that no tile's wait is for them
     KeyWalk<KT, MODE, kCodes> walk;
     walk.begin(A, I, kCodes ? 1 : ES);
-    typename std::conditional_t<kCodes, std::common_type<CodeFetch<DT == RCH_DT_F32 ? RCH_DT_BF16 : DT, Tile, MODE, kCodes ? FMT : RCH_CODES_INT8>>,
-                                std::common_type<Fetch<Tile, MODE>>>::type fetch;
+    Fetcher fetch;
     if constexpr (kCodes) fetch.init(A, I, wave, lane);
     else fetch.init(A, wave, lane);
     lds_char* const tiles = (lds_char*)lds;
     const uint32_t mine = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(tiles)) + wave * (kTileBytes / 4);
+
+    lds_char* const codes = tiles + 2 * kStageBytes + wave * (kTileBytes / 4);
+    const uint32_t own_codes = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(codes));
 
     // The tile on its way: its first key and keys; `walk` is the one after it.
     bool coming = false;
@@ -45,7 +49,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
         if (!coming) return;
         next_key = walk.base;
         next_keys = walk.count();
-        if constexpr (kCodes) fetch.load(A, walk);
+        if constexpr (kCodes) fetch.issue(A, walk, own_codes);
         else fetch.issue(A, walk, mine + to, mine + to + kTileBytes);
         walk.next();
         fetch.look_up(walk);
@@ -55,13 +59,16 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     // Waits for the tile on its way, fetches another one, and tells whether the wave's rows see any of it.
     auto advance = [&]() {
         if constexpr (kCodes) {
-            // Into the half that no wave reads since the last barrier; the next tile's loads are in flight behind it.
+            // The wave's codes have landed; their values go into the half that no wave reads since the last barrier, and the
+            // next codes into their place.
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             at = kStageBytes - at;
-            fetch.commit(tiles + at, tiles + at + kTileBytes);
+            fetch.commit(codes, tiles + at, tiles + at + kTileBytes, lane);
             key = next_key;
             keys = next_keys;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             send(0);
-            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            asm volatile("s_barrier" ::: "memory");
         } else {
             // The tile has landed in every wave's share, and no wave reads the other half any more.
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");

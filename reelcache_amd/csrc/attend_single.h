@@ -221,9 +221,9 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[b][i] *= fade;
         }
-        // bf16: the values' scales go to the weights (rounded once, as they are without; the codes are exact).  fp16 does not
-        // hold such weights: there the scales go to the values.
-        constexpr bool kScaled = DT == RCH_DT_BF16;
+        // 8-bit floats in bf16: the scales, powers of two, go to the weights (whose rounding stays what it is).  fp16 does not
+        // hold such weights, and integers times other scales are rounded as values.
+        constexpr bool kScaled = DT == RCH_DT_BF16 && FMT == RCH_CODES_E4M3;
         f4 v_scale[4];  // of the keys of registers 4 i ..
 #pragma unroll
         for (int i = 0; i < 4; ++i) v_scale[i] = *(lds_f4*)(scales + 32 + 8 * i + 4 * h);

@@ -470,8 +470,8 @@ __device__ __forceinline__ void add_marks(f16v& sum, const f16v& code) {
     }
 }
 
-// One wave's state over the tiles and the arithmetic of a tile of KB * 32 keys.
-template <int DT, int NB, int KB>
+// One wave's state over the tiles and the arithmetic of a tile of KB * 32 keys.  LEAN: with fewer registers.
+template <int DT, int NB, int KB, bool LEAN = false>
 struct RowTile {
     typedef Half<DT> H;
     typedef typename H::type T;
@@ -486,7 +486,7 @@ struct RowTile {
     Reference reference;
     float sum;
     // LDS byte offsets within a tile; of wide heads the first, from which the others follow by an exclusive or.
-    static constexpr bool kWide = NB > 4;
+    static constexpr bool kWide = NB > 4 || LEAN;
     uint32_t k_lane[kWide ? 1 : 2 * NB], v_lane[kWide ? 1 : NB];
     __device__ __forceinline__ uint32_t k_at(int s) const { return kWide ? k_lane[0] ^ (s * 32) : k_lane[s]; }
     __device__ __forceinline__ uint32_t v_at(int b) const { return kWide ? v_lane[0] ^ (b * 64) : v_lane[b]; }
@@ -544,7 +544,7 @@ struct RowTile {
                 for (int i = 0; i < 16; ++i) s[b][i] = seen[b] >> i & 1u ? s[b][i] : -INFINITY;
         }
         // The first values, on their way while the weights are computed.
-        constexpr int kRing = kWide ? 4 : NB;  // values read ahead
+        constexpr int kRing = NB > 4 ? 4 : LEAN ? 2 : NB;  // values read ahead
         vec8 v[kRing];
         if constexpr (!RARE) {
 #pragma unroll
@@ -678,7 +678,7 @@ struct RowTile {
 // 16-byte piece of K (and of Q) feeds four products, and register i of S^T is, as it is, the B operand of the
 // keys that registers i of both halves hold; V^T is read one value a lane.
 template <int NB>
-struct RowTile<RCH_DT_F32, NB, 1> {
+struct RowTile<RCH_DT_F32, NB, 1, false> {
     typedef float T;
     static constexpr int ES = 4, RB = NB <= 2 ? 256 : NB <= 4 ? 512 : 1024, kPieces = RB / 16, KT = 32;
     static __device__ __forceinline__ int k_swizzle(int row) { return row % kPieces; }
