@@ -640,9 +640,10 @@ int rch_codes_read(const rch_codes* args_host, int dtype, void* stream);
  * Pools in codes (codes != RCH_CODES_NONE; q, out in f16 or bf16): keys and values are what the codes stand for,
  * rounded to the dtype (rch_codes_store).
  * Lists (lists_ptr != 0): an item's keys are those of chosen blocks of block_tokens keys, which divide a page.  Its
- * word 10 is the index in lists (int32) of its first entry, the number of a block of the sequence; key_begin and key_end
- * count tiles of 64 (f32, or single: 32) keys from there, ceil(block_tokens / tile) to an entry.  An entry that is no block of the
- * sequence, or lies in a hole, has no keys.
+ * word 10 is the index in lists (int32) of its first entry, the number of a block of the sequence, word 11 their count;
+ * key_begin and key_end count tiles of 64 (f32, or single: 32) keys from there.  tile_unit == block_tokens:
+ * ceil(block_tokens / tile) to an entry; tile_unit == tile (n_rows, not single, blocks of a multiple of tile / 4 keys): over
+ * the entries' keys one after the other.  An entry that is no block of the sequence, or lies in a hole, has no keys.
  */
 #define RCH_ATTEND_ITEM 12
 #define RCH_ATTEND_MERGE 8
@@ -670,7 +671,7 @@ typedef struct rch_attend {
                                       eight channels, and others as the caller likes */
     int64_t most_rows_many, most_rows; /* most rows of one of those, and of one of the others */
     int64_t holes;           /* 1: page tables may hold holes */
-    int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64 */
+    int64_t tile_unit;       /* keys that tiles start over at: page_tokens (a tile lies in one page), or 64; lists: see above */
     int64_t codes;           /* RCH_CODES_* */
     int64_t k_scale_ptr, v_scale_ptr; /* of pools in codes; strides in elements */
     int64_t k_scale_page_stride, k_scale_head_stride, v_scale_page_stride, v_scale_head_stride;

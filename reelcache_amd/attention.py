@@ -279,7 +279,7 @@ class AttentionPlan:
         items[:, 4], items[:, 5], items[:, 6] = begin[which], end[which], head[which]
         items[:, 7], items[:, 8] = keys(which, low, high, part, n)
         items[:, 9] = np.where(n > 1, base[which] + part * rows, -1)
-        items[:, 10] = self._lists_of(which)
+        items[:, 10], items[:, 11] = self._lists_of(which)
         several = parts > 1
         if several.any():
             rows = (end - begin)[several]
@@ -290,8 +290,8 @@ class AttentionPlan:
         return self._ordered(items, high - low, xcd)
 
     def _lists_of(self, which):
-        """Where the chosen blocks of row blocks stand among the lists."""
-        return 0
+        """Where the chosen blocks of row blocks stand among the lists, and their number."""
+        return 0, 0
 
     @staticmethod
     def _ordered(items, cost, xcd):

@@ -7,12 +7,12 @@ namespace rch {
 
 // One item of a plan (rch_attend in reelcache_hip.h).
 struct AttendItem {
-    int table, length, q_row, queries, row_begin, row_end, kv_head, key_begin, key_end, part, list;
+    int table, length, q_row, queries, row_begin, row_end, kv_head, key_begin, key_end, part, list, entries;
 };
 
 __device__ __forceinline__ AttendItem attend_item(const rch_attend& A, int index) {
     const RCH_GLOBAL int32_t* w = gin<int32_t>(A.plan_ptr) + A.items + static_cast<int64_t>(index) * RCH_ATTEND_ITEM;
-    return {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10]};
+    return {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10], w[11]};
 }
 
 // Keys [first, last) that query token i of a sequence sees (apart from holes).
@@ -81,13 +81,13 @@ __device__ __forceinline__ bool sees_any(const rch_attend& A, const AttendItem& 
     return false;
 }
 
-// The same for an item of chosen blocks, whose entries hold `per` tiles each: whether it sees a key of one of them.
-__device__ __forceinline__ bool sees_any_listed(const rch_attend& A, const AttendItem& I, int first, int last, int per) {
+// The same for an item of chosen blocks, whose entries [from, to) hold its tiles: whether it sees a key of one of them.
+__device__ __forceinline__ bool sees_any_listed(const rch_attend& A, const AttendItem& I, int first, int last, int from, int to) {
     const RCH_GLOBAL int32_t* table = gin<int32_t>(A.plan_ptr) + I.table;
     const RCH_GLOBAL int32_t* list = gin<int32_t>(A.lists_ptr) + I.list;
     const int unit = static_cast<int>(A.block_tokens), size = static_cast<int>(A.page_tokens);
     const int blocks = (I.length + unit - 1) / unit;
-    for (int at = I.key_begin / per; at * per < I.key_end; ++at) {
+    for (int at = from; at < to; ++at) {
         const int block = list[at];
         if (block < 0 || block >= blocks) continue;
         const int begin = block * unit, id = table[begin / size];

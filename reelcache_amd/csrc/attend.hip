@@ -394,6 +394,9 @@ int rch_attend_run(const rch_attend* args_host, int dtype, void* stream) {
                         RCH_ATTEND_FAST_DIM);
         if (A.k_token_stride < 0 || A.v_token_stride < 0 || A.k_token_stride > (1 << 22) || A.v_token_stride > (1 << 22))
             return fail(RCH_E_UNSUPPORTED, "rch_attend_run: token rows too far apart for the tiled forms");
+        const int64_t tile = dtype == RCH_DT_F32 ? 32 : 64;
+        if (A.lists_ptr && A.tile_unit != A.block_tokens && (A.single || A.tile_unit != tile || A.block_tokens % (tile / 4)))
+            return fail(RCH_E_CONFIG, "rch_attend_run: tiles start over at each chosen block, or run on over blocks of whole quarters of a tile");
         if (!A.lists_ptr && !(A.tile_unit == 64 || (A.tile_unit == A.page_tokens && A.page_tokens >= 64)))
             return fail(RCH_E_CONFIG, "rch_attend_run: tiles start over at a page of 64 or more tokens, or at 64 keys");
     }

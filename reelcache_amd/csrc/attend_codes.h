@@ -20,16 +20,19 @@ struct CodeFetch {
     static constexpr int NI = kShareRows / kRows;  // loads of a wave's quarter of K, or of V
     static constexpr int kWaveBytes = 2 * NI * 1024;
     float k_scale[NI], v_scale[NI];
-    int row0, piece, pieces;  // the lane's first row, its 16 channels, such pieces of a head
+    // Tiles whose shares are found one by one: a wave's rows lie in one page, and so do those of a page's or block's tile.
+    static constexpr bool kShares = MODE == kShare || MODE == kPack;
+    int share, row0, piece, pieces;  // the share's first row, the lane's first one, its 16 channels, such pieces of a head
     uint32_t k_at[MODE == kRow ? 1 : NI], v_at[MODE == kRow ? 1 : NI];  // byte offsets in a tile of one page
     uint32_t size, magic, dim, k_row, v_row;
     int64_t ks_head, vs_head, ks_page, vs_page;  // scales of the item's head in page 0; bytes of a page
     int ids[MODE == kRow ? NI : 1];
-    int count;  // rows of the tile on its way
+    int count;  // rows of the tile (or share) on its way
 
     __device__ __forceinline__ void init(const rch_attend& A, const AttendItem& I, int wave, int lane) {
         pieces = static_cast<int>(A.head_dim) / 16;
-        row0 = wave * kShareRows + lane / kLanes;
+        share = wave * kShareRows;
+        row0 = share + lane / kLanes;
         piece = lane % kLanes;
         k_row = static_cast<uint32_t>(A.k_token_stride);
         v_row = static_cast<uint32_t>(A.v_token_stride);
@@ -43,8 +46,9 @@ struct CodeFetch {
         if constexpr (MODE != kRow) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                k_at[i] = piece < pieces ? (row0 + i * kRows) * k_row + piece * 16 : kOutOfRange;
-                v_at[i] = piece < pieces ? (row0 + i * kRows) * v_row + piece * 16 : kOutOfRange;
+                const int row = row0 + i * kRows - (kShares ? share : 0);
+                k_at[i] = piece < pieces ? row * k_row + piece * 16 : kOutOfRange;
+                v_at[i] = piece < pieces ? row * v_row + piece * 16 : kOutOfRange;
             }
         }
     }
@@ -52,10 +56,12 @@ struct CodeFetch {
         return size < 64 ? static_cast<int>((x * magic) >> 16) : (x >= size ? 1 : 0);
     }
     __device__ __forceinline__ void look_up(const KeyWalk<KT, MODE, true>& W) {
-        if constexpr (MODE == kRow) {
+        if constexpr (MODE == kShare || MODE == kRow) {
             if (W.done()) return;
             const int keys = W.end - W.base, page0 = W.base / static_cast<int>(size);
             const int off0 = W.base - page0 * static_cast<int>(size);
+            if constexpr (MODE == kShare) ids[0] = W.table[page0 + page_of(off0 + min(share, keys - 1))];
+            else
 #pragma unroll
             for (int i = 0; i < NI; ++i) ids[i] = page_entry(W.table, page0 + page_of(off0 + min(row0 + i * kRows, keys - 1)));
         }
@@ -63,11 +69,27 @@ struct CodeFetch {
 
     // Sends the walk's tile on its way to the wave's LDS at `lds`.  Rows without a key have codes 0.
     __device__ __forceinline__ void issue(const rch_attend& A, const KeyWalk<KT, MODE, true>& W, uint32_t lds) {
-        count = W.count();
         if constexpr (MODE != kRow) {
-            const uint32_t last = static_cast<uint32_t>(count - 1);
-            const u4 kr = tile_rsrc(W.k, last * k_row + dim), vr = tile_rsrc(W.v, last * v_row + dim);
-            const int64_t ks = ks_head + W.id * ks_page + 4 * static_cast<int64_t>(W.in_page), vs = vs_head + W.id * vs_page + 4 * static_cast<int64_t>(W.in_page);
+            int64_t k, v;
+            int id, in_page;
+            if constexpr (kShares) {
+                if constexpr (MODE == kPack) {
+                    W.own(id, in_page, count);
+                } else {
+                    const int x = W.base % static_cast<int>(size) + share;
+                    in_page = x - page_of(x) * static_cast<int>(size);
+                    id = ids[0];
+                    count = id >= 0 && id < W.pages ? max(0, min(W.count() - share, kShareRows)) : 0;
+                }
+                if (count == 0) id = in_page = 0;  // nothing is in its range
+                k = W.k_head + id * W.k_page + in_page * static_cast<int64_t>(k_row);
+                v = W.v_head + id * W.v_page + in_page * static_cast<int64_t>(v_row);
+            } else {
+                id = W.id, in_page = W.in_page, k = W.k, v = W.v;
+                count = W.count();
+            }
+            const u4 kr = tile_rsrc(k, count > 0 ? (count - 1) * k_row + dim : 0), vr = tile_rsrc(v, count > 0 ? (count - 1) * v_row + dim : 0);
+            const int64_t ks = ks_head + id * ks_page + 4 * static_cast<int64_t>(in_page), vs = vs_head + id * vs_page + 4 * static_cast<int64_t>(in_page);
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
                 fetch_buffer(kr, k_at[i], lds + i * 1024);
@@ -75,11 +97,12 @@ struct CodeFetch {
             }
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int row = min(row0 + i * kRows, count - 1);
+                const int row = max(0, min(row0 + i * kRows - (kShares ? share : 0), count - 1));
                 k_scale[i] = gin<float>(ks)[row];
                 v_scale[i] = gin<float>(vs)[row];
             }
         } else {
+            count = W.count();
             const int off0 = W.base % static_cast<int>(size);
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
@@ -118,7 +141,7 @@ struct CodeFetch {
         for (int i = 0; i < NI; ++i) {
             const int row = row0 + i * kRows;
             // (codes behind the last row are 0, their scales another row's)
-            const bool none = MODE != kRow && row >= count;
+            const bool none = MODE != kRow && row - (kShares ? share : 0) >= count;
             put(k_tile + row * RB, 2 * piece, Tile::k_swizzle(row), k[i], none ? 0.0f : k_scale[i]);
             put(v_tile + row * RB, 2 * piece, Tile::v_swizzle(row), v[i], none ? 0.0f : v_scale[i]);
         }

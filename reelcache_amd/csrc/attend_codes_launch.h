@@ -9,8 +9,10 @@ namespace rch {
 template <int DT, int NB, int FMT>
 void launch_codes(const rch_attend& A, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(A.n_rows));
-    if (A.lists_ptr) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kList, FMT>), grid, dim3(256), 0, stream, A);
+    if (A.lists_ptr && A.tile_unit == A.block_tokens) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kList, FMT>), grid, dim3(256), 0, stream, A);
+    else if (A.lists_ptr) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kPack, FMT>), grid, dim3(256), 0, stream, A);
     else if (A.tile_unit == A.page_tokens) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kPage, FMT>), grid, dim3(256), 0, stream, A);
+    else if (A.page_tokens % 16 == 0) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kShare, FMT>), grid, dim3(256), 0, stream, A);
     else hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kRow, FMT>), grid, dim3(256), 0, stream, A);
 }
 

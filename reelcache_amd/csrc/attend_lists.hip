@@ -1,18 +1,25 @@
-// Attention to chosen blocks of keys: each item walks a list of blocks of its sequence, in tiles that start over at each.
+// Attention to chosen blocks of keys: each item walks a list of blocks of its sequence, in tiles that start over at each
+// or run on over them (blocks of a multiple of 16 keys that is none of 64; fp32: 8 and 32).
 #include "attend_rows.h"
 
 namespace rch {
 
 namespace {
 
+template <int DT, int NB>
+void launch(const rch_attend& A, hipStream_t stream) {
+    const dim3 grid(static_cast<uint32_t>(A.n_rows));
+    if (A.tile_unit == A.block_tokens) hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kList, RCH_CODES_NONE>), grid, dim3(256), 0, stream, A);
+    else hipLaunchKernelGGL((attend_rows_kernel<DT, NB, kPack, RCH_CODES_NONE>), grid, dim3(256), 0, stream, A);
+}
+
 template <int DT>
 void launch_dim(const rch_attend& A, hipStream_t stream) {
-    const dim3 grid(static_cast<uint32_t>(A.n_rows));
-    if (A.head_dim <= 64) hipLaunchKernelGGL((attend_rows_kernel<DT, 2, kList, RCH_CODES_NONE>), grid, dim3(256), 0, stream, A);
-    else if (A.head_dim <= 96) hipLaunchKernelGGL((attend_rows_kernel<DT, 3, kList, RCH_CODES_NONE>), grid, dim3(256), 0, stream, A);
-    else if (A.head_dim <= 128) hipLaunchKernelGGL((attend_rows_kernel<DT, 4, kList, RCH_CODES_NONE>), grid, dim3(256), 0, stream, A);
-    else if (A.head_dim <= 192) hipLaunchKernelGGL((attend_rows_kernel<DT, 6, kList, RCH_CODES_NONE>), grid, dim3(256), 0, stream, A);
-    else hipLaunchKernelGGL((attend_rows_kernel<DT, 8, kList, RCH_CODES_NONE>), grid, dim3(256), 0, stream, A);
+    if (A.head_dim <= 64) launch<DT, 2>(A, stream);
+    else if (A.head_dim <= 96) launch<DT, 3>(A, stream);
+    else if (A.head_dim <= 128) launch<DT, 4>(A, stream);
+    else if (A.head_dim <= 192) launch<DT, 6>(A, stream);
+    else launch<DT, 8>(A, stream);
 }
 
 }  // namespace

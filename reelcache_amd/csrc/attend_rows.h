@@ -30,6 +30,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
 
     if constexpr (kCodes) wait_vector_memory();  // the queries, so that no tile's wait is for them
     KeyWalk<KT, MODE, kCodes> walk;
+    if constexpr (MODE == kPack) walk.wave = wave;
     walk.begin(A, I, kCodes ? 1 : ES);
     Fetcher fetch;
     if constexpr (kCodes) fetch.init(A, I, wave, lane);
@@ -44,11 +45,18 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     bool coming = false;
     int next_key = 0, next_keys = 0, at = kStageBytes, key = 0, keys = 0, first = 0, last = 0;
     uint64_t held = ~uint64_t{0};
+    int next_shares[4], shares[4];  // kPack: first keys of the tiles' shares
+    ShareView<KT / 4> view;
     auto send = [&](int to) {
         coming = !walk.done();
         if (!coming) return;
-        next_key = walk.base;
-        next_keys = walk.count();
+        if constexpr (MODE == kPack) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) next_shares[s] = walk.first_key(s);
+        } else {
+            next_key = walk.base;
+            next_keys = walk.count();
+        }
         if constexpr (kCodes) fetch.issue(A, walk, own_codes);
         else fetch.issue(A, walk, mine + to, mine + to + kTileBytes);
         walk.next();
@@ -56,6 +64,11 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     };
     fetch.look_up(walk);
     send(0);
+    auto copy_shares = [&]() {
+        if constexpr (MODE == kPack)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) shares[s] = next_shares[s];
+    };
     // Waits for the tile on its way, fetches another one, and tells whether the wave's rows see any of it.
     auto advance = [&]() {
         if constexpr (kCodes) {
@@ -66,6 +79,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
             fetch.commit(codes, tiles + at, tiles + at + kTileBytes, lane);
             key = next_key;
             keys = next_keys;
+            copy_shares();
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             send(0);
             asm volatile("s_barrier" ::: "memory");
@@ -74,9 +88,14 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             key = next_key;
             keys = next_keys;
+            copy_shares();
             const int other = at;
             at = kStageBytes - at;
             send(other);
+        }
+        if constexpr (MODE == kPack) {
+            view.look(walk, range, shares);
+            return active && view.sees;
         }
         if constexpr (MODE == kShare || MODE == kRow) {
             if (A.holes) {
@@ -87,6 +106,12 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
         return active && range.sees(key, keys);
     };
     auto masked = [&]() {
+        if constexpr (MODE == kPack) {
+            first = 0;
+            last = KT;
+            if (view.masked) held = ShareView<KT / 4>::bits(walk, shares, R.first, R.last);
+            return view.masked;
+        }
         first = R.first - key;
         last = min(R.last - key, keys);
         return range.masked(key, keys, KT) || held != ~uint64_t{0};
@@ -96,7 +121,7 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
         if (!advance()) continue;
         const bool some = masked();
         // (Rows behind the last key, and those of a hole, are zeros: only keys that a row does not see may be anything.)
-        if (some && range.hides(key, keys) && Tile::any_infinite(tiles + at + kTileBytes, lane)) {
+        if (some && (MODE == kPack ? view.hides : range.hides(key, keys)) && Tile::any_infinite(tiles + at + kTileBytes, lane)) {
             rare = true;
             break;
         }
@@ -117,7 +142,9 @@ __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_row
     const float sum = row_sum(tile.sum);
     bool blank = false;
     if (sum == 0.0f) {
-        if constexpr (MODE == kList) blank = sees_any_listed(A, I, R.first, R.last, (static_cast<int>(A.block_tokens) + KT - 1) / KT);
+        const int unit = max(static_cast<int>(A.block_tokens), 1), per = (unit + KT - 1) / KT;
+        if constexpr (MODE == kList) blank = sees_any_listed(A, I, R.first, R.last, I.key_begin / per, (I.key_end + per - 1) / per);
+        else if constexpr (MODE == kPack) blank = sees_any_listed(A, I, R.first, R.last, I.key_begin * KT / unit, min(I.entries, (I.key_end * KT + unit - 1) / unit));
         else blank = sees_any(A, I, R.first, R.last);
     }
     if (I.part >= 0) {

@@ -255,7 +255,8 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
     sum = row_sum(sum);
     bool blank = false;
     if (sum == 0.0f) {
-        if constexpr (MODE == kList) blank = sees_any_listed(A, I, R.first, R.last, (static_cast<int>(A.block_tokens) + KT - 1) / KT);
+        const int per = (static_cast<int>(A.block_tokens) + KT - 1) / KT;
+        if constexpr (MODE == kList) blank = sees_any_listed(A, I, R.first, R.last, I.key_begin / per, (I.key_end + per - 1) / per);
         else blank = sees_any(A, I, R.first, R.last);
     }
     if (I.part >= 0) {

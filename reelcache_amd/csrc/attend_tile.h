@@ -156,7 +156,18 @@ __device__ __forceinline__ int page_entry(const const_int* table, int index) {
 // consecutive keys, and the KT / 4 rows that a wave fetches lie in one page (its size is a multiple of that);
 // kRow: any page size.  The first two take a scalar base to a fetch, the last an address to a lane.
 // kList: chosen blocks of keys, one after the other; a block lies in one page and tiles start over at each.
-enum TileMode { kPage, kShare, kRow, kList };
+// kPack: chosen blocks whose size is a multiple of KT / 4: tiles run on over them, each wave's rows lie in one.
+enum TileMode { kPage, kShare, kRow, kList, kPack };
+
+// Quotients of numbers below 2^31 by one divisor: the reciprocal is rounded down, so a product is one too few at most.
+struct Divider {
+    uint32_t by, reciprocal;
+    __device__ __forceinline__ void init(uint32_t d) { by = d, reciprocal = 0xffffffffu / d; }
+    __device__ __forceinline__ int quotient(int x) const {
+        const uint32_t q = __umulhi(static_cast<uint32_t>(x), reciprocal);
+        return static_cast<int>(q + (static_cast<uint32_t>(x) - q * by >= by ? 1 : 0));
+    }
+};
 
 // The page of a walk's tile and the tile's first row there, for those who ask (pools in codes find the rows' scales by it).
 template <bool KEPT>
@@ -243,7 +254,7 @@ template <int KT, bool KEPT>
 struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
     const const_int *table, *entry;
     int unit, end, pages, blocks;   // tokens of a block, keys and blocks of the sequence
-    int per_page, magic;            // blocks of a page, and what finds a block's page
+    Divider per_page;               // blocks of a page
     int tiles;                      // of the item, the current one among them
     int entries;                    // of the list that are left to read
     int base, left;                 // current tile: first key, keys from it to the block's end
@@ -262,9 +273,8 @@ struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
         block1 = block2;
         page1 = -1;
         if (block1 >= 0 && block1 < blocks) {
-            int index = per_page == 1 ? block1 : static_cast<int>(__umulhi(static_cast<uint32_t>(block1), static_cast<uint32_t>(magic)));
-            if (index * per_page > block1) --index;  // (the reciprocal is rounded up)
-            off1 = (block1 - index * per_page) * unit;
+            const int index = per_page.quotient(block1);
+            off1 = (block1 - index * static_cast<int>(per_page.by)) * unit;
             page1 = table[index];
         }
         block2 = read();
@@ -290,8 +300,7 @@ struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
     __device__ __forceinline__ void begin(const rch_attend& A, const AttendItem& I, int es) {
         table = (const const_int*)(uintptr_t)(A.plan_ptr + 4 * static_cast<int64_t>(I.table));
         unit = static_cast<int>(A.block_tokens);
-        per_page = static_cast<int>(A.page_tokens) / unit;
-        magic = static_cast<int>(0xffffffffu / static_cast<uint32_t>(per_page) + 1);
+        per_page.init(static_cast<uint32_t>(A.page_tokens) / static_cast<uint32_t>(unit));
         end = I.length;
         blocks = (end + unit - 1) / unit;
         pages = static_cast<int>(A.pages);
@@ -328,6 +337,113 @@ struct KeyWalk<KT, kList, KEPT> : TilePlace<KEPT> {
     __device__ __forceinline__ int count() const { return min(end - base, min(left, KT)); }
 };
 
+// The walk over tiles that run on over chosen blocks.  A tile is four shares of KT / 4 rows, each of one block; a wave
+// fetches its own and knows the place of all, for the masks.  Entries are read two tiles ahead, their pages one.
+template <int KT, bool KEPT>
+struct KeyWalk<KT, kPack, KEPT> {
+    static constexpr int S = KT / 4;
+    const const_int *table, *list;
+    int unit, end, pages, blocks;
+    Divider per_block, per_page;  // keys of a block, blocks of a page
+    int wave, at, stop;           // the wave; keys of the list before the current tile, and before the end
+    int block[4], page[4];        // of the current tile's shares: entries and pages (-1: no key)
+    int ahead[4];                 // entries of the next tile
+    int64_t k_head, v_head, k_page, v_page;
+    int k_row, v_row;
+
+    __device__ __forceinline__ bool done() const { return at >= stop; }
+    __device__ __forceinline__ int offset(int s) const {
+        const int x = at + s * S;
+        return x - per_block.quotient(x) * unit;
+    }
+    __device__ __forceinline__ void read(int from) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int x = from + s * S;
+            ahead[s] = -1;
+            if (x < stop) ahead[s] = list[per_block.quotient(x)];
+        }
+    }
+    // The tile at `at` becomes the current one.
+    __device__ __forceinline__ void look_up() {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            block[s] = ahead[s] < blocks ? ahead[s] : -1;
+            page[s] = -1;
+            if (block[s] >= 0) page[s] = table[per_page.quotient(block[s])];
+        }
+        read(at + KT);
+    }
+    __device__ __forceinline__ void begin(const rch_attend& A, const AttendItem& I, int es) {
+        table = (const const_int*)(uintptr_t)(A.plan_ptr + 4 * static_cast<int64_t>(I.table));
+        list = (const const_int*)(uintptr_t)(A.lists_ptr + 4 * static_cast<int64_t>(I.list));
+        unit = static_cast<int>(A.block_tokens);
+        per_block.init(static_cast<uint32_t>(unit));
+        per_page.init(static_cast<uint32_t>(A.page_tokens) / static_cast<uint32_t>(unit));
+        end = I.length;
+        blocks = (end + unit - 1) / unit;
+        pages = static_cast<int>(A.pages);
+        k_head = A.k_ptr + es * I.kv_head * A.k_head_stride;
+        v_head = A.v_ptr + es * I.kv_head * A.v_head_stride;
+        k_page = es * A.k_page_stride;
+        v_page = es * A.v_page_stride;
+        k_row = static_cast<int>(es * A.k_token_stride);
+        v_row = static_cast<int>(es * A.v_token_stride);
+        at = __builtin_amdgcn_readfirstlane(I.key_begin * KT);
+        stop = __builtin_amdgcn_readfirstlane(min(I.key_end * KT, I.entries * unit));
+        read(at);
+        look_up();
+    }
+    __device__ __forceinline__ void next() {
+        at += KT;
+        look_up();
+    }
+    // First key and keys of share s of the current tile (0 keys: -1).
+    __device__ __forceinline__ int first_key(int s) const { return page[s] >= 0 && page[s] < pages ? block[s] * unit + offset(s) : -1; }
+    __device__ __forceinline__ int keys(int first) const { return first < 0 ? 0 : max(0, min(end - first, S)); }
+    // The wave's own share: its page (or -1), the first row there, and its keys.
+    __device__ __forceinline__ void own(int& id, int& in_page, int& rows) const {
+        int b = block[0], x = offset(0);
+        id = page[0];
+#pragma unroll
+        for (int s = 1; s < 4; ++s)
+            if (wave == s) b = block[s], id = page[s], x = offset(s);
+        if (id >= pages) id = -1;
+        rows = id < 0 ? 0 : keys(b * unit + x);
+        in_page = (b - per_page.quotient(max(b, 0)) * static_cast<int>(per_page.by)) * unit + x;
+    }
+};
+
+// What a wave's rows see of a tile of four shares whose first keys are `key` (-1: none).
+template <int S>
+struct ShareView {
+    bool sees, masked, hides;
+    template <typename Walk, typename Range>
+    __device__ __forceinline__ void look(const Walk& W, const Range& R, const int (&key)[4]) {
+        sees = masked = hides = false;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int n = W.keys(key[s]);
+            masked = masked || n < S;
+            sees = sees || (n > 0 && key[s] + n > R.first_low && key[s] < R.last_high);
+            hides = hides || (n > 0 && (key[s] < R.first_high || key[s] + n > R.last_low));
+        }
+        masked = masked || hides;
+    }
+    // Bits of the keys that one row sees.
+    template <typename Walk>
+    static __device__ __forceinline__ uint64_t bits(const Walk& W, const int (&key)[4], int first, int last) {
+        uint64_t all = 0;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int n = W.keys(key[s]), from = max(first - key[s], 0), to = min(last - key[s], n);
+            const uint32_t mask = to > from ? ((1u << to) - 1) & ~((1u << from) - 1) : 0;  // to <= 16
+            all |= static_cast<uint64_t>(mask) << (s * S);
+        }
+        return all;
+    }
+};
+
 // Fetches the calling wave's quarter of a K and a V tile: NI instructions of 1024 bytes each.  Tile: the
 // arithmetic's layout (ES: bytes of an element, RB: LDS bytes of a row, the swizzles).
 template <typename Tile, int MODE>
@@ -352,7 +468,7 @@ struct Fetch {
         if constexpr (MODE != kRow) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int row = row0 + i * kRows, from = MODE == kShare ? row - share : row;
+                const int row = row0 + i * kRows, from = MODE == kShare || MODE == kPack ? row - share : row;
                 const int kc = piece ^ Tile::k_swizzle(row), vc = piece ^ Tile::v_swizzle(row);
                 k_at[i] = kc < pieces ? from * k_row + kc * 16 : kOutOfRange;
                 v_at[i] = vc < pieces ? from * v_row + vc * 16 : kOutOfRange;
@@ -383,8 +499,18 @@ struct Fetch {
 
     __device__ __forceinline__ void issue(const rch_attend& A, const KeyWalk<KT, MODE>& W, uint32_t k_lds, uint32_t v_lds) const {
         if constexpr (MODE != kRow) {
-            int64_t k = W.k, v = W.v;
-            int rows = W.count();
+            int64_t k, v;
+            int rows;
+            if constexpr (MODE == kPack) {
+                k_lds = __builtin_amdgcn_readfirstlane(k_lds), v_lds = __builtin_amdgcn_readfirstlane(v_lds);  // (of wide heads, out of a vector register)
+                int id, in_page;
+                W.own(id, in_page, rows);
+                k = rows > 0 ? W.k_head + id * W.k_page + in_page * static_cast<int64_t>(k_row) : A.plan_ptr;
+                v = rows > 0 ? W.v_head + id * W.v_page + in_page * static_cast<int64_t>(v_row) : A.plan_ptr;
+            } else {
+                k = W.k, v = W.v;
+                rows = W.count();
+            }
             if constexpr (MODE == kShare) {
                 // Rows behind the last key, and those of a dropped page, are out of the buffer's range: zeros.
                 const int x = W.base % static_cast<int>(size) + share, in_page = x - page_of(x) * static_cast<int>(size);

@@ -4,25 +4,12 @@
 // run of queries is (sum of the run's query rows of a key head) . mean, also summed in FP64, so that the order of the sums
 // decides no choice between blocks (two scores of FP32 sums over 128 channels differ in their last places, and then a
 // block more or less is read).  FP64 costs nothing here: a mean is read once for every D products.
-#include "attend.h"
+#include "attend_tile.h"
 #include "codes.h"
 
 namespace rch {
 
 namespace {
-
-typedef __attribute__((address_space(4))) const int32_t const_int;
-
-// Quotients of numbers below 2^31 by one divisor, without a branch: the reciprocal is rounded down, so a product is one too
-// few at most.
-struct Divider {
-    uint32_t by, reciprocal;
-    __device__ __forceinline__ explicit Divider(uint32_t d) : by(d), reciprocal(0xffffffffu / d) {}
-    __device__ __forceinline__ int quotient(int x) const {
-        const uint32_t q = __umulhi(static_cast<uint32_t>(x), reciprocal);
-        return static_cast<int>(q + (static_cast<uint32_t>(x) - q * by >= by ? 1 : 0));
-    }
-};
 
 // V channels of a row of keys (8, in aligned pieces, or 1): fetched, so that several are in flight, then taken as FP64.
 template <int DT, int FMT, int V>
@@ -165,7 +152,8 @@ __device__ __forceinline__ void pool_queries(const rch_blocks& B, const Run& R, 
     constexpr int kAhead = 8;
     const int dim = static_cast<int>(B.head_dim), group = static_cast<int>(B.group), count = R.queries * group;
     const int lanes = dim / V, rows = 256 / lanes, mine = threadIdx.x / lanes, piece = threadIdx.x - mine * lanes;
-    const Divider by_group(group);
+    Divider by_group;
+    by_group.init(group);
     if (threadIdx.x < 256) {
         double sum[V];
 #pragma unroll
@@ -218,7 +206,8 @@ __device__ __forceinline__ void score_blocks(const rch_blocks& B, const Run& R, 
     typedef typename AttendType<DT>::type T;
     constexpr int kAhead = V == 1 ? 1 : 8;
     const int lane = threadIdx.x & 63, dim = static_cast<int>(B.head_dim);
-    const Divider by_page(static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(B.block_tokens));
+    Divider by_page;
+    by_page.init(static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(B.block_tokens));
     const int per = static_cast<int>(by_page.by);
     int width = 1;
     while (width * V < dim && width < 64) width *= 2;
@@ -312,7 +301,8 @@ __device__ __forceinline__ uint32_t joined(uint32_t x, Join join) {
 }
 template <int THREADS, typename Number>
 __device__ __forceinline__ void take_blocks(const rch_blocks& B, const Run& R, int head, Taking& L, Number number) {
-    const Divider by_page(static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(B.block_tokens));
+    Divider by_page;
+    by_page.init(static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(B.block_tokens));
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     auto chosen_by_score = [&](int block) { return block >= R.scored && block < R.scored_end && !(block >= R.kept && block < R.kept_end); };
 

@@ -114,8 +114,11 @@ class BlockPlan(AttentionPlan):
         heads = np.repeat(np.arange(cache.heads, dtype=np.int64), len(which))
         which, low, high = (np.tile(x, cache.heads) for x in (which, low, high))
         self._run_lists = (which * cache.heads + heads) * self.width
-        keys_of_tile = 32 if cache.dtype == torch.float32 or form == "single" else 64
-        tiles, merges = taken[which] * -(-size // keys_of_tile), []
+        tile = 32 if cache.dtype == torch.float32 or form == "single" else 64
+        # Tiles run on over blocks of whole quarters of a tile (the rows of a wave's loads) that are no whole tiles.
+        self._tile_unit = tile if form == "rows" and size % (tile // 4) == 0 and size % tile else size
+        tiles = taken[which] * -(-size // tile) if self._tile_unit == size else -(-taken[which] * size // tile)
+        self._run_taken, merges = taken[which], []
         items = np.empty((0, _lib.ATTEND_ITEM), np.int64)
         if len(which):
             items = self._cut(form, sequence[which], low, high, heads, tiles, lambda which, low, high, part, n: (low, high), merges)
@@ -123,7 +126,10 @@ class BlockPlan(AttentionPlan):
         self._runs_at = self._merges + self._n_merges * _lib.ATTEND_MERGE
 
     def _lists_of(self, which):
-        return self._run_lists[which]
+        return self._run_lists[which], self._run_taken[which]
+
+    def _unit(self):
+        return self._tile_unit
 
 
 class BlockIndex:

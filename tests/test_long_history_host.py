@@ -218,7 +218,7 @@ def _brute(length, queries, size, pages, page_tokens, first, recent, query_block
 def test_runs_and_items_of_a_plan(host, seed):
     """The ranges of every run against the rule stated key by key; every tile of every run's list in one part."""
     rng = np.random.default_rng(seed)
-    size = int(rng.choice([1, 2, 5, 16, 40]))
+    size = int(rng.choice([1, 2, 5, 16, 40, 48, 64]))
     page_tokens = size * int(rng.integers(1, 5))
     dtype = [torch.bfloat16, torch.float32][seed % 2]
     dim, heads, group = int(rng.choice([16, 20, 128, 64, 7])), int(rng.integers(1, 4)), int(rng.integers(1, 4))
@@ -258,15 +258,18 @@ def test_runs_and_items_of_a_plan(host, seed):
     assert at == plan.runs and widest == plan.width
     n_items = sum(plan._counts_of)
     items = words[plan._items:plan._items + n_items * _lib.ATTEND_ITEM].reshape(-1, _lib.ATTEND_ITEM)
-    per, seen = -(-size // (32 if dtype == torch.float32 else 64)), {}
-    for table, length, q_row, n, begin, end, head, low, high, part, at_list, _ in items.tolist():
+    tile, seen = 32 if dtype == torch.float32 else 64, {}
+    packed = plan._unit() != size
+    assert packed == (plan._counts_of[1] > 0 and size % (tile // 4) == 0 and size % tile != 0)
+    tiles_of = (lambda taken: -(-taken * size // tile)) if packed else (lambda taken: taken * -(-size // tile))
+    for table, length, q_row, n, begin, end, head, low, high, part, at_list, entries in items.tolist():
         if begin >= end:
             continue
         run, h = divmod(at_list // max(1, plan.width), heads) if plan.width else (None, head)
         if plan.width:
             number, start, count, taken = lists[run]
             assert h == head and at_list % plan.width == 0 and (q_row, n, length) == (starts[number], queries[number], lengths[number])
-            assert start * group <= begin < end <= (start + count) * group and 0 <= low <= high <= taken * per
+            assert start * group <= begin < end <= (start + count) * group and 0 <= low <= high <= tiles_of(taken) and entries == taken
         for row in range(begin, end):
             seen.setdefault((q_row, head, row), []).append((low, high, run))
     for run, (number, start, count, taken) in lists.items():
@@ -274,7 +277,7 @@ def test_runs_and_items_of_a_plan(host, seed):
             for row in range(start * group, (start + count) * group):
                 parts = sorted(seen.pop((starts[number], head, row)))
                 if plan.width:
-                    assert parts[0][0] == 0 and parts[-1][1] == taken * per and all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
+                    assert parts[0][0] == 0 and parts[-1][1] == tiles_of(taken) and all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
                     assert all(p[2] == run for p in parts)
     assert not seen
 
@@ -386,6 +389,7 @@ def test_abi_refusals():
                               ({"single": 1}, 2, ConfigurationError), ({"single": 1, "codes": 1}, 2, ConfigurationError),
                               ({"single": 1, "codes": 1, "n_general": 0, "n_rows": 1, "group": 33}, 2, ConfigurationError),
                               ({"lists_ptr": 64}, 2, ConfigurationError), ({"lists_ptr": 64, "block_tokens": 3}, 2, ConfigurationError),
+                              ({"lists_ptr": 64, "block_tokens": 2, "n_general": 0, "n_rows": 1, "tile_unit": 64}, 2, ConfigurationError),
                               ({"codes": 1, "n_general": 0, "n_rows": 1, "head_dim": 24, "tile_unit": 64}, 2, UnsupportedError)):
         with pytest.raises(error):
             _lib.call("rch_attend_run", words(_lib.ATTEND_FIELDS, **{**step, **bad}), dtype, None)
@@ -412,15 +416,19 @@ def test_the_plain_codes_are_the_nearest_ones(codes):
     assert lost[1].isnan().all() and not lost[0].float().any()
 
 
-def test_resources_of_listed_tiles_are_written_early_enough(tmp_path):
-    """As for the other tiles that are fetched straight into LDS."""
+@pytest.mark.parametrize("source", ["attend_lists.hip", "attend_int8.hip"])
+def test_resources_are_written_early_enough(source, tmp_path):
+    """As for the other tiles that are fetched straight into LDS; and the registers of a base address."""
     import subprocess
 
+    import test_kernel_code_host as machine
     from reelcache_amd.csrc import build as hip_build
-    from test_kernel_code_host import late_resources
 
     target = tmp_path / "kernels.s"
-    subprocess.run([hip_build._hipcc(), *hip_build.FLAGS, "-w", "--cuda-device-only", "-S", str(hip_build.HERE / "attend_lists.hip"), "-o",
+    subprocess.run([hip_build._hipcc(), *hip_build.FLAGS, "-w", "--cuda-device-only", "-S", str(hip_build.HERE / source), "-o",
                     str(target)], check=True, capture_output=True)
     text = target.read_text()
-    assert text.count("offen lds") > 50 and late_resources(text) == []
+    assert text.count("offen lds") > 50 and machine.late_resources(text) == []
+    if source != "attend_lists.hip":
+        based = re.sub(r"global_load_lds_dwordx4 (v\d+), (s\[\d+:\d+\])", r"buffer_load_dwordx4 \1, \2, 0 offen lds", text)
+        assert based.count("offen lds") > text.count("offen lds") + 50 and machine.late_resources(based) == []

@@ -155,7 +155,8 @@ def test_single_tokens(device, dtype, codes, size, block, heads, group, dim, lay
 @pytest.mark.parametrize("dtype,codes", KINDS)
 @pytest.mark.parametrize("block,window", [(None, None), (1, None), (50, None), (1, 90), (None, 70)])
 @pytest.mark.parametrize("size,length,heads,group,dim,query_block", [(64, 16, 1, 1, 64, 16), (64, 32, 1, 4, 128, 33), (60, 20, 2, 1, 80, 7),
-                                                                     (100, 100, 1, 1, 128, 150), (8, 4, 1, 2, 20, 10)])
+                                                                     (100, 100, 1, 1, 128, 150), (8, 4, 1, 2, 20, 10),
+                                                                     (96, 48, 1, 2, 96, 30)])
 def test_chunks(device, dtype, codes, block, window, size, length, heads, group, dim, query_block):
     """Chunks alone and behind histories, in runs shorter and longer than a block, and rows that see nothing."""
     lengths, queries = [70, 333, 260, 90, 3], [70, 129, 75, 1, 9 if block else 3]
