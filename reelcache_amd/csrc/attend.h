@@ -10,8 +10,10 @@ struct AttendItem {
     int table, length, q_row, queries, row_begin, row_end, kv_head, key_begin, key_end, part, list, entries;
 };
 
+typedef __attribute__((address_space(4))) const int32_t const_int;  // read by scalar loads
+
 __device__ __forceinline__ AttendItem attend_item(const rch_attend& A, int index) {
-    const RCH_GLOBAL int32_t* w = gin<int32_t>(A.plan_ptr) + A.items + static_cast<int64_t>(index) * RCH_ATTEND_ITEM;
+    const const_int* w = (const const_int*)(uintptr_t)(A.plan_ptr + 4 * (A.items + static_cast<int64_t>(index) * RCH_ATTEND_ITEM));
     return {w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7], w[8], w[9], w[10], w[11]};
 }
 

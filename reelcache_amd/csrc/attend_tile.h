@@ -23,7 +23,6 @@
 namespace rch {
 
 typedef __attribute__((address_space(3))) char lds_char;
-typedef __attribute__((address_space(4))) const int32_t const_int;
 
 template <int DT>
 struct Half;
@@ -401,13 +400,15 @@ struct KeyWalk<KT, kPack, KEPT> {
     // First key and keys of share s of the current tile (0 keys: -1).
     __device__ __forceinline__ int first_key(int s) const { return page[s] >= 0 && page[s] < pages ? block[s] * unit + offset(s) : -1; }
     __device__ __forceinline__ int keys(int first) const { return first < 0 ? 0 : max(0, min(end - first, S)); }
+    // (by values: a choice of places would put the four into memory)
+    __device__ __forceinline__ int own(const int (&x)[4]) const {
+        const int a = x[0], b = x[1], c = x[2], d = x[3], low = wave & 1 ? b : a, high = wave & 1 ? d : c;
+        return wave & 2 ? high : low;
+    }
     // The wave's own share: its page (or -1), the first row there, and its keys.
     __device__ __forceinline__ void own(int& id, int& in_page, int& rows) const {
-        int b = block[0], x = offset(0);
-        id = page[0];
-#pragma unroll
-        for (int s = 1; s < 4; ++s)
-            if (wave == s) b = block[s], id = page[s], x = offset(s);
+        const int b = own(block), x = offset(wave);
+        id = own(page);
         if (id >= pages) id = -1;
         rows = id < 0 ? 0 : keys(b * unit + x);
         in_page = (b - per_page.quotient(max(b, 0)) * static_cast<int>(per_page.by)) * unit + x;
