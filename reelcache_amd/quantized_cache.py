@@ -36,7 +36,8 @@ VALUE_DTYPES = (torch.bfloat16, torch.float16)
 
 _FORMATS = {torch.int8: _lib.CODES_INT8, torch.float8_e4m3fn: _lib.CODES_E4M3}
 _Image = ctypes.c_int64 * len(_lib.CODES_FIELDS)
-_AT = {name: _lib.CODES_FIELDS.index(name) for name in ("k_codes_ptr", "k_scales_ptr", "slots_ptr", "pairs_ptr", "rows_ptr")}
+_CODES_AT, _SCALES_AT, _SLOTS_AT, _PAIRS_AT, _ROWS_AT = (
+    _lib.CODES_FIELDS.index(name) for name in ("k_codes_ptr", "k_scales_ptr", "slots_ptr", "pairs_ptr", "rows_ptr"))
 
 
 class QuantizedCache(PagedCache):
@@ -65,6 +66,7 @@ class QuantizedCache(PagedCache):
         need(key_scales.data_ptr() != value_scales.data_ptr(), "keys and values need scales of their own")
         self.key_scales, self.value_scales, self.dtype = key_scales, value_scales, dtype
         self.codes = _FORMATS[keys.dtype]
+        self._scale_bytes = 4 * key_scales.stride(0), 4 * value_scales.stride(0)
         self._geometry += (dtype, key_scales.stride()[1:], value_scales.stride()[1:])
         for scales in (key_scales, value_scales):
             self._take_along(scales.unsqueeze(4), (1, 3, 2))
@@ -89,8 +91,8 @@ class QuantizedCache(PagedCache):
         return self.keys, self.values, self.key_scales, self.value_scales
 
     def _scales(self, layer):
-        return (self.key_scales.data_ptr() + 4 * layer * self.key_scales.stride(0),
-                self.value_scales.data_ptr() + 4 * layer * self.value_scales.stride(0))
+        k_bytes, v_bytes = self._scale_bytes
+        return self.key_scales.data_ptr() + layer * k_bytes, self.value_scales.data_ptr() + layer * v_bytes
 
     def _scale_strides(self):
         return tuple(scales.stride(axis) for scales in (self.key_scales, self.value_scales) for axis in (1, 2))
@@ -111,11 +113,11 @@ class QuantizedCache(PagedCache):
     def _addressed(self, image, layer, dense, slots):
         """A call's fields with its addresses, but those of the positions."""
         fields = _Image.from_buffer_copy(image)
-        at, (k_bytes, v_bytes) = _AT["k_codes_ptr"], self._layer_bytes
+        k_bytes, v_bytes = self._layer_bytes
         fields[0], fields[1] = dense
-        fields[at], fields[at + 1] = self.keys.data_ptr() + layer * k_bytes, self.values.data_ptr() + layer * v_bytes
-        fields[_AT["k_scales_ptr"]], fields[_AT["k_scales_ptr"] + 1] = self._scales(layer)
-        fields[_AT["slots_ptr"]] = slots
+        fields[_CODES_AT], fields[_CODES_AT + 1] = self.keys.data_ptr() + layer * k_bytes, self.values.data_ptr() + layer * v_bytes
+        fields[_SCALES_AT], fields[_SCALES_AT + 1] = self._scales(layer)
+        fields[_SLOTS_AT] = slots
         return fields
 
     def _store_launch(self, sources, positions, grid, tokens):
@@ -123,7 +125,7 @@ class QuantizedCache(PagedCache):
 
     def _launch_store(self, launch, layer, sources, pools, turned, slots, stream):
         fields = self._addressed(launch, layer, sources, slots)
-        fields[_AT["pairs_ptr"]], fields[_AT["rows_ptr"]] = turned
+        fields[_PAIRS_AT], fields[_ROWS_AT] = turned
         _lib.check(_lib.function("rch_codes_store")(fields, _DTYPE_CODES[self.dtype], stream))
 
     def read(self, layer, places, *, out=None):
@@ -152,7 +154,7 @@ class QuantizedCache(PagedCache):
             targets = [x if x.stride(2) == 1 or self.head_dim == 1 else torch.empty(shape, dtype=x.dtype, device=x.device)
                        for x in out]
             known = known_calls(places)
-            key = ("read", self._geometry, *[x.stride() for x in targets])
+            key = ("read", *[x.stride() for x in targets])
             image = known.get(key)
             if image is None:
                 image = known[key] = self._fields(targets, places.tokens)

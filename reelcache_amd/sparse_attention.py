@@ -180,15 +180,20 @@ class BlockIndex:
         need_gpu(cache.device, "a block index")
         if slots.tokens == 0:
             return
-        page, token, head = cache._axes
-        stride = cache.keys.stride()
-        key_scales, strides = cache._scales(layer)[0], cache._scale_strides()
         with entered(cache.device):
+            known = known_calls(slots)
+            key = ("update", self.block_tokens)
+            image = known.get(key)
+            if image is None:
+                page, token, head = cache._axes
+                stride, strides = cache.keys.stride(), cache._scale_strides()
+                image = known[key] = bytes(_fields(**self._sizes(), page_stride=stride[page], token_stride=stride[token],
+                                                   head_stride=stride[head], codes=cache.codes, scale_page_stride=strides[0],
+                                                   scale_head_stride=strides[1], tokens=slots.tokens))
+            fields = _Image.from_buffer_copy(image)
+            fields[0], fields[_AT["keys_ptr"]] = address, cache.keys.data_ptr() + layer * cache._layer_bytes[0]
+            fields[_AT["scales_ptr"]], fields[_AT["slots_ptr"]] = cache._scales(layer)[0], slots.index.data_ptr()
             stream = raw_stream(cache.device)
-            fields = _fields(means_ptr=address, **self._sizes(), keys_ptr=cache.keys.data_ptr() + layer * cache._layer_bytes[0],
-                             page_stride=stride[page], token_stride=stride[token], head_stride=stride[head], codes=cache.codes,
-                             scales_ptr=key_scales, scale_page_stride=strides[0], scale_head_stride=strides[1],
-                             slots_ptr=slots.index.data_ptr(), tokens=slots.tokens)
             _lib.check(_lib.function("rch_blocks_update")(fields, _DTYPE_CODES[cache.dtype], stream))
             if stream != slots.stream:  # the allocator learns of a stream that the index was not made on
                 slots.index.record_stream(torch.cuda.current_stream(cache.device))
