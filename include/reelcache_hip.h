@@ -714,6 +714,7 @@ typedef struct rch_blocks {
 
 #define RCH_BLOCKS_RUN 12
 #define RCH_BLOCKS_TOGETHER 4096
+#define RCH_BLOCKS_TOKENS (1 << 24) /* most tokens of a block */
 int rch_blocks_size(void);
 /* The means of the blocks that hold a slot: over all block_tokens rows, summed in FP64, rounded to FP32 and then to
  * the dtype. */

@@ -97,7 +97,8 @@ BLOCKS_FIELDS = ("means_ptr", "heads", "head_dim", "pages", "page_tokens", "bloc
                  "token_stride", "head_stride", "codes", "scales_ptr", "scale_page_stride", "scale_head_stride", "slots_ptr",
                  "tokens", "q_ptr", "q_token_stride", "q_head_stride", "group", "plan_ptr", "runs", "n_runs", "scores_ptr",
                  "scores", "lists_ptr", "width", "top")
-CODES_NONE, CODES_INT8, CODES_E4M3, CODES_MAX_DIM, BLOCKS_RUN, BLOCKS_TOGETHER = 0, 1, 2, 256, 12, 4096
+CODES_NONE, CODES_INT8, CODES_E4M3, CODES_MAX_DIM = 0, 1, 2, 256
+BLOCKS_RUN, BLOCKS_TOGETHER, BLOCKS_TOKENS = 12, 4096, 1 << 24
 
 _i, _i64, _p = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p
 _SIGNATURES = {

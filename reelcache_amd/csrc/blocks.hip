@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) blocks_update_kernel(const rch_blocks B, 
                     const int at = min(row + a * rows, size - 1);
                     float scale = 0.0f;
                     if constexpr (FMT != RCH_CODES_NONE) scale = gin<float>(scales)[at];
-                    x[a].fetch(keys + R::kBytes * at * B.token_stride, scale);
+                    x[a].fetch(keys + R::kBytes * (at * B.token_stride), scale);
                 }
                 all_issued();
 #pragma unroll
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(1024) blocks_take_kernel(const rch_blocks B) {
 int invalid(const rch_blocks& B, int dtype, const char* what) {
     if (dtype != RCH_DT_F32 && dtype != RCH_DT_F16 && dtype != RCH_DT_BF16) return fail(RCH_E_CONFIG, "%s: dtype must be f32, f16 or bf16", what);
     if (B.heads < 1 || B.heads > 65535 || B.head_dim < 1 || B.head_dim > RCH_ATTEND_MAX_DIM || B.pages < 1 || B.page_tokens < 1 || B.block_tokens < 1
-        || B.page_tokens % B.block_tokens || B.pages > 0x7fffffff || B.page_tokens > 0x7fffffff || B.pages * B.page_tokens > 0x7fffffff)
+        || B.block_tokens > RCH_BLOCKS_TOKENS || B.page_tokens % B.block_tokens || B.pages > 0x7fffffff || B.page_tokens > 0x7fffffff || B.pages * B.page_tokens > 0x7fffffff)
         return fail(RCH_E_CONFIG, "%s: invalid sizes", what);
     return RCH_OK;
 }

@@ -207,7 +207,7 @@ int invalid(const rch_codes& A, int dtype, const char* what) {
     if (dtype != RCH_DT_F16 && dtype != RCH_DT_BF16) return fail(RCH_E_UNSUPPORTED, "%s: codes stand for f16 or bf16 values", what);
     if (A.format != RCH_CODES_INT8 && A.format != RCH_CODES_E4M3) return fail(RCH_E_CONFIG, "%s: unknown format of codes", what);
     if (A.tokens < 0 || A.heads < 1 || A.head_dim < 1 || A.pages < 1 || A.page_tokens < 1 || A.tokens > 0x7fffffff
-        || A.heads > (1 << 18) || A.pages > 0x7fffffff || A.page_tokens > 0x7fffffff || A.pages * A.page_tokens > 0x7fffffff)
+        || A.heads > kHeads * 65535 || A.pages > 0x7fffffff || A.page_tokens > 0x7fffffff || A.pages * A.page_tokens > 0x7fffffff)
         return fail(RCH_E_CONFIG, "%s: invalid sizes", what);
     if (A.head_dim > RCH_CODES_MAX_DIM) return fail(RCH_E_UNSUPPORTED, "%s: heads of at most %d channels", what, RCH_CODES_MAX_DIM);
     if (A.pairs < 0 || 2 * A.pairs > A.head_dim
@@ -226,28 +226,32 @@ bool aligned(const rch_codes& A, int64_t piece) {
     return A.head_dim % piece == 0 && dense % 16 == 0 && codes % piece == 0;
 }
 
+// A grid of `units` threads (a launch has fewer than 2^32 along an axis).
+bool grid_of(const rch_codes& A, int64_t units, dim3* grid) {
+    *grid = dim3(static_cast<uint32_t>((units + 255) / 256), static_cast<uint32_t>((A.heads + kHeads - 1) / kHeads), 2);
+    return units <= 0xffffff00ll;
+}
+
 template <int DT, int FMT, int V, int L>
-void store(const rch_codes& A, dim3 grid, hipStream_t stream) {
-    grid.x = static_cast<uint32_t>((A.tokens + 256 / L - 1) / (256 / L));
+int store(const rch_codes& A, hipStream_t stream) {
+    dim3 grid;
+    if (!grid_of(A, A.tokens * L, &grid)) return fail(RCH_E_CONFIG, "rch_codes_store: too many tokens for one launch");
     hipLaunchKernelGGL((codes_store_kernel<DT, FMT, V, L>), grid, dim3(256), 0, stream, A);
+    return check_launch("rch_codes_store");
 }
 
 template <int DT, int FMT>
 int store_rows(const rch_codes& A, hipStream_t stream) {
-    const dim3 grid(1, static_cast<uint32_t>((A.heads + kHeads - 1) / kHeads), 2);
-    if (!aligned(A, 8)) store<DT, FMT, 4, 64>(A, grid, stream);
-    else if (A.head_dim <= 64) store<DT, FMT, 8, 8>(A, grid, stream);
-    else if (A.head_dim <= 128) store<DT, FMT, 8, 16>(A, grid, stream);
-    else store<DT, FMT, 8, 32>(A, grid, stream);
-    return check_launch("rch_codes_store");
+    if (!aligned(A, 8)) return store<DT, FMT, 4, 64>(A, stream);
+    if (A.head_dim <= 64) return store<DT, FMT, 8, 8>(A, stream);
+    return A.head_dim <= 128 ? store<DT, FMT, 8, 16>(A, stream) : store<DT, FMT, 8, 32>(A, stream);
 }
 
 template <int DT, int FMT>
 int read_rows(const rch_codes& A, hipStream_t stream) {
     const bool wide = aligned(A, 16);
-    const int64_t units = A.tokens * (wide ? A.head_dim / 16 : A.head_dim), blocks = (units + 255) / 256;
-    if (blocks > 0x7fffffff) return fail(RCH_E_CONFIG, "rch_codes_read: grid too large");
-    const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>((A.heads + kHeads - 1) / kHeads), 2);
+    dim3 grid;
+    if (!grid_of(A, A.tokens * (wide ? A.head_dim / 16 : A.head_dim), &grid)) return fail(RCH_E_CONFIG, "rch_codes_read: too many tokens for one launch");
     if (wide) hipLaunchKernelGGL((codes_read_kernel<DT, FMT, 16>), grid, dim3(256), 0, stream, A);
     else hipLaunchKernelGGL((codes_read_kernel<DT, FMT, 1>), grid, dim3(256), 0, stream, A);
     return check_launch("rch_codes_read");

@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 import heapq
 import struct
+import weakref
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -174,9 +175,7 @@ class PagedCache:
         self._moved = 0   # counts what may move or reuse pages: plans and slots built before it are stale
         self._shared = 0  # counts what may share pages: slots built before it are stale
         self._copies = None
-        # What moves along with the pages, as pools [layers, pages, rows or heads, .., width]: (tensor, (page, row, head) axes,
-        # tokens of a row).
-        self._along = []
+        self._along = []  # what moves along with the pages
 
     @classmethod
     def allocate(cls, pages, page_tokens, heads, head_dim, *, layers=1, dtype=torch.bfloat16, device="cuda", layout="BTHD"):
@@ -417,29 +416,30 @@ class PagedCache:
         """Copies pages in every pool: ``moves`` is flat, (source, destination, leading rows) of each."""
         if not moves:
             return
+        along = [(each, pool) for each in self._along if (pool := each.pool()) is not None]
+        self._along = [each for each, _ in along]
         with entered(self.device):
-            where = self.keys.data_ptr(), self.values.data_ptr()
-            if self._copies is None or self._copies[0] != where:  # a copied cache has pools of its own
+            # A copied cache has pools of its own, and others may have come or gone.
+            where = self.keys.data_ptr(), self.values.data_ptr(), *[(each, pool.data_ptr()) for each, pool in along]
+            if self._copies is None or self._copies[0] != where:
                 self._copies = where, [(1, *_pools(pool, self._axes, self.pages, self.page_tokens))
                                        for pool in self._joined_pools()]
-                self._copies[1].extend((tokens, *_pools((pool,), axes, self.pages, pool.shape[axes[1]]))
-                                       for pool, axes, tokens in self._along)
-            table, stream = _pack(moves), raw_stream(self.device)
+                self._copies[1].extend((each.tokens, *_pools((pool,), each.axes, self.pages, pool.shape[each.axes[1]]))
+                                       for each, pool in along)
+            stream, tables = raw_stream(self.device), {}
             for tokens, pools, fields, streams in self._copies[1]:
-                if tokens > 1:  # a row stands for several tokens: the begun one too
-                    table = _pack([-(-word // tokens) if i % 3 == 2 else word for i, word in enumerate(moves)])
+                if tokens not in tables:  # a row may stand for several tokens: the begun one moves too
+                    tables[tokens] = _pack([-(-word // tokens) if i % 3 == 2 else word for i, word in enumerate(moves)])
                 if stream not in streams:  # the allocator learns of a stream that the table was not made on
                     pools.record_stream(torch.cuda.current_stream(self.device))
                     streams.add(stream)
-                _lib.check(_lib.function("rch_pages_copy")(fields, table, len(moves) // 3, stream))
-            torch.autograd.graph.increment_version(self._counted)
+                _lib.check(_lib.function("rch_pages_copy")(fields, tables[tokens], len(moves) // 3, stream))
+            torch.autograd.graph.increment_version((*self._counted, *[pool for _, pool in along if not pool.is_inference()]))
 
     def _take_along(self, pool, axes, tokens=1):
-        """Page copies move a further pool from now on."""
-        self._along.append((pool, axes, tokens))
-        self._copies = None
-        if not pool.is_inference():
-            self._counted += (pool,)
+        """Page copies move a further pool ``[layers, pages, rows or heads, .., width]`` from now on, for as long as it lives:
+        ``axes`` as of the cache's pools, ``tokens`` of a row."""
+        self._along.append(_Along(pool, axes, tokens))
 
     def _joined_pools(self):
         """K and V pools as one group where their strides agree (one launch), else as two."""
@@ -658,6 +658,21 @@ class PagedCache:
         from .sparse_attention import BlockIndex
 
         return BlockIndex.allocate(self, block_tokens)
+
+
+class _Along:
+    """A further pool that moves with the pages: its owner keeps it, not the cache."""
+
+    def __init__(self, pool, axes, tokens):
+        self.pool = weakref.ref(pool) if pool is not None else _gone
+        self.axes, self.tokens = axes, tokens
+
+    def __reduce__(self):  # copies are of the pool's copy
+        return _Along, (self.pool(), self.axes, self.tokens)
+
+
+def _gone():
+    return None
 
 
 def _apart(pool):

@@ -27,7 +27,7 @@ import torch
 from . import _lib
 from ._checks import count, in_memory, need, one_of
 from .errors import ConfigurationError, UnsupportedError
-from .paged_cache import _LAYOUTS, PagedCache, _apart
+from .paged_cache import _LAYOUTS, PagedCache, _apart, _reach
 from .rotary import _DTYPE_CODES, _span, changed, entered, known_calls, need_gpu, position_fields, raw_stream
 
 #: Types of the pools, and of the values that their codes stand for.
@@ -66,10 +66,13 @@ class QuantizedCache(PagedCache):
         need(key_scales.data_ptr() != value_scales.data_ptr(), "keys and values need scales of their own")
         self.key_scales, self.value_scales, self.dtype = key_scales, value_scales, dtype
         self.codes = _FORMATS[keys.dtype]
+        self._scale_reach = _reach(key_scales), _reach(value_scales)
         self._scale_bytes = 4 * key_scales.stride(0), 4 * value_scales.stride(0)
         self._geometry += (dtype, key_scales.stride()[1:], value_scales.stride()[1:])
-        for scales in (key_scales, value_scales):
-            self._take_along(scales.unsqueeze(4), (1, 3, 2))
+        self._counted += tuple(scales for scales in (key_scales, value_scales) if not scales.is_inference())
+        self._moving = tuple(scales.unsqueeze(4) for scales in (key_scales, value_scales))  # as pools of one channel
+        for scales in self._moving:
+            self._take_along(scales, (1, 3, 2))
 
     @classmethod
     def allocate(cls, pages, page_tokens, heads, head_dim, *, codes=torch.int8, layers=1, dtype=torch.bfloat16, device="cuda",
@@ -121,10 +124,14 @@ class QuantizedCache(PagedCache):
         return fields
 
     def _store_launch(self, sources, positions, grid, tokens):
-        return self._fields(sources, tokens, position_fields(positions, grid, tokens, 1, self.head_dim, self.device))
+        return tuple(map(_reach, sources)), self._fields(sources, tokens, position_fields(positions, grid, tokens, 1, self.head_dim, self.device))
 
     def _launch_store(self, launch, layer, sources, pools, turned, slots, stream):
-        fields = self._addressed(launch, layer, sources, slots)
+        reach, image = launch
+        for scales, room in ((self.key_scales.data_ptr(), self._scale_reach[0]), (self.value_scales.data_ptr(), self._scale_reach[1])):
+            if any([x < scales + room and scales < x + n for x, n in zip(sources, reach)]):
+                raise ConfigurationError("what a store reads overlaps the scales that it writes")
+        fields = self._addressed(image, layer, sources, slots)
         fields[_PAIRS_AT], fields[_ROWS_AT] = turned
         _lib.check(_lib.function("rch_codes_store")(fields, _DTYPE_CODES[self.dtype], stream))
 

@@ -43,7 +43,7 @@ class BlockPlan(AttentionPlan):
     :meth:`BlockIndex.plan`, used by :meth:`BlockIndex.select` and :meth:`BlockIndex.attend` in every layer; stale once pages
     moved, and to be built after the step's ``extend``, as every plan.
 
-    ``runs``: their number.  ``width``: blocks of the run that takes most.
+    ``runs``: their number.  ``counts``: blocks that each takes (of every key head).  ``width``: the most of them.
     """
 
     def __init__(self, index, sequences, queries, *, heads, top, query_block=1, first=1, recent=1, block=None, window=None,
@@ -95,7 +95,7 @@ class BlockPlan(AttentionPlan):
         taken = np.concatenate(counts) if counts else np.zeros(0, np.int64)
         fields, sequence, begin, end = (np.concatenate(x) for x in zip(*runs)) if runs else (np.zeros((0, _lib.BLOCKS_RUN), np.int64),
                                                                                             *[taken] * 3)
-        self.runs, self.width = len(taken), int(taken.max(initial=0))
+        self.runs, self.counts, self.width = len(taken), taken.tolist(), int(taken.max(initial=0))
         self._scores = int((fields[:, 6] - fields[:, 5]).max(initial=0)) if self.top else 0
         # Blocks are scored by workgroups of their own, in a launch before the choice, where one to a run would not fill the
         # card (or its LDS).
@@ -149,6 +149,8 @@ class BlockIndex:
              "means must be [layers, pages, blocks of a page, heads, head_dim] of the cache's dtype and device, blocks dividing a page")
         need(means.is_contiguous(), "means must be contiguous")
         need(not means.requires_grad, "means must not require gradients")
+        if cache.page_tokens // blocks > _lib.BLOCKS_TOKENS:
+            raise UnsupportedError(f"a block has at most {_lib.BLOCKS_TOKENS} tokens")
         if cache.head_dim > _lib.ATTEND_MAX_DIM:
             raise UnsupportedError(f"an index takes at most {_lib.ATTEND_MAX_DIM} channels to a head")
         self.cache, self.means, self.block_tokens = cache, means, cache.page_tokens // blocks
@@ -255,8 +257,8 @@ class BlockIndex:
         """Attention of ``q`` over the chosen blocks of one layer.
 
         ``blocks``: what :meth:`select` gave for this plan, or a choice of the caller's own of the same shape and type
-        (contiguous; the same block twice counts twice; a number that is no block of the sequence, or in a dropped page, has
-        no keys); without it, ``q`` and the layer's means choose.  The masks hold within the blocks.  ``q``, ``out``,
+        (contiguous; of a run's ``width`` numbers the first ``plan.counts[run]`` are read; the same block twice counts twice; a
+        number that is no block of the sequence, or in a dropped page, has no keys); without it, ``q`` and the layer's means choose.  The masks hold within the blocks.  ``q``, ``out``,
         ``return_lse`` and the result as in :func:`reelcache_amd.attention.attend`.
         """
         self._layer(layer)

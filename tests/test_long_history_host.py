@@ -6,6 +6,7 @@ import ctypes
 import math
 import pickle
 import re
+import weakref
 from pathlib import Path
 
 import numpy as np
@@ -187,7 +188,7 @@ def test_copied_and_pickled_caches(host):
     slots = cache.extend([a], [6])
     cache.read(0, slots)
     other, moved = copy.deepcopy((cache, index))
-    assert moved.cache is other and moved.means is other._along[-1][0] and moved.means is not index.means
+    assert moved.cache is other and moved.means is other._along[-1].pool() and moved.means is not index.means
     assert pickle.loads(pickle.dumps(slots)).tokens == 6
 
 
@@ -328,7 +329,7 @@ def test_refused_indexes_and_plans(host):
 def test_page_copies_take_the_scales_and_means_along(host, monkeypatch):
     """The launches of a copy: the codes, the scales and the means, with rows of tokens, tokens and blocks."""
     cache = quantised(size=8, layers=3)
-    cache.index(4)
+    index = cache.index(4)
     a = cache.new()
     cache.extend([a], [13])
     b = cache.fork(a)
@@ -339,6 +340,71 @@ def test_page_copies_take_the_scales_and_means_along(host, monkeypatch):
     assert [table for _, table in copies] == [[1, 2, 5], [1, 2, 5], [1, 2, 5], [1, 2, 2]]
     assert [f["pools"] for f in fields] == [6, 3, 3, 3]
     assert [(f["page_rows"], f["segments"], f["row_bytes"]) for f in fields] == [(8, 1, 32), (8, 2, 4), (8, 2, 4), (2, 1, 64)]
+    assert index.means._version == 1  # a saved one notices
+
+
+def _copied(host, cache, sequence):
+    """(table, rows of a page) of the launches of a fork's copy of its begun page."""
+    b = cache.fork(sequence)
+    host.clear()
+    cache.extend([b], [1])
+    found = [(np.frombuffer(arguments[1], dtype=np.int32).tolist()[2], dict(zip(_lib.PAGES_FIELDS, arguments[0]))["page_rows"])
+             for name, arguments in host if name == "rch_pages_copy"]
+    cache.free(b)
+    return found
+
+
+@pytest.mark.parametrize("sizes", [(4, 1, 2), (1, 4, 8)])
+def test_indexes_of_several_block_sizes_move_by_rows_of_their_own(host, sizes):
+    cache = native(size=8)
+    indexes = [cache.index(n) for n in sizes]
+    a = cache.new()
+    cache.extend([a], [13])
+    assert _copied(host, cache, a) == [(5, 8), *[(-(-5 // n), 8 // n) for n in sizes]]
+    assert len(indexes) == len(cache._along)
+
+
+def test_the_cache_keeps_no_index_that_its_owner_dropped(host):
+    cache = quantised(size=8)
+    a = cache.new()
+    cache.extend([a], [13])
+    kept, dropped = cache.index(4), cache.index(2)
+    assert len(_copied(host, cache, a)) == 5
+    means = weakref.ref(dropped.means)
+    del dropped
+    assert means() is None
+    assert _copied(host, cache, a) == [(5, 8), (5, 8), (5, 8), (2, 2)] and kept.means is cache._along[-1].pool()
+    other = copy.deepcopy(cache)  # without its index
+    assert _copied(host, other, a) == [(5, 8)] * 3
+    assert other._moving[0].data_ptr() == other.key_scales.data_ptr() != cache.key_scales.data_ptr()
+
+
+def test_stores_refuse_what_overlaps_the_scales(host):
+    cache = quantised(pages=64, size=4, heads=2, dim=16)
+    slots = cache.extend([cache.new()], [2])
+    dense = torch.zeros(2, 2, 16, dtype=torch.bfloat16)
+    for scales in (cache.key_scales, cache.value_scales):
+        over = scales.view(torch.bfloat16).flatten()[:64].view(2, 2, 16)
+        for k, v in ((over, dense), (dense, over)):
+            with pytest.raises(ConfigurationError, match="scales"):
+                cache.store(1, slots, k, v)
+    cache.store(1, slots, dense, dense)
+
+
+def test_plans_count_the_blocks_that_each_run_takes(host):
+    cache = native(pages=16, size=8)
+    a, b = cache.new(), cache.new()
+    cache.extend([a, b], [80, 20])
+    plan = cache.index(8).plan([a, b], [1, 1], heads=2, top=3)
+    assert (plan.runs, plan.counts, plan.width) == (2, [5, 3], 5)
+
+
+def test_blocks_of_too_many_tokens_are_refused(host):
+    pools = [torch.empty((1, 1, 1 << 25, 1, 1), dtype=torch.bfloat16) for _ in range(2)]
+    cache = paged_cache.PagedCache(*pools)
+    with pytest.raises(UnsupportedError, match="tokens"):
+        cache.index(1 << 25)
+    cache.index(1 << 24)
 
 
 def test_header_matches_the_binding():
@@ -349,6 +415,7 @@ def test_header_matches_the_binding():
     defines = {name: int(value) for name, value in re.findall(r"#define (RCH_[A-Z0-9_]+) (\d+)\b", HEADER.read_text())}
     expected = {"RCH_CODES_NONE": _lib.CODES_NONE, "RCH_CODES_INT8": _lib.CODES_INT8, "RCH_CODES_E4M3": _lib.CODES_E4M3,
                 "RCH_CODES_MAX_DIM": _lib.CODES_MAX_DIM, "RCH_BLOCKS_RUN": _lib.BLOCKS_RUN, "RCH_BLOCKS_TOGETHER": _lib.BLOCKS_TOGETHER}
+    assert "#define RCH_BLOCKS_TOKENS (1 << 24)" in HEADER.read_text() and _lib.BLOCKS_TOKENS == 1 << 24
     assert {name: defines.get(name) for name in expected} == expected
     lib = _lib.library()
     assert lib.rch_codes_size() == 8 * len(_lib.CODES_FIELDS) and lib.rch_blocks_size() == 8 * len(_lib.BLOCKS_FIELDS)

@@ -295,6 +295,62 @@ def test_means_move_with_the_pages(device, dtype, codes):
             assert torch.equal(fresh.means[0, page, j % 4], index.means[0, page, j % 4]), (sequence, j)
 
 
+@pytest.mark.parametrize("sizes", [(16, 1, 4), (1, 32)])
+def test_indexes_of_several_sizes_move_with_the_pages(device, sizes):
+    """A fork's begun page moves in each index by its own rows."""
+    cache = _cache(device, [100], 32, 2, 64, torch.bfloat16)
+    cache.keys.nan_to_num_(0.0)
+    indexes = [_index(cache, n, [100]) for n in sizes]
+    spare = sparse_attention.BlockIndex.allocate(cache, 8)
+    del spare  # moves no more
+    child = cache.fork(0)
+    cache.extend([child], [1])
+    source, target = cache.pages_of(0)[3], cache.pages_of(child)[3]
+    for n, index in zip(sizes, indexes):
+        rows = -(-4 // n)
+        assert source != target and torch.equal(index.means[0, target, :rows], index.means[0, source, :rows])
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+@pytest.mark.parametrize("size,block,dim,query_block", [(1, 1, 64, 1), (2, 1, 80, 5), (16, 1, 128, 64), (3, 3, 20, 2)])
+def test_smallest_pages_and_blocks(device, dtype, codes, size, block, dim, query_block):
+    lengths, queries = [70, 1, 9], [6, 1, 9]
+    cache = _cache(device, lengths, size, 2, dim, dtype, codes)
+    index = _index(cache, block, lengths)
+    q = _queries(queries, 4, dim, dtype, device)
+    _check(cache, index, lengths, queries, q, top=9, query_block=query_block, block=1)
+    _check(cache, index, lengths, [1, 1, 1], q[:3], top=40, first=0, recent=3, window=50)
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+def test_a_run_of_steps(device, dtype, codes):
+    """As a server uses them: a prompt over a history, then single tokens of it and of a fork: stored, their blocks' means
+    brought up to date, and attended to, with one index, while pages are copied and moved."""
+    size, block, heads, group, dim = 32, 16, 2, 4, 128
+    cache = _cache(device, [200, 90], size, heads, dim, dtype, codes)
+    index = _index(cache, block, [200, 90])
+    g = torch.Generator().manual_seed(31)
+
+    def step(counts):
+        sequences = list(range(len(counts)))
+        slots = cache.extend(sequences, counts)
+        n = sum(counts)
+        k, v = (torch.randn((n, heads, dim), generator=g).to(dtype).to(device) for _ in range(2))
+        cache.store(0, slots, k, v)
+        index.update(0, slots)
+        q = torch.randn((n, heads * group, dim), generator=g).to(dtype).to(device)
+        lengths = [cache.tokens(s) for s in sequences]
+        _check(cache, index, lengths, counts, q, top=3, query_block=16, recent=2, block=1)
+
+    step([20, 1])
+    cache.fork(0)  # sequence 2 shares the history
+    for _ in range(3):
+        step([1, 1, 1])
+    step([0, 1, 1])
+    cache.compact()
+    step([1, 1, 15])
+
+
 def test_outputs_strides_and_other_rows(device):
     """``out`` with rows behind the plan's, queries of other orders, an empty plan."""
     dtype = torch.bfloat16
