@@ -74,7 +74,8 @@ __global__ void __launch_bounds__(256) blocks_update_kernel(const rch_blocks B, 
     const int lanes = dim / V, rows = 256 / lanes;  // threads of a row, rows at once
     const int mine = threadIdx.x / lanes, piece = threadIdx.x - mine * lanes, lane = threadIdx.x & 63;
     const RCH_GLOBAL int32_t* slots = gin<int32_t>(B.slots_ptr);
-    const int64_t limit = B.pages * B.page_tokens, per = B.page_tokens / size;
+    const int64_t limit = B.pages * B.page_tokens;
+    const uint32_t per = static_cast<uint32_t>(B.page_tokens) / static_cast<uint32_t>(size);
     // Every wave finds the workgroup's blocks, a lane to a token.
     const int64_t token = static_cast<int64_t>(blockIdx.x) * share + lane;
     const bool there = lane < share && token < B.tokens;
@@ -83,9 +84,9 @@ __global__ void __launch_bounds__(256) blocks_update_kernel(const rch_blocks B, 
     const int number = held ? slot / size : -1;
     uint64_t ends = __ballot(held && !(next >= 0 && next < limit && next / size == number));
     while (ends) {
-        const int64_t block = __shfl(number, __builtin_ctzll(ends));
+        const uint32_t found = __shfl(number, __builtin_ctzll(ends)), page_found = found / per;
         ends &= ends - 1;
-        const int64_t page = block / per, row0 = (block - page * per) * size;
+        const int64_t block = found, page = page_found, row0 = static_cast<int64_t>(found - page_found * per) * size;
         const int64_t keys = B.keys_ptr + R::kBytes * (page * B.page_stride + row0 * B.token_stride + head * B.head_stride + piece * V);
         const int64_t scales = FMT == RCH_CODES_NONE ? 0 : B.scales_ptr + 4 * (page * B.scale_page_stride + head * B.scale_head_stride + row0);
         double sum[V];
