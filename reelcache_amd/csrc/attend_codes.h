@@ -120,11 +120,11 @@ struct CodeFetch {
         }
     }
 
-    // 16 codes' values: two pieces of eight.
-    static __device__ __forceinline__ void put(lds_char* row, int first, int swizzle, u4 codes, float scale) {
+    // 16 codes' values: two pieces of eight, at `place` and `apart` from there.
+    static __device__ __forceinline__ void put(lds_char* row, int place, int apart, u4 codes, float scale) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
-            *reinterpret_cast<__attribute__((address_space(3))) vec8*>(row + ((first + half) ^ swizzle) * 16) =
+            *reinterpret_cast<__attribute__((address_space(3))) vec8*>(row + (half ? place ^ apart : place) * 16) =
                 code_values<DT, FMT>(codes[2 * half], codes[2 * half + 1], scale);
     }
     // Writes the values of the codes that have landed at `raw`.
@@ -142,8 +142,8 @@ struct CodeFetch {
             const int row = row0 + i * kRows;
             // (codes behind the last row are 0, their scales another row's)
             const bool none = MODE != kRow && row - (kShares ? share : 0) >= count;
-            put(k_tile + row * RB, 2 * piece, Tile::k_swizzle(row), k[i], none ? 0.0f : k_scale[i]);
-            put(v_tile + row * RB, 2 * piece, Tile::v_swizzle(row), v[i], none ? 0.0f : v_scale[i]);
+            put(k_tile + row * RB, Tile::k_place(2 * piece) ^ Tile::k_swizzle(row), Tile::k_place(1), k[i], none ? 0.0f : k_scale[i]);
+            put(v_tile + row * RB, Tile::v_place(2 * piece) ^ Tile::v_swizzle(row), Tile::v_place(1), v[i], none ? 0.0f : v_scale[i]);
         }
     }
 };

@@ -10,7 +10,7 @@ namespace rch {
 template <int DT, int NB, int MODE, int FMT>
 __global__ void __launch_bounds__(256, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_rows_kernel(const rch_attend A) {
     constexpr bool kCodes = FMT != RCH_CODES_NONE;
-    typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2, kCodes && NB != 3 && NB != 6> Tile;
+    typedef RowTile<DT, NB, DT == RCH_DT_F32 ? 1 : 2, kCodes && NB != 3 && NB != 6, kCodes> Tile;
     constexpr int KT = Tile::KT, ES = Tile::ES, kTileBytes = KT * Tile::RB;
     constexpr int kStageBytes = 2 * kTileBytes;
     typedef typename std::conditional_t<kCodes, std::common_type<CodeFetch<DT == RCH_DT_F32 ? RCH_DT_BF16 : DT, Tile, MODE, kCodes ? FMT : RCH_CODES_INT8>>,

@@ -597,16 +597,27 @@ __device__ __forceinline__ void add_marks(f16v& sum, const f16v& code) {
     }
 }
 
-// One wave's state over the tiles and the arithmetic of a tile of KB * 32 keys.  LEAN: with fewer registers.
-template <int DT, int NB, int KB, bool LEAN = false>
+// One wave's state over the tiles and the arithmetic of a tile of KB * 32 keys.  LEAN: with fewer registers.  PAIRS: a tile
+// that lanes write two neighbouring pieces of eight channels to (CodeFetch), in two stores.  Eight lanes store 128 bytes at a
+// time, so that every other piece of a row would meet each bank twice: a piece's low bit goes where eight lanes' bits do not
+// (a chunk's kernel spent 66 cycles of LDS on such meetings for a wave's tile, beside 98 of its own).
+template <int DT, int NB, int KB, bool LEAN = false, bool PAIRS = false>
 struct RowTile {
     typedef Half<DT> H;
     typedef typename H::type T;
     typedef typename H::vec8 vec8;
     typedef typename H::vec4 vec4;
     static constexpr int ES = 2, RB = NB <= 2 ? 128 : NB <= 4 ? 256 : 512, kPieces = RB / 16, KT = 32 * KB;
+    static constexpr bool kApart = PAIRS && RB > 128;
     static __device__ __forceinline__ int k_swizzle(int row) { return row % kPieces; }
-    static __device__ __forceinline__ int v_swizzle(int row) { return kPieces >= 16 ? (row & 3) * 4 : ((row >> 1) & 1) * 4; }
+    static __device__ __forceinline__ int v_swizzle(int row) {
+        if constexpr (kApart) return (row & 1) | (row & 2) << 1;
+        if constexpr (PAIRS) return ((row >> 1) & 1) * 4 | (row & 1);
+        return kPieces >= 16 ? (row & 3) * 4 : ((row >> 1) & 1) * 4;
+    }
+    // Where a row's pieces lie, before the exchange of its swizzle (bits change places: sums of bits stay sums).
+    static __device__ __forceinline__ constexpr int k_place(int piece) { return kApart ? piece >> 1 | (piece & 1) * (kPieces / 2) : piece; }
+    static __device__ __forceinline__ constexpr int v_place(int piece) { return kApart ? (piece & ~9) | (piece & 1) << 3 | (piece >> 3 & 1) : piece; }
 
     vec8 q[2 * NB];
     f16v o[NB];
@@ -615,8 +626,8 @@ struct RowTile {
     // LDS byte offsets within a tile; of wide heads the first, from which the others follow by an exclusive or.
     static constexpr bool kWide = NB > 4 || LEAN;
     uint32_t k_lane[kWide ? 1 : 2 * NB], v_lane[kWide ? 1 : NB];
-    __device__ __forceinline__ uint32_t k_at(int s) const { return kWide ? k_lane[0] ^ (s * 32) : k_lane[s]; }
-    __device__ __forceinline__ uint32_t v_at(int b) const { return kWide ? v_lane[0] ^ (b * 64) : v_lane[b]; }
+    __device__ __forceinline__ uint32_t k_at(int s) const { return kWide ? k_lane[0] ^ (k_place(2 * s) * 16) : k_lane[s]; }
+    __device__ __forceinline__ uint32_t v_at(int b) const { return kWide ? v_lane[0] ^ (v_place(4 * b) * 16) : v_lane[b]; }
 
     __device__ __forceinline__ void init(const rch_attend& A, const AttendItem& I, const QueryRow& R, int lane) {
         const int n = lane & 31, h = lane >> 5;
@@ -625,7 +636,7 @@ struct RowTile {
         for (int s = 0; s < 2 * NB; ++s) {
             const int d = 16 * s + 8 * h;
             q[s] = __builtin_bit_cast(vec8, *gin<u4>(R.valid && d < A.head_dim ? at + 2 * d : A.plan_ptr));  // or zeros
-            if (!kWide || s == 0) k_lane[s] = n * RB + (((2 * s + h) ^ k_swizzle(n)) * 16);
+            if (!kWide || s == 0) k_lane[s] = n * RB + ((k_place(2 * s + h) ^ k_swizzle(n)) * 16);
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -779,7 +790,7 @@ struct RowTile {
     // keys 16 c .. 16 c + 15 from there.
     static __device__ __forceinline__ uint32_t value_offset(int b, int lane) {
         const int p = lane & 15, key = 4 * (lane >> 5) + (p >> 2), half = (lane >> 4) & 1;
-        const int piece = (4 * b + 2 * half + ((p & 3) >> 1)) ^ v_swizzle(key);
+        const int piece = v_place(4 * b + 2 * half + ((p & 3) >> 1)) ^ v_swizzle(key);
         return key * RB + piece * 16 + (p & 1) * 8;
     }
     static __device__ __forceinline__ vec8 values(const lds_char* at, int c) {
@@ -805,7 +816,7 @@ struct RowTile {
 // 16-byte piece of K (and of Q) feeds four products, and register i of S^T is, as it is, the B operand of the
 // keys that registers i of both halves hold; V^T is read one value a lane.
 template <int NB>
-struct RowTile<RCH_DT_F32, NB, 1, false> {
+struct RowTile<RCH_DT_F32, NB, 1, false, false> {
     typedef float T;
     static constexpr int ES = 4, RB = NB <= 2 ? 256 : NB <= 4 ? 512 : 1024, kPieces = RB / 16, KT = 32;
     static __device__ __forceinline__ int k_swizzle(int row) { return row % kPieces; }
