@@ -34,6 +34,7 @@ GENERAL_ROWS, ROW_TILE = 16, 128
 _ROWS = {"general": GENERAL_ROWS, "rows": ROW_TILE, "single": _lib.ATTEND_SINGLE_ROWS}
 # What a workgroup's start, end and partial results cost in key tiles, per form (tiled: a step of six sequences of
 # 211 to 5003 tokens takes 58.0 us at 0, 55.4 at 3, 54.8 at 6 and 55.0 at 8; others do not change by more than 2 %).
+# Single tokens over codes: 75.4 us at 2 and 73.9-74.7 at 0 to 6 for four long sequences, 48.4 at 2 and 48.2-51.0 for 64 of up to 4000.
 _OVERHEAD = {"general": 1, "rows": 6, "single": 2}
 _CUS = 256
 # At most this many rows are joined a workgroup to a row, whatever their parts, in one launch (512 rows of 4 parts take
@@ -146,7 +147,8 @@ class AttentionPlan:
         return "rows"
 
     def _form_of(self, tokens):
-        """The form of row blocks of at most ``tokens`` query tokens: :meth:`_form`, or "single" for single tokens over codes."""
+        """The form of row blocks of at most ``tokens`` query tokens: :meth:`_form`, or "single" for single tokens over codes (8
+        of up to 1000 keys take 13.7 us so and 15.4 in rows, 64 of up to 4000 48 and 69, 4 of up to 65536 75 and 99)."""
         form = self._form()
         if form == "rows" and self.cache.codes and tokens <= 1 and self.group <= _lib.ATTEND_SINGLE_ROWS:
             return "single"
@@ -229,7 +231,7 @@ class AttentionPlan:
         if form == "general":
             return _CUS * 4
         dim = self.cache.head_dim  # its tiles fill LDS and registers
-        if form == "single":
+        if form == "single":  # its LDS; 4 long sequences take 99.7 / 76.8 / 75.4 / 91.6 us at 4 / 6 / 8 / 10, 128 channels
             return _CUS * (12 if dim <= 64 else 8 if dim <= 128 else 4)
         return _CUS * (3 if dim <= 64 else 2 if dim <= 128 else 1)
 

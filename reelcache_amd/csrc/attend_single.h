@@ -9,6 +9,10 @@
 // 8-bit values gives a lane eight keys of its channel, in the order that the weights' registers hold them.
 // All rows see the same keys: a key that they do not see gets no weight, and its codes and scale are zeroed in LDS, so that
 // it may be anything; the tile's loads may repeat a valid row where there is none.
+//
+// Measured: 4 tokens of 32 query heads over 20000 to 65536 keys of 8 heads of 128 channels in int8, 65 us at 5.2 TB/s (a large
+// copy reaches 4.8, reads alone 5.4), and 11 of the join; the row tiles of attend_rows.h took 94 in all, since 128 rows of
+// which 4 are there convert every value in full for them.
 #pragma once
 
 #include "attend_tile.h"

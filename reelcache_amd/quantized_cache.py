@@ -12,7 +12,7 @@ Formats, for the largest magnitude ``m`` of a token's head:
 * ``torch.int8``: scale ``max(m / 127, 2**-126)``, codes ``rint(x / scale)`` in -127 .. 127 (off by half a step of m / 127);
 * ``torch.float8_e4m3fn``: scale ``2**e``, the least that holds ``m <= 448 * scale``, codes ``x / scale`` rounded to nearest
   even (off by ``2**-4`` of each value: better for rows with few large channels, and cheaper to read); within +-240 where
-  256 times the scale is more than the cache's ``dtype`` holds.
+  256 times the scale is more than the cache's ``dtype`` holds.  Of a scale that a caller wrote, the power of two counts.
 
 A code ``c`` stands for ``c * scale``, rounded to the cache's ``dtype``.  A token's head that holds an infinity or a NaN
 stands for NaN in all its channels.
