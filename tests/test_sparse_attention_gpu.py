@@ -426,3 +426,39 @@ def test_streams_and_captured_replays(device):
             graphs[1].replay() if side is sides[0] else index.attend(0, q, plan)
     torch.cuda.synchronize(device)
     assert all(torch.equal(a, b) for a, b in zip(outs[1], want))
+
+
+@pytest.mark.parametrize("dtype,codes", [(torch.bfloat16, None), (torch.bfloat16, torch.int8), (torch.float16, torch.float8_e4m3fn)])
+@pytest.mark.parametrize("size,block,dim,layout", [(1024, 32, 16, "BTHD"), (64, 2, 128, "BHTD"), (50, 25, 104, "BTHD")])
+def test_pools_past_32_bits(device, dtype, codes, size, block, dim, layout):
+    """Pages, scales and means that lie more than 2^32 bytes into their pools: the bits of the same sequence in a small
+    cache, stored, read, indexed, chosen and attended to."""
+    heads, n, queries = 2, 6 * size - 7, 130
+    near = (1 << 30) // (size * heads) if dim == 16 else (1 << 32) // (size * heads * dim)  # (of 16 channels the scales lie as far)
+    results = []
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn((n, heads, dim), generator=g).to(dtype).to(device) for _ in range(2))
+    q = torch.randn((queries, 2 * heads, dim), generator=g).to(dtype).to(device)
+    for pages in (9, near + 9):
+        rows = (size, heads) if layout == "BTHD" else (heads, size)
+        if codes is None:
+            cache = paged_cache.PagedCache(*(torch.empty((1, pages, *rows, dim), dtype=dtype, device=device) for _ in range(2)), layout=layout)
+        else:
+            cache = quantized_cache.QuantizedCache.allocate(pages, size, heads, dim, codes=codes, dtype=dtype, device=device, layout=layout)
+        cache.load_tables([([pages - 1 - i for i in range(6)], n)])
+        slots = cache.slots([0], [0], [n])
+        cache.store(0, slots, k, v)
+        index = cache.index(block)
+        index.update(0, slots)
+        found = [*cache.read(0, slots)] if codes is not None else []
+        for count in (queries, 1):
+            plan = index.plan([0], [count], heads=2 * heads, top=5, query_block=16, block=1)
+            blocks = index.select(0, q[:count], plan)
+            found += [blocks, index.attend(0, q[:count], plan, blocks=blocks),
+                      cache.attend(0, q[:count], cache.plan([0], [count], heads=2 * heads, block=1))]
+        results.append([x.cpu() for x in found])
+        far = max(pool[0, pages - 6:].data_ptr() - pool.data_ptr() for pool in (cache.keys, *([] if codes is None else [cache.key_scales])))
+        assert (far > 1 << 32) == (pages > 9)
+        del cache, index, slots, plan
+    for small, large in zip(*results):
+        assert not small.isnan().any() and torch.equal(small, large)
