@@ -37,7 +37,8 @@ _MOST_SCORED = 65535 * 128  # blocks of a run: one workgroup scores 128
 # 8 among 500 32.9 / 34.4, 4 among 125 27.2 / 23.7, 16 among 500 43.5 / 43.8, 39 runs of 12 heads among 270 150.9 / 139.9).
 _FEW_SCORED, _FEW_RUNS = 256, 128
 _Image = ctypes.c_int64 * len(_lib.BLOCKS_FIELDS)
-_AT = {name: index for index, name in enumerate(_lib.BLOCKS_FIELDS)}
+_KEYS_AT, _SCALES_AT, _SLOTS_AT, _Q_AT, _PLAN_AT, _SCORES_AT, _LISTS_AT = (
+    _lib.BLOCKS_FIELDS.index(name) for name in ("keys_ptr", "scales_ptr", "slots_ptr", "q_ptr", "plan_ptr", "scores_ptr", "lists_ptr"))
 
 
 class BlockPlan(AttentionPlan):
@@ -195,8 +196,8 @@ class BlockIndex:
                                                    head_stride=stride[head], codes=cache.codes, scale_page_stride=strides[0],
                                                    scale_head_stride=strides[1], tokens=slots.tokens))
             fields = _Image.from_buffer_copy(image)
-            fields[0], fields[_AT["keys_ptr"]] = address, cache.keys.data_ptr() + layer * cache._layer_bytes[0]
-            fields[_AT["scales_ptr"]], fields[_AT["slots_ptr"]] = cache._scales(layer)[0], slots.index.data_ptr()
+            fields[0], fields[_KEYS_AT] = address, cache.keys.data_ptr() + layer * cache._layer_bytes[0]
+            fields[_SCALES_AT], fields[_SLOTS_AT] = cache._scales(layer)[0], slots.index.data_ptr()
             stream = raw_stream(cache.device)
             _lib.check(_lib.function("rch_blocks_update")(fields, _DTYPE_CODES[cache.dtype], stream))
             if stream != slots.stream:  # the allocator learns of a stream that the index was not made on
@@ -211,9 +212,12 @@ class BlockIndex:
         return BlockPlan(self, sequences, queries, heads=heads, top=top, query_block=query_block, first=first, recent=recent,
                          block=block, window=window, scale=scale)
 
+    def _planned(self, plan):
+        need(isinstance(plan, BlockPlan) and plan.index is self, "a BlockPlan of this index is needed")
+
     def _check(self, q, plan):
         cache = self.cache
-        need(isinstance(plan, BlockPlan) and plan.index is self, "a BlockPlan of this index is needed")
+        self._planned(plan)
         if plan._stamp != cache._moved:
             raise StateError("pages moved or were freed after this plan was built")
         in_memory(q, "q")
@@ -246,9 +250,9 @@ class BlockIndex:
                 scores = None
                 if plan._apart:
                     scores = torch.empty(plan.runs * cache.heads * plan._scores, dtype=torch.int64, device=cache.device)
-                    fields[_AT["scores_ptr"]] = scores.data_ptr()
-                fields[0], fields[_AT["q_ptr"]], fields[_AT["plan_ptr"]] = address, q.data_ptr(), plan.buffer.data_ptr()
-                fields[_AT["lists_ptr"]] = blocks.data_ptr()
+                    fields[_SCORES_AT] = scores.data_ptr()
+                fields[0], fields[_Q_AT], fields[_PLAN_AT] = address, q.data_ptr(), plan.buffer.data_ptr()
+                fields[_LISTS_AT] = blocks.data_ptr()
                 stream = raw_stream(cache.device)
                 if stream != plan._stream:  # the allocator learns of a stream that the tables were not made on
                     plan.buffer.record_stream(torch.cuda.current_stream(cache.device))
@@ -263,12 +267,12 @@ class BlockIndex:
         number that is no block of the sequence, or in a dropped page, has no keys); without it, ``q`` and the layer's means choose.  The masks hold within the blocks.  ``q``, ``out``,
         ``return_lse`` and the result as in :func:`reelcache_amd.attention.attend`.
         """
-        self._layer(layer)
-        self._check(q, plan)
         cache = self.cache
         if blocks is None:
             blocks = self.select(layer, q, plan)
         else:
+            self._layer(layer)
+            self._planned(plan)
             in_memory(blocks, "blocks")
             need(blocks.shape == (plan.runs, cache.heads, plan.width) and blocks.dtype == torch.int32
                  and blocks.device == cache.device and blocks.is_contiguous(),
