@@ -35,7 +35,9 @@ _ROWS = {"general": GENERAL_ROWS, "rows": ROW_TILE, "single": _lib.ATTEND_SINGLE
 # What a workgroup's start, end and partial results cost in key tiles, per form (tiled: a step of six sequences of
 # 211 to 5003 tokens takes 58.0 us at 0, 55.4 at 3, 54.8 at 6 and 55.0 at 8; others do not change by more than 2 %).
 # Single tokens over codes: 75.4 us at 2 and 73.9-74.7 at 0 to 6 for four long sequences, 48.4 at 2 and 48.2-51.0 for 64 of up to 4000.
-_OVERHEAD = {"general": 1, "rows": 6, "single": 2}
+# Chosen blocks ("lists"): prompts over 32 blocks of 32 keys take 76.6 / 76.2 / 75.3 / 75.3 / 77.8 us at 0 / 2 / 3 / 4 / 6, a chunk
+# over 26 of 120 148.7 / 136.1 / 136.3 / 136.4 / 136.7.  Dense steps over codes do not agree (69-84 us, up to 5 % either way).
+_OVERHEAD = {"general": 1, "rows": 6, "lists": 3, "single": 2}
 _CUS = 256
 # At most this many rows are joined a workgroup to a row, whatever their parts, in one launch (512 rows of 4 parts take
 # 4.1 us so, 4.1-5.1 us with a thread per eight channels; a second launch costs 5 us).
@@ -263,8 +265,10 @@ class AttentionPlan:
     def _cut(self, form, sequence, begin, end, head, tiles, keys, merges):
         """Items of row blocks (arrays, one entry to a block) of ``tiles`` key tiles; ``keys`` gives the key range of
         parts ``(block, first tile, last tile, part, parts)``."""
-        owner = sequence * self.cache.heads + head
-        which, low, high, xcd = _share_out(tiles, owner, self._resident(form), _OVERHEAD[form]).T
+        cache = self.cache
+        start = _OVERHEAD["lists" if form == "rows" and self._block_tokens else form]
+        owner = sequence * cache.heads + head
+        which, low, high, xcd = _share_out(tiles, owner, self._resident(form), start).T
         parts = np.bincount(which, minlength=len(tiles))
         part = np.arange(len(which)) - np.repeat(np.cumsum(parts) - parts, parts)
         n = parts[which]

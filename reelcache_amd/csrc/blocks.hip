@@ -451,6 +451,7 @@ __global__ void __launch_bounds__(256) blocks_score_kernel(const rch_blocks B) {
     score_blocks<DT, V, 256>(B, R, head, begin, end, pooled, [&](int block, uint64_t number) { out[block] = number; });
 }
 
+// (1024 threads to a choice among up to 1024 blocks for 4 single tokens: 30.0 us with its score and attention, 512 30.1, 256 32.3)
 __global__ void __launch_bounds__(1024) blocks_take_kernel(const rch_blocks B) {
     __shared__ uint64_t kept[kTogether];
     __shared__ Taking L;
