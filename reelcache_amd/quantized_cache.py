@@ -127,9 +127,10 @@ class QuantizedCache(PagedCache):
         return tuple(map(_reach, sources)), self._fields(sources, tokens, position_fields(positions, grid, tokens, 1, self.head_dim, self.device))
 
     def _launch_store(self, launch, layer, sources, pools, turned, slots, stream):
-        reach, image = launch
-        for scales, room in ((self.key_scales.data_ptr(), self._scale_reach[0]), (self.value_scales.data_ptr(), self._scale_reach[1])):
-            if any([x < scales + room and scales < x + n for x, n in zip(sources, reach)]):
+        (k_reach, v_reach), image = launch
+        k, v = sources
+        for scales, room in zip((self.key_scales.data_ptr(), self.value_scales.data_ptr()), self._scale_reach):
+            if (k < scales + room and scales < k + k_reach) or (v < scales + room and scales < v + v_reach):
                 raise ConfigurationError("what a store reads overlaps the scales that it writes")
         fields = self._addressed(image, layer, sources, slots)
         fields[_PAIRS_AT], fields[_ROWS_AT] = turned
@@ -146,35 +147,37 @@ class QuantizedCache(PagedCache):
             raise ConfigurationError("there is no such layer")
         self._current(places)
         shape = (places.tokens, self.heads, self.head_dim)
-        if out is None:
-            need_gpu(self.device, "a paged cache")
-            with entered(self.device):
-                out = tuple([torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2)])
-            given = False
-        else:
-            out, given = tuple(out), True
+        given = out is not None
+        if given:
+            out = tuple(out)
             self._check_out(out, shape)
-            need_gpu(self.device, "a paged cache")
-        if places.tokens == 0:
-            return out
+        need_gpu(self.device, "a paged cache")
         with entered(self.device):
-            targets = [x if x.stride(2) == 1 or self.head_dim == 1 else torch.empty(shape, dtype=x.dtype, device=x.device)
-                       for x in out]
+            if given:
+                targets = [x if x.stride(2) == 1 or self.head_dim == 1 else torch.empty(shape, dtype=x.dtype, device=x.device)
+                           for x in out]
+            else:
+                targets = out = (torch.empty(shape, dtype=self.dtype, device=self.device),
+                                 torch.empty(shape, dtype=self.dtype, device=self.device))
+            if places.tokens == 0:
+                return out
+            keys, values = targets
             known = known_calls(places)
-            key = ("read", *[x.stride() for x in targets])
+            key = ("read", keys.stride(), values.stride())
             image = known.get(key)
             if image is None:
                 image = known[key] = self._fields(targets, places.tokens)
             stream = raw_stream(self.device)
-            fields = self._addressed(image, layer, [x.data_ptr() for x in targets], places.index.data_ptr())
+            fields = self._addressed(image, layer, (keys.data_ptr(), values.data_ptr()), places.index.data_ptr())
             _lib.check(_lib.function("rch_codes_read")(fields, _DTYPE_CODES[self.dtype], stream))
             if stream != places.stream:  # the allocator learns of a stream that the index was not made on
                 places.index.record_stream(torch.cuda.current_stream(self.device))
-            for x, target in zip(out, targets):
-                if target is not x:
-                    x.copy_(target)
-                elif given:
-                    changed(x)
+            if given:
+                for x, target in zip(out, targets):
+                    if target is not x:
+                        x.copy_(target)
+                    else:
+                        changed(x)
         return out
 
     def _check_out(self, out, shape):
