@@ -53,9 +53,14 @@ class Slots(Remembering):
     stream: int
 
 
+@dataclass(eq=False)
 class Places(Slots):
     """The rows that tokens lie in, for reading them: built by :meth:`PagedCache.places`.  Their pages may be shared; no
-    store takes them."""
+    store takes them.  Stale once pages moved or were freed, and once a sequence of theirs goes on in a copy of its begun
+    page (:meth:`PagedCache.extend`): the rows are another sequence's then."""
+
+    pieces: tuple = field(default=(), repr=False)  # (sequence, its first page of theirs, the pages) of each
+    copied: int = 0  # begun pages that the cache had copied when they last were the sequences'
 
 
 @dataclass(frozen=True, eq=False)
@@ -174,6 +179,7 @@ class PagedCache:
         self._free = list(range(self.pages))
         self._moved = 0   # counts what may move or reuse pages: plans and slots built before it are stale
         self._shared = 0  # counts what may share pages: slots built before it are stale
+        self._copied = 0  # counts begun pages copied: places built before it may be another sequence's
         self._copies = None
         self._along = []  # what moves along with the pages
 
@@ -314,6 +320,7 @@ class PagedCache:
                     moves += (pages[-1], page, begun)
                     pages[-1] = page
                     self._shared += 1
+                    self._copied += 1
                 for _ in range(more):
                     page = heapq.heappop(free)
                     in_use[page] = 1
@@ -342,7 +349,13 @@ class PagedCache:
     def places(self, sequences, starts, counts):
         """The :class:`Places` of tokens ``starts[i] .. starts[i] + counts[i]`` that ``sequences[i]`` has, to read them.
         Their pages may be shared."""
-        return self._slots(*self._stretches(sequences, starts, counts, "places", True), Places)
+        found, starts, counts = self._stretches(sequences, starts, counts, "places", True)
+        made = self._slots(found, starts, counts, Places)
+        size = self.page_tokens
+        made.pieces = tuple((item, start // size, tuple(item.pages[start // size:-(-(start + n) // size)]))
+                            for item, start, n in zip(found, starts, counts) if n)
+        made.copied = self._copied
+        return made
 
     def _stretches(self, sequences, starts, counts, what, shared):
         """Checked (sequences, starts, counts) of tokens that lie in pages."""
@@ -400,8 +413,17 @@ class PagedCache:
         """Refuses slots and places of other caches, and those that pages have moved behind."""
         if not isinstance(slots, Slots) or slots.cache is not self:
             raise ConfigurationError("slots come from this cache")
-        if slots.stamp != (self._moved if isinstance(slots, Places) else self._moved + self._shared):
-            raise StateError("pages moved, were freed or became shared after these slots were built")
+        if not isinstance(slots, Places):
+            if slots.stamp != self._moved + self._shared:
+                raise StateError("pages moved, were freed or became shared after these slots were built")
+            return
+        if slots.stamp != self._moved:
+            raise StateError("pages moved or were freed after these places were built")
+        if slots.copied != self._copied:
+            # Sequences went on in copies of their begun pages: these ones, or others.
+            if any(tuple(item.pages[first:first + len(pages)]) != pages for item, first, pages in slots.pieces):
+                raise StateError("a begun page was copied after these places were built")
+            slots.copied = self._copied
 
     # -----------------------------------------------------------------------------------------
     # Page copies

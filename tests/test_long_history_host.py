@@ -172,6 +172,94 @@ def test_places_may_be_shared_and_slots_may_not(host):
     assert cache.places([a], [4], [2]).index.tolist() == [4, 5]
 
 
+@pytest.mark.parametrize("who", ["quantised", "native"])
+def test_places_are_stale_once_their_page_was_copied(host, who):
+    """The sequence of the places goes on in a copy of its begun page: the old one is another sequence's, which may write
+    it."""
+    cache = quantised(size=8) if who == "quantised" else native(size=8)
+    index = cache.index(4)
+    a = cache.new()
+    cache.extend([a], [13])
+    b = cache.fork(a)
+    begun, whole = cache.places([a], [8], [5]), cache.places([a, b], [0, 0], [8, 8])
+    other = cache.places([b], [8], [5])
+    host.clear()
+    for places in (begun, whole, other):  # a fork alone moves no rows
+        index.update(0, places)
+    cache.extend([a], [1])
+    assert cache.pages_of(a) == [0, 2] and cache.pages_of(b) == [0, 1]
+    assert cache.slots([b], [8], [5]).index.tolist() == begun.index.tolist()  # b may write these rows now
+    calls = len(host)
+    with pytest.raises(StateError):
+        index.update(0, begun)
+    if who == "quantised":
+        with pytest.raises(StateError):
+            cache.read(0, begun)
+    assert len(host) == calls  # nothing was launched
+    for places in (whole, other):  # where the rows stayed, so does what stands for them
+        for _ in range(2):
+            index.update(0, places)
+            if who == "quantised":
+                cache.read(0, places)
+    assert cache.places([a], [8], [6]).index.tolist() == [16, 17, 18, 19, 20, 21]
+
+
+def test_places_of_several_sequences_are_checked_each(host):
+    cache = quantised(size=8)
+    a, c = cache.new(), cache.new()
+    cache.extend([a, c], [13, 5])
+    b = cache.fork(a)
+    mixed = cache.places([c, a], [0, 3], [5, 10])
+    cache.read(0, mixed)
+    cache.extend([b], [1])  # b goes on elsewhere; a keeps its rows
+    cache.read(0, mixed)
+    d = cache.fork(a)
+    cache.extend([a, d], [1, 1])
+    for _ in range(2):
+        with pytest.raises(StateError):
+            cache.read(0, mixed)
+    cache.read(0, cache.places([c, a], [0, 3], [5, 10]))
+
+
+def test_places_stay_when_an_extension_fails(host, monkeypatch):
+    """A copy that could not be launched changes nothing."""
+    cache = quantised(size=8)
+    a = cache.new()
+    cache.extend([a], [13])
+    cache.fork(a)
+    places = cache.places([a], [8], [5])
+    working = _lib.function
+
+    def failing(name):
+        if name == "rch_pages_copy":
+            return lambda *arguments: _lib.E_LAUNCH
+        return working(name)
+
+    monkeypatch.setattr(_lib, "function", failing)
+    with pytest.raises(Exception):
+        cache.extend([a], [1])
+    monkeypatch.setattr(_lib, "function", working)
+    cache.read(0, places)
+
+
+def test_copied_places_follow_the_copied_cache(host):
+    cache = quantised(size=8)
+    a = cache.new()
+    cache.extend([a], [13])
+    cache.fork(a)
+    places = cache.places([a], [8], [5])
+    other, moved = copy.deepcopy((cache, places))
+    other.extend([a], [1])
+    with pytest.raises(StateError):
+        other.read(0, moved)
+    cache.read(0, places)
+    alone = pickle.loads(pickle.dumps(places))
+    alone.cache.read(0, alone)
+    alone.cache.extend([a], [1])
+    with pytest.raises(StateError):
+        alone.cache.read(0, alone)
+
+
 def test_plans_of_codes_take_the_matrix_cores_where_rows_are_whole_pieces(host):
     for dim, tiled in ((16, True), (24, False), (128, True), (104, False), (7, False)):
         cache = quantised(dim=dim)
