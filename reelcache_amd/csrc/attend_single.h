@@ -192,7 +192,23 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
         typedef __attribute__((address_space(3))) u4 lds_u4;
         lds_float* const scales = (lds_float*)(k_tile + 2 * KT * RB);
         if (shown == 0) continue;
-        if constexpr (FMT == RCH_CODES_E4M3) scales[lane] = code_scale<FMT>(scales[lane]);
+        // 8-bit floats in bf16: the values' scales, powers of two, go to the weights, whose rounding stays what it is while the
+        // products are far from bf16's subnormals and its end (a weight of 2^-17 and a scale of 2^-115 would keep two bits).
+        // Scales below 2^-64 and above 2^64 go there by what they differ from 2^-95 and 2^95, in products of their own whose
+        // values take the rest: no product is below 2^-64 of its weight, or more than 2^64 of it.  fp16 does not hold such
+        // weights, and integers times other scales are rounded as values.
+        constexpr bool kScaled = DT == RCH_DT_BF16 && FMT == RCH_CODES_E4M3;
+        float own = 0.0f;
+        uint64_t small = 0, large = 0;  // keys of such scales (bits of the lanes that fetched them)
+        if constexpr (FMT == RCH_CODES_E4M3) {
+            own = code_scale<FMT>(scales[lane]);
+            if constexpr (kScaled) {
+                const bool counts = of_values && (shown >> n & 1u);
+                small = __ballot(counts && own < 0x1p-64f);
+                large = __ballot(counts && own > 0x1p64f);
+            }
+            scales[lane] = (small | large) >> lane & 1u ? 0.0f : own;
+        }
         if (shown != ~0u) {
 #pragma unroll
             for (int i = 0; i < NI; ++i)
@@ -225,9 +241,6 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[b][i] *= fade;
         }
-        // 8-bit floats in bf16: the scales, powers of two, go to the weights (whose rounding stays what it is).  fp16 does not
-        // hold such weights, and integers times other scales are rounded as values.
-        constexpr bool kScaled = DT == RCH_DT_BF16 && FMT == RCH_CODES_E4M3;
         f4 v_scale[4];  // of the keys of registers 4 i ..
 #pragma unroll
         for (int i = 0; i < 4; ++i) v_scale[i] = *(lds_f4*)(scales + 32 + 8 * i + 4 * h);
@@ -238,18 +251,36 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
             const float x = exp2_of(__builtin_fmaf(s[0][i], scale, -reference.value));
             part[i & 3] += x;
             w[i >> 3][i & 7] = static_cast<T>(kScaled ? x * v_scale[i >> 2][i & 3] : x);
+            if constexpr (kScaled) s[0][i] = x;
         }
         sum += (part[0] + part[1]) + (part[2] + part[3]);
+        auto add_values = [&](float unit) {  // unit: what the values' own scale is, where the weights take the rest of it
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                typedef int i2 __attribute__((ext_vector_type(2)));
-                typedef __attribute__((address_space(3))) i2 lds_i2;
-                const i2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(v_tile + v_lane + half * 16 * RB + (v_turn ^ (b * 32))));
-                const uint32_t low = static_cast<uint32_t>(codes[0]), high = static_cast<uint32_t>(codes[1]);
-                if constexpr (kScaled) o[b] = H::mfma(code_values<DT, FMT>(low, high), w[half], o[b]);
-                else o[b] = H::mfma(code_values<DT, FMT>(low, high, v_scale[2 * half], v_scale[2 * half + 1]), w[half], o[b]);
+                for (int b = 0; b < NB; ++b) {
+                    typedef int i2 __attribute__((ext_vector_type(2)));
+                    typedef __attribute__((address_space(3))) i2 lds_i2;
+                    const i2 codes = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)(v_tile + v_lane + half * 16 * RB + (v_turn ^ (b * 32))));
+                    const uint32_t low = static_cast<uint32_t>(codes[0]), high = static_cast<uint32_t>(codes[1]);
+                    if constexpr (kScaled) o[b] = H::mfma(code_values<DT, FMT>(low, high, unit), w[half], o[b]);
+                    else o[b] = H::mfma(code_values<DT, FMT>(low, high, v_scale[2 * half], v_scale[2 * half + 1]), w[half], o[b]);
+                }
+            }
+        };
+        add_values(1.0f);
+        if constexpr (kScaled) {
+            while (__builtin_expect((small | large) != 0, 0)) {
+                const uint64_t these = small ? small : large;
+                const float unit = small ? 0x1p-95f : 0x1p95f, rest = small ? 0x1p95f : 0x1p-95f;
+                if (small) small = 0;
+                else large = 0;
+                scales[lane] = these >> lane & 1u ? own * rest : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v_scale[i] = *(lds_f4*)(scales + 32 + 8 * i + 4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[i >> 3][i & 7] = static_cast<T>(s[0][i] * v_scale[i >> 2][i & 3]);
+                add_values(unit);
             }
         }
     }

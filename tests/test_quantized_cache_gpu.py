@@ -384,3 +384,25 @@ def test_refusals_on_the_device(device):
         cache.plan([0], [1], heads=2)._check(cache.keys[0], cache.values[0])
     before = [t.clone() for t in cache.read(0, places)]
     assert all(torch.equal(a, b) for a, b in zip(cache.read(0, places, out=tuple(out)), before))
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("exponent", [-108, -104, -90, -60, 60, 110])
+@pytest.mark.parametrize("group", [2, 33])
+def test_small_weights_of_small_and_large_values(device, codes, exponent, group):
+    """Values far from 1, and a key of value 0 that takes nearly all of the weight: what the others add is of their weights'
+    precision, about 2^-17 of the largest, whatever their scales (group 2: the form of single tokens)."""
+    dtype, dim, size, lengths = torch.bfloat16, 64, 16, [300, 70]
+    cache = _empty(device, 30, size, 1, dim, codes, dtype)
+    cache.load_tables([(list(range(19)), 300), ([25, 20, 28, 22, 21], 70)])
+    g = torch.Generator().manual_seed(4)
+    k, v = (torch.randn((sum(lengths), 1, dim), generator=g) for _ in range(2))
+    v *= 2.0 ** exponent
+    for at in (7, 300 + 40):
+        k[at], v[at] = 12.0, 0.0
+    cache.store(0, cache.slots([0, 1], [0, 0], lengths), *(x.to(dtype).to(device) for x in (k, v)))
+    q = torch.full((2, group, dim), 0.125) + 0.01 * torch.randn((2, group, dim), generator=g)
+    q = q.to(dtype).to(device)
+    assert cache.plan([0], [1], heads=group)._single == (group == 2)
+    out = _check(cache, lengths, [1, 1], q)
+    assert (out != 0).any(dim=2).all()
