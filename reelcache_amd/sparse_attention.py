@@ -36,9 +36,14 @@ _MOST_SCORED = 65535 * 128  # blocks of a run: one workgroup scores 128
 # _FEW_RUNS workgroups else (choice and attention, apart / together: 4 tokens of 8 key heads among 1000 blocks 29.7 / 38.9 us,
 # 8 among 500 32.9 / 34.4, 4 among 125 27.2 / 23.7, 16 among 500 43.5 / 43.8, 39 runs of 12 heads among 270 150.9 / 139.9).
 _FEW_SCORED, _FEW_RUNS = 256, 128
+# Bytes of the numbers of blocks scored apart (8 for each block, run and key head; one run's at least): a step that needs more
+# chooses run after run, in launches that follow each other (4680 runs of 12 key heads among 8192 blocks: 22.3 ms with 3.7 GB,
+# 1 GB or this, 22.5 with 64 MiB, 24.0 with 16).
+_SCORE_BYTES = 1 << 28
 _Image = ctypes.c_int64 * len(_lib.BLOCKS_FIELDS)
-_KEYS_AT, _SCALES_AT, _SLOTS_AT, _Q_AT, _PLAN_AT, _SCORES_AT, _LISTS_AT = (
-    _lib.BLOCKS_FIELDS.index(name) for name in ("keys_ptr", "scales_ptr", "slots_ptr", "q_ptr", "plan_ptr", "scores_ptr", "lists_ptr"))
+_KEYS_AT, _SCALES_AT, _SLOTS_AT, _Q_AT, _PLAN_AT, _RUNS_AT, _SCORES_AT, _LISTS_AT = (
+    _lib.BLOCKS_FIELDS.index(name)
+    for name in ("keys_ptr", "scales_ptr", "slots_ptr", "q_ptr", "plan_ptr", "runs", "scores_ptr", "lists_ptr"))
 
 
 class BlockPlan(AttentionPlan):
@@ -230,7 +235,8 @@ class BlockIndex:
 
     def select(self, layer, q, plan):
         """The blocks that each run of queries and key head attends to: int32 ``[runs, key heads, width]``, numbers of blocks
-        of the run's sequence in ascending order, -1 behind the last.  ``q``: as in :meth:`attend`."""
+        of the run's sequence in ascending order, -1 behind the last.  ``q``: as in :meth:`attend`.  Long histories are scored
+        in scratch of at most 256 MiB (or what one run's blocks need)."""
         address = self._layer(layer)
         self._check(q, plan)
         cache = self.cache
@@ -247,16 +253,19 @@ class BlockIndex:
                                                        group=plan.group, runs=plan._runs_at, n_runs=plan.runs,
                                                        scores=plan._scores, width=plan.width, top=plan.top))
                 fields = _Image.from_buffer_copy(image)
-                scores = None
+                scores, most = None, plan.runs  # runs of a launch
                 if plan._apart:
-                    scores = torch.empty(plan.runs * cache.heads * plan._scores, dtype=torch.int64, device=cache.device)
+                    most = min(most, max(1, _SCORE_BYTES // (8 * cache.heads * plan._scores)))
+                    scores = torch.empty(most * cache.heads * plan._scores, dtype=torch.int64, device=cache.device)
                     fields[_SCORES_AT] = scores.data_ptr()
                 fields[0], fields[_Q_AT], fields[_PLAN_AT] = address, q.data_ptr(), plan.buffer.data_ptr()
-                fields[_LISTS_AT] = blocks.data_ptr()
                 stream = raw_stream(cache.device)
                 if stream != plan._stream:  # the allocator learns of a stream that the tables were not made on
                     plan.buffer.record_stream(torch.cuda.current_stream(cache.device))
-                _lib.check(_lib.function("rch_blocks_select")(fields, _DTYPE_CODES[cache.dtype], stream))
+                for first in range(0, plan.runs, most):
+                    fields[_RUNS_AT], fields[_RUNS_AT + 1] = plan._runs_at + first * _lib.BLOCKS_RUN, min(most, plan.runs - first)
+                    fields[_LISTS_AT] = blocks.data_ptr() + 4 * first * cache.heads * plan.width
+                    _lib.check(_lib.function("rch_blocks_select")(fields, _DTYPE_CODES[cache.dtype], stream))
         return blocks
 
     def attend(self, layer, q, plan, *, blocks=None, out=None, return_lse=False):

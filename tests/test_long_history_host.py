@@ -587,3 +587,43 @@ def test_resources_are_written_early_enough(source, tmp_path):
     if source != "attend_lists.hip":
         based = re.sub(r"global_load_lds_dwordx4 (v\d+), (s\[\d+:\d+\])", r"buffer_load_dwordx4 \1, \2, 0 offen lds", text)
         assert based.count("offen lds") > text.count("offen lds") + 50 and machine.late_resources(based) == []
+
+
+@pytest.mark.parametrize("least", [0, 1 << 16])
+def test_the_scratch_of_a_choice_is_bounded(host, monkeypatch, least):
+    """Steps whose numbers need more than the bound choose run after run: every run once, each with its own list."""
+    cache = native(pages=6000, size=1, heads=2, dim=8, layers=2)
+    a = cache.new()
+    cache.extend([a], [5500])
+    index = cache.index(1)
+    plan = index.plan([a], [4400], heads=4, top=3)  # every run scores all blocks but the last one's
+    assert plan._apart and plan.runs == 4400 and plan._scores > _lib.BLOCKS_TOGETHER
+    if least:  # a bound below a run's own need
+        monkeypatch.setattr(sparse_attention, "_SCORE_BYTES", least, raising=False)
+    bound = max(least or 1 << 28, cache.heads * plan._scores * 8)
+    assert plan.runs * cache.heads * plan._scores * 8 > bound
+    q = torch.zeros(4400, 4, 8, dtype=torch.bfloat16)
+    host.clear()
+    blocks = index.select(1, q, plan)
+    at = 0
+    for name, call in host:
+        assert name == "rch_blocks_select" and call["n_runs"] >= 1
+        assert call["n_runs"] * cache.heads * call["scores"] * 8 <= bound and call["scores"] == plan._scores and call["scores_ptr"]
+        assert call["runs"] == plan._runs_at + at * _lib.BLOCKS_RUN and call["lists_ptr"] == blocks[at].data_ptr()
+        assert call["q_ptr"] == q.data_ptr() and call["means_ptr"] == index.means[1].data_ptr()
+        at += call["n_runs"]
+    assert at == plan.runs
+
+
+def test_a_choice_within_the_bound_is_one_call(host):
+    cache = native(pages=600, size=1, heads=2, dim=8)
+    a = cache.new()
+    cache.extend([a], [500])
+    index = cache.index(1)
+    for queries, apart in ((20, True), (100, False)):
+        plan = index.plan([a], [queries], heads=2, top=3)
+        assert plan._apart == apart
+        host.clear()
+        blocks = index.select(0, torch.zeros(queries, 2, 8, dtype=torch.bfloat16), plan)
+        (_, call), = host
+        assert (call["runs"], call["n_runs"], call["lists_ptr"]) == (plan._runs_at, queries, blocks.data_ptr()) and bool(call["scores_ptr"]) == apart
