@@ -462,3 +462,133 @@ def test_pools_past_32_bits(device, dtype, codes, size, block, dim, layout):
         del cache, index, slots, plan
     for small, large in zip(*results):
         assert not small.isnan().any() and torch.equal(small, large)
+
+
+def _ranked(means, pooled, held, scored, always, top):
+    """The rule for one run and key head, from exact scores: ``means`` float64 [blocks, D], ``scored`` ascending."""
+    scored = scored[held[scored]]
+    scores = means[scored] @ pooled
+    none = np.isnan(scores)
+    order = scored[np.lexsort((scored, np.where(none, 0.0, -scores), ~none))]
+    return sorted([j for j in always if held[j]] + order[:top].tolist())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("blocks,queries,query_block,heads,group,dim", [
+    (300, 70, 1, 2, 1, 16), (1000, 70, 1, 2, 2, 7), (4096, 64, 1, 2, 1, 8), (4100, 90, 1, 2, 1, 8), (3000, 260, 2, 1, 2, 64),  # a launch
+    (300, 9, 1, 1, 2, 16), (4090, 3, 1, 2, 1, 8), (4500, 4, 1, 1, 1, 16), (4098, 70, 1, 2, 1, 8), (9001, 66, 1, 2, 1, 8),  # two launches
+])
+def test_choices_among_many_blocks(device, dtype, blocks, queries, query_block, heads, group, dim, monkeypatch):
+    """Every path of a choice: numbers in LDS and in memory, in one launch and in two, with equal scores on both sides of every
+    256th and 1024th block, holes and NaN.  Small whole numbers, so that the scores are exact and few."""
+    size, length = 4, blocks * 4 - 1  # the last block is not full
+    cache = paged_cache.PagedCache.allocate(blocks, size, heads, dim, dtype=dtype, device=device)
+    order = np.random.default_rng(blocks).permutation(blocks).tolist()
+    cache.load_tables([(order, length)])
+    index = sparse_attention.BlockIndex.allocate(cache, size)
+    g = torch.Generator().manual_seed(blocks)
+    means = torch.randint(-1, 2, (blocks, heads, dim), generator=g).float()
+    means[torch.randint(0, blocks, (3,), generator=g), 0, 0] = math.nan
+    index.means[0, :, 0] = means[torch.tensor(order).argsort()].to(dtype).to(device)
+    for first in (100, 255, 1023):
+        if first < blocks - 2:
+            cache.drop(0, first, 2)
+    held = np.array(cache.pages_of(0)) >= 0
+    q = torch.randint(-1, 2, (queries, heads * group, dim), generator=g).to(dtype).to(device)
+    rows, exact = q.double().cpu().numpy(), means.double().numpy()
+    for top, first, recent in ((1, 1, 1), (37, 0, 0), (blocks // 3, 2, 3), (blocks - 20, 0, 1), (blocks, 0, 0)):
+        plan = index.plan([0], [queries], heads=heads * group, top=top, query_block=query_block, first=first, recent=recent)
+        assert plan._scores == blocks - 1 - first
+        found = index.select(0, q, plan)
+        assert plan._apart == (plan._scores > (256 if plan.runs * heads < 128 else 4096))
+        if plan._apart and plan.runs > 1:  # the same in several launches
+            with monkeypatch.context() as patch:
+                patch.setattr(sparse_attention, "_SCORE_BYTES", 8 * heads * plan._scores * 2 + 1)
+                assert torch.equal(index.select(0, q, plan), found)
+        found = found.cpu()
+        for run in sorted({0, 1, plan.runs // 2, plan.runs - 1} & set(range(plan.runs))):
+            begin, end = run * query_block, min((run + 1) * query_block, queries)
+            own = (length - queries + end - 1) // size
+            always = sorted({j for j in range(blocks) if j < first or own - recent < j <= own} | {blocks - 1})
+            scored = np.setdiff1d(np.arange(blocks), always)
+            for head in range(heads):
+                pooled = rows[begin:end, head * group:(head + 1) * group].sum(axis=(0, 1))
+                want = _ranked(exact[:, head], pooled, held, scored, always, top)
+                assert found[run, head].tolist() == want + [-1] * (plan.width - len(want)), (top, run, head)
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+def test_means_and_choices_after_compaction(device, dtype, codes):
+    """Pages that moved, each with its means."""
+    lengths = [100, 70, 33]
+    cache = _cache(device, lengths, 32, 2, 64, dtype, codes)
+    index = _index(cache, 8, lengths)
+    kept = [1, 2]
+    before = [[index.means[0, cache.pages_of(s)[j // 4], j % 4].clone() for j in range(lengths[s] // 8)] for s in kept]
+    q = _queries([1, 1], 4, 64, dtype, device)
+    plan = index.plan(kept, [1, 1], heads=4, top=2)
+    blocks, out = index.select(0, q, plan), index.attend(0, q, plan)
+    pages = [cache.pages_of(s) for s in kept]
+    cache.free(0)
+    assert cache.compact() and [cache.pages_of(s) for s in kept] != pages
+    for s, means in zip(kept, before):
+        for j, mean in enumerate(means):
+            assert torch.equal(index.means[0, cache.pages_of(s)[j // 4], j % 4], mean), (s, j)
+    plan = index.plan(kept, [1, 1], heads=4, top=2)
+    assert torch.equal(index.select(0, q, plan), blocks) and torch.equal(index.attend(0, q, plan), out)
+
+
+@pytest.mark.parametrize("dtype,codes", [(torch.bfloat16, None), (torch.bfloat16, torch.float8_e4m3fn), (torch.float16, torch.int8)])
+def test_graphs_and_eager_calls_at_once(device, dtype, codes):
+    """Two captured steps and an eager one on streams of their own, at the same time: each has the results that it has alone.
+    One graph stores into a cache of its own; the other and the eager step share a cache, an index and plans."""
+    lengths, queries = [6000, 130], [60, 1]
+    caches = [_cache(device, lengths, 64, 2, 128, dtype, codes, seed=seed) for seed in (0, 1)]
+    for cache in caches:
+        if codes is None:
+            cache.keys.nan_to_num_(0.0), cache.values.nan_to_num_(0.0)
+    indexes = [_index(cache, 16, lengths) for cache in caches]
+    # Runs of 6000 / 16 blocks: 3 x 2 of them are scored in launches of their own, for single tokens too.
+    plans = [index.plan([0, 1], queries, heads=8, top=200, query_block=30) for index in indexes]
+    tokens = indexes[1].plan([0, 1], [1, 1], heads=8, top=200)
+    assert plans[0]._apart and tokens._apart and plans[0]._n_merges
+    qs = [_queries([61], 8, 128, dtype, device, seed=seed) for seed in range(3)]
+    slots = caches[0].slots([0], [5940], [60])
+    k = torch.randn((60, 2, 128), generator=torch.Generator().manual_seed(1)).to(dtype).to(device)
+
+    def storing():
+        caches[0].store(0, slots, k, k)
+        indexes[0].update(0, slots)
+        blocks = indexes[0].select(0, qs[0], plans[0])
+        return (blocks, *indexes[0].attend(0, qs[0], plans[0], blocks=blocks, return_lse=True))
+
+    def reading(q):
+        return (indexes[1].select(0, q, plans[1]), *indexes[1].attend(0, q, plans[1], return_lse=True), indexes[1].attend(0, q[:2], tokens))
+
+    torch.cuda.synchronize(device)
+    sides = [torch.cuda.Stream(device) for _ in range(3)]
+    graphs, outs = [], []
+    storing(), reading(qs[1])
+    torch.cuda.synchronize(device)
+    for side, step in zip(sides, (storing, lambda: reading(qs[1]))):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            outs.append(step())
+        graphs.append(graph)
+    for replay in range(4):
+        for i, x in enumerate((k, *qs)):
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(10 * replay + i)))
+        torch.cuda.synchronize(device)
+        want = [[t.clone() for t in step] for step in (storing(), reading(qs[1]), reading(qs[2]))]
+        for out in outs:
+            for t in out:
+                t.zero_()
+        torch.cuda.synchronize(device)
+        for side, graph in zip(sides, graphs):
+            with torch.cuda.stream(side):
+                graph.replay()
+        with torch.cuda.stream(sides[2]):
+            eager = reading(qs[2])
+        torch.cuda.synchronize(device)
+        for found, expected in zip((*outs, eager), want):
+            assert all(torch.equal(a, b) for a, b in zip(found, expected)), replay
