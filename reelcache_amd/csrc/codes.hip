@@ -128,13 +128,12 @@ __global__ void __launch_bounds__(256) codes_store_kernel(const rch_codes A) {
         }
     }
     if (pairs && mine && first < 2 * pairs) {
-        int row[3];
-        turning_rows(A, 0, token, row);
+        const TurningRows row = turning_rows(A, 0, token);
         f2 angle[V / 2];
 #pragma unroll
         for (int i = 0; i < V / 2; ++i) {
             angle[i] = f2{1.0f, 0.0f};
-            if (first / 2 + i < pairs) angle[i] = turning_angle(A, row, first / 2 + i);
+            if (first / 2 + i < pairs) angle[i] = turning_angle(A, row, first / 2 + i, pairs);
         }
 #pragma unroll
         for (int u = 0; u < kHeads; ++u)

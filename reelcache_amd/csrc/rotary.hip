@@ -127,14 +127,13 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotaryJobs jobs) {
         return;
     }
 
-    int row[3];
-    turning_rows(J, batch, token, row);
+    const TurningRows row = turning_rows(J, batch, token);
     constexpr int P = HALF ? V : V / 2;
     const int j0 = piece * P;
     float c[P], s[P];
 #pragma unroll
     for (int i = 0; i < P; ++i) {
-        const f2 pair = turning_angle(J, row, j0 + i);
+        const f2 pair = turning_angle(J, row, j0 + i, pairs);
         c[i] = pair[0];
         s[i] = J.inverse ? -pair[1] : pair[1];
     }

@@ -627,3 +627,17 @@ def test_a_choice_within_the_bound_is_one_call(host):
         blocks = index.select(0, torch.zeros(queries, 2, 8, dtype=torch.bfloat16), plan)
         (_, call), = host
         assert (call["runs"], call["n_runs"], call["lists_ptr"]) == (plan._runs_at, queries, blocks.data_ptr()) and bool(call["scores_ptr"]) == apart
+
+
+@pytest.mark.parametrize("source", ["rotary.hip", "codes.hip", "blocks.hip"])
+def test_kernels_keep_their_values_in_registers(source, tmp_path):
+    """No scratch memory: places of rotated tokens written to an array cost every rotation and store 1 to 2 %."""
+    import subprocess
+
+    from reelcache_amd.csrc import build as hip_build
+
+    target = tmp_path / "kernels.s"
+    subprocess.run([hip_build._hipcc(), *hip_build.FLAGS, "-w", "--cuda-device-only", "-S", str(hip_build.HERE / source), "-o",
+                    str(target)], check=True, capture_output=True)
+    sizes = re.findall(r"\.private_segment_fixed_size: (\d+)", target.read_text())
+    assert len(sizes) > 10 and set(sizes) == {"0"}
