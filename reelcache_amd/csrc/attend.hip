@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) attend_general_kernel(const rch_attend A)
         for (int c = 0; c < RCH_ATTEND_MAX_DIM / 64; ++c) acc[c] = 0.0f;
         auto look = [&](const int base, const int from, const int to) {
             const int key = base + lane;
-            bool seen = key >= from && key < to;
+            bool seen = (!LIST || key >= from) && key < to;
             int page = -1;
             if (seen) page = table[key / size];
             seen = seen && page >= 0 && page < A.pages;
