@@ -20,7 +20,7 @@
 extern "C" {
 #endif
 
-#define RCH_ABI_VERSION 24
+#define RCH_ABI_VERSION 25
 
 /* Status codes (mapped to reelcache errors by the host). */
 #define RCH_OK 0
@@ -684,8 +684,10 @@ typedef struct rch_attend {
  * Cuts the row blocks of a plan into parts (host only): block i has tiles[i] key tiles and belongs to owner[i]
  * (blocks of one owner share keys).  parts: int64 [capacity][4] of (block, first tile, last tile, XCD), block
  * after block; *count of them, at most n + 2 * resident + 16.  resident: workgroups that the card runs at
- * once; overhead: what one spends besides its tiles, in tiles.
+ * once; overhead: what one spends besides its tiles, in tiles, with RCH_SHARE_WAVES added for workgroups of one wave
+ * that fill the card by parts alone: parts of single tiles, and an item in as many as half of an XCD's places.
  */
+#define RCH_SHARE_WAVES (1LL << 32)
 int rch_attend_share(const int64_t* tiles, const int64_t* owner, int64_t n, int64_t resident, int64_t overhead, int64_t* parts,
                      int64_t capacity, int64_t* count);
 

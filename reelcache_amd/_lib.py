@@ -16,7 +16,7 @@ import numpy as np
 from .errors import ConfigurationError, UnsupportedError
 
 LIBRARY = Path(__file__).resolve().with_name("libreelcache_hip.so")
-ABI_VERSION = 24
+ABI_VERSION = 25
 
 # Status codes (RCH_E_*).
 OK, E_CONFIG, E_UNSUPPORTED, E_LAUNCH = 0, 1, 2, 3
@@ -83,7 +83,7 @@ ATTEND_FIELDS = ("q_ptr", "k_ptr", "v_ptr", "out_ptr", "lse_ptr", "plan_ptr", "p
                  "v_scale_ptr", "k_scale_page_stride", "k_scale_head_stride", "v_scale_page_stride", "v_scale_head_stride",
                  "lists_ptr", "block_tokens", "single")
 ATTEND_ITEM, ATTEND_MERGE, ATTEND_ZEROS, ATTEND_MAX_DIM, ATTEND_FAST_DIM = 12, 8, 128, 256, 256
-ATTEND_FEW_PARTS, ATTEND_SINGLE_ROWS = 8, 32
+ATTEND_FEW_PARTS, ATTEND_SINGLE_ROWS, SHARE_WAVES = 8, 32, 1 << 32
 PAIRS_INTERLEAVED, PAIRS_HALF = 0, 1
 # rch_codes and rch_blocks (int64 structs read on the host during the call), formats of codes (RCH_CODES_*).
 CODES_FIELDS = ("k_ptr", "v_ptr", "k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride", "k_codes_ptr",

@@ -268,6 +268,8 @@ class AttentionPlan:
         cache = self.cache
         start = _OVERHEAD["lists" if form == "rows" and self._block_tokens else form]
         owner = sequence * cache.heads + head
+        if form == "single":
+            start += _lib.SHARE_WAVES
         which, low, high, xcd = _share_out(tiles, owner, self._resident(form), start).T
         parts = np.bincount(which, minlength=len(tiles))
         part = np.arange(len(which)) - np.repeat(np.cumsum(parts) - parts, parts)

@@ -18,9 +18,14 @@ constexpr int kXcds = 8;
 // short sequences (37 to 1000 tokens) take 13.1 / 14.3 / 21.5 us with parts of at least 2 / 3 / 4 tiles, of 16
 // sequences of 2000 tokens 23.9 / 19.8 us with 2 / 3; of 2 of 16000 tokens 31.7 us with up to 64 parts, 23.1 with 32
 // (their merge grows).
-constexpr int64_t kShortestPart = 3, kMostParts = 32, kManyResident = 128;
-// Of waves of single tokens over codes (8 of 37 to 1000 tokens: 14.6 / 15.0 / 16.7 us with parts of at least 1 / 2 / 3).
-constexpr int64_t kShortestSingle = 1;
+constexpr int64_t kShortestPart = 3, kMostParts = 32;
+// Of waves of single tokens over codes (8 of 37 to 1000 tokens: 14.6 / 15.0 / 16.7 us with parts of at least 1 / 2 / 3), which
+// fill the card by parts alone: an item in up to half of an XCD's places (one sequence of 65536 tokens,
+// 8 key heads of 256 int8 channels: 98 us, and 176 with parts of at least 3 tiles and at most 32 of them).
+constexpr int64_t kShortestWave = 1;
+struct Rule {
+    int64_t fewest, most;  // tiles of a part, parts of an item within an XCD
+};
 
 struct Piece {
     int64_t item, first, last;  // item: rank within the XCD
@@ -75,8 +80,8 @@ bool ending_by(const std::vector<int64_t>& costs, int64_t resident, int64_t over
 
 // Cuts items (longest first) so that `resident` workgroups that take parts in order, longest first, end together as
 // early as they can.
-void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, int64_t fewest, std::vector<Piece>& pieces) {
-    const int64_t n = static_cast<int64_t>(costs.size()), longest = costs[0];
+void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, const Rule& rule, std::vector<Piece>& pieces) {
+    const int64_t n = static_cast<int64_t>(costs.size()), longest = costs[0], fewest = rule.fewest;
     pieces.clear();
     auto whole = [&]() {
         pieces.clear();
@@ -95,9 +100,7 @@ void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, 
             uncut = std::max(uncut, load);
         }
     }
-    // (a form with more workgroups to an XCD than kManyResident, waves of single tokens, is cut further: it fills the card by parts alone)
-    const int64_t most = resident > kManyResident ? resident / 2 : kMostParts;
-    const int64_t shortest = std::max(fewest, (longest + most - 1) / most);
+    const int64_t shortest = std::max(fewest, (longest + rule.most - 1) / rule.most);
     int64_t low = std::max((total + n * overhead) / resident, shortest + overhead), high = uncut;
     std::vector<Piece> found;
     while (50 * low < 49 * high) {  // the earliest end that parts reach, within a fiftieth
@@ -114,7 +117,11 @@ void cut(const std::vector<int64_t>& costs, int64_t resident, int64_t overhead, 
 
 int share_out(const int64_t* tiles, const int64_t* owner, int64_t n, int64_t resident, int64_t overhead, int64_t* parts,
               int64_t capacity, int64_t* count) {
-    const int64_t fewest = resident / kXcds > kManyResident ? kShortestSingle : kShortestPart;
+    const int64_t places = std::max<int64_t>(1, resident / kXcds);
+    const bool waves = overhead >= RCH_SHARE_WAVES;
+    const Rule rule = waves ? Rule{kShortestWave, std::max<int64_t>(1, places / 2)} : Rule{kShortestPart, kMostParts};
+    const int64_t fewest = rule.fewest;
+    overhead -= waves ? RCH_SHARE_WAVES : 0;
     std::vector<int64_t> order(static_cast<size_t>(n)), starts(order.size());
     for (int64_t i = 0; i < n; ++i) order[static_cast<size_t>(i)] = i;
     std::stable_sort(order.begin(), order.end(), [&](int64_t a, int64_t b) { return owner[a] < owner[b]; });
@@ -156,7 +163,7 @@ int share_out(const int64_t* tiles, const int64_t* owner, int64_t n, int64_t res
         auto made = known.find(costs);
         if (made == known.end()) {
             std::vector<Piece> pieces;
-            cut(costs, std::max<int64_t>(1, resident / kXcds), overhead, fewest, pieces);
+            cut(costs, places, overhead, rule, pieces);
             made = known.emplace(std::move(costs), std::move(pieces)).first;
         }
         for (const Piece& p : made->second) {

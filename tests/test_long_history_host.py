@@ -641,3 +641,20 @@ def test_kernels_keep_their_values_in_registers(source, tmp_path):
                     str(target)], check=True, capture_output=True)
     sizes = re.findall(r"\.private_segment_fixed_size: (\d+)", target.read_text())
     assert len(sizes) > 10 and set(sizes) == {"0"}
+
+
+@pytest.mark.parametrize("dim", [64, 128, 144, 192, 256])
+def test_single_tokens_over_codes_fill_the_card_by_parts_at_every_head_size(host, dim):
+    """A form of single waves is cut into as many parts as it says, whatever the number of waves that its heads leave room for:
+    one long sequence of 8 key heads takes half of the places."""
+    cache = quantised(pages=1024, size=64, heads=8, dim=dim, layers=1)
+    cache.load_tables([(list(range(1024)), 65536)])
+    plan = cache.plan([0], [1], heads=32)
+    assert plan._single
+    items = plan.buffer.numpy()[plan._items:plan._items + plan._counts_of[1] * _lib.ATTEND_ITEM].reshape(-1, _lib.ATTEND_ITEM)
+    parts = int((items[:, 5] > items[:, 4]).sum())
+    shortest = -(-1024 // (plan._resident("single") // 16))  # tiles of a part, of a head's 1024
+    assert parts >= 8 * (1024 // shortest), parts
+    short = quantised(pages=64, size=64, heads=8, dim=dim, layers=1)
+    short.load_tables([(list(range(8)), 512)])
+    assert short.plan([0], [1], heads=32)._n_merges  # parts of single tiles

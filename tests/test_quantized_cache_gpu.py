@@ -406,3 +406,24 @@ def test_small_weights_of_small_and_large_values(device, codes, exponent, group)
     assert cache.plan([0], [1], heads=group)._single == (group == 2)
     out = _check(cache, lengths, [1, 1], q)
     assert (out != 0).any(dim=2).all()
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,size", [(144, 64), (256, 64), (256, 16)])
+def test_long_split_histories_of_wide_heads(device, codes, dtype, dim, size):
+    """Parts of few tiles, joined: heads above 128 channels are cut as the others are."""
+    lengths = [9000, 70]
+    cache = _filled(device, lengths, size, 2, dim, codes, dtype)
+    q = torch.randn((2, 6, dim), generator=torch.Generator().manual_seed(3)).to(dtype).to(device)
+    native = _native(cache)
+    plan = cache.plan([0, 1], [1, 1], heads=6)
+    assert plan._single and plan._n_merges == 4  # also of the two tiles of 70 keys
+    out, lse = cache.attend(0, q, plan, return_lse=True)
+    for sequence, length in enumerate(lengths):
+        k, v = (history.history(x[0], "BTHD", cache.pages_of(sequence), length) for x in (native.keys, native.values))
+        for head in range(6):
+            want, bound, logs, log_bound = history.attend(q[sequence:sequence + 1, head].double().cpu(), k[:, head // 3], v[:, head // 3],
+                                                          np.ones((1, length), dtype=bool), dtype)
+            assert oracle.worst(out[sequence:sequence + 1, head], want, bound) <= 0
+            assert oracle.worst(lse[sequence:sequence + 1, head], logs, log_bound) <= 0
