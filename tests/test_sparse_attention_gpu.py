@@ -592,3 +592,50 @@ def test_graphs_and_eager_calls_at_once(device, dtype, codes):
         torch.cuda.synchronize(device)
         for found, expected in zip((*outs, eager), want):
             assert all(torch.equal(a, b) for a, b in zip(found, expected)), replay
+
+
+@pytest.mark.parametrize("dtype,codes", KINDS)
+@pytest.mark.parametrize("dim", [64, 20])
+def test_runs_that_take_nothing(device, dtype, codes, dim):
+    """No leading, recent or chosen block, and every block full: queries that attend to nothing, in every form."""
+    lengths = [256, 64]
+    cache = _cache(device, lengths, 64, 2, dim, dtype, codes)
+    for block in (16, 64):
+        index = _index(cache, block, lengths)
+        for queries in ([1, 1], [40, 3]):
+            q = _queries(queries, 4, dim, dtype, device)
+            plan = index.plan([0, 1], queries, heads=4, top=0, first=0, recent=0, query_block=8)
+            assert plan.width == 0 and index.select(0, q, plan).shape == (plan.runs, 2, 0)
+            out, lse = index.attend(0, q, plan, return_lse=True)
+            assert not out.any() and (lse == -math.inf).all()
+            _check(cache, index, lengths, queries, q, top=1, first=0, recent=0, query_block=8)
+
+
+def test_reads_follow_a_sequence_into_its_copied_page(device):
+    """Two sequences of one history go on apart and rewrite their last rows: each is read as it is, and old places are refused."""
+    dtype = torch.bfloat16
+    cache = quantized_cache.QuantizedCache.allocate(8, 16, 2, 64, codes=torch.int8, dtype=dtype, device=device)
+    index = cache.index(8)
+    a = cache.new()
+    slots = cache.extend([a], [30])
+    g = torch.Generator().manual_seed(2)
+    rows = [torch.randn((30, 2, 64), generator=g).to(dtype).to(device) for _ in range(3)]
+    cache.store(0, slots, rows[0], rows[0])
+    index.update(0, slots)
+    b = cache.fork(a)
+    old = cache.places([a], [0], [30])
+    cache.extend([a], [1])
+    for sequence, x in ((a, rows[1]), (b, rows[2])):
+        slots = cache.slots([sequence], [16], [14])
+        cache.store(0, slots, x[:14], x[:14])
+        index.update(0, slots)
+    for call in (lambda: cache.read(0, old), lambda: index.update(0, old)):
+        with pytest.raises(StateError):
+            call()
+    for sequence, x in ((a, rows[1]), (b, rows[2])):
+        want = history.decode(*history.encode(torch.cat([rows[0][:16], x[:14]]), torch.int8), dtype)
+        for found in cache.read(0, cache.places([sequence], [0], [30])):
+            assert torch.equal(found.cpu(), want)
+        # The mean of its block of rows 16 to 23: a sum in 64 bits, rounded to fp32 and then to the type.
+        mean, exact = index.means[0, cache.pages_of(sequence)[1], 0].double().cpu(), want[16:24].double().mean(dim=0)
+        assert ((mean - exact).abs() <= (oracle.U[dtype] + oracle.F32 + 2.0 ** -40) * 1.01 * exact.abs() + oracle.TINY[dtype]).all()
