@@ -34,7 +34,8 @@ GENERAL_ROWS, ROW_TILE = 16, 128
 _ROWS = {"general": GENERAL_ROWS, "rows": ROW_TILE, "single": _lib.ATTEND_SINGLE_ROWS}
 # What a workgroup's start, end and partial results cost in key tiles, per form (tiled: a step of six sequences of
 # 211 to 5003 tokens takes 58.0 us at 0, 55.4 at 3, 54.8 at 6 and 55.0 at 8; others do not change by more than 2 %).
-# Single tokens over codes: 75.4 us at 2 and 73.9-74.7 at 0 to 6 for four long sequences, 48.4 at 2 and 48.2-51.0 for 64 of up to 4000.
+# Single tokens over codes: four long sequences take 74.0 / 74.2 / 73.2 / 73.0 / 72.0 / 74.0 us at 0 / 1 / 2 / 3 / 4 / 6, 64 of up to
+# 4000 tokens 61.9 / 62.0 / 62.1 / 65.1 / 65.1 / 66.0.
 # Chosen blocks ("lists"): prompts over 32 blocks of 32 keys take 76.6 / 76.2 / 75.3 / 75.3 / 77.8 us at 0 / 2 / 3 / 4 / 6, a chunk
 # over 26 of 120 148.7 / 136.1 / 136.3 / 136.4 / 136.7.  Dense steps over codes do not agree (69-84 us, up to 5 % either way).
 _OVERHEAD = {"general": 1, "rows": 6, "lists": 3, "single": 2}

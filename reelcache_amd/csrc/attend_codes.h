@@ -7,7 +7,7 @@
 // queries, and each tile waited for their reloads and so for the next tile's loads: a chunk of 4680 queries x 32760 keys
 // in e4m3 took 1177 us so.)
 //
-// Bound: the products and what stands beside them.  That chunk takes 1050-1090 us where native pools take 915-945 on the same
+// Bound: the products and what stands beside them.  That chunk takes 1015-1090 us where native pools take 915-945 on the same
 // cards: 7.9 vector instructions to a matrix instruction instead of 6.5, and 61 LDS instructions to a wave's tile instead of
 // 49, as the waves write it.
 #pragma once

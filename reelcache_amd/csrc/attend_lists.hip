@@ -4,7 +4,7 @@
 // Bound: a chunk of 39 runs of 120 queries over 26 of 273 blocks of 120 (12 heads of 128) takes 130-142 us, 600 TFLOP/s: 468
 // row blocks on 512 places, tiles of 64 and 56 keys, and runs that choose apart read 431 MB past the L2 for 201 MB of pools.
 // Single tokens over 31 blocks of 64: 11.8 us, latency.  Blocks of 32 over int8 pages (prompts of up to 1500 queries, heads of
-// 80): 56 us in tiles that run on; choice, attention and join take 75 us so and 105 in tiles that start over, half empty, at each.
+// 80): 56 us in tiles that run on; choice, attention and join take 75 us so and 99 in tiles that start over, half empty, at each.
 #include "attend_rows.h"
 
 namespace rch {

@@ -11,7 +11,8 @@
 // 16 or 32 lanes with eight channels each (a wave's row maxima meet by lane moves, no LDS), and a thread holds that
 // piece of four heads, so that the places and cosines are fetched once for them.  Measured: a chunk of 4680 tokens of 12 heads
 // of 128 bf16 channels stored (rotated) as int8 in 14 us (43 MB, 3 TB/s: 9 us of bytes, 6 of instructions, and the chain place, angles, store), read
-// back in 11.5; a history of 32760 tokens read from e4m3 in 55 us (302 MB, 5.5 TB/s).
+// back in 11.5; a history of 32760 tokens read from e4m3 in 55 us into the same outputs over and over (302 MB, 5.5 TB/s), in 67
+// where every call has other pages and new outputs.
 #include "codes.h"
 #include "turn.h"
 

@@ -46,6 +46,7 @@ class QuantizedCache(PagedCache):
     ``keys``, ``values``: pools as :class:`PagedCache` takes them, of one of :data:`CODE_DTYPES`.  ``key_scales``,
     ``value_scales``: fp32 ``[layers, pages, heads, page_tokens]``, whatever the layout, with unit stride over the tokens.
     ``dtype``: what the codes stand for, and what tokens and queries come in (:data:`VALUE_DTYPES`).
+    Attention is tiled for the matrix cores where ``head_dim`` is a multiple of 16 (16-bit pools: of 8).
     """
 
     _POOL_DTYPES, _POOL_TYPES = CODE_DTYPES, "int8 or float8_e4m3fn"
