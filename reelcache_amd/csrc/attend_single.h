@@ -202,12 +202,14 @@ __global__ void __launch_bounds__(64, NB <= 2 ? 3 : NB <= 4 ? 2 : 1) attend_sing
         uint64_t small = 0, large = 0;  // keys of such scales (bits of the lanes that fetched them)
         if constexpr (FMT == RCH_CODES_E4M3) {
             own = code_scale<FMT>(scales[lane]);
+            bool apart = false;
             if constexpr (kScaled) {
-                const bool counts = of_values && (shown >> n & 1u);
-                small = __ballot(counts && own < 0x1p-64f);
-                large = __ballot(counts && own > 0x1p64f);
+                const bool counts = of_values && (shown >> n & 1u), low = counts && own < 0x1p-64f, high = counts && own > 0x1p64f;
+                small = __ballot(low);
+                large = __ballot(high);
+                apart = low || high;
             }
-            scales[lane] = (small | large) >> lane & 1u ? 0.0f : own;
+            scales[lane] = apart ? 0.0f : own;
         }
         if (shown != ~0u) {
 #pragma unroll
