@@ -658,3 +658,4 @@ def test_single_tokens_over_codes_fill_the_card_by_parts_at_every_head_size(host
     short = quantised(pages=64, size=64, heads=8, dim=dim, layers=1)
     short.load_tables([(list(range(8)), 512)])
     assert short.plan([0], [1], heads=32)._n_merges  # parts of single tiles
+    assert "#define RCH_SHARE_WAVES (1LL << 32)" in HEADER.read_text() and _lib.SHARE_WAVES == 1 << 32
